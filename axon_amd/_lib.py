@@ -78,6 +78,14 @@ SIGNATURES: dict[str, tuple] = {
     "axon_logits_fwd_ws": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "axon_logits_fwd_train": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "axon_logits_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "axon_logits_top_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "axon_logits_top_fwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _i64, _i32, _ptr]),
+    "axon_logits_tokens_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "axon_logits_tokens_fwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _i64, _ptr, _ptr, _ptr, _ptr, _i64,
+                                      _i32, _ptr]),
+    "axon_logits_tokens_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _i64, _ptr, _i32, _ptr, _ptr, _ptr,
+                                      _ptr, _ptr, _ptr, _i64, _ptr]),
     "axon_reverse_scan": (_i32, [_i32, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i64, _i64, _f32, _f32, _ptr, _ptr, _ptr,
                                  _ptr]),
     "axon_masked_whiten_workspace_bytes": (_i64, [_i64]),
@@ -125,7 +133,7 @@ SIGNATURES: dict[str, tuple] = {
                                         _ptr, _ptr, _f32, _i32, _ptr, _f32, _f32, _f32, _ptr, _ptr, _ptr]),
 }
 
-ABI_VERSION = 25
+ABI_VERSION = 26
 MASK_F32, MASK_I64 = 0, 1
 
 _lock = threading.Lock()

@@ -9,6 +9,7 @@ code (``_lib.native()``, csrc/torch_ext.cpp).  Nothing here computes on the CPU.
 
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 
@@ -1148,6 +1149,112 @@ def logits_backward(logits, labels, lse, entropy, g_logprob, g_entropy, inplace=
     )
     return out
 
+
+MAX_TOP = 128  # alternatives per row
+MAX_TOKEN_IDS = 512  # given tokens per row
+
+
+def on_device_of(t):
+    """The device of ``t`` as the current one, for a launch on its current stream."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _top_count(what, k, vocab):
+    if isinstance(k, bool) or not isinstance(k, int):
+        raise TypeError(f"{what}: k must be an int, got {type(k).__name__}")
+    if not 1 <= k <= min(MAX_TOP, vocab):
+        raise ValueError(f"{what}: k must be between 1 and {min(MAX_TOP, vocab)} (at most {MAX_TOP}, at most the "
+                         f"vocabulary), got {k}")
+
+
+def token_ids_arg(what, ids, rows, device):
+    """Token ids ``[rows, k]``: int32 or int64, contiguous, on the device of the rows."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: token_ids must be int32 or int64, got {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"{what}: operands live on different devices")
+    if ids.dim() != 2 or int(ids.shape[0]) != rows:
+        raise ValueError(f"{what}: token_ids {tuple(ids.shape)} do not have one row per token ({rows})")
+    if not 1 <= int(ids.shape[1]) <= MAX_TOKEN_IDS:
+        raise ValueError(f"{what}: between 1 and {MAX_TOKEN_IDS} token ids per row, got {int(ids.shape[1])}")
+    return ids.contiguous()
+
+
+def logits_top(logits, k, labels=None, backward_follows=False):
+    """``(logprob | None, entropy, lse, top_logprobs [tokens, k], top_ids [tokens, k])``; see axon_logits_top_fwd."""
+    n, v, ld = _logits_operands("logits_top", logits, labels)
+    _top_count("logits_top", k, v)
+    require_device(logits, "logits_top")
+    lib = _lib.load()
+    dev, dt = logits.device, _LOGITS_DTYPES[logits.dtype]
+    with on_device_of(logits):
+        out = torch.empty(n * (3 + k), device=dev, dtype=torch.float32)
+        top_ids = torch.empty(n, k, device=dev, dtype=torch.int64)
+        ws_bytes = lib.axon_logits_top_workspace_bytes(dt, n, v)
+        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
+        base = out.data_ptr()
+        check(
+            lib.axon_logits_top_fwd(ptr(logits), dt, ld, n, v, k, ptr(labels),
+                                    int(labels is not None and labels.dtype == torch.int64),
+                                    base if labels is not None else None, base + 4 * n, base + 8 * n, base + 12 * n,
+                                    ptr(top_ids), ptr(ws), ws_bytes, int(backward_follows), stream_ptr()),
+            "axon_logits_top_fwd",
+        )
+    lp, ent, lse = out[: 3 * n].view(3, n).unbind(0)
+    return (lp if labels is not None else None), ent, lse, out[3 * n:].view(n, k), top_ids
+
+
+def logits_tokens(logits, token_ids, backward_follows=False):
+    """``(logprobs [tokens, k], entropy, lse)`` of given tokens; see axon_logits_tokens_fwd."""
+    n, v, ld = _logits_operands("logits_tokens", logits, None)
+    ids = token_ids_arg("logits_tokens", token_ids, n, logits.device)
+    require_device(logits, "logits_tokens")
+    lib = _lib.load()
+    k, dev, dt = int(ids.shape[1]), logits.device, _LOGITS_DTYPES[logits.dtype]
+    with on_device_of(logits):
+        out = torch.empty(n * (2 + k), device=dev, dtype=torch.float32)
+        ws_bytes = lib.axon_logits_tokens_workspace_bytes(dt, n, v)
+        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32) if ws_bytes > 0 else None
+        base = out.data_ptr()
+        check(
+            lib.axon_logits_tokens_fwd(ptr(logits), dt, ld, n, v, ptr(ids), int(ids.dtype == torch.int64), k,
+                                       base + 8 * n, base, base + 4 * n, ptr(ws), max(ws_bytes, 0),
+                                       int(backward_follows), stream_ptr()),
+            "axon_logits_tokens_fwd",
+        )
+    return out[2 * n:].view(n, k), out[:n], out[n: 2 * n]
+
+
+def logits_tokens_backward(logits, token_ids, labels, lse, entropy, g_ids, g_label, g_entropy, inplace=False):
+    """d loss / d logits (written over the logits when ``inplace``) from the gradients of the log-probabilities of
+    ``token_ids`` and of ``labels`` and of the entropy, each of which may be None; see axon_logits_tokens_bwd."""
+    lib = _lib.load()
+    what = "logits_tokens_backward"
+    require_device(logits, what)
+    n, v, ld = _logits_operands(what, logits, labels)
+    k = 0
+    if token_ids is not None:
+        token_ids = token_ids_arg(what, token_ids, n, logits.device)
+        k = int(token_ids.shape[1])
+    g_ids, g_label, g_en = (None if g is None else f32(g) for g in (g_ids, g_label, g_entropy))
+    _same_len(what, n, lse=lse, entropy=entropy, g_label=g_label, g_entropy=g_en)
+    _same_len(what, n * k, g_ids=g_ids)
+    for g in (g_ids, g_label, g_en):
+        if g is not None and g.device != logits.device:
+            raise ValueError(f"{what}: operands live on different devices")
+    with on_device_of(logits):
+        out = logits if inplace else torch.empty_like(logits, memory_format=torch.contiguous_format)
+        ld_d = int(out.stride(0)) if n > 1 else v
+        check(
+            lib.axon_logits_tokens_bwd(ptr(logits), _LOGITS_DTYPES[logits.dtype], ld, n, v, ptr(token_ids),
+                                       int(token_ids is not None and token_ids.dtype == torch.int64), k, ptr(labels),
+                                       int(labels is not None and labels.dtype == torch.int64), ptr(lse), ptr(entropy),
+                                       ptr(g_ids), ptr(g_label), ptr(g_en), ptr(out), ld_d, stream_ptr()),
+            "axon_logits_tokens_bwd",
+        )
+    return out
 
 def gemm_nt(a, b):
     """out[n][m] = sum_k a[m][k] * b[n][k]; bf16 in, fp32 out.  Test/benchmark helper."""

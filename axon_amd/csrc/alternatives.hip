@@ -1,0 +1,495 @@
+// Alternatives of materialised logits: the k largest of every row with their log-probabilities, or the log-probabilities
+// of k given tokens per row, beside the entropy (and the label's log-probability); and the backward of both, which is
+// one: dz_j = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_H (log p_j + H)).
+//
+// Forward: ONE read of the row gives the softmax statistics and, for the k largest, the maxima of the row's segments of
+// 256 bytes, from which select.h finds the few segments that are read again.  Bound by memory.
+#include "logits_rows.h"
+#include "select.h"
+#include <type_traits>
+
+namespace axon {
+
+constexpr int kMaxParts = 64;
+constexpr int kSegVecs = 16;        // 16-byte vectors per segment: what sixteen neighbouring lanes load together
+constexpr int kMaxTokenIds = 512;   // given tokens per row
+
+__device__ __forceinline__ int64_t load_id(const void* ids, int i64, int64_t at) {
+  return i64 ? static_cast<const int64_t*>(ids)[at] : (int64_t) static_cast<const int32_t*>(ids)[at];
+}
+
+// The share of a row that is workgroup `part` of `parts`: whole segments, and some of the elements outside the vectors.
+struct SegSpan {
+  int head, n_vec, n_scalar, n_seg, q_lo, q_hi;
+  template <typename T>
+  __device__ __forceinline__ SegSpan(const T* row, int vocab, int part, int parts) {
+    const RowSpan sp(row, vocab, true, 0, 1);
+    head = sp.head; n_vec = sp.n_vec; n_scalar = sp.n_scalar;
+    n_seg = (n_vec + kSegVecs - 1) / kSegVecs;
+    q_lo = (int)((int64_t)n_seg * part / parts) * kSegVecs;
+    q_hi = min((int)((int64_t)n_seg * (part + 1) / parts) * kSegVecs, n_vec);
+  }
+  template <typename T>
+  __device__ __forceinline__ int scalar(int i) const { return i < head ? i : i + n_vec * Row<T>::kPer; }
+};
+
+// Folds N logits (natural units) into the statistics; their maximum.  A NaN among them makes the sums NaN, as it does
+// those of a softmax; -inf adds nothing.
+template <int N, int M>
+__device__ __forceinline__ float fold_max(Stats& a, const float (&z)[M]) {
+  float m = z[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) m = fmaxf(m, z[j]);
+  const float ml = m * kLog2e;
+  if (ml > a.M) {
+    const float d = fmaxf(a.M - ml, kTiny), f = __builtin_amdgcn_exp2f(d);
+    a.e = f * fmaf(a.s, d, a.e);
+    a.s = a.s * f;
+    a.M = ml;
+  }
+  float s4[4] = {a.s, 0.f, 0.f, 0.f}, e4[4] = {a.e, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float d = fmaf(z[j], kLog2e, -a.M), f = __builtin_amdgcn_exp2f(d);
+    s4[j & 3] += f;
+    e4[j & 3] = fmaf(f, fmaxf(d, kTiny), e4[j & 3]);
+  }
+  a.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  a.e = (e4[0] + e4[1]) + (e4[2] + e4[3]);
+  return m;
+}
+
+__device__ __forceinline__ Stats wave_merge(Stats st) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    Stats o;
+    o.M = __shfl_down(st.M, off, kWave);
+    o.s = __shfl_down(st.s, off, kWave);
+    o.e = __shfl_down(st.e, off, kWave);
+    st = merge(st, o);
+  }
+  return st;
+}
+
+// Maximum over the sixteen lanes of a row of the wavefront, in its last lane.
+__device__ __forceinline__ float row16_max_to_last(float v) {
+  v = fmaxf(v, dpp_or_own<0x111, 0xf>(v));
+  v = fmaxf(v, dpp_or_own<0x112, 0xf>(v));
+  v = fmaxf(v, dpp_or_own<0x114, 0xf>(v));
+  v = fmaxf(v, dpp_or_own<0x118, 0xf>(v));
+  return v;
+}
+
+struct RowOut {
+  float *logprob, *entropy, *lse;  // logprob, entropy may be null
+  const void* labels;              // may be null
+  int labels_i64;
+};
+// (log-sum-exp, entropy) from a row's statistics, and the label's log-probability
+template <typename T>
+__device__ __forceinline__ float write_row(Stats st, int t, const T* row, int vocab, const RowOut& o) {
+  const float L = __log2f(st.s), d = st.e / st.s, lse = (st.M + L) * kLn2;
+  o.lse[t] = lse;
+  if (o.entropy != nullptr) o.entropy[t] = (L - d) * kLn2;
+  if (o.logprob != nullptr) {
+    const int64_t lab = load_id(o.labels, o.labels_i64, t);
+    o.logprob[t] = (lab >= 0 && lab < vocab) ? Row<T>::one(row + lab) - lse : 0.f;
+  }
+  return lse;
+}
+
+struct Picks {
+  const void* ids;  // [n][k]
+  int ids_i64, k;
+  float* out;       // [n][k]
+};
+template <typename T>
+__device__ __forceinline__ void write_picks(const Picks& p, int t, const T* row, int vocab, float lse) {
+  for (int i = threadIdx.x; i < p.k; i += kBlock) {
+    const int64_t id = load_id(p.ids, p.ids_i64, (int64_t)t * p.k + i);
+    p.out[(int64_t)t * p.k + i] = (id >= 0 && id < vocab) ? Row<T>::one(row + id) - lse : 0.f;
+  }
+}
+
+// Workgroup (row, part): blockIdx.x = row * parts + part.  Leaves its statistics in ws[row][part][3] and, with SEG, the
+// maxima of its segments in seg_max[row][seg].  Without SEG and with one part per row it finishes the row.
+// Rows from `cached_from` on are left in the cache in front of the memory, for what reads them next.
+template <typename T, bool SEG>
+__global__ __launch_bounds__(kBlock) void alternatives_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
+                                                                    float* __restrict__ ws, float* __restrict__ seg_max,
+                                                                    int seg_stride, RowOut out, Picks picks, int cached_from) {
+  __shared__ float red[3][kBlock / kWave];
+  __shared__ float s_lse;
+  const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
+  const T* row = logits + (int64_t)t * ld;
+  constexpr int kPer = Row<T>::kPer;
+  const SegSpan sp(row, vocab, part, parts);
+  const T* body = row + sp.head;
+  float* const segs = SEG ? seg_max + (int64_t)t * seg_stride : nullptr;
+  const int tid = threadIdx.x;
+  Stats st{kFloor, 0.f, 0.f};
+  auto keep_max = [&](int q, float m) {
+    if (!SEG) return;
+    m = row16_max_to_last(m);
+    if ((tid & 15) == 15 && (q & ~15) < sp.q_hi) segs[q / kSegVecs] = m;
+  };
+  auto walk = [&](auto cached) {
+    constexpr bool kCached = decltype(cached)::value;
+    int b = sp.q_lo;
+    for (; b + 2 * kBlock <= sp.q_hi; b += 2 * kBlock) {  // two loads in flight per thread
+      float v0[8], v1[8];
+      const int q = b + tid;
+      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v0);
+      Row<T>::template load<kCached>(body + (uint32_t)(q + kBlock) * kPer, v1);
+      keep_max(q, fold_max<kPer>(st, v0));
+      keep_max(q + kBlock, fold_max<kPer>(st, v1));
+    }
+    for (; b < sp.q_hi; b += kBlock) {
+      float v[8];
+      const int q = b + tid;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+      if (q < sp.q_hi) Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v);
+      keep_max(q, fold_max<kPer>(st, v));
+    }
+  };
+  if (t >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
+  for (int i = part * kBlock + tid; i < sp.n_scalar; i += parts * kBlock) {
+    const float v[1] = {Row<T>::one(row + sp.scalar<T>(i))};
+    fold_max<1>(st, v);
+  }
+  st = wave_merge(st);
+  const int lane = tid & (kWave - 1), wave = tid / kWave;
+  if (lane == 0) { red[0][wave] = st.M; red[1][wave] = st.s; red[2][wave] = st.e; }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kBlock / kWave; ++w) st = merge(st, Stats{red[0][w], red[1][w], red[2][w]});
+    if (SEG || parts > 1) {
+      float* o = ws + (int64_t)blockIdx.x * 3;
+      o[0] = st.M; o[1] = st.s; o[2] = st.e;
+    } else {
+      s_lse = write_row<T>(st, t, row, vocab, out);
+    }
+  }
+  if (SEG || parts > 1) return;
+  __syncthreads();
+  write_picks<T>(picks, t, row, vocab, s_lse);
+}
+
+// The statistics of a row's parts (at most kMaxParts), in a fixed tree; the total in thread 0.
+__device__ __forceinline__ Stats merge_parts(const float* ws, int t, int parts) {
+  Stats st{kFloor, 0.f, 0.f};
+  if ((int)threadIdx.x < parts) {
+    const float* o = ws + ((int64_t)t * parts + threadIdx.x) * 3;
+    st = Stats{o[0], o[1], o[2]};
+  }
+  return threadIdx.x < kWave ? wave_merge(st) : st;
+}
+
+// A workgroup per row folds the parts' statistics and picks the given tokens.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void tokens_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
+                                                               const float* __restrict__ ws, RowOut out, Picks picks) {
+  __shared__ float s_lse;
+  const int t = blockIdx.x;
+  const T* row = logits + (int64_t)t * ld;
+  const Stats st = merge_parts(ws, t, parts);
+  if (threadIdx.x == 0) s_lse = write_row<T>(st, t, row, vocab, out);
+  __syncthreads();
+  write_picks<T>(picks, t, row, vocab, s_lse);
+}
+
+// A row of logits as select_top reads it.
+template <typename T>
+struct LogitsSource {
+  static constexpr int kPer = Row<T>::kPer, kItems = kSegVecs;
+  const T* row;
+  const float* seg_max;
+  SegSpan sp;
+  int vocab;
+  __device__ int n_segs() const { return sp.n_seg; }
+  __device__ uint32_t max_key(int i) const { return order_key(seg_max[i]); }
+  __device__ int limit() const { return vocab; }
+  __device__ int load(const int* segs, int j, float (&v)[kPer]) const {
+    const int q = segs[j / kSegVecs] * kSegVecs + (j & (kSegVecs - 1));
+    if (q >= sp.n_vec) return -1;
+    float x[8];
+    const int at = sp.head + q * kPer;
+    Row<T>::template load<true>(row + at, x);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = x[e];
+    return at;
+  }
+  __device__ int n_single() const { return sp.n_scalar; }
+  __device__ float single(int i, int& index) const {
+    index = sp.scalar<T>(i);
+    return Row<T>::one(row + index);
+  }
+};
+
+// A workgroup per row: folds the parts' statistics, selects the k largest.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void top_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
+                                                            const float* __restrict__ ws, const float* __restrict__ seg_max,
+                                                            int seg_stride, int k, RowOut out, float* __restrict__ top_logprobs,
+                                                            int64_t* __restrict__ top_ids) {
+  __shared__ SelectLds s;
+  __shared__ float s_lse;
+  const int t = blockIdx.x;
+  const T* row = logits + (int64_t)t * ld;
+  const Stats st = merge_parts(ws, t, parts);
+  if (threadIdx.x == 0) s_lse = write_row<T>(st, t, row, vocab, out);
+  __syncthreads();
+  const float lse = s_lse;
+  const LogitsSource<T> src{row, seg_max + (int64_t)t * seg_stride, SegSpan(row, vocab, 0, 1), vocab};
+  select_top<kBlock>(src, k, s, threadIdx.x, [&](int rank, float z, int index) {
+    top_logprobs[(int64_t)t * k + rank] = z - lse;
+    top_ids[(int64_t)t * k + rank] = index;
+  });
+}
+
+// Upstream gradients of a row's chosen tokens: k of them, and a label's.  Either may be absent (g null).
+struct TokenGrads {
+  const void* ids;  // [n][k]
+  const float* g;   // [n][k]
+  const void* labels;
+  const float* g_label;
+  int ids_i64, k, labels_i64;
+};
+
+// dz_j = sum_i g_i [j = id_i] - p_j (G + g_H (log p_j + H)), G the sum of the g of the ids in the vocabulary.
+// The row is streamed without a look at the ids; the few elements that have one are written again afterwards, from
+// logits that were read before (dlogits may be the logits' own storage).  Equal ids of a row add up in their order, in the
+// thread of the first of them, so that the result repeats bit for bit.  Rows are walked from the last to the first, as
+// the forward leaves them in the cache.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void tokens_grad_kernel(const T* logits, int64_t ld, int vocab, TokenGrads tg,
+                                                             const float* __restrict__ lse, const float* __restrict__ entropy,
+                                                             const float* __restrict__ g_entropy, T* dlogits, int64_t ld_d,
+                                                             int vec_ok, int parts) {
+  constexpr int kMost = kMaxTokenIds + 1, kSlots = (kMost + kBlock - 1) / kBlock;
+  __shared__ int ids[kMost];
+  __shared__ float gs[kMost];
+  __shared__ float red[kBlock / kWave];
+  const int b = gridDim.x - 1 - blockIdx.x, t = b / parts, part = b - t * parts, tid = threadIdx.x;
+  const T* row = logits + (int64_t)t * ld;
+  T* out = dlogits + (int64_t)t * ld_d;
+  constexpr int kPer = Row<T>::kPer;
+  const int with_label = tg.g_label != nullptr, n_ids = (tg.g != nullptr ? tg.k : 0) + with_label;
+  float sum = 0.f;
+  for (int i = tid; i < n_ids; i += kBlock) {
+    const bool lab = with_label && i == 0;
+    const int64_t at = (int64_t)t * tg.k + i - with_label;
+    const int64_t id = lab ? load_id(tg.labels, tg.labels_i64, t) : load_id(tg.ids, tg.ids_i64, at);
+    const bool ok = id >= 0 && id < vocab;
+    const float g = !ok ? 0.f : lab ? tg.g_label[t] : tg.g[at];
+    ids[i] = ok ? (int)id : -1;
+    gs[i] = g;
+    sum += g;
+  }
+  sum = wave_sum(sum);
+  if ((tid & (kWave - 1)) == 0) red[tid / kWave] = sum;
+  __syncthreads();
+  const float G = (red[0] + red[1]) + (red[2] + red[3]);
+  const float lse_v = lse[t], g_en = g_entropy ? g_entropy[t] : 0.f, H = g_entropy ? entropy[t] : 0.f;
+  auto grad = [&](float z) {
+    const float lp = z - lse_v, p = __expf(lp);
+    return p * ((p > 0.f) ? fmaf(-g_en, lp + H, -G) : -G);  // a probability of 0 takes nothing from the entropy
+  };
+  const RowSpan sp(row, vocab, vec_ok != 0, part, parts);
+  // the ids that are this part's, each in the thread of its first occurrence
+  float again[kSlots];
+  int where[kSlots];
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * kBlock;
+    where[u] = -1;
+    if (i >= n_ids) continue;
+    const int id = ids[i];
+    if (id < 0) continue;
+    const int in = id - sp.head, q = in / kPer;
+    const int single = in < 0 ? id : id - sp.n_vec * kPer;  // its number among the elements outside the vectors
+    const bool vec = in >= 0 && q < sp.n_vec;
+    if (vec ? (q < sp.q_lo || q >= sp.q_hi) : (single / kBlock % parts != part)) continue;
+    float total = 0.f;
+    bool first = true;
+    for (int j = 0; j < n_ids; ++j) {
+      if (ids[j] != id) continue;
+      if (j < i) { first = false; break; }
+      total += gs[j];
+    }
+    if (!first) continue;
+    where[u] = id;
+    again[u] = grad(Row<T>::one(row + id)) + total;
+  }
+  __syncthreads();  // nothing of the row is written before these are read
+  const T* body = row + sp.head;
+  T* body_out = out + sp.head;
+  auto finish = [&](int q, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = grad(v[j]);
+    Row<T>::store(body_out + (uint32_t)q * kPer, v);
+  };
+  int q = sp.q_hi - 1 - tid;
+  for (; q - kBlock >= sp.q_lo; q -= 2 * kBlock) {  // two loads in flight per thread
+    float v0[8], v1[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v0);
+    Row<T>::load(body + (uint32_t)(q - kBlock) * kPer, v1);
+    finish(q, v0);
+    finish(q - kBlock, v1);
+  }
+  for (; q >= sp.q_lo; q -= kBlock) {
+    float v[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v);
+    finish(q, v);
+  }
+  for (int i = part * kBlock + tid; i < sp.n_scalar; i += parts * kBlock) {
+    const int j = sp.scalar<T>(i);
+    Row<T>::store_one(out + j, grad(Row<T>::one(row + j)));
+  }
+  // the stores above are acknowledged before another thread of the workgroup writes the same element
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0)
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u)
+    if (where[u] >= 0) Row<T>::store_one(out + where[u], again[u]);
+}
+
+}  // namespace axon
+
+using namespace axon;
+
+namespace {
+
+// Workgroups per row: as in logits.hip, except that rows this few are always split (the second launch is there anyway).
+int row_parts(int64_t n, int64_t vocab, int elem_bytes) {
+  if (n >= 1536) return 1;
+  const int64_t fill = 8192 / (n > 0 ? n : 1), work = vocab * elem_bytes / (8 * 16 * kBlock);
+  const int64_t p = fill < work ? fill : work;
+  return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
+}
+
+constexpr int64_t kCacheBytes = int64_t(256) << 20;
+
+int elem_bytes(int dtype) { return dtype == AXON_LOGITS_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == AXON_LOGITS_F32 || dtype == AXON_LOGITS_BF16; }
+int64_t seg_stride(int dtype, int64_t vocab) {
+  const int64_t per = 16 / elem_bytes(dtype) * kSegVecs;
+  return (vocab + per - 1) / per;
+}
+
+int check_rows(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v) {
+  if (n < 0 || v <= 0 || ld < v || !dtype_ok(dtype)) return AXON_ERR_ARG;
+  if (n >= (int64_t)1 << 25 || v >= (int64_t)1 << 30) return AXON_ERR_SHAPE;  // rows times parts are a grid
+  if (n > 0 && (!logits || reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) != 0)) return AXON_ERR_ARG;
+  return AXON_OK;
+}
+
+int cached_from(int64_t n, int64_t vocab, int eb, int bwd_follows) {
+  const int64_t cached = bwd_follows ? kCacheBytes / (vocab * eb) : 0;
+  return (int)(cached < n ? n - cached : 0);
+}
+
+}  // namespace
+
+#define AXON_ROWS(dtype, CALL)                     \
+  do {                                             \
+    if ((dtype) == AXON_LOGITS_F32) CALL(float);   \
+    else CALL(unsigned short);                     \
+  } while (0)
+
+extern "C" int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
+  return n * (row_parts(n, vocab, elem_bytes(dtype)) * 3 + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
+}
+
+extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, int64_t k,
+                                   const void* labels, int labels_i64, float* logprob, float* entropy, float* lse,
+                                   float* top_logprobs, int64_t* top_ids, float* workspace, int64_t workspace_bytes,
+                                   int bwd_follows, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc != AXON_OK) return rc;
+  if (k < 1 || k > kMaxTop || k > vocab) return AXON_ERR_SHAPE;
+  if (n == 0) return AXON_OK;
+  if (!lse || !top_logprobs || !top_ids || !workspace || (logprob && !labels)) return AXON_ERR_ARG;
+  if (axon_logits_top_workspace_bytes(dtype, n, vocab) > workspace_bytes) return AXON_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
+  float* const seg_max = workspace + n * parts * 3;
+  const int stride = (int)seg_stride(dtype, vocab), from = cached_from(n, vocab, eb, bwd_follows);
+  const RowOut out{logprob, entropy, lse, labels, labels_i64};
+#define AXON_TOP(T)                                                                                                        \
+  do {                                                                                                                     \
+    hipLaunchKernelGGL((alternatives_stats_kernel<T, true>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,             \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, seg_max, stride, out, Picks{}, from); \
+    AXON_CHECK_LAUNCH();                                                                                                   \
+    hipLaunchKernelGGL((top_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld,  \
+                       (int)vocab, parts, workspace, seg_max, stride, (int)k, out, top_logprobs, top_ids);                 \
+  } while (0)
+  AXON_ROWS(dtype, AXON_TOP);
+#undef AXON_TOP
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int64_t axon_logits_tokens_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
+  const int parts = row_parts(n, vocab, elem_bytes(dtype));
+  return parts > 1 ? n * parts * 3 * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids,
+                                      int ids_i64, int64_t k, float* logprobs, float* entropy, float* lse, float* workspace,
+                                      int64_t workspace_bytes, int bwd_follows, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc != AXON_OK) return rc;
+  if (k < 1 || k > kMaxTokenIds) return AXON_ERR_SHAPE;
+  if (n == 0) return AXON_OK;
+  if (!lse || !ids || !logprobs) return AXON_ERR_ARG;
+  const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
+  const int64_t need = axon_logits_tokens_workspace_bytes(dtype, n, vocab);
+  if (need > 0 && (!workspace || need > workspace_bytes)) return AXON_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  const RowOut out{nullptr, entropy, lse, nullptr, 0};
+  const Picks picks{ids, ids_i64, (int)k, logprobs};
+  const int from = cached_from(n, vocab, eb, bwd_follows);
+#define AXON_TOKENS(T)                                                                                                      \
+  do {                                                                                                                      \
+    hipLaunchKernelGGL((alternatives_stats_kernel<T, false>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,             \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, nullptr, 0, out, picks, from);      \
+    AXON_CHECK_LAUNCH();                                                                                                    \
+    if (parts > 1)                                                                                                          \
+      hipLaunchKernelGGL((tokens_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),  \
+                         ld, (int)vocab, parts, workspace, out, picks);                                                     \
+  } while (0)
+  AXON_ROWS(dtype, AXON_TOKENS);
+#undef AXON_TOKENS
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids,
+                                      int ids_i64, int64_t k, const void* labels, int labels_i64, const float* lse,
+                                      const float* entropy, const float* g_ids, const float* g_label, const float* g_entropy,
+                                      void* dlogits, int64_t ld_d, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc != AXON_OK) return rc;
+  if (k < 0 || k > kMaxTokenIds) return AXON_ERR_SHAPE;
+  if (n == 0) return AXON_OK;
+  if (!lse || !dlogits || ld_d < vocab || reinterpret_cast<uintptr_t>(dlogits) % elem_bytes(dtype) != 0) return AXON_ERR_ARG;
+  if ((g_ids && !ids) || (g_label && !labels) || (g_entropy && !entropy)) return AXON_ERR_ARG;
+  const hipStream_t st = (hipStream_t)stream;
+  const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
+  // every row of dlogits sits on the same offset from a 16-byte boundary as the row of logits
+  const int vec_ok = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0 &&
+                     (n <= 1 || ((ld - ld_d) * eb) % 16 == 0);
+  const TokenGrads tg{ids, g_ids, labels, g_label, ids_i64, (int)k, labels_i64};
+#define AXON_GRAD(T)                                                                                                       \
+  hipLaunchKernelGGL((tokens_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,                             \
+                     static_cast<const T*>(logits), ld, (int)vocab, tg, lse, entropy, g_entropy, static_cast<T*>(dlogits), \
+                     ld_d, vec_ok, parts)
+  AXON_ROWS(dtype, AXON_GRAD);
+#undef AXON_GRAD
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}

@@ -1,0 +1,175 @@
+// The k largest of a row, exactly, equal values by ascending index, without looking at the whole row again.
+//
+// A row is cut into segments of consecutive elements, whose maxima the pass that reads the row anyway has left.  Ordered
+// by (maximum descending, index ascending), the first k segments hold the k first elements by (value descending, index
+// ascending): an element of any other segment has k segments before its own, and the maximum of each of them comes
+// before it.  So the maxima are selected from first, then the elements of k segments, those only that reach the smallest
+// of the k maxima: about as many as are wanted.
+#pragma once
+#include "common.h"
+
+namespace axon {
+
+constexpr int kMaxTop = 128;       // alternatives per row
+constexpr int kCandidates = 1024;  // elements that reach the smallest of the k maxima and are ranked against each other
+
+// Unsigned integers in the order of the floats; -0 equals 0, NaN is below everything.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return x != x ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+// ... and of (value descending, index ascending)
+__device__ __forceinline__ uint64_t order_key(float x, int index) {
+  return ((uint64_t)order_key(x) << 32) | (0xffffffffu - (uint32_t)index);
+}
+
+struct SelectLds {
+  uint64_t cand[kCandidates];
+  int hist[256];
+  int segs[kMaxTop], equal[kMaxTop];
+  int n_segs, n_equal, n_cand, bin, before;
+};
+
+// NT threads work on a row: a wavefront (64), whose LDS accesses are carried out in order, or a workgroup.
+template <int NT>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (NT == kWave) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  else __syncthreads();
+}
+
+// The k-th largest of n keys (1 <= k <= n), eight bits at a time; `ties`: how many of the keys equal to it are among
+// the k.  key_at(i) is asked for every i once per eight bits.
+template <int NT, class Key, class KeyAt>
+__device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds& s, int tid, int& ties) {
+  Key prefix = 0, mask = 0;
+  int rest = k;
+  for (int shift = 8 * (int)sizeof(Key) - 8; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+    group_sync<NT>();
+    for (int i = tid; i < n; i += NT) {
+      const Key key = key_at(i);
+      if ((key & mask) == prefix) atomicAdd(&s.hist[(int)(key >> shift) & 255], 1);
+    }
+    group_sync<NT>();
+    if (tid < kWave) {  // lane l: bins 255 - 4 l and the three below
+      int c[4], sum = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
+      int upto = sum;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int o = __shfl_up(upto, off, kWave);
+        if (tid >= off) upto += o;
+      }
+      int before = upto - sum;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; }
+        before += c[q];
+      }
+    }
+    group_sync<NT>();
+    prefix |= (Key)s.bin << shift;
+    mask |= (Key)255 << shift;
+    rest -= s.before;
+  }
+  ties = rest;
+  return prefix;
+}
+
+// `src`: maxima of its segments, max_key(i) for i < n_segs(); the elements of the segments in `segs`, kPer consecutive ones
+// per item: load(segs, j, v) returns the index of the first, or -1 where there is none (elements from limit() on do not
+// count); and n_single() elements outside all segments, single(i, index).  out(rank, value, index) for rank < k.
+template <int NT, class Src, class Out>
+__device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, int tid, Out out) {
+  const int n = src.n_segs();
+  uint32_t least = 0;  // what an element has to reach
+  if (tid == 0) s.n_segs = s.n_equal = s.n_cand = 0;
+  if (n > k) {
+    int ties;
+    auto key_at = [&](int i) { return src.max_key(i); };
+    least = kth_largest<NT, uint32_t>(key_at, n, k, s, tid, ties);
+    for (int i = tid; i < n; i += NT) {
+      const uint32_t key = key_at(i);
+      if (key > least) s.segs[atomicAdd(&s.n_segs, 1)] = i;  // fewer than k
+      if (key == least) {
+        const int at = atomicAdd(&s.n_equal, 1);
+        if (at < ties) s.equal[at] = i;
+      }
+    }
+    group_sync<NT>();
+    if (s.n_equal == ties) {
+      const int at = s.n_segs;
+      group_sync<NT>();
+      for (int i = tid; i < ties; i += NT) s.segs[at + i] = s.equal[i];
+    } else {  // more segments with that maximum than are wanted: the first of them
+      int one;
+      auto first = [&](int i) { return key_at(i) == least ? 0xffffffffu - (uint32_t)i : 0u; };
+      const uint32_t last = kth_largest<NT, uint32_t>(first, n, ties, s, tid, one);
+      for (int i = tid; i < n; i += NT)
+        if (first(i) >= last) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+    }
+  } else {
+    for (int i = tid; i < n; i += NT) s.segs[i] = i;
+  }
+  group_sync<NT>();
+  const int n_items = (n < k ? n : k) * Src::kItems, limit = src.limit();
+  auto offer = [&](float x, int index) {
+    if (order_key(x) < least) return;
+    const int at = atomicAdd(&s.n_cand, 1);
+    if (at < kCandidates) s.cand[at] = order_key(x, index);
+  };
+  for (int j = tid; j < n_items; j += NT) {
+    float v[Src::kPer];
+    const int i0 = src.load(s.segs, j, v);
+    if (i0 < 0) continue;
+#pragma unroll
+    for (int e = 0; e < Src::kPer; ++e)
+      if (i0 + e < limit) offer(v[e], i0 + e);
+  }
+  for (int i = tid; i < src.n_single(); i += NT) {
+    int index;
+    const float x = src.single(i, index);
+    offer(x, index);
+  }
+  group_sync<NT>();
+  int c = s.n_cand;
+  if (c > kCandidates) {  // a run of equal values, as a rule: the k-th key itself, from the elements of the segments
+    const int n_el = n_items * Src::kPer + src.n_single();
+    auto element = [&](int i) -> uint64_t {
+      if (i >= n_items * Src::kPer) {
+        int index;
+        const float x = src.single(i - n_items * Src::kPer, index);
+        return order_key(x, index);
+      }
+      float v[Src::kPer];
+      const int i0 = src.load(s.segs, i / Src::kPer, v), e = i % Src::kPer;
+      if (i0 < 0 || i0 + e >= limit) return 0;
+      float x = v[0];
+#pragma unroll
+      for (int q = 1; q < Src::kPer; ++q) x = e == q ? v[q] : x;
+      return order_key(x, i0 + e);
+    };
+    int one;
+    const uint64_t last = kth_largest<NT, uint64_t>(element, n_el, k, s, tid, one);
+    if (tid == 0) s.n_cand = 0;
+    group_sync<NT>();
+    for (int i = tid; i < n_el; i += NT) {
+      const uint64_t key = element(i);
+      if (key >= last) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+    }
+    group_sync<NT>();
+    c = k;
+  }
+  for (int i = tid; i < c; i += NT) {
+    const uint64_t mine = s.cand[i];
+    int rank = 0;
+    for (int j = 0; j < c; ++j) rank += s.cand[j] > mine;
+    if (rank < k) out(rank, key_value((uint32_t)(mine >> 32)), (int)(0xffffffffu - (uint32_t)mine));
+  }
+}
+
+}  // namespace axon

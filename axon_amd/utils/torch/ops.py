@@ -7,16 +7,23 @@ kernel reads each row once for both quantities; the backward reads it once more 
 over the logits themselves when ``inplace_backward`` is set (the behaviour of the flash-attn cross entropy
 the reference prefers, :70-75).  ``logprobs_and_entropy_from_logits`` returns both from a single pass and
 has a single backward; the reference runs two functions over the same logits.
+
+Two functions have no counterpart in the reference, which knows one token per position:
+``top_logprobs_from_logits`` returns the best alternatives of every position beside the label's log-probability and
+the entropy (a teacher's scores, a decoder's report), ``token_logprobs_from_logits`` the log-probabilities of several
+given tokens per position (a student's side of it).  Both are differentiable.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
 from axon_amd import _ops
 
 __all__ = ["logprobs_from_logits", "entropy_from_logits", "entropy_from_logits_with_chunking",
-           "logprobs_and_entropy_from_logits"]
+           "logprobs_and_entropy_from_logits", "TopLogprobs", "top_logprobs_from_logits", "token_logprobs_from_logits"]
 
 
 def _rows(logits):
@@ -71,3 +78,78 @@ def entropy_from_logits_with_chunking(logits: torch.Tensor, chunk_size: int = 20
     """Same values as ``entropy_from_logits`` (ops.py:112-120); the reference chunks over tokens to bound its
     fp32 temporaries, of which there are none here, so ``chunk_size`` is accepted and not used."""
     return entropy_from_logits(logits)
+
+
+class TopLogprobs(NamedTuple):
+    """What is known of every position: fp32 ``[...]`` log-probability of its label (None without labels) and entropy,
+    fp32 ``[..., k]`` log-probabilities and int64 ``[..., k]`` ids of its k best tokens, best first."""
+
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def _distinct_rows(logits):
+    """``[rows, vocab]`` with rows that do not share storage."""
+    if logits.dim() < 1:
+        raise ValueError("logits must be [..., vocab]")
+    flat = _rows(logits)
+    return flat.contiguous() if flat.shape[0] > 1 and flat.stride(0) < flat.shape[1] else flat
+
+
+class _Alternatives(torch.autograd.Function):
+    """The k largest logits of every row (``ids`` None) or given ones, their log-probabilities and what goes with them."""
+
+    @staticmethod
+    def forward(ctx, logits, k, ids, labels, inplace_backward):
+        flat = _distinct_rows(logits)
+        batch = logits.shape[:-1]
+        ctx.set_materialize_grads(False)
+        lab = labels.reshape(-1).contiguous() if labels is not None else None
+        if ids is None:
+            logprob, entropy, lse, top_logprobs, ids = _ops.logits_top(flat, k, lab, ctx.needs_input_grad[0])
+            top_ids = ids.view(*batch, k)
+            ctx.mark_non_differentiable(top_ids)
+        else:
+            ids = ids.reshape(flat.shape[0], ids.shape[-1])
+            top_logprobs, entropy, lse = _ops.logits_tokens(flat, ids, ctx.needs_input_grad[0])
+            logprob = top_ids = None
+        ctx.save_for_backward(flat, ids, lab, lse, entropy)
+        ctx.shape, ctx.spent = logits.shape, False
+        # writing the gradient over the logits is only possible when `flat` is the caller's storage
+        ctx.inplace = bool(inplace_backward) and flat.data_ptr() == logits.data_ptr()
+        return (logprob.view(batch) if logprob is not None else None, entropy.view(batch),
+                top_logprobs.view(*batch, top_logprobs.shape[-1]), top_ids)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprob, g_entropy, g_top, _g_ids):
+        if g_logprob is None and g_entropy is None and g_top is None:
+            return (None,) * 5
+        if ctx.spent:
+            raise RuntimeError("the logits' storage holds the gradient of an earlier backward (inplace_backward)")
+        flat, ids, lab, lse, entropy = ctx.saved_tensors
+        ctx.spent = ctx.inplace
+        grad = _ops.logits_tokens_backward(flat, ids, lab, lse, entropy, g_top, g_logprob, g_entropy, inplace=ctx.inplace)
+        return grad.view(ctx.shape), None, None, None, None
+
+
+def top_logprobs_from_logits(logits: torch.Tensor, k: int, labels: torch.Tensor | None = None,
+                             inplace_backward: bool = False) -> TopLogprobs:
+    """The ``k`` best tokens (at most 128) of every position of ``logits`` ``[..., vocab]`` (fp32 or bf16, already divided
+    by the temperature): see ``TopLogprobs``.  Equal logits are ordered by ascending id.  ``labels`` ``[...]``: also the
+    log-probability of these (0 for a label outside the vocabulary).  Differentiable with respect to the logits; the
+    ids are constants.  A position whose logits hold a NaN, or nothing but -inf, has NaN log-probabilities."""
+    return TopLogprobs(*_Alternatives.apply(logits, k, None, labels, inplace_backward))
+
+
+def token_logprobs_from_logits(logits: torch.Tensor, token_ids: torch.Tensor, inplace_backward: bool = False):
+    """``(logprobs [..., k], entropy [...])``: the log-probabilities of ``k`` given tokens per position (at most 512, int32
+    or int64 ``[..., k]``; an id outside the vocabulary is a filler: its log-probability is 0 and its gradient goes
+    nowhere) and the entropy, fp32, from one read of ``logits`` ``[..., vocab]``.  Differentiable with respect to the
+    logits; ids may occur more than once in a position."""
+    if token_ids.dim() != logits.dim() or token_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"token_ids {tuple(token_ids.shape)} do not lie beside logits {tuple(logits.shape)}")
+    _, entropy, logprobs, _ = _Alternatives.apply(logits, 0, token_ids, None, inplace_backward)
+    return logprobs, entropy

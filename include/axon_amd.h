@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define AXON_AMD_ABI_VERSION 25
+#define AXON_AMD_ABI_VERSION 26
 
 enum {
   AXON_OK = 0,
@@ -647,6 +647,34 @@ int axon_logits_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_
                     const void* labels, int labels_are_i64, const float* lse, const float* entropy,
                     const float* g_logprob, const float* g_entropy, void* dlogits, int64_t ld_dlogits,
                     void* stream);
+
+/* Alternatives of materialised logits (no reference counterpart; the reference's logprobs_from_logits,
+ * axon/utils/torch/ops.py:39-102, knows one token per position).  Operands as above, logits aligned to their element.
+ *   _top_fwd: the k largest logits of every row (1 <= k <= 128, k <= vocab), in descending order, equal ones by
+ *        ascending id: top_ids [n][k] int64 and top_logprobs [n][k] = logit - lse; beside them logprob (with labels),
+ *        entropy (either may be NULL) and lse.  A row with a NaN has NaN everywhere but in top_ids, which then rank
+ *        the NaN below everything; a row of -inf alone has NaN log-probabilities and the lowest ids.
+ *   _tokens_fwd: logprobs [n][k] of the given ids [n][k] (int32 or int64, 1 <= k <= 512), 0 for an id outside
+ *        [0, vocab); entropy may be NULL.
+ *   _tokens_bwd: the backward of both, one read and one write of the rows:
+ *        dlogits[t][j] = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_entropy[t] (log p_j + entropy[t])),
+ *        i over ids [n][k] with g_ids [n][k] and the label with g_label [n]; either pair and g_entropy may be NULL.
+ *        Ids outside the vocabulary are left out, equal ids of a row add up.  In the logits' dtype; dlogits may be the
+ *        logits' own storage.
+ *   Workspace: 4-byte aligned, its contents do not matter.  bwd_follows: as axon_logits_fwd_train. */
+int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t vocab);
+int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, int64_t k,
+                        const void* labels, int labels_are_i64, float* logprob, float* entropy, float* lse,
+                        float* top_logprobs, int64_t* top_ids, float* workspace, int64_t workspace_bytes,
+                        int bwd_follows, void* stream);
+int64_t axon_logits_tokens_workspace_bytes(int dtype, int64_t n, int64_t vocab);
+int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids,
+                           int ids_are_i64, int64_t k, float* logprobs, float* entropy, float* lse,
+                           float* workspace, int64_t workspace_bytes, int bwd_follows, void* stream);
+int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids,
+                           int ids_are_i64, int64_t k, const void* labels, int labels_are_i64, const float* lse,
+                           const float* entropy, const float* g_ids, const float* g_label, const float* g_entropy,
+                           void* dlogits, int64_t ld_dlogits, void* stream);
 
 /* KL penalty inside the reward, the tensor part of apply_kl_penalty (axon/utils/rl/kl.py:276-322):
  *   kld = kl_penalty(old_logp, ref_logp, kl_type) * mask      (types as in axon_kl_penalty)

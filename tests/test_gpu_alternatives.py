@@ -1,0 +1,342 @@
+"""Top alternatives and log-probabilities of given tokens from materialised logits, against the same in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from axon_amd import _ops
+from axon_amd.utils.torch.ops import (logprobs_and_entropy_from_logits, token_logprobs_from_logits,
+                                      top_logprobs_from_logits)
+
+pytestmark = pytest.mark.gpu
+
+# How far a log-probability may be off, |logit| <= 32: the sum of exponentials is added up in chains of at most 300
+# roundings of 2^-24 (2e-5 at the worst, were they all of one sign: 300 * 6e-8), each exponential is off by the rounding
+# of an argument of up to 60 in 2^-24 and by 2^-22 (4e-6, weighted by its probability), the final additions by four
+# roundings of a number of up to 46 (1.1e-5).
+LP_TOL = 4e-5
+# The entropy is formed from the same sums, its terms weighted by up to |log p|, of which 12 is the average at most.
+ENT_TOL = 12 * 2e-5
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def logits_of(pattern, n, v, dtype, seed):
+    g = gen(seed)
+    z = torch.randn(n, v, generator=g, device="cuda") * 3
+    if pattern == "constant":
+        z = torch.full_like(z, 0.75)
+    elif pattern == "few_values":
+        z = torch.randint(-1, 2, (n, v), generator=g, device="cuda").float()
+    elif pattern == "rising":
+        z = torch.arange(v, device="cuda").float().expand(n, v) * (16.0 / v)
+    elif pattern == "falling":
+        z = torch.arange(v, 0, -1, device="cuda").float().expand(n, v) * (16.0 / v)
+    elif pattern == "signed_zero":
+        z = torch.where(torch.rand(n, v, generator=g, device="cuda") < 0.5, 0.0, -0.0)
+    elif pattern == "banned":
+        z[torch.rand(n, v, generator=g, device="cuda") < 0.9] = -math.inf
+        z[:, v // 2] = 1.0
+    elif pattern == "one_block":  # all that is large lies in one run
+        z[:, v // 3: v // 3 + 300] += 20.0
+    elif pattern == "peaked":
+        z[:, v // 2] += 25.0
+    return z.clamp(-math.inf, 31.0).to(dtype).contiguous()
+
+
+def reference(z, ids, g_ids=None, g_ent=None):
+    """Log-probabilities of ids (0 outside the vocabulary), entropy; the gradient and the size of its terms."""
+    z = z.double()
+    log_p = torch.log_softmax(z, 1)
+    p = log_p.exp()
+    plogp = torch.where(p > 0, p * log_p, torch.zeros_like(p))
+    ent = -plogp.sum(1)
+    ok = (ids >= 0) & (ids < z.shape[1])
+    at = torch.where(ok, ids, torch.zeros_like(ids)).long()
+    lp = torch.where(ok, log_p.gather(1, at), torch.zeros((), dtype=torch.float64, device=z.device))
+    if g_ids is None:
+        return lp, ent
+    up = torch.where(ok, g_ids.double(), torch.zeros((), dtype=torch.float64, device=z.device))
+    onehot = torch.zeros_like(z).scatter_add_(1, at, up)
+    G, ge = up.sum(1, keepdim=True), g_ent.double()[:, None]
+    grad = onehot - p * G - ge * (plogp + p * ent[:, None])
+    size = (torch.zeros_like(z).scatter_add_(1, at, up.abs()) + p * up.abs().sum(1, keepdim=True)
+            + ge.abs() * (plogp.abs() + p * (ent[:, None] + 1)))
+    return lp, ent, grad, size
+
+
+def order(z, k):
+    return torch.sort(z.double() + 0.0, dim=1, descending=True, stable=True).indices[:, :k]
+
+
+def check_grad(got, ref, size, dtype):
+    """A probability's relative error is that of its logarithm (LP_TOL) and of two roundings; a bf16 gradient is rounded
+    once more (2^-8)."""
+    bound = 2 * ENT_TOL * size + 1e-30
+    if dtype == torch.bfloat16:
+        bound = bound + 2.0 ** -8 * ref.abs()
+    worst = ((got.double() - ref).abs() / bound).max().item()
+    assert worst <= 1.0, worst
+
+
+def laid_out(z, layout):
+    """The same values in another place: rows further apart, off a 16-byte boundary, or with another dimension."""
+    n, v = z.shape
+    if layout == "plain":
+        return z
+    if layout == "strided":
+        buf = torch.full((n, v + 5), 99.0, device=z.device, dtype=z.dtype)
+        buf[:, :v] = z
+        return buf[:, :v]
+    buf = torch.full((n * v + 3,), 99.0, device=z.device, dtype=z.dtype)
+    buf[3:] = z.reshape(-1)
+    return buf[3:].view(n, v)
+
+
+TOP_CASES = [
+    # n, vocab, k, dtype, pattern, layout
+    (1, 1, 1, torch.float32, "random", "plain"),
+    (3, 5, 5, torch.bfloat16, "random", "shifted"),
+    (2, 17, 3, torch.float32, "random", "shifted"),
+    (5, 127, 64, torch.bfloat16, "few_values", "plain"),
+    (4, 129, 128, torch.float32, "random", "strided"),
+    (7, 1000, 20, torch.bfloat16, "constant", "plain"),
+    (3, 4099, 128, torch.bfloat16, "constant", "shifted"),
+    (2, 40000, 128, torch.float32, "constant", "plain"),
+    (3, 40000, 128, torch.bfloat16, "few_values", "strided"),
+    (6, 4099, 20, torch.float32, "rising", "plain"),
+    (6, 4099, 20, torch.float32, "falling", "strided"),
+    (3, 50257, 128, torch.bfloat16, "one_block", "plain"),
+    (2, 33000, 128, torch.float32, "one_block", "shifted"),
+    (5, 3001, 100, torch.float32, "signed_zero", "plain"),
+    (9, 2048, 50, torch.bfloat16, "banned", "plain"),
+    (3, 600, 128, torch.float32, "banned", "plain"),
+    (1, 151936, 20, torch.bfloat16, "random", "plain"),
+    (3, 201088, 5, torch.float32, "peaked", "plain"),
+    (61, 50257, 7, torch.bfloat16, "random", "plain"),
+    (1600, 777, 33, torch.bfloat16, "random", "plain"),
+    (1537, 2051, 1, torch.float32, "few_values", "plain"),
+]
+
+
+@pytest.mark.parametrize("n,v,k,dtype,pattern,layout", TOP_CASES)
+def test_top_alternatives(n, v, k, dtype, pattern, layout):
+    z = logits_of(pattern, n, v, dtype, 11 * n + v)
+    ids = order(z, k)
+    labels = torch.randint(0, v, (n,), generator=gen(5), device="cuda")
+    labels[-1] = v if n > 1 else 0  # a label outside the vocabulary
+    lp, ent = reference(z, torch.cat([ids, labels[:, None]], 1))
+    r = top_logprobs_from_logits(laid_out(z, layout), k, labels)
+    assert r.top_ids.dtype == torch.int64 and torch.equal(r.top_ids, ids)
+    both = torch.cat([r.top_logprobs, r.logprobs[:, None]], 1).double()
+    finite = torch.isfinite(lp)
+    assert torch.equal(torch.isfinite(both), finite)
+    assert (both - lp)[finite].abs().max() <= LP_TOL and (both[~finite] == -math.inf).all()
+    assert (r.entropy.double() - ent).abs().max() <= ENT_TOL
+    bare = top_logprobs_from_logits(z, k)
+    assert bare.logprobs is None and torch.equal(bare.top_ids, ids)
+
+
+def test_rows_without_a_softmax():
+    """NaN and infinities stay in their row; ids are valid wherever the values are not."""
+    z = logits_of("random", 5, 3000, torch.float32, 3)
+    good = top_logprobs_from_logits(z, 9)
+    z[0, 77] = math.nan
+    z[1] = -math.inf
+    z[2, 5] = math.inf
+    z[3] = math.nan
+    r = top_logprobs_from_logits(z, 9)
+    assert torch.isnan(r.top_logprobs[[0, 1, 3]]).all() and torch.isnan(r.entropy[[0, 1, 2, 3]]).all()
+    assert torch.isnan(r.top_logprobs[2, 0])
+    assert torch.equal(r.top_ids[1], torch.arange(9, device="cuda")) and torch.equal(r.top_ids[3], torch.arange(9, device="cuda"))
+    assert r.top_ids[2, 0] == 5 and 77 not in r.top_ids[0].tolist()
+    assert torch.equal(r.top_ids[4], good.top_ids[4]) and torch.equal(r.top_logprobs[4], good.top_logprobs[4])
+
+
+GRAD_CASES = [
+    (1, 9, 3, torch.float32, "random", "plain"),
+    (3, 129, 20, torch.bfloat16, "random", "shifted"),
+    (61, 4099, 64, torch.bfloat16, "random", "plain"),
+    (5, 3000, 20, torch.float32, "banned", "strided"),
+    (2, 40000, 128, torch.bfloat16, "constant", "plain"),
+    (187, 50257, 8, torch.float32, "peaked", "plain"),
+    (1540, 515, 5, torch.bfloat16, "random", "plain"),
+]
+
+
+@pytest.mark.parametrize("n,v,k,dtype,pattern,layout", GRAD_CASES)
+def test_top_alternatives_gradient(n, v, k, dtype, pattern, layout):
+    z = logits_of(pattern, n, v, dtype, n + v)
+    g = gen(n)
+    g_top, g_lp, g_en = (torch.randn(*s, generator=g, device="cuda") for s in ((n, k), (n,), (n,)))
+    labels = torch.randint(0, v, (n,), generator=g, device="cuda", dtype=torch.int32)
+    labels[0] = order(z, 1)[0, 0]  # a label that is an alternative too
+    labels[-1] = -100
+    x = laid_out(z, layout).requires_grad_(True)
+    r = top_logprobs_from_logits(x, k, labels)
+    got, = torch.autograd.grad([r.top_logprobs, r.logprobs, r.entropy], x, [g_top, g_lp, g_en])
+    assert got.dtype == dtype and got.shape == x.shape
+    ids = torch.cat([labels[:, None].long(), order(z, k)], 1)
+    _, _, ref, size = reference(z, ids, torch.cat([g_lp[:, None], g_top], 1), g_en)
+    check_grad(got, ref, size, dtype)
+
+
+@pytest.mark.parametrize("n,v,k,dtype,layout,ids_dtype", [
+    (1, 1, 1, torch.float32, "plain", torch.int64),
+    (4, 33, 40, torch.bfloat16, "shifted", torch.int32),  # more ids than tokens: repeats
+    (3, 1000, 512, torch.float32, "plain", torch.int64),
+    (50, 32768, 16, torch.bfloat16, "strided", torch.int64),
+    (187, 151936, 8, torch.bfloat16, "plain", torch.int32),
+    (1600, 777, 20, torch.float32, "plain", torch.int64),
+])
+def test_given_tokens(n, v, k, dtype, layout, ids_dtype):
+    z = logits_of("random", n, v, dtype, n + 7 * v)
+    g = gen(v)
+    ids = torch.randint(-2, v + 2, (n, k), generator=g, device="cuda").clamp(max=v + 1).to(ids_dtype)
+    if v > 2:
+        ids[0, 0], ids[0, -1] = v - 1, v - 1
+    g_ids, g_en = torch.randn(n, k, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    lp, ent, ref, size = reference(z, ids, g_ids, g_en)
+    for inplace in (False, True):
+        x = laid_out(z.clone(), layout).requires_grad_(True)
+        got_lp, got_ent = token_logprobs_from_logits(x, ids, inplace_backward=inplace)
+        assert (got_lp.double() - lp).abs().max() <= LP_TOL and (got_ent.double() - ent).abs().max() <= ENT_TOL
+        got, = torch.autograd.grad([got_lp, got_ent], x, [g_ids, g_en])
+        assert (got.data_ptr() == x.data_ptr()) == inplace
+        check_grad(got, ref, size, dtype)
+        if inplace and layout == "strided":  # what lies between the rows is left as it was
+            assert (x.detach().as_strided((n, v + 5), (v + 5, 1))[:-1, v:] == 99.0).all()
+
+
+def test_gradients_agree_with_differences():
+    n, v, k = 3, 40, 6
+    g = gen(1)
+    z = torch.randn(n, v, generator=g, device="cuda")
+    ids = torch.randint(0, v, (n, k), generator=g, device="cuda")
+    w, we = torch.randn(n, k, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    x = z.clone().requires_grad_(True)
+    lp, ent = token_logprobs_from_logits(x, ids)
+    grad, = torch.autograd.grad((lp * w).sum() + (ent * we).sum(), x)
+
+    def value(zz):
+        a, b = reference(zz, ids)
+        return ((a * w).sum() + (b * we).sum()).item()
+
+    for t, j in ((0, 0), (0, int(ids[0, 0])), (1, 7), (2, 39), (2, int(ids[2, 3]))):
+        h = 1e-5
+        up, down = z.double().clone(), z.double().clone()
+        up[t, j] += h
+        down[t, j] -= h
+        # the difference's own error is h^2 times a third derivative, and 1e-16 * |value| / h
+        assert abs((value(up) - value(down)) / (2 * h) - grad[t, j].item()) <= 1e-4
+
+
+def test_one_gradient_at_a_time_and_leading_dimensions():
+    z = logits_of("random", 6, 500, torch.float32, 8)
+    x = z.view(2, 3, 500).clone().requires_grad_(True)
+    r = top_logprobs_from_logits(x, 4, torch.zeros(2, 3, dtype=torch.int64, device="cuda"))
+    assert r.top_ids.shape == (2, 3, 4) and r.logprobs.shape == r.entropy.shape == (2, 3)
+    assert not r.top_ids.requires_grad and r.top_logprobs.requires_grad
+    ids, none = order(z, 4), torch.zeros(6, 4, device="cuda")
+    zero = torch.zeros(6, device="cuda")
+    one, = torch.autograd.grad(r.top_logprobs.sum(), x, retain_graph=True)
+    _, _, ref, size = reference(z, ids, none + 1, zero)
+    check_grad(one.view(6, 500), ref, size, torch.float32)
+    one, = torch.autograd.grad(r.entropy.sum(), x, retain_graph=True)
+    _, _, ref, size = reference(z, ids, none, zero + 1)
+    check_grad(one.view(6, 500), ref, size, torch.float32)
+    one, = torch.autograd.grad(r.logprobs.sum(), x)
+    _, _, ref, size = reference(z, torch.zeros(6, 1, dtype=torch.int64, device="cuda"), zero[:, None] + 1, zero)
+    check_grad(one.view(6, 500), ref, size, torch.float32)
+
+
+def test_agrees_with_the_operator_for_one_label():
+    """One given token per position is what logprobs_and_entropy_from_logits computes; the two read a row in the same
+    order, and differ by the roundings of LP_TOL at most."""
+    z = logits_of("random", 33, 5000, torch.bfloat16, 2)
+    lab = torch.randint(0, 5000, (33,), generator=gen(3), device="cuda")
+    a, b = logprobs_and_entropy_from_logits(z, lab), token_logprobs_from_logits(z, lab[:, None])
+    assert (a[0] - b[0][:, 0]).abs().max() <= LP_TOL and (a[1] - b[1]).abs().max() <= ENT_TOL
+
+
+def test_expanded_rows_and_empty_batches():
+    row = logits_of("random", 1, 700, torch.float32, 4)
+    x = row.clone().requires_grad_(True)
+    r = top_logprobs_from_logits(x.expand(5, 700), 3, inplace_backward=True)
+    assert torch.equal(r.top_ids, order(row, 3).expand(5, 3))
+    got, = torch.autograd.grad(r.top_logprobs.sum(), x)
+    _, _, ref, size = reference(row, order(row, 3), torch.full((1, 3), 5.0, device="cuda"), torch.zeros(1, device="cuda"))
+    check_grad(got, ref, size, torch.float32)
+    e = torch.empty(0, 700, device="cuda", requires_grad=True)
+    r = top_logprobs_from_logits(e, 3, torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert r.top_ids.shape == (0, 3) and r.logprobs.shape == (0,)
+    lp, ent = token_logprobs_from_logits(e, torch.empty(0, 2, dtype=torch.int64, device="cuda"))
+    assert lp.shape == (0, 2)
+    assert torch.autograd.grad(lp.sum() + ent.sum(), e)[0].shape == (0, 700)
+
+
+def test_an_inplace_backward_runs_once():
+    x = logits_of("random", 3, 300, torch.float32, 1).requires_grad_(True)
+    lp, _ = token_logprobs_from_logits(x, torch.zeros(3, 1, dtype=torch.int64, device="cuda"), inplace_backward=True)
+    torch.autograd.grad(lp.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="inplace_backward"):
+        torch.autograd.grad(lp.sum(), x)
+
+
+def test_results_repeat_bit_for_bit():
+    z = logits_of("random", 40, 50257, torch.bfloat16, 6)
+    ids = torch.randint(0, 3, (40, 64), generator=gen(2), device="cuda")  # many repeats
+    g_ids, g_en = torch.randn(40, 64, generator=gen(3), device="cuda"), torch.randn(40, generator=gen(4), device="cuda")
+
+    def once():
+        x = z.clone().requires_grad_(True)
+        lp, ent = token_logprobs_from_logits(x, ids)
+        r = top_logprobs_from_logits(z, 64)
+        return [lp.detach(), ent.detach(), r.top_logprobs, r.top_ids,
+                torch.autograd.grad([lp, ent], x, [g_ids, g_en])[0]]
+
+    first = once()
+    for _ in range(3):
+        for a, b in zip(first, once()):
+            assert torch.equal(a, b)
+
+
+def test_captured_and_replayed():
+    """Forward and backward as a graph, replayed on other inputs with eager work between the replays."""
+    n, v, k = 30, 32768, 12
+    z = torch.empty(n, v, device="cuda", dtype=torch.bfloat16)
+    g_top, g_en = torch.randn(n, k, generator=gen(1), device="cuda"), torch.randn(n, generator=gen(2), device="cuda")
+
+    def step():
+        _, ent, lse, lp, ids = _ops.logits_top(z, k)
+        return lp, ent, ids, _ops.logits_tokens_backward(z, ids, None, lse, ent, g_top, None, g_en)
+
+    z.copy_(logits_of("random", n, v, torch.bfloat16, 1))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (2, 3, 4):
+        z.copy_(logits_of("few_values" if seed == 3 else "random", n, v, torch.bfloat16, seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_on_another_stream():
+    z = logits_of("random", 64, 50257, torch.bfloat16, 9)
+    want = top_logprobs_from_logits(z, 10)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = top_logprobs_from_logits(z, 10)
+    side.synchronize()
+    assert torch.equal(got.top_ids, want.top_ids) and torch.equal(got.top_logprobs, want.top_logprobs)
