@@ -56,7 +56,7 @@ def rows_of(t: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> Rows:
     return Rows(int(b), int(b * s), int(s), None, tuple(t.shape))
 
 
-def _on_16_bytes(t: torch.Tensor) -> torch.Tensor:
+def on_16_bytes(t: torch.Tensor) -> torch.Tensor:
     """The kernels move four values per access: a view that starts off a 16-byte boundary is copied."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -66,7 +66,7 @@ def f32(t: torch.Tensor) -> torch.Tensor:
         t = t.detach()
     if t.dtype != torch.float32 or not t.is_contiguous():  # the usual operand passes through untouched
         t = t.to(torch.float32).contiguous()
-    return _on_16_bytes(t)
+    return on_16_bytes(t)
 
 
 def mask_arg(mask: torch.Tensor):
@@ -76,10 +76,10 @@ def mask_arg(mask: torch.Tensor):
     if not mask.is_contiguous():
         mask = mask.contiguous()
     if mask.dtype == torch.int64:
-        return _on_16_bytes(mask), MASK_I64
+        return on_16_bytes(mask), MASK_I64
     if mask.dtype != torch.float32:
         mask = mask.to(torch.float32)
-    return _on_16_bytes(mask), MASK_F32
+    return on_16_bytes(mask), MASK_F32
 
 
 def _same_len(what: str, n: int, **tensors) -> None:
@@ -708,11 +708,11 @@ def _head_operands(what, hidden, weight, labels, seq_start):
         raise ValueError(f"{what}: hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
     if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise ValueError(f"{what}: hidden and weight must be bf16")
-    if labels.dtype not in (torch.int32, torch.int64):
+    if labels is not None and labels.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: labels must be int32 or int64")
-    if not (hidden.is_contiguous() and weight.is_contiguous() and labels.is_contiguous()):
+    if not all(t.is_contiguous() for t in (hidden, weight, labels) if t is not None):
         raise ValueError(f"{what}: operands must be contiguous")
-    if weight.device != hidden.device or labels.device != hidden.device:
+    if weight.device != hidden.device or (labels is not None and labels.device != hidden.device):
         raise ValueError(f"{what}: operands live on different devices")
     n = int(hidden.shape[0])
     _same_len(what, n, labels=labels)
@@ -1255,6 +1255,99 @@ def logits_tokens_backward(logits, token_ids, labels, lse, entropy, g_ids, g_lab
             "axon_logits_tokens_bwd",
         )
     return out
+
+
+# Bytes of fp32 logits that a call of the head with alternatives holds at most: longer batches are cut into blocks of
+# tokens (2.5 GB: 4096 tokens of the 151936 vocabulary; never fewer than 256).
+TOP_LOGITS_BYTES = 2560 << 20
+
+
+def _top_block(n, v):
+    per_tile = 4 * 256 * ((v + 255) // 256 * 256)
+    return min(n, max(1, TOP_LOGITS_BYTES // per_tile) * 256)
+
+
+def lmhead_top(hidden, weight, k, labels=None, inv_temperature=1.0, softcap=0.0):
+    """``(logprobs | None, entropy, lse, entropy_b, top_logprobs [tokens, k], top_ids [tokens, k])``; see
+    axon_lmhead_top_fwd.  Block of tokens by block, so that the logits held do not grow with the batch."""
+    what = "lmhead_top"
+    n, h, v = _head_operands(what, hidden, weight, labels, None)
+    _top_count(what, k, v)
+    require_device(hidden, what)
+    lib = _lib.load()
+    dev = hidden.device
+    with on_device_of(hidden):
+        block = _top_block(n, v)
+        ws_bytes = lib.axon_lmhead_top_workspace_bytes(block, h, v)
+        if ws_bytes < 0:
+            raise _lib.AxonAmdError(f"axon_lmhead_top_fwd: unsupported shape tokens={n} hidden={h} vocab={v} (hidden % 32 != 0?)")
+        out = torch.empty(4, n, device=dev, dtype=torch.float32)
+        top_logprobs = torch.empty(n, k, device=dev, dtype=torch.float32)
+        top_ids = torch.empty(n, k, device=dev, dtype=torch.int64)
+        ws = torch.empty(ws_bytes if n else 0, device=dev, dtype=torch.uint8)
+        base = out.data_ptr()
+        for a in range(0, n, max(block, 1)):
+            lab = None if labels is None else labels.data_ptr() + a * labels.element_size()
+            lp, ent, lse, eb = (base + 4 * (i * n + a) for i in range(4))
+            check(lib.axon_lmhead_top_fwd(hidden.data_ptr() + a * h * 2, ptr(weight), lab,
+                                          int(labels is not None and labels.dtype == torch.int64), min(block, n - a), h, v,
+                                          float(inv_temperature), float(softcap), k, lp if lab else None, ent, lse, eb,
+                                          top_logprobs.data_ptr() + a * k * 4, top_ids.data_ptr() + a * k * 8, ptr(ws),
+                                          ws_bytes, stream_ptr()), "axon_lmhead_top_fwd")
+    lp, ent, lse, eb = out.unbind(0)
+    return (lp if labels is not None else None), ent, lse, eb, top_logprobs, top_ids
+
+
+def lmhead_tokens(hidden, weight, token_ids, inv_temperature=1.0, softcap=0.0):
+    """``(logprobs [tokens, k], entropy, lse, entropy_b)`` of given tokens; see axon_lmhead_tokens_fwd."""
+    what = "lmhead_tokens"
+    n, h, v = _head_operands(what, hidden, weight, None, None)
+    ids = token_ids_arg(what, token_ids, n, hidden.device)
+    require_device(hidden, what)
+    lib = _lib.load()
+    k, dev = int(ids.shape[1]), hidden.device
+    with on_device_of(hidden):
+        ws_bytes = lib.axon_lmhead_fwd_workspace_bytes(n, h, v)
+        if ws_bytes < 0:
+            raise _lib.AxonAmdError(f"axon_lmhead_tokens_fwd: unsupported shape tokens={n} hidden={h} vocab={v} (hidden % 32 != 0?)")
+        out = torch.empty(3, n, device=dev, dtype=torch.float32)
+        logprobs = torch.empty(n, k, device=dev, dtype=torch.float32)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        check(lib.axon_lmhead_tokens_fwd(ptr(hidden), ptr(weight), ptr(ids), int(ids.dtype == torch.int64), n, h, v,
+                                         float(inv_temperature), float(softcap), k, ptr(logprobs), ptr(out[0]),
+                                         ptr(out[1]), ptr(out[2]), ptr(ws), ws_bytes, stream_ptr()),
+              "axon_lmhead_tokens_fwd")
+    return logprobs, out[0], out[1], out[2]
+
+
+def lmhead_tokens_backward(g_logprobs, g_entropy, hidden, weight, token_ids, logprobs, lse, entropy_b, inv_temperature=1.0,
+                           softcap=0.0):
+    """``(d_hidden, d_weight)`` in bf16 from the gradients of the log-probabilities of ``token_ids`` (one more per
+    position than the forward's limit: a label's) and of the entropy (or None); see axon_lmhead_tokens_bwd."""
+    what = "lmhead_tokens_backward"
+    n, h, v = _head_operands(what, hidden, weight, None, None)
+    k = int(token_ids.shape[1])
+    _same_len(what, n, g_entropy=g_entropy, lse=lse, entropy_b=entropy_b)
+    _same_len(what, n * k, token_ids=token_ids, g_logprobs=g_logprobs, logprobs=logprobs)
+    require_device(hidden, what)
+    lib = _lib.load()
+    g_lp, lps = f32(g_logprobs), f32(logprobs)
+    g_en = None if g_entropy is None else f32(g_entropy)
+    for t in (token_ids, g_lp, lps, g_en):
+        if t is not None and t.device != hidden.device:
+            raise ValueError(f"{what}: operands live on different devices")
+    ids = token_ids.contiguous()
+    with on_device_of(hidden):
+        d_hidden, d_weight = torch.empty_like(hidden), torch.empty_like(weight)
+        ws_bytes = lib.axon_lmhead_tokens_bwd_workspace_bytes(n, h, v)
+        if ws_bytes < 0:
+            raise _lib.AxonAmdError(f"axon_lmhead_tokens_bwd: unsupported shape tokens={n} hidden={h} vocab={v}")
+        ws = torch.empty(ws_bytes, device=hidden.device, dtype=torch.uint8)
+        check(lib.axon_lmhead_tokens_bwd(ptr(g_lp), ptr(g_en), ptr(hidden), ptr(weight), ptr(ids),
+                                         int(ids.dtype == torch.int64), k, ptr(lps), ptr(lse), ptr(entropy_b), n, h, v,
+                                         float(inv_temperature), float(softcap), ptr(d_hidden), ptr(d_weight), ptr(ws),
+                                         ws_bytes, stream_ptr()), "axon_lmhead_tokens_bwd")
+    return d_hidden, d_weight
 
 def gemm_nt(a, b):
     """out[n][m] = sum_k a[m][k] * b[n][k]; bf16 in, fp32 out.  Test/benchmark helper."""

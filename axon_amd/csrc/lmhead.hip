@@ -16,6 +16,7 @@
 #include "common.h"
 #include "dweight_rows.h"
 #include "gemm_nt.h"
+#include "select.h"
 #include <vector>
 
 namespace axon {
@@ -32,7 +33,9 @@ struct FwdParams {
   // [parts][n_tokens][3]: running max in log2 units of the scaled logit, sum 2^(x*c - max), sum (x*c - max) * 2^(x*c - max);
   // side by side, so that sixteen tokens of a part are 192 contiguous bytes for the kernel that folds them
   float* stats;
-  float* pm;   // [parts][n_tokens]: the max once more, where the backward reads it (null: it does not)
+  // [parts][n_tokens]: the max once more, where the backward reads it (null: it does not); kKeepTop: the maximum of the
+  // accumulators themselves, by which the largest are selected
+  float* pm;
   int n_tokens, vocab;
   float c;     // inv_temperature * log2(e)
   float cap, inv_cap;  // logit soft-capping cap * tanh(logit / cap) (SOFTCAP kernels only)
@@ -40,7 +43,7 @@ struct FwdParams {
   int halved;          // the walk's last tiles that are computed in two halves of 128 vocabulary rows
 };
 // What a forward leaves for its backward beside the statistics.
-enum Keep { kKeepNone, kKeepStash, kKeepLogits };
+enum Keep { kKeepNone, kKeepStash, kKeepLogits, kKeepTop };
 
 // What a stashing forward leaves for the backward: for every logit, w = 2^(y - M) as fp16, where
 // y is the scaled logit in log2 units and M the maximum of y over the 128 vocabulary rows of the
@@ -59,6 +62,7 @@ constexpr int kStashWaveVecs = 2048;  // uint4 per wavefront sub-tile
 // contiguous kilobyte per store:  uint4 index = ((tile * 4 + wave) * 64 + j * 8 + i) * 64 + lane.
 constexpr int64_t kLogitsTileBytes = 262144;
 constexpr int kLogitsWaveVecs = 4096;  // uint4 per wavefront sub-tile
+// kKeepTop: the same logits, for the selection of every token's largest (lmhead_top_kernel).
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -145,7 +149,7 @@ __device__ __forceinline__ void rows_spread4(float x, float (&o)[4]) {
 template <bool MASKED, bool SOFTCAP, Keep KEEP, int BM, int BN>
 __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdParams& p, const LanePos& lp,
                                              const TilePos& t, int part, uint4* kept_tile, float* lds) {
-  constexpr bool STASH = KEEP == kKeepStash;
+  constexpr bool STASH = KEEP == kKeepStash, LOGITS = KEEP == kKeepLogits || KEEP == kKeepTop;
   constexpr bool kHalf = BM < kBlocks;
   constexpr int kRun = kBlocks / 2;  // blocks that a lane adds up in one go
   constexpr int kGroups = (BN + 3) / 4;
@@ -165,7 +169,9 @@ __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdPa
   };
   // columns 4 g .. 4 g + 3, read from the accumulators where they are needed (SOFTCAP: through cap * tanh(. / cap))
   float x[kHalf ? kGroups : 1][BM][4][4];
+  float raw[kGroups];  // kKeepTop: the part's maxima before the cap, as max_of has those behind it
   auto take = [&](int g) {
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < BM; ++i)
 #pragma unroll
@@ -175,11 +181,16 @@ __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdPa
 #pragma unroll
         for (int r = 0; r < 4; ++r) z[r] = read_acc(acc[i][4 * g + q], r);
         if (SOFTCAP) {
-          if (KEEP == kKeepLogits) keep_logits(i, 4 * g + q, z);  // what is kept is not capped
+          if (LOGITS) keep_logits(i, 4 * g + q, z);  // what is kept is not capped
+          if (KEEP == kKeepTop) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top[q] = row_ok(i, r) ? fmaxf(top[q], z[r]) : top[q];
+          }
 #pragma unroll
           for (int r = 0; r < 4; ++r) z[r] = p.cap * fast_tanh(z[r] * p.inv_cap);
         }
       }
+    if (SOFTCAP && KEEP == kKeepTop) raw[g] = rows_reduce4(top, [](float a, float b) { return fmaxf(a, b); });
   };
   // the part's maxima over this wavefront's rows of columns 4 g .. 4 g + 3, row r of the lanes that of column 4 g + r;
   // the four lanes that hold the same token (lane ^ 16, lane ^ 32) share one reference
@@ -205,6 +216,7 @@ __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdPa
       o[1] = sum;
       o[2] = prod;
       if (STASH) p.pm[at] = M;
+      if (KEEP == kKeepTop) p.pm[at] = raw[g];
     }
   };
   float* const mine = lds + lp.wave * 1024 + lp.lane;  // per wavefront: 8 x 64 of each of the two sums
@@ -215,16 +227,21 @@ __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdPa
     for (int g = 0; g < kGroups; ++g) {
       take(g);
       mine[g * 64] = mxs[g] = max_of(g);
+      if (SOFTCAP && KEEP == kKeepTop) mine[(kBlocks + g) * 64] = raw[g];
     }
     __syncthreads();
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) mxs[g] = fmaxf(mxs[g], other[g * 64]);
+    for (int g = 0; g < kGroups; ++g) {
+      mxs[g] = fmaxf(mxs[g], other[g * 64]);
+      if (SOFTCAP && KEEP == kKeepTop) raw[g] = fmaxf(raw[g], other[(kBlocks + g) * 64]);
+    }
     __syncthreads();
   }
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
     if (!kHalf) take(g);
     const float mx = kHalf ? mxs[g] : max_of(g);
+    if (!SOFTCAP && KEEP == kKeepTop) raw[g] = mx;
     mxs[g] = (MASKED && mx == -INFINITY) ? kEmptyMax : mx * p.c;
     float M[4], s4[4] = {}, e4[4] = {};
     rows_spread4(mxs[g], M);
@@ -244,7 +261,7 @@ __device__ __forceinline__ void fwd_epilogue(AccTileOf<BM, BN>& acc, const FwdPa
         for (int r = 0; r < 4; ++r) {
           // one store under the arithmetic of a block: all of them at the epilogue's head make it wait for their way out
           // (GSPO step of 6007 x 896 x 151936 5443 -> 5362 us)
-          if (KEEP == kKeepLogits && !SOFTCAP && i < BM && r == 0) keep_logits(i, j, x[kHalf ? g : 0][i][q]);
+          if (LOGITS && !SOFTCAP && i < BM && r == 0) keep_logits(i, j, x[kHalf ? g : 0][i][q]);
           if (i < BM) w[i % 2][r] = row_ok(i, r) ? fast_exp2(y[i % 3][r]) : 0.f;
           if (i > 0) {
             const int b = i - 1;
@@ -364,6 +381,18 @@ __global__ __launch_bounds__(kGemmThreads) void lmhead_fwd_softcap_stash_kernel(
   fwd_body<Loop, true, kKeepStash>(g, p, tiles_m, tiles_n);
 }
 
+template <class Loop>
+__global__ __launch_bounds__(kGemmThreads) void lmhead_fwd_top_kernel(GemmOperands g, FwdParams p, int tiles_m,
+                                                                      int tiles_n) {
+  fwd_body<Loop, false, kKeepTop>(g, p, tiles_m, tiles_n);
+}
+
+template <class Loop>
+__global__ __launch_bounds__(kGemmThreads) void lmhead_fwd_softcap_top_kernel(GemmOperands g, FwdParams p, int tiles_m,
+                                                                              int tiles_n) {
+  fwd_body<Loop, true, kKeepTop>(g, p, tiles_m, tiles_n);
+}
+
 template <bool SOFTCAP>
 __global__ __launch_bounds__(kGemmThreads) void lmhead_fwd_logits_kernel(GemmOperands g, FwdParams p,
                                                                          int tiles_m, int tiles_n) {
@@ -422,6 +451,7 @@ __global__ __launch_bounds__(256) void seq_start_kernel(const int32_t* __restric
   is_start[v] = bits;
 }
 
+// `labels` and `logprobs` may both be null: no label's logit is wanted.
 // The last kernel of the forward: folds a token's partials into lse, entropy_b and entropy, forms the label's logit
 // and with it logprob[n] = softcap(hidden[n] . W[label[n]]) / T - lse[n].
 // A token's partials are folded in 256 groups, group c taking c, c + 256, ... (a chain of five for 151936 vocabulary
@@ -450,9 +480,9 @@ __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
   for (int t = 0; t < PER; ++t)  // a valid token; the results of those beyond the last are dropped below
     nc[t] = min(blockIdx.x * TOK + t * T + (int)(threadIdx.x % T), n_tokens - 1);
   // the first token's label is on its way while the partials are folded
-  int64_t lab = 0;
+  int64_t lab = -1;
   const int n_dot = blockIdx.x * TOK + wave;
-  if (wave < TOK && n_dot < n_tokens) lab = (int64_t)labels[aligned_pos(n_dot, n_tokens, is_start, last_dst)];
+  if (labels && wave < TOK && n_dot < n_tokens) lab = (int64_t)labels[aligned_pos(n_dot, n_tokens, is_start, last_dst)];
   // a group beyond the number of partials holds an empty set (s = 0 below any reference)
   float M[SUB][PER], s[SUB][PER], e[SUB][PER];
 #pragma unroll
@@ -504,7 +534,7 @@ __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
   for (int k = wave; k < TOK; k += kWaves) {  // label dots
     const int nk = blockIdx.x * TOK + k;
     if (nk >= n_tokens) break;
-    if (k != wave) lab = (int64_t)labels[aligned_pos(nk, n_tokens, is_start, last_dst)];
+    if (labels && k != wave) lab = (int64_t)labels[aligned_pos(nk, n_tokens, is_start, last_dst)];
     float dot = 0.f;
     if (lab >= 0 && lab < vocab) {
       const uint4* h = reinterpret_cast<const uint4*>(hidden + (int64_t)nk * hidden_sz);
@@ -540,7 +570,7 @@ __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
   const bool start = is_start && is_start[dst];
   entropy[dst] = start ? 0.f : (L - d) * kLn2;
   // (logit*c - M) is formed in one rounding, then log2(sum) is subtracted: no cancellation
-  logprobs[dst] = start ? 0.f : (fmaf(dots[tok], inv_temp * kLog2e, -Mt) - L) * kLn2;
+  if (logprobs) logprobs[dst] = start ? 0.f : (fmaf(dots[tok], inv_temp * kLog2e, -Mt) - L) * kLn2;
 }
 
 // ----------------------------------------------------------------------------
@@ -551,7 +581,7 @@ struct DlogitParams {
   const float* entropy_b;
   const float* dlogprobs;
   const float* dentropy;  // may be null
-  const void* labels;
+  const void* labels;  // null: no token has one
   int labels_i64;
   __bf16* dl;    // [n_pad][chunk_cols]   token-major
   __bf16* dlT;   // [chunk_cols][n_pad]   vocab-major; null: not wanted (the dWeight GEMM reads dl as a K-major operand)
@@ -624,8 +654,9 @@ struct TokenCoef {
     ca = (-g_lp + g_en * eb) * p.inv_temp;
     cb = -g_en * p.inv_temp * p.inv_temp;
     gl = g_lp * p.inv_temp;
-    const int64_t lab = p.labels_i64 ? static_cast<const int64_t*>(p.labels)[src]
-                                     : (int64_t) static_cast<const int32_t*>(p.labels)[src];
+    const int64_t lab = !p.labels      ? -1
+                        : p.labels_i64 ? static_cast<const int64_t*>(p.labels)[src]
+                                       : (int64_t) static_cast<const int32_t*>(p.labels)[src];
     const int64_t lab_rel64 = lab - m0_abs;
     lab_rel = (lab_rel64 >= 0 && lab_rel64 < kTile) ? (int)lab_rel64 : -1;
   }
@@ -982,6 +1013,174 @@ __global__ __launch_bounds__(64) void lmhead_dlogit_logits_kernel(DlogitParams p
   else
     dlogit_stage_logits<SOFTCAP, false>(x, j0, p, lp, t, stage);
   dlogit_copy_out_half(stage, j0, p, lp, t);
+}
+
+// ----------------------------------------------------------------------------
+// Several tokens per position: the largest of the kept logits, the logits of given tokens, their gradients
+// ----------------------------------------------------------------------------
+
+// A token's kept logits as select_top reads them: its segments are the parts of 128 vocabulary rows, an item is the four
+// rows that one lane of the tile had.
+struct HeadSource {
+  static constexpr int kPer = 4, kItems = kWaveTile / 4;
+  const float4* column;  // the token's place in the first tile of its column
+  const float* maxima;   // its part maxima, `stride` apart
+  int64_t stride, tile_step;
+  int parts, vocab;
+  __device__ int n_segs() const { return parts; }
+  __device__ uint32_t max_key(int i) const { return order_key(maxima[i * stride]); }
+  __device__ int limit() const { return vocab; }
+  __device__ int load(const int* segs, int j, float (&v)[4]) const {
+    const int part = segs[j / kItems], i = (j % kItems) >> 2, lq = j & 3;
+    const float4 x = column[(part >> 1) * tile_step + (part & 1) * 2 * kLogitsWaveVecs + i * 64 + lq * 16];
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    return part * kWaveTile + i * kBlk + lq * 4;
+  }
+  __device__ int n_single() const { return 0; }
+  __device__ float single(int, int& index) const { index = 0; return 0.f; }
+};
+
+struct TopParams {
+  const float4* tiles;
+  const float* pm;   // [parts][n_tokens], of the accumulators
+  const float* lse;
+  float* top_logprobs;
+  int64_t* top_ids;
+  const void* labels;  // may be null
+  float* logprobs;     // of the labels: a label outside the vocabulary gets 0 here
+  int n_tokens, vocab, parts, tiles_n, k, labels_i64;
+  float inv_temp, cap, inv_cap;
+  int staged;        // the maxima of the workgroup's tokens fit in LDS
+};
+
+// A wavefront per token, four neighbouring tokens per workgroup, whose part maxima are staged together.
+constexpr int kTopTokens = 4;
+__global__ __launch_bounds__(kTopTokens * kWave) void lmhead_top_kernel(TopParams p) {
+  extern __shared__ __align__(16) char smem[];
+  SelectLds* const sel = reinterpret_cast<SelectLds*>(smem);
+  float* const staged = reinterpret_cast<float*>(smem + kTopTokens * sizeof(SelectLds));
+  const int n0 = blockIdx.x * kTopTokens, wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  if (p.staged) {
+    for (int i = threadIdx.x; i < p.parts * kTopTokens; i += kTopTokens * kWave) {
+      const int n = min(n0 + (i & (kTopTokens - 1)), p.n_tokens - 1);
+      staged[i] = p.pm[(int64_t)(i / kTopTokens) * p.n_tokens + n];
+    }
+    __syncthreads();
+  }
+  const int n = n0 + wave;
+  if (n >= p.n_tokens) return;
+  const int tn = n / kTile, in = n % kTile;
+  HeadSource src;
+  src.column = p.tiles + (int64_t)tn * 4 * kLogitsWaveVecs + (in / kWaveTile) * kLogitsWaveVecs +
+               (in % kWaveTile) / kBlk * kBlocks * 64 + in % kBlk;
+  src.tile_step = (int64_t)p.tiles_n * 4 * kLogitsWaveVecs;
+  src.maxima = p.staged ? staged + wave : p.pm + n;
+  src.stride = p.staged ? kTopTokens : p.n_tokens;
+  src.parts = p.parts;
+  src.vocab = p.vocab;
+  const float lse = p.lse[n];
+  if (p.labels && lane == 0) {
+    const int64_t lab = p.labels_i64 ? static_cast<const int64_t*>(p.labels)[n] : (int64_t) static_cast<const int32_t*>(p.labels)[n];
+    if (lab < 0 || lab >= p.vocab) p.logprobs[n] = 0.f;
+  }
+  select_top<kWave>(src, p.k, sel[wave], lane, [&](int rank, float z, int index) {
+    if (p.cap != 0.f) z = p.cap * fast_tanh(z * p.inv_cap);
+    p.top_logprobs[(int64_t)n * p.k + rank] = fmaf(z, p.inv_temp, -lse);
+    p.top_ids[(int64_t)n * p.k + rank] = index;
+  });
+}
+
+struct TokenArgs {
+  const void* ids;  // [n][k]; an id outside the vocabulary is a filler
+  int ids_i64, k;
+  float* logprobs;       // [n][k]: written by the forward, read by the backward
+  const float* g;        // [n][k], backward
+  __device__ __forceinline__ int64_t id(int64_t at) const {
+    return ids_i64 ? static_cast<const int64_t*>(ids)[at] : (int64_t) static_cast<const int32_t*>(ids)[at];
+  }
+};
+
+// logprobs[n][i] = softcap(hidden[n] . W[ids[n][i]]) / T - lse[n]: a workgroup per token, a wavefront per id.
+__global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restrict__ hidden, const __bf16* __restrict__ weight,
+                                                           int hidden_sz, int vocab, TokenArgs a, float inv_temp, float cap,
+                                                           const float* __restrict__ lse) {
+  const int n = blockIdx.x, lane = threadIdx.x & 63;
+  const uint4* h = reinterpret_cast<const uint4*>(hidden + (int64_t)n * hidden_sz);
+  const float lse_n = lse[n];
+  for (int i = threadIdx.x >> 6; i < a.k; i += 4) {
+    const int64_t at = (int64_t)n * a.k + i, id = a.id(at);
+    const bool ok = id >= 0 && id < vocab;
+    float dot = 0.f;
+    if (ok) {
+      const uint4* w = reinterpret_cast<const uint4*>(weight + id * hidden_sz);
+#pragma unroll 4
+      for (int c = lane; c < hidden_sz / 8; c += 64) {
+        const uint4 hv = h[c], wv = w[c];
+        const uint32_t hs[4] = {hv.x, hv.y, hv.z, hv.w}, ws[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          dot = fmaf(__uint_as_float(hs[q] << 16), __uint_as_float(ws[q] << 16), dot);
+          dot = fmaf(__uint_as_float(hs[q] & 0xffff0000u), __uint_as_float(ws[q] & 0xffff0000u), dot);
+        }
+      }
+    }
+    dot = wave_sum(dot);
+    if (cap != 0.f) dot = cap * fast_tanh(dot / cap);
+    if (lane == 0) a.logprobs[at] = ok ? fmaf(dot, inv_temp, -lse_n) : 0.f;
+  }
+}
+
+// G[n] = sum of the gradients of a token's ids in the vocabulary: what its softmax is multiplied by.  A wavefront per token.
+__global__ __launch_bounds__(256) void token_grad_sum_kernel(TokenArgs a, int n_tokens, int vocab, float* __restrict__ sums) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= n_tokens) return;
+  float sum = 0.f;
+  for (int i = lane; i < a.k; i += 64) {
+    const int64_t at = (int64_t)n * a.k + i, id = a.id(at);
+    sum += (id >= 0 && id < vocab) ? a.g[at] : 0.f;
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) sums[n] = sum;
+}
+
+// The dlogits of the ids of a vocabulary chunk, over what was formed there as if no token had one:
+//   dl = (sum of the gradients of this id - p (G + g_H (z - E[z]))) / T * (1 - (capped logit / cap)^2)
+// rounded once, as those around it.  A wavefront per token; equal ids of a token add up in their order, in the lane of the
+// first of them.
+constexpr int kMaxTokenArgs = 513;  // given tokens per position (kMaxTokenIds and a label)
+__global__ __launch_bounds__(256) void token_dlogits_kernel(DlogitParams p, TokenArgs a, int64_t chunk_rows) {
+  __shared__ int ids[4][kMaxTokenArgs];
+  __shared__ float gs[4][kMaxTokenArgs];
+  const int wave = threadIdx.x >> 6, n = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
+  if (n >= p.n_tokens) return;
+  for (int i = lane; i < a.k; i += 64) {
+    const int64_t at = (int64_t)n * a.k + i, id = a.id(at);
+    ids[wave][i] = (id >= 0 && id < p.vocab) ? (int)id : -1;
+    gs[wave][i] = a.g[at];
+  }
+  group_sync<kWave>();
+  const float G = p.dlogprobs[n], g_en = p.dentropy ? p.dentropy[n] : 0.f, lse = p.lse[n], mean = p.entropy_b[n];
+  for (int i = lane; i < a.k; i += 64) {
+    const int id = ids[wave][i];
+    if (id < p.v_begin || id >= p.v_begin + chunk_rows) continue;
+    float total = 0.f;
+    bool first = true;
+    for (int j = 0; j < a.k; ++j) {
+      if (ids[wave][j] != id) continue;
+      if (j < i) { first = false; break; }
+      total += gs[wave][j];
+    }
+    if (!first) continue;
+    const float lp = a.logprobs[(int64_t)n * a.k + i], z = lp + lse;
+    float d = fmaf(-fast_exp2(lp * kLog2e), fmaf(g_en, z - mean, G), total) * p.inv_temp;
+    if (p.cap != 0.f) {
+      const float bent = z / (p.inv_temp * p.cap);
+      d *= fmaf(-bent, bent, 1.f);
+    }
+    const int64_t m = id - p.v_begin;
+    p.dl[(int64_t)n * p.ld_dl + m] = (__bf16)d;
+    if (p.dlT) p.dlT[m * p.ld_dlT + n] = (__bf16)d;
+  }
 }
 
 // ----------------------------------------------------------------------------
@@ -1717,12 +1916,13 @@ int fwd_impl(const void* hidden, const void* weight, const void* labels, int lab
              int64_t h, int64_t v, float inv_temp, float softcap, const uint8_t* is_start,
              int64_t last_dst, float* logprobs, float* entropy, float* lse, float* entropy_b,
              void* workspace, int64_t ws_bytes, void* stash, int64_t stash_bytes, void* stream,
-             PhaseTimer* timer, bool is_block = false, Keep keep = kKeepStash) {
+             PhaseTimer* timer, bool is_block = false, Keep keep = kKeepStash, float* top_max = nullptr,
+             bool label_optional = false) {
   int rc = check_head_shape(n, h, v);
   if (rc != AXON_OK) return rc;
   if (n == 0) return AXON_OK;
-  if (!hidden || !weight || !labels || !logprobs || !entropy || !lse || !entropy_b || !workspace)
-    return AXON_ERR_ARG;
+  if (!hidden || !weight || !entropy || !lse || !entropy_b || !workspace) return AXON_ERR_ARG;
+  if (label_optional ? !labels != !logprobs : !labels || !logprobs) return AXON_ERR_ARG;
   if (!(inv_temp > 0.f) || !(softcap >= 0.f)) return AXON_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15)
     return AXON_ERR_ARG;
@@ -1734,7 +1934,10 @@ int fwd_impl(const void* hidden, const void* weight, const void* labels, int lab
   float* pm = nullptr;
   if (stash) {
     if (reinterpret_cast<uintptr_t>(stash) & 15) return AXON_ERR_ARG;
-    if (keep == kKeepLogits) {
+    if (keep == kKeepTop) {
+      sw.tiles = static_cast<uint4*>(stash);
+      pm = top_max;
+    } else if (keep == kKeepLogits) {
       const int64_t bytes = logits_bytes(n, h, v);
       if (bytes == 0) return AXON_ERR_SHAPE;
       if (bytes > stash_bytes) return AXON_ERR_WORKSPACE;
@@ -1758,6 +1961,15 @@ int fwd_impl(const void* hidden, const void* weight, const void* labels, int lab
     if (stash && keep == kKeepLogits) {
       rc = softcap > 0.f ? launch_fwd_logits<true>(g, p, st) : launch_fwd_logits<false>(g, p, st);
       if (rc != AXON_OK) return rc;
+    } else if (stash && keep == kKeepTop) {
+      if (dma_ok(g) && narrow_columns(n) < kBlocks) {
+        rc = softcap > 0.f ? launch_fwd_narrow<true, kKeepTop>(g, p, st) : launch_fwd_narrow<false, kKeepTop>(g, p, st);
+        if (rc != AXON_OK) return rc;
+      } else if (softcap > 0.f) {
+        AXON_LAUNCH_GEMM_PLUS(lmhead_fwd_softcap_top_kernel, g, p, st, p.halved);
+      } else {
+        AXON_LAUNCH_GEMM_PLUS(lmhead_fwd_top_kernel, g, p, st, p.halved);
+      }
     } else if (dma_ok(g) && narrow_columns(n) < kBlocks) {
       rc = stash ? softcap > 0.f ? launch_fwd_narrow<true, kKeepStash>(g, p, st)
                                  : launch_fwd_narrow<false, kKeepStash>(g, p, st)
@@ -1820,7 +2032,7 @@ int bwd_impl(const float* dlogprobs, const float* dentropy, const void* hidden, 
              int64_t n, int64_t h, int64_t v, float inv_temp, float softcap,
              const uint8_t* is_start, void* d_hidden, void* d_weight, int64_t chunk, void* workspace,
              int64_t ws_bytes, const void* stash, int64_t stash_bytes, void* stream, PhaseTimer* timer,
-             const BlockArgs& blk = BlockArgs()) {
+             const BlockArgs& blk = BlockArgs(), const TokenArgs* tokens = nullptr) {
   int rc = check_head_shape(n, h, v);
   if (rc != AXON_OK) return rc;
   if (chunk < 0 || chunk % kTile != 0) return AXON_ERR_ARG;
@@ -1832,7 +2044,7 @@ int bwd_impl(const float* dlogprobs, const float* dentropy, const void* hidden, 
   if (dw_bf16 && !d_weight) return AXON_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   if (n == 0) return axon_fill_zero(d_weight, v * h * 2, stream);
-  if (!dlogprobs || !hidden || !labels || !lse || !entropy_b || !d_hidden || !workspace)
+  if (!dlogprobs || !hidden || (!labels && !tokens) || !lse || !entropy_b || !d_hidden || !workspace)
     return AXON_ERR_ARG;
   if (!(inv_temp > 0.f) || !(softcap >= 0.f)) return AXON_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight) |
@@ -1905,6 +2117,10 @@ int bwd_impl(const float* dlogprobs, const float* dentropy, const void* hidden, 
         AXON_LAUNCH_GEMM(lmhead_dlogit_softcap_kernel, g, p, st);
       } else {
         AXON_LAUNCH_GEMM(lmhead_dlogit_kernel, g, p, st);
+      }
+      if (tokens) {
+        hipLaunchKernelGGL(token_dlogits_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, p, *tokens, vc);
+        AXON_CHECK_LAUNCH();
       }
     }
     // B2: dHidden[n][h] (+)= sum_v dl[n][v] * W[v0 + v][h], the weight read K-major where it lies
@@ -2355,4 +2571,116 @@ extern "C" int axon_scale_bf16_pair_unless_one(void* x, int64_t nx, void* y, int
 
 extern "C" int axon_scale_bf16_unless_one(void* x, int64_t n, const float* scale, void* stream) {
   return axon_scale_bf16_pair_unless_one(x, n, nullptr, 0, scale, stream);
+}
+
+// ----------------------------------------------------------------------------
+// Several tokens per position
+// ----------------------------------------------------------------------------
+namespace {
+
+// Behind the forward's own workspace: the part maxima, then the kept logits, a tile for every 256 tokens x 256 rows.
+struct TopWs {
+  float* maxima;
+  uint4* tiles;
+  int64_t bytes;
+};
+TopWs top_ws(int64_t n, int64_t v, void* base) {
+  const FwdWs f = fwd_ws(n, v, base);
+  char* p = static_cast<char*>(base);
+  TopWs w;
+  w.maxima = reinterpret_cast<float*>(p + f.bytes);
+  const int64_t maxima = round_up((int64_t)f.parts * n * 4, kAlign);
+  w.tiles = reinterpret_cast<uint4*>(p + f.bytes + maxima);
+  w.bytes = f.bytes + maxima + (round_up(v, kTile) / kTile) * (round_up(n, kTile) / kTile) * kLogitsTileBytes;
+  return w;
+}
+
+constexpr int64_t kTopLdsBytes = 150 * 1024;
+
+}  // namespace
+
+extern "C" int64_t axon_lmhead_top_workspace_bytes(int64_t n, int64_t h, int64_t v) {
+  const int rc = check_head_shape(n, h, v);
+  return rc != AXON_OK ? rc : top_ws(n, v, nullptr).bytes + kAlign;
+}
+
+extern "C" int axon_lmhead_top_fwd(const void* hidden, const void* weight, const void* labels, int labels_i64, int64_t n,
+                                   int64_t h, int64_t v, float inv_temp, float softcap, int64_t k, float* logprobs,
+                                   float* entropy, float* lse, float* entropy_b, float* top_logprobs, int64_t* top_ids,
+                                   void* workspace, int64_t ws_bytes, void* stream) {
+  const int shape = check_head_shape(n, h, v);
+  if (shape != AXON_OK) return shape;
+  if (k < 1 || k > kMaxTop || k > v) return AXON_ERR_SHAPE;
+  if (n == 0) return AXON_OK;
+  if (!workspace || !top_logprobs || !top_ids) return AXON_ERR_ARG;
+  char* base = reinterpret_cast<char*>(round_up(reinterpret_cast<int64_t>(workspace), kAlign));
+  const TopWs w = top_ws(n, v, base);
+  if ((base - static_cast<char*>(workspace)) + w.bytes > ws_bytes) return AXON_ERR_WORKSPACE;
+  const int rc = fwd_impl(hidden, weight, labels, labels_i64, n, h, v, inv_temp, softcap, nullptr, 0, logprobs, entropy, lse,
+                          entropy_b, base, w.bytes, w.tiles, 0, stream, nullptr, false, kKeepTop, w.maxima, true);
+  if (rc != AXON_OK) return rc;
+  TopParams p;
+  p.tiles = reinterpret_cast<const float4*>(w.tiles);
+  p.pm = w.maxima;  p.lse = lse;  p.top_logprobs = top_logprobs;  p.top_ids = top_ids;
+  p.labels = labels;  p.labels_i64 = labels_i64;  p.logprobs = logprobs;
+  p.n_tokens = (int)n;  p.vocab = (int)v;  p.k = (int)k;
+  p.parts = (int)(round_up(v, kTile) / kTile) * 2;
+  p.tiles_n = (int)(round_up(n, kTile) / kTile);
+  p.inv_temp = inv_temp;  p.cap = softcap;  p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+  const int64_t select = kTopTokens * (int64_t)sizeof(SelectLds), staged = (int64_t)p.parts * kTopTokens * 4;
+  p.staged = select + staged <= kTopLdsBytes;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(lmhead_top_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)kTopLdsBytes) != hipSuccess)
+    return AXON_ERR_LAUNCH;
+  hipLaunchKernelGGL(lmhead_top_kernel, dim3((unsigned)((n + kTopTokens - 1) / kTopTokens)), dim3(kTopTokens * kWave),
+                     (unsigned)(select + (p.staged ? staged : 0)), (hipStream_t)stream, p);
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int axon_lmhead_tokens_fwd(const void* hidden, const void* weight, const void* ids, int ids_i64, int64_t n,
+                                      int64_t h, int64_t v, float inv_temp, float softcap, int64_t k, float* logprobs,
+                                      float* entropy, float* lse, float* entropy_b, void* workspace, int64_t ws_bytes,
+                                      void* stream) {
+  const int shape = check_head_shape(n, h, v);
+  if (shape != AXON_OK) return shape;
+  if (k < 1 || k > kMaxTokenArgs) return AXON_ERR_SHAPE;
+  if (n == 0) return AXON_OK;
+  if (!ids || !logprobs) return AXON_ERR_ARG;
+  const int rc = fwd_impl(hidden, weight, nullptr, 0, n, h, v, inv_temp, softcap, nullptr, 0, nullptr, entropy, lse, entropy_b,
+                          workspace, ws_bytes, nullptr, 0, stream, nullptr, false, kKeepNone, nullptr, true);
+  if (rc != AXON_OK) return rc;
+  const TokenArgs a{ids, ids_i64, (int)k, logprobs, nullptr};
+  hipLaunchKernelGGL(token_logits_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream,
+                     static_cast<const __bf16*>(hidden), static_cast<const __bf16*>(weight), (int)h, (int)v, a, inv_temp,
+                     softcap, lse);
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int64_t axon_lmhead_tokens_bwd_workspace_bytes(int64_t n, int64_t h, int64_t v) {
+  const int64_t bwd = axon_lmhead_bwd_workspace_bytes(n, h, v, 0);
+  return bwd < 0 ? bwd : bwd + round_up(n * 4, kAlign) + kAlign;
+}
+
+extern "C" int axon_lmhead_tokens_bwd(const float* g_logprobs, const float* g_entropy, const void* hidden, const void* weight,
+                                      const void* ids, int ids_i64, int64_t k, const float* logprobs, const float* lse,
+                                      const float* entropy_b, int64_t n, int64_t h, int64_t v, float inv_temp, float softcap,
+                                      void* d_hidden, void* d_weight, void* workspace, int64_t ws_bytes, void* stream) {
+  const int shape = check_head_shape(n, h, v);
+  if (shape != AXON_OK) return shape;
+  if (k < 1 || k > kMaxTokenArgs) return AXON_ERR_SHAPE;
+  if (!weight || !d_weight) return AXON_ERR_ARG;
+  if (n == 0) return axon_fill_zero(d_weight, v * h * 2, stream);
+  if (!g_logprobs || !ids || !logprobs || !workspace) return AXON_ERR_ARG;
+  char* base = reinterpret_cast<char*>(round_up(reinterpret_cast<int64_t>(workspace), kAlign));
+  const int64_t sums = round_up(n * 4, kAlign), left = ws_bytes - (base - static_cast<char*>(workspace)) - sums;
+  if (left < 0) return AXON_ERR_WORKSPACE;
+  float* const G = reinterpret_cast<float*>(base);
+  const TokenArgs a{ids, ids_i64, (int)k, const_cast<float*>(logprobs), g_logprobs};
+  hipLaunchKernelGGL(token_grad_sum_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a, (int)n, (int)v,
+                     G);
+  AXON_CHECK_LAUNCH();
+  return bwd_impl(G, g_entropy, hidden, weight, nullptr, 0, lse, entropy_b, n, h, v, inv_temp, softcap, nullptr, d_hidden,
+                  d_weight, 0, base + sums, left, nullptr, 0, stream, nullptr, BlockArgs(), &a);
 }

@@ -44,14 +44,14 @@ _REDUCTIONS = ("none", "sum", "mean")
 _warned_rounding = False
 
 
-def _warn_rounded_to_bf16(hidden_dtype, weight_dtype) -> None:
+def _warn_rounded_to_bf16(hidden_dtype, weight_dtype, what="linear_cross_entropy") -> None:
     global _warned_rounding
     if _warned_rounding:
         return
     _warned_rounding = True
     import warnings
 
-    warnings.warn(f"linear_cross_entropy: hidden ({hidden_dtype}) / weight ({weight_dtype}) are rounded to bfloat16 "
+    warnings.warn(f"{what}: hidden ({hidden_dtype}) / weight ({weight_dtype}) are rounded to bfloat16 "
                   "before the head (the kernels compute in bf16 with fp32 accumulation); each call makes a bf16 copy "
                   "of such an operand and casts its gradient back", stacklevel=3)
 

@@ -85,3 +85,52 @@ def test_the_c_entry_points_check_their_arguments():
     for bad in (dict(ids=None), dict(labels=None), dict(lse=None), dict(ent=None), dict(out=None), dict(ld_d=99), dict(out=p + 1)):
         assert bwd(**bad) == -1, bad
     assert bwd(k=513) == bwd(k=-1) == -2
+
+
+def test_the_heads_operands_are_checked_on_the_host():
+    from axon_amd.utils.kernel.linear_top_logprobs import linear_token_logprobs, linear_top_logprobs
+
+    h, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(50, 64, dtype=torch.bfloat16)
+    ids = torch.zeros(4, 2, dtype=torch.int64)
+    for bad in (dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
+                dict(logit_softcapping=-1.0), dict(logit_softcapping=float("nan")), dict(labels=torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            linear_top_logprobs(h, w, 3, **bad)
+    for hh, ww in ((h.double(), w), (h, w.long()), (h, w[:, :32]), (h, w[0]), (h.view(-1)[0], w)):
+        with pytest.raises(ValueError):
+            linear_top_logprobs(hh, ww, 3)
+    for bad in (ids[0], ids[:3], ids[None]):
+        with pytest.raises(ValueError):
+            linear_token_logprobs(h, w, bad)
+    for call in (lambda: linear_top_logprobs(h, w, 3), lambda: linear_token_logprobs(h, w, ids)):
+        with pytest.raises(_lib.AxonAmdError, match="no CPU fallback"):
+            call()
+
+
+def test_the_heads_c_entry_points_check_their_arguments():
+    lib = _lib.load()
+    p = (ctypes.addressof(ctypes.create_string_buffer(64)) + 15) & ~15
+    big = 1 << 40
+    assert lib.axon_lmhead_top_workspace_bytes(4, 64, 50) > 0
+    assert lib.axon_lmhead_top_workspace_bytes(4, 33, 50) == -2 and lib.axon_lmhead_top_workspace_bytes(4, 0, 50) == -1
+
+    def top(h=p, w=p, lab=None, n=4, hs=64, v=50, inv_t=1.0, cap=0.0, k=3, lp=None, ent=p, lse=p, eb=p, tl=p, ti=p, ws=p, wb=big):
+        return lib.axon_lmhead_top_fwd(h, w, lab, 1, n, hs, v, inv_t, cap, k, lp, ent, lse, eb, tl, ti, ws, wb, None)
+
+    assert top(n=0) == 0
+    for bad in (dict(h=None), dict(w=None), dict(lab=p), dict(lp=p), dict(ent=None), dict(lse=None), dict(eb=None), dict(tl=None),
+                dict(ti=None), dict(ws=None), dict(inv_t=0.0), dict(cap=-1.0), dict(h=p + 2), dict(n=-1)):
+        assert top(**bad) == -1, bad
+    assert top(k=0) == top(k=129) == top(k=51) == top(hs=33) == -2
+    assert top(wb=lib.axon_lmhead_top_workspace_bytes(4, 64, 50) - 512) == -3
+
+    def fwd(ids=p, k=3, lp=p, n=4, wb=big):
+        return lib.axon_lmhead_tokens_fwd(p, p, ids, 1, n, 64, 50, 1.0, 0.0, k, lp, p, p, p, p, wb, None)
+
+    assert fwd(n=0) == 0 and fwd(ids=None) == fwd(lp=None) == -1 and fwd(k=0) == fwd(k=514) == -2 and fwd(wb=0) == -3
+
+    def bwd(g=p, ids=p, k=3, lp=p, dw=p, ws=p, wb=0, n=4):
+        return lib.axon_lmhead_tokens_bwd(g, p, p, p, ids, 1, k, lp, p, p, n, 64, 50, 1.0, 0.0, p, dw, ws, wb, None)
+
+    assert bwd(g=None) == bwd(ids=None) == bwd(lp=None) == bwd(dw=None) == bwd(ws=None) == -1
+    assert bwd(k=0) == bwd(k=514) == -2 and bwd() == -3
