@@ -94,6 +94,11 @@ SIGNATURES: dict[str, tuple] = {
                                       _i32, _ptr]),
     "axon_logits_tokens_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _i64, _ptr, _i32, _ptr, _ptr, _ptr,
                                       _ptr, _ptr, _ptr, _i64, _ptr]),
+    "axon_router_balance_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "axon_router_balance_fwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _i64, _ptr, _i32, _ptr, _i32, _ptr, _i64, _i32,
+                                       _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "axon_router_balance_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i32, _ptr, _i64, _i32, _ptr, _ptr, _ptr,
+                                       _ptr, _ptr]),
     "axon_reverse_scan": (_i32, [_i32, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i64, _i64, _f32, _f32, _ptr, _ptr, _ptr,
                                  _ptr]),
     "axon_masked_whiten_workspace_bytes": (_i64, [_i64]),

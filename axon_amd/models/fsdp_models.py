@@ -9,6 +9,9 @@ reference that is ``CausalLM.forward_fn`` around the HF model and the fused LM h
 
 The two side terms and the two entropy metrics come out of ONE kernel pass
 (``axon_side_terms``) instead of three ``agg_loss`` calls and an elementwise KL chain.
+
+A model with routed experts may return its ``router_logits`` too: their balance loss (``router_balance_loss``) is then one
+more term (the reference has none here).
 """
 
 from __future__ import annotations
@@ -17,7 +20,7 @@ import numpy as np
 import torch
 
 from axon_amd import _lib, _ops
-from axon_amd.trainer.algos.loss import compute_loss_fn
+from axon_amd.trainer.algos.loss import compute_loss_fn, router_balance_loss
 from axon_amd.utils.rl.sampler import compute_sampler_corr_metrics_from_logprobs
 
 
@@ -44,8 +47,31 @@ class _SideTerms(torch.autograd.Function):
         return d_ent, d_lp, None, None, None, None, None, None
 
 
-def loss_from_outputs(data, log_prob, entropy, meta_info):
+def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
+    """``(balance loss, largest load of an expert relative to the mean of its layer)``, both on the device.  All tokens of a
+    packed batch count, in a padded one those of ``attention_mask`` (where the batch has it)."""
+    if router_logits is None:
+        raise ValueError("router_aux_loss_coef is set, but the model returned no router_logits")
+    if "router_top_k" not in args:
+        raise ValueError("router_aux_loss_coef needs router_top_k, the experts per token")
+    mask, seqs = (b.get("attention_mask", None) if cu is None else None), None
+    if args.get("router_balance_per_sequence", False):
+        seqs = cu
+        if seqs is None:  # padded: a row is a sequence
+            rows, length = entropy.shape
+            seqs = torch.arange(rows + 1, device=entropy.device, dtype=torch.int32) * length
+    balance, counts = router_balance_loss(router_logits, args["router_top_k"], token_mask=mask, cu_seqlens=seqs,
+                                          expert_ids=router_expert_ids, score_fn=args.get("router_score_fn", "softmax"))
+    counts = counts.view(-1, counts.shape[-1]).float()
+    load = counts.amax(1) * counts.shape[1] / counts.sum(1).clamp(min=1)
+    return balance, load.max()
+
+
+def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, router_expert_ids=None):
     """Everything of ``forward_backward_fn`` after the model forward (fsdp_models.py:224-278).
+
+    With ``loss_fn_args["router_aux_loss_coef"]`` the balance loss of ``router_logits`` times that coefficient is added, with
+    ``router_top_k``, ``router_score_fn`` ("softmax") and ``router_balance_per_sequence`` (False) from the same arguments.
 
     Returns ``(scaled_loss, metrics)``.  ``data.batch["log_probs"]`` is set; ``response_mask`` may be
     overwritten by the sampler correction hook, while the side terms keep the mask they were given
@@ -98,14 +124,24 @@ def loss_from_outputs(data, log_prob, entropy, meta_info):
         loss = loss - ent_agg * entropy_coef
     if kl_coef != 0:
         loss = loss + kl_agg * kl_coef
+    router_coef = loss_fn_args.get("router_aux_loss_coef", 0)
+    router_vals = []
+    if router_coef != 0:
+        balance, load = _router_term(b, cu, entropy, loss_fn_args, router_logits, router_expert_ids)
+        loss = loss + balance * router_coef
+        router_vals = [balance.detach(), load]
     # one readback for pg_loss and the side-term metrics
-    vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4]]).tolist()
+    vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4], *router_vals]).tolist()
     metrics["pg_loss"] = vals[0] * n_micro_batches
     metrics["entropy"] = vals[1] * n_micro_batches
     metrics["entropy_token_mean"] = vals[3] / max(vals[4], 1.0)
     if kl_coef != 0:
         metrics["kl_loss"] = vals[2] * n_micro_batches
         metrics["kl_coef"] = kl_coef
+    if router_vals:
+        metrics["router_balance_loss"] = vals[5] * n_micro_batches
+        metrics["router_max_load"] = vals[6]
+        metrics["router_aux_loss_coef"] = router_coef
     return loss * dp_replicas, metrics
 
 
@@ -115,4 +151,5 @@ class CausalLM:
         """Per micro-batch forward + loss; ``data`` is a DataProto.  Returns ``(scaled_loss, metrics)``."""
         model_inputs = {**data.batch, **data.non_tensor_batch}
         result = module(model_inputs, {**meta_info, "temperature": meta_info["temperature"], "calculate_entropy": True})
-        return loss_from_outputs(data, result["log_probs"], result["entropys"], meta_info)
+        return loss_from_outputs(data, result["log_probs"], result["entropys"], meta_info, result.get("router_logits", None),
+                                 result.get("router_expert_ids", None))

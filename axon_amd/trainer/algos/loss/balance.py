@@ -1,0 +1,111 @@
+"""Balance loss of a mixture of experts and the experts' loads, with the gradient of the router logits.
+
+The term that a trainer adds to the policy loss of a model with routed experts, beside the entropy bonus and the KL penalty
+(the reference leaves it to the model's own code, and has no operator for it).  For a layer and T unmasked tokens
+
+    loss = sum_e (experts / (k T)) c_e * (1 / T) sum_t p_te
+
+with ``p`` the router's scores of a token (softmax, or sigmoids divided by their sum) and ``c_e`` how often expert ``e`` was
+chosen, which is a constant for the gradient: 1 where scores and choices are uniform.  The mean over the layers is returned;
+with ``cu_seqlens`` the loss is formed for every sequence by itself and averaged over the sequences that have unmasked tokens.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from axon_amd import _ops
+
+__all__ = ["router_balance_loss"]
+
+
+class _RouterBalance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, top_k, token_mask, cu_seqlens, expert_ids, score_fn, stacked, *logits):
+        layers = list(logits[0].unbind(0)) if stacked else [t.reshape(-1, t.shape[-1]) for t in logits]
+        batch = _ops.router_batch(layers, token_mask, cu_seqlens, score_fn)
+        loss, counts, coef, scale = _ops.router_balance(batch, top_k, expert_ids)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(counts)
+        ctx.layout = batch.ld, batch.mask_kind, batch.score, len(layers)
+        ctx.shapes, ctx.stacked = [t.shape for t in logits], stacked
+        ctx.save_for_backward(*batch.logits, batch.mask, batch.cu, coef, scale)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss, _g_counts):
+        wanted = ctx.needs_input_grad[6:]
+        if g_loss is None or not any(wanted):
+            return (None,) * (6 + len(wanted))
+        ld, kind, score, n_layers = ctx.layout
+        saved = ctx.saved_tensors
+        rows, (mask, cu, coef, scale) = list(saved[:n_layers]), saved[n_layers:]
+        batch = _ops.RouterBatch(rows, ld, mask, kind, cu, score)
+        new = lambda shape: torch.empty(shape, device=rows[0].device, dtype=rows[0].dtype)  # noqa: E731
+        if ctx.stacked:
+            grads = [new(ctx.shapes[0])]
+            parts = list(grads[0].unbind(0))
+        else:
+            grads = [new(shape) if want else None for shape, want in zip(ctx.shapes, wanted)]
+            parts = grads
+        _ops.router_balance_backward(batch, coef, scale, g_loss, parts)
+        return (None,) * 6 + tuple(grads)
+
+
+def _ids_per_layer(expert_ids, layers, rows, top_k, device):
+    what = "router_balance_loss"
+    if isinstance(expert_ids, torch.Tensor):
+        ids = list(expert_ids.unbind(0)) if expert_ids.dim() == 3 else [expert_ids]
+    else:
+        ids = list(expert_ids)
+    if len(ids) != layers:
+        raise ValueError(f"{what}: expert_ids for {len(ids)} layers, logits of {layers}")
+    out = []
+    for t in ids:
+        if t.dtype not in (torch.int32, torch.int64) or t.dtype != ids[0].dtype:
+            raise ValueError(f"{what}: expert_ids must be int32 or int64, the same in all layers")
+        if t.device != device:
+            raise ValueError(f"{what}: operands live on different devices")
+        if t.dim() < 2 or int(t.shape[-1]) != top_k or int(t.numel()) != rows * top_k:
+            raise ValueError(f"{what}: expert_ids {tuple(t.shape)} are not {top_k} per token of {rows}")
+        out.append(t.reshape(rows, top_k).contiguous())
+    return out
+
+
+def router_balance_loss(router_logits, top_k: int, *, token_mask=None, cu_seqlens=None, expert_ids=None,
+                        score_fn: str = "softmax"):
+    """``(loss, counts)``: the balance loss (0-d fp32) and how often every expert was chosen (int64 ``[layers, experts]``).
+
+    * ``router_logits``: one ``[..., experts]`` tensor per layer in a list or tuple (as a model returns them), one tensor
+      ``[layers, tokens, experts]``, or ``[tokens, experts]`` of a single layer (``counts`` is then ``[experts]``); fp32 or
+      bf16, at most 1024 experts, the same shape in all layers.  The gradient comes back in the logits' type.
+    * ``top_k``: experts per token.  The choices are the ``top_k`` largest logits, equal ones by ascending expert, or
+      ``expert_ids`` (int32 or int64, ``[..., top_k]`` per layer in the same arrangement): what the router chose, where that
+      is not the order of these logits (a selection bias, replayed routes).  An id outside the experts chooses nothing.
+    * ``token_mask``: as many entries as tokens, shared by the layers; a token counts where it is not zero.
+    * ``cu_seqlens``: int32 ``[sequences + 1]``: the loss per sequence, averaged.  Tokens of no sequence count nowhere.
+    * ``score_fn``: ``"softmax"`` or ``"sigmoid"``.
+
+    A batch without unmasked tokens has loss 0 and a zero gradient.  Nothing is read back; sums repeat bit for bit."""
+    what = "router_balance_loss"
+    if isinstance(top_k, bool) or not isinstance(top_k, int):
+        raise TypeError(f"{what}: top_k must be an int, got {type(top_k).__name__}")
+    single = isinstance(router_logits, torch.Tensor) and router_logits.dim() == 2
+    stacked = isinstance(router_logits, torch.Tensor) and not single
+    if stacked and router_logits.dim() != 3:
+        raise ValueError(f"{what}: a tensor of router logits must be [tokens, experts] or [layers, tokens, experts], got "
+                         f"{tuple(router_logits.shape)}")
+    tensors = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
+    if not tensors or (stacked and router_logits.shape[0] == 0):
+        raise ValueError(f"{what}: no layers")
+    if any(t.dim() < 2 or t.shape[-1] < 1 for t in tensors):
+        raise ValueError(f"{what}: every layer's logits must be [..., experts]")
+    layers, experts = (int(router_logits.shape[0]) if stacked else len(tensors)), int(tensors[0].shape[-1])
+    if not 1 <= top_k <= experts:
+        raise ValueError(f"{what}: top_k must be between 1 and the {experts} experts, got {top_k}")
+    rows = int(tensors[0].numel()) // experts // (layers if stacked else 1)
+    if expert_ids is not None:
+        expert_ids = _ids_per_layer(expert_ids, layers, rows, top_k, tensors[0].device)
+    loss, counts = _RouterBalance.apply(top_k, token_mask, cu_seqlens, expert_ids, score_fn, stacked, *tensors)
+    return loss, counts[0] if single else counts

@@ -705,6 +705,28 @@ int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld, int64_t n,
                            const float* entropy, const float* g_ids, const float* g_label, const float* g_entropy,
                            void* dlogits, int64_t ld_dlogits, void* stream);
 
+/* Balance loss of a mixture of experts and the experts' loads (no reference counterpart).  For every layer and every
+ * sequence (cu: int32 [n_seqs + 1]; NULL with n_seqs 1: the batch as one) with T > 0 unmasked tokens
+ *   sum_e experts / (k T^2) c_e P_e,  P_e = sum over the unmasked tokens of p_te,  c_e = how often they chose expert e,
+ * averaged over these sequences and over the layers: 1 where scores and choices are uniform.  p: softmax of a token's logits
+ * (score 0), or their sigmoids divided by their sum (score 1).  Choices: the token's k largest logits, equal ones by ascending
+ * expert, or the given ids [n][k] (an id outside [0, experts) chooses nothing).  The choices are constants for the gradient.
+ *   logits, ids, dlogits: HOST arrays of one device pointer per layer: logits [n][experts] (row stride ld, dtype
+ *        AXON_LOGITS_F32 or AXON_LOGITS_BF16), ids NULL or [n][k], dlogits [n][experts] contiguous (an entry may be NULL:
+ *        that layer wants no gradient).  mask [n] (NULL: all tokens count), a token counts where it is not zero.
+ *   loss [1], scale [1], coef [n_seqs][layers][experts] (what the backward reads), counts int64 [layers][experts].
+ *   Tokens of no sequence count nowhere and get a zero gradient.  1 <= k <= experts <= 1024.  Workspace 8-byte aligned.
+ *   g_loss: DEVICE scalar, the loss's upstream gradient. */
+int64_t axon_router_balance_workspace_bytes(int64_t n_tokens, int64_t n_seqs, int64_t layers, int64_t experts);
+int axon_router_balance_fwd(const void* const* logits, int dtype, int64_t ld, int64_t layers, int64_t n_tokens,
+                            int64_t experts, int64_t k, const void* const* ids, int ids_are_i64, const void* mask,
+                            int mask_kind, const int32_t* cu_seqlens, int64_t n_seqs, int score, float* loss, float* coef,
+                            float* scale, int64_t* counts, void* workspace, int64_t workspace_bytes, void* stream);
+int axon_router_balance_bwd(const void* const* logits, int dtype, int64_t ld, int64_t layers, int64_t n_tokens,
+                            int64_t experts, const void* mask, int mask_kind, const int32_t* cu_seqlens, int64_t n_seqs,
+                            int score, const float* coef, const float* scale, const float* g_loss, void* const* dlogits,
+                            void* stream);
+
 /* KL penalty inside the reward, the tensor part of apply_kl_penalty (axon/utils/rl/kl.py:276-322):
  *   kld = kl_penalty(old_logp, ref_logp, kl_type) * mask      (types as in axon_kl_penalty)
  *   rewards = scores - beta * kld
