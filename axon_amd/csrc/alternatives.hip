@@ -18,44 +18,55 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int i64, int64_t at)
   return i64 ? static_cast<const int64_t*>(ids)[at] : (int64_t) static_cast<const int32_t*>(ids)[at];
 }
 
-// The share of a row that is workgroup `part` of `parts`: whole segments, and some of the elements outside the vectors.
+// A row as it is walked: the 16-byte vectors of its aligned middle in tiles of 256 (4 KB), one wavefront each at a time; the
+// share of workgroup `part` of `parts` is whole tiles, and some of the elements outside the vectors.
+constexpr int kTileVecs = 256;
 struct SegSpan {
-  int head, n_vec, n_scalar, n_seg, q_lo, q_hi;
+  int head, n_vec, n_scalar, n_seg, tile_lo, tile_hi;
   template <typename T>
   __device__ __forceinline__ SegSpan(const T* row, int vocab, int part, int parts) {
     const RowSpan sp(row, vocab, true, 0, 1);
     head = sp.head; n_vec = sp.n_vec; n_scalar = sp.n_scalar;
     n_seg = (n_vec + kSegVecs - 1) / kSegVecs;
-    q_lo = (int)((int64_t)n_seg * part / parts) * kSegVecs;
-    q_hi = min((int)((int64_t)n_seg * (part + 1) / parts) * kSegVecs, n_vec);
+    const int tiles = (n_vec + kTileVecs - 1) / kTileVecs;
+    tile_lo = (int)((int64_t)tiles * part / parts);
+    tile_hi = (int)((int64_t)tiles * (part + 1) / parts);
   }
   template <typename T>
   __device__ __forceinline__ int scalar(int i) const { return i < head ? i : i + n_vec * Row<T>::kPer; }
 };
 
-// Folds N logits (natural units) into the statistics; their maximum.  A NaN among them makes the sums NaN, as it does
-// those of a softmax; -inf adds nothing.
-template <int N, int M>
-__device__ __forceinline__ float fold_max(Stats& a, const float (&z)[M]) {
-  float m = z[0];
+// Folds U times N logits (natural units) into the statistics, given the maxima of the U sets: one rescale at most.  A NaN
+// among the logits makes the sums NaN, as it does those of a softmax; -inf adds nothing.
+template <int N, int U, int M>
+__device__ __forceinline__ void fold_all(Stats& a, const float (&z)[U][M], const float (&set_max)[U]) {
+  float m = set_max[0];
 #pragma unroll
-  for (int j = 1; j < N; ++j) m = fmaxf(m, z[j]);
-  const float ml = m * kLog2e;
-  if (ml > a.M) {
-    const float d = fmaxf(a.M - ml, kTiny), f = __builtin_amdgcn_exp2f(d);
+  for (int u = 1; u < U; ++u) m = fmaxf(m, set_max[u]);
+  m *= kLog2e;
+  if (m > a.M) {
+    const float d = fmaxf(a.M - m, kTiny), f = __builtin_amdgcn_exp2f(d);
     a.e = f * fmaf(a.s, d, a.e);
     a.s = a.s * f;
-    a.M = ml;
+    a.M = m;
   }
   float s4[4] = {a.s, 0.f, 0.f, 0.f}, e4[4] = {a.e, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float d = fmaf(z[j], kLog2e, -a.M), f = __builtin_amdgcn_exp2f(d);
-    s4[j & 3] += f;
-    e4[j & 3] = fmaf(f, fmaxf(d, kTiny), e4[j & 3]);
-  }
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = fmaf(z[u][j], kLog2e, -a.M), f = __builtin_amdgcn_exp2f(d);
+      s4[j & 3] += f;
+      e4[j & 3] = fmaf(f, fmaxf(d, kTiny), e4[j & 3]);
+    }
   a.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
   a.e = (e4[0] + e4[1]) + (e4[2] + e4[3]);
+}
+template <int N, int M>
+__device__ __forceinline__ float max_of(const float (&z)[M]) {
+  float m = z[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) m = fmaxf(m, z[j]);
   return m;
 }
 
@@ -71,13 +82,31 @@ __device__ __forceinline__ Stats wave_merge(Stats st) {
   return st;
 }
 
-// Maximum over the sixteen lanes of a row of the wavefront, in its last lane.
-__device__ __forceinline__ float row16_max_to_last(float v) {
-  v = fmaxf(v, dpp_or_own<0x111, 0xf>(v));
-  v = fmaxf(v, dpp_or_own<0x112, 0xf>(v));
-  v = fmaxf(v, dpp_or_own<0x114, 0xf>(v));
-  v = fmaxf(v, dpp_or_own<0x118, 0xf>(v));
-  return v;
+// The lanes of a wavefront as rows of sixteen: row 1 of a changes place with row 0 of b and row 3 of a with row 2 of b, or
+// rows 2 and 3 of a with rows 0 and 1 of b.  Written as instructions: through the builtins the compiler takes the two
+// results for one value.  The s_nop covers the wait states that the swaps need after a vector instruction.
+__device__ __forceinline__ void swap_rows16(float& a, float& b) {
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void swap_rows32(float& a, float& b) {
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+
+// A tile's 256 vectors in the lanes: lane 16 r + c loads, of every 64 consecutive ones, number 16 (c / 4) + 4 r + c % 4, so
+// that a segment's sixteen vectors of load u lie in the four lanes of the same c / 4 in each row.
+__device__ __forceinline__ int tile_vec(int lane) { return ((lane & 12) << 2) + ((lane >> 4) << 2) + (lane & 3); }
+// The maxima of the tile's sixteen segments from those of a lane's four vectors: segment 4 u + c / 4 in the lanes 16 u + c.
+// Three swaps carry the four values over the rows at once, two steps the rest: 13 instructions for 4 KB, where a reduction
+// of each value by itself took 32 and its store as many again.
+__device__ __forceinline__ float tile_maxima(const float (&v)[4]) {
+  float a = v[0], b = v[1], c = v[2], d = v[3];
+  swap_rows16(a, b);
+  swap_rows16(c, d);
+  float x = fmaxf(a, b), y = fmaxf(c, d);
+  swap_rows32(x, y);
+  x = fmaxf(x, y);
+  x = fmaxf(x, dpp_or_own<0xb1, 0xf>(x));  // lane ^ 1
+  return fmaxf(x, dpp_or_own<0x4e, 0xf>(x));  // lane ^ 2
 }
 
 struct RowOut {
@@ -111,13 +140,61 @@ __device__ __forceinline__ void write_picks(const Picks& p, int t, const T* row,
   }
 }
 
-// Workgroup (row, part): blockIdx.x = row * parts + part.  Leaves its statistics in ws[row][part][3] and, with SEG, the
-// maxima of its segments in seg_max[row][seg].  Without SEG and with one part per row it finishes the row.
+// A row of logits as select_top reads it.
+template <typename T>
+struct LogitsSource {
+  static constexpr int kPer = Row<T>::kPer, kItems = kSegVecs;
+  const T* row;
+  const float* seg_max;  // LDS or global
+  SegSpan sp;
+  int vocab;
+  __device__ int n_segs() const { return sp.n_seg; }
+  __device__ uint32_t max_key(int i) const { return order_key(seg_max[i]); }
+  __device__ int limit() const { return vocab; }
+  __device__ int load(const int* segs, int j, float (&v)[kPer]) const {
+    const int q = segs[j / kSegVecs] * kSegVecs + (j & (kSegVecs - 1));
+    if (q >= sp.n_vec) return -1;
+    float x[8];
+    const int at = sp.head + q * kPer;
+    Row<T>::template load<true>(row + at, x);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = x[e];
+    return at;
+  }
+  __device__ int n_single() const { return sp.n_scalar; }
+  __device__ float single(int i, int& index) const {
+    index = sp.scalar<T>(i);
+    return Row<T>::one(row + index);
+  }
+};
+
+struct TopOut {
+  float* logprobs;  // [n][k]
+  int64_t* ids;     // [n][k]
+  int k;
+};
+template <typename T>
+__device__ __forceinline__ void write_top(const TopOut& o, int t, const T* row, int vocab, const float* seg_max, float lse,
+                                          SelectLds& s) {
+  const LogitsSource<T> src{row, seg_max, SegSpan(row, vocab, 0, 1), vocab};
+  select_top<kBlock>(src, o.k, s, threadIdx.x, [&](int rank, float z, int index) {
+    o.logprobs[(int64_t)t * o.k + rank] = z - lse;
+    o.ids[(int64_t)t * o.k + rank] = index;
+  });
+}
+
+// What is wanted of a row beside its statistics.
+enum Want { kTokens, kTop };
+
+// Workgroup (row, part): blockIdx.x = row * parts + part.  Where a row has one part it is finished here: a row's selection
+// runs beside the reading of the rows that the compute unit's other workgroups have (the maxima of its segments are in
+// LDS).  Else the statistics go to ws[row][part][3] and the maxima to seg_max[row][seg], for the kernels below.
 // Rows from `cached_from` on are left in the cache in front of the memory, for what reads them next.
-template <typename T, bool SEG>
-__global__ __launch_bounds__(kBlock) void alternatives_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
-                                                                    float* __restrict__ ws, float* __restrict__ seg_max,
-                                                                    int seg_stride, RowOut out, Picks picks, int cached_from) {
+template <typename T, Want WANT>
+__global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
+                                                              float* __restrict__ ws, float* __restrict__ seg_max, int seg_stride,
+                                                              RowOut out, Picks picks, TopOut top, int cached_from) {
+  extern __shared__ __align__(16) char smem[];
   __shared__ float red[3][kBlock / kWave];
   __shared__ float s_lse;
   const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
@@ -125,55 +202,61 @@ __global__ __launch_bounds__(kBlock) void alternatives_stats_kernel(const T* __r
   constexpr int kPer = Row<T>::kPer;
   const SegSpan sp(row, vocab, part, parts);
   const T* body = row + sp.head;
-  float* const segs = SEG ? seg_max + (int64_t)t * seg_stride : nullptr;
-  const int tid = threadIdx.x;
+  const bool whole = parts == 1 && seg_max == nullptr;
+  float* const segs = reinterpret_cast<float*>(smem + sizeof(SelectLds));  // where the row is finished here
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   Stats st{kFloor, 0.f, 0.f};
-  auto keep_max = [&](int q, float m) {
-    if (!SEG) return;
-    m = row16_max_to_last(m);
-    if ((tid & 15) == 15 && (q & ~15) < sp.q_hi) segs[q / kSegVecs] = m;
-  };
   auto walk = [&](auto cached) {
     constexpr bool kCached = decltype(cached)::value;
-    int b = sp.q_lo;
-    for (; b + 2 * kBlock <= sp.q_hi; b += 2 * kBlock) {  // two loads in flight per thread
-      float v0[8], v1[8];
-      const int q = b + tid;
-      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v0);
-      Row<T>::template load<kCached>(body + (uint32_t)(q + kBlock) * kPer, v1);
-      keep_max(q, fold_max<kPer>(st, v0));
-      keep_max(q + kBlock, fold_max<kPer>(st, v1));
-    }
-    for (; b < sp.q_hi; b += kBlock) {
-      float v[8];
-      const int q = b + tid;
+    const int mine = tile_vec(lane);
+    for (int tile = sp.tile_lo + wave; tile < sp.tile_hi; tile += kBlock / kWave) {
+      float v[4][8], m[4];
+      const int q0 = tile * kTileVecs + mine;
+      if ((tile + 1) * kTileVecs <= sp.n_vec) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
-      if (q < sp.q_hi) Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v);
-      keep_max(q, fold_max<kPer>(st, v));
+        for (int u = 0; u < 4; ++u) Row<T>::template load<kCached>(body + (uint32_t)(q0 + u * kWave) * kPer, v[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) v[u][j] = -INFINITY;
+          if (q0 + u * kWave < sp.n_vec) Row<T>::template load<kCached>(body + (uint32_t)(q0 + u * kWave) * kPer, v[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m[u] = max_of<kPer>(v[u]);
+      fold_all<kPer>(st, v, m);
+      if (WANT == kTop) {
+        const float best = tile_maxima(m);
+        const int seg = tile * (kTileVecs / kSegVecs) + (lane >> 2);
+        if ((lane & 3) == 0 && seg < sp.n_seg) {
+          if (whole) segs[seg] = best;
+          else seg_max[(int64_t)t * seg_stride + seg] = best;
+        }
+      }
     }
   };
   if (t >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
   for (int i = part * kBlock + tid; i < sp.n_scalar; i += parts * kBlock) {
-    const float v[1] = {Row<T>::one(row + sp.scalar<T>(i))};
-    fold_max<1>(st, v);
+    const float v[1][1] = {{Row<T>::one(row + sp.scalar<T>(i))}};
+    fold_all<1>(st, v, v[0]);
   }
   st = wave_merge(st);
-  const int lane = tid & (kWave - 1), wave = tid / kWave;
   if (lane == 0) { red[0][wave] = st.M; red[1][wave] = st.s; red[2][wave] = st.e; }
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < kBlock / kWave; ++w) st = merge(st, Stats{red[0][w], red[1][w], red[2][w]});
-    if (SEG || parts > 1) {
+    if (!whole) {
       float* o = ws + (int64_t)blockIdx.x * 3;
       o[0] = st.M; o[1] = st.s; o[2] = st.e;
     } else {
       s_lse = write_row<T>(st, t, row, vocab, out);
     }
   }
-  if (SEG || parts > 1) return;
+  if (!whole) return;
   __syncthreads();
-  write_picks<T>(picks, t, row, vocab, s_lse);
+  if (WANT == kTop) write_top<T>(top, t, row, vocab, segs, s_lse, *reinterpret_cast<SelectLds*>(smem));
+  else write_picks<T>(picks, t, row, vocab, s_lse);
 }
 
 // The statistics of a row's parts (at most kMaxParts), in a fixed tree; the total in thread 0.
@@ -199,40 +282,11 @@ __global__ __launch_bounds__(kBlock) void tokens_finish_kernel(const T* __restri
   write_picks<T>(picks, t, row, vocab, s_lse);
 }
 
-// A row of logits as select_top reads it.
-template <typename T>
-struct LogitsSource {
-  static constexpr int kPer = Row<T>::kPer, kItems = kSegVecs;
-  const T* row;
-  const float* seg_max;
-  SegSpan sp;
-  int vocab;
-  __device__ int n_segs() const { return sp.n_seg; }
-  __device__ uint32_t max_key(int i) const { return order_key(seg_max[i]); }
-  __device__ int limit() const { return vocab; }
-  __device__ int load(const int* segs, int j, float (&v)[kPer]) const {
-    const int q = segs[j / kSegVecs] * kSegVecs + (j & (kSegVecs - 1));
-    if (q >= sp.n_vec) return -1;
-    float x[8];
-    const int at = sp.head + q * kPer;
-    Row<T>::template load<true>(row + at, x);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = x[e];
-    return at;
-  }
-  __device__ int n_single() const { return sp.n_scalar; }
-  __device__ float single(int i, int& index) const {
-    index = sp.scalar<T>(i);
-    return Row<T>::one(row + index);
-  }
-};
-
 // A workgroup per row: folds the parts' statistics, selects the k largest.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void top_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
                                                             const float* __restrict__ ws, const float* __restrict__ seg_max,
-                                                            int seg_stride, int k, RowOut out, float* __restrict__ top_logprobs,
-                                                            int64_t* __restrict__ top_ids) {
+                                                            int seg_stride, RowOut out, TopOut top) {
   __shared__ SelectLds s;
   __shared__ float s_lse;
   const int t = blockIdx.x;
@@ -240,12 +294,7 @@ __global__ __launch_bounds__(kBlock) void top_finish_kernel(const T* __restrict_
   const Stats st = merge_parts(ws, t, parts);
   if (threadIdx.x == 0) s_lse = write_row<T>(st, t, row, vocab, out);
   __syncthreads();
-  const float lse = s_lse;
-  const LogitsSource<T> src{row, seg_max + (int64_t)t * seg_stride, SegSpan(row, vocab, 0, 1), vocab};
-  select_top<kBlock>(src, k, s, threadIdx.x, [&](int rank, float z, int index) {
-    top_logprobs[(int64_t)t * k + rank] = z - lse;
-    top_ids[(int64_t)t * k + rank] = index;
-  });
+  write_top<T>(top, t, row, vocab, seg_max + (int64_t)t * seg_stride, s_lse, s);
 }
 
 // Upstream gradients of a row's chosen tokens: k of them, and a label's.  Either may be absent (g null).
@@ -378,6 +427,10 @@ int64_t seg_stride(int dtype, int64_t vocab) {
   return (vocab + per - 1) / per;
 }
 
+// What a workgroup that finishes its row holds in LDS; more than this and the rows are finished by a kernel of their own.
+constexpr int64_t kMaxTopLds = 48 * 1024;
+int64_t top_lds(int dtype, int64_t vocab) { return (int64_t)sizeof(SelectLds) + seg_stride(dtype, vocab) * 4; }
+
 int check_rows(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v) {
   if (n < 0 || v <= 0 || ld < v || !dtype_ok(dtype)) return AXON_ERR_ARG;
   if (n >= (int64_t)1 << 25 || v >= (int64_t)1 << 30) return AXON_ERR_SHAPE;  // rows times parts are a grid
@@ -400,7 +453,9 @@ int cached_from(int64_t n, int64_t vocab, int eb, int bwd_follows) {
 
 extern "C" int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
   if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
-  return n * (row_parts(n, vocab, elem_bytes(dtype)) * 3 + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
+  const int parts = row_parts(n, vocab, elem_bytes(dtype));
+  if (parts == 1 && top_lds(dtype, vocab) <= kMaxTopLds) return 0;
+  return n * (parts * 3 + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
 }
 
 extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, int64_t k,
@@ -411,20 +466,27 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
   if (rc != AXON_OK) return rc;
   if (k < 1 || k > kMaxTop || k > vocab) return AXON_ERR_SHAPE;
   if (n == 0) return AXON_OK;
-  if (!lse || !top_logprobs || !top_ids || !workspace || (logprob && !labels)) return AXON_ERR_ARG;
-  if (axon_logits_top_workspace_bytes(dtype, n, vocab) > workspace_bytes) return AXON_ERR_WORKSPACE;
+  if (!lse || !top_logprobs || !top_ids || (logprob && !labels)) return AXON_ERR_ARG;
+  const int64_t need = axon_logits_top_workspace_bytes(dtype, n, vocab);
+  if (need > 0 && !workspace) return AXON_ERR_ARG;
+  if (need > workspace_bytes) return AXON_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
   const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
-  float* const seg_max = workspace + n * parts * 3;
+  const bool whole = need == 0;
+  float* const seg_max = whole ? nullptr : workspace + n * parts * 3;
   const int stride = (int)seg_stride(dtype, vocab), from = cached_from(n, vocab, eb, bwd_follows);
+  const unsigned lds = whole ? (unsigned)top_lds(dtype, vocab) : 0;
   const RowOut out{logprob, entropy, lse, labels, labels_i64};
+  const TopOut top{top_logprobs, top_ids, (int)k};
 #define AXON_TOP(T)                                                                                                        \
   do {                                                                                                                     \
-    hipLaunchKernelGGL((alternatives_stats_kernel<T, true>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,             \
-                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, seg_max, stride, out, Picks{}, from); \
+    hipLaunchKernelGGL((alternatives_kernel<T, kTop>), dim3((unsigned)(n * parts)), dim3(kBlock), lds, st,                 \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, seg_max, stride, out, Picks{}, top, \
+                       from);                                                                                              \
     AXON_CHECK_LAUNCH();                                                                                                   \
-    hipLaunchKernelGGL((top_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld,  \
-                       (int)vocab, parts, workspace, seg_max, stride, (int)k, out, top_logprobs, top_ids);                 \
+    if (!whole)                                                                                                            \
+      hipLaunchKernelGGL((top_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),    \
+                         ld, (int)vocab, parts, workspace, seg_max, stride, out, top);                                     \
   } while (0)
   AXON_ROWS(dtype, AXON_TOP);
 #undef AXON_TOP
@@ -455,8 +517,9 @@ extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld,
   const int from = cached_from(n, vocab, eb, bwd_follows);
 #define AXON_TOKENS(T)                                                                                                      \
   do {                                                                                                                      \
-    hipLaunchKernelGGL((alternatives_stats_kernel<T, false>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,             \
-                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, nullptr, 0, out, picks, from);      \
+    hipLaunchKernelGGL((alternatives_kernel<T, kTokens>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,                 \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, workspace, nullptr, 0, out, picks, TopOut{},   \
+                       from);                                                                                               \
     AXON_CHECK_LAUNCH();                                                                                                    \
     if (parts > 1)                                                                                                          \
       hipLaunchKernelGGL((tokens_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),  \

@@ -10,8 +10,9 @@
 
 namespace axon {
 
-constexpr int kMaxTop = 128;       // alternatives per row
-constexpr int kCandidates = 1024;  // elements that reach the smallest of the k maxima and are ranked against each other
+constexpr int kMaxTop = 128;      // alternatives per row
+constexpr int kCandidates = 512;  // elements that reach the smallest maximum taken and are ranked against each other
+constexpr int kMaxSegs = 2 * kMaxTop;  // segments taken: the first k and a few more where that saves a look
 
 // Unsigned integers in the order of the floats; -0 equals 0, NaN is below everything.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -29,8 +30,9 @@ __device__ __forceinline__ uint64_t order_key(float x, int index) {
 struct SelectLds {
   uint64_t cand[kCandidates];
   int hist[256];
-  int segs[kMaxTop], equal[kMaxTop];
-  int n_segs, n_equal, n_cand, bin, before;
+  int segs[kMaxSegs];
+  uint32_t range[2][4];
+  int n_segs, n_cand, bin, before, upto;
 };
 
 // NT threads work on a row: a wavefront (64), whose LDS accesses are carried out in order, or a workgroup.
@@ -80,6 +82,83 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
   return prefix;
 }
 
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
+  return v;
+}
+
+// The segments that are looked at, to s.segs: those whose maximum reaches a bound (returned) that at least k maxima reach.
+// The keys' range is cut into 256 bins and the bin of the k-th taken whole if that makes at most half as many again; else
+// the bin is cut again, down to one key, of whose segments the first are taken then.  A row of a model's logits takes one cut.
+template <int NT, class Src>
+__device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k, SelectLds& s, int tid) {
+  const int lane = tid & (kWave - 1), wave = tid / kWave, most = k + k / 2 + 8;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int i = tid; i < n; i += NT) {
+    const uint32_t key = src.max_key(i);
+    lo = min(lo, key);
+    hi = max(hi, key);
+  }
+  lo = ~wave_max_u32(~lo);
+  hi = wave_max_u32(hi);
+  if (NT > kWave) {
+    if (lane == 0) { s.range[0][wave] = lo; s.range[1][wave] = hi; }
+    group_sync<NT>();
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) { lo = min(lo, s.range[0][w]); hi = max(hi, s.range[1][w]); }
+  }
+  int rest = k, above = 0;  // of the segments in the range, `rest` are wanted; `above`: segments above the range
+  uint32_t least;
+  for (uint32_t width = hi - lo;;) {  // the range: lo .. lo + width
+    const int shift = width < 256 ? 0 : 24 - __builtin_clz(width);
+    for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+    group_sync<NT>();
+    for (int i = tid; i < n; i += NT) {
+      const uint32_t at = src.max_key(i) - lo;
+      if (at <= width) atomicAdd(&s.hist[at >> shift], 1);
+    }
+    group_sync<NT>();
+    if (tid < kWave) {  // lane l: bins 255 - 4 l and the three below
+      int c[4], sum = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
+      int upto = sum;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int o = __shfl_up(upto, off, kWave);
+        if (tid >= off) upto += o;
+      }
+      int before = upto - sum;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; s.upto = before + c[q]; }
+        before += c[q];
+      }
+    }
+    group_sync<NT>();
+    least = lo + ((uint32_t)s.bin << shift);
+    if (above + s.upto <= most || shift == 0) break;
+    above += s.before;
+    rest -= s.before;
+    const uint32_t last = lo + width;
+    lo = least;
+    width = min((1u << shift) - 1, last - lo);
+  }
+  const int ties = rest - s.before;  // at a bin of one key: how many of its segments are wanted
+  if (above + s.upto <= most) {
+    for (int i = tid; i < n; i += NT)
+      if (src.max_key(i) >= least) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+    return least;
+  }
+  int one;
+  auto first = [&](int i) { return src.max_key(i) == least ? 0xffffffffu - (uint32_t)i : 0u; };
+  const uint32_t last = kth_largest<NT, uint32_t>(first, n, ties, s, tid, one);
+  for (int i = tid; i < n; i += NT)
+    if (src.max_key(i) > least || first(i) >= last) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+  return least;
+}
+
 // `src`: maxima of its segments, max_key(i) for i < n_segs(); the elements of the segments in `segs`, kPer consecutive ones
 // per item: load(segs, j, v) returns the index of the first, or -1 where there is none (elements from limit() on do not
 // count); and n_single() elements outside all segments, single(i, index).  out(rank, value, index) for rank < k.
@@ -87,36 +166,14 @@ template <int NT, class Src, class Out>
 __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, int tid, Out out) {
   const int n = src.n_segs();
   uint32_t least = 0;  // what an element has to reach
-  if (tid == 0) s.n_segs = s.n_equal = s.n_cand = 0;
+  if (tid == 0) s.n_segs = s.n_cand = 0;
   if (n > k) {
-    int ties;
-    auto key_at = [&](int i) { return src.max_key(i); };
-    least = kth_largest<NT, uint32_t>(key_at, n, k, s, tid, ties);
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t key = key_at(i);
-      if (key > least) s.segs[atomicAdd(&s.n_segs, 1)] = i;  // fewer than k
-      if (key == least) {
-        const int at = atomicAdd(&s.n_equal, 1);
-        if (at < ties) s.equal[at] = i;
-      }
-    }
-    group_sync<NT>();
-    if (s.n_equal == ties) {
-      const int at = s.n_segs;
-      group_sync<NT>();
-      for (int i = tid; i < ties; i += NT) s.segs[at + i] = s.equal[i];
-    } else {  // more segments with that maximum than are wanted: the first of them
-      int one;
-      auto first = [&](int i) { return key_at(i) == least ? 0xffffffffu - (uint32_t)i : 0u; };
-      const uint32_t last = kth_largest<NT, uint32_t>(first, n, ties, s, tid, one);
-      for (int i = tid; i < n; i += NT)
-        if (first(i) >= last) s.segs[atomicAdd(&s.n_segs, 1)] = i;
-    }
+    least = choose_segments<NT>(src, n, k, s, tid);
   } else {
     for (int i = tid; i < n; i += NT) s.segs[i] = i;
   }
   group_sync<NT>();
-  const int n_items = (n < k ? n : k) * Src::kItems, limit = src.limit();
+  const int n_items = (n > k ? s.n_segs : n) * Src::kItems, limit = src.limit();
   auto offer = [&](float x, int index) {
     if (order_key(x) < least) return;
     const int at = atomicAdd(&s.n_cand, 1);

@@ -56,17 +56,17 @@ def test_the_c_entry_points_check_their_arguments():
     """Status codes of calls that a kernel must not see: null pointers, sizes, small workspaces, unaligned rows."""
     lib = _lib.load()
     p = ctypes.addressof(ctypes.create_string_buffer(64)) & ~15  # any address: nothing is read
-    ws = lib.axon_logits_top_workspace_bytes(0, 2, 100)
+    ws = lib.axon_logits_top_workspace_bytes(0, 2, 100000)
     assert ws > 0 and lib.axon_logits_top_workspace_bytes(7, 2, 100) < 0 and lib.axon_logits_top_workspace_bytes(0, 2, 0) < 0
 
-    def top(logits=p, dtype=0, ld=100, n=2, v=100, k=3, logprob=None, labels=None, lse=p, lp=p, ids=p, w=p, wb=ws):
+    def top(logits=p, dtype=0, ld=100000, n=2, v=100000, k=3, logprob=None, labels=None, lse=p, lp=p, ids=p, w=p, wb=ws):
         return lib.axon_logits_top_fwd(logits, dtype, ld, n, v, k, labels, 1, logprob, p, lse, lp, ids, w, wb, 0, None)
 
     assert top(n=0) == 0
-    for bad in (dict(logits=None), dict(dtype=2), dict(ld=99), dict(n=-1), dict(v=0), dict(lse=None), dict(lp=None),
+    for bad in (dict(logits=None), dict(dtype=2), dict(ld=99999), dict(n=-1), dict(v=0), dict(lse=None), dict(lp=None),
                 dict(ids=None), dict(w=None), dict(logprob=p), dict(logits=p + 2)):
         assert top(**bad) == -1, bad
-    for bad in (dict(k=0), dict(k=129), dict(k=101), dict(n=1 << 25), dict(v=1 << 30, ld=1 << 30)):
+    for bad in (dict(k=0), dict(k=129), dict(k=101, v=100), dict(n=1 << 25), dict(v=1 << 30, ld=1 << 30)):
         assert top(**bad) == -2, bad
     assert top(wb=ws - 1) == -3
 
