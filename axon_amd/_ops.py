@@ -10,7 +10,6 @@ code (``_lib.native()``, csrc/torch_ext.cpp).  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import contextlib
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -669,6 +668,8 @@ class Timer:
             raise _lib.AxonAmdError("axon_timer_create failed")
 
     def collect(self) -> dict:
+        import ctypes
+
         ms, cnt = (ctypes.c_float * 8)(), (ctypes.c_int32 * 8)()
         check(self._lib.axon_timer_collect(self.handle, ms, cnt), "axon_timer_collect")
         return {name: {"ms": float(ms[i]), "launches": int(cnt[i])} for i, name in enumerate(_PHASES) if cnt[i]}
@@ -1181,81 +1182,6 @@ def token_ids_arg(what, ids, rows, device):
     return ids.contiguous()
 
 
-def logits_top(logits, k, labels=None, backward_follows=False):
-    """``(logprob | None, entropy, lse, top_logprobs [tokens, k], top_ids [tokens, k])``; see axon_logits_top_fwd."""
-    n, v, ld = _logits_operands("logits_top", logits, labels)
-    _top_count("logits_top", k, v)
-    require_device(logits, "logits_top")
-    lib = _lib.load()
-    dev, dt = logits.device, _LOGITS_DTYPES[logits.dtype]
-    with on_device_of(logits):
-        out = torch.empty(n * (3 + k), device=dev, dtype=torch.float32)
-        top_ids = torch.empty(n, k, device=dev, dtype=torch.int64)
-        ws_bytes = lib.axon_logits_top_workspace_bytes(dt, n, v)
-        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
-        base = out.data_ptr()
-        check(
-            lib.axon_logits_top_fwd(ptr(logits), dt, ld, n, v, k, ptr(labels),
-                                    int(labels is not None and labels.dtype == torch.int64),
-                                    base if labels is not None else None, base + 4 * n, base + 8 * n, base + 12 * n,
-                                    ptr(top_ids), ptr(ws), ws_bytes, int(backward_follows), stream_ptr()),
-            "axon_logits_top_fwd",
-        )
-    lp, ent, lse = out[: 3 * n].view(3, n).unbind(0)
-    return (lp if labels is not None else None), ent, lse, out[3 * n:].view(n, k), top_ids
-
-
-def logits_tokens(logits, token_ids, backward_follows=False):
-    """``(logprobs [tokens, k], entropy, lse)`` of given tokens; see axon_logits_tokens_fwd."""
-    n, v, ld = _logits_operands("logits_tokens", logits, None)
-    ids = token_ids_arg("logits_tokens", token_ids, n, logits.device)
-    require_device(logits, "logits_tokens")
-    lib = _lib.load()
-    k, dev, dt = int(ids.shape[1]), logits.device, _LOGITS_DTYPES[logits.dtype]
-    with on_device_of(logits):
-        out = torch.empty(n * (2 + k), device=dev, dtype=torch.float32)
-        ws_bytes = lib.axon_logits_tokens_workspace_bytes(dt, n, v)
-        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32) if ws_bytes > 0 else None
-        base = out.data_ptr()
-        check(
-            lib.axon_logits_tokens_fwd(ptr(logits), dt, ld, n, v, ptr(ids), int(ids.dtype == torch.int64), k,
-                                       base + 8 * n, base, base + 4 * n, ptr(ws), max(ws_bytes, 0),
-                                       int(backward_follows), stream_ptr()),
-            "axon_logits_tokens_fwd",
-        )
-    return out[2 * n:].view(n, k), out[:n], out[n: 2 * n]
-
-
-def logits_tokens_backward(logits, token_ids, labels, lse, entropy, g_ids, g_label, g_entropy, inplace=False):
-    """d loss / d logits (written over the logits when ``inplace``) from the gradients of the log-probabilities of
-    ``token_ids`` and of ``labels`` and of the entropy, each of which may be None; see axon_logits_tokens_bwd."""
-    lib = _lib.load()
-    what = "logits_tokens_backward"
-    require_device(logits, what)
-    n, v, ld = _logits_operands(what, logits, labels)
-    k = 0
-    if token_ids is not None:
-        token_ids = token_ids_arg(what, token_ids, n, logits.device)
-        k = int(token_ids.shape[1])
-    g_ids, g_label, g_en = (None if g is None else f32(g) for g in (g_ids, g_label, g_entropy))
-    _same_len(what, n, lse=lse, entropy=entropy, g_label=g_label, g_entropy=g_en)
-    _same_len(what, n * k, g_ids=g_ids)
-    for g in (g_ids, g_label, g_en):
-        if g is not None and g.device != logits.device:
-            raise ValueError(f"{what}: operands live on different devices")
-    with on_device_of(logits):
-        out = logits if inplace else torch.empty_like(logits, memory_format=torch.contiguous_format)
-        ld_d = int(out.stride(0)) if n > 1 else v
-        check(
-            lib.axon_logits_tokens_bwd(ptr(logits), _LOGITS_DTYPES[logits.dtype], ld, n, v, ptr(token_ids),
-                                       int(token_ids is not None and token_ids.dtype == torch.int64), k, ptr(labels),
-                                       int(labels is not None and labels.dtype == torch.int64), ptr(lse), ptr(entropy),
-                                       ptr(g_ids), ptr(g_label), ptr(g_en), ptr(out), ld_d, stream_ptr()),
-            "axon_logits_tokens_bwd",
-        )
-    return out
-
-
 # Bytes of fp32 logits that a call of the head with alternatives holds at most: longer batches are cut into blocks of
 # tokens (2.5 GB: 4096 tokens of the 151936 vocabulary; never fewer than 256).
 TOP_LOGITS_BYTES = 2560 << 20
@@ -1348,99 +1274,6 @@ def lmhead_tokens_backward(g_logprobs, g_entropy, hidden, weight, token_ids, log
                                          ws_bytes, stream_ptr()), "axon_lmhead_tokens_bwd")
     return d_hidden, d_weight
 
-
-MAX_EXPERTS = 1024
-ROUTER_SCORES = {"softmax": 0, "sigmoid": 1}
-
-
-@dataclass
-class RouterBatch:
-    """Checked operands of the balance loss: one ``[tokens, experts]`` tensor per layer, all with row stride ``ld``."""
-
-    logits: list
-    ld: int
-    mask: torch.Tensor | None
-    mask_kind: int
-    cu: torch.Tensor | None
-    score: int
-
-    @property
-    def n_seqs(self):
-        return 1 if self.cu is None else int(self.cu.numel()) - 1
-
-    @property
-    def head(self):  # dtype, ld, layers, tokens, experts as the entry points take them
-        x = self.logits[0]
-        return _LOGITS_DTYPES[x.dtype], self.ld, len(self.logits), int(x.shape[0]), int(x.shape[1])
-
-    @property
-    def tail(self):
-        return ptr(self.mask), self.mask_kind, ptr(self.cu), self.n_seqs, self.score
-
-
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*(None if t is None else t.data_ptr() for t in tensors))
-
-
-def router_batch(layers, token_mask, cu_seqlens, score_fn):
-    """``RouterBatch`` of the layers' router logits (2-D, one per layer)."""
-    what = "router_balance_loss"
-    if score_fn not in ROUTER_SCORES:
-        raise ValueError(f"{what}: score_fn must be one of {sorted(ROUTER_SCORES)}, got {score_fn!r}")
-    first = layers[0]
-    if first.dtype not in _LOGITS_DTYPES:
-        raise ValueError(f"{what}: router logits must be fp32 or bf16, got {first.dtype}")
-    n, e = first.shape
-    if not 1 <= e <= MAX_EXPERTS:
-        raise ValueError(f"{what}: between 1 and {MAX_EXPERTS} experts, got {e}")
-    for t in layers:
-        if t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
-            raise ValueError(f"{what}: the layers' logits must agree in shape, type and device")
-    mask, kind = None, MASK_F32
-    if token_mask is not None:
-        if int(token_mask.numel()) != n:
-            raise ValueError(f"{what}: token_mask has {int(token_mask.numel())} entries for {n} tokens")
-        if token_mask.device != first.device:
-            raise ValueError(f"{what}: operands live on different devices")
-        mask, kind = mask_arg(token_mask)
-    cu = None
-    if cu_seqlens is not None:
-        if cu_seqlens.dim() != 1 or int(cu_seqlens.numel()) < 1:
-            raise ValueError(f"{what}: cu_seqlens must be [sequences + 1]")
-        cu = cu_seqlens.to(device=first.device, dtype=torch.int32).contiguous()
-    require_device(first, what)
-    ld = int(first.stride(0)) if n > 1 else int(e)
-    same = all(t.stride(1) == 1 and (n <= 1 or int(t.stride(0)) == ld) for t in layers) and ld >= e
-    rows = [t.detach() for t in layers] if same else [t.detach().contiguous() for t in layers]
-    return RouterBatch(rows, ld if same else int(e), mask, kind, cu, ROUTER_SCORES[score_fn])
-
-
-def router_balance(batch: RouterBatch, k, expert_ids=None):
-    """``(loss [], counts int64 [layers, experts], coef, scale)``; see axon_router_balance_fwd.  ``expert_ids``: one
-    ``[tokens, k]`` tensor per layer, or None."""
-    lib = _lib.load()
-    dt, ld, layers, n, e = batch.head
-    dev = batch.logits[0].device
-    with on_device_of(batch.logits[0]):
-        loss, scale = torch.empty((), device=dev, dtype=torch.float32), torch.empty(1, device=dev, dtype=torch.float32)
-        coef = torch.empty(batch.n_seqs, layers, e, device=dev, dtype=torch.float32)
-        counts = torch.empty(layers, e, device=dev, dtype=torch.int64)
-        ws_bytes = lib.axon_router_balance_workspace_bytes(n, batch.n_seqs, layers, e)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        ids = None if expert_ids is None else _pointers(expert_ids)
-        ids_i64 = int(expert_ids is not None and expert_ids[0].dtype == torch.int64)
-        check(lib.axon_router_balance_fwd(_pointers(batch.logits), dt, ld, layers, n, e, k, ids, ids_i64, *batch.tail, ptr(loss),
-                                          ptr(coef), ptr(scale), ptr(counts), ptr(ws), ws_bytes, stream_ptr()),
-              "axon_router_balance_fwd")
-    return loss, counts, coef, scale
-
-
-def router_balance_backward(batch: RouterBatch, coef, scale, g_loss, dlogits):
-    """Gradients into ``dlogits`` (one contiguous tensor per layer, or None); see axon_router_balance_bwd."""
-    g = g_loss.detach().reshape(1).to(device=coef.device, dtype=torch.float32)
-    with on_device_of(batch.logits[0]):
-        check(_lib.load().axon_router_balance_bwd(_pointers(batch.logits), *batch.head, *batch.tail, ptr(coef), ptr(scale),
-                                                  ptr(g), _pointers(dlogits), stream_ptr()), "axon_router_balance_bwd")
 
 def gemm_nt(a, b):
     """out[n][m] = sum_k a[m][k] * b[n][k]; bf16 in, fp32 out.  Test/benchmark helper."""

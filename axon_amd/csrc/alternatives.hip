@@ -12,7 +12,7 @@ namespace axon {
 
 constexpr int kMaxParts = 64;
 constexpr int kSegVecs = 16;        // 16-byte vectors per segment: what sixteen neighbouring lanes load together
-constexpr int kMaxTokenIds = 512;   // given tokens per row
+constexpr int kMaxTokenIds = AXON_MAX_TOKEN_IDS;  // given tokens per row
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int i64, int64_t at) {
   return i64 ? static_cast<const int64_t*>(ids)[at] : (int64_t) static_cast<const int32_t*>(ids)[at];

@@ -15,7 +15,7 @@
 namespace axon {
 
 constexpr int kMaxLayers = 64;     // per launch: their pointers travel as kernel arguments
-constexpr int kMaxExperts = 1024;
+constexpr int kMaxExperts = AXON_MAX_EXPERTS;
 
 enum Score { kSoftmax = 0, kSigmoid = 1 };
 

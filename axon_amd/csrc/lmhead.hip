@@ -1050,44 +1050,50 @@ struct TopParams {
   float* logprobs;     // of the labels: a label outside the vocabulary gets 0 here
   int n_tokens, vocab, parts, tiles_n, k, labels_i64;
   float inv_temp, cap, inv_cap;
-  int staged;        // the maxima of the workgroup's tokens fit in LDS
+  int staged;        // a token's maxima fit in LDS
 };
 
-// A wavefront per token, four neighbouring tokens per workgroup, whose part maxima are staged together.
-constexpr int kTopTokens = 4;
-__global__ __launch_bounds__(kTopTokens * kWave) void lmhead_top_kernel(TopParams p) {
+// A workgroup per token.  The maxima of sixteen neighbouring tokens lie in the same cache lines: their workgroups are given to
+// one XCD (workgroups go round the eight of them), where all but the first find them in its L2.  A wavefront per token and
+// four tokens per workgroup, with the maxima in LDS: 8 x 151936, 20 alternatives, 31 us, 4096 x 151936 128 us.
+constexpr int kXcds = 8, kNeighbours = 16;
+__global__ __launch_bounds__(kBlock) void lmhead_top_kernel(TopParams p) {
   extern __shared__ __align__(16) char smem[];
-  SelectLds* const sel = reinterpret_cast<SelectLds*>(smem);
-  float* const staged = reinterpret_cast<float*>(smem + kTopTokens * sizeof(SelectLds));
-  const int n0 = blockIdx.x * kTopTokens, wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  SelectLds& sel = *reinterpret_cast<SelectLds*>(smem);
+  float* const staged = reinterpret_cast<float*>(smem + sizeof(SelectLds));
+  const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds, tid = threadIdx.x;
+  const int n = (turn / kNeighbours * kXcds + xcd) * kNeighbours + turn % kNeighbours;
+  if (n >= p.n_tokens) return;
   if (p.staged) {
-    for (int i = threadIdx.x; i < p.parts * kTopTokens; i += kTopTokens * kWave) {
-      const int n = min(n0 + (i & (kTopTokens - 1)), p.n_tokens - 1);
-      staged[i] = p.pm[(int64_t)(i / kTopTokens) * p.n_tokens + n];
-    }
+    for (int i = tid; i < p.parts; i += kBlock) staged[i] = p.pm[(int64_t)i * p.n_tokens + n];
     __syncthreads();
   }
-  const int n = n0 + wave;
-  if (n >= p.n_tokens) return;
   const int tn = n / kTile, in = n % kTile;
   HeadSource src;
   src.column = p.tiles + (int64_t)tn * 4 * kLogitsWaveVecs + (in / kWaveTile) * kLogitsWaveVecs +
                (in % kWaveTile) / kBlk * kBlocks * 64 + in % kBlk;
   src.tile_step = (int64_t)p.tiles_n * 4 * kLogitsWaveVecs;
-  src.maxima = p.staged ? staged + wave : p.pm + n;
-  src.stride = p.staged ? kTopTokens : p.n_tokens;
   src.parts = p.parts;
   src.vocab = p.vocab;
   const float lse = p.lse[n];
-  if (p.labels && lane == 0) {
+  if (p.labels && tid == 0) {
     const int64_t lab = p.labels_i64 ? static_cast<const int64_t*>(p.labels)[n] : (int64_t) static_cast<const int32_t*>(p.labels)[n];
     if (lab < 0 || lab >= p.vocab) p.logprobs[n] = 0.f;
   }
-  select_top<kWave>(src, p.k, sel[wave], lane, [&](int rank, float z, int index) {
+  auto out = [&](int rank, float z, int index) {
     if (p.cap != 0.f) z = p.cap * fast_tanh(z * p.inv_cap);
     p.top_logprobs[(int64_t)n * p.k + rank] = fmaf(z, p.inv_temp, -lse);
     p.top_ids[(int64_t)n * p.k + rank] = index;
-  });
+  };
+  if (p.staged) {
+    src.maxima = staged;
+    src.stride = 1;
+    select_top<kBlock>(src, p.k, sel, tid, out);
+  } else {
+    src.maxima = p.pm + n;
+    src.stride = p.n_tokens;
+    select_top<kBlock>(src, p.k, sel, tid, out);
+  }
 }
 
 struct TokenArgs {
@@ -1147,7 +1153,7 @@ __global__ __launch_bounds__(256) void token_grad_sum_kernel(TokenArgs a, int n_
 //   dl = (sum of the gradients of this id - p (G + g_H (z - E[z]))) / T * (1 - (capped logit / cap)^2)
 // rounded once, as those around it.  A wavefront per token; equal ids of a token add up in their order, in the lane of the
 // first of them.
-constexpr int kMaxTokenArgs = 513;  // given tokens per position (kMaxTokenIds and a label)
+constexpr int kMaxTokenArgs = AXON_MAX_TOKEN_IDS + 1;  // given tokens per position, and a label
 __global__ __launch_bounds__(256) void token_dlogits_kernel(DlogitParams p, TokenArgs a, int64_t chunk_rows) {
   __shared__ int ids[4][kMaxTokenArgs];
   __shared__ float gs[4][kMaxTokenArgs];
@@ -2595,7 +2601,7 @@ TopWs top_ws(int64_t n, int64_t v, void* base) {
   return w;
 }
 
-constexpr int64_t kTopLdsBytes = 150 * 1024;
+constexpr int64_t kTopLdsBytes = 48 * 1024;  // beyond: the maxima are read where they lie
 
 }  // namespace
 
@@ -2627,12 +2633,10 @@ extern "C" int axon_lmhead_top_fwd(const void* hidden, const void* weight, const
   p.parts = (int)(round_up(v, kTile) / kTile) * 2;
   p.tiles_n = (int)(round_up(n, kTile) / kTile);
   p.inv_temp = inv_temp;  p.cap = softcap;  p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
-  const int64_t select = kTopTokens * (int64_t)sizeof(SelectLds), staged = (int64_t)p.parts * kTopTokens * 4;
+  const int64_t select = (int64_t)sizeof(SelectLds), staged = (int64_t)p.parts * 4;
   p.staged = select + staged <= kTopLdsBytes;
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(lmhead_top_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)kTopLdsBytes) != hipSuccess)
-    return AXON_ERR_LAUNCH;
-  hipLaunchKernelGGL(lmhead_top_kernel, dim3((unsigned)((n + kTopTokens - 1) / kTopTokens)), dim3(kTopTokens * kWave),
+  const int64_t span = kXcds * kNeighbours;
+  hipLaunchKernelGGL(lmhead_top_kernel, dim3((unsigned)((n + span - 1) / span * span)), dim3(kBlock),
                      (unsigned)(select + (p.staged ? staged : 0)), (hipStream_t)stream, p);
   AXON_CHECK_LAUNCH();
   return AXON_OK;

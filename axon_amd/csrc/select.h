@@ -10,7 +10,7 @@
 
 namespace axon {
 
-constexpr int kMaxTop = 128;      // alternatives per row
+constexpr int kMaxTop = AXON_MAX_TOP;  // alternatives per row
 constexpr int kCandidates = 512;  // elements that reach the smallest maximum taken and are ranked against each other
 constexpr int kMaxSegs = 2 * kMaxTop;  // segments taken: the first k and a few more where that saves a look
 

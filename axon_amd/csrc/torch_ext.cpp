@@ -14,8 +14,13 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/grad_mode.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -409,6 +414,335 @@ struct FinishedLoss : torch::autograd::Function<FinishedLoss> {
   }
 };
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Alternatives of materialised logits and the router's balance loss: operators with an autograd node of their own.
+// ---------------------------------------------------------------------------------------------------------------------
+
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+[[noreturn]] void refuse(const char* what, const std::string& why) { throw py::value_error(std::string(what) + ": " + why); }
+
+std::string shape_text(const Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + (t.dim() == 1 ? ",)" : ")");
+}
+
+int logits_dtype(const char* what, const Tensor& t) {
+  if (t.scalar_type() == at::kFloat) return AXON_LOGITS_F32;
+  if (t.scalar_type() == at::kBFloat16) return AXON_LOGITS_BF16;
+  refuse(what, std::string("logits must be fp32 or bf16, got ") + c10::toString(t.scalar_type()));
+}
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+int is_i64(const Tensor& t) { return t.scalar_type() == at::kLong; }
+
+// Rows of logits as the kernels read them: [rows, vocab], unit stride over the vocabulary, rows that do not share storage.
+Tensor rows_of_logits(const Tensor& logits) {
+  if (logits.dim() < 1) throw py::value_error("logits must be [..., vocab]");
+  const int64_t v = logits.size(-1);
+  Tensor flat = logits.detach().reshape({v > 0 ? logits.numel() / v : 0, v});
+  if (flat.stride(1) != 1 || (flat.size(0) > 1 && flat.stride(0) < v)) flat = flat.contiguous();
+  return flat;
+}
+int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// What a saved-tensor hook has handed back is looked at again: a pointer into host memory would fault the GPU.
+void same_place(const char* what, const Tensor& like, std::initializer_list<const Tensor*> others) {
+  require_device(like, what);
+  for (const Tensor* t : others) {
+    if (!t->defined()) continue;
+    if (t->device() != like.device()) refuse(what, "operands live on different devices");
+    if (!t->is_contiguous()) refuse(what, "operands must be contiguous");
+  }
+}
+
+// A gradient that cannot be differentiated again says so, instead of being a constant.
+Tensor once(Tensor grad, const char* what) {
+  if (!at::GradMode::is_enabled()) return grad;
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": the gradient cannot be differentiated again", 1);
+  return (*error)({grad.detach().requires_grad_(true)})[0];
+}
+
+struct AlternativesNode : torch::autograd::Node {
+  SavedVariable rows, ids, labels, lse, entropy;
+  std::vector<int64_t> shape;
+  bool inplace = false, spent = false;
+  static constexpr const char* kWhat = "logits_tokens_backward";
+  std::string name() const override { return "AlternativesBackward"; }
+  void release_variables() override {
+    for (SavedVariable* s : {&rows, &ids, &labels, &lse, &entropy}) s->reset_data();
+  }
+  // gradients of entropy, log-probabilities of the tokens, log-probability of the label (with labels)
+  variable_list apply(variable_list&& g) override {
+    const Tensor x = rows.unpack(), at = ids.unpack(), lab = labels.unpack(), l = lse.unpack(),
+                 ent = entropy.unpack(shared_from_this());
+    const bool with_label = g.size() > 2 && g[2].defined();
+    if (!g[0].defined() && !g[1].defined() && !with_label) return {Tensor()};
+    if (spent) throw AxonError("the logits' storage holds the gradient of an earlier backward (inplace_backward)");
+    std::optional<at::NoGradGuard> no_grad(std::in_place);
+    const Tensor g_en = g[0].defined() ? f32(g[0]) : Tensor(), g_ids = g[1].defined() ? f32(g[1]) : Tensor(),
+                 g_lab = with_label ? f32(g[2]) : Tensor();
+    same_place(kWhat, x, {&at, &lab, &l, &ent, &g_en, &g_ids, &g_lab});
+    const int dtype = logits_dtype(kWhat, x);
+    const int64_t n = x.size(0), v = x.size(1), k = at.size(1);
+    if (x.stride(1) != 1 || (n > 1 && x.stride(0) < v)) refuse(kWhat, "logits must be [tokens, vocab] with unit stride over the vocabulary");
+    same_len(kWhat, "lse", n, l);
+    same_len(kWhat, "entropy", n, ent);
+    same_len(kWhat, "ids", n * k, at);
+    if (g_en.defined()) same_len(kWhat, "g_entropy", n, g_en);
+    if (g_ids.defined()) same_len(kWhat, "g_logprobs", n * k, g_ids);
+    if (g_lab.defined()) { same_len(kWhat, "g_label", n, g_lab); same_len(kWhat, "labels", n, lab); }
+    const c10::DeviceGuard device(x.device());
+    Tensor out = inplace ? x : at::empty({n, v}, x.options());
+    check(axon_logits_tokens_bwd(x.data_ptr(), dtype, row_stride(x), n, v, at.data_ptr(), is_i64(at), k, ptr(lab),
+                                 lab.defined() && is_i64(lab), (const float*)l.data_ptr(), (const float*)ent.data_ptr(),
+                                 (const float*)ptr(g_ids), (const float*)ptr(g_lab), (const float*)ptr(g_en), out.data_ptr(),
+                                 row_stride(out), ::stream()),
+          "axon_logits_tokens_bwd");
+    spent = inplace;
+    out = out.view(shape);
+    no_grad.reset();
+    return {once(std::move(out), kWhat)};
+  }
+};
+
+// The k best tokens of every position (ids_in none) or given ones: (label's log-probability or none, entropy, log-probabilities
+// [..., k], ids).
+std::tuple<OptTensor, Tensor, Tensor, Tensor> alternatives(const char* what, const Tensor& logits, int64_t k, const OptTensor& ids_in,
+                                                           const OptTensor& labels, bool inplace) {
+  const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
+  Tensor entropy, lp, label_lp, lse, ids, lab, rows;
+  std::vector<int64_t> batch(logits.sizes().begin(), logits.dim() ? logits.sizes().end() - 1 : logits.sizes().end());
+  {
+    const at::NoGradGuard no_grad;
+    rows = rows_of_logits(logits);
+    const int64_t n = rows.size(0), v = rows.size(1);
+    const int dtype = logits_dtype(what, rows);
+    if (labels) {
+      if (!is_index(*labels)) refuse(what, "labels must be int32 or int64");
+      if (labels->device() != logits.device()) refuse(what, "operands live on different devices");
+      same_len(what, "labels", n, *labels);
+      lab = labels->reshape({n}).contiguous();
+    }
+    if (ids_in) {
+      const Tensor& t = *ids_in;
+      if (!is_index(t)) refuse(what, std::string("token_ids must be int32 or int64, got ") + c10::toString(t.scalar_type()));
+      if (t.device() != logits.device()) refuse(what, "operands live on different devices");
+      if (t.dim() != logits.dim() || t.sizes().slice(0, t.dim() - 1) != logits.sizes().slice(0, logits.dim() - 1))
+        refuse(what, "token_ids " + shape_text(t) + " do not lie beside logits " + shape_text(logits));
+      k = t.size(-1);
+      if (k < 1 || k > AXON_MAX_TOKEN_IDS)
+        refuse(what, "between 1 and " + std::to_string(AXON_MAX_TOKEN_IDS) + " token ids per position, got " + std::to_string(k));
+      ids = t.reshape({n, k}).contiguous();
+    } else if (const int64_t most = std::min<int64_t>(AXON_MAX_TOP, v); k < 1 || k > most) {
+      refuse(what, "k must be between 1 and " + std::to_string(most) + " (at most " + std::to_string(AXON_MAX_TOP) +
+                       ", at most the vocabulary), got " + std::to_string(k));
+    }
+    require_device(rows, what);
+    const c10::DeviceGuard device(rows.device());
+    std::vector<int64_t> wide = batch;
+    wide.push_back(k);
+    entropy = at::empty(batch, opts(rows));
+    lp = at::empty(wide, opts(rows));
+    lse = at::empty({n}, opts(rows));
+    if (lab.defined()) label_lp = at::empty(batch, opts(rows));
+    const int64_t need = ids_in ? axon_logits_tokens_workspace_bytes(dtype, n, v) : axon_logits_top_workspace_bytes(dtype, n, v);
+    const Tensor ws = need > 0 ? at::empty({need / 4}, opts(rows)) : Tensor();
+    float *const ent_p = entropy.data_ptr<float>(), *const lse_p = lse.data_ptr<float>(), *const lp_p = lp.data_ptr<float>();
+    if (ids_in) {
+      check(axon_logits_tokens_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, ids.data_ptr(), is_i64(ids), k, lp_p, ent_p,
+                                   lse_p, (float*)ptr(ws), std::max<int64_t>(need, 0), wants_grad, stream()),
+            "axon_logits_tokens_fwd");
+    } else {
+      ids = at::empty(wide, opts(rows, at::kLong));
+      check(axon_logits_top_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, k, ptr(lab), lab.defined() && is_i64(lab),
+                                (float*)ptr(label_lp), ent_p, lse_p, lp_p, ids.data_ptr<int64_t>(), (float*)ptr(ws),
+                                std::max<int64_t>(need, 0), wants_grad, stream()),
+            "axon_logits_top_fwd");
+    }
+  }
+  if (wants_grad) {
+    std::shared_ptr<AlternativesNode> node(new AlternativesNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->shape = logits.sizes().vec();
+    // writing the gradient over the logits is only possible in the caller's own storage
+    node->inplace = inplace && rows.data_ptr() == logits.data_ptr();
+    torch::autograd::set_history(entropy, node);
+    torch::autograd::set_history(lp, node);
+    if (label_lp.defined()) torch::autograd::set_history(label_lp, node);
+    node->rows = SavedVariable(rows, false);
+    node->ids = SavedVariable(ids.reshape({rows.size(0), k}), false);
+    node->labels = SavedVariable(lab, false);
+    node->lse = SavedVariable(lse, false);
+    node->entropy = SavedVariable(entropy, true);
+  }
+  return {label_lp.defined() ? OptTensor(label_lp) : OptTensor(), entropy, lp, ids};
+}
+
+// The layers' router logits as the entry points take them.
+struct RouterRows {
+  std::vector<const void*> ptrs;
+  int64_t ld = 0, n = 0, experts = 0;
+  int dtype = 0;
+};
+// Rows of all layers with one row stride; a layer that lies otherwise is copied.
+RouterRows router_rows(const char* what, variable_list& rows) {
+  RouterRows r;
+  const Tensor& first = rows[0];
+  r.n = first.size(0);
+  r.experts = first.size(1);
+  r.dtype = logits_dtype(what, first);
+  r.ld = r.n > 1 ? first.stride(0) : r.experts;
+  bool same = r.ld >= r.experts;
+  for (const Tensor& t : rows) {
+    if (t.dim() != 2 || t.size(0) != r.n || t.size(1) != r.experts || t.scalar_type() != first.scalar_type() || t.device() != first.device())
+      refuse(what, "the layers' logits must agree in shape, type and device");
+    same = same && t.stride(1) == 1 && (r.n <= 1 || t.stride(0) == r.ld);
+  }
+  if (!same) {
+    for (Tensor& t : rows) t = t.contiguous();
+    r.ld = r.experts;
+  }
+  r.ptrs.reserve(rows.size());
+  for (const Tensor& t : rows) r.ptrs.push_back(t.data_ptr());
+  return r;
+}
+
+struct RouterBalanceNode : torch::autograd::Node {
+  std::vector<SavedVariable> rows;
+  SavedVariable mask, cu, coef, scale;
+  std::vector<std::vector<int64_t>> shapes;  // of the inputs
+  bool stacked = false;
+  int mask_kind = 0, score = 0;
+  static constexpr const char* kWhat = "router_balance_loss";
+  std::string name() const override { return "RouterBalanceBackward"; }
+  void release_variables() override {
+    for (SavedVariable& s : rows) s.reset_data();
+    for (SavedVariable* s : {&mask, &cu, &coef, &scale}) s->reset_data();
+  }
+  variable_list apply(variable_list&& g) override {
+    variable_list grads(shapes.size());
+    variable_list x;
+    x.reserve(rows.size());
+    for (SavedVariable& s : rows) x.push_back(s.unpack());
+    const Tensor m = mask.unpack(), offsets = cu.unpack(), c = coef.unpack(), sc = scale.unpack();
+    if (!g[0].defined()) return grads;
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor up = f32(g[0]);
+      same_place(kWhat, x[0], {&m, &offsets, &c, &sc, &up});
+      const RouterRows r = router_rows(kWhat, x);
+      const int64_t layers = (int64_t)x.size(), seqs = offsets.defined() ? offsets.numel() - 1 : 1;
+      same_len(kWhat, "coefficients", seqs * layers * r.experts, c);
+      same_len(kWhat, "upstream gradient", 1, up);
+      same_len(kWhat, "scale", 1, sc);
+      for (const std::vector<int64_t>& shape : shapes)
+        if (c10::multiply_integers(shape) != r.n * r.experts * (stacked ? layers : 1)) refuse(kWhat, "the saved logits have another size");
+      if (m.defined()) same_len(kWhat, "token_mask", r.n, m);
+      const c10::DeviceGuard device(x[0].device());
+      std::vector<void*> out(layers, nullptr);
+      for (size_t i = 0; i < shapes.size(); ++i) {
+        if (!task_should_compute_output(i)) continue;
+        grads[i] = at::empty(shapes[i], x[0].options());
+        char* const p = static_cast<char*>(grads[i].data_ptr());
+        if (!stacked) out[i] = p;
+        else for (int64_t l = 0; l < layers; ++l) out[l] = p + l * r.n * r.experts * (int64_t)x[0].element_size();
+      }
+      check(axon_router_balance_bwd(r.ptrs.data(), r.dtype, r.ld, layers, r.n, r.experts, ptr(m), mask_kind,
+                                    (const int32_t*)ptr(offsets), seqs, score, (const float*)ptr(c), (const float*)ptr(sc),
+                                    (const float*)ptr(up), out.data(), ::stream()),
+            "axon_router_balance_bwd");
+    }
+    if (at::GradMode::is_enabled())
+      for (Tensor& t : grads)
+        if (t.defined()) t = once(t, kWhat);
+    return grads;
+  }
+};
+
+// (loss, counts [layers, experts]); `logits`: the layers' [..., experts] or, stacked, one [layers, tokens, experts]; ids: one
+// [..., k] per layer, or none.
+std::tuple<Tensor, Tensor> router_balance(const variable_list& logits, bool stacked, int64_t k, const OptTensor& token_mask,
+                                          const OptTensor& cu_seqlens, const std::optional<variable_list>& expert_ids, int score) {
+  const char* const what = RouterBalanceNode::kWhat;
+  bool wants_grad = false;
+  for (const Tensor& t : logits) wants_grad = wants_grad || t.requires_grad();
+  wants_grad = wants_grad && at::GradMode::is_enabled();
+  variable_list rows, ids;
+  Tensor mask, cu, loss, scale, coef, counts;
+  int kind = 0;
+  {
+    const at::NoGradGuard no_grad;
+    if (stacked) {
+      rows = logits[0].detach().unbind(0);
+    } else {
+      rows.reserve(logits.size());
+      for (const Tensor& t : logits) {
+        Tensor d = t.detach();
+        rows.push_back(d.dim() == 2 ? d : d.reshape({d.numel() / d.size(-1), d.size(-1)}));
+      }
+    }
+    const Tensor first = rows[0];
+    const int64_t n = first.size(0), e = first.size(1), layers = (int64_t)rows.size();
+    if (e > AXON_MAX_EXPERTS) refuse(what, "between 1 and " + std::to_string(AXON_MAX_EXPERTS) + " experts, got " + std::to_string(e));
+    const RouterRows r = router_rows(what, rows);
+    if (token_mask) {
+      same_len(what, "token_mask", n, *token_mask);
+      if (token_mask->device() != first.device()) refuse(what, "operands live on different devices");
+      std::tie(mask, kind) = mask_arg(*token_mask);
+    }
+    if (cu_seqlens) {
+      if (cu_seqlens->dim() != 1 || cu_seqlens->numel() < 1) refuse(what, "cu_seqlens must be [sequences + 1]");
+      cu = cu_seqlens->detach().to(first.device(), at::kInt).contiguous();
+    }
+    std::vector<const void*> id_ptrs;
+    if (expert_ids) {
+      if ((int64_t)expert_ids->size() != layers)
+        refuse(what, "expert_ids for " + std::to_string(expert_ids->size()) + " layers, logits of " + std::to_string(layers));
+      for (const Tensor& t : *expert_ids) {
+        if (!is_index(t) || t.scalar_type() != expert_ids->front().scalar_type())
+          refuse(what, "expert_ids must be int32 or int64, the same in all layers");
+        if (t.device() != first.device()) refuse(what, "operands live on different devices");
+        if (t.dim() < 2 || t.size(-1) != k || t.numel() != n * k)
+          refuse(what, "expert_ids " + shape_text(t) + " are not " + std::to_string(k) + " per token of " + std::to_string(n));
+        ids.push_back(t.contiguous());
+        id_ptrs.push_back(ids.back().data_ptr());
+      }
+    }
+    require_device(first, what);
+    const c10::DeviceGuard device(first.device());
+    const int64_t seqs = cu.defined() ? cu.numel() - 1 : 1;
+    loss = at::empty({}, opts(first));
+    scale = at::empty({1}, opts(first));
+    coef = at::empty({seqs, layers, e}, opts(first));
+    counts = at::empty({layers, e}, opts(first, at::kLong));
+    const int64_t bytes = axon_router_balance_workspace_bytes(n, seqs, layers, e);
+    const Tensor ws = at::empty({bytes}, opts(first, at::kByte));
+    check(axon_router_balance_fwd(r.ptrs.data(), r.dtype, r.ld, layers, n, e, k, expert_ids ? id_ptrs.data() : nullptr,
+                                  expert_ids ? is_i64(ids[0]) : 0, ptr(mask), kind, (const int32_t*)ptr(cu), seqs, score,
+                                  loss.data_ptr<float>(), coef.data_ptr<float>(), scale.data_ptr<float>(),
+                                  counts.data_ptr<int64_t>(), ws.data_ptr(), bytes, stream()),
+          "axon_router_balance_fwd");
+  }
+  if (wants_grad) {
+    std::shared_ptr<RouterBalanceNode> node(new RouterBalanceNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    torch::autograd::set_history(loss, node);
+    node->rows.reserve(rows.size());
+    for (const Tensor& t : rows) node->rows.emplace_back(t, false);
+    node->mask = SavedVariable(mask, false);
+    node->cu = SavedVariable(cu, false);
+    node->coef = SavedVariable(coef, false);
+    node->scale = SavedVariable(scale, false);
+    for (const Tensor& t : logits) node->shapes.push_back(t.sizes().vec());
+    node->stacked = stacked;
+    node->mask_kind = kind;
+    node->score = score;
+  }
+  return {loss, counts};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -437,4 +771,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scale_f32", &scale_f32, unlocked);
   m.def("finished_loss", [](const Tensor& x, const Tensor& acc, const Tensor& grad, double factor,
                             int64_t slot) { return FinishedLoss::apply(x, acc, grad, factor, slot); }, unlocked);
+  m.def("top_logprobs", [](const Tensor& logits, int64_t k, const OptTensor& labels, bool inplace) {
+    return alternatives("top_logprobs_from_logits", logits, k, OptTensor(), labels, inplace);
+  }, unlocked);
+  m.def("token_logprobs", [](const Tensor& logits, const Tensor& token_ids, bool inplace) {
+    return alternatives("token_logprobs_from_logits", logits, 0, token_ids, OptTensor(), inplace);
+  }, unlocked);
+  m.def("router_balance", &router_balance, unlocked);
 }

@@ -14,63 +14,11 @@ from __future__ import annotations
 
 import torch
 
-from axon_amd import _ops
+from axon_amd import _lib
 
 __all__ = ["router_balance_loss"]
 
-
-class _RouterBalance(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, top_k, token_mask, cu_seqlens, expert_ids, score_fn, stacked, *logits):
-        layers = list(logits[0].unbind(0)) if stacked else [t.reshape(-1, t.shape[-1]) for t in logits]
-        batch = _ops.router_batch(layers, token_mask, cu_seqlens, score_fn)
-        loss, counts, coef, scale = _ops.router_balance(batch, top_k, expert_ids)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(counts)
-        ctx.layout = batch.ld, batch.mask_kind, batch.score, len(layers)
-        ctx.shapes, ctx.stacked = [t.shape for t in logits], stacked
-        ctx.save_for_backward(*batch.logits, batch.mask, batch.cu, coef, scale)
-        return loss, counts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_loss, _g_counts):
-        wanted = ctx.needs_input_grad[6:]
-        if g_loss is None or not any(wanted):
-            return (None,) * (6 + len(wanted))
-        ld, kind, score, n_layers = ctx.layout
-        saved = ctx.saved_tensors
-        rows, (mask, cu, coef, scale) = list(saved[:n_layers]), saved[n_layers:]
-        batch = _ops.RouterBatch(rows, ld, mask, kind, cu, score)
-        new = lambda shape: torch.empty(shape, device=rows[0].device, dtype=rows[0].dtype)  # noqa: E731
-        if ctx.stacked:
-            grads = [new(ctx.shapes[0])]
-            parts = list(grads[0].unbind(0))
-        else:
-            grads = [new(shape) if want else None for shape, want in zip(ctx.shapes, wanted)]
-            parts = grads
-        _ops.router_balance_backward(batch, coef, scale, g_loss, parts)
-        return (None,) * 6 + tuple(grads)
-
-
-def _ids_per_layer(expert_ids, layers, rows, top_k, device):
-    what = "router_balance_loss"
-    if isinstance(expert_ids, torch.Tensor):
-        ids = list(expert_ids.unbind(0)) if expert_ids.dim() == 3 else [expert_ids]
-    else:
-        ids = list(expert_ids)
-    if len(ids) != layers:
-        raise ValueError(f"{what}: expert_ids for {len(ids)} layers, logits of {layers}")
-    out = []
-    for t in ids:
-        if t.dtype not in (torch.int32, torch.int64) or t.dtype != ids[0].dtype:
-            raise ValueError(f"{what}: expert_ids must be int32 or int64, the same in all layers")
-        if t.device != device:
-            raise ValueError(f"{what}: operands live on different devices")
-        if t.dim() < 2 or int(t.shape[-1]) != top_k or int(t.numel()) != rows * top_k:
-            raise ValueError(f"{what}: expert_ids {tuple(t.shape)} are not {top_k} per token of {rows}")
-        out.append(t.reshape(rows, top_k).contiguous())
-    return out
+_SCORES = {"softmax": 0, "sigmoid": 1}
 
 
 def router_balance_loss(router_logits, top_k: int, *, token_mask=None, cu_seqlens=None, expert_ids=None,
@@ -101,11 +49,12 @@ def router_balance_loss(router_logits, top_k: int, *, token_mask=None, cu_seqlen
         raise ValueError(f"{what}: no layers")
     if any(t.dim() < 2 or t.shape[-1] < 1 for t in tensors):
         raise ValueError(f"{what}: every layer's logits must be [..., experts]")
-    layers, experts = (int(router_logits.shape[0]) if stacked else len(tensors)), int(tensors[0].shape[-1])
+    experts = int(tensors[0].shape[-1])
     if not 1 <= top_k <= experts:
         raise ValueError(f"{what}: top_k must be between 1 and the {experts} experts, got {top_k}")
-    rows = int(tensors[0].numel()) // experts // (layers if stacked else 1)
-    if expert_ids is not None:
-        expert_ids = _ids_per_layer(expert_ids, layers, rows, top_k, tensors[0].device)
-    loss, counts = _RouterBalance.apply(top_k, token_mask, cu_seqlens, expert_ids, score_fn, stacked, *tensors)
+    if score_fn not in _SCORES:
+        raise ValueError(f"{what}: score_fn must be one of {sorted(_SCORES)}, got {score_fn!r}")
+    if isinstance(expert_ids, torch.Tensor):
+        expert_ids = list(expert_ids.unbind(0)) if expert_ids.dim() == 3 else [expert_ids]
+    loss, counts = _lib.native().router_balance(tensors, stacked, top_k, token_mask, cu_seqlens, expert_ids, _SCORES[score_fn])
     return loss, counts[0] if single else counts

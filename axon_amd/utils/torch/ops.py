@@ -20,7 +20,7 @@ from typing import NamedTuple
 
 import torch
 
-from axon_amd import _ops
+from axon_amd import _lib, _ops
 
 __all__ = ["logprobs_from_logits", "entropy_from_logits", "entropy_from_logits_with_chunking",
            "logprobs_and_entropy_from_logits", "TopLogprobs", "top_logprobs_from_logits", "token_logprobs_from_logits"]
@@ -90,66 +90,22 @@ class TopLogprobs(NamedTuple):
     top_ids: torch.Tensor
 
 
-def _distinct_rows(logits):
-    """``[rows, vocab]`` with rows that do not share storage."""
-    if logits.dim() < 1:
-        raise ValueError("logits must be [..., vocab]")
-    flat = _rows(logits)
-    return flat.contiguous() if flat.shape[0] > 1 and flat.stride(0) < flat.shape[1] else flat
-
-
-class _Alternatives(torch.autograd.Function):
-    """The k largest logits of every row (``ids`` None) or given ones, their log-probabilities and what goes with them."""
-
-    @staticmethod
-    def forward(ctx, logits, k, ids, labels, inplace_backward):
-        flat = _distinct_rows(logits)
-        batch = logits.shape[:-1]
-        ctx.set_materialize_grads(False)
-        lab = labels.reshape(-1).contiguous() if labels is not None else None
-        if ids is None:
-            logprob, entropy, lse, top_logprobs, ids = _ops.logits_top(flat, k, lab, ctx.needs_input_grad[0])
-            top_ids = ids.view(*batch, k)
-            ctx.mark_non_differentiable(top_ids)
-        else:
-            ids = ids.reshape(flat.shape[0], ids.shape[-1])
-            top_logprobs, entropy, lse = _ops.logits_tokens(flat, ids, ctx.needs_input_grad[0])
-            logprob = top_ids = None
-        ctx.save_for_backward(flat, ids, lab, lse, entropy)
-        ctx.shape, ctx.spent = logits.shape, False
-        # writing the gradient over the logits is only possible when `flat` is the caller's storage
-        ctx.inplace = bool(inplace_backward) and flat.data_ptr() == logits.data_ptr()
-        return (logprob.view(batch) if logprob is not None else None, entropy.view(batch),
-                top_logprobs.view(*batch, top_logprobs.shape[-1]), top_ids)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_top, _g_ids):
-        if g_logprob is None and g_entropy is None and g_top is None:
-            return (None,) * 5
-        if ctx.spent:
-            raise RuntimeError("the logits' storage holds the gradient of an earlier backward (inplace_backward)")
-        flat, ids, lab, lse, entropy = ctx.saved_tensors
-        ctx.spent = ctx.inplace
-        grad = _ops.logits_tokens_backward(flat, ids, lab, lse, entropy, g_top, g_logprob, g_entropy, inplace=ctx.inplace)
-        return grad.view(ctx.shape), None, None, None, None
-
-
 def top_logprobs_from_logits(logits: torch.Tensor, k: int, labels: torch.Tensor | None = None,
                              inplace_backward: bool = False) -> TopLogprobs:
     """The ``k`` best tokens (at most 128) of every position of ``logits`` ``[..., vocab]`` (fp32 or bf16, already divided
     by the temperature): see ``TopLogprobs``.  Equal logits are ordered by ascending id.  ``labels`` ``[...]``: also the
     log-probability of these (0 for a label outside the vocabulary).  Differentiable with respect to the logits; the
     ids are constants.  A position whose logits hold a NaN, or nothing but -inf, has NaN log-probabilities."""
-    return TopLogprobs(*_Alternatives.apply(logits, k, None, labels, inplace_backward))
+    if isinstance(k, bool) or not isinstance(k, int):
+        raise TypeError(f"top_logprobs_from_logits: k must be an int, got {type(k).__name__}")
+    return TopLogprobs(*_lib.native().top_logprobs(logits, min(k, 1 << 40), labels, bool(inplace_backward)))
 
 
 def token_logprobs_from_logits(logits: torch.Tensor, token_ids: torch.Tensor, inplace_backward: bool = False):
     """``(logprobs [..., k], entropy [...])``: the log-probabilities of ``k`` given tokens per position (at most 512, int32
     or int64 ``[..., k]``; an id outside the vocabulary is a filler: its log-probability is 0 and its gradient goes
     nowhere) and the entropy, fp32, from one read of ``logits`` ``[..., vocab]``.  Differentiable with respect to the
-    logits; ids may occur more than once in a position."""
-    if token_ids.dim() != logits.dim() or token_ids.shape[:-1] != logits.shape[:-1]:
-        raise ValueError(f"token_ids {tuple(token_ids.shape)} do not lie beside logits {tuple(logits.shape)}")
-    _, entropy, logprobs, _ = _Alternatives.apply(logits, 0, token_ids, None, inplace_backward)
+    logits; ids may occur more than once in a position.  With ``inplace_backward`` (here and above) the backward writes
+    d loss / d logits over the logits' storage, and can run once."""
+    _, entropy, logprobs, _ = _lib.native().token_logprobs(logits, token_ids, bool(inplace_backward))
     return logprobs, entropy

@@ -691,6 +691,7 @@ int axon_logits_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_
  *        Ids outside the vocabulary are left out, equal ids of a row add up.  In the logits' dtype; dlogits may be the
  *        logits' own storage.
  *   Workspace: 4-byte aligned, its contents do not matter.  bwd_follows: as axon_logits_fwd_train. */
+enum { AXON_MAX_TOP = 128, AXON_MAX_TOKEN_IDS = 512 };
 int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t vocab);
 int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, int64_t k,
                         const void* labels, int labels_are_i64, float* logprob, float* entropy, float* lse,
@@ -717,6 +718,7 @@ int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld, int64_t n,
  *   loss [1], scale [1], coef [n_seqs][layers][experts] (what the backward reads), counts int64 [layers][experts].
  *   Tokens of no sequence count nowhere and get a zero gradient.  1 <= k <= experts <= 1024.  Workspace 8-byte aligned.
  *   g_loss: DEVICE scalar, the loss's upstream gradient. */
+enum { AXON_MAX_EXPERTS = 1024 };
 int64_t axon_router_balance_workspace_bytes(int64_t n_tokens, int64_t n_seqs, int64_t layers, int64_t experts);
 int axon_router_balance_fwd(const void* const* logits, int dtype, int64_t ld, int64_t layers, int64_t n_tokens,
                             int64_t experts, int64_t k, const void* const* ids, int ids_are_i64, const void* mask,

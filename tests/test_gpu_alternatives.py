@@ -5,7 +5,6 @@ import math
 import pytest
 import torch
 
-from axon_amd import _ops
 from axon_amd.utils.torch.ops import (logprobs_and_entropy_from_logits, token_logprobs_from_logits,
                                       top_logprobs_from_logits)
 
@@ -311,10 +310,12 @@ def test_captured_and_replayed():
     g_top, g_en = torch.randn(n, k, generator=gen(1), device="cuda"), torch.randn(n, generator=gen(2), device="cuda")
 
     def step():
-        _, ent, lse, lp, ids = _ops.logits_top(z, k)
-        return lp, ent, ids, _ops.logits_tokens_backward(z, ids, None, lse, ent, g_top, None, g_en)
+        r = top_logprobs_from_logits(z, k)
+        grad, = torch.autograd.grad([r.top_logprobs, r.entropy], z, [g_top, g_en])
+        return r.top_logprobs.detach(), r.entropy.detach(), r.top_ids, grad
 
     z.copy_(logits_of("random", n, v, torch.bfloat16, 1))
+    z.requires_grad_(True)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -324,7 +325,8 @@ def test_captured_and_replayed():
     with torch.cuda.graph(graph):
         held = step()
     for seed in (2, 3, 4):
-        z.copy_(logits_of("few_values" if seed == 3 else "random", n, v, torch.bfloat16, seed))
+        with torch.no_grad():
+            z.copy_(logits_of("few_values" if seed == 3 else "random", n, v, torch.bfloat16, seed))
         graph.replay()
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
@@ -340,3 +342,43 @@ def test_on_another_stream():
         got = top_logprobs_from_logits(z, 10)
     side.synchronize()
     assert torch.equal(got.top_ids, want.top_ids) and torch.equal(got.top_logprobs, want.top_logprobs)
+
+
+def test_saved_tensors_from_a_hook_are_looked_at_again():
+    """A hook that hands back tensors in host memory, or others than were saved, refuses the backward: nothing is launched."""
+    z = logits_of("random", 3, 300, torch.float32, 2)
+
+    def backward_with(unpack):
+        x = z.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            r = top_logprobs_from_logits(x, 3, torch.zeros(3, dtype=torch.int64, device="cuda"))
+        return torch.autograd.grad(r.top_logprobs.sum() + r.logprobs.sum(), x)[0]
+
+    want = backward_with(lambda t: t)
+    assert torch.equal(backward_with(lambda t: t.clone()), want)
+    for unpack in (lambda t: t.cpu(), lambda t: t.cpu() if t.dim() == 1 else t, lambda t: t.cpu() if t.dtype == torch.int64 else t,
+                   lambda t: t[:2] if t.dim() == 2 else t, lambda t: t[:1] if t.dim() == 1 else t):
+        with pytest.raises(RuntimeError):
+            backward_with(unpack)
+
+
+def test_a_gradient_is_not_differentiated_again():
+    x = logits_of("random", 3, 300, torch.float32, 2).requires_grad_(True)
+    lp, _ = token_logprobs_from_logits(x, torch.zeros(3, 1, dtype=torch.int64, device="cuda"))
+    g, = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):  # a penalty on the gradient is no constant
+        (lp.sum() + g.square().sum()).backward()
+    with pytest.raises(RuntimeError, match="second time|freed"):
+        lp2, _ = token_logprobs_from_logits(x, torch.zeros(3, 1, dtype=torch.int64, device="cuda"))
+        torch.autograd.grad(lp2.sum(), x)
+        torch.autograd.grad(lp2.sum(), x)
+
+
+def test_a_logit_changed_before_the_backward_is_noticed():
+    x = logits_of("random", 3, 300, torch.float32, 2).requires_grad_(True)
+    y = x * 1
+    lp, _ = token_logprobs_from_logits(y, torch.zeros(3, 1, dtype=torch.int64, device="cuda"))
+    with torch.no_grad():
+        y.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(lp.sum(), x)
