@@ -11,6 +11,7 @@
 // sequence in a fixed order, so that results repeat bit for bit.
 #include "common.h"
 #include "select.h"
+#include <algorithm>
 
 namespace axon {
 
@@ -26,10 +27,11 @@ struct BalanceParams {
   int n_tokens, experts, k, chunk, n_chunks, layers, first_layer;  // layers: of the whole call
   const void* mask;        // may be null
   const int32_t* cu;       // null: one sequence of all tokens
-  int n_seqs, ids_i64, quads;  // quads: rows can be read four elements at a time
+  int n_seqs, ids_i64, quads;  // quads: rows can be read four elements at a time (1), or sixteen bytes (2)
   float* part_p;           // [slots][layers][experts]
   int* part_c;             // the same
   int* part_t;             // [slots]
+  int* ticket;                 // zeroed by the first kernel
   unsigned long long* counts;  // [layers][experts]
   const float* coef;       // [n_seqs][layers][experts]
   const float* scale;      // what the mean over sequences and layers multiplies by
@@ -68,16 +70,69 @@ template <> struct RouterRow<__bf16> {
   static __device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
 };
 
-// Reductions over the G lanes of a row, the result in each of them.
+// Reductions over the G lanes of a row, the result in each of them: DPP steps inside sixteen lanes, register swaps beyond (a
+// shuffle would take a trip through the LDS crossbar with a wait behind it).  All 64 lanes have to be active.
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp(T v) {
+  const int i = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, i, CTRL, 0xf, 0xf, true));  // every lane has a source
+}
+// The compiler takes the two results of a swap for one value where the builtin is used; the s_nop covers the wait states
+// behind the instruction that has written the operands.
+template <class T, class Op>
+__device__ __forceinline__ T over_rows16(T v, Op op) {
+  T w = v;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+  return op(v, w);
+}
+template <class T, class Op>
+__device__ __forceinline__ T over_rows32(T v, Op op) {
+  T w = v;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+  return op(v, w);
+}
 template <int G, class T, class Op>
 __device__ __forceinline__ T row_reduce(T v, Op op) {
-#pragma unroll
-  for (int off = 1; off < G; off <<= 1) v = op(v, __shfl_xor(v, off, kWave));
+  if (G > 1) v = op(v, dpp<0xb1>(v));    // lane ^ 1
+  if (G > 2) v = op(v, dpp<0x4e>(v));    // lane ^ 2
+  if (G > 4) v = op(v, dpp<0x141>(v));   // the mirror lane of eight: any of the other four
+  if (G > 8) v = op(v, dpp<0x140>(v));   // the mirror lane of sixteen
+  if (G > 16) v = over_rows16(v, op);
+  if (G > 32) v = over_rows32(v, op);
+  return v;
+}
+// The other way: over the lanes of a wavefront that hold the same experts of different rows (the same lane modulo G).
+template <int G, class T, class Op>
+__device__ __forceinline__ T column_reduce(T v, Op op) {
+  if (G <= 1) v = op(v, dpp<0xb1>(v));
+  if (G <= 2) v = op(v, dpp<0x4e>(v));
+  if (G <= 4) v = op(v, dpp<0x124>(v));  // turned by four inside sixteen lanes
+  if (G <= 8) v = op(v, dpp<0x128>(v));  // by eight
+  if (G <= 16) v = over_rows16(v, op);
+  if (G <= 32) v = over_rows32(v, op);
   return v;
 }
 
+struct Add { template <class T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; } };
+struct MaxF { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct MaxU { __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); } };
+
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* row, int e0, int experts, bool quads, float (&x)[V]) {
+__device__ __forceinline__ void load_row(const T* row, int e0, int experts, int quads, float (&x)[V]) {
+  if (sizeof(T) == 2 && quads == 2) {
+#pragma unroll
+    for (int j = 0; j < V; j += 8) {
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      u32x4 w = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};  // -inf
+      if (e0 + j < experts) w = *reinterpret_cast<const u32x4*>(row + e0 + j);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x[j + 2 * q] = __uint_as_float(w[q] << 16);
+        x[j + 2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < V; j += 4) {
     float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -93,30 +148,115 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int experts, bool
   }
 }
 
-// p of a row's logits and, for sigmoids, 1 - sigmoid (from the exponential where the sigmoid is close to 1, and would
-// cancel).  What lies beyond the experts (-inf) gets p = 0.
+// A row's scores are w * inv; for sigmoids also 1 - sigmoid (from the exponential where the sigmoid is close to 1, and would
+// cancel).  What lies beyond the experts (-inf) gets w = 0.
 template <int G, int V, int SCORE>
-__device__ __forceinline__ void scores(const float (&x)[V], float (&p)[V], float (&rest)[V]) {
+__device__ __forceinline__ float scores(const float (&x)[V], float (&w)[V], float (&rest)[V]) {
+  constexpr float kLog2e = 1.4426950408889634f;
   float sum = 0.f;
   if (SCORE == kSoftmax) {
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) m = fmaxf(m, x[j]);
-    m = row_reduce<G>(m, [](float a, float b) { return fmaxf(a, b); });
+    m = row_reduce<G>(m, MaxF());
+    const float ml = m * kLog2e;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += p[j] = __expf(x[j] - m);
+    for (int j = 0; j < V; ++j) sum += w[j] = __builtin_amdgcn_exp2f(fmaf(x[j], kLog2e, -ml));
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float ex = __expf(-x[j]);
-      sum += p[j] = __frcp_rn(1.f + ex);
-      rest[j] = x[j] > 0.f ? ex * p[j] : 1.f - p[j];
+      const float ex = __builtin_amdgcn_exp2f(x[j] * -kLog2e);
+      sum += w[j] = __builtin_amdgcn_rcpf(1.f + ex);
+      rest[j] = x[j] > 0.f ? ex * w[j] : 1.f - w[j];
     }
   }
-  sum = row_reduce<G>(sum, [](float a, float b) { return a + b; });
-  const float inv = 1.f / sum;
+  return __builtin_amdgcn_rcpf(row_reduce<G>(sum, Add()));
+}
+
+// Keys in descending order (Batcher's odd-even merge sort: 19 exchanges for eight).
+template <int V>
+__device__ __forceinline__ void sort_keys(uint32_t (&s)[V]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) p[j] *= inv;
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t a = s[i + j], b = s[i + j + k];
+            s[i + j] = max(a, b);
+            s[i + j + k] = min(a, b);
+          }
+}
+
+// Ordered keys of a lane's elements; 0 where there is no expert.  fp32: the value's 32 bits.  bf16: the value's 16 bits above
+// the index, so that no two keys of a row are equal (two values at a time: sign and magnitude to an integer in the order of
+// the values, -0 to that of 0).
+template <typename T, int V>
+__device__ __forceinline__ void make_keys(const float (&x)[V], int e0, int experts, uint32_t (&key)[V]) {
+  if (sizeof(T) == 2) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t low = 0xffff - e0;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(x[j + 1]), __float_as_uint(x[j]), 0x07060302u);
+      const s16x2 sign = __builtin_bit_cast(s16x2, w) >> 15, mag = __builtin_bit_cast(s16x2, w & 0x7fff7fffu);
+      const uint32_t u = __builtin_bit_cast(uint32_t, (s16x2)((mag ^ sign) - sign)) ^ 0x80008000u;
+      key[j] = e0 + j < experts ? (u << 16) | (low - j) : 0u;
+      key[j + 1] = e0 + j + 1 < experts ? (u & 0xffff0000u) | (low - j - 1) : 0u;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) key[j] = e0 + j < experts ? max(order_key(x[j]), 1u) : 0u;
+}
+
+// Adds 1 to cnt of the lane's elements that are among the row's k first by (value descending, index ascending), where `in`.
+// Every lane sorts its keys; k times the lane with the largest head gives it up.  bf16: the last head given up is the bound.
+// fp32: equal heads go to the first lane, and of a lane's equal keys the first ones count.
+template <typename T, int G, int V>
+__device__ __forceinline__ void count_choices(const float (&x)[V], int e0, int experts, int k, bool in, int lane, int (&cnt)[V]) {
+  constexpr bool kUnique = sizeof(T) == 2;
+  uint32_t key[V], s[V];
+  make_keys<T>(x, e0, experts, key);
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = key[j];
+  sort_keys(s);
+  uint32_t bound = 0;
+  int given = 0;
+  for (int i = 0; i < k; ++i) {
+    const uint32_t best = row_reduce<G>(s[0], MaxU());
+    bool mine = s[0] == best;
+    if (kUnique) {
+      bound = best;
+    } else {
+      const uint64_t have = __builtin_amdgcn_ballot_w64(mine) >> (lane & ~(G - 1));
+      mine = mine && (have & ((uint64_t(1) << (lane & (G - 1))) - 1)) == 0;
+      bound = mine ? best : bound;
+      given += mine;
+    }
+    const uint32_t m = mine ? ~0u : 0u;  // as bits: selects between neighbours become selects by index
+#pragma unroll
+    for (int j = 0; j + 1 < V; ++j) s[j] = (s[j + 1] & m) | (s[j] & ~m);
+    s[V - 1] &= ~m;
+  }
+  if (kUnique) {
+    bound = in ? max(bound, 1u) : 0xffffffffu;  // no key is that large: its lower half is at most 0xffff, of a NaN
+#pragma unroll
+    for (int j = 0; j < V; ++j) cnt[j] += key[j] >= bound;
+    return;
+  }
+  if (!in || given == 0) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) given -= key[j] > bound;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const bool equal = key[j] == bound && given > 0;
+    given -= equal;
+    cnt[j] += equal || key[j] > bound;
+  }
 }
 
 template <int KIND>
@@ -150,6 +290,7 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, La
   const T* const x0 = static_cast<const T*>(logits.p[layer]);
   const void* const chosen = ids.p[layer];
   const int64_t out_layer = p.first_layer + layer;
+  if (out_layer == 0 && chunk == 0 && tid == 0) *p.ticket = 0;
   if (chunk == 0)
     for (int e = tid; e < p.experts; e += kBlock) p.counts[out_layer * p.experts + e] = 0;
   const int c0 = chunk * p.chunk, c1 = min(c0 + p.chunk, p.n_tokens);
@@ -158,39 +299,21 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, La
     if (tid == 0) s_tokens = 0;
     __syncthreads();
     float acc[V] = {};
+    int cnt[V] = {}, tokens = 0;
     for (int b = t0; b < t1; b += kRows) {  // the same number of times for all threads
       const int t = b + tid / G;
       const bool in = t < t1 && counts_in<MASK>(p.mask, t);
-      float x[V], pr[V], rest[V];
+      float x[V], w[V], rest[V];
       load_row<T, V>(x0 + (int64_t)(t < t1 ? t : t0) * p.ld, e0, p.experts, p.quads, x);
-      scores<G, V, SCORE>(x, pr, rest);
+      const float inv = scores<G, V, SCORE>(x, w, rest);
+      if (in) {
+        ++tokens;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += in ? pr[j] : 0.f;
-      if (in && lane_g == 0) atomicAdd(&s_tokens, 1);
-      if (chosen == nullptr) {
-        uint32_t key[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) key[j] = e0 + j < p.experts ? max(order_key(x[j]), 1u) : 0u;  // 0: taken
-        for (int i = 0; i < p.k; ++i) {
-          uint32_t m = key[0];
-#pragma unroll
-          for (int j = 1; j < V; ++j) m = max(m, key[j]);
-          const uint32_t best = row_reduce<G>(m, [](uint32_t a, uint32_t b2) { return max(a, b2); });
-          // equal logits go to the lowest expert: the first lane of the row that has one
-          const uint64_t have = __builtin_amdgcn_ballot_w64(m == best) >> (lane & ~(G - 1));
-          if (__builtin_ctzll(have) == lane_g) {
-            bool open = true;
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (open && key[j] == best) {
-                key[j] = 0;
-                open = false;
-                if (in) atomicAdd(&hist[e0 + j], 1);
-              }
-          }
-        }
+        for (int j = 0; j < V; ++j) acc[j] = fmaf(w[j], inv, acc[j]);
       }
+      if (chosen == nullptr) count_choices<T, G>(x, e0, p.experts, p.k, in, lane, cnt);
     }
+    if (lane_g == 0 && tokens > 0) atomicAdd(&s_tokens, tokens);
     if (chosen != nullptr) {
       for (int i = tid; i < (t1 - t0) * p.k; i += kBlock) {
         const int t = t0 + i / p.k;
@@ -202,9 +325,12 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, La
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-#pragma unroll
-      for (int off = G; off < kWave; off <<= 1) acc[j] += __shfl_xor(acc[j], off, kWave);
+      acc[j] = column_reduce<G>(acc[j], Add());
       if (lane < G) red[wave][e0 + j] = acc[j];
+      if (chosen == nullptr) {
+        cnt[j] = column_reduce<G>(cnt[j], Add());
+        if (lane < G && cnt[j]) atomicAdd(&hist[e0 + j], cnt[j]);
+      }
     }
     __syncthreads();
     const int64_t slot = chunk + seq;
@@ -219,54 +345,74 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, La
 }
 
 // Workgroup (sequence, layer): adds its partials, leaves E / (k T^2) c per expert for the backward, the loads and the
-// sequence's loss.
+// sequence's loss.  The workgroup that draws the last ticket adds the losses, in a fixed order, to the mean over the sequences
+// that have tokens and the layers.  Up to 256 experts the chunks are shared by groups of threads (one load at a time and
+// thread, and a launch for the mean: 48 x 8192 x 128 18 us).
 __global__ __launch_bounds__(kBlock) void balance_sum_kernel(BalanceParams p, float* __restrict__ coef, double* __restrict__ losses,
-                                                             int* __restrict__ tokens) {
-  __shared__ double red[kBlock / kWave];
-  const int seq = blockIdx.x % p.n_seqs, layer = blockIdx.x / p.n_seqs, tid = threadIdx.x;
+                                                             int* __restrict__ tokens, float* __restrict__ loss,
+                                                             float* __restrict__ scale) {
+  __shared__ double prob[kBlock];
+  __shared__ int cnt[kBlock];
+  __shared__ double red[2][kBlock / kWave];
+  __shared__ int s_last;
+  const int seq = blockIdx.x % p.n_seqs, layer = blockIdx.x / p.n_seqs, tid = threadIdx.x, lane = tid & (kWave - 1);
   const int a = p.cu ? max(p.cu[seq], 0) : 0, b = min(p.cu ? p.cu[seq + 1] : p.n_tokens, p.n_tokens);
   const int first = a / p.chunk, last = b > a ? (b - 1) / p.chunk : first - 1;
   int n = 0;
-  for (int c = first; c <= last; ++c) n += p.part_t[c + seq];
+  for (int c = first + lane; c <= last; c += kWave) n += p.part_t[c + seq];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
   const double w = n > 0 ? (double)p.experts / ((double)p.k * n * n) : 0.0;
+  const int width = p.experts >= kBlock ? kBlock : 1 << (32 - __builtin_clz(p.experts - 1 | 1));  // at least the experts
+  const int groups = kBlock / width, group = tid / width;
   double sum = 0.0;
-  for (int e = tid; e < p.experts; e += kBlock) {
-    double prob = 0.0;
-    int cnt = 0;
-    for (int c = first; c <= last; ++c) {
-      const int64_t at = ((int64_t)(c + seq) * p.layers + layer) * p.experts + e;
-      prob += p.part_p[at];
-      cnt += p.part_c[at];
+  for (int e0 = 0; e0 < p.experts; e0 += width) {
+    const int e = e0 + (tid & (width - 1));
+    double pr = 0.0;
+    int ct = 0;
+    if (e < p.experts) {
+#pragma unroll 4
+      for (int c = first + group; c <= last; c += groups) {
+        const int64_t at = ((int64_t)(c + seq) * p.layers + layer) * p.experts + e;
+        pr += p.part_p[at];
+        ct += p.part_c[at];
+      }
     }
-    const double wc = w * cnt;
-    coef[((int64_t)seq * p.layers + layer) * p.experts + e] = (float)wc;
-    if (cnt) atomicAdd(&p.counts[(int64_t)layer * p.experts + e], (unsigned long long)cnt);
-    sum += n > 0 ? wc * prob : 0.0;
+    prob[tid] = pr;
+    cnt[tid] = ct;
+    __syncthreads();
+    if (group == 0 && e < p.experts) {
+      for (int g = 1; g < groups; ++g) { pr += prob[g * width + tid]; ct += cnt[g * width + tid]; }
+      const double wc = w * ct;
+      coef[((int64_t)seq * p.layers + layer) * p.experts + e] = (float)wc;
+      if (ct) atomicAdd(&p.counts[(int64_t)layer * p.experts + e], (unsigned long long)ct);
+      sum += n > 0 ? wc * pr : 0.0;
+    }
+    __syncthreads();
   }
   sum = wave_sum_d(sum);
-  if ((tid & (kWave - 1)) == 0) red[tid / kWave] = sum;
+  if (lane == 0) red[0][tid / kWave] = sum;
   __syncthreads();
   if (tid == 0) {
-    losses[(int64_t)seq * p.layers + layer] = (red[0] + red[1]) + (red[2] + red[3]);
+    losses[(int64_t)seq * p.layers + layer] = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
     if (layer == 0) tokens[seq] = n;
+    __threadfence();
+    s_last = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   }
-}
-
-// One workgroup: the mean over the sequences that have tokens and the layers.
-__global__ __launch_bounds__(kBlock) void balance_mean_kernel(const double* __restrict__ losses, const int* __restrict__ tokens,
-                                                              int n_seqs, int layers, float* __restrict__ loss,
-                                                              float* __restrict__ scale) {
-  __shared__ double red[2][kBlock / kWave];
-  double sum = 0.0, with = 0.0;
-  for (int i = threadIdx.x; i < n_seqs * layers; i += kBlock) sum += losses[i];
-  for (int i = threadIdx.x; i < n_seqs; i += kBlock) with += tokens[i] > 0 ? 1.0 : 0.0;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  sum = 0.0;
+  double with = 0.0;
+  for (int i = tid; i < p.n_seqs * p.layers; i += kBlock) sum += losses[i];
+  for (int i = tid; i < p.n_seqs; i += kBlock) with += tokens[i] > 0 ? 1.0 : 0.0;
   sum = wave_sum_d(sum);
   with = wave_sum_d(with);
-  if ((threadIdx.x & (kWave - 1)) == 0) { red[0][threadIdx.x / kWave] = sum; red[1][threadIdx.x / kWave] = with; }
+  if (lane == 0) { red[0][tid / kWave] = sum; red[1][tid / kWave] = with; }
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < kBlock / kWave; ++w) { sum += red[0][w]; with += red[1][w]; }
-  const double s = with > 0.0 ? 1.0 / (with * layers) : 0.0;
+  if (tid != 0) return;
+  for (int v = 1; v < kBlock / kWave; ++v) { sum += red[0][v]; with += red[1][v]; }
+  const double s = with > 0.0 ? 1.0 / (with * p.layers) : 0.0;
   *loss = (float)(sum * s);
   *scale = (float)s;
 }
@@ -310,17 +456,18 @@ __global__ __launch_bounds__(kBlock) void balance_bwd_kernel(BalanceParams p, La
     for (int b = t0; b < t1; b += kRows) {
       const int t = b + tid / G;
       const bool in = t < t1 && counts_in<MASK>(p.mask, t);
-      float x[V], pr[V], rest[V], d[V], dot = 0.f;
+      float x[V], w[V], rest[V], d[V], dot = 0.f;
       load_row<T, V>(x0 + (int64_t)(t < t1 ? t : t0) * p.ld, e0, p.experts, p.quads, x);
-      scores<G, V, SCORE>(x, pr, rest);
+      const float inv = scores<G, V, SCORE>(x, w, rest);
 #pragma unroll
-      for (int j = 0; j < V; ++j) dot = fmaf(pr[j], wc[j], dot);
-      dot = row_reduce<G>(dot, [](float u, float v) { return u + v; });
+      for (int j = 0; j < V; ++j) dot = fmaf(w[j], wc[j], dot);
+      dot = row_reduce<G>(dot, Add()) * inv;
+      const float by = factor * inv;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float slope = pr[j];
+        float slope = w[j] * by;
         if (SCORE == kSigmoid) slope *= rest[j];
-        d[j] = in ? factor * slope * (wc[j] - dot) : 0.f;
+        d[j] = in ? slope * (wc[j] - dot) : 0.f;
       }
       if (t < t1) store(t, d);
     }
@@ -343,7 +490,7 @@ int chunk_of(int64_t n, int64_t layers) {
 
 struct BalanceWs {
   float* part_p;
-  int *part_c, *part_t, *tokens;
+  int *part_c, *part_t, *tokens, *ticket;
   double* losses;
   int64_t bytes;
 };
@@ -356,6 +503,7 @@ BalanceWs balance_ws(int64_t n, int64_t n_seqs, int64_t layers, int64_t experts,
   w.part_c = reinterpret_cast<int*>(p);     p += cells * 4;
   w.part_t = reinterpret_cast<int*>(p);     p += slots * 4;
   w.tokens = reinterpret_cast<int*>(p);     p += n_seqs * 4;
+  w.ticket = reinterpret_cast<int*>(p);     p += 4;
   w.bytes = p - static_cast<char*>(base);
   return w;
 }
@@ -376,11 +524,11 @@ int check_balance(const void* const* logits, int dtype, int64_t ld, int64_t laye
   return AXON_OK;
 }
 
-// rows of every layer can be read four elements at a time
-bool quads_ok(const void* const* ptrs, int64_t layers, int64_t ld, int64_t experts, int eb) {
+// how rows of every layer can be read: sixteen bytes at a time (2), four elements (1), one (0)
+int quads_ok(const void* const* ptrs, int64_t layers, int64_t ld, int64_t experts, int eb) {
   uintptr_t bits = (uintptr_t)(ld * eb) | (uintptr_t)(experts * eb);
   for (int64_t l = 0; l < layers; ++l) bits |= reinterpret_cast<uintptr_t>(ptrs[l]);  // a null is on every boundary
-  return bits % (4 * eb) == 0;
+  return bits % 16 == 0 ? 2 : bits % (4 * eb) == 0 ? 1 : 0;
 }
 
 template <typename T, int SCORE, int MASK, bool BWD>
@@ -452,7 +600,7 @@ extern "C" int axon_router_balance_fwd(const void* const* logits, int dtype, int
   p.chunk = chunk_of(n, layers);
   p.n_chunks = (int)((n + p.chunk - 1) / p.chunk);
   p.mask = mask;  p.cu = cu;  p.n_seqs = (int)n_seqs;  p.ids_i64 = ids_i64;
-  p.part_p = w.part_p;  p.part_c = w.part_c;  p.part_t = w.part_t;
+  p.part_p = w.part_p;  p.part_c = w.part_c;  p.part_t = w.part_t;  p.ticket = w.ticket;
   p.counts = reinterpret_cast<unsigned long long*>(counts);
   const int eb = dtype == AXON_LOGITS_F32 ? 4 : 2;
   for (int64_t l0 = 0; l0 < layers; l0 += kMaxLayers) {
@@ -464,9 +612,8 @@ extern "C" int axon_router_balance_fwd(const void* const* logits, int dtype, int
     rc = launch_typed<false>(dtype, score, mask_kind, p, x, c, nl, st);
     if (rc != AXON_OK) return rc;
   }
-  hipLaunchKernelGGL(balance_sum_kernel, dim3((unsigned)(n_seqs * layers)), dim3(kBlock), 0, st, p, coef, w.losses, w.tokens);
-  AXON_CHECK_LAUNCH();
-  hipLaunchKernelGGL(balance_mean_kernel, dim3(1), dim3(kBlock), 0, st, w.losses, w.tokens, (int)n_seqs, (int)layers, loss, scale);
+  hipLaunchKernelGGL(balance_sum_kernel, dim3((unsigned)(n_seqs * layers)), dim3(kBlock), 0, st, p, coef, w.losses, w.tokens, loss,
+                     scale);
   AXON_CHECK_LAUNCH();
   return AXON_OK;
 }
@@ -494,7 +641,7 @@ extern "C" int axon_router_balance_bwd(const void* const* logits, int dtype, int
     LayerPtrs x{}, d{};
     for (int l = 0; l < nl; ++l) { x.p[l] = logits[l0 + l]; d.p[l] = dlogits[l0 + l]; }
     p.first_layer = (int)l0;
-    p.quads = quads_ok(x.p, nl, ld, experts, eb) && quads_ok(d.p, nl, experts, experts, eb);
+    p.quads = std::min(quads_ok(x.p, nl, ld, experts, eb), quads_ok(d.p, nl, experts, experts, eb));
     rc = launch_typed<true>(dtype, score, mask_kind, p, x, d, nl, (hipStream_t)stream);
     if (rc != AXON_OK) return rc;
   }
