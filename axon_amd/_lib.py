@@ -63,13 +63,14 @@ SIGNATURES: dict[str, tuple] = {
                                        _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "axon_lmhead_scatter_rows": (_i32, [_ptr, _ptr, _i64, _i64, _ptr, _ptr]),
     "axon_lmhead_top_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "axon_lmhead_top_logits_bytes": (_i64, [_i64, _i64, _i64]),
     "axon_lmhead_top_fwd": (_i32, [_ptr, _ptr, _ptr, _i32, _i64, _i64, _i64, _f32, _f32, _i64, _ptr, _ptr, _ptr, _ptr,
-                                   _ptr, _ptr, _ptr, _i64, _ptr]),
+                                   _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
     "axon_lmhead_tokens_fwd": (_i32, [_ptr, _ptr, _ptr, _i32, _i64, _i64, _i64, _f32, _f32, _i64, _ptr, _ptr, _ptr,
-                                      _ptr, _ptr, _i64, _ptr]),
+                                      _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
     "axon_lmhead_tokens_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "axon_lmhead_tokens_bwd": (_i32, [_ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64,
-                                      _f32, _f32, _ptr, _ptr, _ptr, _i64, _ptr]),
+                                      _f32, _f32, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
     "axon_gemm_nt_bf16": (_i32, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr]),
     "axon_gemm_bf16": (_i32, [_ptr, _i64, _i32, _ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _i64, _ptr]),
     "axon_row_stats_workspace_bytes": (_i64, [_i64]),

@@ -1182,9 +1182,13 @@ def token_ids_arg(what, ids, rows, device):
     return ids.contiguous()
 
 
-# Bytes of fp32 logits that a call of the head with alternatives holds at most: longer batches are cut into blocks of
-# tokens (2.5 GB: 4096 tokens of the 151936 vocabulary; never fewer than 256).
+# Bytes of fp32 logits that a call of the head with several tokens per position holds at most (2.5 GB: 4096 tokens of the
+# 151936 vocabulary).  A forward with alternatives cuts longer batches into blocks of tokens, never fewer than 256; a forward
+# of which a gradient is wanted leaves its logits to the backward where those of the whole call fit, and memory has room for
+# as much again.  From a hidden size of 768 on, where the product that recomputes them costs more than writing and reading them;
+# the gradients are the same bit for bit.
 TOP_LOGITS_BYTES = 2560 << 20
+TOP_KEEP_LOGITS_MIN_HIDDEN = 768
 
 
 def _top_block(n, v):
@@ -1192,9 +1196,20 @@ def _top_block(n, v):
     return min(n, max(1, TOP_LOGITS_BYTES // per_tile) * 256)
 
 
-def lmhead_top(hidden, weight, k, labels=None, inv_temperature=1.0, softcap=0.0):
-    """``(logprobs | None, entropy, lse, entropy_b, top_logprobs [tokens, k], top_ids [tokens, k])``; see
-    axon_lmhead_top_fwd.  Block of tokens by block, so that the logits held do not grow with the batch."""
+def _logits_to_keep(n, h, v, dev):
+    """Bytes of the logits that a forward over all ``n`` tokens leaves to its backward, or 0."""
+    if n == 0 or h < TOP_KEEP_LOGITS_MIN_HIDDEN or h % 64 != 0:
+        return 0
+    need = int(_lib.load().axon_lmhead_top_logits_bytes(n, h, v))
+    if need > TOP_LOGITS_BYTES or (not torch.cuda.is_current_stream_capturing() and not _fits_twice(need, dev)):
+        return 0
+    return need
+
+
+def lmhead_top(hidden, weight, k, labels=None, inv_temperature=1.0, softcap=0.0, backward_follows=False):
+    """``(logprobs | None, entropy, lse, entropy_b, top_logprobs [tokens, k], top_ids [tokens, k], logits | None)``; see
+    axon_lmhead_top_fwd.  Block of tokens by block, so that the logits held do not grow with the batch; ``logits``: those of
+    all tokens, for ``lmhead_tokens_backward``."""
     what = "lmhead_top"
     n, h, v = _head_operands(what, hidden, weight, labels, None)
     _top_count(what, k, v)
@@ -1204,12 +1219,15 @@ def lmhead_top(hidden, weight, k, labels=None, inv_temperature=1.0, softcap=0.0)
     with on_device_of(hidden):
         block = _top_block(n, v)
         ws_bytes = lib.axon_lmhead_top_workspace_bytes(block, h, v)
+        logits_bytes = lib.axon_lmhead_top_logits_bytes(block, h, v)
         if ws_bytes < 0:
             raise _lib.AxonAmdError(f"axon_lmhead_top_fwd: unsupported shape tokens={n} hidden={h} vocab={v} (hidden % 32 != 0?)")
+        kept = backward_follows and block == n and _logits_to_keep(n, h, v, dev) > 0
         out = torch.empty(4, n, device=dev, dtype=torch.float32)
         top_logprobs = torch.empty(n, k, device=dev, dtype=torch.float32)
         top_ids = torch.empty(n, k, device=dev, dtype=torch.int64)
         ws = torch.empty(ws_bytes if n else 0, device=dev, dtype=torch.uint8)
+        logits = torch.empty(logits_bytes if n else 0, device=dev, dtype=torch.uint8)
         base = out.data_ptr()
         for a in range(0, n, max(block, 1)):
             lab = None if labels is None else labels.data_ptr() + a * labels.element_size()
@@ -1218,13 +1236,13 @@ def lmhead_top(hidden, weight, k, labels=None, inv_temperature=1.0, softcap=0.0)
                                           int(labels is not None and labels.dtype == torch.int64), min(block, n - a), h, v,
                                           float(inv_temperature), float(softcap), k, lp if lab else None, ent, lse, eb,
                                           top_logprobs.data_ptr() + a * k * 4, top_ids.data_ptr() + a * k * 8, ptr(ws),
-                                          ws_bytes, stream_ptr()), "axon_lmhead_top_fwd")
+                                          ws_bytes, ptr(logits), logits_bytes, stream_ptr()), "axon_lmhead_top_fwd")
     lp, ent, lse, eb = out.unbind(0)
-    return (lp if labels is not None else None), ent, lse, eb, top_logprobs, top_ids
+    return (lp if labels is not None else None), ent, lse, eb, top_logprobs, top_ids, logits if kept else None
 
 
-def lmhead_tokens(hidden, weight, token_ids, inv_temperature=1.0, softcap=0.0):
-    """``(logprobs [tokens, k], entropy, lse, entropy_b)`` of given tokens; see axon_lmhead_tokens_fwd."""
+def lmhead_tokens(hidden, weight, token_ids, inv_temperature=1.0, softcap=0.0, backward_follows=False):
+    """``(logprobs [tokens, k], entropy, lse, entropy_b, logits | None)`` of given tokens; see axon_lmhead_tokens_fwd."""
     what = "lmhead_tokens"
     n, h, v = _head_operands(what, hidden, weight, None, None)
     ids = token_ids_arg(what, token_ids, n, hidden.device)
@@ -1238,17 +1256,20 @@ def lmhead_tokens(hidden, weight, token_ids, inv_temperature=1.0, softcap=0.0):
         out = torch.empty(3, n, device=dev, dtype=torch.float32)
         logprobs = torch.empty(n, k, device=dev, dtype=torch.float32)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        keep = _logits_to_keep(n, h, v, dev) if backward_follows else 0
+        logits = torch.empty(keep, device=dev, dtype=torch.uint8) if keep else None
         check(lib.axon_lmhead_tokens_fwd(ptr(hidden), ptr(weight), ptr(ids), int(ids.dtype == torch.int64), n, h, v,
                                          float(inv_temperature), float(softcap), k, ptr(logprobs), ptr(out[0]),
-                                         ptr(out[1]), ptr(out[2]), ptr(ws), ws_bytes, stream_ptr()),
+                                         ptr(out[1]), ptr(out[2]), ptr(ws), ws_bytes, ptr(logits), keep, stream_ptr()),
               "axon_lmhead_tokens_fwd")
-    return logprobs, out[0], out[1], out[2]
+    return logprobs, out[0], out[1], out[2], logits
 
 
 def lmhead_tokens_backward(g_logprobs, g_entropy, hidden, weight, token_ids, logprobs, lse, entropy_b, inv_temperature=1.0,
-                           softcap=0.0):
+                           softcap=0.0, logits=None):
     """``(d_hidden, d_weight)`` in bf16 from the gradients of the log-probabilities of ``token_ids`` (one more per
-    position than the forward's limit: a label's) and of the entropy (or None); see axon_lmhead_tokens_bwd."""
+    position than the forward's limit: a label's) and of the entropy (or None); ``logits``: what the forward kept, or None.
+    See axon_lmhead_tokens_bwd."""
     what = "lmhead_tokens_backward"
     n, h, v = _head_operands(what, hidden, weight, None, None)
     k = int(token_ids.shape[1])
@@ -1256,11 +1277,16 @@ def lmhead_tokens_backward(g_logprobs, g_entropy, hidden, weight, token_ids, log
     _same_len(what, n * k, token_ids=token_ids, g_logprobs=g_logprobs, logprobs=logprobs)
     require_device(hidden, what)
     lib = _lib.load()
-    g_lp, lps = f32(g_logprobs), f32(logprobs)
+    g_lp, lps, lse, mean = f32(g_logprobs), f32(logprobs), f32(lse), f32(entropy_b)
     g_en = None if g_entropy is None else f32(g_entropy)
-    for t in (token_ids, g_lp, lps, g_en):
+    # the operands may come back from a saved-tensor hook: a pointer into host memory would fault the GPU
+    for t in (token_ids, g_lp, lps, lse, mean, g_en, logits):
         if t is not None and t.device != hidden.device:
             raise ValueError(f"{what}: operands live on different devices")
+    if token_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: token_ids must be int32 or int64")
+    if logits is not None and (logits.dtype != torch.uint8 or not logits.is_contiguous() or logits.data_ptr() % 16 != 0):
+        raise ValueError(f"{what}: logits must be the uint8 tensor that the forward returned")
     ids = token_ids.contiguous()
     with on_device_of(hidden):
         d_hidden, d_weight = torch.empty_like(hidden), torch.empty_like(weight)
@@ -1269,11 +1295,11 @@ def lmhead_tokens_backward(g_logprobs, g_entropy, hidden, weight, token_ids, log
             raise _lib.AxonAmdError(f"axon_lmhead_tokens_bwd: unsupported shape tokens={n} hidden={h} vocab={v}")
         ws = torch.empty(ws_bytes, device=hidden.device, dtype=torch.uint8)
         check(lib.axon_lmhead_tokens_bwd(ptr(g_lp), ptr(g_en), ptr(hidden), ptr(weight), ptr(ids),
-                                         int(ids.dtype == torch.int64), k, ptr(lps), ptr(lse), ptr(entropy_b), n, h, v,
+                                         int(ids.dtype == torch.int64), k, ptr(lps), ptr(lse), ptr(mean), n, h, v,
                                          float(inv_temperature), float(softcap), ptr(d_hidden), ptr(d_weight), ptr(ws),
-                                         ws_bytes, stream_ptr()), "axon_lmhead_tokens_bwd")
+                                         ws_bytes, ptr(logits), 0 if logits is None else int(logits.numel()), stream_ptr()),
+              "axon_lmhead_tokens_bwd")
     return d_hidden, d_weight
-
 
 def gemm_nt(a, b):
     """out[n][m] = sum_k a[m][k] * b[n][k]; bf16 in, fp32 out.  Test/benchmark helper."""

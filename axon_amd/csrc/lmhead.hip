@@ -1019,6 +1019,17 @@ __global__ __launch_bounds__(64) void lmhead_dlogit_logits_kernel(DlogitParams p
 // Several tokens per position: the largest of the kept logits, the logits of given tokens, their gradients
 // ----------------------------------------------------------------------------
 
+// Where a token's kept logits begin: its place in the first tile of its column of tiles.
+__device__ __forceinline__ const float4* kept_column(const float4* tiles, int n) {
+  const int tn = n / kTile, in = n % kTile;
+  return tiles + (int64_t)tn * 4 * kLogitsWaveVecs + (in / kWaveTile) * kLogitsWaveVecs +
+         (in % kWaveTile) / kBlk * kBlocks * 64 + in % kBlk;
+}
+// The four vocabulary rows from part * 128 + i * 16 + lq * 4 on; tile_step: vectors of a row of tiles.
+__device__ __forceinline__ int64_t kept_vec(int part, int i, int lq, int64_t tile_step) {
+  return (part >> 1) * tile_step + (part & 1) * 2 * kLogitsWaveVecs + i * 64 + lq * 16;
+}
+
 // A token's kept logits as select_top reads them: its segments are the parts of 128 vocabulary rows, an item is the four
 // rows that one lane of the tile had.
 struct HeadSource {
@@ -1032,7 +1043,7 @@ struct HeadSource {
   __device__ int limit() const { return vocab; }
   __device__ int load(const int* segs, int j, float (&v)[4]) const {
     const int part = segs[j / kItems], i = (j % kItems) >> 2, lq = j & 3;
-    const float4 x = column[(part >> 1) * tile_step + (part & 1) * 2 * kLogitsWaveVecs + i * 64 + lq * 16];
+    const float4 x = column[kept_vec(part, i, lq, tile_step)];
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
     return part * kWaveTile + i * kBlk + lq * 4;
   }
@@ -1068,10 +1079,8 @@ __global__ __launch_bounds__(kBlock) void lmhead_top_kernel(TopParams p) {
     for (int i = tid; i < p.parts; i += kBlock) staged[i] = p.pm[(int64_t)i * p.n_tokens + n];
     __syncthreads();
   }
-  const int tn = n / kTile, in = n % kTile;
   HeadSource src;
-  src.column = p.tiles + (int64_t)tn * 4 * kLogitsWaveVecs + (in / kWaveTile) * kLogitsWaveVecs +
-               (in % kWaveTile) / kBlk * kBlocks * 64 + in % kBlk;
+  src.column = kept_column(p.tiles, n);
   src.tile_step = (int64_t)p.tiles_n * 4 * kLogitsWaveVecs;
   src.parts = p.parts;
   src.vocab = p.vocab;
@@ -1134,6 +1143,25 @@ __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restr
     if (cap != 0.f) dot = cap * fast_tanh(dot / cap);
     if (lane == 0) a.logprobs[at] = ok ? fmaf(dot, inv_temp, -lse_n) : 0.f;
   }
+}
+
+// The same from kept logits: a thread per id.
+__global__ __launch_bounds__(256) void token_picks_kernel(const float4* __restrict__ tiles, int tiles_n, int64_t n_ids, int vocab,
+                                                          TokenArgs a, float inv_temp, float cap, const float* __restrict__ lse) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n_ids) return;
+  const int n = (int)(at / a.k);
+  const int64_t id = a.id(at);
+  float lp = 0.f;
+  if (id >= 0 && id < vocab) {
+    const int v = (int)id;
+    const float4* const four = kept_column(tiles, n) + kept_vec(v / kWaveTile, v % kWaveTile / kBlk, v % kBlk / 4,
+                                                                 (int64_t)tiles_n * 4 * kLogitsWaveVecs);
+    float z = reinterpret_cast<const float*>(four)[v & 3];
+    if (cap != 0.f) z = cap * fast_tanh(z / cap);
+    lp = fmaf(z, inv_temp, -lse[n]);
+  }
+  a.logprobs[at] = lp;
 }
 
 // G[n] = sum of the gradients of a token's ids in the vocabulary: what its softmax is multiplied by.  A wavefront per token.
@@ -1964,7 +1992,10 @@ int fwd_impl(const void* hidden, const void* weight, const void* labels, int lab
               softcap > 0.f ? 1.f / softcap : 0.f, sw.tiles, dma_ok(g) ? halved_tiles(n, v) : 0};
   {
     Span span(timer, 0);
-    if (stash && keep == kKeepLogits) {
+    if (stash && keep == kKeepLogits && label_optional && dma_ok(g) && narrow_columns(n) < kBlocks) {
+      rc = softcap > 0.f ? launch_fwd_narrow<true, kKeepLogits>(g, p, st) : launch_fwd_narrow<false, kKeepLogits>(g, p, st);
+      if (rc != AXON_OK) return rc;
+    } else if (stash && keep == kKeepLogits) {
       rc = softcap > 0.f ? launch_fwd_logits<true>(g, p, st) : launch_fwd_logits<false>(g, p, st);
       if (rc != AXON_OK) return rc;
     } else if (stash && keep == kKeepTop) {
@@ -2584,22 +2615,20 @@ extern "C" int axon_scale_bf16_unless_one(void* x, int64_t n, const float* scale
 // ----------------------------------------------------------------------------
 namespace {
 
-// Behind the forward's own workspace: the part maxima, then the kept logits, a tile for every 256 tokens x 256 rows.
+// Behind the forward's own workspace: the part maxima.
 struct TopWs {
   float* maxima;
-  uint4* tiles;
   int64_t bytes;
 };
 TopWs top_ws(int64_t n, int64_t v, void* base) {
   const FwdWs f = fwd_ws(n, v, base);
-  char* p = static_cast<char*>(base);
   TopWs w;
-  w.maxima = reinterpret_cast<float*>(p + f.bytes);
-  const int64_t maxima = round_up((int64_t)f.parts * n * 4, kAlign);
-  w.tiles = reinterpret_cast<uint4*>(p + f.bytes + maxima);
-  w.bytes = f.bytes + maxima + (round_up(v, kTile) / kTile) * (round_up(n, kTile) / kTile) * kLogitsTileBytes;
+  w.maxima = reinterpret_cast<float*>(static_cast<char*>(base) + f.bytes);
+  w.bytes = f.bytes + round_up((int64_t)f.parts * n * 4, kAlign);
   return w;
 }
+// a tile for every 256 tokens x 256 vocabulary rows
+int64_t top_logits_bytes(int64_t n, int64_t v) { return (round_up(v, kTile) / kTile) * (round_up(n, kTile) / kTile) * kLogitsTileBytes; }
 
 constexpr int64_t kTopLdsBytes = 48 * 1024;  // beyond: the maxima are read where they lie
 
@@ -2610,23 +2639,29 @@ extern "C" int64_t axon_lmhead_top_workspace_bytes(int64_t n, int64_t h, int64_t
   return rc != AXON_OK ? rc : top_ws(n, v, nullptr).bytes + kAlign;
 }
 
+extern "C" int64_t axon_lmhead_top_logits_bytes(int64_t n, int64_t h, int64_t v) {
+  const int rc = check_head_shape(n, h, v);
+  return rc != AXON_OK ? rc : top_logits_bytes(n, v);
+}
+
 extern "C" int axon_lmhead_top_fwd(const void* hidden, const void* weight, const void* labels, int labels_i64, int64_t n,
                                    int64_t h, int64_t v, float inv_temp, float softcap, int64_t k, float* logprobs,
                                    float* entropy, float* lse, float* entropy_b, float* top_logprobs, int64_t* top_ids,
-                                   void* workspace, int64_t ws_bytes, void* stream) {
+                                   void* workspace, int64_t ws_bytes, void* logits, int64_t logits_bytes, void* stream) {
   const int shape = check_head_shape(n, h, v);
   if (shape != AXON_OK) return shape;
   if (k < 1 || k > kMaxTop || k > v) return AXON_ERR_SHAPE;
   if (n == 0) return AXON_OK;
-  if (!workspace || !top_logprobs || !top_ids) return AXON_ERR_ARG;
+  if (!workspace || !logits || !top_logprobs || !top_ids || (reinterpret_cast<uintptr_t>(logits) & 15)) return AXON_ERR_ARG;
+  if (top_logits_bytes(n, v) > logits_bytes) return AXON_ERR_WORKSPACE;
   char* base = reinterpret_cast<char*>(round_up(reinterpret_cast<int64_t>(workspace), kAlign));
   const TopWs w = top_ws(n, v, base);
   if ((base - static_cast<char*>(workspace)) + w.bytes > ws_bytes) return AXON_ERR_WORKSPACE;
   const int rc = fwd_impl(hidden, weight, labels, labels_i64, n, h, v, inv_temp, softcap, nullptr, 0, logprobs, entropy, lse,
-                          entropy_b, base, w.bytes, w.tiles, 0, stream, nullptr, false, kKeepTop, w.maxima, true);
+                          entropy_b, base, w.bytes, logits, 0, stream, nullptr, false, kKeepTop, w.maxima, true);
   if (rc != AXON_OK) return rc;
   TopParams p;
-  p.tiles = reinterpret_cast<const float4*>(w.tiles);
+  p.tiles = static_cast<const float4*>(logits);
   p.pm = w.maxima;  p.lse = lse;  p.top_logprobs = top_logprobs;  p.top_ids = top_ids;
   p.labels = labels;  p.labels_i64 = labels_i64;  p.logprobs = logprobs;
   p.n_tokens = (int)n;  p.vocab = (int)v;  p.k = (int)k;
@@ -2645,16 +2680,23 @@ extern "C" int axon_lmhead_top_fwd(const void* hidden, const void* weight, const
 extern "C" int axon_lmhead_tokens_fwd(const void* hidden, const void* weight, const void* ids, int ids_i64, int64_t n,
                                       int64_t h, int64_t v, float inv_temp, float softcap, int64_t k, float* logprobs,
                                       float* entropy, float* lse, float* entropy_b, void* workspace, int64_t ws_bytes,
-                                      void* stream) {
+                                      void* logits, int64_t logits_bytes, void* stream) {
   const int shape = check_head_shape(n, h, v);
   if (shape != AXON_OK) return shape;
   if (k < 1 || k > kMaxTokenArgs) return AXON_ERR_SHAPE;
   if (n == 0) return AXON_OK;
   if (!ids || !logprobs) return AXON_ERR_ARG;
   const int rc = fwd_impl(hidden, weight, nullptr, 0, n, h, v, inv_temp, softcap, nullptr, 0, nullptr, entropy, lse, entropy_b,
-                          workspace, ws_bytes, nullptr, 0, stream, nullptr, false, kKeepNone, nullptr, true);
+                          workspace, ws_bytes, logits, logits_bytes, stream, nullptr, false, kKeepLogits, nullptr, true);
   if (rc != AXON_OK) return rc;
   const TokenArgs a{ids, ids_i64, (int)k, logprobs, nullptr};
+  if (logits) {
+    hipLaunchKernelGGL(token_picks_kernel, dim3((unsigned)((n * k + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       static_cast<const float4*>(logits), (int)(round_up(n, kTile) / kTile), n * k, (int)v, a, inv_temp, softcap,
+                       lse);
+    AXON_CHECK_LAUNCH();
+    return AXON_OK;
+  }
   hipLaunchKernelGGL(token_logits_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream,
                      static_cast<const __bf16*>(hidden), static_cast<const __bf16*>(weight), (int)h, (int)v, a, inv_temp,
                      softcap, lse);
@@ -2670,7 +2712,8 @@ extern "C" int64_t axon_lmhead_tokens_bwd_workspace_bytes(int64_t n, int64_t h, 
 extern "C" int axon_lmhead_tokens_bwd(const float* g_logprobs, const float* g_entropy, const void* hidden, const void* weight,
                                       const void* ids, int ids_i64, int64_t k, const float* logprobs, const float* lse,
                                       const float* entropy_b, int64_t n, int64_t h, int64_t v, float inv_temp, float softcap,
-                                      void* d_hidden, void* d_weight, void* workspace, int64_t ws_bytes, void* stream) {
+                                      void* d_hidden, void* d_weight, void* workspace, int64_t ws_bytes, const void* logits,
+                                      int64_t logits_bytes, void* stream) {
   const int shape = check_head_shape(n, h, v);
   if (shape != AXON_OK) return shape;
   if (k < 1 || k > kMaxTokenArgs) return AXON_ERR_SHAPE;
@@ -2685,6 +2728,9 @@ extern "C" int axon_lmhead_tokens_bwd(const float* g_logprobs, const float* g_en
   hipLaunchKernelGGL(token_grad_sum_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a, (int)n, (int)v,
                      G);
   AXON_CHECK_LAUNCH();
+  BlockArgs blk;
+  blk.is_block = logits != nullptr;  // logits for any shape
+  blk.keep = kKeepLogits;
   return bwd_impl(G, g_entropy, hidden, weight, nullptr, 0, lse, entropy_b, n, h, v, inv_temp, softcap, nullptr, d_hidden,
-                  d_weight, 0, base + sums, left, nullptr, 0, stream, nullptr, BlockArgs(), &a);
+                  d_weight, 0, base + sums, left, logits, logits_bytes, stream, nullptr, blk, &a);
 }

@@ -28,7 +28,7 @@ __device__ __forceinline__ uint64_t order_key(float x, int index) {
 }
 
 struct SelectLds {
-  uint64_t cand[kCandidates];
+  alignas(16) uint64_t cand[kCandidates];
   int hist[256];
   int segs[kMaxSegs];
   uint32_t range[2][4];
@@ -40,6 +40,33 @@ template <int NT>
 __device__ __forceinline__ void group_sync() {
   if constexpr (NT == kWave) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   else __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
+  return v;
+}
+
+// Smallest and largest over the threads.
+template <int NT>
+__device__ __forceinline__ void group_range(SelectLds& s, int tid, uint32_t& lo, uint32_t& hi) {
+  lo = ~wave_max_u32(~lo);
+  hi = wave_max_u32(hi);
+  if (NT == kWave) return;
+  if ((tid & (kWave - 1)) == 0) { s.range[0][tid / kWave] = lo; s.range[1][tid / kWave] = hi; }
+  group_sync<NT>();
+#pragma unroll
+  for (int w = 0; w < NT / kWave; ++w) { lo = min(lo, s.range[0][w]); hi = max(hi, s.range[1][w]); }
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_upto(int v, int lane) {
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int o = __shfl_up(v, off, kWave);
+    if (lane >= off) v += o;
+  }
+  return v;
 }
 
 // The k-th largest of n keys (1 <= k <= n), eight bits at a time; `ties`: how many of the keys equal to it are among
@@ -60,13 +87,7 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
       int c[4], sum = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
-      int upto = sum;
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const int o = __shfl_up(upto, off, kWave);
-        if (tid >= off) upto += o;
-      }
-      int before = upto - sum;
+      int before = wave_upto(sum, tid) - sum;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; }
@@ -82,54 +103,61 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
   return prefix;
 }
 
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+// A row's keys in the threads' registers, up to NT * kHeld of them, requested together: a loop that asks for one at a time is
+// a trip to LDS or L2 each, and there are three such loops.  More are asked for again wherever they are needed.
+template <int NT, class Src>
+struct HeldKeys {
+  static constexpr int kHeld = NT == kWave ? 20 : 8;
+  const Src& src;
+  const int n, tid;
+  uint32_t key[kHeld];
+  __device__ __forceinline__ HeldKeys(const Src& s, int n_, int tid_) : src(s), n(n_), tid(tid_) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
-  return v;
-}
+    for (int u = 0; u < kHeld; ++u) {
+      if (u * NT >= n) break;
+      key[u] = tid + u * NT < n ? src.max_key(tid + u * NT) : 0u;
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      if (u * NT >= n) break;
+      if (tid + u * NT < n) f(tid + u * NT, key[u]);
+    }
+    for (int i = tid + kHeld * NT; i < n; i += NT) f(i, src.max_key(i));
+  }
+};
 
 // The segments that are looked at, to s.segs: those whose maximum reaches a bound (returned) that at least k maxima reach.
-// The keys' range is cut into 256 bins and the bin of the k-th taken whole if that makes at most half as many again; else
+// The keys' range is cut into 256 bins and the bin of the k-th taken whole if that makes at most a quarter more; else
 // the bin is cut again, down to one key, of whose segments the first are taken then.  A row of a model's logits takes one cut.
 template <int NT, class Src>
 __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k, SelectLds& s, int tid) {
-  const int lane = tid & (kWave - 1), wave = tid / kWave, most = k + k / 2 + 8;
+  const int most = k + k / 4 + 8;
+  const HeldKeys<NT, Src> keys(src, n, tid);
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i = tid; i < n; i += NT) {
-    const uint32_t key = src.max_key(i);
+  keys.each([&](int, uint32_t key) {
     lo = min(lo, key);
     hi = max(hi, key);
-  }
-  lo = ~wave_max_u32(~lo);
-  hi = wave_max_u32(hi);
-  if (NT > kWave) {
-    if (lane == 0) { s.range[0][wave] = lo; s.range[1][wave] = hi; }
-    group_sync<NT>();
-#pragma unroll
-    for (int w = 0; w < NT / kWave; ++w) { lo = min(lo, s.range[0][w]); hi = max(hi, s.range[1][w]); }
-  }
+  });
+  group_range<NT>(s, tid, lo, hi);
   int rest = k, above = 0;  // of the segments in the range, `rest` are wanted; `above`: segments above the range
   uint32_t least;
   for (uint32_t width = hi - lo;;) {  // the range: lo .. lo + width
     const int shift = width < 256 ? 0 : 24 - __builtin_clz(width);
     for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
     group_sync<NT>();
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t at = src.max_key(i) - lo;
+    keys.each([&](int, uint32_t key) {
+      const uint32_t at = key - lo;
       if (at <= width) atomicAdd(&s.hist[at >> shift], 1);
-    }
+    });
     group_sync<NT>();
     if (tid < kWave) {  // lane l: bins 255 - 4 l and the three below
       int c[4], sum = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
-      int upto = sum;
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const int o = __shfl_up(upto, off, kWave);
-        if (tid >= off) upto += o;
-      }
-      int before = upto - sum;
+      int before = wave_upto(sum, tid) - sum;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; s.upto = before + c[q]; }
@@ -145,17 +173,19 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
     lo = least;
     width = min((1u << shift) - 1, last - lo);
   }
-  const int ties = rest - s.before;  // at a bin of one key: how many of its segments are wanted
   if (above + s.upto <= most) {
-    for (int i = tid; i < n; i += NT)
-      if (src.max_key(i) >= least) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+    keys.each([&](int i, uint32_t key) {
+      if (key >= least) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+    });
     return least;
   }
+  const int ties = rest - s.before;  // at a bin of one key: how many of its segments are wanted
   int one;
   auto first = [&](int i) { return src.max_key(i) == least ? 0xffffffffu - (uint32_t)i : 0u; };
   const uint32_t last = kth_largest<NT, uint32_t>(first, n, ties, s, tid, one);
-  for (int i = tid; i < n; i += NT)
-    if (src.max_key(i) > least || first(i) >= last) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+  keys.each([&](int i, uint32_t key) {
+    if (key > least || (key == least && 0xffffffffu - (uint32_t)i >= last)) s.segs[atomicAdd(&s.n_segs, 1)] = i;
+  });
   return least;
 }
 
@@ -179,13 +209,31 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     const int at = atomicAdd(&s.n_cand, 1);
     if (at < kCandidates) s.cand[at] = order_key(x, index);
   };
-  for (int j = tid; j < n_items; j += NT) {
-    float v[Src::kPer];
-    const int i0 = src.load(s.segs, j, v);
-    if (i0 < 0) continue;
+  // an item of which no element reaches the bound, as most, costs a comparison (the bound 0 takes everything, NaN included)
+  const float bound = least == 0 ? -INFINITY : key_value(least);
+  auto any = [&](const float (&v)[Src::kPer]) {
+    float m = v[0];
 #pragma unroll
-    for (int e = 0; e < Src::kPer; ++e)
-      if (i0 + e < limit) offer(v[e], i0 + e);
+    for (int e = 1; e < Src::kPer; ++e) m = fmaxf(m, v[e]);
+    return least == 0 || m >= bound;
+  };
+  // four loads under way together: one at a time is a trip to memory each
+  constexpr int kDeep = 4;
+  for (int j0 = tid; j0 < n_items; j0 += kDeep * NT) {
+    float v[kDeep][Src::kPer];
+    int i0[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      i0[u] = -1;
+      if (j0 + u * NT < n_items) i0[u] = src.load(s.segs, j0 + u * NT, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      if (i0[u] < 0 || !any(v[u])) continue;
+#pragma unroll
+      for (int e = 0; e < Src::kPer; ++e)
+        if (i0[u] + e < limit) offer(v[u][e], i0[u] + e);
+    }
   }
   for (int i = tid; i < src.n_single(); i += NT) {
     int index;
@@ -221,11 +269,76 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     group_sync<NT>();
     c = k;
   }
+  // Ranks.  Few candidates are each compared with all; more are first put in order of 256 bins of their range, and compared
+  // inside their bin.
+  auto put = [&](int rank, uint64_t key) {
+    if (rank < k) out(rank, key_value((uint32_t)(key >> 32)), (int)(0xffffffffu - (uint32_t)key));
+  };
+  if (c <= kWave) {
+    if (tid == 0) s.cand[c] = 0;  // to a whole number of pairs
+    group_sync<NT>();
+    if (tid < c) {
+      const uint64_t mine = s.cand[tid];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < c; j += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s.cand + j);
+        rank += (two.x > mine) + (two.y > mine);
+      }
+      put(rank, mine);
+    }
+    return;
+  }
+  uint32_t lo = 0xffffffffu, hi = 0;
   for (int i = tid; i < c; i += NT) {
-    const uint64_t mine = s.cand[i];
-    int rank = 0;
-    for (int j = 0; j < c; ++j) rank += s.cand[j] > mine;
-    if (rank < k) out(rank, key_value((uint32_t)(mine >> 32)), (int)(0xffffffffu - (uint32_t)mine));
+    const uint32_t key = (uint32_t)(s.cand[i] >> 32);
+    lo = min(lo, key);
+    hi = max(hi, key);
+  }
+  group_range<NT>(s, tid, lo, hi);
+  const int shift = hi - lo < 256 ? 0 : 24 - __builtin_clz(hi - lo);
+  for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+  group_sync<NT>();
+  // a candidate's bin, and its number among those of the bin that came before it
+  constexpr int kSlots = kCandidates / NT;
+  uint64_t mine[kSlots];
+  int bin[kSlots], nth[kSlots];
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    if (u * NT >= c) break;
+    if (tid + u * NT >= c) continue;
+    mine[u] = s.cand[tid + u * NT];
+    bin[u] = ((uint32_t)(mine[u] >> 32) - lo) >> shift;
+    nth[u] = atomicAdd(&s.hist[bin[u]], 1);
+  }
+  group_sync<NT>();
+  if (tid < kWave) {  // hist[b]: how many lie in higher bins; lane l has bins 255 - 4 l and the three below
+    int n4[4], sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += n4[q] = s.hist[255 - 4 * tid - q];
+    int before = wave_upto(sum, tid) - sum;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s.hist[255 - 4 * tid - q] = before;
+      before += n4[q];
+    }
+  }
+  group_sync<NT>();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    if (u * NT >= c) break;
+    if (tid + u * NT < c) s.cand[s.hist[bin[u]] + nth[u]] = mine[u];
+  }
+  group_sync<NT>();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    if (u * NT >= c) break;
+    if (tid + u * NT >= c) continue;
+    int rank = s.hist[bin[u]];
+    if (rank >= k) continue;
+    const int end = bin[u] > 0 ? s.hist[bin[u] - 1] : c;
+    for (int j = rank; j < end; ++j) rank += s.cand[j] > mine[u];
+    put(rank, mine[u]);
   }
 }
 

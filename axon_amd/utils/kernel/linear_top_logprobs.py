@@ -10,7 +10,8 @@ them and a student that is trained on them need more (the reference has no such 
   accumulation; fp16 and fp32 operands are rounded first and receive their gradients in their own dtype), ``H`` a multiple
   of 32; outputs are fp32 in the shape of ``hidden`` without its last dimension (and with ``k`` behind it);
 * both are differentiable with respect to ``hidden`` and ``weight`` through log-probabilities and entropy; the ids of the
-  alternatives are constants.  The backward recomputes the logits, as ``linear_cross_entropy``'s does;
+  alternatives are constants.  The backward takes the fp32 logits that the forward has kept for it where those of all
+  tokens take at most 2.5 GB (and memory has room for as much again), and recomputes them else, to the same gradients;
 * the alternatives (at most 128) are ordered by the product's fp32 result, before temperature and soft cap (which keep that
   order, but may round different logits to one), equal ones by ascending id; a position's fp32 logits are held while its
   block of tokens is selected from (2.5 GB whatever the number of tokens), never all of them;
@@ -59,15 +60,16 @@ class _LinearAlternatives(torch.autograd.Function):
         rows, w, inv_t, cap = _operands(what, hidden, weight, temperature, logit_softcapping)
         batch, n = hidden.shape[:-1], rows.shape[0]
         top_ids = label_lp = None
+        want_grad = bool(ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
         if ids is None:
             lab = labels.reshape(-1).contiguous() if labels is not None else None
-            label_lp, entropy, lse, mean, lp, at = _ops.lmhead_top(rows, w, k, lab, inv_t, cap)
+            label_lp, entropy, lse, mean, lp, at, logits = _ops.lmhead_top(rows, w, k, lab, inv_t, cap, want_grad)
             top_ids = at.view(*batch, k)
             ctx.mark_non_differentiable(top_ids)
         else:
             lab, at = None, ids.reshape(n, ids.shape[-1])
-            lp, entropy, lse, mean = _ops.lmhead_tokens(rows, w, at, inv_t, cap)
-        ctx.save_for_backward(rows, w, at, lp, lab, label_lp, lse, mean)
+            lp, entropy, lse, mean, logits = _ops.lmhead_tokens(rows, w, at, inv_t, cap, want_grad)
+        ctx.save_for_backward(rows, w, at, lp, lab, label_lp, lse, mean, logits)
         ctx.shape, ctx.in_dtypes, ctx.scalars = hidden.shape, (hidden.dtype, weight.dtype), (inv_t, cap)
         return (label_lp.view(batch) if label_lp is not None else None, entropy.view(batch),
                 lp.view(*batch, lp.shape[1]), top_ids)
@@ -77,7 +79,7 @@ class _LinearAlternatives(torch.autograd.Function):
     def backward(ctx, g_label, g_entropy, g_lp, _g_ids):
         if g_label is None and g_entropy is None and g_lp is None:
             return (None,) * 8
-        rows, w, at, lp, lab, label_lp, lse, mean = ctx.saved_tensors
+        rows, w, at, lp, lab, label_lp, lse, mean, logits = ctx.saved_tensors
         n, k = lp.shape
         g = torch.zeros_like(lp) if g_lp is None else g_lp.reshape(n, k)
         if g_label is not None:  # the label is one more token of its position
@@ -85,7 +87,7 @@ class _LinearAlternatives(torch.autograd.Function):
             lp = torch.cat([label_lp[:, None], lp], 1)
             g = torch.cat([g_label.reshape(n, 1), g], 1)
         g_en = None if g_entropy is None else g_entropy.reshape(n)
-        d_hidden, d_weight = _ops.lmhead_tokens_backward(g, g_en, rows, w, at, lp, lse, mean, *ctx.scalars)
+        d_hidden, d_weight = _ops.lmhead_tokens_backward(g, g_en, rows, w, at, lp, lse, mean, *ctx.scalars, logits)
         return (d_hidden.view(ctx.shape).to(ctx.in_dtypes[0]), d_weight.to(ctx.in_dtypes[1]), None, None, None, None, None,
                 None)
 

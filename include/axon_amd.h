@@ -267,30 +267,33 @@ int axon_lmhead_block_can_group(int64_t hidden, int64_t vocab, int64_t vocab_chu
  * axon_lmhead_fwd; ids and logprobs are [n_tokens][k].
  *   _top_fwd: the k largest logits of every position (1 <= k <= 128, k <= vocab), by the product's fp32 result before
  *        temperature and soft cap, in descending order, equal ones by ascending id: top_ids (int64) and their
- *        log-probabilities top_logprobs; beside them logprobs of `labels` (both or neither NULL) and the entropy.  The
- *        workspace holds the call's logits in fp32 (4 bytes x tokens x vocab, whole tiles of 256): callers cut long
- *        batches into calls.
+ *        log-probabilities top_logprobs; beside them logprobs of `labels` (both or neither NULL) and the entropy.  `logits`
+ *        (axon_lmhead_top_logits_bytes, 16-byte aligned) holds the call's logits in fp32 (4 bytes x tokens x vocab, whole
+ *        tiles of 256): callers cut long batches into calls.
  *   _tokens_fwd: logprobs of the given ids (int32 or int64, 1 <= k <= 513), 0 for an id outside [0, vocab), and the
- *        entropy; workspace: axon_lmhead_fwd_workspace_bytes.  No logits are kept.
+ *        entropy; workspace: axon_lmhead_fwd_workspace_bytes.  `logits` NULL: none are kept; else as above, for hidden sizes
+ *        that are multiples of 64.
  *   _tokens_bwd: d_hidden and d_weight (bf16) from the gradients of these logprobs (g_logprobs) and of the entropy
  *        (g_entropy, may be NULL); `logprobs`, `lse`, `entropy_b` are what either forward returned for these ids.  Equal
- *        ids of a position add up, ids outside the vocabulary are left out.  The logits are recomputed, as by
- *        axon_lmhead_bwd. */
+ *        ids of a position add up, ids outside the vocabulary are left out.  `logits`: what either forward left there for
+ *        the same operands (hidden % 64 == 0), or NULL: they are recomputed, to the same gradients. */
 int64_t axon_lmhead_top_workspace_bytes(int64_t n_tokens, int64_t hidden, int64_t vocab);
+int64_t axon_lmhead_top_logits_bytes(int64_t n_tokens, int64_t hidden, int64_t vocab);
 int axon_lmhead_top_fwd(const void* hidden_bf16, const void* weight_bf16, const void* labels, int labels_are_i64,
                         int64_t n_tokens, int64_t hidden, int64_t vocab, float inv_temperature, float softcap, int64_t k,
                         float* logprobs, float* entropy, float* lse, float* entropy_b, float* top_logprobs,
-                        int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream);
+                        int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* logits, int64_t logits_bytes,
+                        void* stream);
 int axon_lmhead_tokens_fwd(const void* hidden_bf16, const void* weight_bf16, const void* ids, int ids_are_i64,
                            int64_t n_tokens, int64_t hidden, int64_t vocab, float inv_temperature, float softcap,
                            int64_t k, float* logprobs, float* entropy, float* lse, float* entropy_b, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+                           int64_t workspace_bytes, void* logits, int64_t logits_bytes, void* stream);
 int64_t axon_lmhead_tokens_bwd_workspace_bytes(int64_t n_tokens, int64_t hidden, int64_t vocab);
 int axon_lmhead_tokens_bwd(const float* g_logprobs, const float* g_entropy, const void* hidden_bf16,
                            const void* weight_bf16, const void* ids, int ids_are_i64, int64_t k, const float* logprobs,
                            const float* lse, const float* entropy_b, int64_t n_tokens, int64_t hidden, int64_t vocab,
                            float inv_temperature, float softcap, void* d_hidden_bf16, void* d_weight_bf16,
-                           void* workspace, int64_t workspace_bytes, void* stream);
+                           void* workspace, int64_t workspace_bytes, const void* logits, int64_t logits_bytes, void* stream);
 
 /* How many bf16 copies of a chunk's dlogits the backward (axon_lmhead_bwd, axon_lmhead_block_bwd) writes for
  * this shape: 1 = token-major only (the weight-gradient GEMM reads it K-major), 2 = token-major and

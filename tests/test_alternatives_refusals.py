@@ -114,23 +114,26 @@ def test_the_heads_c_entry_points_check_their_arguments():
     assert lib.axon_lmhead_top_workspace_bytes(4, 64, 50) > 0
     assert lib.axon_lmhead_top_workspace_bytes(4, 33, 50) == -2 and lib.axon_lmhead_top_workspace_bytes(4, 0, 50) == -1
 
-    def top(h=p, w=p, lab=None, n=4, hs=64, v=50, inv_t=1.0, cap=0.0, k=3, lp=None, ent=p, lse=p, eb=p, tl=p, ti=p, ws=p, wb=big):
-        return lib.axon_lmhead_top_fwd(h, w, lab, 1, n, hs, v, inv_t, cap, k, lp, ent, lse, eb, tl, ti, ws, wb, None)
+    def top(h=p, w=p, lab=None, n=4, hs=64, v=50, inv_t=1.0, cap=0.0, k=3, lp=None, ent=p, lse=p, eb=p, tl=p, ti=p, ws=p, wb=big, z=p,
+            zb=big):
+        return lib.axon_lmhead_top_fwd(h, w, lab, 1, n, hs, v, inv_t, cap, k, lp, ent, lse, eb, tl, ti, ws, wb, z, zb, None)
 
     assert top(n=0) == 0
     for bad in (dict(h=None), dict(w=None), dict(lab=p), dict(lp=p), dict(ent=None), dict(lse=None), dict(eb=None), dict(tl=None),
-                dict(ti=None), dict(ws=None), dict(inv_t=0.0), dict(cap=-1.0), dict(h=p + 2), dict(n=-1)):
+                dict(ti=None), dict(ws=None), dict(inv_t=0.0), dict(cap=-1.0), dict(h=p + 2), dict(n=-1), dict(z=None), dict(z=p + 8)):
         assert top(**bad) == -1, bad
     assert top(k=0) == top(k=129) == top(k=51) == top(hs=33) == -2
     assert top(wb=lib.axon_lmhead_top_workspace_bytes(4, 64, 50) - 512) == -3
+    assert top(zb=lib.axon_lmhead_top_logits_bytes(4, 64, 50) - 1) == -3 and lib.axon_lmhead_top_logits_bytes(4, 33, 50) == -2
 
-    def fwd(ids=p, k=3, lp=p, n=4, wb=big):
-        return lib.axon_lmhead_tokens_fwd(p, p, ids, 1, n, 64, 50, 1.0, 0.0, k, lp, p, p, p, p, wb, None)
+    def fwd(ids=p, k=3, lp=p, n=4, wb=big, hs=64, z=None, zb=0):
+        return lib.axon_lmhead_tokens_fwd(p, p, ids, 1, n, hs, 50, 1.0, 0.0, k, lp, p, p, p, p, wb, z, zb, None)
 
     assert fwd(n=0) == 0 and fwd(ids=None) == fwd(lp=None) == -1 and fwd(k=0) == fwd(k=514) == -2 and fwd(wb=0) == -3
+    assert fwd(z=p, zb=16) == -3 and fwd(z=p + 8, zb=big) == -1 and fwd(z=p, zb=big, hs=96) == -2
 
     def bwd(g=p, ids=p, k=3, lp=p, dw=p, ws=p, wb=0, n=4):
-        return lib.axon_lmhead_tokens_bwd(g, p, p, p, ids, 1, k, lp, p, p, n, 64, 50, 1.0, 0.0, p, dw, ws, wb, None)
+        return lib.axon_lmhead_tokens_bwd(g, p, p, p, ids, 1, k, lp, p, p, n, 64, 50, 1.0, 0.0, p, dw, ws, wb, None, 0, None)
 
     assert bwd(g=None) == bwd(ids=None) == bwd(lp=None) == bwd(dw=None) == bwd(ws=None) == -1
     assert bwd(k=0) == bwd(k=514) == -2 and bwd() == -3

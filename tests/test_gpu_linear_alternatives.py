@@ -140,7 +140,7 @@ def test_vocabulary_chunks():
     hid, w, lab = operands(n, h, v, 5)
     ids = torch.stack([lab, (lab + 1) % v, torch.full_like(lab, -1)], 1)
     g = torch.randn(n, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
-    lp, ent, lse, mean = _ops.lmhead_tokens(hid, w, ids)
+    lp, ent, lse, mean, _ = _ops.lmhead_tokens(hid, w, ids)
     d_h, d_w = _ops.lmhead_tokens_backward(g, None, hid, w, ids, lp, lse, mean)
     part = torch.arange(0, n, 997, device="cuda")
     ref = Reference(hid[part], w, 1.0, None)
@@ -244,17 +244,21 @@ def test_a_student_on_a_teachers_alternatives():
     assert abs(loss.item() - value(student_h.double()).item()) <= 2 * ENT_TOL
 
 
-def test_results_repeat_and_replay():
+@pytest.mark.parametrize("h", [128, 768])
+def test_results_repeat_and_replay(h):
     """Forward and backward repeat bit for bit, eagerly and as a graph replayed on other inputs."""
-    n, h, v, k = 130, 128, 4096, 9
+    n, v, k = 130, 4096, 9
     hid, w, _ = operands(n, h, v, 7)
     ids = torch.randint(0, 5, (n, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
     g = torch.randn(n, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
 
+    hid.requires_grad_(True)
+    w.requires_grad_(True)
+
     def step():
-        _, ent, lse, mean, lp, top = _ops.lmhead_top(hid, w, k)
-        lp2, ent2, lse2, mean2 = _ops.lmhead_tokens(hid, w, ids)
-        return [ent, lp, top, lp2, *_ops.lmhead_tokens_backward(g, ent, hid, w, ids, lp2, lse2, mean2)]
+        r = linear_top_logprobs(hid, w, k)
+        lp, ent = linear_token_logprobs(hid, w, ids)
+        return [r.entropy.detach(), r.top_ids, lp.detach(), *torch.autograd.grad([r.top_logprobs, ent, lp], [hid, w], [g, g[:, 0], g])]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -265,8 +269,59 @@ def test_results_repeat_and_replay():
     with torch.cuda.graph(graph):
         held = step()
     for seed in (7, 8, 9):
-        hid.copy_(operands(n, h, v, seed)[0])
+        with torch.no_grad():
+            hid.copy_(operands(n, h, v, seed)[0])
         graph.replay()
         torch.cuda.synchronize()
         for a, b, c in zip(held, step(), step()):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("n,h,v,temperature,cap", [(40, 768, 3000, 1.0, None), (190, 832, 2051, 0.7, 20.0), (300, 768, 5000, 1.0, None),
+                                                   (513, 1024, 2048, 1.3, 30.0)])
+def test_kept_logits_give_the_same_gradients(monkeypatch, n, h, v, temperature, cap):
+    """Bit for bit, whether the backward takes the logits that the forward has kept or recomputes them."""
+    hid, w, lab = operands(n, h, v, 6)
+    ids = torch.randint(-1, v, (n, 7), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    g = torch.randn(n, 7, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    hid.requires_grad_(True)
+    w.requires_grad_(True)
+
+    def step():
+        lp, ent = linear_token_logprobs(hid, w, ids, temperature, cap)
+        r = linear_top_logprobs(hid, w, 7, lab, temperature, cap)
+        saved = [t for t in lp.grad_fn.saved_tensors + r.entropy.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8]
+        a = torch.autograd.grad([lp, ent], [hid, w], [g, g[:, 0]])
+        b = torch.autograd.grad([r.top_logprobs, r.logprobs], [hid, w], [g, g[:, 1]])
+        return lp.detach(), r.top_ids, [*a, *b], len(saved)
+
+    lp, top, grads, kept = step()
+    assert kept == 2
+    monkeypatch.setattr(_ops, "TOP_KEEP_LOGITS_MIN_HIDDEN", 1 << 30)
+    lp2, top2, grads2, kept = step()
+    assert kept == 0 and torch.equal(top, top2) and (lp - lp2).abs().max() <= lp_tol(cap or 0, 1 / temperature)
+    # the given tokens' log-probabilities come from the product here and from a dot there: their dlogits, of relative error
+    # LP_TOL, may round to the other neighbour in bf16; the alternatives' are the same numbers
+    assert all(torch.equal(x, y) for x, y in zip(grads[2:], grads2[2:]))
+    ref = Reference(hid.detach(), w.detach(), 1 / temperature, cap)
+    for pair in (grads[:2], grads2[:2]):
+        ref.check_grads(ids, g, g[:, 0], *pair)
+
+
+def test_saved_tensors_from_a_hook_are_looked_at_again():
+    n, h, v = 20, 768, 600
+    hid, w, lab = operands(n, h, v, 3)
+
+    def backward_with(unpack):
+        a, b = hid.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            r = linear_top_logprobs(a, b, 3, lab)
+        return torch.autograd.grad(r.top_logprobs.sum() + r.logprobs.sum(), [a, b])
+
+    want = backward_with(lambda t: t)
+    assert all(torch.equal(x, y) for x, y in zip(backward_with(lambda t: t.clone()), want))
+    for unpack in (lambda t: t.cpu(), lambda t: t.cpu() if t.dim() == 1 and t.dtype == torch.float32 else t,
+                   lambda t: t.cpu() if t.dtype == torch.int64 else t, lambda t: t.cpu() if t.dtype == torch.uint8 else t,
+                   lambda t: t[:-16] if t.dtype == torch.uint8 else t, lambda t: t[:5] if t.dim() == 2 and t.dtype == torch.float32 else t):
+        with pytest.raises((RuntimeError, ValueError)):
+            backward_with(unpack)
