@@ -27,8 +27,11 @@ __device__ __forceinline__ uint64_t order_key(float x, int index) {
   return ((uint64_t)order_key(x) << 32) | (0xffffffffu - (uint32_t)index);
 }
 
+constexpr int kHits = 96;  // items that hold a candidate and are gone through an element per thread
 struct SelectLds {
   alignas(16) uint64_t cand[kCandidates];
+  float hits[kHits][8];
+  int hit_at[kHits], n_hits;
   int hist[256];
   int segs[kMaxSegs];
   uint32_t range[2][4];
@@ -42,10 +45,30 @@ __device__ __forceinline__ void group_sync() {
   else __syncthreads();
 }
 
+// Permutations by DPP in which every lane has a source, and the sums up to a lane, whose missing sources are 0.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_of(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
-  return v;
+  v = max(v, lane_of<0xb1>(v));
+  v = max(v, lane_of<0x4e>(v));
+  v = max(v, lane_of<0x141>(v));
+  v = max(v, lane_of<0x140>(v));
+  const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+  return max(max(a, b), max(c, d));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add_i(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_upto(int v) {
+  v = dpp_add_i<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add_i<0x112, 0xf>(v);
+  v = dpp_add_i<0x114, 0xf>(v);
+  v = dpp_add_i<0x118, 0xf>(v);
+  v = dpp_add_i<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  return dpp_add_i<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 
 // Smallest and largest over the threads.
@@ -59,16 +82,6 @@ __device__ __forceinline__ void group_range(SelectLds& s, int tid, uint32_t& lo,
 #pragma unroll
   for (int w = 0; w < NT / kWave; ++w) { lo = min(lo, s.range[0][w]); hi = max(hi, s.range[1][w]); }
 }
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int wave_upto(int v, int lane) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int o = __shfl_up(v, off, kWave);
-    if (lane >= off) v += o;
-  }
-  return v;
-}
-
 // The k-th largest of n keys (1 <= k <= n), eight bits at a time; `ties`: how many of the keys equal to it are among
 // the k.  key_at(i) is asked for every i once per eight bits.
 template <int NT, class Key, class KeyAt>
@@ -87,7 +100,7 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
       int c[4], sum = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
-      int before = wave_upto(sum, tid) - sum;
+      int before = wave_upto(sum) - sum;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; }
@@ -157,7 +170,7 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
       int c[4], sum = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum += c[q] = s.hist[255 - 4 * tid - q];
-      int before = wave_upto(sum, tid) - sum;
+      int before = wave_upto(sum) - sum;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (before < rest && before + c[q] >= rest) { s.bin = 255 - 4 * tid - q; s.before = before; s.upto = before + c[q]; }
@@ -196,7 +209,7 @@ template <int NT, class Src, class Out>
 __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, int tid, Out out) {
   const int n = src.n_segs();
   uint32_t least = 0;  // what an element has to reach
-  if (tid == 0) s.n_segs = s.n_cand = 0;
+  if (tid == 0) s.n_segs = s.n_cand = s.n_hits = 0;
   if (n > k) {
     least = choose_segments<NT>(src, n, k, s, tid);
   } else {
@@ -230,10 +243,24 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
 #pragma unroll
     for (int u = 0; u < kDeep; ++u) {
       if (i0[u] < 0 || !any(v[u])) continue;
+      const int hit = atomicAdd(&s.n_hits, 1);
+      if (hit < kHits) {
+        s.hit_at[hit] = i0[u];
 #pragma unroll
-      for (int e = 0; e < Src::kPer; ++e)
-        if (i0[u] + e < limit) offer(v[u][e], i0[u] + e);
+        for (int e = 0; e < Src::kPer; ++e) s.hits[hit][e] = v[u][e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < Src::kPer; ++e)
+          if (i0[u] + e < limit) offer(v[u][e], i0[u] + e);
+      }
     }
+  }
+  group_sync<NT>();
+  // few items hold a candidate: their elements one per thread (all elements of every item: eight times the instructions in each
+  // wavefront that has one)
+  for (int i = tid, n_el = min(s.n_hits, kHits) * Src::kPer; i < n_el; i += NT) {
+    const int index = s.hit_at[i / Src::kPer] + i % Src::kPer;
+    if (index < limit) offer(s.hits[i / Src::kPer][i % Src::kPer], index);
   }
   for (int i = tid; i < src.n_single(); i += NT) {
     int index;
@@ -316,7 +343,7 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     int n4[4], sum = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) sum += n4[q] = s.hist[255 - 4 * tid - q];
-    int before = wave_upto(sum, tid) - sum;
+    int before = wave_upto(sum) - sum;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       s.hist[255 - 4 * tid - q] = before;
