@@ -410,10 +410,20 @@ using namespace axon;
 
 namespace {
 
-// Workgroups per row: as in logits.hip, except that rows this few are always split (the second launch is there anyway).
+// Workgroups per row of the backward: as in logits.hip, whose backward moves the same bytes.
 int row_parts(int64_t n, int64_t vocab, int elem_bytes) {
   if (n >= 1536) return 1;
   const int64_t fill = 8192 / (n > 0 ? n : 1), work = vocab * elem_bytes / (8 * 16 * kBlock);
+  const int64_t p = fill < work ? fill : work;
+  return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
+}
+// ... and of the forward.  From 512 rows on a row is left to one workgroup, which finishes it (20 alternatives, split / whole, us:
+// 512 x 201088 fp32 82 / 72, 1300 x 201088 194 / 184, 1500 x 151936 bf16 92 / 83, 512 x 151936 bf16 42 / 45; 320 x 201088
+// 55 / 65).  Fewer rows are split into about 2048 pieces, what the part holds at once, of at least a tile per wavefront (250 x
+// 151936 bf16 25.9 us for 27.0 with 8192 pieces, 400 32.5 for 35.4; one row 11.8 for 12.4 with pieces twice as long).
+int fwd_parts(int64_t n, int64_t vocab, int elem_bytes) {
+  if (n >= 512) return 1;
+  const int64_t fill = 2048 / (n > 0 ? n : 1), work = vocab * elem_bytes / (kTileVecs * 16 * (kBlock / kWave));
   const int64_t p = fill < work ? fill : work;
   return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
 }
@@ -453,7 +463,7 @@ int cached_from(int64_t n, int64_t vocab, int eb, int bwd_follows) {
 
 extern "C" int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
   if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
-  const int parts = row_parts(n, vocab, elem_bytes(dtype));
+  const int parts = fwd_parts(n, vocab, elem_bytes(dtype));
   if (parts == 1 && top_lds(dtype, vocab) <= kMaxTopLds) return 0;
   return n * (parts * 3 + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
 }
@@ -471,7 +481,7 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
   if (need > 0 && !workspace) return AXON_ERR_ARG;
   if (need > workspace_bytes) return AXON_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
-  const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
+  const int eb = elem_bytes(dtype), parts = fwd_parts(n, vocab, eb);
   const bool whole = need == 0;
   float* const seg_max = whole ? nullptr : workspace + n * parts * 3;
   const int stride = (int)seg_stride(dtype, vocab), from = cached_from(n, vocab, eb, bwd_follows);
@@ -496,7 +506,7 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
 
 extern "C" int64_t axon_logits_tokens_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
   if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
-  const int parts = row_parts(n, vocab, elem_bytes(dtype));
+  const int parts = fwd_parts(n, vocab, elem_bytes(dtype));
   return parts > 1 ? n * parts * 3 * (int64_t)sizeof(float) : 0;
 }
 
@@ -508,7 +518,7 @@ extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld,
   if (k < 1 || k > kMaxTokenIds) return AXON_ERR_SHAPE;
   if (n == 0) return AXON_OK;
   if (!lse || !ids || !logprobs) return AXON_ERR_ARG;
-  const int eb = elem_bytes(dtype), parts = row_parts(n, vocab, eb);
+  const int eb = elem_bytes(dtype), parts = fwd_parts(n, vocab, eb);
   const int64_t need = axon_logits_tokens_workspace_bytes(dtype, n, vocab);
   if (need > 0 && (!workspace || need > workspace_bytes)) return AXON_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
