@@ -114,16 +114,11 @@ struct RowOut {
   const void* labels;              // may be null
   int labels_i64;
 };
-// (log-sum-exp, entropy) from a row's statistics, and the label's log-probability
-template <typename T>
-__device__ __forceinline__ float write_row(Stats st, int t, const T* row, int vocab, const RowOut& o) {
+// A row's log-sum-exp and entropy from its statistics.
+__device__ __forceinline__ float write_row(Stats st, int t, const RowOut& o) {
   const float L = __log2f(st.s), d = st.e / st.s, lse = (st.M + L) * kLn2;
   o.lse[t] = lse;
   if (o.entropy != nullptr) o.entropy[t] = (L - d) * kLn2;
-  if (o.logprob != nullptr) {
-    const int64_t lab = load_id(o.labels, o.labels_i64, t);
-    o.logprob[t] = (lab >= 0 && lab < vocab) ? Row<T>::one(row + lab) - lse : 0.f;
-  }
   return lse;
 }
 
@@ -141,9 +136,9 @@ __device__ __forceinline__ void write_picks(const Picks& p, int t, const T* row,
 }
 
 // A row of logits as select_top reads it.
-template <typename T>
+template <typename T, int HELD>
 struct LogitsSource {
-  static constexpr int kPer = Row<T>::kPer, kItems = kSegVecs;
+  static constexpr int kPer = Row<T>::kPer, kItems = kSegVecs, kHeld = HELD;
   const T* row;
   const float* seg_max;  // LDS or global
   SegSpan sp;
@@ -173,18 +168,35 @@ struct TopOut {
   int64_t* ids;     // [n][k]
   int k;
 };
-template <typename T>
-__device__ __forceinline__ void write_top(const TopOut& o, int t, const T* row, int vocab, const float* seg_max, float lse,
-                                          SelectLds& s) {
-  const LogitsSource<T> src{row, seg_max, SegSpan(row, vocab, 0, 1), vocab};
-  select_top<kBlock>(src, o.k, s, threadIdx.x, [&](int rank, float z, int index) {
-    o.logprobs[(int64_t)t * o.k + rank] = z - lse;
-    o.ids[(int64_t)t * o.k + rank] = index;
-  });
-}
-
 // What is wanted of a row beside its statistics.
 enum Want { kTokens, kTop };
+
+// The end of a row: log-sum-exp and entropy from its statistics (in thread 0), then what is wanted of it.  HELD: how many
+// maxima a thread holds, 0 where they are in LDS.
+template <typename T, Want WANT, int HELD>
+__device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vocab, const float* seg_max, const RowOut& out,
+                                           const Picks& picks, const TopOut& top, SelectLds* sel) {
+  __shared__ float s_lse;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_lse = write_row(st, t, out);
+  if (WANT == kTokens) {
+    __syncthreads();
+    write_picks<T>(picks, t, row, vocab, s_lse);
+    return;
+  }
+  // the last thread asks for the label's logit here and uses it at the end: the label is a trip to memory, its logit another
+  const bool with_label = tid == kBlock - 1 && out.logprob != nullptr;
+  const int64_t lab = with_label ? load_id(out.labels, out.labels_i64, t) : -1;
+  const bool inside = lab >= 0 && lab < vocab;
+  const float label_z = inside ? Row<T>::one(row + lab) : 0.f;
+  // (the selection's own barriers come before the first use of s_lse)
+  const LogitsSource<T, HELD> src{row, seg_max, SegSpan(row, vocab, 0, 1), vocab};
+  select_top<kBlock>(src, top.k, *sel, tid, [&](int rank, float z, int index) {
+    top.logprobs[(int64_t)t * top.k + rank] = z - s_lse;
+    top.ids[(int64_t)t * top.k + rank] = index;
+  });
+  if (with_label) out.logprob[t] = inside ? label_z - s_lse : 0.f;
+}
 
 // Workgroup (row, part): blockIdx.x = row * parts + part.  Where a row has one part it is finished here: a row's selection
 // runs beside the reading of the rows that the compute unit's other workgroups have (the maxima of its segments are in
@@ -196,7 +208,6 @@ __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restric
                                                               RowOut out, Picks picks, TopOut top, int cached_from) {
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[3][kBlock / kWave];
-  __shared__ float s_lse;
   const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
   const T* row = logits + (int64_t)t * ld;
   constexpr int kPer = Row<T>::kPer;
@@ -244,19 +255,14 @@ __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restric
   st = wave_merge(st);
   if (lane == 0) { red[0][wave] = st.M; red[1][wave] = st.s; red[2][wave] = st.e; }
   __syncthreads();
-  if (tid == 0) {
+  if (tid == 0)
     for (int w = 1; w < kBlock / kWave; ++w) st = merge(st, Stats{red[0][w], red[1][w], red[2][w]});
-    if (!whole) {
-      float* o = ws + (int64_t)blockIdx.x * 3;
-      o[0] = st.M; o[1] = st.s; o[2] = st.e;
-    } else {
-      s_lse = write_row<T>(st, t, row, vocab, out);
-    }
+  if (whole) {
+    finish_row<T, WANT, 0>(st, t, row, vocab, segs, out, picks, top, reinterpret_cast<SelectLds*>(smem));
+  } else if (tid == 0) {
+    float* o = ws + (int64_t)blockIdx.x * 3;
+    o[0] = st.M; o[1] = st.s; o[2] = st.e;
   }
-  if (!whole) return;
-  __syncthreads();
-  if (WANT == kTop) write_top<T>(top, t, row, vocab, segs, s_lse, *reinterpret_cast<SelectLds*>(smem));
-  else write_picks<T>(picks, t, row, vocab, s_lse);
 }
 
 // The statistics of a row's parts (at most kMaxParts), in a fixed tree; the total in thread 0.
@@ -269,32 +275,20 @@ __device__ __forceinline__ Stats merge_parts(const float* ws, int t, int parts) 
   return threadIdx.x < kWave ? wave_merge(st) : st;
 }
 
-// A workgroup per row folds the parts' statistics and picks the given tokens.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void tokens_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
-                                                               const float* __restrict__ ws, RowOut out, Picks picks) {
-  __shared__ float s_lse;
-  const int t = blockIdx.x;
-  const T* row = logits + (int64_t)t * ld;
-  const Stats st = merge_parts(ws, t, parts);
-  if (threadIdx.x == 0) s_lse = write_row<T>(st, t, row, vocab, out);
-  __syncthreads();
-  write_picks<T>(picks, t, row, vocab, s_lse);
-}
-
-// A workgroup per row: folds the parts' statistics, selects the k largest.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void top_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
-                                                            const float* __restrict__ ws, const float* __restrict__ seg_max,
-                                                            int seg_stride, RowOut out, TopOut top) {
+// The end of rows that several workgroups have read, by a workgroup per row.  (In the launch before, by the workgroup that draws
+// a row's last ticket: one row of 151936 11.6 us for 12.5, but 61 x 201088 fp32 34 for 21 and 187 x 151936 51 for 23, for the
+// maxima that have to be written through to the level that the XCDs share.)
+template <typename T, Want WANT>
+__global__ __launch_bounds__(kBlock) void alternatives_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
+                                                                     const float* __restrict__ ws,
+                                                                     const float* __restrict__ seg_max, int seg_stride, RowOut out,
+                                                                     Picks picks, TopOut top) {
   __shared__ SelectLds s;
-  __shared__ float s_lse;
   const int t = blockIdx.x;
   const T* row = logits + (int64_t)t * ld;
-  const Stats st = merge_parts(ws, t, parts);
-  if (threadIdx.x == 0) s_lse = write_row<T>(st, t, row, vocab, out);
-  __syncthreads();
-  write_top<T>(top, t, row, vocab, seg_max + (int64_t)t * seg_stride, s_lse, s);
+  // 13 maxima per thread: 3328, 201088 fp32 logits have 3142
+  finish_row<T, WANT, 13>(merge_parts(ws, t, parts), t, row, vocab, WANT == kTop ? seg_max + (int64_t)t * seg_stride : nullptr,
+                          out, picks, top, &s);
 }
 
 // Upstream gradients of a row's chosen tokens: k of them, and a label's.  Either may be absent (g null).
@@ -495,8 +489,8 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
                        from);                                                                                              \
     AXON_CHECK_LAUNCH();                                                                                                   \
     if (!whole)                                                                                                            \
-      hipLaunchKernelGGL((top_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),    \
-                         ld, (int)vocab, parts, workspace, seg_max, stride, out, top);                                     \
+      hipLaunchKernelGGL((alternatives_finish_kernel<T, kTop>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),    \
+                         ld, (int)vocab, parts, workspace, seg_max, stride, out, Picks{}, top);                                     \
   } while (0)
   AXON_ROWS(dtype, AXON_TOP);
 #undef AXON_TOP
@@ -532,8 +526,8 @@ extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld,
                        from);                                                                                               \
     AXON_CHECK_LAUNCH();                                                                                                    \
     if (parts > 1)                                                                                                          \
-      hipLaunchKernelGGL((tokens_finish_kernel<T>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),  \
-                         ld, (int)vocab, parts, workspace, out, picks);                                                     \
+      hipLaunchKernelGGL((alternatives_finish_kernel<T, kTokens>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits),  \
+                         ld, (int)vocab, parts, workspace, nullptr, 0, out, picks, TopOut{});                                                     \
   } while (0)
   AXON_ROWS(dtype, AXON_TOKENS);
 #undef AXON_TOKENS

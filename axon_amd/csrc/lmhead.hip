@@ -1033,7 +1033,7 @@ __device__ __forceinline__ int64_t kept_vec(int part, int i, int lq, int64_t til
 // A token's kept logits as select_top reads them: its segments are the parts of 128 vocabulary rows, an item is the four
 // rows that one lane of the tile had.
 struct HeadSource {
-  static constexpr int kPer = 4, kItems = kWaveTile / 4;
+  static constexpr int kPer = 4, kItems = kWaveTile / 4, kHeld = 0;
   const float4* column;  // the token's place in the first tile of its column
   const float* maxima;   // its part maxima, `stride` apart
   int64_t stride, tile_step;

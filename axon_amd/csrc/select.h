@@ -116,14 +116,15 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
   return prefix;
 }
 
-// A row's keys in the threads' registers, up to NT * kHeld of them, requested together: a loop that asks for one at a time is
-// a trip to LDS or L2 each, and there are three such loops.  More are asked for again wherever they are needed.
+// A row's keys in the threads' registers, up to NT * Src::kHeld of them, requested together: where they are in memory, a loop
+// that asks for one at a time is a trip there each, and there are three such loops.  More are asked for again wherever they are
+// needed, as are those in LDS, which a loop reads faster than code for every number of them runs.
 template <int NT, class Src>
 struct HeldKeys {
-  static constexpr int kHeld = NT == kWave ? 20 : 8;
+  static constexpr int kHeld = Src::kHeld;
   const Src& src;
   const int n, tid;
-  uint32_t key[kHeld];
+  uint32_t key[kHeld > 0 ? kHeld : 1];
   __device__ __forceinline__ HeldKeys(const Src& s, int n_, int tid_) : src(s), n(n_), tid(tid_) {
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
@@ -202,7 +203,7 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
   return least;
 }
 
-// `src`: maxima of its segments, max_key(i) for i < n_segs(); the elements of the segments in `segs`, kPer consecutive ones
+// `src`: maxima of its segments, max_key(i) for i < n_segs() (kHeld: see HeldKeys); the elements of the segments in `segs`, kPer consecutive ones
 // per item: load(segs, j, v) returns the index of the first, or -1 where there is none (elements from limit() on do not
 // count); and n_single() elements outside all segments, single(i, index).  out(rank, value, index) for rank < k.
 template <int NT, class Src, class Out>

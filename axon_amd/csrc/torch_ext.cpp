@@ -464,6 +464,11 @@ Tensor once(Tensor grad, const char* what) {
   return (*error)({grad.detach().requires_grad_(true)})[0];
 }
 
+// Forward-mode gradients are not offered: a tangent would be dropped without a word.
+void no_tangent(const char* what, const Tensor& t) {
+  if (t._fw_grad(0).defined()) throw AxonError(std::string(what) + ": forward-mode differentiation is not supported");
+}
+
 struct AlternativesNode : torch::autograd::Node {
   SavedVariable rows, ids, labels, lse, entropy;
   std::vector<int64_t> shape;
@@ -512,6 +517,7 @@ struct AlternativesNode : torch::autograd::Node {
 std::tuple<OptTensor, Tensor, Tensor, Tensor> alternatives(const char* what, const Tensor& logits, int64_t k, const OptTensor& ids_in,
                                                            const OptTensor& labels, bool inplace) {
   const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
+  no_tangent(what, logits);
   Tensor entropy, lp, label_lp, lse, ids, lab, rows;
   std::vector<int64_t> batch(logits.sizes().begin(), logits.dim() ? logits.sizes().end() - 1 : logits.sizes().end());
   {
@@ -678,7 +684,10 @@ std::tuple<Tensor, Tensor> router_balance(const variable_list& logits, bool stac
                                           const OptTensor& cu_seqlens, const std::optional<variable_list>& expert_ids, int score) {
   const char* const what = RouterBalanceNode::kWhat;
   bool wants_grad = false;
-  for (const Tensor& t : logits) wants_grad = wants_grad || t.requires_grad();
+  for (const Tensor& t : logits) {
+    wants_grad = wants_grad || t.requires_grad();
+    no_tangent(what, t);
+  }
   wants_grad = wants_grad && at::GradMode::is_enabled();
   variable_list rows, ids;
   Tensor mask, cu, loss, scale, coef, counts;

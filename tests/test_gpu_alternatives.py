@@ -382,3 +382,32 @@ def test_a_logit_changed_before_the_backward_is_noticed():
         y.add_(1)
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(lp.sum(), x)
+
+
+def test_two_streams_at_once():
+    """Batches of few rows, whose rows several workgroups share: calls that overlap on two streams, and calls of other shapes in
+    between, leave each other's counters alone."""
+    zs = [logits_of("random", n, v, torch.bfloat16, n) for n, v in ((3, 151936), (70, 50257), (300, 32768), (1, 151936))]
+    ids = [torch.randint(0, z.shape[1], (z.shape[0], 4), generator=gen(i), device="cuda") for i, z in enumerate(zs)]
+    want = [(top_logprobs_from_logits(z, 9), token_logprobs_from_logits(z, i)) for z, i in zip(zs, ids)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for s, out in zip(streams, got):
+            with torch.cuda.stream(s):
+                out.append([(top_logprobs_from_logits(z, 9), token_logprobs_from_logits(z, i)) for z, i in zip(zs, ids)])
+    torch.cuda.synchronize()
+    for out in got[0] + got[1]:
+        for (a, b), (c, d) in zip(out, want):
+            assert torch.equal(a.top_ids, c.top_ids) and torch.equal(a.top_logprobs, c.top_logprobs) and torch.equal(a.entropy, c.entropy)
+            assert torch.equal(b[0], d[0]) and torch.equal(b[1], d[1])
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    z = logits_of("random", 2, 50, torch.float32, 1)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            top_logprobs_from_logits(fwd.make_dual(z, torch.ones_like(z)), 3)

@@ -120,6 +120,13 @@ def test_sequences(lens, layers, e, k, dtype, score):
     check([x.detach() for x in xs], k, cu=cu, score=score)
 
 
+def test_tokens_before_the_first_sequence():
+    """They belong to none, like those behind the last."""
+    xs, m, _ = case(2, 700, 24, 3, torch.float32, 8, torch.int64)
+    cu = torch.tensor([290, 300, 300, 690], dtype=torch.int32, device="cuda")
+    check(xs, 3, mask=m, cu=cu)
+
+
 @pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
 def test_given_choices(ids_dtype):
     xs, m, g = case(3, 300, 64, 6, torch.bfloat16, 5, torch.float32)
