@@ -210,7 +210,7 @@ __device__ __forceinline__ void make_keys(const float (&x)[V], int e0, int exper
     return;
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) key[j] = e0 + j < experts ? max(order_key(x[j]), 1u) : 0u;
+  for (int j = 0; j < V; ++j) key[j] = e0 + j < experts ? order_key(x[j]) : 0u;
 }
 
 // Adds 1 to cnt of the lane's elements that are among the row's k first by (value descending, index ascending), where `in`.

@@ -14,10 +14,11 @@ constexpr int kMaxTop = AXON_MAX_TOP;  // alternatives per row
 constexpr int kCandidates = 512;  // elements that reach the smallest maximum taken and are ranked against each other
 constexpr int kMaxSegs = 2 * kMaxTop;  // segments taken: the first k and a few more where that saves a look
 
-// Unsigned integers in the order of the floats; -0 equals 0, NaN is below everything.
+// Unsigned integers in the order of the floats; -0 equals 0, and NaN equals -inf, as a maximum that passes it by has it (so
+// that a segment's key is never above those of all its elements).
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
-  return x != x ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return x != x ? 0x007fffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
@@ -223,13 +224,13 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     const int at = atomicAdd(&s.n_cand, 1);
     if (at < kCandidates) s.cand[at] = order_key(x, index);
   };
-  // an item of which no element reaches the bound, as most, costs a comparison (the bound 0 takes everything, NaN included)
+  // an item of which no element reaches the bound, as most, costs a comparison (NaN passes it)
   const float bound = least == 0 ? -INFINITY : key_value(least);
   auto any = [&](const float (&v)[Src::kPer]) {
     float m = v[0];
 #pragma unroll
     for (int e = 1; e < Src::kPer; ++e) m = fmaxf(m, v[e]);
-    return least == 0 || m >= bound;
+    return !(m < bound);
   };
   // four loads under way together: one at a time is a trip to memory each
   constexpr int kDeep = 4;

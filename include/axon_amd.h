@@ -684,8 +684,8 @@ int axon_logits_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_
  * axon/utils/torch/ops.py:39-102, knows one token per position).  Operands as above, logits aligned to their element.
  *   _top_fwd: the k largest logits of every row (1 <= k <= 128, k <= vocab), in descending order, equal ones by
  *        ascending id: top_ids [n][k] int64 and top_logprobs [n][k] = logit - lse; beside them logprob (with labels),
- *        entropy (either may be NULL) and lse.  A row with a NaN has NaN everywhere but in top_ids, which then rank
- *        the NaN below everything; a row of -inf alone has NaN log-probabilities and the lowest ids.
+ *        entropy (either may be NULL) and lse.  A row with a NaN has NaN everywhere but in top_ids, for which a
+ *        NaN counts as -inf; a row of -inf alone has NaN log-probabilities and the lowest ids.
  *   _tokens_fwd: logprobs [n][k] of the given ids [n][k] (int32 or int64, 1 <= k <= 512), 0 for an id outside
  *        [0, vocab); entropy may be NULL.
  *   _tokens_bwd: the backward of both, one read and one write of the rows:

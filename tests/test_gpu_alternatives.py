@@ -155,6 +155,25 @@ def test_rows_without_a_softmax():
     assert torch.equal(r.top_ids[4], good.top_ids[4]) and torch.equal(r.top_logprobs[4], good.top_logprobs[4])
 
 
+@pytest.mark.parametrize("v,dtype", [(3000, torch.float32), (3000, torch.bfloat16), (12, torch.float32), (151936, torch.bfloat16)])
+@pytest.mark.parametrize("k", [1, 7])
+def test_ids_are_valid_whatever_the_row_holds(v, dtype, k):
+    """NaN counts as -inf for the ids: every row gets k different ids of the vocabulary, the lowest where nothing tells them
+    apart.  (The last segment of a row is filled up with -inf, which a row of NaN alone has to reach.)"""
+    z = logits_of("random", 4, v, dtype, 3)
+    z[0] = math.nan
+    z[1, : v - 1] = math.nan
+    z[2, ::2] = math.nan
+    z[3] = -math.inf
+    z[3, v // 2] = math.nan
+    for many in (1, 200):  # rows that several workgroups share, and rows that one finishes
+        r = top_logprobs_from_logits(z.repeat(many, 1), k)
+        for row in range(4):
+            want = order(torch.where(torch.isnan(z[row]), torch.tensor(-math.inf, dtype=dtype, device="cuda"), z[row])[None], k)[0]
+            assert (r.top_ids[row::4] == want).all()
+            assert torch.isnan(r.top_logprobs[row::4]).all() and torch.isnan(r.entropy[row::4]).all()
+
+
 GRAD_CASES = [
     (1, 9, 3, torch.float32, "random", "plain"),
     (3, 129, 20, torch.bfloat16, "random", "shifted"),

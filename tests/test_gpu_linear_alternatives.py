@@ -325,3 +325,14 @@ def test_saved_tensors_from_a_hook_are_looked_at_again():
                    lambda t: t[:-16] if t.dtype == torch.uint8 else t, lambda t: t[:5] if t.dim() == 2 and t.dtype == torch.float32 else t):
         with pytest.raises((RuntimeError, ValueError)):
             backward_with(unpack)
+
+
+@pytest.mark.parametrize("n,v,k", [(3, 500, 4), (300, 2000, 1), (300, 40000, 9)])
+def test_a_row_of_nan_has_valid_ids(n, v, k):
+    hid, w, lab = operands(n, 64, v, 4)
+    want = linear_top_logprobs(hid, w, k, lab)
+    hid[1] = math.nan
+    r = linear_top_logprobs(hid, w, k, lab)
+    assert torch.equal(r.top_ids[1], torch.arange(k, device="cuda")) and torch.isnan(r.top_logprobs[1]).all()
+    others = torch.arange(n, device="cuda") != 1
+    assert torch.equal(r.top_ids[others], want.top_ids[others]) and torch.equal(r.top_logprobs[others], want.top_logprobs[others])
