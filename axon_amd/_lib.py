@@ -147,7 +147,7 @@ SIGNATURES: dict[str, tuple] = {
                                         _ptr, _ptr, _f32, _i32, _ptr, _f32, _f32, _f32, _ptr, _ptr, _ptr]),
 }
 
-ABI_VERSION = 26
+ABI_VERSION = 27
 MASK_F32, MASK_I64 = 0, 1
 
 _lock = threading.Lock()

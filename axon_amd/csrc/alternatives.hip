@@ -110,16 +110,57 @@ __device__ __forceinline__ float tile_maxima(const float (&v)[4]) {
 }
 
 struct RowOut {
-  float *logprob, *entropy, *lse;  // logprob, entropy may be null
+  float *logprob, *entropy, *lse;  // logprob, entropy may be null; lse [2][n]
   const void* labels;              // may be null
-  int labels_i64;
+  int labels_i64, n;
 };
-// A row's log-sum-exp and entropy from its statistics.
-__device__ __forceinline__ float write_row(Stats st, int t, const RowOut& o) {
-  const float L = __log2f(st.s), d = st.e / st.s, lse = (st.M + L) * kLn2;
-  o.lse[t] = lse;
-  if (o.entropy != nullptr) o.entropy[t] = (L - d) * kLn2;
-  return lse;
+// A log-sum-exp and what its rounding to 32 bits has left of it: the log-probability of logit z is (z - lse) - rest.
+struct RowLse {
+  float lse, rest;
+  __device__ __forceinline__ float logprob(float z) const { return (z - lse) - rest; }
+};
+// Statistics whose largest logit is beyond this (in log2 units) do not give a log-probability: 32 bits of a log-sum-exp of
+// -1e9, which a mask has left nothing of, are multiples of 64, and the scaled statistics of the type's lowest value overflow.
+constexpr float kFarFromZero = 16384.f;
+__device__ __forceinline__ bool needs_care(const Stats& st) { return !(st.s > 0.f) || !(fabsf(st.M) < kFarFromZero); }
+
+// Log-sum-exp and entropy of such a row, and of one that has NaN or infinite logits or none but -inf: two passes over it, the
+// differences from the largest logit formed before they are scaled.  The result in thread 0.
+template <typename T>
+__device__ __forceinline__ RowLse careful_row(const T* row, int vocab, float& entropy, float (&red)[3][kBlock / kWave]) {
+  const RowSpan sp(row, vocab, true, 0, 1);
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+  auto each = [&](auto f) {
+    for (int q = tid; q < sp.n_vec; q += kBlock) {
+      float v[8];
+      Row<T>::template load<true>(row + sp.head + (uint32_t)q * Row<T>::kPer, v);
+#pragma unroll
+      for (int j = 0; j < Row<T>::kPer; ++j) f(v[j]);
+    }
+    for (int i = tid; i < sp.n_scalar; i += kBlock) f(Row<T>::one(row + sp.scalar<T>(i)));
+  };
+  float m = -INFINITY;
+  each([&](float z) { m = fmaxf(m, z); });
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+  if (lane == 0) red[0][wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float s = 0.f, e = 0.f;
+  each([&](float z) {
+    const float d = (z - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+    s += f;
+    e = fmaf(f, fmaxf(d, kTiny), e);
+  });
+  s = wave_sum(s);
+  e = wave_sum(e);
+  if (lane == 0) { red[1][wave] = s; red[2][wave] = e; }
+  __syncthreads();
+  s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  e = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  const float L = __log2f(s), lse = fmaf(L, kLn2, m);
+  entropy = (L - e / s) * kLn2;
+  return RowLse{lse, fmaf(L, kLn2, m - lse)};
 }
 
 struct Picks {
@@ -128,10 +169,10 @@ struct Picks {
   float* out;       // [n][k]
 };
 template <typename T>
-__device__ __forceinline__ void write_picks(const Picks& p, int t, const T* row, int vocab, float lse) {
+__device__ __forceinline__ void write_picks(const Picks& p, int t, const T* row, int vocab, RowLse lse) {
   for (int i = threadIdx.x; i < p.k; i += kBlock) {
     const int64_t id = load_id(p.ids, p.ids_i64, (int64_t)t * p.k + i);
-    p.out[(int64_t)t * p.k + i] = (id >= 0 && id < vocab) ? Row<T>::one(row + id) - lse : 0.f;
+    p.out[(int64_t)t * p.k + i] = (id >= 0 && id < vocab) ? lse.logprob(Row<T>::one(row + id)) : 0.f;
   }
 }
 
@@ -171,16 +212,34 @@ struct TopOut {
 // What is wanted of a row beside its statistics.
 enum Want { kTokens, kTop };
 
-// The end of a row: log-sum-exp and entropy from its statistics (in thread 0), then what is wanted of it.  HELD: how many
+// The end of a row: log-sum-exp and entropy from its statistics (in thread 0) or by looking again, then what is wanted of it.  HELD: how many
 // maxima a thread holds, 0 where they are in LDS.
 template <typename T, Want WANT, int HELD>
 __device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vocab, const float* seg_max, const RowOut& out,
                                            const Picks& picks, const TopOut& top, SelectLds* sel) {
-  __shared__ float s_lse;
+  __shared__ RowLse s_lse;
+  __shared__ float red[3][kBlock / kWave];
+  __shared__ int s_care;
   const int tid = threadIdx.x;
-  if (tid == 0) s_lse = write_row(st, t, out);
-  if (WANT == kTokens) {
+  auto write_row = [&](RowLse lse, float entropy) {
+    s_lse = lse;
+    out.lse[t] = lse.lse;
+    out.lse[(int64_t)out.n + t] = lse.rest;
+    if (out.entropy != nullptr) out.entropy[t] = entropy;
+  };
+  if (tid == 0) {
+    const float L = __log2f(st.s);
+    write_row({(st.M + L) * kLn2, 0.f}, (L - st.e / st.s) * kLn2);
+    s_care = needs_care(st);
+  }
+  __syncthreads();
+  if (s_care) {
+    float entropy;
+    const RowLse lse = careful_row<T>(row, vocab, entropy, red);
+    if (tid == 0) write_row(lse, entropy);
     __syncthreads();
+  }
+  if (WANT == kTokens) {
     write_picks<T>(picks, t, row, vocab, s_lse);
     return;
   }
@@ -189,13 +248,12 @@ __device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vo
   const int64_t lab = with_label ? load_id(out.labels, out.labels_i64, t) : -1;
   const bool inside = lab >= 0 && lab < vocab;
   const float label_z = inside ? Row<T>::one(row + lab) : 0.f;
-  // (the selection's own barriers come before the first use of s_lse)
   const LogitsSource<T, HELD> src{row, seg_max, SegSpan(row, vocab, 0, 1), vocab};
-  select_top<kBlock>(src, top.k, *sel, tid, [&](int rank, float z, int index) {
-    top.logprobs[(int64_t)t * top.k + rank] = z - s_lse;
+  select_top(src, top.k, *sel, tid, [&](int rank, float z, int index) {
+    top.logprobs[(int64_t)t * top.k + rank] = s_lse.logprob(z);
     top.ids[(int64_t)t * top.k + rank] = index;
   });
-  if (with_label) out.logprob[t] = inside ? label_z - s_lse : 0.f;
+  if (with_label) out.logprob[t] = inside ? s_lse.logprob(label_z) : 0.f;
 }
 
 // Workgroup (row, part): blockIdx.x = row * parts + part.  Where a row has one part it is finished here: a row's selection
@@ -307,7 +365,8 @@ struct TokenGrads {
 // the forward leaves them in the cache.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void tokens_grad_kernel(const T* logits, int64_t ld, int vocab, TokenGrads tg,
-                                                             const float* __restrict__ lse, const float* __restrict__ entropy,
+                                                             int n, const float* __restrict__ lse,
+                                                             const float* __restrict__ entropy,
                                                              const float* __restrict__ g_entropy, T* dlogits, int64_t ld_d,
                                                              int vec_ok, int parts) {
   constexpr int kMost = kMaxTokenIds + 1, kSlots = (kMost + kBlock - 1) / kBlock;
@@ -334,10 +393,11 @@ __global__ __launch_bounds__(kBlock) void tokens_grad_kernel(const T* logits, in
   if ((tid & (kWave - 1)) == 0) red[tid / kWave] = sum;
   __syncthreads();
   const float G = (red[0] + red[1]) + (red[2] + red[3]);
-  const float lse_v = lse[t], g_en = g_entropy ? g_entropy[t] : 0.f, H = g_entropy ? entropy[t] : 0.f;
-  auto grad = [&](float z) {
-    const float lp = z - lse_v, p = __expf(lp);
-    return p * ((p > 0.f) ? fmaf(-g_en, lp + H, -G) : -G);  // a probability of 0 takes nothing from the entropy
+  const float lse_v = lse[t], rest = lse[n + t], g_en = g_entropy ? g_entropy[t] : 0.f;
+  const float H = (g_entropy ? entropy[t] : 0.f) - rest, rest2 = rest * kLog2e;
+  auto grad = [&](float z) {  // log p = z - lse - rest
+    const float d = z - lse_v, p = __builtin_amdgcn_exp2f(fmaf(d, kLog2e, -rest2));
+    return p * ((p > 0.f) ? fmaf(-g_en, d + H, -G) : -G);  // a probability of 0 takes nothing from the entropy
   };
   const RowSpan sp(row, vocab, vec_ok != 0, part, parts);
   // the ids that are this part's, each in the thread of its first occurrence
@@ -437,7 +497,7 @@ int64_t top_lds(int dtype, int64_t vocab) { return (int64_t)sizeof(SelectLds) + 
 
 int check_rows(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v) {
   if (n < 0 || v <= 0 || ld < v || !dtype_ok(dtype)) return AXON_ERR_ARG;
-  if (n >= (int64_t)1 << 25 || v >= (int64_t)1 << 30) return AXON_ERR_SHAPE;  // rows times parts are a grid
+  if (n >= (int64_t)1 << 24 || v >= (int64_t)1 << 30) return AXON_ERR_SHAPE;  // rows times parts are a grid
   if (n > 0 && (!logits || reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) != 0)) return AXON_ERR_ARG;
   return AXON_OK;
 }
@@ -480,7 +540,7 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
   float* const seg_max = whole ? nullptr : workspace + n * parts * 3;
   const int stride = (int)seg_stride(dtype, vocab), from = cached_from(n, vocab, eb, bwd_follows);
   const unsigned lds = whole ? (unsigned)top_lds(dtype, vocab) : 0;
-  const RowOut out{logprob, entropy, lse, labels, labels_i64};
+  const RowOut out{logprob, entropy, lse, labels, labels_i64, (int)n};
   const TopOut top{top_logprobs, top_ids, (int)k};
 #define AXON_TOP(T)                                                                                                        \
   do {                                                                                                                     \
@@ -516,7 +576,7 @@ extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld,
   const int64_t need = axon_logits_tokens_workspace_bytes(dtype, n, vocab);
   if (need > 0 && (!workspace || need > workspace_bytes)) return AXON_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
-  const RowOut out{nullptr, entropy, lse, nullptr, 0};
+  const RowOut out{nullptr, entropy, lse, nullptr, 0, (int)n};
   const Picks picks{ids, ids_i64, (int)k, logprobs};
   const int from = cached_from(n, vocab, eb, bwd_follows);
 #define AXON_TOKENS(T)                                                                                                      \
@@ -553,7 +613,7 @@ extern "C" int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld,
   const TokenGrads tg{ids, g_ids, labels, g_label, ids_i64, (int)k, labels_i64};
 #define AXON_GRAD(T)                                                                                                       \
   hipLaunchKernelGGL((tokens_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st,                             \
-                     static_cast<const T*>(logits), ld, (int)vocab, tg, lse, entropy, g_entropy, static_cast<T*>(dlogits), \
+                     static_cast<const T*>(logits), ld, (int)vocab, tg, (int)n, lse, entropy, g_entropy, static_cast<T*>(dlogits), \
                      ld_d, vec_ok, parts)
   AXON_ROWS(dtype, AXON_GRAD);
 #undef AXON_GRAD

@@ -154,14 +154,14 @@ template <int G, int V, int SCORE>
 __device__ __forceinline__ float scores(const float (&x)[V], float (&w)[V], float (&rest)[V]) {
   constexpr float kLog2e = 1.4426950408889634f;
   float sum = 0.f;
-  if (SCORE == kSoftmax) {
+  if constexpr (SCORE == kSoftmax) {
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) m = fmaxf(m, x[j]);
     m = row_reduce<G>(m, MaxF());
-    const float ml = m * kLog2e;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += w[j] = __builtin_amdgcn_exp2f(fmaf(x[j], kLog2e, -ml));
+    for (int j = 0; j < V; ++j) sum += w[j] = __builtin_amdgcn_exp2f((x[j] - m) * kLog2e);  // m * log2(e) may overflow
+    return __builtin_amdgcn_rcpf(row_reduce<G>(sum, Add()));
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -169,8 +169,18 @@ __device__ __forceinline__ float scores(const float (&x)[V], float (&w)[V], floa
       sum += w[j] = __builtin_amdgcn_rcpf(1.f + ex);
       rest[j] = x[j] > 0.f ? ex * w[j] : 1.f - w[j];
     }
+    sum = row_reduce<G>(sum, Add());
+    // rows whose sigmoids are all next to nothing: there they are exponentials, to a relative 2^-90, and their ratios a softmax
+    const bool tiny = sum < 0x1p-90f;
+    if (__builtin_amdgcn_ballot_w64(tiny) != 0) {
+      float s[V], unused[V];
+      const float inv = scores<G, V, kSoftmax>(x, s, unused);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = tiny ? s[j] : w[j];
+      return tiny ? inv : __builtin_amdgcn_rcpf(sum);
+    }
+    return __builtin_amdgcn_rcpf(sum);
   }
-  return __builtin_amdgcn_rcpf(row_reduce<G>(sum, Add()));
 }
 
 // Keys in descending order (Batcher's odd-even merge sort: 19 exchanges for eight).

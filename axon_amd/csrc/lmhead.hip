@@ -451,7 +451,6 @@ __global__ __launch_bounds__(256) void seq_start_kernel(const int32_t* __restric
   is_start[v] = bits;
 }
 
-// `labels` and `logprobs` may both be null: no label's logit is wanted.
 // The last kernel of the forward: folds a token's partials into lse, entropy_b and entropy, forms the label's logit
 // and with it logprob[n] = softcap(hidden[n] . W[label[n]]) / T - lse[n].
 // A token's partials are folded in 256 groups, group c taking c, c + 256, ... (a chain of five for 151936 vocabulary
@@ -462,7 +461,7 @@ __global__ __launch_bounds__(256) void seq_start_kernel(const int32_t* __restric
 // PER = 2 once a workgroup per 16 tokens would be more than one per CU.  The label dots (one wavefront per token) run
 // before the barrier, beside the folds of the other wavefronts. 187 tokens x 896 x 151936 5.9 us (11.0 with three
 // arrays of partials, 64 groups and 16 tokens per workgroup), 700 x 4096 11.9 (19.0), 1500 x 896 9.8 (12.8), 3001 x
-// 2880 x 201088 22.5 (31.4), 8192 x 4096 41.4 (49.0).
+// 2880 x 201088 22.5 (31.4), 8192 x 4096 41.4 (49.0).  `labels` and `logprobs` are null where no label's logit is wanted.
 template <int T, int PER, typename LabelT>
 __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
     const float* __restrict__ stats, int parts, const __bf16* __restrict__ hidden, const __bf16* __restrict__ weight,
@@ -1097,11 +1096,11 @@ __global__ __launch_bounds__(kBlock) void lmhead_top_kernel(TopParams p) {
   if (p.staged) {
     src.maxima = staged;
     src.stride = 1;
-    select_top<kBlock>(src, p.k, sel, tid, out);
+    select_top(src, p.k, sel, tid, out);
   } else {
     src.maxima = p.pm + n;
     src.stride = p.n_tokens;
-    select_top<kBlock>(src, p.k, sel, tid, out);
+    select_top(src, p.k, sel, tid, out);
   }
 }
 
@@ -1192,7 +1191,7 @@ __global__ __launch_bounds__(256) void token_dlogits_kernel(DlogitParams p, Toke
     ids[wave][i] = (id >= 0 && id < p.vocab) ? (int)id : -1;
     gs[wave][i] = a.g[at];
   }
-  group_sync<kWave>();
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wavefront's own entries, in order
   const float G = p.dlogprobs[n], g_en = p.dentropy ? p.dentropy[n] : 0.f, lse = p.lse[n], mean = p.entropy_b[n];
   for (int i = lane; i < a.k; i += 64) {
     const int id = ids[wave][i];

@@ -39,12 +39,7 @@ struct SelectLds {
   int n_segs, n_cand, bin, before, upto;
 };
 
-// NT threads work on a row: a wavefront (64), whose LDS accesses are carried out in order, or a workgroup.
-template <int NT>
-__device__ __forceinline__ void group_sync() {
-  if constexpr (NT == kWave) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  else __syncthreads();
-}
+constexpr int NT = kBlock;  // threads that work on a row: a workgroup
 
 // Permutations by DPP in which every lane has a source, and the sums up to a lane, whose missing sources are 0.
 template <int CTRL>
@@ -73,30 +68,28 @@ __device__ __forceinline__ int wave_upto(int v) {
 }
 
 // Smallest and largest over the threads.
-template <int NT>
 __device__ __forceinline__ void group_range(SelectLds& s, int tid, uint32_t& lo, uint32_t& hi) {
   lo = ~wave_max_u32(~lo);
   hi = wave_max_u32(hi);
-  if (NT == kWave) return;
   if ((tid & (kWave - 1)) == 0) { s.range[0][tid / kWave] = lo; s.range[1][tid / kWave] = hi; }
-  group_sync<NT>();
+  __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / kWave; ++w) { lo = min(lo, s.range[0][w]); hi = max(hi, s.range[1][w]); }
 }
 // The k-th largest of n keys (1 <= k <= n), eight bits at a time; `ties`: how many of the keys equal to it are among
 // the k.  key_at(i) is asked for every i once per eight bits.
-template <int NT, class Key, class KeyAt>
+template <class Key, class KeyAt>
 __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds& s, int tid, int& ties) {
   Key prefix = 0, mask = 0;
   int rest = k;
   for (int shift = 8 * (int)sizeof(Key) - 8; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
-    group_sync<NT>();
+    __syncthreads();
     for (int i = tid; i < n; i += NT) {
       const Key key = key_at(i);
       if ((key & mask) == prefix) atomicAdd(&s.hist[(int)(key >> shift) & 255], 1);
     }
-    group_sync<NT>();
+    __syncthreads();
     if (tid < kWave) {  // lane l: bins 255 - 4 l and the three below
       int c[4], sum = 0;
 #pragma unroll
@@ -108,7 +101,7 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
         before += c[q];
       }
     }
-    group_sync<NT>();
+    __syncthreads();
     prefix |= (Key)s.bin << shift;
     mask |= (Key)255 << shift;
     rest -= s.before;
@@ -120,7 +113,7 @@ __device__ __forceinline__ Key kth_largest(KeyAt key_at, int n, int k, SelectLds
 // A row's keys in the threads' registers, up to NT * Src::kHeld of them, requested together: where they are in memory, a loop
 // that asks for one at a time is a trip there each, and there are three such loops.  More are asked for again wherever they are
 // needed, as are those in LDS, which a loop reads faster than code for every number of them runs.
-template <int NT, class Src>
+template <class Src>
 struct HeldKeys {
   static constexpr int kHeld = Src::kHeld;
   const Src& src;
@@ -147,27 +140,27 @@ struct HeldKeys {
 // The segments that are looked at, to s.segs: those whose maximum reaches a bound (returned) that at least k maxima reach.
 // The keys' range is cut into 256 bins and the bin of the k-th taken whole if that makes at most a quarter more; else
 // the bin is cut again, down to one key, of whose segments the first are taken then.  A row of a model's logits takes one cut.
-template <int NT, class Src>
+template <class Src>
 __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k, SelectLds& s, int tid) {
   const int most = k + k / 4 + 8;
-  const HeldKeys<NT, Src> keys(src, n, tid);
+  const HeldKeys<Src> keys(src, n, tid);
   uint32_t lo = 0xffffffffu, hi = 0;
   keys.each([&](int, uint32_t key) {
     lo = min(lo, key);
     hi = max(hi, key);
   });
-  group_range<NT>(s, tid, lo, hi);
+  group_range(s, tid, lo, hi);
   int rest = k, above = 0;  // of the segments in the range, `rest` are wanted; `above`: segments above the range
   uint32_t least;
   for (uint32_t width = hi - lo;;) {  // the range: lo .. lo + width
     const int shift = width < 256 ? 0 : 24 - __builtin_clz(width);
     for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
-    group_sync<NT>();
+    __syncthreads();
     keys.each([&](int, uint32_t key) {
       const uint32_t at = key - lo;
       if (at <= width) atomicAdd(&s.hist[at >> shift], 1);
     });
-    group_sync<NT>();
+    __syncthreads();
     if (tid < kWave) {  // lane l: bins 255 - 4 l and the three below
       int c[4], sum = 0;
 #pragma unroll
@@ -179,7 +172,7 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
         before += c[q];
       }
     }
-    group_sync<NT>();
+    __syncthreads();
     least = lo + ((uint32_t)s.bin << shift);
     if (above + s.upto <= most || shift == 0) break;
     above += s.before;
@@ -197,7 +190,7 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
   const int ties = rest - s.before;  // at a bin of one key: how many of its segments are wanted
   int one;
   auto first = [&](int i) { return src.max_key(i) == least ? 0xffffffffu - (uint32_t)i : 0u; };
-  const uint32_t last = kth_largest<NT, uint32_t>(first, n, ties, s, tid, one);
+  const uint32_t last = kth_largest<uint32_t>(first, n, ties, s, tid, one);
   keys.each([&](int i, uint32_t key) {
     if (key > least || (key == least && 0xffffffffu - (uint32_t)i >= last)) s.segs[atomicAdd(&s.n_segs, 1)] = i;
   });
@@ -207,17 +200,17 @@ __device__ __forceinline__ uint32_t choose_segments(const Src& src, int n, int k
 // `src`: maxima of its segments, max_key(i) for i < n_segs() (kHeld: see HeldKeys); the elements of the segments in `segs`, kPer consecutive ones
 // per item: load(segs, j, v) returns the index of the first, or -1 where there is none (elements from limit() on do not
 // count); and n_single() elements outside all segments, single(i, index).  out(rank, value, index) for rank < k.
-template <int NT, class Src, class Out>
+template <class Src, class Out>
 __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, int tid, Out out) {
   const int n = src.n_segs();
   uint32_t least = 0;  // what an element has to reach
   if (tid == 0) s.n_segs = s.n_cand = s.n_hits = 0;
   if (n > k) {
-    least = choose_segments<NT>(src, n, k, s, tid);
+    least = choose_segments(src, n, k, s, tid);
   } else {
     for (int i = tid; i < n; i += NT) s.segs[i] = i;
   }
-  group_sync<NT>();
+  __syncthreads();
   const int n_items = (n > k ? s.n_segs : n) * Src::kItems, limit = src.limit();
   auto offer = [&](float x, int index) {
     if (order_key(x) < least) return;
@@ -257,7 +250,7 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
       }
     }
   }
-  group_sync<NT>();
+  __syncthreads();
   // few items hold a candidate: their elements one per thread (all elements of every item: eight times the instructions in each
   // wavefront that has one)
   for (int i = tid, n_el = min(s.n_hits, kHits) * Src::kPer; i < n_el; i += NT) {
@@ -269,7 +262,7 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     const float x = src.single(i, index);
     offer(x, index);
   }
-  group_sync<NT>();
+  __syncthreads();
   int c = s.n_cand;
   if (c > kCandidates) {  // a run of equal values, as a rule: the k-th key itself, from the elements of the segments
     const int n_el = n_items * Src::kPer + src.n_single();
@@ -288,14 +281,14 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
       return order_key(x, i0 + e);
     };
     int one;
-    const uint64_t last = kth_largest<NT, uint64_t>(element, n_el, k, s, tid, one);
+    const uint64_t last = kth_largest<uint64_t>(element, n_el, k, s, tid, one);
     if (tid == 0) s.n_cand = 0;
-    group_sync<NT>();
+    __syncthreads();
     for (int i = tid; i < n_el; i += NT) {
       const uint64_t key = element(i);
       if (key >= last) s.cand[atomicAdd(&s.n_cand, 1)] = key;
     }
-    group_sync<NT>();
+    __syncthreads();
     c = k;
   }
   // Ranks.  Few candidates are each compared with all; more are first put in order of 256 bins of their range, and compared
@@ -305,7 +298,7 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
   };
   if (c <= kWave) {
     if (tid == 0) s.cand[c] = 0;  // to a whole number of pairs
-    group_sync<NT>();
+    __syncthreads();
     if (tid < c) {
       const uint64_t mine = s.cand[tid];
       int rank = 0;
@@ -324,10 +317,10 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     lo = min(lo, key);
     hi = max(hi, key);
   }
-  group_range<NT>(s, tid, lo, hi);
+  group_range(s, tid, lo, hi);
   const int shift = hi - lo < 256 ? 0 : 24 - __builtin_clz(hi - lo);
   for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
-  group_sync<NT>();
+  __syncthreads();
   // a candidate's bin, and its number among those of the bin that came before it
   constexpr int kSlots = kCandidates / NT;
   uint64_t mine[kSlots];
@@ -340,7 +333,7 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
     bin[u] = ((uint32_t)(mine[u] >> 32) - lo) >> shift;
     nth[u] = atomicAdd(&s.hist[bin[u]], 1);
   }
-  group_sync<NT>();
+  __syncthreads();
   if (tid < kWave) {  // hist[b]: how many lie in higher bins; lane l has bins 255 - 4 l and the three below
     int n4[4], sum = 0;
 #pragma unroll
@@ -352,13 +345,13 @@ __device__ __forceinline__ void select_top(const Src& src, int k, SelectLds& s, 
       before += n4[q];
     }
   }
-  group_sync<NT>();
+  __syncthreads();
 #pragma unroll
   for (int u = 0; u < kSlots; ++u) {
     if (u * NT >= c) break;
     if (tid + u * NT < c) s.cand[s.hist[bin[u]] + nth[u]] = mine[u];
   }
-  group_sync<NT>();
+  __syncthreads();
 #pragma unroll
   for (int u = 0; u < kSlots; ++u) {
     if (u * NT >= c) break;

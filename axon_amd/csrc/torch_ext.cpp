@@ -457,6 +457,11 @@ void same_place(const char* what, const Tensor& like, std::initializer_list<cons
   }
 }
 
+void same_type(const char* what, at::ScalarType type, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->scalar_type() != type) refuse(what, "a saved tensor has come back in another type");
+}
+
 // A gradient that cannot be differentiated again says so, instead of being a constant.
 Tensor once(Tensor grad, const char* what) {
   if (!at::GradMode::is_enabled()) return grad;
@@ -492,7 +497,9 @@ struct AlternativesNode : torch::autograd::Node {
     const int dtype = logits_dtype(kWhat, x);
     const int64_t n = x.size(0), v = x.size(1), k = at.size(1);
     if (x.stride(1) != 1 || (n > 1 && x.stride(0) < v)) refuse(kWhat, "logits must be [tokens, vocab] with unit stride over the vocabulary");
-    same_len(kWhat, "lse", n, l);
+    same_type(kWhat, at::kFloat, {&l, &ent});
+    if (!is_index(at) || (lab.defined() && !is_index(lab))) refuse(kWhat, "a saved tensor has come back in another type");
+    same_len(kWhat, "lse", 2 * n, l);
     same_len(kWhat, "entropy", n, ent);
     same_len(kWhat, "ids", n * k, at);
     if (g_en.defined()) same_len(kWhat, "g_entropy", n, g_en);
@@ -551,7 +558,7 @@ std::tuple<OptTensor, Tensor, Tensor, Tensor> alternatives(const char* what, con
     wide.push_back(k);
     entropy = at::empty(batch, opts(rows));
     lp = at::empty(wide, opts(rows));
-    lse = at::empty({n}, opts(rows));
+    lse = at::empty({2, n}, opts(rows));
     if (lab.defined()) label_lp = at::empty(batch, opts(rows));
     const int64_t need = ids_in ? axon_logits_tokens_workspace_bytes(dtype, n, v) : axon_logits_top_workspace_bytes(dtype, n, v);
     const Tensor ws = need > 0 ? at::empty({need / 4}, opts(rows)) : Tensor();
@@ -640,6 +647,9 @@ struct RouterBalanceNode : torch::autograd::Node {
       same_place(kWhat, x[0], {&m, &offsets, &c, &sc, &up});
       const RouterRows r = router_rows(kWhat, x);
       const int64_t layers = (int64_t)x.size(), seqs = offsets.defined() ? offsets.numel() - 1 : 1;
+      same_type(kWhat, at::kFloat, {&c, &sc});
+      same_type(kWhat, at::kInt, {&offsets});
+      same_type(kWhat, mask_kind == AXON_MASK_I64 ? at::kLong : at::kFloat, {&m});
       same_len(kWhat, "coefficients", seqs * layers * r.experts, c);
       same_len(kWhat, "upstream gradient", 1, up);
       same_len(kWhat, "scale", 1, sc);

@@ -174,6 +174,60 @@ def test_ids_are_valid_whatever_the_row_holds(v, dtype, k):
             assert torch.isnan(r.top_logprobs[row::4]).all() and torch.isnan(r.entropy[row::4]).all()
 
 
+def test_signaling_nan_hides_nothing():
+    """A NaN of any bits beside a row's largest logit."""
+    for dtype, ints, bits in ((torch.float32, torch.int32, 0x7f800001), (torch.bfloat16, torch.int16, 0x7f81)):
+        z = torch.randn(4, 6000, generator=gen(2), device="cuda").to(dtype)
+        z[:, 2048] = 30.0
+        for row, at in enumerate((2047, 2049, 2055, 2060)):
+            z[row, at] = torch.tensor(bits, dtype=ints, device="cuda").view(dtype)
+        clean = torch.where(torch.isnan(z), torch.tensor(-math.inf, dtype=dtype, device="cuda"), z)
+        for many in (1, 150):
+            r = top_logprobs_from_logits(z.repeat(many, 1), 5)
+            assert (r.top_ids.view(many, 4, 5) == order(clean, 5)).all() and torch.isnan(r.top_logprobs).all()
+
+
+def far_rows(v, dtype, g):
+    """Rows whose log-sum-exp is far from 0: what a mask of a large number or of the type's lowest has left nothing of."""
+    lowest = torch.finfo(dtype).min
+    z = torch.randn(9, v, generator=g, device="cuda") * 3
+    z[0] = -1e9
+    z[1] = lowest
+    z[2] = z[2] * 1000 - 1e9
+    z[3] += 20000
+    z[4] -= 60000
+    z[5, : v // 2] = lowest  # a mask that leaves something
+    z[6] = lowest
+    z[6, v // 2] = -1e33
+    z[7] = torch.finfo(dtype).max
+    z[8] = -3e30
+    z[8, ::2] = lowest
+    return z.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [12, 3001, 151936])
+def test_rows_far_from_zero(v, dtype):
+    """A log-probability is off by LP_TOL and two roundings of its own size (the difference from the log-sum-exp, and what is
+    left of that): the sums of such a row go in chains of at most 600 (3.5e-5), its final additions are of numbers up to 12."""
+    g = gen(v)
+    z, k = far_rows(v, dtype, g), 5
+    for many in (1, 60):  # rows that several workgroups share, and rows that one finishes
+        x = z.repeat(many, 1).requires_grad_(True)
+        ids = torch.cat([order(z, k), torch.randint(0, v, (9, 3), generator=g, device="cuda")], 1).repeat(many, 1)
+        g_ids, g_en = torch.randn(9 * many, 8, generator=g, device="cuda"), torch.randn(9 * many, generator=g, device="cuda")
+        lp, ent, ref, size = reference(x.detach(), ids, g_ids, g_en)
+        r = top_logprobs_from_logits(x, k, ids[:, 6])
+        assert torch.equal(r.top_ids, ids[:, :k])
+        got_lp, got_ent = token_logprobs_from_logits(x, ids)
+        for got, want in ((r.top_logprobs, lp[:, :k]), (r.logprobs, lp[:, 6]), (got_lp, lp)):
+            assert ((got.double() - want).abs() <= LP_TOL + 2.0 ** -23 * want.abs()).all()
+        for got in (r.entropy, got_ent):
+            assert (got.double() - ent).abs().max() <= ENT_TOL
+        grad, = torch.autograd.grad([got_lp, got_ent], x, [g_ids, g_en])
+        check_grad(grad, ref, size, dtype)
+
+
 GRAD_CASES = [
     (1, 9, 3, torch.float32, "random", "plain"),
     (3, 129, 20, torch.bfloat16, "random", "shifted"),
