@@ -58,7 +58,11 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
     if args.get("router_balance_per_sequence", False):
         seqs = cu
         if seqs is None:  # padded: a row is a sequence
-            rows, length = entropy.shape
+            rows, one = entropy.shape[0], router_logits[0]  # a layer, where there are several
+            tokens = (one.numel() // one.shape[-1] if one.dim() > 1 else router_logits.shape[0])
+            length, odd = divmod(tokens, rows)
+            if odd:
+                raise ValueError(f"router_logits of {tokens} tokens do not belong to {rows} rows of one length")
             seqs = torch.arange(rows + 1, device=entropy.device, dtype=torch.int32) * length
     balance, counts = router_balance_loss(router_logits, args["router_top_k"], token_mask=mask, cu_seqlens=seqs,
                                           expert_ids=router_expert_ids, score_fn=args.get("router_score_fn", "softmax"))
@@ -70,8 +74,10 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
 def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, router_expert_ids=None):
     """Everything of ``forward_backward_fn`` after the model forward (fsdp_models.py:224-278).
 
-    With ``loss_fn_args["router_aux_loss_coef"]`` the balance loss of ``router_logits`` times that coefficient is added, with
-    ``router_top_k``, ``router_score_fn`` ("softmax") and ``router_balance_per_sequence`` (False) from the same arguments.
+    With ``loss_fn_args["router_aux_loss_coef"]`` the balance loss of ``router_logits`` times that coefficient is added, as
+    the mean over the micro-batches of a step and the data-parallel replicas (the other terms are their sums: they are
+    divided by counts over all of these), with ``router_top_k``, ``router_score_fn`` ("softmax") and
+    ``router_balance_per_sequence`` (False) from the same arguments.
 
     Returns ``(scaled_loss, metrics)``.  ``data.batch["log_probs"]`` is set; ``response_mask`` may be
     overwritten by the sampler correction hook, while the side terms keep the mask they were given
@@ -128,7 +134,7 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
     router_vals = []
     if router_coef != 0:
         balance, load = _router_term(b, cu, entropy, loss_fn_args, router_logits, router_expert_ids)
-        loss = loss + balance * router_coef
+        loss = loss + balance * (router_coef / (n_micro_batches * dp_replicas))
         router_vals = [balance.detach(), load]
     # one readback for pg_loss and the side-term metrics
     vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4], *router_vals]).tolist()
@@ -139,7 +145,7 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
         metrics["kl_loss"] = vals[2] * n_micro_batches
         metrics["kl_coef"] = kl_coef
     if router_vals:
-        metrics["router_balance_loss"] = vals[5] * n_micro_batches
+        metrics["router_balance_loss"] = vals[5]
         metrics["router_max_load"] = vals[6]
         metrics["router_aux_loss_coef"] = router_coef
     return loss * dp_replicas, metrics
