@@ -3,7 +3,10 @@
 // one: dz_j = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_H (log p_j + H)).
 //
 // Forward: ONE read of the row gives the softmax statistics and, for the k largest, the maxima of the row's segments of
-// 256 bytes, from which select.h finds the few segments that are read again.  Bound by memory.
+// 256 bytes, from which select.h finds the few segments that are read again.  Bound by memory: 4096 x 151936 bf16 with 20
+// alternatives and a label 209 us, 5.9 TB/s (a large device copy 4.8 to 5.0, read and write); 1500 x 151936 fp32 with 32 given
+// tokens 144 us, 6.3 TB/s.  Short batches are bound by the two launches' latency: one row of 151936 5.3 + 7.5 us, of which the
+// selection's trips to memory are most.
 #include "logits_rows.h"
 #include "select.h"
 #include <type_traits>
@@ -125,7 +128,8 @@ constexpr float kFarFromZero = 16384.f;
 __device__ __forceinline__ bool needs_care(const Stats& st) { return !(st.s > 0.f) || !(fabsf(st.M) < kFarFromZero); }
 
 // Log-sum-exp and entropy of such a row, and of one that has NaN or infinite logits or none but -inf: two passes over it, the
-// differences from the largest logit formed before they are scaled.  The result in thread 0.
+// differences from the largest logit formed before they are scaled.  64 rows of 151936, finished by a workgroup each: 88 us, where
+// other rows take 8.  The result in thread 0.
 template <typename T>
 __device__ __forceinline__ RowLse careful_row(const T* row, int vocab, float& entropy, float (&red)[3][kBlock / kWave]) {
   const RowSpan sp(row, vocab, true, 0, 1);
@@ -362,7 +366,8 @@ struct TokenGrads {
 // The row is streamed without a look at the ids; the few elements that have one are written again afterwards, from
 // logits that were read before (dlogits may be the logits' own storage).  Equal ids of a row add up in their order, in the
 // thread of the first of them, so that the result repeats bit for bit.  Rows are walked from the last to the first, as
-// the forward leaves them in the cache.
+// the forward leaves them in the cache.  Bound by memory: 1500 x 151936 fp32 360 us, 5.1 TB/s read and written; 2047 x 50257
+// bf16, rows on every boundary, 83 us, 5.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void tokens_grad_kernel(const T* logits, int64_t ld, int vocab, TokenGrads tg,
                                                              int n, const float* __restrict__ lse,

@@ -289,6 +289,9 @@ __device__ __forceinline__ void each_run(const BalanceParams& p, int c0, int c1,
   }
 }
 
+// Workgroup (chunk, layer).  48 layers x 8192 x 128 bf16, 8 choices: 61 us, where one read of the logits is 21: bound by
+// instructions, those of the choices (a sort of a lane's eight keys, then eight times the largest head of sixteen lanes): with
+// given choices it is 27 us.
 template <typename T, int G, int V, int SCORE, int MASK>
 __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, LayerPtrs logits, LayerPtrs ids) {
   constexpr int kRows = kBlock / G, kE = G * V;
@@ -356,8 +359,8 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(BalanceParams p, La
 
 // Workgroup (sequence, layer): adds its partials, leaves E / (k T^2) c per expert for the backward, the loads and the
 // sequence's loss.  The workgroup that draws the last ticket adds the losses, in a fixed order, to the mean over the sequences
-// that have tokens and the layers.  Up to 256 experts the chunks are shared by groups of threads (one load at a time and
-// thread, and a launch for the mean: 48 x 8192 x 128 18 us).
+// that have tokens and the layers.  Up to 256 experts the chunks are shared by groups of threads: 48 x
+// 8192 x 128 7 us (one load at a time and thread, and a launch for the mean: 18).
 __global__ __launch_bounds__(kBlock) void balance_sum_kernel(BalanceParams p, float* __restrict__ coef, double* __restrict__ losses,
                                                              int* __restrict__ tokens, float* __restrict__ loss,
                                                              float* __restrict__ scale) {
@@ -427,6 +430,8 @@ __global__ __launch_bounds__(kBlock) void balance_sum_kernel(BalanceParams p, fl
   *scale = (float)s;
 }
 
+// The gradient, a row in the lanes that had it in the forward; nothing but the coefficients is kept from there.  48 x 8192 x 128
+// bf16 38 us, 5.3 TB/s read and written: memory.
 template <typename T, int G, int V, int SCORE, int MASK>
 __global__ __launch_bounds__(kBlock) void balance_bwd_kernel(BalanceParams p, LayerPtrs logits, LayerPtrs grads) {
   constexpr int kRows = kBlock / G;

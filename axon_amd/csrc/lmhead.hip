@@ -1065,7 +1065,8 @@ struct TopParams {
 
 // A workgroup per token.  The maxima of sixteen neighbouring tokens lie in the same cache lines: their workgroups are given to
 // one XCD (workgroups go round the eight of them), where all but the first find them in its L2.  A wavefront per token and
-// four tokens per workgroup, with the maxima in LDS: 8 x 151936, 20 alternatives, 31 us, 4096 x 151936 128 us.
+// four tokens per workgroup, with the maxima in LDS: 8 x 151936, 20 alternatives, 31 us, 4096 x 151936 128 us; this way 11 and
+// 98, the latency of a token's few trips to memory, and the 5 KB of maxima that each of them reads.
 constexpr int kXcds = 8, kNeighbours = 16;
 __global__ __launch_bounds__(kBlock) void lmhead_top_kernel(TopParams p) {
   extern __shared__ __align__(16) char smem[];
@@ -1115,6 +1116,8 @@ struct TokenArgs {
 };
 
 // logprobs[n][i] = softcap(hidden[n] . W[ids[n][i]]) / T - lse[n]: a workgroup per token, a wavefront per id.
+// Bound by the rows of the weight that it gathers: 1001 x 64 ids, hidden 896, 27 us, 4.2 TB/s; 4096 x 20, hidden 4096, 118 us,
+// 5.7 TB/s.
 __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restrict__ hidden, const __bf16* __restrict__ weight,
                                                            int hidden_sz, int vocab, TokenArgs a, float inv_temp, float cap,
                                                            const float* __restrict__ lse) {
@@ -1144,7 +1147,7 @@ __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restr
   }
 }
 
-// The same from kept logits: a thread per id.
+// The same from kept logits: a thread per id.  1001 x 64 ids 6 us, a scattered read of four bytes each.
 __global__ __launch_bounds__(256) void token_picks_kernel(const float4* __restrict__ tiles, int tiles_n, int64_t n_ids, int vocab,
                                                           TokenArgs a, float inv_temp, float cap, const float* __restrict__ lse) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -1176,7 +1179,8 @@ __global__ __launch_bounds__(256) void token_grad_sum_kernel(TokenArgs a, int n_
   if (lane == 0) sums[n] = sum;
 }
 
-// The dlogits of the ids of a vocabulary chunk, over what was formed there as if no token had one:
+// The dlogits of the ids of a vocabulary chunk, over what was formed there as if no token had one (1001 x
+// 64 ids 13 to 18 us, 2500 x 16 9 us):
 //   dl = (sum of the gradients of this id - p (G + g_H (z - E[z]))) / T * (1 - (capped logit / cap)^2)
 // rounded once, as those around it.  A wavefront per token; equal ids of a token add up in their order, in the lane of the
 // first of them.
