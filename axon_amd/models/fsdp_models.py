@@ -60,7 +60,7 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
         if seqs is None:  # padded: a row is a sequence
             rows, one = entropy.shape[0], router_logits[0]  # a layer, where there are several
             tokens = (one.numel() // one.shape[-1] if one.dim() > 1 else router_logits.shape[0])
-            length, odd = divmod(tokens, rows)
+            length, odd = divmod(tokens, max(rows, 1))
             if odd:
                 raise ValueError(f"router_logits of {tokens} tokens do not belong to {rows} rows of one length")
             seqs = torch.arange(rows + 1, device=entropy.device, dtype=torch.int32) * length

@@ -228,6 +228,49 @@ def test_rows_far_from_zero(v, dtype):
         check_grad(grad, ref, size, dtype)
 
 
+def test_rows_whose_maxima_do_not_fit_in_lds():
+    """700001 fp32 logits are 10938 segments: rows that a workgroup would finish are finished by a second launch."""
+    z = logits_of("random", 8, 700001, torch.float32, 6)
+    z[3] = 1.0
+    r = top_logprobs_from_logits(z.repeat(65, 1), 40)
+    assert (r.top_ids.view(65, 8, 40) == order(z, 40)).all()
+    few = top_logprobs_from_logits(z, 40)
+    lp, ent = reference(z, order(z, 40))
+    # chains of 700001 / 256 roundings
+    for got, entropy in ((r.top_logprobs[-8:], r.entropy[-8:]), (few.top_logprobs, few.entropy)):
+        assert (got.double() - lp).abs().max() <= LP_TOL + 2735 * 2.0 ** -24
+        assert (entropy.double() - ent).abs().max() <= ENT_TOL + 14 * 2735 * 2.0 ** -24
+
+
+def test_logits_written_to_before_the_backward_are_noticed():
+    z = logits_of("random", 4, 300, torch.float32, 2)
+    for op in (lambda x: top_logprobs_from_logits(x, 3).top_logprobs, lambda x: token_logprobs_from_logits(x, torch.zeros(4, 1, dtype=torch.int64, device="cuda"))[0]):
+        x = z.clone().requires_grad_(True) * 1
+        out = op(x)
+        with torch.no_grad():
+            x += 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    z = logits_of("random", 3, 1000, torch.bfloat16, 1)
+    buf = torch.empty(2 ** 31 + 5000, dtype=torch.bfloat16, device="cuda")
+    far = buf.as_strided((3, 1000), (2 ** 30 + 8, 1))
+    far.copy_(z)
+    ids = torch.randint(0, 1000, (3, 6), generator=gen(1), device="cuda")
+    g = torch.randn(3, 6, generator=gen(2), device="cuda")
+    results = []
+    for x in (z.clone(), far):
+        x = x.detach().requires_grad_(True)
+        r = top_logprobs_from_logits(x, 9, ids[:, 0])
+        lp, ent = token_logprobs_from_logits(x, ids, inplace_backward=True)
+        grad, = torch.autograd.grad([lp, ent], x, [g, g[:, 0].clone()])
+        assert grad.data_ptr() == x.data_ptr()
+        results.append([r.top_ids, r.top_logprobs.detach(), r.logprobs.detach(), lp.detach(), ent.detach(), grad.clone()])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 GRAD_CASES = [
     (1, 9, 3, torch.float32, "random", "plain"),
     (3, 129, 20, torch.bfloat16, "random", "shifted"),

@@ -315,6 +315,14 @@ def test_rows_far_from_zero(e, dtype):
     check([y.to(dtype)], k, score="sigmoid")
 
 
+def test_offsets_beyond_32_bits():
+    xs, _, _ = case(1, 3, 16, 2, torch.bfloat16, 5)
+    buf = torch.empty(2 ** 31 + 5000, dtype=torch.bfloat16, device="cuda")
+    far = buf.as_strided((3, 16), (2 ** 30 + 8, 1))
+    far.copy_(xs[0])
+    check([far.detach()], 2)
+
+
 def test_a_saved_tensor_of_another_type_is_refused():
     xs, m, _ = case(2, 30, 16, 2, torch.float32, 3, torch.int64)
     leaves = [x.clone().requires_grad_(True) for x in xs]
