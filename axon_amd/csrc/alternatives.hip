@@ -53,7 +53,7 @@ __device__ __forceinline__ void fold_all(Stats& a, const float (&z)[U][M], const
     a.s = a.s * f;
     a.M = m;
   }
-  float s4[4] = {a.s, 0.f, 0.f, 0.f}, e4[4] = {a.e, 0.f, 0.f, 0.f};
+  float s4[4] = {}, e4[4] = {};  // what is there joins at the end: one rounding of its size, not one per logit
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -62,8 +62,8 @@ __device__ __forceinline__ void fold_all(Stats& a, const float (&z)[U][M], const
       s4[j & 3] += f;
       e4[j & 3] = fmaf(f, fmaxf(d, kTiny), e4[j & 3]);
     }
-  a.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-  a.e = (e4[0] + e4[1]) + (e4[2] + e4[3]);
+  a.s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  a.e += (e4[0] + e4[1]) + (e4[2] + e4[3]);
 }
 template <int N, int M>
 __device__ __forceinline__ float max_of(const float (&z)[M]) {
@@ -122,6 +122,22 @@ struct RowLse {
   float lse, rest;
   __device__ __forceinline__ float logprob(float z) const { return (z - lse) - rest; }
 };
+__device__ __forceinline__ float two_sum(float a, float b, float& left) {  // a + b, and what its rounding has left
+  const float s = a + b, bb = s - a;
+  left = (a - (s - bb)) + (b - bb);
+  return s;
+}
+// From a row's statistics: ln 2 (M + log2 s).  Every probability of the gradient has the error of this number (one row of 26152
+// fp32 logits, the best at 25: 1e-6 as it stands), so the exponent of s is added by itself, and what kLog2e has been rounded by is
+// taken back: the statistics are those of exp((1 + delta) z), whose logarithm is larger by delta times the mean of z.
+__device__ __forceinline__ RowLse row_lse(const Stats& st) {
+  constexpr float kLn2Left = 0.6931471805599453 - (double)kLn2, kDelta = (double)kLog2e * 0.6931471805599453 - 1.0;
+  float left, rest;
+  const float t = two_sum(st.M, (float)__builtin_amdgcn_frexp_expf(st.s), left);
+  const float part = left + __log2f(__builtin_amdgcn_frexp_mantf(st.s)), hi = t * kLn2;
+  const float lse = two_sum(hi, fmaf(part, kLn2, fmaf(t, kLn2Left, fmaf(t, kLn2, -hi)) - kDelta * kLn2 * (st.M + st.e / st.s)), rest);
+  return RowLse{lse, rest};
+}
 // Statistics whose largest logit is beyond this (in log2 units) do not give a log-probability: 32 bits of a log-sum-exp of
 // -1e9, which a mask has left nothing of, are multiples of 64, and the scaled statistics of the type's lowest value overflow.
 constexpr float kFarFromZero = 16384.f;
@@ -232,8 +248,7 @@ __device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vo
     if (out.entropy != nullptr) out.entropy[t] = entropy;
   };
   if (tid == 0) {
-    const float L = __log2f(st.s);
-    write_row({(st.M + L) * kLn2, 0.f}, (L - st.e / st.s) * kLn2);
+    write_row(row_lse(st), (__log2f(st.s) - st.e / st.s) * kLn2);
     s_care = needs_care(st);
   }
   __syncthreads();

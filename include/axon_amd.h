@@ -682,8 +682,8 @@ int axon_logits_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_
 
 /* Alternatives of materialised logits (no reference counterpart; the reference's logprobs_from_logits,
  * axon/utils/torch/ops.py:39-102, knows one token per position).  Operands as above, logits aligned to their element,
- * at most 2^24 rows.  lse [2][n]: the rows' log-sum-exps and, behind them, what their rounding to 32 bits has left of those
- * that are far from 0 (a row that a mask of -1e9 has left nothing of), 0 in others.
+ * at most 2^24 rows.  lse [2][n]: the rows' log-sum-exps and, behind them, what their rounding to 32 bits has left (most of
+ * it where they are far from 0, as of a row that a mask of -1e9 has left nothing of).
  *   _top_fwd: the k largest logits of every row (1 <= k <= 128, k <= vocab), in descending order, equal ones by
  *        ascending id: top_ids [n][k] int64 and top_logprobs [n][k] = logit - (lse + rest); beside them logprob (with labels),
  *        entropy (either may be NULL) and lse.  A row with a NaN has NaN everywhere but in top_ids, for which a
