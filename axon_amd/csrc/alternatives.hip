@@ -4,7 +4,7 @@
 //
 // Forward: ONE read of the row gives the softmax statistics and, for the k largest, the maxima of the row's segments of
 // 256 bytes, from which select.h finds the few segments that are read again.  Bound by memory: 4096 x 151936 bf16 with 20
-// alternatives and a label 209 us, 5.9 TB/s (a large device copy 4.8 to 5.0, read and write); 1500 x 151936 fp32 with 32 given
+// alternatives and a label 214 us, 5.8 TB/s (a large device copy 4.8 to 5.0, read and write); 1500 x 151936 fp32 with 32 given
 // tokens 144 us, 6.3 TB/s.  Short batches are bound by the two launches' latency: one row of 151936 5.3 + 7.5 us, of which the
 // selection's trips to memory are most.
 #include "logits_rows.h"
@@ -14,6 +14,7 @@
 namespace axon {
 
 constexpr int kMaxParts = 64;
+constexpr int kPartFloats = 4;      // what a part of a row leaves: M, e, s in two
 constexpr int kSegVecs = 16;        // 16-byte vectors per segment: what sixteen neighbouring lanes load together
 constexpr int kMaxTokenIds = AXON_MAX_TOKEN_IDS;  // given tokens per row
 
@@ -39,16 +40,21 @@ struct SegSpan {
   __device__ __forceinline__ int scalar(int i) const { return i < head ? i : i + n_vec * Row<T>::kPer; }
 };
 
-// Folds U times N logits (natural units) into the statistics, given the maxima of the U sets: one rescale at most.  A NaN
-// among the logits makes the sums NaN, as it does those of a softmax; -inf adds nothing.
+// Statistics of a set of logits: M >= every one of them (the largest, once there is one), s = sum 2^d, e = sum d 2^d over
+// d = (z - M) log2(e).  The difference comes first: scaled by themselves, the type's lowest value overflows, -1e9 is off by 64,
+// and every logit by what log2(e) has been rounded by (with the scaled maximum subtracted in one fused operation: 209 us for 215,
+// log-probabilities near 0 off by 3e-6 of themselves for 4e-7).
+constexpr float kLowest = -3.402823466e38f;
+
+// Folds U times N logits into a thread's statistics, given the maxima of the U sets: one rescale at most.  A NaN or +inf among
+// the logits makes the sums NaN, as it does those of a softmax; -inf adds nothing.
 template <int N, int U, int M>
 __device__ __forceinline__ void fold_all(Stats& a, const float (&z)[U][M], const float (&set_max)[U]) {
   float m = set_max[0];
 #pragma unroll
   for (int u = 1; u < U; ++u) m = fmaxf(m, set_max[u]);
-  m *= kLog2e;
   if (m > a.M) {
-    const float d = fmaxf(a.M - m, kTiny), f = __builtin_amdgcn_exp2f(d);
+    const float d = fmaxf((a.M - m) * kLog2e, kTiny), f = __builtin_amdgcn_exp2f(d);
     a.e = f * fmaf(a.s, d, a.e);
     a.s = a.s * f;
     a.M = m;
@@ -58,7 +64,7 @@ __device__ __forceinline__ void fold_all(Stats& a, const float (&z)[U][M], const
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = fmaf(z[u][j], kLog2e, -a.M), f = __builtin_amdgcn_exp2f(d);
+      const float d = (z[u][j] - a.M) * kLog2e, f = __builtin_amdgcn_exp2f(d);
       s4[j & 3] += f;
       e4[j & 3] = fmaf(f, fmaxf(d, kTiny), e4[j & 3]);
     }
@@ -73,15 +79,22 @@ __device__ __forceinline__ float max_of(const float (&z)[M]) {
   return m;
 }
 
-__device__ __forceinline__ Stats wave_merge(Stats st) {
+// The threads' statistics together: the sum in 64 bits, since its roundings at each of the dozen merges are what the logarithm of a
+// sum near 1 would consist of (a row with one likely token).
+struct RowStats {
+  float M, e;
+  double s;
+};
+__device__ __forceinline__ RowStats merge(const RowStats& a, const RowStats& b) {
+  const float M = fmaxf(a.M, b.M);
+  const float d1 = fmaxf((a.M - M) * kLog2e, kTiny), d2 = fmaxf((b.M - M) * kLog2e, kTiny);
+  const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
+  return {M, f1 * fmaf((float)a.s, d1, a.e) + f2 * fmaf((float)b.s, d2, b.e), a.s * f1 + b.s * f2};
+}
+__device__ __forceinline__ RowStats wave_merge(RowStats st) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    Stats o;
-    o.M = __shfl_down(st.M, off, kWave);
-    o.s = __shfl_down(st.s, off, kWave);
-    o.e = __shfl_down(st.e, off, kWave);
-    st = merge(st, o);
-  }
+  for (int off = 32; off > 0; off >>= 1)
+    st = merge(st, RowStats{__shfl_down(st.M, off, kWave), __shfl_down(st.e, off, kWave), __shfl_down(st.s, off, kWave)});
   return st;
 }
 
@@ -122,65 +135,18 @@ struct RowLse {
   float lse, rest;
   __device__ __forceinline__ float logprob(float z) const { return (z - lse) - rest; }
 };
-__device__ __forceinline__ float two_sum(float a, float b, float& left) {  // a + b, and what its rounding has left
-  const float s = a + b, bb = s - a;
-  left = (a - (s - bb)) + (b - bb);
-  return s;
+// ln s of s >= 1 from its exponent and its mantissa in [0.7, 1.4), by the series of 2 artanh: to 2^-23 of itself also near s = 1.
+__device__ __forceinline__ double log_of_sum(double s) {
+  int ex = __builtin_amdgcn_frexp_exp(s);
+  double m = __builtin_amdgcn_frexp_mant(s);
+  if (m < 0.70710678) { m *= 2.0; ex -= 1; }
+  const float f = (float)(m - 1.0) / (float)(m + 1.0), f2 = f * f;
+  const float series = fmaf(f2, fmaf(f2, fmaf(f2, fmaf(f2, 1.f / 9, 1.f / 7), 1.f / 5), 1.f / 3), 1.f);
+  return (double)ex * 0.6931471805599453 + (double)(2.f * f * series);
 }
-// From a row's statistics: ln 2 (M + log2 s).  Every probability of the gradient has the error of this number (one row of 26152
-// fp32 logits, the best at 25: 1e-6 as it stands), so the exponent of s is added by itself, and what kLog2e has been rounded by is
-// taken back: the statistics are those of exp((1 + delta) z), whose logarithm is larger by delta times the mean of z.
-__device__ __forceinline__ RowLse row_lse(const Stats& st) {
-  constexpr float kLn2Left = 0.6931471805599453 - (double)kLn2, kDelta = (double)kLog2e * 0.6931471805599453 - 1.0;
-  float left, rest;
-  const float t = two_sum(st.M, (float)__builtin_amdgcn_frexp_expf(st.s), left);
-  const float part = left + __log2f(__builtin_amdgcn_frexp_mantf(st.s)), hi = t * kLn2;
-  const float lse = two_sum(hi, fmaf(part, kLn2, fmaf(t, kLn2Left, fmaf(t, kLn2, -hi)) - kDelta * kLn2 * (st.M + st.e / st.s)), rest);
-  return RowLse{lse, rest};
-}
-// Statistics whose largest logit is beyond this (in log2 units) do not give a log-probability: 32 bits of a log-sum-exp of
-// -1e9, which a mask has left nothing of, are multiples of 64, and the scaled statistics of the type's lowest value overflow.
-constexpr float kFarFromZero = 16384.f;
-__device__ __forceinline__ bool needs_care(const Stats& st) { return !(st.s > 0.f) || !(fabsf(st.M) < kFarFromZero); }
-
-// Log-sum-exp and entropy of such a row, and of one that has NaN or infinite logits or none but -inf: two passes over it, the
-// differences from the largest logit formed before they are scaled.  64 rows of 151936, finished by a workgroup each: 88 us, where
-// other rows take 8.  The result in thread 0.
-template <typename T>
-__device__ __forceinline__ RowLse careful_row(const T* row, int vocab, float& entropy, float (&red)[3][kBlock / kWave]) {
-  const RowSpan sp(row, vocab, true, 0, 1);
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
-  auto each = [&](auto f) {
-    for (int q = tid; q < sp.n_vec; q += kBlock) {
-      float v[8];
-      Row<T>::template load<true>(row + sp.head + (uint32_t)q * Row<T>::kPer, v);
-#pragma unroll
-      for (int j = 0; j < Row<T>::kPer; ++j) f(v[j]);
-    }
-    for (int i = tid; i < sp.n_scalar; i += kBlock) f(Row<T>::one(row + sp.scalar<T>(i)));
-  };
-  float m = -INFINITY;
-  each([&](float z) { m = fmaxf(m, z); });
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  float s = 0.f, e = 0.f;
-  each([&](float z) {
-    const float d = (z - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-    s += f;
-    e = fmaf(f, fmaxf(d, kTiny), e);
-  });
-  s = wave_sum(s);
-  e = wave_sum(e);
-  if (lane == 0) { red[1][wave] = s; red[2][wave] = e; }
-  __syncthreads();
-  s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  e = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
-  const float L = __log2f(s), lse = fmaf(L, kLn2, m);
-  entropy = (L - e / s) * kLn2;
-  return RowLse{lse, fmaf(L, kLn2, m - lse)};
+__device__ __forceinline__ RowLse row_lse(const RowStats& st, double ln_s) {
+  const float lse = st.s > 0.0 ? (float)((double)st.M + ln_s) : NAN;  // NaN: a row of -inf alone
+  return RowLse{lse, (float)(((double)st.M - lse) + ln_s)};
 }
 
 struct Picks {
@@ -232,33 +198,22 @@ struct TopOut {
 // What is wanted of a row beside its statistics.
 enum Want { kTokens, kTop };
 
-// The end of a row: log-sum-exp and entropy from its statistics (in thread 0) or by looking again, then what is wanted of it.  HELD: how many
+// The end of a row: log-sum-exp and entropy from its statistics (in thread 0), then what is wanted of it.  HELD: how many
 // maxima a thread holds, 0 where they are in LDS.
 template <typename T, Want WANT, int HELD>
-__device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vocab, const float* seg_max, const RowOut& out,
+__device__ __forceinline__ void finish_row(RowStats st, int t, const T* row, int vocab, const float* seg_max, const RowOut& out,
                                            const Picks& picks, const TopOut& top, SelectLds* sel) {
   __shared__ RowLse s_lse;
-  __shared__ float red[3][kBlock / kWave];
-  __shared__ int s_care;
   const int tid = threadIdx.x;
-  auto write_row = [&](RowLse lse, float entropy) {
-    s_lse = lse;
-    out.lse[t] = lse.lse;
-    out.lse[(int64_t)out.n + t] = lse.rest;
-    if (out.entropy != nullptr) out.entropy[t] = entropy;
-  };
   if (tid == 0) {
-    write_row(row_lse(st), (__log2f(st.s) - st.e / st.s) * kLn2);
-    s_care = needs_care(st);
-  }
-  __syncthreads();
-  if (s_care) {
-    float entropy;
-    const RowLse lse = careful_row<T>(row, vocab, entropy, red);
-    if (tid == 0) write_row(lse, entropy);
-    __syncthreads();
+    const double ln_s = log_of_sum(st.s);
+    s_lse = row_lse(st, ln_s);
+    out.lse[t] = s_lse.lse;
+    out.lse[(int64_t)out.n + t] = s_lse.rest;
+    if (out.entropy != nullptr) out.entropy[t] = (float)ln_s - st.e / (float)st.s * kLn2;
   }
   if (WANT == kTokens) {
+    __syncthreads();
     write_picks<T>(picks, t, row, vocab, s_lse);
     return;
   }
@@ -267,6 +222,7 @@ __device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vo
   const int64_t lab = with_label ? load_id(out.labels, out.labels_i64, t) : -1;
   const bool inside = lab >= 0 && lab < vocab;
   const float label_z = inside ? Row<T>::one(row + lab) : 0.f;
+  // (the selection's own barriers come before the first use of s_lse)
   const LogitsSource<T, HELD> src{row, seg_max, SegSpan(row, vocab, 0, 1), vocab};
   select_top(src, top.k, *sel, tid, [&](int rank, float z, int index) {
     top.logprobs[(int64_t)t * top.k + rank] = s_lse.logprob(z);
@@ -277,14 +233,15 @@ __device__ __forceinline__ void finish_row(Stats st, int t, const T* row, int vo
 
 // Workgroup (row, part): blockIdx.x = row * parts + part.  Where a row has one part it is finished here: a row's selection
 // runs beside the reading of the rows that the compute unit's other workgroups have (the maxima of its segments are in
-// LDS).  Else the statistics go to ws[row][part][3] and the maxima to seg_max[row][seg], for the kernels below.
+// LDS).  Else the statistics go to ws[row][part][kPartFloats] and the maxima to seg_max[row][seg], for the kernels below.
 // Rows from `cached_from` on are left in the cache in front of the memory, for what reads them next.
 template <typename T, Want WANT>
 __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int parts,
                                                               float* __restrict__ ws, float* __restrict__ seg_max, int seg_stride,
                                                               RowOut out, Picks picks, TopOut top, int cached_from) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ float red[3][kBlock / kWave];
+  __shared__ float red[2][kBlock / kWave];
+  __shared__ double red_s[kBlock / kWave];
   const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
   const T* row = logits + (int64_t)t * ld;
   constexpr int kPer = Row<T>::kPer;
@@ -293,7 +250,7 @@ __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restric
   const bool whole = parts == 1 && seg_max == nullptr;
   float* const segs = reinterpret_cast<float*>(smem + sizeof(SelectLds));  // where the row is finished here
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  Stats st{kFloor, 0.f, 0.f};
+  Stats mine_st{kLowest, 0.f, 0.f};
   auto walk = [&](auto cached) {
     constexpr bool kCached = decltype(cached)::value;
     const int mine = tile_vec(lane);
@@ -313,7 +270,7 @@ __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restric
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) m[u] = max_of<kPer>(v[u]);
-      fold_all<kPer>(st, v, m);
+      fold_all<kPer>(mine_st, v, m);
       if (WANT == kTop) {
         const float best = tile_maxima(m);
         const int seg = tile * (kTileVecs / kSegVecs) + (lane >> 2);
@@ -327,27 +284,27 @@ __global__ __launch_bounds__(kBlock) void alternatives_kernel(const T* __restric
   if (t >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
   for (int i = part * kBlock + tid; i < sp.n_scalar; i += parts * kBlock) {
     const float v[1][1] = {{Row<T>::one(row + sp.scalar<T>(i))}};
-    fold_all<1>(st, v, v[0]);
+    fold_all<1>(mine_st, v, v[0]);
   }
-  st = wave_merge(st);
-  if (lane == 0) { red[0][wave] = st.M; red[1][wave] = st.s; red[2][wave] = st.e; }
+  RowStats st = wave_merge(RowStats{mine_st.M, mine_st.e, mine_st.s});
+  if (lane == 0) { red[0][wave] = st.M; red[1][wave] = st.e; red_s[wave] = st.s; }
   __syncthreads();
   if (tid == 0)
-    for (int w = 1; w < kBlock / kWave; ++w) st = merge(st, Stats{red[0][w], red[1][w], red[2][w]});
+    for (int w = 1; w < kBlock / kWave; ++w) st = merge(st, RowStats{red[0][w], red[1][w], red_s[w]});
   if (whole) {
     finish_row<T, WANT, 0>(st, t, row, vocab, segs, out, picks, top, reinterpret_cast<SelectLds*>(smem));
   } else if (tid == 0) {
-    float* o = ws + (int64_t)blockIdx.x * 3;
-    o[0] = st.M; o[1] = st.s; o[2] = st.e;
+    float* o = ws + (int64_t)blockIdx.x * kPartFloats;
+    o[0] = st.M; o[1] = st.e; o[2] = (float)st.s; o[3] = (float)(st.s - (float)st.s);
   }
 }
 
 // The statistics of a row's parts (at most kMaxParts), in a fixed tree; the total in thread 0.
-__device__ __forceinline__ Stats merge_parts(const float* ws, int t, int parts) {
-  Stats st{kFloor, 0.f, 0.f};
+__device__ __forceinline__ RowStats merge_parts(const float* ws, int t, int parts) {
+  RowStats st{kLowest, 0.f, 0.0};
   if ((int)threadIdx.x < parts) {
-    const float* o = ws + ((int64_t)t * parts + threadIdx.x) * 3;
-    st = Stats{o[0], o[1], o[2]};
+    const float* o = ws + ((int64_t)t * parts + threadIdx.x) * kPartFloats;
+    st = RowStats{o[0], o[1], (double)o[2] + (double)o[3]};
   }
   return threadIdx.x < kWave ? wave_merge(st) : st;
 }
@@ -539,7 +496,7 @@ extern "C" int64_t axon_logits_top_workspace_bytes(int dtype, int64_t n, int64_t
   if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
   const int parts = fwd_parts(n, vocab, elem_bytes(dtype));
   if (parts == 1 && top_lds(dtype, vocab) <= kMaxTopLds) return 0;
-  return n * (parts * 3 + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
+  return n * (parts * kPartFloats + seg_stride(dtype, vocab)) * (int64_t)sizeof(float);
 }
 
 extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, int64_t k,
@@ -557,7 +514,7 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
   const hipStream_t st = (hipStream_t)stream;
   const int eb = elem_bytes(dtype), parts = fwd_parts(n, vocab, eb);
   const bool whole = need == 0;
-  float* const seg_max = whole ? nullptr : workspace + n * parts * 3;
+  float* const seg_max = whole ? nullptr : workspace + n * parts * kPartFloats;
   const int stride = (int)seg_stride(dtype, vocab), from = cached_from(n, vocab, eb, bwd_follows);
   const unsigned lds = whole ? (unsigned)top_lds(dtype, vocab) : 0;
   const RowOut out{logprob, entropy, lse, labels, labels_i64, (int)n};
@@ -581,7 +538,7 @@ extern "C" int axon_logits_top_fwd(const void* logits, int dtype, int64_t ld, in
 extern "C" int64_t axon_logits_tokens_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
   if (n < 0 || vocab <= 0 || !dtype_ok(dtype)) return AXON_ERR_ARG;
   const int parts = fwd_parts(n, vocab, elem_bytes(dtype));
-  return parts > 1 ? n * parts * 3 * (int64_t)sizeof(float) : 0;
+  return parts > 1 ? n * parts * kPartFloats * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int axon_logits_tokens_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids,
