@@ -5,7 +5,7 @@
 // Forward: ONE read of the row gives the softmax statistics and, for the k largest, the maxima of the row's segments of
 // 256 bytes, from which select.h finds the few segments that are read again.  Bound by memory: 4096 x 151936 bf16 with 20
 // alternatives and a label 214 us, 5.8 TB/s (a large device copy 4.8 to 5.0, read and write); 1500 x 151936 fp32 with 32 given
-// tokens 144 us, 6.3 TB/s.  Short batches are bound by the two launches' latency: one row of 151936 5.3 + 7.5 us, of which the
+// tokens 149 us, 6.1 TB/s.  Short batches are bound by the two launches' latency: one row of 151936 5.4 + 7.0 us, of which the
 // selection's trips to memory are most.
 #include "logits_rows.h"
 #include "select.h"
