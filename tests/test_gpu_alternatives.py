@@ -242,6 +242,22 @@ def test_rows_whose_maxima_do_not_fit_in_lds():
         assert (entropy.double() - ent).abs().max() <= ENT_TOL + 14 * 2735 * 2.0 ** -24
 
 
+@pytest.mark.parametrize("n", [3, 600])
+def test_rows_with_one_likely_token(n):
+    """The largest logit, near 29, adds exactly 1 to the sum, all others together at most 2^-22 (what is lost of them beside
+    it); the difference from the log-sum-exp and its rest is exact: log-probabilities of almost 0 to 2^-22, not to 30 times the
+    rounding of a factor (4e-7)."""
+    z = logits_of("random", n, 2000, torch.float32, 9).clamp(max=10.5)
+    z[:, 777] = 29 + torch.rand(n, generator=gen(3), device="cuda")
+    others = torch.exp(z.double() - z[:, 777:778].double()).sum(1) - 1
+    assert others.max() < 2.0 ** -22
+    at = torch.full((n, 1), 777, device="cuda")
+    want = reference(z, at)[0]
+    r = top_logprobs_from_logits(z, 1, at[:, 0])
+    for got in (r.top_logprobs, r.logprobs[:, None], token_logprobs_from_logits(z, at)[0]):
+        assert (got.double() - want).abs().max() <= 2.0 ** -22
+
+
 def test_logits_written_to_before_the_backward_are_noticed():
     z = logits_of("random", 4, 300, torch.float32, 2)
     for op in (lambda x: top_logprobs_from_logits(x, 3).top_logprobs, lambda x: token_logprobs_from_logits(x, torch.zeros(4, 1, dtype=torch.int64, device="cuda"))[0]):
