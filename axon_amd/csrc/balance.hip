@@ -201,19 +201,23 @@ __device__ __forceinline__ void sort_keys(uint32_t (&s)[V]) {
           }
 }
 
-// Ordered keys of a lane's elements; 0 where there is no expert.  fp32: the value's 32 bits.  bf16: the value's 16 bits above
-// the index, so that no two keys of a row are equal (two values at a time: sign and magnitude to an integer in the order of
-// the values, -0 to that of 0).
+// Ordered keys of a lane's elements; 0 where there is no expert (no expert's key is 0).  fp32: the value's 32 bits.  bf16: the
+// value's 16 bits above the index, so that no two keys of a row are equal (two values at a time: sign and magnitude to an
+// integer in the order of the values, -0 to that of 0).  A NaN has the value of -inf in both.
 template <typename T, int V>
 __device__ __forceinline__ void make_keys(const float (&x)[V], int e0, int experts, uint32_t (&key)[V]) {
   if (sizeof(T) == 2) {
     typedef short s16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     const uint32_t low = 0xffff - e0;
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(x[j + 1]), __float_as_uint(x[j]), 0x07060302u);
       const s16x2 sign = __builtin_bit_cast(s16x2, w) >> 15, mag = __builtin_bit_cast(s16x2, w & 0x7fff7fffu);
-      const uint32_t u = __builtin_bit_cast(uint32_t, (s16x2)((mag ^ sign) - sign)) ^ 0x80008000u;
+      // +inf moves to the largest integer, a positive NaN wraps to where the negative ones are: below -inf, which takes them up
+      const s16x2 value = __builtin_bit_cast(s16x2, __builtin_bit_cast(u16x2, (s16x2)((mag ^ sign) - sign)) + (unsigned short)0x7f);
+      const s16x2 ordered = __builtin_elementwise_max(value, (s16x2)(short)(0x7f - 0x7f80));
+      const uint32_t u = __builtin_bit_cast(uint32_t, ordered) ^ 0x80008000u;
       key[j] = e0 + j < experts ? (u << 16) | (low - j) : 0u;
       key[j + 1] = e0 + j + 1 < experts ? (u & 0xffff0000u) | (low - j - 1) : 0u;
     }
@@ -252,13 +256,13 @@ __device__ __forceinline__ void count_choices(const float (&x)[V], int e0, int e
     for (int j = 0; j + 1 < V; ++j) s[j] = (s[j + 1] & m) | (s[j] & ~m);
     s[V - 1] &= ~m;
   }
+  if (!in) return;  // whatever its row holds
   if (kUnique) {
-    bound = in ? max(bound, 1u) : 0xffffffffu;  // no key is that large: its lower half is at most 0xffff, of a NaN
 #pragma unroll
     for (int j = 0; j < V; ++j) cnt[j] += key[j] >= bound;
     return;
   }
-  if (!in || given == 0) return;
+  if (given == 0) return;
 #pragma unroll
   for (int j = 0; j < V; ++j) given -= key[j] > bound;
 #pragma unroll

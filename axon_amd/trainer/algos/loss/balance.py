@@ -28,10 +28,12 @@ def router_balance_loss(router_logits, top_k: int, *, token_mask=None, cu_seqlen
     * ``router_logits``: one ``[..., experts]`` tensor per layer in a list or tuple (as a model returns them), one tensor
       ``[layers, tokens, experts]``, or ``[tokens, experts]`` of a single layer (``counts`` is then ``[experts]``); fp32 or
       bf16, at most 1024 experts, the same shape in all layers.  The gradient comes back in the logits' type.
-    * ``top_k``: experts per token.  The choices are the ``top_k`` largest logits, equal ones by ascending expert, or
-      ``expert_ids`` (int32 or int64, ``[..., top_k]`` per layer in the same arrangement): what the router chose, where that
-      is not the order of these logits (a selection bias, replayed routes).  An id outside the experts chooses nothing.
-    * ``token_mask``: as many entries as tokens, shared by the layers; a token counts where it is not zero.
+    * ``top_k``: experts per token.  The choices are the ``top_k`` largest logits, equal ones by ascending expert and a NaN as
+      -inf (the loss of a batch that has one is NaN), or ``expert_ids`` (int32 or int64, ``[..., top_k]`` per layer in the
+      same arrangement): what the router chose, where that is not the order of these logits (a selection bias, replayed
+      routes).  An id outside the experts chooses nothing.
+    * ``token_mask``: as many entries as tokens, shared by the layers; a token counts where it is not zero (what its
+      row holds does not matter otherwise).
     * ``cu_seqlens``: int32 ``[sequences + 1]``: the loss per sequence, averaged.  Tokens of no sequence count nowhere.
     * ``score_fn``: ``"softmax"`` or ``"sigmoid"``.
 

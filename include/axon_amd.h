@@ -716,7 +716,8 @@ int axon_logits_tokens_bwd(const void* logits, int dtype, int64_t ld, int64_t n,
  *   sum_e experts / (k T^2) c_e P_e,  P_e = sum over the unmasked tokens of p_te,  c_e = how often they chose expert e,
  * averaged over these sequences and over the layers: 1 where scores and choices are uniform.  p: softmax of a token's logits
  * (score 0), or their sigmoids divided by their sum (score 1).  Choices: the token's k largest logits, equal ones by ascending
- * expert, or the given ids [n][k] (an id outside [0, experts) chooses nothing).  The choices are constants for the gradient.
+ * expert and a NaN as -inf, or the given ids [n][k] (an id outside [0, experts) chooses nothing).  The choices are constants
+ * for the gradient.  What lies in a masked token's row does not matter.
  *   logits, ids, dlogits: HOST arrays of one device pointer per layer: logits [n][experts] (row stride ld, dtype
  *        AXON_LOGITS_F32 or AXON_LOGITS_BF16), ids NULL or [n][k], dlogits [n][experts] contiguous (an entry may be NULL:
  *        that layer wants no gradient).  mask [n] (NULL: all tokens count), a token counts where it is not zero.

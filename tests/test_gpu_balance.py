@@ -371,3 +371,54 @@ def test_saved_tensors_from_a_hook_are_looked_at_again():
                    lambda t: t[:20] if t.dim() == 2 else t, lambda t: t[:2] if t.dtype == torch.int32 else t):
         with pytest.raises(RuntimeError):
             backward_with(unpack)
+
+
+@pytest.mark.parametrize("bits", [0x7FFF, 0x7FC0, 0x7F81, 0x7F80, 0xFFFF, 0xFFC0, 0xFF81, 0xFF80])
+@pytest.mark.parametrize("e,k", [(6, 2), (60, 4), (128, 8), (700, 3)])
+def test_masked_rows_of_any_bf16_pattern_do_not_matter(e, k, bits):
+    """NaN of every kind and infinities at expert 0 and elsewhere in rows that the mask leaves out, the first of a run among them:
+    the results are those of zeros there, bit for bit."""
+    xs, _, _ = case(2, 75, e, k, torch.bfloat16, e)
+    cu = torch.tensor([0, 33, 75], dtype=torch.int32, device="cuda")
+    mask = torch.ones(75, dtype=torch.int64, device="cuda")
+    off = torch.tensor([0, 33, 34, 74], device="cuda")
+    mask[off] = 0
+    odd = torch.tensor([bits], dtype=torch.int32, device="cuda").to(torch.int16).view(torch.bfloat16)
+    clean, bad = [], []
+    for x in xs:
+        y = x.clone()
+        y[off] = 0
+        z = y.clone()
+        z[off, 0] = odd
+        z[33] = odd
+        z[34, e - 1] = odd
+        clean.append(y.requires_grad_(True))
+        bad.append(z.requires_grad_(True))
+    for score in ("softmax", "sigmoid"):
+        for seqs in (None, cu):
+            want, got = (router_balance_loss(x, k, token_mask=mask, cu_seqlens=seqs, score_fn=score) for x in (clean, bad))
+            assert torch.equal(got[1], want[1]) and got[1].sum().item() == 2 * 71 * k
+            assert torch.equal(got[0], want[0])
+            for a, b in zip(torch.autograd.grad(got[0], bad), torch.autograd.grad(want[0], clean)):
+                assert torch.equal(a, b) and not a[off].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("e,k", [(3, 2), (60, 4), (128, 128), (700, 9)])
+def test_a_nan_counts_as_the_lowest_for_the_choices(e, k, dtype):
+    """In rows that count, whatever its sign and its bits: as -inf, equal ones by ascending expert; the loss is then NaN."""
+    g = torch.Generator(device="cuda").manual_seed(e)
+    x = torch.randint(-2, 3, (40, e), generator=g, device="cuda").to(dtype)
+    word, bits = (torch.int16, (0x7FFF, 0x7FC0, 0x7F81, -1, -0x40, -0x7F)) if dtype == torch.bfloat16 else (
+        torch.int32, (0x7FFFFFFF, 0x7FC00000, 0x7F800001, -1, -0x400000, -0x7FFFFF))
+    for i, b in enumerate(bits):
+        odd = torch.tensor([b], dtype=word, device="cuda").view(dtype)
+        assert torch.isnan(odd).all()
+        x[i, : e - i % 2] = odd  # all of a row, and all but its last
+        x[10 + i, i % e] = odd
+        x[20 + i, ::2] = odd
+    x[30, ::2], x[31] = -math.inf, math.inf
+    loss, counts = router_balance_loss(x, k)
+    low = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+    chosen = torch.sort(low.double(), dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(counts, torch.bincount(chosen.flatten(), minlength=e)) and torch.isnan(loss)
