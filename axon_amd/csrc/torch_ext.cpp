@@ -485,11 +485,11 @@ struct AlternativesNode : torch::autograd::Node {
   }
   // gradients of entropy, log-probabilities of the tokens, log-probability of the label (with labels)
   variable_list apply(variable_list&& g) override {
-    const Tensor x = rows.unpack(), at = ids.unpack(), lab = labels.unpack(), l = lse.unpack(),
-                 ent = entropy.unpack(shared_from_this());
     const bool with_label = g.size() > 2 && g[2].defined();
     if (!g[0].defined() && !g[1].defined() && !with_label) return {Tensor()};
     if (spent) throw AxonError("the logits' storage holds the gradient of an earlier backward (inplace_backward)");
+    const Tensor x = rows.unpack(), at = ids.unpack(), lab = labels.unpack(), l = lse.unpack(),
+                 ent = entropy.unpack(shared_from_this());
     std::optional<at::NoGradGuard> no_grad(std::in_place);
     const Tensor g_en = g[0].defined() ? f32(g[0]) : Tensor(), g_ids = g[1].defined() ? f32(g[1]) : Tensor(),
                  g_lab = with_label ? f32(g[2]) : Tensor();
@@ -513,6 +513,8 @@ struct AlternativesNode : torch::autograd::Node {
                                  row_stride(out), ::stream()),
           "axon_logits_tokens_bwd");
     spent = inplace;
+    // what has been saved of these logits by others is no longer there: they refuse, as after any write in place
+    if (inplace && !x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
     out = out.view(shape);
     no_grad.reset();
     return {once(std::move(out), kWhat)};

@@ -36,7 +36,7 @@ def _rows(logits):
 class _LogitsHead(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, want_entropy, inplace_backward):
-        flat = _rows(logits)
+        flat = _rows(logits.detach())
         lab = labels.reshape(-1).contiguous() if labels is not None else None
         logprob, entropy, lse = _ops.logits_forward(flat, lab, want_entropy, ctx.needs_input_grad[0])
         ctx.save_for_backward(flat, lab, lse, entropy)
@@ -54,6 +54,8 @@ class _LogitsHead(torch.autograd.Function):
         g_lp = g_logprob.reshape(-1) if g_logprob is not None and lab is not None else None
         g_en = g_entropy.reshape(-1) if g_entropy is not None and entropy is not None else None
         grad = _ops.logits_backward(flat, lab, lse, entropy, g_lp, g_en, inplace=ctx.inplace)
+        if ctx.inplace and not flat.is_inference():  # others that have saved these logits refuse, as after any write in place
+            torch.autograd.graph.increment_version(flat)
         return grad.view(ctx.shape), None, None, None
 
 
@@ -65,7 +67,8 @@ def logprobs_and_entropy_from_logits(logits: torch.Tensor, labels: torch.Tensor,
 
 def logprobs_from_logits(logits: torch.Tensor, labels: torch.Tensor, inplace_backward: bool = True) -> torch.Tensor:
     """Per-token log-probability of ``labels`` (ops.py:39-67), fp32, shape ``logits.shape[:-1]``.  With
-    ``inplace_backward`` the backward writes d loss / d logits over the logits' storage."""
+    ``inplace_backward`` the backward writes d loss / d logits over the logits' storage; a backward that runs after it and
+    needs these logits raises torch's error of a tensor modified in place."""
     return _LogitsHead.apply(logits, labels, False, inplace_backward)[0]
 
 
@@ -106,6 +109,7 @@ def token_logprobs_from_logits(logits: torch.Tensor, token_ids: torch.Tensor, in
     or int64 ``[..., k]``; an id outside the vocabulary is a filler: its log-probability is 0 and its gradient goes
     nowhere) and the entropy, fp32, from one read of ``logits`` ``[..., vocab]``.  Differentiable with respect to the
     logits; ids may occur more than once in a position.  With ``inplace_backward`` (here and above) the backward writes
-    d loss / d logits over the logits' storage, and can run once."""
+    d loss / d logits over the logits' storage, and can run once; another operator's backward that runs after it and needs
+    these logits raises torch's error of a tensor modified in place."""
     _, entropy, logprobs, _ = _lib.native().token_logprobs(logits, token_ids, bool(inplace_backward))
     return logprobs, entropy
