@@ -55,12 +55,13 @@ class _LinearAlternatives(torch.autograd.Function):
     """The k best tokens of every row (``ids`` None) or given ones, and a label: their log-probabilities."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, k, ids, labels, temperature, logit_softcapping, what):
+    def forward(ctx, hidden, weight, k, ids, labels, temperature, logit_softcapping, what, grad_enabled):
         ctx.set_materialize_grads(False)
         rows, w, inv_t, cap = _operands(what, hidden, weight, temperature, logit_softcapping)
         batch, n = hidden.shape[:-1], rows.shape[0]
         top_ids = label_lp = None
-        want_grad = bool(ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
+        # needs_input_grad is true of a trainable weight under no_grad too, where no backward can come
+        want_grad = grad_enabled and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
         if ids is None:
             lab = labels.reshape(-1).contiguous() if labels is not None else None
             label_lp, entropy, lse, mean, lp, at, logits = _ops.lmhead_top(rows, w, k, lab, inv_t, cap, want_grad)
@@ -78,7 +79,7 @@ class _LinearAlternatives(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_label, g_entropy, g_lp, _g_ids):
         if g_label is None and g_entropy is None and g_lp is None:
-            return (None,) * 8
+            return (None,) * 9
         rows, w, at, lp, lab, label_lp, lse, mean, logits = ctx.saved_tensors
         n, k = lp.shape
         g = torch.zeros_like(lp) if g_lp is None else g_lp.reshape(n, k)
@@ -88,8 +89,7 @@ class _LinearAlternatives(torch.autograd.Function):
             g = torch.cat([g_label.reshape(n, 1), g], 1)
         g_en = None if g_entropy is None else g_entropy.reshape(n)
         d_hidden, d_weight = _ops.lmhead_tokens_backward(g, g_en, rows, w, at, lp, lse, mean, *ctx.scalars, logits)
-        return (d_hidden.view(ctx.shape).to(ctx.in_dtypes[0]), d_weight.to(ctx.in_dtypes[1]), None, None, None, None, None,
-                None)
+        return d_hidden.view(ctx.shape).to(ctx.in_dtypes[0]), d_weight.to(ctx.in_dtypes[1]), *(None,) * 7
 
 
 def linear_top_logprobs(hidden, weight, k, labels=None, temperature=1.0, logit_softcapping=None) -> TopLogprobs:
@@ -98,7 +98,7 @@ def linear_top_logprobs(hidden, weight, k, labels=None, temperature=1.0, logit_s
     if labels is not None and labels.shape != hidden.shape[:-1]:
         raise ValueError(f"linear_top_logprobs: labels {tuple(labels.shape)} do not lie beside hidden {tuple(hidden.shape)}")
     return TopLogprobs(*_LinearAlternatives.apply(hidden, weight, k, None, labels, temperature, logit_softcapping,
-                                                  "linear_top_logprobs"))
+                                                  "linear_top_logprobs", torch.is_grad_enabled()))
 
 
 def linear_token_logprobs(hidden, weight, token_ids, temperature=1.0, logit_softcapping=None):
@@ -107,5 +107,5 @@ def linear_token_logprobs(hidden, weight, token_ids, temperature=1.0, logit_soft
         raise ValueError(f"linear_token_logprobs: token_ids {tuple(token_ids.shape)} do not lie beside hidden "
                          f"{tuple(hidden.shape)}")
     _, entropy, logprobs, _ = _LinearAlternatives.apply(hidden, weight, 0, token_ids, None, temperature, logit_softcapping,
-                                                        "linear_token_logprobs")
+                                                        "linear_token_logprobs", torch.is_grad_enabled())
     return logprobs, entropy

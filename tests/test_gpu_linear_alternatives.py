@@ -337,3 +337,28 @@ def test_a_row_of_nan_has_valid_ids(n, v, k):
     assert torch.equal(r.top_ids[1], torch.arange(k, device="cuda")) and torch.isnan(r.top_logprobs[1]).all()
     others = torch.arange(n, device="cuda") != 1
     assert torch.equal(r.top_ids[others], want.top_ids[others]) and torch.equal(r.top_logprobs[others], want.top_logprobs[others])
+
+
+def test_scoring_without_gradients_keeps_no_logits():
+    """Under ``no_grad`` a head that could be trained costs what any other does."""
+    n, h, v = 600, 768, 20000
+    hid, w, lab = operands(n, h, v, 3)
+    trained = w.clone().requires_grad_(True)
+    logits = n * v * 4
+
+    def peak_of(op):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = op()
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - before, out
+
+    ids = lab[:, None].expand(n, 4)
+    with torch.no_grad():
+        plain, (lp, ent) = peak_of(lambda: linear_token_logprobs(hid, trained, ids))
+    assert plain < logits // 2 and not lp.requires_grad
+    frozen, (lp2, ent2) = peak_of(lambda: linear_token_logprobs(hid, w, ids))
+    assert frozen == plain and torch.equal(lp, lp2) and torch.equal(ent, ent2)
+    held, (lp3, _) = peak_of(lambda: linear_token_logprobs(hid, trained, ids))
+    assert held >= logits and lp3.requires_grad

@@ -543,3 +543,30 @@ def test_fused_step_block_plans():
     assert sequence_blocks(cu, 512) == [(0, 2), (2, 3), (3, 5), (5, 6)]
     assert sequence_blocks(cu, 499) is None
     assert sequence_blocks([0, 0, 5, 5, 5], 8) == [(0, 4)]
+
+
+@pytest.mark.parametrize("grad_mode,trainable,wanted", [(True, True, True), (True, False, False), (False, True, False)])
+def test_several_tokens_through_the_head_keep_something_for_a_backward_that_can_come(monkeypatch, grad_mode, trainable, wanted):
+    from axon_amd import _lib, _ops
+    from axon_amd.utils.kernel import linear_top_logprobs as m
+
+    seen = []
+    one = torch.zeros(3)
+
+    def top(rows, w, k, lab, inv_t, cap, backward_follows):
+        seen.append(backward_follows)
+        return None, one.clone(), one.clone(), one.clone(), torch.zeros(3, k), torch.zeros(3, k, dtype=torch.int64), None
+
+    def tokens(rows, w, ids, inv_t, cap, backward_follows):
+        seen.append(backward_follows)
+        return torch.zeros(3, ids.shape[1]), one.clone(), one.clone(), one.clone(), None
+
+    monkeypatch.setattr(_lib, "require_device", lambda t, what: None)
+    monkeypatch.setattr(_ops, "lmhead_top", top)
+    monkeypatch.setattr(_ops, "lmhead_tokens", tokens)
+    hidden = torch.zeros(3, 32, dtype=torch.bfloat16)
+    weight = torch.zeros(10, 32, dtype=torch.bfloat16, requires_grad=trainable)
+    with torch.set_grad_enabled(grad_mode):
+        m.linear_top_logprobs(hidden, weight, 2)
+        m.linear_token_logprobs(hidden, weight, torch.zeros(3, 2, dtype=torch.int64))
+    assert seen == [wanted, wanted]
