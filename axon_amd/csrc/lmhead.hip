@@ -461,13 +461,14 @@ __global__ __launch_bounds__(256) void seq_start_kernel(const int32_t* __restric
 // PER = 2 once a workgroup per 16 tokens would be more than one per CU.  The label dots (one wavefront per token) run
 // before the barrier, beside the folds of the other wavefronts. 187 tokens x 896 x 151936 5.9 us (11.0 with three
 // arrays of partials, 64 groups and 16 tokens per workgroup), 700 x 4096 11.9 (19.0), 1500 x 896 9.8 (12.8), 3001 x
-// 2880 x 201088 22.5 (31.4), 8192 x 4096 41.4 (49.0).  `labels` and `logprobs` are null where no label's logit is wanted.
+// 2880 x 201088 22.5 (31.4), 8192 x 4096 41.4 (49.0).  `labels` and `logprobs` are null where no label's logit is wanted;
+// `terms` (may be null): what token_logprob wants of every token.
 template <int T, int PER, typename LabelT>
 __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
     const float* __restrict__ stats, int parts, const __bf16* __restrict__ hidden, const __bf16* __restrict__ weight,
     const LabelT* __restrict__ labels, int n_tokens, int hidden_sz, int vocab, float inv_temp, float cap,
     float* __restrict__ lse, float* __restrict__ entropy_b, float* __restrict__ entropy,
-    float* __restrict__ logprobs, const uint8_t* __restrict__ is_start, int last_dst) {
+    float* __restrict__ logprobs, const uint8_t* __restrict__ is_start, int last_dst, float2* __restrict__ terms) {
   constexpr int TOK = T * PER, kWaves = 16, kGroups = 256, SUB = kGroups * T / 1024;
   constexpr int kDeep = 8 / (SUB * PER) < 1 ? 1 : 8 / (SUB * PER);
   __shared__ float red[3][kWaves][TOK];
@@ -565,6 +566,7 @@ __global__ __launch_bounds__(1024) void lmhead_finish_kernel(
   const float d = et / st;
   lse[n] = (Mt + L) * kLn2;
   entropy_b[n] = (Mt + d) * kLn2;
+  if (terms) terms[n] = make_float2(Mt, L);
   const int dst = aligned_pos(n, n_tokens, is_start, last_dst);
   const bool start = is_start && is_start[dst];
   entropy[dst] = start ? 0.f : (L - d) * kLn2;
@@ -1050,16 +1052,25 @@ struct HeadSource {
   __device__ float single(int, int& index) const { index = 0; return 0.f; }
 };
 
+// The log-probability of a logit (capped, before the temperature) as the label's is formed: the difference from the largest logit in
+// one rounding, then the logarithm of the sum.  From the log-sum-exp in 32 bits, whose rounding is up to 1e-6 where it is 16 to
+// 32, a likely token's had no digit right and could be above 0; what the sum's own roundings leave above 0 is cut off.
+// terms: the token's largest logit (log2 units) and the log2 of its sum; c: inverse temperature times log2(e).
+__device__ __forceinline__ float token_logprob(float z, float c, float2 terms) {
+  const float lp = (fmaf(z, c, -terms.x) - terms.y) * kLn2;
+  return lp > 0.f ? 0.f : lp;  // NaN stays
+}
+
 struct TopParams {
   const float4* tiles;
   const float* pm;   // [parts][n_tokens], of the accumulators
-  const float* lse;
+  const float2* terms;
   float* top_logprobs;
   int64_t* top_ids;
   const void* labels;  // may be null
   float* logprobs;     // of the labels: a label outside the vocabulary gets 0 here
   int n_tokens, vocab, parts, tiles_n, k, labels_i64;
-  float inv_temp, cap, inv_cap;
+  float c, cap, inv_cap;
   int staged;        // a token's maxima fit in LDS
 };
 
@@ -1084,14 +1095,14 @@ __global__ __launch_bounds__(kBlock) void lmhead_top_kernel(TopParams p) {
   src.tile_step = (int64_t)p.tiles_n * 4 * kLogitsWaveVecs;
   src.parts = p.parts;
   src.vocab = p.vocab;
-  const float lse = p.lse[n];
+  const float2 terms = p.terms[n];
   if (p.labels && tid == 0) {
     const int64_t lab = p.labels_i64 ? static_cast<const int64_t*>(p.labels)[n] : (int64_t) static_cast<const int32_t*>(p.labels)[n];
     if (lab < 0 || lab >= p.vocab) p.logprobs[n] = 0.f;
   }
   auto out = [&](int rank, float z, int index) {
     if (p.cap != 0.f) z = p.cap * fast_tanh(z * p.inv_cap);
-    p.top_logprobs[(int64_t)n * p.k + rank] = fmaf(z, p.inv_temp, -lse);
+    p.top_logprobs[(int64_t)n * p.k + rank] = token_logprob(z, p.c, terms);
     p.top_ids[(int64_t)n * p.k + rank] = index;
   };
   if (p.staged) {
@@ -1115,15 +1126,15 @@ struct TokenArgs {
   }
 };
 
-// logprobs[n][i] = softcap(hidden[n] . W[ids[n][i]]) / T - lse[n]: a workgroup per token, a wavefront per id.
+// logprobs[n][i] = softcap(hidden[n] . W[ids[n][i]]) / T - logsumexp: a workgroup per token, a wavefront per id.
 // Bound by the rows of the weight that it gathers: 1001 x 64 ids, hidden 896, 27 us, 4.2 TB/s; 4096 x 20, hidden 4096, 118 us,
 // 5.7 TB/s.
 __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restrict__ hidden, const __bf16* __restrict__ weight,
-                                                           int hidden_sz, int vocab, TokenArgs a, float inv_temp, float cap,
-                                                           const float* __restrict__ lse) {
+                                                           int hidden_sz, int vocab, TokenArgs a, float c, float cap,
+                                                           float inv_cap, const float2* __restrict__ terms) {
   const int n = blockIdx.x, lane = threadIdx.x & 63;
   const uint4* h = reinterpret_cast<const uint4*>(hidden + (int64_t)n * hidden_sz);
-  const float lse_n = lse[n];
+  const float2 terms_n = terms[n];
   for (int i = threadIdx.x >> 6; i < a.k; i += 4) {
     const int64_t at = (int64_t)n * a.k + i, id = a.id(at);
     const bool ok = id >= 0 && id < vocab;
@@ -1131,8 +1142,8 @@ __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restr
     if (ok) {
       const uint4* w = reinterpret_cast<const uint4*>(weight + id * hidden_sz);
 #pragma unroll 4
-      for (int c = lane; c < hidden_sz / 8; c += 64) {
-        const uint4 hv = h[c], wv = w[c];
+      for (int u = lane; u < hidden_sz / 8; u += 64) {
+        const uint4 hv = h[u], wv = w[u];
         const uint32_t hs[4] = {hv.x, hv.y, hv.z, hv.w}, ws[4] = {wv.x, wv.y, wv.z, wv.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -1142,14 +1153,15 @@ __global__ __launch_bounds__(256) void token_logits_kernel(const __bf16* __restr
       }
     }
     dot = wave_sum(dot);
-    if (cap != 0.f) dot = cap * fast_tanh(dot / cap);
-    if (lane == 0) a.logprobs[at] = ok ? fmaf(dot, inv_temp, -lse_n) : 0.f;
+    if (cap != 0.f) dot = cap * fast_tanh(dot * inv_cap);
+    if (lane == 0) a.logprobs[at] = ok ? token_logprob(dot, c, terms_n) : 0.f;
   }
 }
 
 // The same from kept logits: a thread per id.  1001 x 64 ids 6 us, a scattered read of four bytes each.
 __global__ __launch_bounds__(256) void token_picks_kernel(const float4* __restrict__ tiles, int tiles_n, int64_t n_ids, int vocab,
-                                                          TokenArgs a, float inv_temp, float cap, const float* __restrict__ lse) {
+                                                          TokenArgs a, float c, float cap, float inv_cap,
+                                                          const float2* __restrict__ terms) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= n_ids) return;
   const int n = (int)(at / a.k);
@@ -1160,8 +1172,8 @@ __global__ __launch_bounds__(256) void token_picks_kernel(const float4* __restri
     const float4* const four = kept_column(tiles, n) + kept_vec(v / kWaveTile, v % kWaveTile / kBlk, v % kBlk / 4,
                                                                  (int64_t)tiles_n * 4 * kLogitsWaveVecs);
     float z = reinterpret_cast<const float*>(four)[v & 3];
-    if (cap != 0.f) z = cap * fast_tanh(z / cap);
-    lp = fmaf(z, inv_temp, -lse[n]);
+    if (cap != 0.f) z = cap * fast_tanh(z * inv_cap);
+    lp = token_logprob(z, c, terms[n]);
   }
   a.logprobs[at] = lp;
 }
@@ -1622,6 +1634,7 @@ int set_lds(K kernel) {
 
 struct FwdWs {
   float* stats;
+  float2* terms;  // several tokens per position: what their log-probabilities are formed from
   int parts;
   int64_t bytes;
 };
@@ -1629,7 +1642,9 @@ FwdWs fwd_ws(int64_t n, int64_t vocab, void* base) {
   FwdWs w;
   w.parts = (int)(round_up(vocab, kTile) / kTile) * 2;
   w.stats = static_cast<float*>(base);
-  w.bytes = round_up((int64_t)w.parts * n * 12, kAlign);
+  const int64_t stats = round_up((int64_t)w.parts * n * 12, kAlign);
+  w.terms = reinterpret_cast<float2*>(static_cast<char*>(base) + stats);
+  w.bytes = stats + round_up(n * (int64_t)sizeof(float2), kAlign);
   return w;
 }
 
@@ -2037,7 +2052,7 @@ int fwd_impl(const void* hidden, const void* weight, const void* labels, int lab
   hipLaunchKernelGGL((lmhead_finish_kernel<T, PER, LabelT>), grid, dim3(1024), 0, st, w.stats, w.parts,          \
                      static_cast<const __bf16*>(hidden), static_cast<const __bf16*>(weight),                     \
                      static_cast<const LabelT*>(labels), (int)n, (int)h, (int)v, inv_temp, softcap, lse,         \
-                     entropy_b, entropy, logprobs, is_start, (int)last_dst)
+                     entropy_b, entropy, logprobs, is_start, (int)last_dst, label_optional ? w.terms : nullptr)
   if (n <= 4 * kCus) AXON_FINISH(4, 1);
   else if (n <= 16 * kCus) AXON_FINISH(16, 1);
   else AXON_FINISH(16, 2);
@@ -2665,12 +2680,12 @@ extern "C" int axon_lmhead_top_fwd(const void* hidden, const void* weight, const
   if (rc != AXON_OK) return rc;
   TopParams p;
   p.tiles = static_cast<const float4*>(logits);
-  p.pm = w.maxima;  p.lse = lse;  p.top_logprobs = top_logprobs;  p.top_ids = top_ids;
+  p.pm = w.maxima;  p.terms = fwd_ws(n, v, base).terms;  p.top_logprobs = top_logprobs;  p.top_ids = top_ids;
   p.labels = labels;  p.labels_i64 = labels_i64;  p.logprobs = logprobs;
   p.n_tokens = (int)n;  p.vocab = (int)v;  p.k = (int)k;
   p.parts = (int)(round_up(v, kTile) / kTile) * 2;
   p.tiles_n = (int)(round_up(n, kTile) / kTile);
-  p.inv_temp = inv_temp;  p.cap = softcap;  p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+  p.c = inv_temp * kLog2e;  p.cap = softcap;  p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
   const int64_t select = (int64_t)sizeof(SelectLds), staged = (int64_t)p.parts * 4;
   p.staged = select + staged <= kTopLdsBytes;
   const int64_t span = kXcds * kNeighbours;
@@ -2693,16 +2708,18 @@ extern "C" int axon_lmhead_tokens_fwd(const void* hidden, const void* weight, co
                           workspace, ws_bytes, logits, logits_bytes, stream, nullptr, false, kKeepLogits, nullptr, true);
   if (rc != AXON_OK) return rc;
   const TokenArgs a{ids, ids_i64, (int)k, logprobs, nullptr};
+  const float c = inv_temp * kLog2e, inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+  const float2* const terms = fwd_ws(n, v, reinterpret_cast<char*>(round_up(reinterpret_cast<int64_t>(workspace), kAlign))).terms;
   if (logits) {
     hipLaunchKernelGGL(token_picks_kernel, dim3((unsigned)((n * k + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                       static_cast<const float4*>(logits), (int)(round_up(n, kTile) / kTile), n * k, (int)v, a, inv_temp, softcap,
-                       lse);
+                       static_cast<const float4*>(logits), (int)(round_up(n, kTile) / kTile), n * k, (int)v, a, c, softcap, inv_cap,
+                       terms);
     AXON_CHECK_LAUNCH();
     return AXON_OK;
   }
   hipLaunchKernelGGL(token_logits_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream,
-                     static_cast<const __bf16*>(hidden), static_cast<const __bf16*>(weight), (int)h, (int)v, a, inv_temp,
-                     softcap, lse);
+                     static_cast<const __bf16*>(hidden), static_cast<const __bf16*>(weight), (int)h, (int)v, a, c, softcap,
+                     inv_cap, terms);
   AXON_CHECK_LAUNCH();
   return AXON_OK;
 }

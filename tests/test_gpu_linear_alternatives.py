@@ -362,3 +362,40 @@ def test_scoring_without_gradients_keeps_no_logits():
     assert frozen == plain and torch.equal(lp, lp2) and torch.equal(ent, ent2)
     held, (lp3, _) = peak_of(lambda: linear_token_logprobs(hid, trained, ids))
     assert held >= logits and lp3.requires_grad
+
+
+@pytest.mark.parametrize("h", [64, 768])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("temperature,cap", [(1.0, None), (0.7, None), (0.7, 30.0)])
+def test_positions_with_one_likely_token(n, h, temperature, cap):
+    """A probability is at most 1, its logarithm at most 0; without a soft cap, whose argument is formed in another order there, the
+    token has the value that the head gives a label with the same exact logit, in every form.
+
+    A likely token's log-probability is off by its sum of exponentials: up to 20 additions in a tile's lane, three among lanes, 24
+    merges of two roundings, of 2^-24 each, an exponential and a logarithm of 2^-22 near 1, an argument that is rounded
+    once (60 * 2^-24 * what is not 0 of its difference): 71 * 2^-24 + 2 * 2^-22 < 6e-6, with a soft cap lp_tol's term for it more."""
+    hid, w, lab = operands(n, h, 5003, n + h, peak=0.0)
+    shift = w.float().abs().max() / 3  # entries of w are multiples of a quarter of this
+    rows = (w.float() / shift)[lab]
+    # label logits of 10 to 46 above the others' centre (|row|^2 shift peak, |row|^2 about h)
+    peak = torch.linspace(10, 46, n, device="cuda")[:, None] / (rows.square().sum(1, keepdim=True) * shift)
+    step = 2.0 ** -4
+    hid = (((hid.float() / 4 + peak * rows) / step).round().clamp(-127, 127) * step).bfloat16()
+    ref = Reference(hid, w, 1 / temperature, cap)
+    ids = ref.order(3)
+    want, best = ref.pick(lab[:, None])[:, 0], ref.pick(ids)
+    assert want.max() > -1e-5 and want.min() < -1e-3
+    r = linear_top_logprobs(hid, w, 3, lab, temperature, cap)
+    wg = w.clone().requires_grad_(True)
+    plain = linear_token_logprobs(hid, w, lab[:, None], temperature, cap)[0][:, 0]
+    kept = linear_token_logprobs(hid, wg, lab[:, None], temperature, cap)[0].detach()[:, 0]
+    assert torch.equal(r.top_ids, ids)
+    tol = 6e-6 + (lp_tol(cap, 1 / temperature) - LP_TOL if cap else 0)
+    for got, exact in ((plain, want), (kept, want), (r.top_logprobs[:, 0], best[:, 0])):
+        assert (got <= 0).all()
+        assert (got.double() - exact).abs().max() <= tol
+    assert torch.equal(kept, plain)
+    at = ids[:, 0] == lab
+    assert at.sum() > n // 2 and torch.equal(r.top_logprobs[at, 0], plain[at])
+    if not cap:
+        assert torch.equal(plain, r.logprobs.clamp(max=0))
