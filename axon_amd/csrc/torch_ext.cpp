@@ -537,7 +537,8 @@ std::tuple<OptTensor, Tensor, Tensor, Tensor> alternatives(const char* what, con
     if (labels) {
       if (!is_index(*labels)) refuse(what, "labels must be int32 or int64");
       if (labels->device() != logits.device()) refuse(what, "operands live on different devices");
-      same_len(what, "labels", n, *labels);
+      if (labels->sizes() != at::IntArrayRef(batch))
+        refuse(what, "labels " + shape_text(*labels) + " do not lie beside logits " + shape_text(logits));
       lab = labels->reshape({n}).contiguous();
     }
     if (ids_in) {

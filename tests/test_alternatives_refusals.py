@@ -137,3 +137,10 @@ def test_the_heads_c_entry_points_check_their_arguments():
 
     assert bwd(g=None) == bwd(ids=None) == bwd(lp=None) == bwd(dw=None) == bwd(ws=None) == -1
     assert bwd(k=0) == bwd(k=514) == -2 and bwd() == -3
+
+
+@pytest.mark.parametrize("labels", [(3, 2), (6,), (1, 2, 3), (2, 3, 1), (2, 1, 3)])
+def test_labels_of_another_arrangement_are_refused(labels):
+    """As many as there are positions, but not where they lie: which belongs to which is not guessed."""
+    with pytest.raises(ValueError, match="do not lie beside"):
+        top_logprobs_from_logits(torch.zeros(2, 3, 50), 3, torch.zeros(labels, dtype=torch.int64))
