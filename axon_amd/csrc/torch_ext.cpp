@@ -496,7 +496,7 @@ struct AlternativesNode : torch::autograd::Node {
     same_place(kWhat, x, {&at, &lab, &l, &ent, &g_en, &g_ids, &g_lab});
     const int dtype = logits_dtype(kWhat, x);
     const int64_t n = x.size(0), v = x.size(1), k = at.size(1);
-    if (x.stride(1) != 1 || (n > 1 && x.stride(0) < v)) refuse(kWhat, "logits must be [tokens, vocab] with unit stride over the vocabulary");
+    if ((v > 1 && x.stride(1) != 1) || (n > 1 && x.stride(0) < v)) refuse(kWhat, "logits must be [tokens, vocab] with unit stride over the vocabulary");
     same_type(kWhat, at::kFloat, {&l, &ent});
     if (!is_index(at) || (lab.defined() && !is_index(lab))) refuse(kWhat, "a saved tensor has come back in another type");
     same_len(kWhat, "lse", 2 * n, l);

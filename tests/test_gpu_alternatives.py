@@ -543,3 +543,16 @@ def test_forward_mode_is_refused():
     with fwd.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             top_logprobs_from_logits(fwd.make_dual(z, torch.ones_like(z)), 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_vocabulary_of_one_token_in_any_layout(dtype):
+    """Its stride says nothing: a column of a matrix, a transposed row."""
+    wide = torch.randn(5, 7, device="cuda", generator=gen(1)).to(dtype)
+    for z in (wide[:, :1], wide[:1, :5].t(), wide[:, 3:4], wide.t()[:5, 2:3]):
+        x = z.detach().requires_grad_(True)
+        r = top_logprobs_from_logits(x, 1, torch.zeros(5, dtype=torch.int64, device="cuda"))
+        lp, ent = token_logprobs_from_logits(x, torch.tensor([[0, 1]], device="cuda").expand(5, 2))
+        assert not any(t.any() for t in (r.top_ids, r.top_logprobs, r.logprobs, r.entropy, lp, ent))
+        grad, = torch.autograd.grad([r.top_logprobs.sum() + r.logprobs.sum() + lp.sum() + ent.sum()], x)
+        assert grad.shape == (5, 1) and grad.dtype == dtype and not grad.any()
