@@ -14,6 +14,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
@@ -660,25 +661,19 @@ struct RouterBalanceNode : torch::autograd::Node {
         if (c10::multiply_integers(shape) != r.n * r.experts * (stacked ? layers : 1)) refuse(kWhat, "the saved logits have another size");
       if (m.defined()) same_len(kWhat, "token_mask", r.n, m);
       const c10::DeviceGuard device(x[0].device());
-      // the gradients of a list of layers lie in one allocation, made without the dispatcher (48 allocations took the host 80 us,
-      // 48 views 25; as it is the whole backward takes 117, where autograd alone takes 98 to hand 48 ready tensors back)
-      const int64_t eb = (int64_t)x[0].element_size(), cells = r.n * r.experts, step = (cells + 7) / 8 * 8;
-      const Tensor all = at::empty({stacked ? 0 : step * layers}, x[0].options());
-      char* const base = static_cast<char*>(all.data_ptr());
+      // Every layer's gradient is a tensor with a storage of its own, which is kept, saved, resized or freed alone (48 of them,
+      // without the dispatcher: 80 us of host time more than one allocation that they share).
+      const int64_t eb = (int64_t)x[0].element_size(), cells = r.n * r.experts;
+      c10::Allocator* const allocator = at::empty({0}, x[0].options()).storage().allocator();  // the one of tensors on this device
       std::vector<void*> out(layers, nullptr);
       for (size_t i = 0; i < shapes.size(); ++i) {
         if (!task_should_compute_output(i)) continue;
-        const auto& shape = shapes[i];
-        c10::SmallVector<int64_t, 4> strides(shape.size(), 1);
-        for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) strides[d] = strides[d + 1] * std::max<int64_t>(shape[d + 1], 1);
-        if (stacked) {
-          grads[i] = at::empty(shape, x[0].options());
-          for (int64_t l = 0; l < layers; ++l) out[l] = static_cast<char*>(grads[i].data_ptr()) + l * cells * eb;
-        } else {
-          grads[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-          grads[i].unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides, (int64_t)i * step);
-          out[i] = base + (int64_t)i * step * eb;
-        }
+        grads[i] = at::detail::empty_generic(shapes[i], allocator, c10::DispatchKeySet(c10::DispatchKey::CUDA), x[0].scalar_type(),
+                                             std::nullopt);
+        char* const base = static_cast<char*>(grads[i].data_ptr());
+        if (!stacked) out[i] = base;
+        else
+          for (int64_t l = 0; l < layers; ++l) out[l] = base + l * cells * eb;
       }
       check(axon_router_balance_bwd(r.ptrs.data(), r.dtype, r.ld, layers, r.n, r.experts, ptr(m), mask_kind,
                                     (const int32_t*)ptr(offsets), seqs, score, (const float*)ptr(c), (const float*)ptr(sc),

@@ -422,3 +422,20 @@ def test_a_nan_counts_as_the_lowest_for_the_choices(e, k, dtype):
     low = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
     chosen = torch.sort(low.double(), dim=1, descending=True, stable=True).indices[:, :k]
     assert torch.equal(counts, torch.bincount(chosen.flatten(), minlength=e)) and torch.isnan(loss)
+
+
+@pytest.mark.parametrize("n,e", [(130, 40), (7, 3), (1, 1)])
+def test_every_layers_gradient_has_its_own_storage(n, e):
+    """What is kept, saved or resized of one layer's gradient is that layer's alone."""
+    xs, _, _ = case(4, n, e, 1, torch.bfloat16, 9)
+    xs = [x.requires_grad_(i != 2) for i, x in enumerate(xs)]
+    router_balance_loss(xs, 1)[0].backward()
+    grads = [x.grad for x in xs if x.grad is not None]
+    assert len(grads) == 3
+    for d in grads:
+        assert d.untyped_storage().nbytes() == n * e * 2 and d.storage_offset() == 0 and d.is_contiguous()
+    assert len({d.untyped_storage().data_ptr() for d in grads}) == 3
+    kept = [d.clone() for d in grads]
+    grads[0].add_(1)
+    grads[1].untyped_storage().resize_(0)
+    assert torch.equal(grads[2], kept[2]) and torch.equal(grads[0], kept[0] + 1)
