@@ -33,6 +33,7 @@ except Exception:  # pragma: no cover - transformers is optional for this mirror
 class CausalLMOutputForPPO(_Base):
     log_probs: torch.FloatTensor | None = None
     entropy: torch.FloatTensor | None = None
+    router_logits: tuple[torch.FloatTensor, ...] | None = None  # of a body with routed experts (no counterpart in the reference)
 
 
 def select_rolled_labels(pre_rolled_labels, labels, input_ids, backend: str = "forward_with_hip_backend"):
@@ -111,4 +112,5 @@ def forward_with_hip_backend(
         past_key_values=getattr(outputs, "past_key_values", None),
         hidden_states=getattr(outputs, "hidden_states", None),
         attentions=getattr(outputs, "attentions", None),
+        router_logits=getattr(outputs, "router_logits", None),
     )

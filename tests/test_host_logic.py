@@ -570,3 +570,28 @@ def test_several_tokens_through_the_head_keep_something_for_a_backward_that_can_
         m.linear_top_logprobs(hidden, weight, 2)
         m.linear_token_logprobs(hidden, weight, torch.zeros(3, 2, dtype=torch.int64))
     assert seen == [wanted, wanted]
+
+
+@pytest.mark.parametrize("routed", [True, False])
+def test_the_model_forward_passes_on_the_router_logits(monkeypatch, routed):
+    """What the body says of its routers reaches the output, for the balance term of the loss; a dense body has none."""
+    import types
+
+    from axon_amd.models.transformers import dense_common as m
+
+    monkeypatch.setattr(m, "linear_cross_entropy", lambda h, w, labels, *a: (torch.zeros(labels.shape), torch.ones(labels.shape)))
+    routers = (torch.randn(6, 4), torch.randn(6, 4))
+
+    class Outputs(tuple):
+        router_logits = routers
+
+    class Model:
+        config = types.SimpleNamespace(output_attentions=False, output_hidden_states=False)
+        lm_head = types.SimpleNamespace(weight=torch.zeros(10, 32))
+
+        def model(self, **kwargs):
+            return (Outputs if routed else tuple)((torch.zeros(1, 6, 32),))
+
+    out = m.forward_with_hip_backend(Model(), input_ids=torch.arange(6).view(1, 6), return_dict=True)
+    assert out.log_probs.shape == (1, 6) and out.entropy.shape == (1, 6)
+    assert out.router_logits is (routers if routed else None)
