@@ -48,18 +48,28 @@ class _SideTerms(torch.autograd.Function):
 
 
 def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
-    """``(balance loss, largest load of an expert relative to the mean of its layer)``, both on the device.  All tokens of a
-    packed batch count, in a padded one those of ``attention_mask`` (where the batch has it)."""
+    """``(balance loss, largest load of an expert relative to the mean of its layer, misfit)``, all on the device.  All tokens of
+    a packed batch count, in a padded one those of ``attention_mask`` (where the batch has it).  Routers that saw fewer tokens
+    than a padded batch has entries saw them packed (remove-padding): the mask's tokens, row after row; ``misfit`` (else None)
+    is how many tokens too many the mask has for that."""
     if router_logits is None:
         raise ValueError("router_aux_loss_coef is set, but the model returned no router_logits")
     if "router_top_k" not in args:
         raise ValueError("router_aux_loss_coef needs router_top_k, the experts per token")
-    mask, seqs = (b.get("attention_mask", None) if cu is None else None), None
-    if args.get("router_balance_per_sequence", False):
+    mask, seqs, misfit = (b.get("attention_mask", None) if cu is None else None), None, None
+    if isinstance(router_logits, torch.Tensor):  # [layers, tokens, experts] or [tokens, experts]
+        tokens = router_logits.shape[max(router_logits.dim() - 2, 0)]
+    else:
+        tokens = sum(t.numel() // max(t.shape[-1], 1) for t in router_logits[:1])
+    per_sequence = args.get("router_balance_per_sequence", False)
+    if mask is not None and tokens < mask.numel():
+        ends = (mask != 0).sum(-1).cumsum(0)
+        seqs = torch.nn.functional.pad(ends if per_sequence else ends[-1:], (1, 0)).to(torch.int32)
+        mask, misfit = None, (ends[-1] - tokens).float()
+    elif per_sequence:
         seqs = cu
         if seqs is None:  # padded: a row is a sequence
-            rows, one = entropy.shape[0], router_logits[0]  # a layer, where there are several
-            tokens = (one.numel() // one.shape[-1] if one.dim() > 1 else router_logits.shape[0])
+            rows = entropy.shape[0]
             length, odd = divmod(tokens, max(rows, 1))
             if odd:
                 raise ValueError(f"router_logits of {tokens} tokens do not belong to {rows} rows of one length")
@@ -68,7 +78,7 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
                                           expert_ids=router_expert_ids, score_fn=args.get("router_score_fn", "softmax"))
     counts = counts.view(-1, counts.shape[-1]).float()
     load = counts.amax(1) * counts.shape[1] / counts.sum(1).clamp(min=1)
-    return balance, load.max()
+    return balance, load.max(), misfit
 
 
 def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, router_expert_ids=None):
@@ -77,7 +87,8 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
     With ``loss_fn_args["router_aux_loss_coef"]`` the balance loss of ``router_logits`` times that coefficient is added, as
     the mean over the micro-batches of a step and the data-parallel replicas (the other terms are their sums: they are
     divided by counts over all of these), with ``router_top_k``, ``router_score_fn`` ("softmax") and
-    ``router_balance_per_sequence`` (False) from the same arguments.
+    ``router_balance_per_sequence`` (False) from the same arguments.  Routers that saw a padded batch packed (remove-padding)
+    are recognised by their number of tokens, which has to be that of ``attention_mask``.
 
     Returns ``(scaled_loss, metrics)``.  ``data.batch["log_probs"]`` is set; ``response_mask`` may be
     overwritten by the sampler correction hook, while the side terms keep the mask they were given
@@ -133,11 +144,13 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
     router_coef = loss_fn_args.get("router_aux_loss_coef", 0)
     router_vals = []
     if router_coef != 0:
-        balance, load = _router_term(b, cu, entropy, loss_fn_args, router_logits, router_expert_ids)
+        balance, load, misfit = _router_term(b, cu, entropy, loss_fn_args, router_logits, router_expert_ids)
         loss = loss + balance * (router_coef / (n_micro_batches * dp_replicas))
-        router_vals = [balance.detach(), load]
+        router_vals = [balance.detach(), load] + ([misfit] if misfit is not None else [])
     # one readback for pg_loss and the side-term metrics
     vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4], *router_vals]).tolist()
+    if vals[7:] and vals[7] != 0:
+        raise ValueError("router_logits are neither of the padded batch's tokens nor of those that attention_mask keeps")
     metrics["pg_loss"] = vals[0] * n_micro_batches
     metrics["entropy"] = vals[1] * n_micro_batches
     metrics["entropy_token_mean"] = vals[3] / max(vals[4], 1.0)

@@ -73,3 +73,16 @@ def test_the_c_entry_points_check_their_arguments():
     assert bwd(n=0) == 0
     for bad in (dict(x=None), dict(x=one), dict(coef=None), dict(scale=None), dict(g=None), dict(d=None), dict(d=odd)):
         assert bwd(**bad) == -1, bad
+
+
+@pytest.mark.parametrize("per_sequence", [False, True])
+def test_a_loss_term_without_layers_or_tokens(per_sequence):
+    """The operator's own errors, also where there is no layer or token to ask for its size."""
+    from axon_amd.models.fsdp_models import _router_term
+
+    args = {"router_top_k": 2, "router_balance_per_sequence": per_sequence}
+    with pytest.raises(ValueError, match="no layers"):
+        _router_term({}, None, torch.zeros(2, 3), args, [], None)
+    for router in (torch.zeros(0, 4), (torch.zeros(0, 4),), torch.zeros(3, 0, 4)):
+        with pytest.raises(_lib.AxonAmdError, match="no CPU fallback"):
+            _router_term({}, None, torch.zeros(2, 0), args, router, None)

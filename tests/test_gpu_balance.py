@@ -439,3 +439,45 @@ def test_every_layers_gradient_has_its_own_storage(n, e):
     grads[0].add_(1)
     grads[1].untyped_storage().resize_(0)
     assert torch.equal(grads[2], kept[2]) and torch.equal(grads[0], kept[0] + 1)
+
+
+@pytest.mark.parametrize("per_sequence", [False, True])
+@pytest.mark.parametrize("keep", [0.7, 0.05])
+def test_packed_routers_beside_a_padded_batch(per_sequence, keep):
+    """Remove-padding: the routers saw the tokens that attention_mask keeps, the batch and its outputs are padded."""
+    rows, length, e, k = 5, 60, 16, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    att = (torch.rand(rows, length, generator=g, device="cuda") < keep).long()
+    att[2] = 0  # a row of which nothing is left
+    att[0, 0] = 1
+    n = int(att.sum())
+    xs, _, _ = case(2, n, e, k, torch.float32, 6)
+    lp = torch.randn(rows, length, generator=g, device="cuda")
+    args = {"router_aux_loss_coef": 0.1, "router_top_k": k, "router_balance_per_sequence": per_sequence}
+
+    def run(router):
+        data = DataProto.from_dict(tensors={"old_log_probs": lp, "advantages": lp, "response_mask": torch.ones_like(lp),
+                                            "attention_mask": att})
+        meta = {"loss_fn": "ppo", "loss_fn_args": args, "dp_replicas": 1, "temperature": 1.0}
+        module = lambda inputs, m: {"log_probs": lp, "entropys": lp.abs(), "router_logits": router}  # noqa: E731
+        return CausalLM.forward_backward_fn(module, data, meta)
+
+    leaves = [x.clone().requires_grad_(True) for x in xs]
+    loss, metrics = run(leaves)
+    cu = torch.nn.functional.pad(att.sum(1).cumsum(0), (1, 0)).int() if per_sequence else None
+    want, counts = router_balance_loss(xs, k, cu_seqlens=cu)
+    load = (counts.amax(1) / counts.double().mean(1)).max().item()
+    assert metrics["router_balance_loss"] == want.item() and abs(metrics["router_max_load"] - load) <= 4 * 2.0 ** -24 * load
+    ref = reference(xs, k, None, cu, None, "softmax")
+    for d, r, size in zip(torch.autograd.grad(loss, leaves), ref[2], ref[3]):
+        assert ((d.double() - 0.1 * r).abs() <= 3 * REL * 0.1 * size + 1e-30).all()
+    assert run(torch.stack(xs))[1]["router_balance_loss"] == want.item()
+    for wrong in ([x[:-1] for x in xs], [torch.cat([x, x[:1]]) for x in xs]):
+        with pytest.raises(ValueError, match="attention_mask"):
+            run(wrong)
+    with pytest.raises(ValueError):  # more tokens than the batch has entries
+        run([torch.zeros(rows * length + 1, e, device="cuda")])
+    whole = [torch.randn(rows, length, e, generator=g, device="cuda")]
+    att_loss = router_balance_loss(whole, k, token_mask=att,
+                                   cu_seqlens=torch.arange(rows + 1, dtype=torch.int32, device="cuda") * length if per_sequence else None)[0]
+    assert run(whole)[1]["router_balance_loss"] == att_loss.item()
