@@ -1200,8 +1200,8 @@ def _logits_to_keep(n, h, v, dev):
     """Bytes of the logits that a forward over all ``n`` tokens leaves to its backward, or 0."""
     if n == 0 or h < TOP_KEEP_LOGITS_MIN_HIDDEN or h % 64 != 0:
         return 0
-    need = int(_lib.load().axon_lmhead_top_logits_bytes(n, h, v))
-    if need > TOP_LOGITS_BYTES or (not torch.cuda.is_current_stream_capturing() and not _fits_twice(need, dev)):
+    need = int(_lib.load().axon_lmhead_block_logits_bytes(n, h, v))
+    if need <= 0 or need > TOP_LOGITS_BYTES or (not torch.cuda.is_current_stream_capturing() and not _fits_twice(need, dev)):
         return 0
     return need
 

@@ -272,7 +272,7 @@ int axon_lmhead_block_can_group(int64_t hidden, int64_t vocab, int64_t vocab_chu
  *        tiles of 256): callers cut long batches into calls.
  *   _tokens_fwd: logprobs of the given ids (int32 or int64, 1 <= k <= 513), 0 for an id outside [0, vocab), and the
  *        entropy; workspace: axon_lmhead_fwd_workspace_bytes.  `logits` NULL: none are kept; else as above, for hidden sizes
- *        that are multiples of 64.
+ *        that are multiples of 64 below 2^21 (axon_lmhead_block_logits_bytes is not 0).
  *   _tokens_bwd: d_hidden and d_weight (bf16) from the gradients of these logprobs (g_logprobs) and of the entropy
  *        (g_entropy, may be NULL); `logprobs`, `lse`, `entropy_b` are what either forward returned for these ids.  Equal
  *        ids of a position add up, ids outside the vocabulary are left out.  `logits`: what either forward left there for

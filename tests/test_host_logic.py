@@ -595,3 +595,13 @@ def test_the_model_forward_passes_on_the_router_logits(monkeypatch, routed):
     out = m.forward_with_hip_backend(Model(), input_ids=torch.arange(6).view(1, 6), return_dict=True)
     assert out.log_probs.shape == (1, 6) and out.entropy.shape == (1, 6)
     assert out.router_logits is (routers if routed else None)
+
+
+def test_logits_are_kept_for_the_shapes_of_the_kernels_that_keep_them(monkeypatch):
+    """Hidden sizes whose rows are too long for the fast main loop recompute them, as those that are no multiple of 64."""
+    from axon_amd import _ops
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    kept = {h: _ops._logits_to_keep(3, h, 500, None) for h in (64, 768, 800, 832, (1 << 21) - 64, 1 << 21, (1 << 21) + 64)}
+    tiles = 2 * 262144  # 500 rows of the vocabulary, 3 tokens
+    assert kept == {64: 0, 768: tiles, 800: 0, 832: tiles, (1 << 21) - 64: tiles, 1 << 21: 0, (1 << 21) + 64: 0}
