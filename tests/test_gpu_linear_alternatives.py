@@ -399,3 +399,31 @@ def test_positions_with_one_likely_token(n, h, temperature, cap):
     assert at.sum() > n // 2 and torch.equal(r.top_logprobs[at, 0], plain[at])
     if not cap:
         assert torch.equal(plain, r.logprobs.clamp(max=0))
+
+
+def test_weight_gradients_on_both_sides_of_every_chunk_border():
+    """A backward in pieces of the vocabulary: rows of d_weight at the ends of every piece, and of ids' own, element by element."""
+    n, h, v, k = 16640, 64, 66048, 3
+    hid, w, lab = operands(n, h, v, 5)
+    ids = torch.stack([lab, (lab + 1) % v, torch.full_like(lab, -1)], 1)
+    g = torch.randn(n, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    g_en = torch.randn(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) * 0.1
+    lp, _, lse, mean, _ = _ops.lmhead_tokens(hid, w, ids)
+    _, d_w = _ops.lmhead_tokens_backward(g, g_en, hid, w, ids, lp, lse, mean)
+    pieces = sorted({c + i for c in range(0, v, 256) for i in (-1, 0)} & set(range(v)))  # whatever the pieces' length
+    rows = torch.tensor(sorted({*pieces, 1, v - 2, v - 1, *lab[:8].tolist(), *ids[:8, 1].tolist()}), device="cuda")
+    h64, w64 = hid.double(), w.double()
+    up, got = g[:, :2].double(), d_w[rows].double()
+    ref, off = torch.zeros_like(got), torch.zeros_like(got)
+    for a in range(0, n, 1664):
+        c = slice(a, a + 1664)
+        log_p = torch.log_softmax(h64[c] @ w64.t(), 1)
+        entropy = -(log_p.exp() * log_p).sum(1, keepdim=True)
+        z = log_p[:, rows]
+        p, G, ge = z.exp(), up[c].sum(1, keepdim=True), g_en[c, None].double()
+        same = [(ids[c, i, None] == rows).double() * up[c, i, None] for i in (0, 1)]
+        d = same[0] + same[1] - p * (G + ge * (z + entropy))
+        size = same[0].abs() + same[1].abs() + p * (up[c].abs().sum(1, keepdim=True) + ge.abs() * (z.abs() + entropy + 1))
+        ref += d.t() @ h64[c]
+        off += (2.0 ** -8 * d.abs() + 2 * ENT_TOL * size).t() @ h64[c].abs()
+    assert ((got - ref).abs() <= off + 2.0 ** -8 * ref.abs() + 1e-30).all()
