@@ -1185,8 +1185,12 @@ def token_ids_arg(what, ids, rows, device):
 # Bytes of fp32 logits that a call of the head with several tokens per position holds at most (2.5 GB: 4096 tokens of the
 # 151936 vocabulary).  A forward with alternatives cuts longer batches into blocks of tokens, never fewer than 256; a forward
 # of which a gradient is wanted leaves its logits to the backward where those of the whole call fit, and memory has room for
-# as much again.  From a hidden size of 768 on, where the product that recomputes them costs more than writing and reading them;
-# the gradients are the same bit for bit.
+# as much again.  From a hidden size of 768 on: the product that recomputes them costs more than writing and reading them from 512
+# to 640 on, by 5 % and more from 768 on (16 given tokens, kept / recomputed, us: 1001 x h x 151936 h 256 613 / 554, 512 745 /
+# 745, 640 864 / 892, 768 900 / 960, 1024 1066 / 1170; 3000 x h x 32768 512 460 / 456, 768 584 / 620), below it the memory
+# is not worth it.  A pass that the host bounds pays 20 us for the look at the memory (61 x 1024 x 32768 240 / 225).  The
+# gradients of alternatives are the same bit for bit; given tokens' log-probabilities come from the product where the logits
+# are kept and from a dot per token where they are not, and differ in the last bits of 32, as their gradients then do.
 TOP_LOGITS_BYTES = 2560 << 20
 TOP_KEEP_LOGITS_MIN_HIDDEN = 768
 

@@ -293,7 +293,7 @@ __device__ __forceinline__ void each_run(const BalanceParams& p, int c0, int c1,
   }
 }
 
-// Workgroup (chunk, layer).  48 layers x 8192 x 128 bf16, 8 choices: 61 us, where one read of the logits is 21: bound by
+// Workgroup (chunk, layer).  48 layers x 8192 x 128 bf16, 8 choices: 65 us, where one read of the logits is 21: bound by
 // instructions, those of the choices (a sort of a lane's eight keys, then eight times the largest head of sixteen lanes): with
 // given choices it is 27 us.
 template <typename T, int G, int V, int SCORE, int MASK>

@@ -11,7 +11,9 @@ them and a student that is trained on them need more (the reference has no such 
   of 32; outputs are fp32 in the shape of ``hidden`` without its last dimension (and with ``k`` behind it);
 * both are differentiable with respect to ``hidden`` and ``weight`` through log-probabilities and entropy; the ids of the
   alternatives are constants.  The backward takes the fp32 logits that the forward has kept for it where those of all
-  tokens take at most 2.5 GB (and memory has room for as much again), and recomputes them else, to the same gradients;
+  tokens take at most 2.5 GB (and memory has room for as much again), and recomputes them else: to the same gradients of
+  alternatives, bit for bit, while the log-probabilities of given tokens, which come from the kept logits or from a dot per
+  token, and their gradients may differ in the last bits;
 * the alternatives (at most 128) are ordered by the product's fp32 result, before temperature and soft cap (which keep that
   order, but may round different logits to one), equal ones by ascending id; a position's fp32 logits are held while its
   block of tokens is selected from (2.5 GB whatever the number of tokens), never all of them;
