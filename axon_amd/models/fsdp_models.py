@@ -63,7 +63,7 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
         tokens = sum(t.numel() // max(t.shape[-1], 1) for t in router_logits[:1])
     per_sequence = args.get("router_balance_per_sequence", False)
     if mask is not None and tokens < mask.numel():
-        ends = (mask != 0).sum(-1).cumsum(0)
+        ends = (mask != 0).reshape(-1, mask.shape[-1]).sum(-1).cumsum(0)
         seqs = torch.nn.functional.pad(ends if per_sequence else ends[-1:], (1, 0)).to(torch.int32)
         mask, misfit = None, (ends[-1] - tokens).float()
     elif per_sequence:

@@ -96,9 +96,10 @@ class TopLogprobs(NamedTuple):
 def top_logprobs_from_logits(logits: torch.Tensor, k: int, labels: torch.Tensor | None = None,
                              inplace_backward: bool = False) -> TopLogprobs:
     """The ``k`` best tokens (at most 128) of every position of ``logits`` ``[..., vocab]`` (fp32 or bf16, already divided
-    by the temperature): see ``TopLogprobs``.  Equal logits are ordered by ascending id.  ``labels`` ``[...]``, in the same arrangement: also the
-    log-probability of these (0 for a label outside the vocabulary).  Differentiable with respect to the logits; the
-    ids are constants.  A position whose logits hold a NaN, or nothing but -inf, has NaN log-probabilities."""
+    by the temperature): see ``TopLogprobs``.  Equal logits are ordered by ascending id.  ``labels`` ``[...]``, in the same
+    arrangement: also the log-probability of these (0 for a label outside the vocabulary).  Differentiable with respect to
+    the logits; the ids are constants.  A position whose logits hold a NaN, or nothing but -inf, has NaN
+    log-probabilities."""
     if isinstance(k, bool) or not isinstance(k, int):
         raise TypeError(f"top_logprobs_from_logits: k must be an int, got {type(k).__name__}")
     return TopLogprobs(*_lib.native().top_logprobs(logits, min(k, 1 << 40), labels, bool(inplace_backward)))

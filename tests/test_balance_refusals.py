@@ -86,3 +86,12 @@ def test_a_loss_term_without_layers_or_tokens(per_sequence):
     for router in (torch.zeros(0, 4), (torch.zeros(0, 4),), torch.zeros(3, 0, 4)):
         with pytest.raises(_lib.AxonAmdError, match="no CPU fallback"):
             _router_term({}, None, torch.zeros(2, 0), args, router, None)
+
+
+def test_an_attention_mask_of_one_dimension_is_one_row():
+    """Beside packed routers too: the operator itself refuses what is not on a GPU."""
+    from axon_amd.models.fsdp_models import _router_term
+
+    for router in (torch.zeros(4, 8), torch.zeros(6, 8)):
+        with pytest.raises(_lib.AxonAmdError, match="no CPU fallback"):
+            _router_term({"attention_mask": torch.ones(6, dtype=I64)}, None, torch.zeros(1, 6), {"router_top_k": 2}, router, None)
