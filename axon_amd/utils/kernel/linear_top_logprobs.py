@@ -16,7 +16,8 @@ them and a student that is trained on them need more (the reference has no such 
   token, and their gradients may differ in the last bits;
 * the alternatives (at most 128) are ordered by the product's fp32 result, before temperature and soft cap (which keep that
   order, but may round different logits to one), equal ones by ascending id; a position's fp32 logits are held while its
-  block of tokens is selected from (2.5 GB whatever the number of tokens), never all of them;
+  block of tokens is selected from (2.5 GB whatever the number of tokens), never all of them.  A label that is one of them
+  has its log-probability from a dot of its own, which may differ from the alternative's in the last bits;
 * given tokens (at most 512 per position): an id outside the vocabulary is a filler, with log-probability 0 and no gradient;
   an id may occur more than once.
 """
