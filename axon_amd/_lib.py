@@ -100,6 +100,11 @@ SIGNATURES: dict[str, tuple] = {
                                        _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "axon_router_balance_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i32, _ptr, _i64, _i32, _ptr, _ptr, _ptr,
                                        _ptr, _ptr]),
+    "axon_controls_apply": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr]),
+    "axon_controls_apply_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
+    "axon_controls_logprob_workspace_bytes": (_i64, [_i64, _i64]),
+    "axon_controls_logprob_fwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "axon_controls_logprob_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "axon_reverse_scan": (_i32, [_i32, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i64, _i64, _f32, _f32, _ptr, _ptr, _ptr,
                                  _ptr]),
     "axon_masked_whiten_workspace_bytes": (_i64, [_i64]),
@@ -147,7 +152,21 @@ SIGNATURES: dict[str, tuple] = {
                                         _ptr, _ptr, _f32, _i32, _ptr, _f32, _f32, _f32, _ptr, _ptr, _ptr]),
 }
 
-ABI_VERSION = 27
+ABI_VERSION = 28
+
+
+class ControlsStruct(ctypes.Structure):
+    """``axon_controls`` of the header."""
+
+    _fields_ = [("token_ids", _ptr), ("n_tokens", _i64), ("n_seqs", _i64), ("uniform_len", _i64), ("cu_seqlens", _ptr),
+                ("own_mask", _ptr), ("token_ids_i64", _i32), ("mask_kind", _i32), ("every_position", _i32),
+                ("bias_ids_i64", _i32), ("bias_per_seq", _i32), ("allowed_index_i64", _i32), ("repetition", _ptr),
+                ("frequency", _ptr), ("presence", _ptr), ("temperature", _ptr), ("repetition_all", _f32),
+                ("frequency_all", _f32), ("presence_all", _f32), ("temperature_all", _f32), ("bias_ids", _ptr),
+                ("bias", _ptr), ("n_bias", _i64), ("allowed", _ptr), ("allowed_rows", _i64), ("allowed_stride", _i64),
+                ("allowed_index", _ptr)]
+
+
 MASK_F32, MASK_I64 = 0, 1
 
 _lock = threading.Lock()

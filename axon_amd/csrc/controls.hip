@@ -1,0 +1,544 @@
+// What a sampler does to a position's logits before it draws: penalties for tokens that the sequence holds already, biases,
+// a grammar's mask, the temperature.  Written out (for a decoder), or as the log-probability of a label and the entropy of
+// what is left (for a trainer, which has to score a rollout under the distribution that it was drawn from), forward and
+// backward.
+//
+//   y_j = (z_j > 0 ? z_j / rep : z_j rep  where j is in the row's history)  - freq count_j - pres [count_j > 0] + bias_j,
+//   -inf where the row's mask has a 0 bit;  out = y / T;  log p = out - logsumexp(out).
+//
+// A wavefront owns 2048 consecutive ids of the vocabulary and walks a run of rows: the ids stay the same from row to row,
+// so what the histories do to them is kept where it is used (the sum of the additive terms in LDS, whether an id was
+// seen in a bit of the owning lane), and a row of a packed batch differs from the row before by ONE token.  Vectors are
+// loaded at whatever boundary a row of an odd vocabulary starts on, so that lanes keep their ids.
+#include "logits_rows.h"
+
+namespace axon {
+
+constexpr int kIds = 2048;               // ids of a wavefront
+constexpr int kLaneIds = kIds / kWave;   // 32, one bit each
+constexpr int kWaves = kBlock / kWave;
+constexpr int kGroupIds = kIds * kWaves;  // ids of a workgroup
+constexpr int kMaxRun = kWave;            // rows of a run: a lane holds what belongs to a row
+
+enum Mode { kStats, kGrad, kApply, kApplyGrad };
+
+// 16-byte vectors on any boundary of their elements.
+template <typename T> struct Unaligned;
+template <> struct Unaligned<float> {
+  static constexpr int kPer = 4;
+  typedef f32x4 Raw;
+  struct __attribute__((packed, aligned(4))) Box { Raw v; };
+  __device__ static Raw load(const float* p) { return reinterpret_cast<const Box*>(p)->v; }
+  __device__ static float get(const Raw& r, int j) { return r[j]; }
+  __device__ static void store(float* p, const float* v) {
+    Box b;
+    b.v = Raw{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<Box*>(p) = b;
+  }
+};
+template <> struct Unaligned<unsigned short> {
+  static constexpr int kPer = 8;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+  struct __attribute__((packed, aligned(2))) Box { Raw v; };
+  __device__ static Raw load(const unsigned short* p) { return reinterpret_cast<const Box*>(p)->v; }
+  __device__ static float get(const Raw& r, int j) {
+    return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16));
+  }
+  __device__ static void store(unsigned short* p, const float* v) {
+    Box b;
+    b.v = Raw{f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
+    *reinterpret_cast<Box*>(p) = b;
+  }
+};
+
+__device__ __forceinline__ int64_t index_at(const void* p, int i64, int64_t at) {
+  return i64 ? static_cast<const int64_t*>(p)[at] : (int64_t) static_cast<const int32_t*>(p)[at];
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// What one lane has written to LDS, for the others of its wavefront: LDS serves a wavefront in order, the compiler is told to.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+constexpr float kNoLogit = -3.402823466e38f;  // the reference of a set without a logit: any there is is at least as large
+
+// A token of a history: its id, or -1 where it counts for nothing; bit 30 where the model has generated it.
+constexpr int kOwn = 1 << 30;
+__device__ __forceinline__ int history_token(const axon_controls& c, int64_t at, int vocab) {
+  const int64_t id = index_at(c.token_ids, c.token_ids_i64, at);
+  if (id < 0 || id >= vocab) return -1;
+  const bool own = c.own_mask == nullptr || (c.mask_kind == AXON_MASK_I64 ? static_cast<const int64_t*>(c.own_mask)[at] != 0
+                                                                         : static_cast<const float*>(c.own_mask)[at] != 0.f);
+  return (int)id | (own ? kOwn : 0);
+}
+
+// The additive part of what controls do to one id.
+__device__ __forceinline__ float penalty(int count, float frequency, float presence) {
+  return count > 0 ? fmaf(frequency, (float)count, presence) : 0.f;
+}
+
+struct RowIo {
+  const void* labels;  // [rows]
+  int labels_i64;
+  float* label_y;             // [rows], kStats
+  float4* parts;              // [rows][chunks] (M, s, e), kStats
+  const float* stats;         // [3][rows]: the row's log-sum-exp in two parts and its entropy, kGrad
+  const float *g_logprob, *g_entropy;
+};
+
+// The additive terms of a wavefront's ids in LDS, in the order in which the lanes read them: 16 bytes of neighbouring
+// lanes lie side by side.
+template <int PER>
+__device__ __forceinline__ int slot(int off) {
+  return PER == 4 ? off : (off & ~511) | ((off & 4) << 6) | ((off & 0x1f8) >> 1) | (off & 3);
+}
+
+template <typename T, Mode MODE, bool ADJ, bool MASK>
+__global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
+                                                          axon_controls c, RowIo io, const T* other, int64_t ld_other, T* out,
+                                                          int64_t ld_out) {
+  constexpr int kPer = Unaligned<T>::kPer, kVecs = kLaneIds / kPer;
+  __shared__ uint32_t s_adj[ADJ ? kGroupIds : 1];  // counts (bit 31: seen) while they are collected, then floats
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int groups = (chunks + kWaves - 1) / kWaves;
+  const int first = (int)(blockIdx.x / groups) * run, group = (int)(blockIdx.x % groups);
+  const int last = min(first + run, n_rows);
+  const int chunk = group * kWaves + wave, base = chunk * kIds;
+
+  // what belongs to row first + lane
+  const int mine = min(first + lane, n_rows - 1);
+  int seq = 0, start = 0, state = -1, label = -1, token = -1;
+  const int64_t n_seqs = c.n_seqs;
+  if (n_seqs > 0) {
+    if (!c.every_position) seq = mine;
+    else if (c.uniform_len > 0) seq = (int)(mine / c.uniform_len);
+    else seq = RowFinder::upper4(c.cu_seqlens, 0, (int)n_seqs, mine);
+    seq = min(max(seq, 0), (int)n_seqs - 1);
+  }
+  int64_t begin = 0, end = 0;  // the row's history
+  if (ADJ && c.token_ids != nullptr) {
+    begin = c.uniform_len > 0 ? (int64_t)seq * c.uniform_len : (int64_t)c.cu_seqlens[seq];
+    end = c.uniform_len > 0 ? begin + c.uniform_len : (int64_t)c.cu_seqlens[seq + 1];
+    if (c.every_position) {
+      if (mine < begin || mine >= end) begin = mine + 1;  // a position of no sequence
+      end = (int64_t)mine + 1;
+    }
+    begin = max(begin, (int64_t)0);
+    end = min(end, c.n_tokens);
+    start = (int)begin;
+    if (c.every_position && begin < end) token = history_token(c, end - 1, vocab);
+  } else {
+    start = c.bias_per_seq ? seq : 0;  // no history: rows differ where their biases do
+  }
+  const float rep_l = c.repetition ? c.repetition[seq] : c.repetition_all;
+  const float freq_l = c.frequency ? c.frequency[seq] : c.frequency_all;
+  const float pres_l = c.presence ? c.presence[seq] : c.presence_all;
+  const float inv_t_l = 1.f / (c.temperature ? c.temperature[seq] : c.temperature_all);
+  if (MASK) {
+    const int64_t s = c.allowed_index ? index_at(c.allowed_index, c.allowed_index_i64, mine) : (c.allowed_rows == 1 ? 0 : mine);
+    state = s >= 0 && s < c.allowed_rows ? (int)s : -1;
+  }
+  if (MODE == kStats || MODE == kGrad) {
+    const int64_t l = index_at(io.labels, io.labels_i64, mine);
+    label = l >= 0 && l < vocab ? (int)l : -1;
+  }
+  float lse_l = 0.f, rest_l = 0.f, ent_l = 0.f, glp_l = 0.f, gen_l = 0.f;
+  if (MODE == kGrad) {
+    lse_l = io.stats[mine];
+    rest_l = io.stats[(int64_t)n_rows + mine];
+    ent_l = io.stats[2 * (int64_t)n_rows + mine];
+    glp_l = io.g_logprob && label >= 0 ? io.g_logprob[mine] : 0.f;
+    gen_l = io.g_entropy ? io.g_entropy[mine] : 0.f;
+  }
+
+  uint32_t* const adj = s_adj + (ADJ ? wave * kIds : 0);
+  const float* const adj_f = reinterpret_cast<const float*>(adj);
+  uint32_t seen = 0;  // bit u * kPer + j: this lane's id of vector u, element j
+  uint32_t touched = 0;  // bit u: some lane's vector u is not left as it is
+  // counts and seen bits in LDS to additive terms, biases with them
+  auto settle = [&](int row) {
+    const float f = lane_value(freq_l, row), a = lane_value(pres_l, row);
+    const int sq = lane_value(seq, row);
+    uint32_t any = 0;
+    seen = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      uint32_t some = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = slot<kPer>((u * kWave + lane) * kPer + j);
+        const uint32_t w = adj[at];
+        some |= w;
+        seen |= (w >> 31) << (u * kPer + j);
+        adj[at] = __float_as_uint(penalty((int)(w & 0x7fffffffu), f, a));
+      }
+      if (__any(some != 0)) any |= 1u << u;
+    }
+    wave_sync();
+    for (int64_t i0 = 0; i0 < c.n_bias; i0 += kWave) {
+      const int64_t i = i0 + lane, at = (c.bias_per_seq ? (int64_t)sq * c.n_bias : 0) + i;
+      const int64_t off = i < c.n_bias ? index_at(c.bias_ids, c.bias_ids_i64, at) - base : -1;
+      const bool in = off >= 0 && off < kIds && off + base < vocab;
+      if (in) atomicAdd(reinterpret_cast<float*>(adj) + slot<kPer>((int)off), -c.bias[at]);
+      const int u = in ? (int)off / (kWave * kPer) : -1;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v)
+        if (__any(u == v)) any |= 1u << v;
+    }
+    touched = any;
+    wave_sync();
+  };
+
+  if (ADJ) {  // the history before the run's first row, by the whole workgroup (of the row itself, where a row is a sequence)
+    for (int i = tid; i < kGroupIds; i += kBlock) s_adj[i] = 0;
+    __syncthreads();
+    const int from = lane_value(start, 0);
+    const int64_t upto = c.every_position ? first : lane_value((int)end, 0);  // offsets are 32-bit integers
+    if (c.token_ids != nullptr)
+      for (int64_t i = from + tid; i < upto; i += kBlock) {
+        const int t = history_token(c, i, vocab);
+        const int off = t < 0 ? -1 : (t & (kOwn - 1)) - group * kGroupIds;
+        if (off >= 0 && off < kGroupIds) {
+          uint32_t* const w = s_adj + (off & ~(kIds - 1)) + slot<kPer>(off & (kIds - 1));
+          atomicOr(w, 0x80000000u);
+          if (t & kOwn) atomicAdd(w, 1u);
+        }
+      }
+    __syncthreads();
+  }
+  if (chunk >= chunks) return;
+  if (ADJ) settle(0);
+
+  const bool whole = base + kIds <= vocab;
+  for (int r = 0; r < last - first; ++r) {
+    const int64_t row = first + r;
+    const float rep = lane_value(rep_l, r), inv_rep = 1.f / rep, inv_t = lane_value(inv_t_l, r);
+    if (ADJ && c.every_position) {
+      if (r > 0 && lane_value(start, r) != lane_value(start, r - 1)) {  // another sequence
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) adj[i * kWave + lane] = 0;
+        wave_sync();
+        settle(r);
+      }
+      const int t = lane_value(token, r);
+      const int id = t & (kOwn - 1), off = id - base;
+      if (t >= 0 && off >= 0 && off < kIds) {  // the row's own token, counted anew: a sum of additions would drift
+        const int u = off / (kWave * kPer), at = off / kPer % kWave, j = off % kPer;
+        if (lane == at) seen |= 1u << (u * kPer + j);
+        touched |= 1u << u;
+        if (t & kOwn) {
+          int count = 0;
+          for (int64_t i = lane_value(start, r) + lane; i <= row; i += kWave) count += history_token(c, i, vocab) == t;
+          count = (int)wave_sum((float)count);
+          float b = 0.f;
+          const int64_t at_bias = c.bias_per_seq ? (int64_t)lane_value(seq, r) * c.n_bias : 0;
+          for (int64_t i = 0; i < c.n_bias; ++i)
+            if (index_at(c.bias_ids, c.bias_ids_i64, at_bias + i) == id) b += c.bias[at_bias + i];
+          if (lane == at) adj[slot<kPer>(off)] = __float_as_uint(penalty(count, lane_value(freq_l, r), lane_value(pres_l, r)) - b);
+          wave_sync();
+        }
+      }
+    }
+    const T* const x = logits + row * ld + base;
+    const int st = MASK ? lane_value(state, r) : -1;
+    const uint8_t* const words = reinterpret_cast<const uint8_t*>(c.allowed + (int64_t)(st < 0 ? 0 : st) * c.allowed_stride);
+
+    float z[kLaneIds], y[kLaneIds];
+    auto read = [&](const T* from, float (&v)[kLaneIds]) {
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        const int id0 = (u * kWave + lane) * kPer;
+        if (whole || base + id0 + kPer <= vocab) {
+          const auto raw = Unaligned<T>::load(from + id0);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) v[u * kPer + j] = Unaligned<T>::get(raw, j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) v[u * kPer + j] = base + id0 + j < vocab ? Row<T>::one(from + id0 + j) : -INFINITY;
+        }
+      }
+    };
+    read(x, z);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int id0 = (u * kWave + lane) * kPer;
+      uint32_t keep = (1u << kPer) - 1;
+      if (MASK && st >= 0) keep = base + id0 < vocab ? (uint32_t)words[(base + id0) >> 3] >> (id0 & 7) : 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = u * kPer + j;
+        float v = z[i];
+        if (ADJ && (touched >> u & 1)) {
+          if (seen >> i & 1) v = v > 0.f ? v * inv_rep : v * rep;
+          v -= adj_f[slot<kPer>(id0 + j)];
+        }
+        y[i] = (MASK && !(keep >> j & 1)) ? -INFINITY : v;
+      }
+    }
+
+    if (MODE == kStats) {
+      float m = y[0];
+#pragma unroll
+      for (int i = 1; i < kLaneIds; ++i) m = fmaxf(m, y[i]);
+      m = wave_max(m);
+      const float M = m > -INFINITY ? m : kNoLogit, k = inv_t * kLog2e;
+      float s4[4] = {}, e4[4] = {};
+#pragma unroll
+      for (int i = 0; i < kLaneIds; ++i) {
+        const float d = (y[i] - M) * k, f = __builtin_amdgcn_exp2f(d);
+        s4[i & 3] += f;
+        e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
+      }
+      const float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
+      if (lane == 0) io.parts[row * chunks + chunk] = make_float4(M, s, e, 0.f);
+      const int l = lane_value(label, r) - base;
+      if (l >= 0 && l < kIds) {
+        const int i = l / (kWave * kPer) * kPer + l % kPer;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < kLaneIds; ++q) v = q == i ? y[q] : v;
+        if (lane == l / kPer % kWave) io.label_y[row] = v;
+      }
+    } else {
+      float* const d = z;  // what is written
+      if (MODE == kApply) {
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) d[i] = y[i] * inv_t;
+      } else {
+        float up[kLaneIds];
+        if (MODE == kApplyGrad) {
+          read(other + row * ld_other + base, up);
+        } else {
+          const float lse = lane_value(lse_l, r), rest = lane_value(rest_l, r), H = lane_value(ent_l, r);
+          const float g_lp = lane_value(glp_l, r), g_en = lane_value(gen_l, r), k = inv_t * kLog2e;
+          const int l = lane_value(label, r) - base;
+          const int at = l >= 0 && l < kIds && lane == l / kPer % kWave ? l / (kWave * kPer) * kPer + l % kPer : -1;
+#pragma unroll
+          for (int i = 0; i < kLaneIds; ++i) {
+            const float t = fmaf(y[i] - lse, k, -rest), p = __builtin_amdgcn_exp2f(t);
+            // a probability of 0 takes nothing from the entropy
+            up[i] = p * (p > 0.f ? fmaf(-g_en, fmaf(t, kLn2, H), -g_lp) : -g_lp) + (i == at ? g_lp : 0.f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) {
+          float slope = inv_t;
+          if (ADJ && (touched >> (i / kPer) & 1) && (seen >> i & 1)) slope *= z[i] > 0.f ? inv_rep : rep;
+          d[i] = y[i] == -INFINITY ? 0.f : up[i] * slope;
+        }
+      }
+      T* const o = out + row * ld_out + base;
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        const int id0 = (u * kWave + lane) * kPer;
+        if (whole || base + id0 + kPer <= vocab) {
+          Unaligned<T>::store(o + id0, d + u * kPer);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (base + id0 + j < vocab) Row<T>::store_one(o + id0 + j, d[u * kPer + j]);
+        }
+      }
+    }
+  }
+}
+
+// A row's chunks together, by a wavefront, in 64 bits: log-probability of the label, entropy, and what the backward reads.
+// In units of y (before the temperature T): lse = T ln sum exp(y / T) rounded to 32 bits, and in log2 units what that rounding has
+// left, so that log2 p = (y - lse) log2(e) / T - rest.
+__global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int vocab, int chunks, axon_controls c, RowIo io,
+                                                                 float* logprob, float* entropy, float* stats) {
+  const int row = (int)(blockIdx.x * kWaves + threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+  if (row >= n_rows) return;
+  float M = kNoLogit;
+  for (int i = lane; i < chunks; i += kWave) M = fmaxf(M, io.parts[(int64_t)row * chunks + i].x);
+  M = wave_max(M);
+  float inv_t = 1.f / c.temperature_all;
+  if (c.temperature != nullptr) {
+    int64_t seq = !c.every_position ? row : c.uniform_len > 0 ? row / c.uniform_len : RowFinder::upper4(c.cu_seqlens, 0, (int)c.n_seqs, row);
+    inv_t = 1.f / c.temperature[min(max(seq, (int64_t)0), c.n_seqs - 1)];
+  }
+  const float k = inv_t * kLog2e;
+  double s = 0.0, e = 0.0;
+  for (int i = lane; i < chunks; i += kWave) {
+    const float4 p = io.parts[(int64_t)row * chunks + i];
+    const float d = fmaxf((p.x - M) * k, kTiny), f = __builtin_amdgcn_exp2f(d);
+    s += (double)p.y * f;
+    e += (double)(f * fmaf(p.y, d, p.z));
+  }
+  s = wave_sum_d(s);
+  e = wave_sum_d(e);
+  if (lane != 0) return;
+  float lse = 0.f, rest = 0.f, H = 0.f, lp = 0.f;
+  const int64_t l = index_at(io.labels, io.labels_i64, row);
+  const bool inside = l >= 0 && l < vocab;
+  if (s == 0.0) {  // nothing is left
+    lp = inside ? -INFINITY : 0.f;
+  } else {
+    const double log2_s = log2(s);
+    lse = (float)((double)M + log2_s / (double)k);
+    rest = (float)(((double)M - (double)lse) * (double)k + log2_s);
+    H = (float)((log2_s - e / s) * 0.6931471805599453);
+    if (inside) lp = (float)((((double)io.label_y[row] - (double)lse) * (double)k - (double)rest) * 0.6931471805599453);
+  }
+  logprob[row] = lp;
+  if (entropy != nullptr) entropy[row] = H;
+  stats[row] = lse;
+  stats[(int64_t)n_rows + row] = rest;
+  stats[2 * (int64_t)n_rows + row] = H;
+}
+
+}  // namespace axon
+
+using namespace axon;
+
+namespace {
+
+int elem_bytes(int dtype) { return dtype == AXON_LOGITS_F32 ? 4 : 2; }
+
+int check_rows(const void* p, int dtype, int64_t ld, int64_t n, int64_t v) {
+  if (n < 0 || v <= 0 || ld < v || (dtype != AXON_LOGITS_F32 && dtype != AXON_LOGITS_BF16)) return AXON_ERR_ARG;
+  if (n >= (int64_t)1 << 24 || v >= kOwn) return AXON_ERR_SHAPE;
+  if (n > 0 && (!p || reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype) != 0)) return AXON_ERR_ARG;
+  return AXON_OK;
+}
+
+// Whether the operands of the controls are there and belong to n rows.
+int check_controls(const axon_controls* c, int64_t n, int64_t v) {
+  if (!c || c->n_seqs < 0 || c->n_tokens < 0 || c->uniform_len < 0 || c->n_bias < 0 || c->allowed_rows < 0) return AXON_ERR_ARG;
+  if (n == 0) return AXON_OK;
+  if (c->n_seqs >= INT32_MAX || c->n_tokens >= INT32_MAX || c->n_bias >= INT32_MAX || c->allowed_rows >= INT32_MAX) return AXON_ERR_SHAPE;
+  const bool per_seq = c->repetition || c->frequency || c->presence || c->temperature || (c->n_bias && c->bias_per_seq) || c->token_ids;
+  if (per_seq) {
+    if (c->n_seqs == 0) return AXON_ERR_ARG;
+    if (c->uniform_len > 0) {
+      if (c->n_seqs > INT32_MAX / c->uniform_len) return AXON_ERR_SHAPE;
+      if (c->token_ids && c->n_seqs * c->uniform_len != c->n_tokens) return AXON_ERR_SHAPE;
+      if (c->every_position && n != c->n_seqs * c->uniform_len) return AXON_ERR_SHAPE;
+    } else if (!c->cu_seqlens && (c->every_position || c->token_ids)) {
+      return AXON_ERR_ARG;
+    }
+    if (!c->every_position && n != c->n_seqs) return AXON_ERR_SHAPE;
+    if (c->every_position && c->token_ids && n != c->n_tokens) return AXON_ERR_SHAPE;
+  }
+  if (c->mask_kind != AXON_MASK_F32 && c->mask_kind != AXON_MASK_I64) return AXON_ERR_ARG;
+  if (c->n_bias > 0 && (!c->bias_ids || !c->bias)) return AXON_ERR_ARG;
+  if (c->allowed) {
+    if (c->allowed_rows < 1 || c->allowed_stride < (v + 31) / 32) return AXON_ERR_SHAPE;
+    if (!c->allowed_index && c->allowed_rows != 1 && c->allowed_rows != n) return AXON_ERR_SHAPE;
+  }
+  const auto positive = [](float x) { return x > 0.f && x <= 3.402823466e38f; };
+  const auto finite = [](float x) { return x - x == 0.f; };
+  if (!c->repetition && !positive(c->repetition_all)) return AXON_ERR_ARG;
+  if (!c->temperature && !positive(c->temperature_all)) return AXON_ERR_ARG;
+  if ((!c->frequency && !finite(c->frequency_all)) || (!c->presence && !finite(c->presence_all))) return AXON_ERR_ARG;
+  return AXON_OK;
+}
+
+int chunks_of(int64_t vocab) { return (int)((vocab + kIds - 1) / kIds); }
+
+// Rows of a run: about eight rounds of the 4096 wavefronts that the part holds.
+int run_of(int64_t n, int64_t vocab) {
+  const int64_t r = n * chunks_of(vocab) / (8 * 4096);
+  return (int)(r < 1 ? 1 : (r < kMaxRun ? r : kMaxRun));
+}
+
+template <Mode MODE>
+int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls& given, const RowIo& io,
+           const void* other, int64_t ld_other, void* out, int64_t ld_out, hipStream_t st) {
+  axon_controls c = given;
+  const bool penalties = c.repetition || c.frequency || c.presence || c.repetition_all != 1.f || c.frequency_all != 0.f || c.presence_all != 0.f;
+  if (!penalties) c.token_ids = nullptr;  // nobody asks for the history
+  const bool adj = (penalties && c.token_ids) || c.n_bias > 0, mask = c.allowed != nullptr;
+  const int chunks = chunks_of(vocab), groups = (chunks + kWaves - 1) / kWaves;
+  const int run = adj && !c.every_position ? 1 : run_of(n, vocab);
+  const int64_t grid = (n + run - 1) / run * groups;
+  if (grid >= INT32_MAX) return AXON_ERR_SHAPE;
+#define AXON_CONTROLS(T, A, M)                                                                                             \
+  hipLaunchKernelGGL((controls_kernel<T, MODE, A, M>), dim3((unsigned)grid), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
+                     (int)n, (int)vocab, chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out)
+#define AXON_CONTROLS_OF(T)                                  \
+  do {                                                       \
+    if (adj && mask) AXON_CONTROLS(T, true, true);           \
+    else if (adj) AXON_CONTROLS(T, true, false);             \
+    else if (mask) AXON_CONTROLS(T, false, true);            \
+    else AXON_CONTROLS(T, false, false);                     \
+  } while (0)
+  if (dtype == AXON_LOGITS_F32) AXON_CONTROLS_OF(float);
+  else AXON_CONTROLS_OF(unsigned short);
+#undef AXON_CONTROLS_OF
+#undef AXON_CONTROLS
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+}  // namespace
+
+extern "C" int axon_controls_apply(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
+                                   void* out, int64_t ld_out, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK) rc = check_rows(out, dtype, ld_out, n, vocab);
+  if (rc == AXON_OK) rc = check_controls(controls, n, vocab);
+  if (rc != AXON_OK || n == 0) return rc;
+  return launch<kApply>(logits, dtype, ld, n, vocab, *controls, RowIo{}, nullptr, 0, out, ld_out, (hipStream_t)stream);
+}
+
+extern "C" int axon_controls_apply_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab,
+                                       const axon_controls* controls, const void* g_out, int64_t ld_g, void* dlogits, int64_t ld_d,
+                                       void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK) rc = check_rows(g_out, dtype, ld_g, n, vocab);
+  if (rc == AXON_OK) rc = check_rows(dlogits, dtype, ld_d, n, vocab);
+  if (rc == AXON_OK) rc = check_controls(controls, n, vocab);
+  if (rc != AXON_OK || n == 0) return rc;
+  return launch<kApplyGrad>(logits, dtype, ld, n, vocab, *controls, RowIo{}, g_out, ld_g, dlogits, ld_d, (hipStream_t)stream);
+}
+
+extern "C" int64_t axon_controls_logprob_workspace_bytes(int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0 || vocab >= kOwn) return AXON_ERR_ARG;
+  return n * (chunks_of(vocab) * (int64_t)sizeof(float4) + (int64_t)sizeof(float));
+}
+
+extern "C" int axon_controls_logprob_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab,
+                                         const axon_controls* controls, const void* labels, int labels_i64, float* logprob,
+                                         float* entropy, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK) rc = check_controls(controls, n, vocab);
+  if (rc != AXON_OK || n == 0) return rc;
+  if (!labels || !logprob || !stats) return AXON_ERR_ARG;
+  if (!workspace || workspace_bytes < axon_controls_logprob_workspace_bytes(n, vocab) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return AXON_ERR_WORKSPACE;
+  const int chunks = chunks_of(vocab);
+  RowIo io{};
+  io.labels = labels;
+  io.labels_i64 = labels_i64;
+  io.parts = static_cast<float4*>(workspace);
+  io.label_y = reinterpret_cast<float*>(io.parts + n * chunks);
+  const hipStream_t st = (hipStream_t)stream;
+  rc = launch<kStats>(logits, dtype, ld, n, vocab, *controls, io, nullptr, 0, nullptr, 0, st);
+  if (rc != AXON_OK) return rc;
+  hipLaunchKernelGGL(controls_finish_kernel, dim3((unsigned)((n + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, (int)n, (int)vocab, chunks,
+                     *controls, io, logprob, entropy, stats);
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab,
+                                         const axon_controls* controls, const void* labels, int labels_i64, const float* stats,
+                                         const float* g_logprob, const float* g_entropy, void* dlogits, int64_t ld_d, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK) rc = check_rows(dlogits, dtype, ld_d, n, vocab);
+  if (rc == AXON_OK) rc = check_controls(controls, n, vocab);
+  if (rc != AXON_OK || n == 0) return rc;
+  if (!labels || !stats) return AXON_ERR_ARG;
+  RowIo io{};
+  io.labels = labels;
+  io.labels_i64 = labels_i64;
+  io.stats = stats;
+  io.g_logprob = g_logprob;
+  io.g_entropy = g_entropy;
+  return launch<kGrad>(logits, dtype, ld, n, vocab, *controls, io, nullptr, 0, dlogits, ld_d, (hipStream_t)stream);
+}

@@ -25,8 +25,10 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <mutex>
@@ -769,6 +771,323 @@ std::tuple<Tensor, Tensor> router_balance(const variable_list& logits, bool stac
   return {loss, counts};
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Controls of logits: what a sampler does to them before it draws.
+// ---------------------------------------------------------------------------------------------------------------------
+
+// The operands of axon_controls, checked and held.  Nothing is computed here: the tensors are read by every launch.
+class Controls {
+ public:
+  enum Which { kTokens, kOffsets, kOwnMask, kRepetition, kFrequency, kPresence, kTemperature, kBiasIds, kBias, kAllowed, kIndex, kCount };
+  typedef std::pair<double, OptTensor> Value;  // for all sequences, or one for each
+
+  Controls(const OptTensor& token_ids, const OptTensor& cu_seqlens, bool every_position, const OptTensor& own_mask, const Value& repetition,
+           const Value& frequency, const Value& presence, const OptTensor& bias_ids, const OptTensor& bias, const OptTensor& allowed,
+           const OptTensor& allowed_index, const Value& temperature) {
+    const at::NoGradGuard no_grad;
+    c_.every_position = every_position;
+    c_.n_seqs = -1;  // not known yet
+    if (cu_seqlens) {
+      if (cu_seqlens->dim() != 1 || cu_seqlens->numel() < 1) refuse(kWhat, "cu_seqlens must be [sequences + 1]");
+      hold(kOffsets, cu_seqlens->detach().to(at::kInt).contiguous());
+      c_.cu_seqlens = (const int32_t*)ptr(held_[kOffsets]);
+      c_.n_seqs = cu_seqlens->numel() - 1;
+    }
+    if (token_ids) {
+      if (!is_index(*token_ids)) refuse(kWhat, std::string("token_ids must be int32 or int64, got ") + c10::toString(token_ids->scalar_type()));
+      if (!cu_seqlens) {
+        if (token_ids->dim() != 1 && token_ids->dim() != 2) refuse(kWhat, "token_ids must be [sequences, length], or packed with cu_seqlens");
+        c_.uniform_len = token_ids->size(-1);
+        c_.n_seqs = token_ids->dim() == 2 ? token_ids->size(0) : 1;
+      }
+      if (token_ids->numel() >= INT32_MAX) refuse(kWhat, "more tokens than 32 bits count");
+      c_.n_tokens = token_ids->numel();
+      hold(kTokens, token_ids->detach().contiguous());
+      c_.token_ids = held_[kTokens].data_ptr();
+      c_.token_ids_i64 = is_i64(*token_ids);
+    }
+    if (own_mask) {
+      if (!token_ids || own_mask->numel() != token_ids->numel()) refuse(kWhat, "response_mask does not lie beside token_ids");
+      auto m = mask_arg(*own_mask);
+      c_.mask_kind = m.second;
+      hold(kOwnMask, std::move(m.first));
+      c_.own_mask = ptr(held_[kOwnMask]);
+    }
+    c_.repetition_all = (float)repetition.first;
+    c_.frequency_all = (float)frequency.first;
+    c_.presence_all = (float)presence.first;
+    c_.temperature_all = (float)temperature.first;
+    c_.repetition = value(kRepetition, repetition, "repetition_penalty");
+    c_.frequency = value(kFrequency, frequency, "frequency_penalty");
+    c_.presence = value(kPresence, presence, "presence_penalty");
+    c_.temperature = value(kTemperature, temperature, "temperature");
+    const auto usable = [](float x, bool positive) { return std::isfinite(x) && (!positive || x > 0.f); };
+    if (!usable(c_.repetition_all, true)) refuse(kWhat, "repetition_penalty must be positive");
+    if (!usable(c_.temperature_all, true)) refuse(kWhat, "temperature must be positive");
+    if (!usable(c_.frequency_all, false) || !usable(c_.presence_all, false)) refuse(kWhat, "frequency_penalty and presence_penalty must be finite");
+    if (!token_ids && (c_.repetition || c_.frequency || c_.presence || c_.repetition_all != 1.f || c_.frequency_all != 0.f || c_.presence_all != 0.f))
+      refuse(kWhat, "penalties need token_ids");
+    if (bias_ids.has_value() != bias.has_value()) refuse(kWhat, "bias_ids and bias come together");
+    if (bias) {
+      if (!is_index(*bias_ids)) refuse(kWhat, "bias_ids must be int32 or int64");
+      if (bias_ids->sizes() != bias->sizes() || bias->dim() < 1 || bias->dim() > 2)
+        refuse(kWhat, "bias_ids " + shape_text(*bias_ids) + " and bias " + shape_text(*bias) + " must both be [k] or [sequences, k]");
+      constant(*bias, "bias");
+      if (bias->dim() == 2) sequences(bias->size(0), "bias");
+      c_.bias_per_seq = bias->dim() == 2;
+      c_.n_bias = bias->size(-1);
+      c_.bias_ids_i64 = is_i64(*bias_ids);
+      hold(kBiasIds, bias_ids->detach().contiguous());
+      hold(kBias, f32(*bias));
+      c_.bias_ids = held_[kBiasIds].data_ptr();
+      c_.bias = (const float*)held_[kBias].data_ptr();
+    }
+    if (allowed_index && !allowed) refuse(kWhat, "allowed_index without allowed");
+    if (allowed) {
+      if (allowed->scalar_type() != at::kInt || allowed->dim() < 1 || allowed->dim() > 2 || allowed->size(-1) < 1 || allowed->size(0) < 1)
+        refuse(kWhat, "allowed must be int32 [words] or [masks, words], 32 tokens a word");
+      Tensor a = allowed->dim() == 1 ? allowed->detach().unsqueeze(0) : allowed->detach();
+      if (a.stride(1) != 1 || (a.size(0) > 1 && a.stride(0) < a.size(1))) a = a.contiguous();
+      c_.allowed = (const int32_t*)a.data_ptr();
+      c_.allowed_rows = a.size(0);
+      c_.allowed_stride = a.size(0) > 1 ? a.stride(0) : a.size(1);
+      words_ = a.size(1);
+      hold(kAllowed, std::move(a));
+      if (allowed_index) {
+        if (!is_index(*allowed_index)) refuse(kWhat, "allowed_index must be int32 or int64");
+        hold(kIndex, allowed_index->detach().contiguous());
+        c_.allowed_index = held_[kIndex].data_ptr();
+        c_.allowed_index_i64 = is_i64(*allowed_index);
+      }
+    }
+  }
+
+  // For n rows of v logits that lie where `like` does.
+  axon_controls of(const char* what, const Tensor& like, int64_t n, int64_t v) const {
+    axon_controls c = c_;
+    for (const Tensor& t : held_)
+      if (t.defined() && t.device() != like.device()) refuse(what, "logits and controls live on different devices");
+    if (c.every_position ? (c.token_ids && n != c.n_tokens) : (c.n_seqs >= 0 && n != c.n_seqs))
+      refuse(what, std::to_string(n) + " rows of logits for controls of " +
+                       (c.every_position ? std::to_string(c.n_tokens) + " positions" : std::to_string(c.n_seqs) + " sequences"));
+    if (c.every_position && !c.cu_seqlens && c.uniform_len == 0 && c.n_seqs >= 0)
+      refuse(what, "values for each sequence need token_ids or cu_seqlens");
+    if (c.n_seqs < 0) c.n_seqs = 0;
+    if (c.allowed) {
+      if (words_ < (v + 31) / 32) refuse(what, "allowed has " + std::to_string(words_) + " words for a vocabulary of " + std::to_string(v));
+      const Tensor& index = held_[kIndex];
+      if (index.defined() ? index.numel() != n : (c.allowed_rows != 1 && c.allowed_rows != n))
+        refuse(what, "allowed needs one mask, one for each of the " + std::to_string(n) + " rows, or an allowed_index of as many entries");
+    }
+    return c;
+  }
+  const Tensor& held(int i) const { return held_[i]; }
+
+ private:
+  static constexpr const char* kWhat = "LogitControls";
+  void hold(Which i, Tensor t) { held_[i] = std::move(t); }
+  void constant(const Tensor& t, const char* name) {
+    if (t.requires_grad()) refuse(kWhat, std::string(name) + " has no gradient: pass it detached");
+  }
+  void sequences(int64_t n, const char* name) {
+    if (c_.n_seqs >= 0 && n != c_.n_seqs)
+      refuse(kWhat, std::string(name) + " for " + std::to_string(n) + " sequences of " + std::to_string(c_.n_seqs));
+    c_.n_seqs = n;
+  }
+  const float* value(Which i, const Value& v, const char* name) {
+    if (!v.second) return nullptr;
+    if (v.second->dim() != 1 || !v.second->is_floating_point()) refuse(kWhat, std::string(name) + " must be a number or a float tensor [sequences]");
+    constant(*v.second, name);
+    sequences(v.second->numel(), name);
+    hold(i, f32(*v.second));
+    return (const float*)ptr(held_[i]);
+  }
+
+  axon_controls c_{};
+  std::array<Tensor, kCount> held_;
+  int64_t words_ = 0;
+};
+
+// The controls' tensors as a node saves them: one that is written to before the backward is noticed.
+struct SavedControls {
+  std::shared_ptr<Controls> controls;
+  std::vector<SavedVariable> held;
+  void save(std::shared_ptr<Controls> c) {
+    for (int i = 0; i < Controls::kCount; ++i)
+      if (c->held(i).defined()) held.emplace_back(c->held(i), false);
+    controls = std::move(c);
+  }
+  void release() {
+    for (SavedVariable& s : held) s.reset_data();
+  }
+  const Controls& unpack() {
+    for (SavedVariable& s : held) (void)s.unpack();  // raises where one has changed
+    return *controls;
+  }
+};
+
+// The saved rows of logits, as a hook may have handed them back.
+void check_saved_rows(const char* what, const Tensor& x) {
+  require_device(x, what);
+  if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < x.size(1)))
+    refuse(what, "logits must be [tokens, vocab] with unit stride over the vocabulary");
+}
+
+struct ControlledLogitsNode : torch::autograd::Node {
+  SavedVariable rows;
+  SavedControls controls;
+  std::vector<int64_t> shape;
+  static constexpr const char* kWhat = "controlled_logits_backward";
+  std::string name() const override { return "ControlledLogitsBackward"; }
+  void release_variables() override {
+    rows.reset_data();
+    controls.release();
+  }
+  variable_list apply(variable_list&& g) override {
+    if (!g[0].defined()) return {Tensor()};
+    const Tensor x = rows.unpack();
+    const Controls& ctl = controls.unpack();
+    Tensor out;
+    {
+      const at::NoGradGuard no_grad;
+      check_saved_rows(kWhat, x);
+      const int64_t n = x.size(0), v = x.size(1);
+      const int dtype = logits_dtype(kWhat, x);
+      if (g[0].numel() != n * v || g[0].device() != x.device()) refuse(kWhat, "the gradient does not lie beside the logits");
+      const Tensor up = rows_of_logits(g[0].to(x.scalar_type()));
+      const axon_controls c = ctl.of(kWhat, x, n, v);
+      const c10::DeviceGuard device(x.device());
+      out = at::empty({n, v}, x.options());
+      check(axon_controls_apply_bwd(x.data_ptr(), dtype, row_stride(x), n, v, &c, up.data_ptr(), row_stride(up), out.data_ptr(), v,
+                                    ::stream()),
+            "axon_controls_apply_bwd");
+      out = out.view(shape);
+    }
+    return {once(std::move(out), kWhat)};
+  }
+};
+
+Tensor controlled_logits(const Tensor& logits, std::shared_ptr<Controls> controls, bool inplace) {
+  const char* const what = "controlled_logits";
+  const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
+  no_tangent(what, logits);
+  if (inplace && wants_grad) refuse(what, "logits that require a gradient cannot be written over");
+  Tensor rows, out;
+  {
+    const at::NoGradGuard no_grad;
+    rows = rows_of_logits(logits);
+    const int64_t n = rows.size(0), v = rows.size(1);
+    const int dtype = logits_dtype(what, rows);
+    if (inplace && rows.data_ptr() != logits.data_ptr()) refuse(what, "logits can be written over only where their rows lie as they are read");
+    const axon_controls c = controls->of(what, rows, n, v);
+    require_device(rows, what);
+    const c10::DeviceGuard device(rows.device());
+    out = inplace ? rows : at::empty({n, v}, rows.options());
+    check(axon_controls_apply(rows.data_ptr(), dtype, row_stride(rows), n, v, &c, out.data_ptr(), row_stride(out), stream()),
+          "axon_controls_apply");
+    if (inplace && !logits.is_inference()) logits.unsafeGetTensorImpl()->bump_version();
+    out = inplace ? logits : out.view(logits.sizes());
+  }
+  if (wants_grad) {
+    std::shared_ptr<ControlledLogitsNode> node(new ControlledLogitsNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->shape = logits.sizes().vec();
+    torch::autograd::set_history(out, node);
+    node->rows = SavedVariable(rows, false);
+    node->controls.save(std::move(controls));
+  }
+  return out;
+}
+
+struct ControlledLogprobsNode : torch::autograd::Node {
+  SavedVariable rows, labels, stats;
+  SavedControls controls;
+  std::vector<int64_t> shape;
+  bool inplace = false, spent = false;
+  static constexpr const char* kWhat = "controlled_logprobs_backward";
+  std::string name() const override { return "ControlledLogprobsBackward"; }
+  void release_variables() override {
+    for (SavedVariable* s : {&rows, &labels, &stats}) s->reset_data();
+    controls.release();
+  }
+  // gradients of the log-probability and the entropy
+  variable_list apply(variable_list&& g) override {
+    if (!g[0].defined() && !g[1].defined()) return {Tensor()};
+    if (spent) throw AxonError("the logits' storage holds the gradient of an earlier backward (inplace_backward)");
+    const Tensor x = rows.unpack(), lab = labels.unpack(), st = stats.unpack();
+    const Controls& ctl = controls.unpack();
+    Tensor out;
+    {
+      const at::NoGradGuard no_grad;
+      check_saved_rows(kWhat, x);
+      const int64_t n = x.size(0), v = x.size(1);
+      const Tensor g_lp = g[0].defined() ? f32(g[0]) : Tensor(), g_en = g[1].defined() ? f32(g[1]) : Tensor();
+      same_place(kWhat, x, {&lab, &st, &g_lp, &g_en});
+      const int dtype = logits_dtype(kWhat, x);
+      same_type(kWhat, at::kFloat, {&st});
+      if (!is_index(lab)) refuse(kWhat, "a saved tensor has come back in another type");
+      same_len(kWhat, "labels", n, lab);
+      same_len(kWhat, "statistics", 3 * n, st);
+      if (g_lp.defined()) same_len(kWhat, "g_logprobs", n, g_lp);
+      if (g_en.defined()) same_len(kWhat, "g_entropy", n, g_en);
+      const axon_controls c = ctl.of(kWhat, x, n, v);
+      const c10::DeviceGuard device(x.device());
+      out = inplace ? x : at::empty({n, v}, x.options());
+      check(axon_controls_logprob_bwd(x.data_ptr(), dtype, row_stride(x), n, v, &c, lab.data_ptr(), is_i64(lab), (const float*)st.data_ptr(),
+                                      (const float*)ptr(g_lp), (const float*)ptr(g_en), out.data_ptr(), row_stride(out), ::stream()),
+            "axon_controls_logprob_bwd");
+      spent = inplace;
+      if (inplace && !x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+      out = out.view(shape);
+    }
+    return {once(std::move(out), kWhat)};
+  }
+};
+
+// (log-probability of the label, entropy)
+std::tuple<Tensor, Tensor> controlled_logprobs(const Tensor& logits, const Tensor& labels, std::shared_ptr<Controls> controls, bool inplace) {
+  const char* const what = "controlled_logprobs_from_logits";
+  const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
+  no_tangent(what, logits);
+  Tensor rows, lab, lp, entropy, stats;
+  {
+    const at::NoGradGuard no_grad;
+    rows = rows_of_logits(logits);
+    const int64_t n = rows.size(0), v = rows.size(1);
+    const int dtype = logits_dtype(what, rows);
+    const std::vector<int64_t> batch(logits.sizes().begin(), logits.sizes().end() - 1);
+    if (!is_index(labels)) refuse(what, "labels must be int32 or int64");
+    if (labels.device() != logits.device()) refuse(what, "operands live on different devices");
+    if (labels.sizes() != at::IntArrayRef(batch))
+      refuse(what, "labels " + shape_text(labels) + " do not lie beside logits " + shape_text(logits));
+    lab = labels.detach().reshape({n}).contiguous();
+    const axon_controls c = controls->of(what, rows, n, v);
+    require_device(rows, what);
+    const c10::DeviceGuard device(rows.device());
+    lp = at::empty(batch, opts(rows));
+    entropy = at::empty(batch, opts(rows));
+    stats = at::empty({3, n}, opts(rows));
+    const int64_t need = axon_controls_logprob_workspace_bytes(n, v);
+    const Tensor ws = at::empty({std::max<int64_t>(need, 0)}, opts(rows, at::kByte));
+    check(axon_controls_logprob_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, &c, lab.data_ptr(), is_i64(lab), lp.data_ptr<float>(),
+                                    entropy.data_ptr<float>(), stats.data_ptr<float>(), ws.data_ptr(), need, stream()),
+          "axon_controls_logprob_fwd");
+  }
+  if (wants_grad) {
+    std::shared_ptr<ControlledLogprobsNode> node(new ControlledLogprobsNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->shape = logits.sizes().vec();
+    node->inplace = inplace && rows.data_ptr() == logits.data_ptr();
+    torch::autograd::set_history(lp, node);
+    torch::autograd::set_history(entropy, node);
+    node->rows = SavedVariable(rows, false);
+    node->labels = SavedVariable(lab, false);
+    node->stats = SavedVariable(stats, false);
+    node->controls.save(std::move(controls));
+  }
+  return {lp, entropy};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -804,4 +1123,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return alternatives("token_logprobs_from_logits", logits, 0, token_ids, OptTensor(), inplace);
   }, unlocked);
   m.def("router_balance", &router_balance, unlocked);
+  py::class_<Controls, std::shared_ptr<Controls>>(m, "Controls")
+      .def(py::init<const OptTensor&, const OptTensor&, bool, const OptTensor&, const Controls::Value&, const Controls::Value&,
+                    const Controls::Value&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Controls::Value&>(),
+           unlocked);
+  m.def("controlled_logits", &controlled_logits, unlocked);
+  m.def("controlled_logprobs", &controlled_logprobs, unlocked);
 }

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define AXON_AMD_ABI_VERSION 27
+#define AXON_AMD_ABI_VERSION 28
 
 enum {
   AXON_OK = 0,
@@ -734,6 +734,49 @@ int axon_router_balance_bwd(const void* const* logits, int dtype, int64_t ld, in
                             int64_t experts, const void* mask, int mask_kind, const int32_t* cu_seqlens, int64_t n_seqs,
                             int score, const float* coef, const float* scale, const float* g_loss, void* const* dlogits,
                             void* stream);
+
+/* What a sampler does to a position's logits before it draws, in this order (the reference has no such operator):
+ *   y = z > 0 ? z / rep : z * rep   for the ids of the row's history
+ *   y -= freq * count + pres        for the ids that occur count > 0 times among its own tokens
+ *   y += bias                       for the given ids (an id that comes twice: both)
+ *   y = -inf                        where the row's mask has a 0 bit, whatever the logit is
+ *   out = y / T
+ * Sequences are rows of tokens (cu_seqlens, or uniform_len > 0 and NULL).  every_position 1: row r of the logits is position
+ * r of the tokens and its history the tokens of its sequence up to and with r; 0: row r belongs to sequence r, whose tokens
+ * are all its history.  Own tokens: those with own_mask != 0 (NULL: all).  An id outside [0, vocab) counts for nothing.
+ * Passed by the host; its pointers are device memory. */
+typedef struct axon_controls {
+  const void* token_ids; /* [n_tokens] int32 or int64; NULL: no history */
+  int64_t n_tokens, n_seqs, uniform_len;
+  const int32_t* cu_seqlens; /* [n_seqs + 1], or NULL with uniform_len, or with every_position 0 and no token_ids */
+  const void* own_mask;      /* [n_tokens], NULL: all */
+  int token_ids_i64, mask_kind, every_position;
+  int bias_ids_i64, bias_per_seq, allowed_index_i64;
+  const float *repetition, *frequency, *presence, *temperature; /* [n_seqs], or NULL: the scalars */
+  float repetition_all, frequency_all, presence_all, temperature_all;
+  const void* bias_ids; /* [n_bias], or [n_seqs][n_bias] with bias_per_seq */
+  const float* bias;
+  int64_t n_bias;
+  const int32_t* allowed; /* [allowed_rows][allowed_stride]: bit i of word w for id 32 w + i; NULL: no mask */
+  int64_t allowed_rows, allowed_stride;
+  const void* allowed_index; /* [rows]: the mask of a row, none where outside [0, allowed_rows); NULL: row r, or the only one */
+} axon_controls;
+/* out [n][vocab] (row stride ld_out) in the logits' type (AXON_LOGITS_*); out may be the logits' own storage. */
+int axon_controls_apply(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
+                        void* out, int64_t ld_out, void* stream);
+/* dlogits = g_out * d out / d logits, 0 where out is -inf. */
+int axon_controls_apply_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
+                            const void* g_out, int64_t ld_g, void* dlogits, int64_t ld_d, void* stream);
+/* log softmax(out)[label] (0 for a label outside the vocabulary) and the entropy (may be NULL) of softmax(out), fp32; a row
+ * that nothing is left of: -inf, 0 and no gradient.  stats [3][n]: what the backward reads.  Workspace 16-byte aligned.
+ * dlogits may be the logits' own storage; g_logprob, g_entropy may be NULL. */
+int64_t axon_controls_logprob_workspace_bytes(int64_t n, int64_t vocab);
+int axon_controls_logprob_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
+                              const void* labels, int labels_are_i64, float* logprob, float* entropy, float* stats, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
+                              const void* labels, int labels_are_i64, const float* stats, const float* g_logprob,
+                              const float* g_entropy, void* dlogits, int64_t ld_d, void* stream);
 
 /* KL penalty inside the reward, the tensor part of apply_kl_penalty (axon/utils/rl/kl.py:276-322):
  *   kld = kl_penalty(old_logp, ref_logp, kl_type) * mask      (types as in axon_kl_penalty)

@@ -1,0 +1,400 @@
+"""Controls of logits (penalties, biases, masks, temperature) against their definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from axon_amd.utils.torch.controls import LogitControls, controlled_logits, controlled_logprobs_from_logits
+from axon_amd.utils.torch.ops import (logprobs_and_entropy_from_logits, token_logprobs_from_logits, top_logprobs_from_logits)
+
+import controls_reference as R
+
+pytestmark = pytest.mark.gpu
+
+# A controlled logit in fp32: the factor 1 / r is rounded, the product with it, the penalty, the two additions, the factor 1 / T
+# and the product with it: seven roundings of 2^-24 of no more than what is added up.
+Y_ROUNDINGS = 7 * 2.0 ** -24
+# A log-probability of logits of at most 80: a logit is off by Y_ROUNDINGS (3.4e-5), and so may all the others be to the other
+# side; exponentials and their sums by 2e-5 (chains of 8 and of 6 roundings, an argument of up to 150 in 2^-24 weighted by its
+# probability); the last additions by two roundings of 80.
+LP_TOL = 1.1e-4
+# The entropy is made of the same terms, weighted by up to |log p|, of which 12 is the average at most.
+ENT_TOL = 12 * LP_TOL
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def case(seed, lens, v, positions, dtype, *, per_seq=False, bias=0, masks="none", ids=torch.int64, own=True, scale=4.0,
+         penalties=True, temperature=0.8):
+    """Logits, LogitControls' arguments and the reference's."""
+    g, n_seqs, total = gen(seed), len(lens), sum(lens)
+    rows = n_seqs if positions == "last" else total
+    rand = lambda *s: torch.rand(*s, generator=g, device="cuda")
+    z = (torch.randn(rows, v, generator=g, device="cuda") * scale).to(dtype)
+    tokens = (rand(total) ** 3 * v).long().clamp(max=v - 1)
+    tokens[rand(total) < 0.05] = -1
+    tokens[rand(total) < 0.05] = v + 3
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    response = (rand(total) < 0.6).float() if own else None
+    mk = lambda lo, hi: lo + (hi - lo) * rand(n_seqs) if per_seq else lo + 0.6 * (hi - lo)
+    how = dict(repetition=mk(0.8, 1.5), frequency=mk(-0.2, 0.5), presence=mk(-0.2, 0.6)) if penalties else {}
+    if per_seq or temperature != 1.0:
+        how["temperature"] = mk(0.7, 1.5) if per_seq else temperature
+    kw = {f"{k}_penalty" if k != "temperature" else k: x for k, x in how.items()}
+    if bias:
+        shape = (n_seqs, bias) if per_seq else (bias,)
+        b_ids = torch.randint(-1, v + 2, shape, generator=g, device="cuda")
+        b = torch.randn(shape, generator=g, device="cuda")
+        if bias > 2:
+            b_ids[..., 1] = b_ids[..., 0]  # twice
+            b[..., 2] = -math.inf
+        kw.update(bias_ids=b_ids.to(ids), bias=b)
+        how.update(bias_ids=b_ids.cpu(), bias=b.cpu())
+    if masks != "none":
+        count = {"shared": 1, "rows": rows, "states": 7}[masks]
+        keep = rand(count, v) < 0.7
+        keep[::2] = rand(len(keep[::2]), v) < 3.0 / v  # few tokens, or none
+        if count > 3:
+            keep[3] = False
+        kw["allowed"] = R.pack(keep)
+        if masks == "states":
+            index = torch.randint(-2, count + 2, (rows,), generator=g, device="cuda")
+            kw["allowed_index"] = index.to(ids)
+            how["keep"] = [keep[i] if 0 <= i < count else None for i in index.tolist()]
+        else:
+            how["keep"] = [keep[0 if count == 1 else i] for i in range(rows)]
+    args = dict(kw, positions=positions)
+    if penalties or per_seq:
+        args.update(cu_seqlens=cu)
+    if penalties:
+        args.update(token_ids=tokens.to(ids), response_mask=response)
+    ref = dict(how, own=response if penalties else None)
+    return z, args, (R.spans_of(lens, positions), tokens if penalties else None, ref)
+
+
+def reference(z, ref):
+    spans, tokens, how = ref
+    return R.controlled(z, spans, tokens, **how)
+
+
+CASES = [
+    # seed, lens, vocab, positions, dtype, options
+    (1, [1], 1, "last", torch.float32, dict()),
+    (2, [1, 3], 5, "all", torch.bfloat16, dict(masks="rows")),
+    (3, [5, 1, 9], 31, "last", torch.bfloat16, dict(per_seq=True, bias=3)),
+    (4, [7, 4], 33, "all", torch.float32, dict(per_seq=True, bias=4, masks="states", ids=torch.int32)),
+    (5, [40, 1, 1, 30], 2047, "all", torch.bfloat16, dict(masks="shared")),
+    (6, [130], 2048, "all", torch.float32, dict(bias=5)),
+    (7, [0, 12, 0, 0, 7, 0], 2049, "all", torch.bfloat16, dict(per_seq=True, bias=70)),
+    (8, [0, 12, 400], 2049, "last", torch.float32, dict(per_seq=True, masks="rows")),
+    (9, [300, 2, 90], 5003, "all", torch.bfloat16, dict(per_seq=True, masks="states", bias=9)),
+    (10, [3, 4], 16391, "all", torch.bfloat16, dict(penalties=False, masks="rows", temperature=1.0)),
+    (11, [3, 4], 16391, "last", torch.float32, dict(penalties=False, bias=40)),
+    (12, [9, 8], 8200, "all", torch.bfloat16, dict(penalties=False, per_seq=True, bias=40, own=False)),
+    (13, [11, 70], 50257, "last", torch.bfloat16, dict(own=False, masks="shared", bias=300)),
+    (14, [20, 30], 50257, "all", torch.bfloat16, dict(masks="states")),
+    (15, [6], 151936, "all", torch.float32, dict(masks="rows", bias=20)),
+    (16, [2500, 3], 700, "last", torch.bfloat16, dict()),
+    (17, [5, 6], 3001, "all", torch.float32, dict(penalties=False, temperature=1.0)),
+]
+
+
+@pytest.mark.parametrize("seed,lens,v,positions,dtype,options", CASES)
+def test_logits_written_out(seed, lens, v, positions, dtype, options):
+    z, args, ref = case(seed, lens, v, positions, dtype, **options)
+    want, slope, size = reference(z, ref)
+    z.requires_grad_(True)
+    out = controlled_logits(z, LogitControls(**args))
+    assert out.dtype == dtype and out.shape == z.shape
+    got = out.detach().double().cpu()
+    banned = want == -math.inf
+    assert torch.equal(got == -math.inf, banned)
+    bound = Y_ROUNDINGS * size + (2.0 ** -8 * want.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30
+    assert ((got - want).abs()[~banned] <= bound[~banned]).all()
+    up = torch.randn(z.shape, generator=gen(seed + 100), device="cuda").to(dtype)
+    grad, = torch.autograd.grad(out, z, up)
+    ref_grad = up.double().cpu() * slope
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    assert grad.dtype == dtype and ((grad.double().cpu() - ref_grad).abs() <= (4 * 2.0 ** -24 + half) * ref_grad.abs()).all()
+    with torch.no_grad():  # over the logits themselves: the same
+        same = z.detach().clone()
+        assert controlled_logits(same, LogitControls(**args), inplace=True).data_ptr() == same.data_ptr()
+        assert torch.equal(same, out.detach())
+
+
+@pytest.mark.parametrize("seed,lens,v,positions,dtype,options", CASES)
+def test_scored(seed, lens, v, positions, dtype, options):
+    z, args, ref = case(seed, lens, v, positions, dtype, **options)
+    out, slope, _ = reference(z, ref)
+    n, g = z.shape[0], gen(seed + 200)
+    labels = torch.randint(0, v, (n,), generator=g, device="cuda")
+    labels[-1] = v if n > 1 else 0
+    g_lp, g_ent = torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    lp, ent, grad, size = R.scored(out, slope, labels, g_lp, g_ent)
+    z.requires_grad_(True)
+    got_lp, got_ent = controlled_logprobs_from_logits(z, labels, LogitControls(**args))
+    finite = torch.isfinite(lp)
+    assert torch.equal(torch.isfinite(got_lp.cpu()), finite) and (got_lp.cpu()[~finite] == -math.inf).all()
+    assert ((got_lp.detach().double().cpu() - lp).abs()[finite] <= LP_TOL).all()
+    assert ((got_ent.detach().double().cpu() - ent).abs() <= ENT_TOL).all()
+    got, = torch.autograd.grad([got_lp, got_ent], z, [g_lp, g_ent])
+    bound = 2 * ENT_TOL * size + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30
+    assert got.dtype == dtype and ((got.double().cpu() - grad).abs() <= bound).all()
+    twin = z.detach().clone().requires_grad_(True)
+    again = controlled_logprobs_from_logits(twin * 1.0, labels.to(torch.int32), LogitControls(**args), inplace_backward=True)
+    over, = torch.autograd.grad(again, twin, [g_lp, g_ent])
+    assert torch.equal(over, got) and torch.equal(again[0], got_lp)
+    for i, g_only in ((0, g_lp), (1, g_ent)):  # one upstream gradient alone
+        zero = torch.zeros_like(g_only)
+        o = controlled_logprobs_from_logits(z, labels, LogitControls(**args))
+        one, = torch.autograd.grad(o[i], z, g_only, retain_graph=True)
+        both, = torch.autograd.grad(o, z, [g_only, zero] if i == 0 else [zero, g_only])
+        assert torch.equal(one, both)
+
+
+def test_without_controls_it_is_the_plain_log_probability():
+    z = torch.randn(70, 9000, generator=gen(1), device="cuda")
+    labels = torch.randint(0, 9000, (70,), generator=gen(2), device="cuda")
+    lp, ent = controlled_logprobs_from_logits(z, labels, LogitControls())
+    lp0, ent0 = logprobs_and_entropy_from_logits(z, labels)
+    assert (lp - lp0).abs().max() <= LP_TOL and (ent - ent0).abs().max() <= ENT_TOL
+    assert torch.equal(controlled_logits(z, LogitControls()), z)
+
+
+@pytest.mark.parametrize("positions", ["all", "last"])
+def test_padded_batches_are_packed_ones(positions):
+    """[sequences, length] with an attention mask on either side, against the sequences packed."""
+    lens, v, b, t = [5, 9, 1, 7], 4100, 4, 9
+    z, args, _ = case(31, lens, v, positions, torch.bfloat16, bias=3)
+    tokens, cu, resp = args["token_ids"], args["cu_seqlens"].tolist(), args["response_mask"]
+    attention = torch.zeros(b, t, dtype=torch.int64, device="cuda")
+    ids = torch.full((b, t), 17, device="cuda")  # what padding holds does not matter
+    response = torch.ones(b, t, device="cuda")
+    where = []
+    for i, (a, e) in enumerate(zip(cu[:-1], cu[1:])):
+        at = slice(t - (e - a), t) if i % 2 else slice(0, e - a)
+        attention[i, at], ids[i, at], response[i, at] = 1, tokens[a:e], resp[a:e]
+        where.append(torch.arange(t, device="cuda")[at] + i * t)
+    packed = controlled_logits(z, LogitControls(**args))
+    padded_args = {k: x for k, x in args.items() if k != "cu_seqlens"}
+    padded_args.update(token_ids=ids, response_mask=response, attention_mask=attention)
+    if positions == "last":
+        out = controlled_logits(z, LogitControls(**padded_args))
+    else:
+        full = torch.zeros(b * t, v, dtype=z.dtype, device="cuda")
+        full[torch.cat(where)] = z
+        out = controlled_logits(full.view(b, t, v), LogitControls(**padded_args)).view(b * t, v)[torch.cat(where)]
+    assert torch.equal(out, packed)
+
+
+def test_what_is_masked_does_not_matter():
+    """NaN, infinities and the type's lowest where the mask forbids; a mask that leaves one token, and none."""
+    v = 6000
+    for dtype in (torch.float32, torch.bfloat16):
+        z = torch.randn(6, v, generator=gen(4), device="cuda").to(dtype)
+        keep = torch.rand(6, v, generator=gen(5), device="cuda") < 0.5
+        keep[3], keep[4] = False, False
+        keep[3, 4000] = True
+        labels = keep.float().argmax(1)
+        dirty = z.clone()
+        for row, x in enumerate((math.nan, math.inf, -math.inf, torch.finfo(dtype).min, math.nan)):
+            dirty[row][~keep[row]] = x
+        dirty[5][keep[5]] = torch.finfo(dtype).min  # everything that is left is the type's lowest: they are equal
+        z[5][keep[5]] = 0.0
+        a, b = dirty.requires_grad_(True), z.clone().requires_grad_(True)
+        ctl = LogitControls(allowed=R.pack(keep))
+        ra, rb = (controlled_logprobs_from_logits(x, labels, ctl) for x in (a, b))
+        assert torch.equal(ra[0][:5], rb[0][:5]) and torch.equal(ra[1][:5], rb[1][:5])
+        left = keep[5].sum().item()
+        for r in (ra, rb):
+            assert abs(r[0][5].item() + math.log(left)) <= LP_TOL and abs(r[1][5].item() - math.log(left)) <= ENT_TOL
+            assert r[0][3] == 0 and r[1][3] == 0 and r[0][4] == -math.inf and r[1][4] == 0
+        ones = [torch.ones(6, device="cuda")] * 2
+        ga, gb = (torch.autograd.grad(r, x, ones)[0] for r, x in ((ra, a), (rb, b)))
+        assert torch.equal(ga[:5], gb[:5]) and (ga[4] == 0).all() and (ga[~keep] == 0).all()
+        assert torch.equal(controlled_logits(a.detach(), ctl)[~keep], torch.full_like(a[~keep], -math.inf).detach())
+    # without a mask in the way they show
+    bad = torch.zeros(3, v, device="cuda")
+    bad[0, 5], bad[1, 5] = math.nan, math.inf
+    lp, ent = controlled_logprobs_from_logits(bad, torch.zeros(3, dtype=torch.int64, device="cuda"), LogitControls())
+    assert torch.isnan(lp[:2]).all() and torch.isnan(ent[:2]).all() and abs(lp[2].item() + math.log(v)) <= LP_TOL
+
+
+def test_rows_that_lie_elsewhere():
+    """Rows further apart, off every boundary, transposed, a view with more dimensions."""
+    lens, v = [9, 6], 5001
+    z, args, _ = case(41, lens, v, "all", torch.bfloat16, masks="states", bias=5)
+    labels = torch.randint(0, v, (15,), generator=gen(1), device="cuda")
+    ctl = LogitControls(**args)
+    want, want_lp = controlled_logits(z, ctl), controlled_logprobs_from_logits(z, labels, ctl)[0]
+    for off in (1, 3, 8):
+        buf = torch.full((15 * (v + 7) + off,), 99.0, device="cuda", dtype=z.dtype)
+        view = buf[off:].view(15, v + 7)[:, :v]
+        view.copy_(z)
+        assert torch.equal(controlled_logits(view, ctl), want)
+        assert torch.equal(controlled_logprobs_from_logits(view, labels, ctl)[0], want_lp)
+        controlled_logits(view, ctl, inplace=True)
+        assert torch.equal(view, want)
+        rest = buf[off:].view(15, v + 7)[:, v:]
+        assert (rest == 99.0).all() and (buf[:off] == 99.0).all()  # rows' neighbours are left as they were
+    across = z.t().contiguous().t()
+    assert torch.equal(controlled_logits(across, ctl), want)
+    with pytest.raises(ValueError, match="written over"):
+        controlled_logits(across, ctl, inplace=True)
+    assert torch.equal(controlled_logits(z.view(3, 5, v), ctl), want.view(3, 5, v))
+    wide = R.pack(torch.rand(4, v + 500, generator=gen(3), device="cuda") < 0.5)[:, : (v + 31) // 32]  # masks with a stride
+    assert torch.equal(controlled_logits(z[:4], LogitControls(allowed=wide)),
+                       controlled_logits(z[:4], LogitControls(allowed=wide.contiguous())))
+
+
+def test_gradients_against_differences():
+    """Central differences in the direction of the gradient, fp32, of a smooth function of both outputs."""
+    z, args, _ = case(51, [6, 9], 700, "all", torch.float32, masks="states", bias=4, scale=1.5)
+    labels = torch.randint(0, 700, (15,), generator=gen(1), device="cuda")
+    ctl = LogitControls(**args)
+    weight = torch.randn(15, generator=gen(2), device="cuda")
+
+    def f(x):
+        lp, ent = controlled_logprobs_from_logits(x, labels, ctl)
+        return (weight * torch.where(torch.isfinite(lp), lp, torch.zeros_like(lp))).double().sum() + 0.3 * ent.double().sum()
+
+    x = z.clone().requires_grad_(True)
+    f(x).backward()
+    x.grad[(z.abs() < 0.1)] = 0.0  # a logit that changes its sign changes its slope
+    step = 0.02 / x.grad.norm()
+    numeric = (f(z + step * x.grad) - f(z - step * x.grad)).item() / (2 * step.item())
+    # the third derivative's share is step^2 |g|^2 / 6 of at most 10; the values are off by 30 LP_TOL at most
+    exact = x.grad.double().square().sum().item()
+    assert abs(numeric - exact) <= 0.01 * exact + 30 * LP_TOL / step.item()
+
+
+def test_long_histories_and_many_rows():
+    """A history of many tokens of few kinds, counted exactly, over runs that begin inside a sequence."""
+    v, n = 3000, 5000
+    tokens = torch.randint(0, 7, (n,), generator=gen(1), device="cuda") * 401
+    z = torch.zeros(n, v, device="cuda")
+    out = controlled_logits(z, LogitControls(tokens[None], frequency_penalty=0.125, presence_penalty=0.5))
+    count = torch.nn.functional.one_hot(tokens, v).cumsum(0)
+    assert torch.equal(out, -(0.125 * count + 0.5 * (count > 0)).float())  # numbers of few bits: nothing is rounded
+    last = controlled_logits(z[:1], LogitControls(tokens[None], positions="last", frequency_penalty=0.125))
+    assert torch.equal(last[0], -0.125 * count[-1].float())
+
+
+def test_offsets_beyond_32_bits():
+    """Logits of more than 2^32 bytes: the last rows are those of a short batch."""
+    v, n = 151936, 15000  # 4.5 GB of bf16
+    z = torch.zeros(n, v, device="cuda", dtype=torch.bfloat16)
+    z[-4:] = torch.randn(4, v, generator=gen(1), device="cuda").bfloat16()
+    tokens = torch.randint(0, v, (n,), generator=gen(2), device="cuda")
+    cu = torch.tensor([0, n - 4, n], dtype=torch.int32, device="cuda")
+    labels = torch.randint(0, v, (n,), generator=gen(3), device="cuda")
+    kw = dict(repetition_penalty=1.3, presence_penalty=0.5)
+    lp, ent = controlled_logprobs_from_logits(z, labels, LogitControls(tokens, cu, **kw))
+    few = LogitControls(tokens[-4:].contiguous(), torch.tensor([0, 4], dtype=torch.int32, device="cuda"), **kw)
+    lp4, ent4 = controlled_logprobs_from_logits(z[-4:], labels[-4:], few)
+    assert torch.equal(lp[-4:], lp4) and torch.equal(ent[-4:], ent4)
+    out = controlled_logits(z, LogitControls(tokens, cu, **kw))
+    assert torch.equal(out[-4:], controlled_logits(z[-4:], few))
+
+
+def test_results_repeat_bit_for_bit():
+    z, args, _ = case(61, [200, 90, 3], 20000, "all", torch.bfloat16, bias=30, masks="states")
+    labels = torch.randint(0, 20000, (293,), generator=gen(1), device="cuda")
+    x = z.requires_grad_(True)
+    runs = []
+    for _ in range(3):
+        r = controlled_logprobs_from_logits(x, labels, LogitControls(**args))
+        runs.append([*r, *torch.autograd.grad([t.sum() for t in r], x)])
+    assert all(torch.equal(a, b) for other in runs[1:] for a, b in zip(runs[0], other))
+
+
+def test_another_stream_and_a_captured_graph():
+    lens, v = [30, 12], 7001
+    z, args, _ = case(71, lens, v, "all", torch.bfloat16, masks="states", bias=5)
+    labels = torch.randint(0, v, (42,), generator=gen(1), device="cuda")
+    want = controlled_logprobs_from_logits(z, labels, LogitControls(**args))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = controlled_logprobs_from_logits(z, labels, LogitControls(**args))
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+    x = z.clone().requires_grad_(True)
+    g = torch.randn(42, generator=gen(2), device="cuda")
+
+    def step():
+        lp, ent = controlled_logprobs_from_logits(x, labels, LogitControls(**args))
+        grad, = torch.autograd.grad([lp, ent], x, [g, -g])
+        return lp.detach(), ent.detach(), grad, controlled_logits(x.detach(), LogitControls(**args))
+
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(42, v, generator=gen(80 + seed), device="cuda"))
+            args["token_ids"].copy_(torch.randint(0, v, (42,), generator=gen(90 + seed), device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in outs]
+        assert all(torch.equal(a, b) for a, b in zip(replayed, step()))
+        torch.cuda.synchronize()
+
+
+def test_with_the_operators_beside_it():
+    """A constrained decoder's report, and a student's log-probabilities of a teacher's tokens under the same grammar."""
+    lens, v = [9, 4], 3000
+    z, args, ref = case(81, lens, v, "all", torch.float32, masks="states", bias=5)
+    out, slope, _ = reference(z, ref)
+    labels = torch.randint(0, v, (13,), generator=gen(1), device="cuda")
+    x = z.requires_grad_(True)
+    y = controlled_logits(x, LogitControls(**args))
+    top = top_logprobs_from_logits(y, 3, labels)
+    lp, ent = controlled_logprobs_from_logits(x, labels, LogitControls(**args))
+    alive = torch.isfinite(top.entropy)
+    assert torch.equal(alive.cpu(), (out > -math.inf).any(1))
+    a, b = top.logprobs[alive], lp[alive]
+    both = torch.isfinite(a)
+    assert torch.equal(both, torch.isfinite(b)) and ((a - b).abs()[both] <= 2 * LP_TOL).all()
+    assert ((top.entropy - ent).abs()[alive] <= 2 * ENT_TOL).all()
+    tokens = top.top_ids[alive]
+    s, _ = token_logprobs_from_logits(y[alive], tokens)
+    g = torch.randn(s.shape, generator=gen(3), device="cuda")
+    open_ = torch.isfinite(s)
+    grad, = torch.autograd.grad((torch.where(open_, s, torch.zeros_like(s)) * g).sum(), x)
+    z64 = z.detach().double().cpu().requires_grad_(True)
+    # the same chain by hand: d/dy of the log-probabilities, times dy/dz
+    p = torch.softmax(out[alive.cpu()], 1)
+    up = torch.where(open_.cpu(), g.double().cpu(), torch.zeros(s.shape, dtype=torch.float64))
+    dy = torch.zeros_like(p).scatter_add_(1, tokens.cpu(), up) - p * up.sum(1, keepdim=True)
+    want = torch.zeros_like(z64)
+    want[alive.cpu()] = dy
+    assert ((grad.double().cpu() - want * slope).abs() <= 2 * ENT_TOL * slope * up.abs().sum(1).max()).all()
+
+
+def test_tensors_changed_before_the_backward_are_noticed():
+    z, args, _ = case(91, [9, 4], 900, "all", torch.float32, masks="states")
+    labels = torch.zeros(13, dtype=torch.int64, device="cuda")
+    for name in ("token_ids", "allowed", "allowed_index"):
+        x = z.clone().requires_grad_(True)
+        lp, _ = controlled_logprobs_from_logits(x, labels, LogitControls(**args))
+        args[name].add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            lp.sum().backward()
+    x = (z * 1.0).requires_grad_(True)
+    y = x * 1.0
+    lp, _ = controlled_logprobs_from_logits(y, labels, LogitControls(**args))
+    out = controlled_logits(y, LogitControls(**args))
+    with torch.no_grad():
+        controlled_logits(y.detach(), LogitControls(**args), inplace=True)
+    for t in (lp, out):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            t.sum().backward(retain_graph=True)
