@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libaxon_amd.so")
 EXT_PATH = os.path.join(_HERE, "_torch_ext.so")
-SOURCES = ("capi.hip", "rows.hip", "loss.hip", "owned.hip", "diag.hip", "returns.hip", "cov.hip", "logits.hip", "alternatives.hip", "controls.hip", "balance.hip", "step.hip", "lmhead.hip")
+SOURCES = ("capi.hip", "rows.hip", "loss.hip", "owned.hip", "diag.hip", "returns.hip", "cov.hip", "logits.hip", "alternatives.hip", "controls.hip", "distill.hip", "balance.hip", "step.hip", "lmhead.hip")
 
 HIPCC_FLAGS = (
     "--offload-arch=gfx950",

@@ -1,0 +1,531 @@
+// Distillation from a teacher's top logits: per position, a divergence between the teacher's probabilities q of k given tokens
+// and the student's p of the same tokens under the softmax over the whole vocabulary, optionally with what is left of both as
+// one more outcome, and its gradient with respect to the student's logits.
+//
+// Every divergence is a function of the outcomes' log-probabilities lp, with G_o = dL / dlp_o:
+//   forward  sum q (lq - lp)                                  G = -q
+//   reverse  sum p (lp - lq)                                  G = p (lp - lq + 1)
+//   jsd      m = b q + (1 - b) p:  sum b q (lq - lm) + (1 - b) p (lp - lm)   G = (1 - b) p (lp - lm)
+//   dz_j = (sum_{o: id_o = j} G_o - p_j sum_o G_o + [j is not given] G_rest p_j / p_rest) / T
+// so that a row is its softmax statistics, k gathered logits, and one multiple of p_j for all tokens that are not given.  What
+// the student has left over is summed over these tokens themselves: 1 minus the rest has no digits where it matters.
+#include "logits_rows.h"
+
+namespace axon {
+
+constexpr int kMaxParts = 64;
+constexpr int kMaxIds = AXON_MAX_TOKEN_IDS;
+constexpr int kMaxShare = 49152;  // vectors of a workgroup's share: a byte each in LDS says which of its elements are given
+
+struct Teacher {
+  const void* ids;        // [n][k]
+  const float* logprobs;  // [n][k]
+  const float* weights;   // [n], null: all rows count
+  int ids_i64, k, divergence, tail;
+  float beta, inv_t;
+};
+__device__ __forceinline__ int teacher_id(const Teacher& t, int64_t at, int vocab) {
+  const int64_t id = t.ids_i64 ? static_cast<const int64_t*>(t.ids)[at] : (int64_t) static_cast<const int32_t*>(t.ids)[at];
+  return id >= 0 && id < vocab ? (int)id : -1;
+}
+
+// What a row leaves for its backward: the student's log-sum-exp (of z, before the temperature) in two parts, the multiple of
+// p_j for tokens that are not given, and that for those that are.
+enum Coef { kLse, kRest, kOut, kIn, kCoefs };
+struct RowOut {
+  float *losses, *covered;
+  float* grads;  // [n][k]: G of every given token
+  float* coef;   // [kCoefs][n]
+  int n;
+};
+
+// Sum of 2^((z - M) log2(e) / T) over a set of logits and their largest.
+struct Sum { float M, s; };
+constexpr float kLowest = -3.402823466e38f;
+template <int N>
+__device__ __forceinline__ void fold(Sum& a, const float (&z)[8], float k) {
+  float m = z[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) m = fmaxf(m, z[j]);
+  if (m > a.M) {
+    a.s *= __builtin_amdgcn_exp2f((a.M - m) * k);
+    a.M = m;
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((z[j] - a.M) * k);
+  a.s += s;
+}
+
+// The bytes that say which elements of a share's vectors are given, and the same for the few elements outside vectors.
+struct Given {
+  uint32_t* bytes;   // LDS, a byte per vector of [q_lo, q_hi)
+  uint32_t* single;  // LDS, a bit per element outside the vectors
+};
+template <typename T>
+__device__ __forceinline__ void mark_given(const Given& g, const Teacher& t, int64_t row, int vocab, const RowSpan& sp, int threads) {
+  constexpr int kPer = Row<T>::kPer;
+  const int words = (sp.q_hi - sp.q_lo + 3) / 4;
+  for (int i = threadIdx.x; i < words; i += threads) g.bytes[i] = 0;
+  if (threadIdx.x == 0) *g.single = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.k; i += threads) {
+    const int id = teacher_id(t, row * t.k + i, vocab);
+    if (id < 0) continue;
+    const int in = id - sp.head, q = in >= 0 ? in / kPer : -1;
+    if (q >= 0 && q < sp.n_vec) {
+      const int at = q - sp.q_lo;
+      if (at >= 0 && q < sp.q_hi) atomicOr(g.bytes + (at >> 2), 1u << ((at & 3) * 8 + in % kPer));
+    } else {
+      atomicOr(g.single, 1u << (in < 0 ? id : id - sp.n_vec * kPer));
+    }
+  }
+  __syncthreads();
+}
+
+// Workgroup (row, part): the statistics of its share of the row, of what is not given where that is an outcome (REST), in
+// parts[row][part].
+template <typename T, bool REST>
+__global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
+                                                               float4* __restrict__ parts) {
+  extern __shared__ __align__(16) uint32_t s_given[];
+  __shared__ uint32_t s_single;
+  __shared__ float red[2][kBlock / kWave];
+  const int row_i = blockIdx.x / n_parts, part = blockIdx.x % n_parts, tid = threadIdx.x;
+  if (t.weights != nullptr && t.weights[row_i] == 0.f) return;
+  const T* row = logits + (int64_t)row_i * ld;
+  constexpr int kPer = Row<T>::kPer;
+  const RowSpan sp(row, vocab, true, part, n_parts);
+  if (REST) mark_given<T>(Given{s_given, &s_single}, t, row_i, vocab, sp, kBlock);
+  const uint8_t* const given = reinterpret_cast<const uint8_t*>(s_given);
+  const T* body = row + sp.head;
+  const float k = t.inv_t * kLog2e;
+  Sum st{kLowest, 0.f};
+  auto one = [&](int q, float (&v)[8]) {
+    if (REST) {
+      const uint32_t out = given[q - sp.q_lo];
+      if (out != 0) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] = (out >> j & 1) ? -INFINITY : v[j];
+      }
+    }
+    fold<kPer>(st, v, k);
+  };
+  int q = sp.q_lo + tid;
+  for (; q + kBlock < sp.q_hi; q += 2 * kBlock) {
+    float v0[8], v1[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v0);
+    Row<T>::load(body + (uint32_t)(q + kBlock) * kPer, v1);
+    one(q, v0);
+    one(q + kBlock, v1);
+  }
+  for (; q < sp.q_hi; q += kBlock) {
+    float v[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v);
+    one(q, v);
+  }
+  if (part == 0 && tid < sp.n_scalar && !(REST && (s_single >> tid & 1))) {
+    const float v[8] = {Row<T>::one(row + sp.scalar<T>(tid))};
+    fold<1>(st, v, k);
+  }
+  const float m = wave_max(st.M);
+  const float s = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
+  if ((tid & (kWave - 1)) == 0) { red[0][tid / kWave] = m; red[1][tid / kWave] = s; }
+  __syncthreads();
+  if (tid != 0) return;
+  float M = red[0][0];
+  for (int w = 1; w < kBlock / kWave; ++w) M = fmaxf(M, red[0][w]);
+  double total = 0.0;
+  for (int w = 0; w < kBlock / kWave; ++w) total += (double)red[1][w] * __builtin_amdgcn_exp2f((red[0][w] - M) * k);
+  parts[blockIdx.x] = make_float4(M, (float)total, (float)(total - (float)total), 0.f);
+}
+
+// One outcome: its share of the loss and G.
+struct Term { double loss, g; };
+__device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) {
+  const double q = exp(lq), p = exp(lp);
+  if (t.divergence == AXON_DISTILL_FORWARD) return {q > 0.0 ? q * (lq - lp) : q - q, -q};
+  if (t.divergence == AXON_DISTILL_REVERSE) {
+    if (p == 0.0) return {0.0, 0.0};
+    const double d = p * (lp - lq);
+    return {d, d + p};
+  }
+  const double b = (double)t.beta, lm = log(b * q + (1.0 - b) * p);
+  const double mine = p == 0.0 ? 0.0 : (1.0 - b) * p * (lp - lm);
+  return {(q == 0.0 ? 0.0 : b * q * (lq - lm)) + mine, mine};
+}
+
+struct FinishLds {
+  int id[kMaxIds];
+  double red[kBlock / kWave][4];
+  double total[4];
+};
+__device__ __forceinline__ void sum4(double (&v)[4], FinishLds& s) {
+  const int wave = threadIdx.x / kWave;
+  __syncthreads();  // `total` of the sum before has been read
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = wave_sum_d(v[i]);
+  if ((threadIdx.x & (kWave - 1)) == 0 && wave < kBlock / kWave)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.red[wave][i] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = 0.0;
+    for (int w = 0; w < kBlock / kWave; ++w) v[i] += s.red[w][i];
+  }
+}
+
+// The outcomes of a row, given the statistics of the row (or, REST, of what is not given): losses, G, and the row's coefficients.
+// By the first kBlock threads of a workgroup; the others come along to the barriers.
+template <typename T, bool REST>
+__device__ __forceinline__ void finish_row(int row_i, const T* row, int vocab, const Teacher& t, const RowOut& out, float M_in, double s_in,
+                                           FinishLds& lds) {
+  constexpr int kSlots = kMaxIds / kBlock;
+  const int tid = threadIdx.x;
+  const bool mine = tid < kBlock;
+  const double inv_t = (double)t.inv_t;
+  float z[kSlots];
+  double lq[kSlots];
+  int id[kSlots];
+  bool first[kSlots];
+  float M = M_in;
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * kBlock;
+    id[u] = -1;
+    z[u] = -INFINITY;
+    lq[u] = -INFINITY;
+    if (mine && i < t.k) {
+      id[u] = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
+      if (id[u] >= 0) {
+        z[u] = Row<T>::one(row + id[u]);
+        lq[u] = (double)t.logprobs[(int64_t)row_i * t.k + i];
+      }
+      lds.id[i] = id[u];
+    }
+  }
+  __syncthreads();
+  // the largest of the given ones, and of their teacher's log-probabilities, for all
+  float best = -INFINITY, best_q = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    best = fmaxf(best, z[u]);
+    best_q = fmaxf(best_q, (float)lq[u]);
+    first[u] = id[u] >= 0;
+    if (REST && id[u] >= 0)
+      for (int j = 0; j < tid + u * kBlock; ++j) first[u] = first[u] && lds.id[j] != id[u];
+  }
+  best = wave_max(best);
+  best_q = wave_max(best_q);
+  if (mine && (tid & (kWave - 1)) == 0) { lds.red[tid / kWave][0] = best; lds.red[tid / kWave][1] = best_q; }
+  __syncthreads();
+  for (int w = 0; w < kBlock / kWave; ++w) {
+    M = fmaxf(M, (float)lds.red[w][0]);
+    best_q = fmaxf(best_q, (float)lds.red[w][1]);
+  }
+  const double scale_in = exp(((double)M_in - (double)M) * inv_t);  // of the statistics to the reference M
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    if (id[u] < 0) continue;
+    if (REST && first[u]) v[0] += exp(((double)z[u] - (double)M) * inv_t);
+    if (t.tail == AXON_DISTILL_RENORMALIZE) v[1] += exp(lq[u] - (double)best_q);
+    if (REST) v[2] += exp(lq[u]);
+  }
+  sum4(v, lds);
+  const double s_rest = s_in * scale_in, s = REST ? s_rest + v[0] : s_rest;
+  const double ln_s = s > 0.0 ? log(s) : (double)NAN;  // a row of -inf alone has no softmax
+  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log(v[1]) : 0.0;
+  const double q_rest = fmax(1.0 - v[2], 0.0), lp_rest = log(s_rest) - ln_s;
+  double w[4] = {0.0, 0.0, 0.0, 0.0};  // loss, sum of G, covered
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * kBlock;
+    if (!mine || i >= t.k) continue;
+    Term o{0.0, 0.0};
+    if (id[u] >= 0) {
+      const double lp = ((double)z[u] - (double)M) * inv_t - ln_s;
+      o = outcome(t, lq[u] - norm_q, lp);
+      w[2] += exp(lp);
+    }
+    w[0] += o.loss;
+    w[1] += o.g;
+    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
+  }
+  sum4(w, lds);
+  if (tid != 0) return;
+  double out_scale = 0.0;
+  if (REST) {
+    const Term o = outcome(t, log(q_rest), lp_rest);
+    w[0] += o.loss;
+    w[1] += o.g;
+    out_scale = s_rest > 0.0 ? o.g * exp(-lp_rest) : 0.0;
+  }
+  const float lse = (float)((double)M + ln_s / inv_t);
+  out.losses[row_i] = (float)w[0];
+  out.covered[row_i] = (float)w[2];
+  float* const c = out.coef + row_i;
+  c[(int64_t)kLse * out.n] = lse;
+  c[(int64_t)kRest * out.n] = (float)((((double)M - (double)lse) * inv_t + ln_s) * 1.4426950408889634);
+  c[(int64_t)kOut * out.n] = (float)(out_scale - w[1]);
+  c[(int64_t)kIn * out.n] = (float)-w[1];
+}
+
+// Rows whose statistics several workgroups have left, or one, by a workgroup per row.
+template <typename T, bool REST>
+__global__ __launch_bounds__(kBlock) void distill_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
+                                                                const float4* __restrict__ parts, RowOut out) {
+  __shared__ FinishLds lds;
+  const int row_i = blockIdx.x, lane = threadIdx.x & (kWave - 1);
+  if (t.weights != nullptr && t.weights[row_i] == 0.f) {
+    if (threadIdx.x == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
+    return;
+  }
+  float M = kLowest;
+  double s = 0.0;
+  const float4 p = lane < n_parts ? parts[(int64_t)row_i * n_parts + lane] : make_float4(kLowest, 0.f, 0.f, 0.f);
+  M = wave_max(p.x);
+  s = wave_sum_d(((double)p.y + (double)p.z) * exp(((double)p.x - (double)M) * (double)t.inv_t));
+  finish_row<T, REST>(row_i, logits + (int64_t)row_i * ld, vocab, t, out, M, s, lds);
+}
+
+// Workgroup (row, part): dlogits of its share.  The row is streamed without a look at the given tokens; their few elements are
+// written again afterwards, from logits that were read before (dlogits may be the logits' own storage).  Equal ids of a row add
+// up in their order, in the thread of the first of them.  upstream: of every row's loss, or (weights) one for all, and where that
+// is 1 the gradient is there already (`ready`).
+template <typename T>
+__global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, int64_t ld, int vocab, Teacher t, RowOut saved,
+                                                              const float* __restrict__ upstream, int ready, T* dlogits, int64_t ld_d,
+                                                              int vec_ok, int n_parts) {
+  constexpr int kPer = Row<T>::kPer, kSlots = kMaxIds / kBlock;
+  __shared__ int ids[kMaxIds];
+  const int b = gridDim.x - 1 - blockIdx.x, row_i = b / n_parts, part = b - row_i * n_parts, tid = threadIdx.x;
+  const float up = upstream != nullptr ? upstream[t.weights != nullptr ? 0 : row_i] : 1.f;
+  if (ready && up == 1.f) return;
+  const float w = t.weights != nullptr ? t.weights[row_i] : 1.f;
+  const bool skip = t.weights != nullptr && w == 0.f;
+  const float g = up * w * t.inv_t;
+  const T* row = logits + (int64_t)row_i * ld;
+  T* out = dlogits + (int64_t)row_i * ld_d;
+  const float* const c = saved.coef + row_i;
+  const float lse = skip ? 0.f : c[(int64_t)kLse * saved.n], rest = skip ? 0.f : c[(int64_t)kRest * saved.n];
+  const float c_out = skip ? 0.f : g * c[(int64_t)kOut * saved.n], c_in = skip ? 0.f : g * c[(int64_t)kIn * saved.n];
+  const float k = t.inv_t * kLog2e;
+  auto prob = [&](float z) { return __builtin_amdgcn_exp2f(fmaf(z - lse, k, -rest)); };
+  const RowSpan sp(row, vocab, vec_ok != 0, part, n_parts);
+  float again[kSlots];
+  int where[kSlots];
+  for (int i = tid; i < t.k; i += kBlock) ids[i] = skip ? -1 : teacher_id(t, (int64_t)row_i * t.k + i, vocab);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * kBlock;
+    where[u] = -1;
+    const int id = i < t.k ? ids[i] : -1;
+    if (id < 0) continue;
+    const int in = id - sp.head, q = in / kPer;
+    const bool vec = in >= 0 && q < sp.n_vec;
+    if (vec) {
+      if (q < sp.q_lo || q >= sp.q_hi) continue;
+    } else if ((in < 0 ? id : id - sp.n_vec * kPer) / kBlock % n_parts != part) {
+      continue;
+    }
+    float total = 0.f;
+    bool first = true;
+    for (int j = 0; j < t.k && first; ++j) {
+      if (ids[j] != id) continue;
+      first = j >= i;
+      total += saved.grads[(int64_t)row_i * t.k + j];
+    }
+    if (!first) continue;
+    where[u] = id;
+    again[u] = fmaf(prob(Row<T>::one(row + id)), c_in, g * total);
+  }
+  __syncthreads();  // nothing of the row is written before these are read
+  const T* body = row + sp.head;
+  T* body_out = out + sp.head;
+  auto finish = [&](int q, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = prob(v[j]) * c_out;
+    Row<T>::store(body_out + (uint32_t)q * kPer, v);
+  };
+  if (skip) {
+    for (int q = sp.q_lo + tid; q < sp.q_hi; q += kBlock) {
+      const float v[8] = {};
+      Row<T>::store(body_out + (uint32_t)q * kPer, v);
+    }
+    for (int i = part * kBlock + tid; i < sp.n_scalar; i += n_parts * kBlock) Row<T>::store_one(out + sp.scalar<T>(i), 0.f);
+    return;
+  }
+  int q = sp.q_hi - 1 - tid;
+  for (; q - kBlock >= sp.q_lo; q -= 2 * kBlock) {  // two loads in flight per thread
+    float v0[8], v1[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v0);
+    Row<T>::load(body + (uint32_t)(q - kBlock) * kPer, v1);
+    finish(q, v0);
+    finish(q - kBlock, v1);
+  }
+  for (; q >= sp.q_lo; q -= kBlock) {
+    float v[8];
+    Row<T>::load(body + (uint32_t)q * kPer, v);
+    finish(q, v);
+  }
+  for (int i = part * kBlock + tid; i < sp.n_scalar; i += n_parts * kBlock) {
+    const int j = sp.scalar<T>(i);
+    Row<T>::store_one(out + j, prob(Row<T>::one(row + j)) * c_out);
+  }
+  // the stores above are acknowledged before another thread of the workgroup writes the same element
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0)
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u)
+    if (where[u] >= 0) Row<T>::store_one(out + where[u], again[u]);
+}
+
+// sum_t w_t loss_t in 64 bits, in a fixed order.
+constexpr int kSumBlock = 1024;
+__global__ __launch_bounds__(kSumBlock) void distill_sum_kernel(const float* __restrict__ losses, const float* __restrict__ weights, int n,
+                                                                float* __restrict__ loss) {
+  __shared__ double red[kSumBlock / kWave];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kSumBlock) {
+    const float w = weights[i];
+    if (w != 0.f) s += (double)w * (double)losses[i];
+  }
+  s = wave_sum_d(s);
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kSumBlock / kWave; ++w) s += red[w];
+  *loss = (float)s;
+}
+
+}  // namespace axon
+
+using namespace axon;
+
+namespace {
+
+int elem_bytes(int dtype) { return dtype == AXON_LOGITS_F32 ? 4 : 2; }
+
+int check_rows(const void* p, int dtype, int64_t ld, int64_t n, int64_t v) {
+  if (n < 0 || v <= 0 || ld < v || (dtype != AXON_LOGITS_F32 && dtype != AXON_LOGITS_BF16)) return AXON_ERR_ARG;
+  if (n >= (int64_t)1 << 24 || v > (int64_t)kMaxShare * kMaxParts) return AXON_ERR_SHAPE;
+  if (n > 0 && (!p || reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype) != 0)) return AXON_ERR_ARG;
+  return AXON_OK;
+}
+
+int check_teacher(const void* ids, const float* logprobs, int64_t k, int divergence, int tail, float beta, float temperature) {
+  if (k < 1 || k > kMaxIds) return AXON_ERR_SHAPE;
+  if (!ids || !logprobs || divergence < AXON_DISTILL_FORWARD || divergence > AXON_DISTILL_JSD || tail < AXON_DISTILL_DROP ||
+      tail > AXON_DISTILL_RENORMALIZE)
+    return AXON_ERR_ARG;
+  if (!(temperature > 0.f) || !(temperature <= 3.402823466e38f)) return AXON_ERR_ARG;
+  if (divergence == AXON_DISTILL_JSD && !(beta > 0.f && beta < 1.f)) return AXON_ERR_ARG;
+  return AXON_OK;
+}
+
+// Workgroups per row of the backward: as in logits.hip, whose backward moves the same bytes.
+int grad_parts(int64_t n, int64_t vocab, int eb) {
+  if (n >= 1536) return 1;
+  const int64_t fill = 8192 / (n > 0 ? n : 1), work = vocab * eb / (8 * 16 * kBlock);
+  const int64_t p = fill < work ? fill : work;
+  return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
+}
+// ... and of the forward: about 2048 pieces, what the part holds at once, none of them beyond what LDS describes.
+int stats_parts(int64_t n, int64_t vocab, int eb) {
+  const int64_t fill = 2048 / (n > 0 ? n : 1), work = vocab * eb / (4 * 16 * kBlock), least = (vocab * eb / 16 + kMaxShare - 1) / kMaxShare;
+  int64_t p = fill < work ? fill : work;
+  p = p < least ? least : p;
+  return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
+}
+
+}  // namespace
+
+#define AXON_ROWS(dtype, CALL)                  \
+  do {                                          \
+    if ((dtype) == AXON_LOGITS_F32) CALL(float); \
+    else CALL(unsigned short);                  \
+  } while (0)
+
+extern "C" int64_t axon_distill_workspace_bytes(int dtype, int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0 || (dtype != AXON_LOGITS_F32 && dtype != AXON_LOGITS_BF16)) return AXON_ERR_ARG;
+  return n * stats_parts(n, vocab, elem_bytes(dtype)) * (int64_t)sizeof(float4);
+}
+
+extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_i64,
+                                const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
+                                float temperature, float* losses, float* covered, float* grads, float* coef, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK && n > 0) rc = check_teacher(ids, teacher_logprobs, k, divergence, tail, beta, temperature);
+  if (rc != AXON_OK || n == 0) return rc;
+  if (!losses || !covered || !grads || !coef) return AXON_ERR_ARG;
+  if (!workspace || workspace_bytes < axon_distill_workspace_bytes(dtype, n, vocab) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return AXON_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  const int eb = elem_bytes(dtype), parts = stats_parts(n, vocab, eb);
+  const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail, beta, 1.f / temperature};
+  const RowOut out{losses, covered, grads, coef, (int)n};
+  float4* const ws = static_cast<float4*>(workspace);
+  const unsigned lds = (unsigned)(((vocab * eb / 16 + parts - 1) / parts + 1 + 3) / 4 * 4);
+#define AXON_FWD(T, REST)                                                                                                          \
+  do {                                                                                                                             \
+    hipLaunchKernelGGL((distill_stats_kernel<T, REST>), dim3((unsigned)(n * parts)), dim3(kBlock), REST ? lds : 0, st,             \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, t, ws);                                               \
+    AXON_CHECK_LAUNCH();                                                                                                           \
+    hipLaunchKernelGGL((distill_finish_kernel<T, REST>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
+                       (int)vocab, parts, t, ws, out);                                                                             \
+  } while (0)
+#define AXON_FWD_OF(T) \
+  do {                 \
+    if (tail == AXON_DISTILL_REST) AXON_FWD(T, true); else AXON_FWD(T, false); \
+  } while (0)
+  AXON_ROWS(dtype, AXON_FWD_OF);
+#undef AXON_FWD_OF
+#undef AXON_FWD
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_i64,
+                                int64_t k, const float* weights, float temperature, const float* grads, const float* coef,
+                                const float* upstream, int ready, void* dlogits, int64_t ld_d, void* stream) {
+  int rc = check_rows(logits, dtype, ld, n, vocab);
+  if (rc == AXON_OK) rc = check_rows(dlogits, dtype, ld_d, n, vocab);
+  if (rc != AXON_OK || n == 0) return rc;
+  if (k < 1 || k > kMaxIds) return AXON_ERR_SHAPE;
+  if (!ids || !grads || !coef || !(temperature > 0.f) || (!upstream && !weights) || (ready && (!weights || !upstream))) return AXON_ERR_ARG;
+  const hipStream_t st = (hipStream_t)stream;
+  const int eb = elem_bytes(dtype), parts = grad_parts(n, vocab, eb);
+  // every row of dlogits sits on the same offset from a 16-byte boundary as the row of logits
+  const int vec_ok = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0 &&
+                     (n <= 1 || ((ld - ld_d) * eb) % 16 == 0);
+  const Teacher t{ids, nullptr, weights, ids_i64, (int)k, 0, 0, 0.f, 1.f / temperature};
+  const RowOut saved{nullptr, nullptr, const_cast<float*>(grads), const_cast<float*>(coef), (int)n};
+#define AXON_GRAD(T)                                                                                                              \
+  hipLaunchKernelGGL((distill_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
+                     (int)vocab, t, saved, upstream, ready, static_cast<T*>(dlogits), ld_d, vec_ok, parts)
+  AXON_ROWS(dtype, AXON_GRAD);
+#undef AXON_GRAD
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+extern "C" int axon_distill_loss(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_i64,
+                                 const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
+                                 float temperature, float* loss, float* losses, float* covered, float* grads, float* coef, void* dlogits,
+                                 int64_t ld_d, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!loss || (n > 0 && !weights)) return AXON_ERR_ARG;
+  int rc = dlogits ? check_rows(dlogits, dtype, ld_d, n, vocab) : AXON_OK;
+  if (rc == AXON_OK)
+    rc = axon_distill_fwd(logits, dtype, ld, n, vocab, ids, ids_i64, teacher_logprobs, k, weights, divergence, tail, beta, temperature, losses,
+                          covered, grads, coef, workspace, workspace_bytes, stream);
+  if (rc == AXON_OK && dlogits)
+    rc = axon_distill_bwd(logits, dtype, ld, n, vocab, ids, ids_i64, k, weights, temperature, grads, coef, nullptr, 0, dlogits, ld_d, stream);
+  if (rc != AXON_OK) return rc;
+  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumBlock), 0, (hipStream_t)stream, losses, weights, (int)n, loss);
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}

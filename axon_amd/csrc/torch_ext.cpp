@@ -1088,6 +1088,149 @@ std::tuple<Tensor, Tensor> controlled_logprobs(const Tensor& logits, const Tenso
   return {lp, entropy};
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Distillation from a teacher's top logits.
+// ---------------------------------------------------------------------------------------------------------------------
+
+// The graph that the current stream is being captured into, 0 outside of a capture.
+unsigned long long capture_id() {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)::stream(), &status, &id) != hipSuccess) throw AxonError("the state of the stream cannot be asked for");
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
+struct DistillNode : torch::autograd::Node {
+  SavedVariable rows, ids, grads, coef, weights;
+  Tensor ready;  // with weights: the gradient of an upstream gradient of 1, which the forward has left
+  unsigned long long captured = 0;  // ... into this graph
+  std::vector<int64_t> shape;
+  float temperature = 1.f;
+  bool weighted = false, inplace = false, spent = false;
+  static constexpr const char* kWhat = "distillation_backward";
+  std::string name() const override { return "DistillationBackward"; }
+  void release_variables() override {
+    for (SavedVariable* s : {&rows, &ids, &grads, &coef, &weights}) s->reset_data();
+    ready.reset();
+  }
+  variable_list apply(variable_list&& g) override {
+    if (!g[0].defined()) return {Tensor()};
+    if (spent) throw AxonError("the logits' storage holds the gradient of an earlier backward (inplace_backward)");
+    const Tensor x = rows.unpack(), at = ids.unpack(), gr = grads.unpack(), co = coef.unpack(), w = weights.unpack();
+    Tensor out;
+    {
+      const at::NoGradGuard no_grad;
+      check_saved_rows(kWhat, x);
+      const int64_t n = x.size(0), v = x.size(1);
+      const Tensor up = f32(g[0]);
+      same_place(kWhat, x, {&at, &gr, &co, &w, &up});
+      const int dtype = logits_dtype(kWhat, x);
+      same_type(kWhat, at::kFloat, {&gr, &co, &w});
+      if (!is_index(at) || at.dim() != 2) refuse(kWhat, "a saved tensor has come back in another type");
+      const int64_t k = at.size(1);
+      same_len(kWhat, "ids", n * k, at);
+      same_len(kWhat, "gradients", n * k, gr);
+      same_len(kWhat, "coefficients", 4 * n, co);
+      same_len(kWhat, "upstream gradient", weighted ? 1 : n, up);
+      if (weighted) same_len(kWhat, "token_weights", n, w);
+      const c10::DeviceGuard device(x.device());
+      // The gradient that the forward has left is handed on once, and only where a replay of this launch comes behind one of the
+      // forward's: what a caller does to it must not come back.
+      const bool there = ready.defined() && captured == capture_id();
+      out = there ? ready : inplace ? x : at::empty({n, v}, x.options());
+      ready.reset();
+      check(axon_distill_bwd(x.data_ptr(), dtype, row_stride(x), n, v, at.data_ptr(), is_i64(at), k, (const float*)ptr(w), temperature,
+                             (const float*)gr.data_ptr(), (const float*)co.data_ptr(), (const float*)up.data_ptr(), there, out.data_ptr(),
+                             row_stride(out), ::stream()),
+            "axon_distill_bwd");
+      spent = inplace;
+      if (inplace && !x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+      out = out.view(shape);
+    }
+    return {once(std::move(out), kWhat)};
+  }
+};
+
+// (weighted sum of the losses or none, losses, covered)
+std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& logits, const Tensor& teacher_ids, const Tensor& teacher_logprobs,
+                                              const OptTensor& token_weights, int divergence, int tail, double beta, double temperature,
+                                              bool inplace) {
+  const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
+  no_tangent(what, logits);
+  Tensor rows, ids, w, loss, losses, covered, grads, coef, ready;
+  {
+    const at::NoGradGuard no_grad;
+    rows = rows_of_logits(logits);
+    const int64_t n = rows.size(0), v = rows.size(1);
+    const int dtype = logits_dtype(what, rows);
+    const std::vector<int64_t> batch(logits.sizes().begin(), logits.sizes().end() - 1);
+    if (!is_index(teacher_ids)) refuse(what, std::string("teacher_ids must be int32 or int64, got ") + c10::toString(teacher_ids.scalar_type()));
+    if (!teacher_logprobs.is_floating_point()) refuse(what, "teacher_logprobs must be floating point");
+    if (teacher_ids.dim() != logits.dim() || teacher_ids.sizes().slice(0, teacher_ids.dim() - 1) != at::IntArrayRef(batch))
+      refuse(what, "teacher_ids " + shape_text(teacher_ids) + " do not lie beside logits " + shape_text(logits));
+    if (teacher_logprobs.sizes() != teacher_ids.sizes())
+      refuse(what, "teacher_logprobs " + shape_text(teacher_logprobs) + " do not lie beside teacher_ids " + shape_text(teacher_ids));
+    if (teacher_logprobs.requires_grad()) refuse(what, "teacher_logprobs have no gradient: pass them detached");
+    const int64_t k = teacher_ids.size(-1);
+    if (k < 1 || k > AXON_MAX_TOKEN_IDS)
+      refuse(what, "between 1 and " + std::to_string(AXON_MAX_TOKEN_IDS) + " teacher_ids per position, got " + std::to_string(k));
+    for (const Tensor* t : {&teacher_ids, &teacher_logprobs})
+      if (t->device() != logits.device()) refuse(what, "operands live on different devices");
+    if (token_weights) {
+      if (token_weights->sizes() != at::IntArrayRef(batch))
+        refuse(what, "token_weights " + shape_text(*token_weights) + " do not lie beside logits " + shape_text(logits));
+      if (token_weights->requires_grad()) refuse(what, "token_weights have no gradient: pass them detached");
+      if (token_weights->device() != logits.device()) refuse(what, "operands live on different devices");
+    }
+    require_device(rows, what);
+    const c10::DeviceGuard device(rows.device());
+    ids = teacher_ids.reshape({n, k}).contiguous();
+    const Tensor lq = f32(teacher_logprobs);
+    if (token_weights) w = f32(*token_weights);
+    losses = at::empty(batch, opts(rows));
+    covered = at::empty(batch, opts(rows));
+    grads = at::empty({n, k}, opts(rows));
+    coef = at::empty({4, n}, opts(rows));
+    const int64_t need = axon_distill_workspace_bytes(dtype, n, v);
+    const Tensor ws = at::empty({std::max<int64_t>(need, 0)}, opts(rows, at::kByte));
+    float *const losses_p = losses.data_ptr<float>(), *const covered_p = covered.data_ptr<float>(), *const grads_p = grads.data_ptr<float>(),
+                *const coef_p = coef.data_ptr<float>();
+    if (token_weights) {
+      loss = at::empty({}, opts(rows));
+      if (wants_grad) ready = at::empty({n, v}, rows.options());
+      check(axon_distill_loss(rows.data_ptr(), dtype, row_stride(rows), n, v, ids.data_ptr(), is_i64(ids), (const float*)lq.data_ptr(), k,
+                              (const float*)w.data_ptr(), divergence, tail, (float)beta, (float)temperature, loss.data_ptr<float>(), losses_p,
+                              covered_p, grads_p, coef_p, wants_grad ? ready.data_ptr() : nullptr, v, ws.data_ptr(), need, stream()),
+            "axon_distill_loss");
+    } else {
+      check(axon_distill_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, ids.data_ptr(), is_i64(ids), (const float*)lq.data_ptr(), k, nullptr,
+                             divergence, tail, (float)beta, (float)temperature, losses_p, covered_p, grads_p, coef_p, ws.data_ptr(), need,
+                             stream()),
+            "axon_distill_fwd");
+    }
+  }
+  if (wants_grad) {
+    std::shared_ptr<DistillNode> node(new DistillNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->shape = logits.sizes().vec();
+    node->weighted = token_weights.has_value();
+    node->inplace = !node->weighted && inplace && rows.data_ptr() == logits.data_ptr();
+    node->temperature = (float)temperature;
+    torch::autograd::set_history(node->weighted ? loss : losses, node);
+    node->rows = SavedVariable(rows, false);
+    node->ids = SavedVariable(ids, false);
+    node->grads = SavedVariable(grads, false);
+    node->coef = SavedVariable(coef, false);
+    node->weights = SavedVariable(w, false);
+    if (node->weighted) {
+      const c10::DeviceGuard device(rows.device());
+      node->captured = capture_id();
+      node->ready = std::move(ready);
+    }
+  }
+  return {loss.defined() ? OptTensor(loss) : OptTensor(), losses, covered};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1127,6 +1270,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init<const OptTensor&, const OptTensor&, bool, const OptTensor&, const Controls::Value&, const Controls::Value&,
                     const Controls::Value&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Controls::Value&>(),
            unlocked);
+  m.def("distill", [](const Tensor& logits, const Tensor& ids, const Tensor& logprobs, const OptTensor& weights, int divergence, int tail,
+                      double beta, double temperature, bool inplace) {
+    return distill(weights ? "distillation_loss_from_logits" : "distillation_from_logits", logits, ids, logprobs, weights, divergence, tail,
+                   beta, temperature, inplace);
+  }, unlocked);
   m.def("controlled_logits", &controlled_logits, unlocked);
   m.def("controlled_logprobs", &controlled_logprobs, unlocked);
 }

@@ -778,6 +778,36 @@ int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t
                               const void* labels, int labels_are_i64, const float* stats, const float* g_logprob,
                               const float* g_entropy, void* dlogits, int64_t ld_d, void* stream);
 
+/* Distillation from a teacher's top logits (no reference counterpart).  Per position, with q the teacher's probabilities of k given
+ * tokens (ids [n][k] int32 or int64, an id outside [0, vocab) is a filler; log-probabilities [n][k]) and p the student's,
+ * softmax(logits / temperature) over the whole vocabulary:
+ *   AXON_DISTILL_FORWARD  sum q log(q / p),  AXON_DISTILL_REVERSE  sum p log(p / q),
+ *   AXON_DISTILL_JSD      beta sum q log(q / m) + (1 - beta) sum p log(p / m),  m = beta q + (1 - beta) p,  0 < beta < 1
+ * over the given tokens (AXON_DISTILL_DROP), over these with q divided by its sum (AXON_DISTILL_RENORMALIZE), or with what is
+ * left of both, 1 - sum q and the student's tokens that are not given, as one more outcome (AXON_DISTILL_REST).  An id that
+ * comes twice is two outcomes.  1 <= k <= AXON_MAX_TOKEN_IDS, vocab at most 3145728.
+ *   losses, covered [n]: the divergence, and the student's probability of the given tokens.  grads [n][k], coef [4][n]: what
+ *        the backward reads.  Workspace 16-byte aligned.
+ *   weights [n] (may be NULL in _fwd): a row of weight 0 is not looked at: loss, covered and gradient are 0.
+ *   _bwd: dlogits from the losses' gradients upstream [n], or, with weights, weights[row] * upstream[0] (upstream NULL: 1).  With
+ *        `ready` the caller has the gradient of upstream 1 in dlogits, and nothing is written where upstream[0] is that.
+ *        dlogits may be the logits' own storage.
+ *   _loss: loss[0] = sum weights * losses, and dlogits (NULL: not wanted) of that loss beside it. */
+enum { AXON_DISTILL_FORWARD = 0, AXON_DISTILL_REVERSE = 1, AXON_DISTILL_JSD = 2 };
+enum { AXON_DISTILL_DROP = 0, AXON_DISTILL_REST = 1, AXON_DISTILL_RENORMALIZE = 2 };
+int64_t axon_distill_workspace_bytes(int dtype, int64_t n, int64_t vocab);
+int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
+                     const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
+                     float temperature, float* losses, float* covered, float* grads, float* coef, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
+                     int64_t k, const float* weights, float temperature, const float* grads, const float* coef,
+                     const float* upstream, int ready, void* dlogits, int64_t ld_d, void* stream);
+int axon_distill_loss(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
+                      const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
+                      float temperature, float* loss, float* losses, float* covered, float* grads, float* coef, void* dlogits,
+                      int64_t ld_d, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* KL penalty inside the reward, the tensor part of apply_kl_penalty (axon/utils/rl/kl.py:276-322):
  *   kld = kl_penalty(old_logp, ref_logp, kl_type) * mask      (types as in axon_kl_penalty)
  *   rewards = scores - beta * kld
