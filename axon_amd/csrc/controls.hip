@@ -30,6 +30,7 @@ template <> struct Unaligned<float> {
   struct __attribute__((packed, aligned(4))) Box { Raw v; };
   __device__ static Raw load(const float* p) { return reinterpret_cast<const Box*>(p)->v; }
   __device__ static float get(const Raw& r, int j) { return r[j]; }
+  __device__ static void set(Raw& r, int j, const float* p) { r[j] = *p; }
   __device__ static void store(float* p, const float* v) {
     Box b;
     b.v = Raw{v[0], v[1], v[2], v[3]};
@@ -44,6 +45,7 @@ template <> struct Unaligned<unsigned short> {
   __device__ static float get(const Raw& r, int j) {
     return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16));
   }
+  __device__ static void set(Raw& r, int j, const unsigned short* p) { r[j >> 1] |= (uint32_t)*p << ((j & 1) * 16); }  // of a 0
   __device__ static void store(unsigned short* p, const float* v) {
     Box b;
     b.v = Raw{f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
@@ -63,6 +65,8 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+constexpr float kBanned = -1e30f;  // stands for -inf where a product with it has to stay finite
+constexpr float kFar = 1e9f;       // a reference in log2 units whose rounding (64) leaves the exponentials in range
 constexpr float kNoLogit = -3.402823466e38f;  // the reference of a set without a logit: any there is is at least as large
 
 // A token of a history: its id, or -1 where it counts for nothing; bit 30 where the model has generated it.
@@ -85,7 +89,7 @@ struct RowIo {
   int labels_i64;
   float* label_y;             // [rows], kStats
   float4* parts;              // [rows][chunks] (M, s, e), kStats
-  const float* stats;         // [3][rows]: the row's log-sum-exp in two parts and its entropy, kGrad
+  const float* stats;         // [3][rows]: what controls_finish_kernel has left, kGrad
   const float *g_logprob, *g_entropy;
 };
 
@@ -96,16 +100,23 @@ __device__ __forceinline__ int slot(int off) {
   return PER == 4 ? off : (off & ~511) | ((off & 4) << 6) | ((off & 0x1f8) >> 1) | (off & 3);
 }
 
+// Bits of one lane's ids as masks of 32 bits, and a choice by such a mask: two instructions per element and no branch.
+__device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) { return (uint32_t)((int32_t)(bits << (31 - i)) >> 31); }
+__device__ __forceinline__ float pick(uint32_t mask, float yes, float no) {
+  return __uint_as_float((mask & __float_as_uint(yes)) | (~mask & __float_as_uint(no)));
+}
+
 template <typename T, Mode MODE, bool ADJ, bool MASK>
 __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
                                                           axon_controls c, RowIo io, const T* other, int64_t ld_other, T* out,
                                                           int64_t ld_out) {
   constexpr int kPer = Unaligned<T>::kPer, kVecs = kLaneIds / kPer;
-  __shared__ uint32_t s_adj[ADJ ? kGroupIds : 1];  // counts (bit 31: seen) while they are collected, then floats
+  constexpr uint32_t kVecBits = (1u << kPer) - 1;
+  __shared__ __align__(16) uint32_t s_adj[ADJ ? kGroupIds : 4];  // counts (bit 31: seen) while they are collected, then floats
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int groups = (chunks + kWaves - 1) / kWaves;
   const int first = (int)(blockIdx.x / groups) * run, group = (int)(blockIdx.x % groups);
-  const int last = min(first + run, n_rows);
+  const int rows = min(run, n_rows - first);
   const int chunk = group * kWaves + wave, base = chunk * kIds;
 
   // what belongs to row first + lane
@@ -145,18 +156,20 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
     const int64_t l = index_at(io.labels, io.labels_i64, mine);
     label = l >= 0 && l < vocab ? (int)l : -1;
   }
-  float lse_l = 0.f, rest_l = 0.f, ent_l = 0.f, glp_l = 0.f, gen_l = 0.f;
+  // kGrad: dz = 2^t (A + B t) slope with t = (y - M) log2(e) / T, the row's constants in A and B
+  float top_l = 0.f, a_l = 0.f, b_l = 0.f, glp_l = 0.f;
   if (MODE == kGrad) {
-    lse_l = io.stats[mine];
-    rest_l = io.stats[(int64_t)n_rows + mine];
-    ent_l = io.stats[2 * (int64_t)n_rows + mine];
-    glp_l = io.g_logprob && label >= 0 ? io.g_logprob[mine] : 0.f;
-    gen_l = io.g_entropy ? io.g_entropy[mine] : 0.f;
+    top_l = io.stats[mine];
+    const float sum = io.stats[(int64_t)n_rows + mine], ls = __log2f(sum), H = io.stats[2 * (int64_t)n_rows + mine];
+    const float g_en = io.g_entropy ? io.g_entropy[mine] : 0.f;
+    const float q = inv_t_l / sum, g_lp = io.g_logprob && label >= 0 ? io.g_logprob[mine] : 0.f;
+    glp_l = g_lp * inv_t_l;
+    a_l = q * -fmaf(g_en, fmaf(-kLn2, ls, H), g_lp);
+    b_l = q * -g_en * kLn2;
   }
 
   uint32_t* const adj = s_adj + (ADJ ? wave * kIds : 0);
-  const float* const adj_f = reinterpret_cast<const float*>(adj);
-  uint32_t seen = 0;  // bit u * kPer + j: this lane's id of vector u, element j
+  uint32_t seen = 0;     // bit u * kPer + j: this lane's id of vector u, element j
   uint32_t touched = 0;  // bit u: some lane's vector u is not left as it is
   // counts and seen bits in LDS to additive terms, biases with them
   auto settle = [&](int row) {
@@ -166,16 +179,19 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
     seen = 0;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
-      uint32_t some = 0;
+      uint32_t w[kPer], some = 0;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int at = slot<kPer>((u * kWave + lane) * kPer + j);
-        const uint32_t w = adj[at];
-        some |= w;
-        seen |= (w >> 31) << (u * kPer + j);
-        adj[at] = __float_as_uint(penalty((int)(w & 0x7fffffffu), f, a));
+        w[j] = adj[slot<kPer>((u * kWave + lane) * kPer + j)];
+        some |= w[j];
       }
-      if (__any(some != 0)) any |= 1u << u;
+      if (!__any(some != 0)) continue;  // 0 is 0.f
+      any |= 1u << u;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        seen |= (w[j] >> 31) << (u * kPer + j);
+        adj[slot<kPer>((u * kWave + lane) * kPer + j)] = __float_as_uint(penalty((int)(w[j] & 0x7fffffffu), f, a));
+      }
     }
     wave_sync();
     for (int64_t i0 = 0; i0 < c.n_bias; i0 += kWave) {
@@ -210,19 +226,44 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
     __syncthreads();
   }
   if (chunk >= chunks) return;
-  if (ADJ) settle(0);
 
+  // the ids of this lane that there are
   const bool whole = base + kIds <= vocab;
-  for (int r = 0; r < last - first; ++r) {
+  uint32_t there = ~0u;
+  if (!whole) {
+    there = 0;
+#pragma unroll
+    for (int i = 0; i < kLaneIds; ++i) there |= (uint32_t)(base + ((i / kPer) * kWave + lane) * kPer + i % kPer < vocab) << i;
+  }
+  auto mask_of = [&](int r) {  // what of them row r may keep
+    const int st = lane_value(state, r);
+    if (st < 0) return there;
+    const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(c.allowed + (int64_t)st * c.allowed_stride) + base / 8;
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int id0 = (u * kWave + lane) * kPer;
+      if (whole || base + id0 < vocab) m |= (bytes[id0 >> 3] >> (id0 & 7) & kVecBits) << (u * kPer);
+    }
+    return m & there;
+  };
+
+  uint32_t keep_next = MASK ? mask_of(0) : there;
+  for (int r = 0; r < rows; ++r) {
     const int64_t row = first + r;
-    const float rep = lane_value(rep_l, r), inv_rep = 1.f / rep, inv_t = lane_value(inv_t_l, r);
-    if (ADJ && c.every_position) {
-      if (r > 0 && lane_value(start, r) != lane_value(start, r - 1)) {  // another sequence
+    const float inv_t = lane_value(inv_t_l, r), k = inv_t * kLog2e, rep = lane_value(rep_l, r), inv_rep = 1.f / rep;
+    uint32_t keep = keep_next;
+    // masks of single bits are made where they are used: 32 of them held over the rows are 32 registers
+    asm volatile("" : "+v"(keep), "+v"(seen));
+    if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
+      if (r > 0) {
 #pragma unroll
         for (int i = 0; i < kLaneIds; ++i) adj[i * kWave + lane] = 0;
         wave_sync();
-        settle(r);
       }
+      settle(r);
+    }
+    if (ADJ && c.every_position) {
       const int t = lane_value(token, r);
       const int id = t & (kOwn - 1), off = id - base;
       if (t >= 0 && off >= 0 && off < kIds) {  // the row's own token, counted anew: a sum of additions would drift
@@ -243,112 +284,162 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
       }
     }
     const T* const x = logits + row * ld + base;
-    const int st = MASK ? lane_value(state, r) : -1;
-    const uint8_t* const words = reinterpret_cast<const uint8_t*>(c.allowed + (int64_t)(st < 0 ? 0 : st) * c.allowed_stride);
+    const int l = MODE == kStats || MODE == kGrad ? lane_value(label, r) - base : -1;
+    const bool has_label = l >= 0 && l < kIds;
+    const int label_lane = l / kPer % kWave, label_at = l / (kWave * kPer) * kPer + l % kPer;
 
-    float z[kLaneIds], y[kLaneIds];
-    auto read = [&](const T* from, float (&v)[kLaneIds]) {
+    // what is not kept is not read either
+    typename Unaligned<T>::Raw raw[kVecs], raw_g[MODE == kApplyGrad ? kVecs : 1];
+    auto read = [&](const T* from, typename Unaligned<T>::Raw(&into)[kVecs]) {
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) {
         const int id0 = (u * kWave + lane) * kPer;
-        if (whole || base + id0 + kPer <= vocab) {
-          const auto raw = Unaligned<T>::load(from + id0);
+        into[u] = typename Unaligned<T>::Raw{};
+        if (MASK || !whole) {
+          if ((keep >> (u * kPer) & kVecBits) == 0) continue;
+          if (!whole && base + id0 + kPer > vocab) {
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) v[u * kPer + j] = Unaligned<T>::get(raw, j);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) v[u * kPer + j] = base + id0 + j < vocab ? Row<T>::one(from + id0 + j) : -INFINITY;
-        }
-      }
-    };
-    read(x, z);
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int id0 = (u * kWave + lane) * kPer;
-      uint32_t keep = (1u << kPer) - 1;
-      if (MASK && st >= 0) keep = base + id0 < vocab ? (uint32_t)words[(base + id0) >> 3] >> (id0 & 7) : 0;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int i = u * kPer + j;
-        float v = z[i];
-        if (ADJ && (touched >> u & 1)) {
-          if (seen >> i & 1) v = v > 0.f ? v * inv_rep : v * rep;
-          v -= adj_f[slot<kPer>(id0 + j)];
-        }
-        y[i] = (MASK && !(keep >> j & 1)) ? -INFINITY : v;
-      }
-    }
-
-    if (MODE == kStats) {
-      float m = y[0];
-#pragma unroll
-      for (int i = 1; i < kLaneIds; ++i) m = fmaxf(m, y[i]);
-      m = wave_max(m);
-      const float M = m > -INFINITY ? m : kNoLogit, k = inv_t * kLog2e;
-      float s4[4] = {}, e4[4] = {};
-#pragma unroll
-      for (int i = 0; i < kLaneIds; ++i) {
-        const float d = (y[i] - M) * k, f = __builtin_amdgcn_exp2f(d);
-        s4[i & 3] += f;
-        e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
-      }
-      const float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
-      if (lane == 0) io.parts[row * chunks + chunk] = make_float4(M, s, e, 0.f);
-      const int l = lane_value(label, r) - base;
-      if (l >= 0 && l < kIds) {
-        const int i = l / (kWave * kPer) * kPer + l % kPer;
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < kLaneIds; ++q) v = q == i ? y[q] : v;
-        if (lane == l / kPer % kWave) io.label_y[row] = v;
-      }
-    } else {
-      float* const d = z;  // what is written
-      if (MODE == kApply) {
-#pragma unroll
-        for (int i = 0; i < kLaneIds; ++i) d[i] = y[i] * inv_t;
-      } else {
-        float up[kLaneIds];
-        if (MODE == kApplyGrad) {
-          read(other + row * ld_other + base, up);
-        } else {
-          const float lse = lane_value(lse_l, r), rest = lane_value(rest_l, r), H = lane_value(ent_l, r);
-          const float g_lp = lane_value(glp_l, r), g_en = lane_value(gen_l, r), k = inv_t * kLog2e;
-          const int l = lane_value(label, r) - base;
-          const int at = l >= 0 && l < kIds && lane == l / kPer % kWave ? l / (kWave * kPer) * kPer + l % kPer : -1;
-#pragma unroll
-          for (int i = 0; i < kLaneIds; ++i) {
-            const float t = fmaf(y[i] - lse, k, -rest), p = __builtin_amdgcn_exp2f(t);
-            // a probability of 0 takes nothing from the entropy
-            up[i] = p * (p > 0.f ? fmaf(-g_en, fmaf(t, kLn2, H), -g_lp) : -g_lp) + (i == at ? g_lp : 0.f);
+            for (int j = 0; j < kPer; ++j)
+              if (base + id0 + j < vocab) Unaligned<T>::set(into[u], j, from + id0 + j);
+            continue;
           }
         }
+        into[u] = Unaligned<T>::load(from + id0);
+      }
+    };
+    read(x, raw);
+    if constexpr (MODE == kApplyGrad) read(other + row * ld_other + base, raw_g);
+    if (MASK) keep_next = r + 1 < rows ? mask_of(r + 1) : 0;
+    const bool masked = (MASK || !whole) && __any(keep != ~0u);
+    const bool repeats = ADJ && rep != 1.f;
+
+    // vector u under the controls, before the temperature; banned: what stands for -inf.  slope: dy / dz of every element.
+    auto controlled = [&](int u, float banned, float (&y)[kPer], float (&slope)[kPer]) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) { y[j] = Unaligned<T>::get(raw[u], j); slope[j] = 1.f; }
+      if (ADJ && (touched >> u & 1)) {
+        float sub[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) sub[j] = __uint_as_float(adj[slot<kPer>((u * kWave + lane) * kPer + j)]);
+        if (repeats) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) slope[j] = pick(bit_mask(seen, u * kPer + j), y[j] > 0.f ? inv_rep : rep, 1.f);
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) y[j] = fmaf(y[j], slope[j], -sub[j]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) y[j] = pick(bit_mask(keep, u * kPer + j), y[j], banned);
+      }
+    };
+
+    if constexpr (MODE == kStats) {
+      float4* const part = io.parts + row * chunks + chunk;
+      if (masked && !__any(keep != 0)) {
+        if (lane == 0) *part = make_float4(kNoLogit, 0.f, 0.f, 0.f);
+        if (has_label && lane == label_lane) io.label_y[row] = -INFINITY;
+        continue;
+      }
+      // y against a reference c in log2 units, c = M k rounded: one instruction per element, and what c is off by is the
+      // same for all of them and taken back at the end
+      float y[kLaneIds], m = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        float v[kPer], slope[kPer];
+        controlled(u, kBanned, v, slope);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) { y[u * kPer + j] = v[j]; m = fmaxf(m, v[j]); }
+      }
+      m = wave_max(m);
+      float M = m, cc = m * k;
+      bool plain = fabsf(cc) < kFar && m > kBanned;
+      float s4[4] = {}, e4[4] = {};
+      if (plain) {
 #pragma unroll
         for (int i = 0; i < kLaneIds; ++i) {
-          float slope = inv_t;
-          if (ADJ && (touched >> (i / kPer) & 1) && (seen >> i & 1)) slope *= z[i] > 0.f ? inv_rep : rep;
-          d[i] = y[i] == -INFINITY ? 0.f : up[i] * slope;
+          const float d = fmaf(y[i], k, -cc), f = __builtin_amdgcn_exp2f(d);
+          s4[i & 3] += f;
+          e4[i & 3] = fmaf(f, d, e4[i & 3]);
+        }
+        plain = !__any(e4[0] + e4[1] + e4[2] + e4[3] != e4[0] + e4[1] + e4[2] + e4[3]);
+      }
+      if (!plain) {  // logits far from 0, or infinite, or not numbers: by differences, what is banned at -inf
+        cc = 0.f;
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) {
+          if (masked) y[i] = pick(bit_mask(keep, i), y[i], -INFINITY);
+          m = fmaxf(m, y[i]);
+        }
+        m = wave_max(m);
+        M = m > -INFINITY ? m : kNoLogit;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s4[i] = e4[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) {
+          const float d = (y[i] - M) * k, f = __builtin_amdgcn_exp2f(d);
+          s4[i & 3] += f;
+          e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
         }
       }
+      float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
+      if (plain) {  // 2^(y k - c) = 2^((y - M) k + off)
+        const float off = fmaf(M, k, -cc), back = __builtin_amdgcn_exp2f(-off);
+        e = fmaf(-off, s, e) * back;
+        s *= back;
+      }
+      if (lane == 0) *part = make_float4(M, s, e, 0.f);
+      if (has_label) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < kLaneIds; ++i) v = i == label_at ? y[i] : v;
+        if (lane == label_lane) io.label_y[row] = keep >> label_at & 1 ? v : -INFINITY;
+      }
+    } else {
       T* const o = out + row * ld_out + base;
+      const float top = lane_value(top_l, r), A = lane_value(a_l, r), B = lane_value(b_l, r), g_lp = lane_value(glp_l, r);
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) {
         const int id0 = (u * kWave + lane) * kPer;
+        float y[kPer], slope[kPer], d[kPer];
+        controlled(u, -INFINITY, y, slope);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (MODE == kApply) {
+            d[j] = y[j] * inv_t;
+          } else if (MODE == kApplyGrad) {
+            d[j] = y[j] == -INFINITY ? 0.f : Unaligned<T>::get(raw_g[MODE == kApplyGrad ? u : 0], j) * (slope[j] * inv_t);
+          } else {
+            // a probability of 0 takes nothing from the entropy
+            const float t = (y[j] - top) * k;
+            d[j] = __builtin_amdgcn_exp2f(t) * fmaf(B, fmaxf(t, kTiny), A);
+          }
+        }
+        if (MODE == kGrad && has_label && label_at / kPer == u) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (lane == label_lane && label_at % kPer == j && y[j] != -INFINITY) d[j] += g_lp;
+        }
+        if (MODE == kGrad && ADJ && (touched >> u & 1) && repeats) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) d[j] *= slope[j];
+        }
         if (whole || base + id0 + kPer <= vocab) {
-          Unaligned<T>::store(o + id0, d + u * kPer);
+          Unaligned<T>::store(o + id0, d);
         } else {
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
-            if (base + id0 + j < vocab) Row<T>::store_one(o + id0 + j, d[u * kPer + j]);
+            if (base + id0 + j < vocab) Row<T>::store_one(o + id0 + j, d[j]);
         }
       }
     }
   }
 }
 
-// A row's chunks together, by a wavefront, in 64 bits: log-probability of the label, entropy, and what the backward reads.
-// In units of y (before the temperature T): lse = T ln sum exp(y / T) rounded to 32 bits, and in log2 units what that rounding has
-// left, so that log2 p = (y - lse) log2(e) / T - rest.
+// A row's chunks together, by a wavefront, in 64 bits: log-probability of the label, entropy, and what the backward reads: the
+// largest y (before the temperature), the sum of 2^((y - M) log2(e) / T), the entropy.  A row that nothing is left of has
+// M = 0, of which its -inf are far enough.
 __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int vocab, int chunks, axon_controls c, RowIo io,
                                                                  float* logprob, float* entropy, float* stats) {
   const int row = (int)(blockIdx.x * kWaves + threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
@@ -372,22 +463,22 @@ __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int
   s = wave_sum_d(s);
   e = wave_sum_d(e);
   if (lane != 0) return;
-  float lse = 0.f, rest = 0.f, H = 0.f, lp = 0.f;
+  float sum = 1.f, H = 0.f, lp = 0.f;
   const int64_t l = index_at(io.labels, io.labels_i64, row);
   const bool inside = l >= 0 && l < vocab;
   if (s == 0.0) {  // nothing is left
     lp = inside ? -INFINITY : 0.f;
+    M = 0.f;
   } else {
-    const double log2_s = log2(s);
-    lse = (float)((double)M + log2_s / (double)k);
-    rest = (float)(((double)M - (double)lse) * (double)k + log2_s);
-    H = (float)((log2_s - e / s) * 0.6931471805599453);
-    if (inside) lp = (float)((((double)io.label_y[row] - (double)lse) * (double)k - (double)rest) * 0.6931471805599453);
+    const double ls = log2(s);
+    sum = (float)s;
+    H = (float)((ls - e / s) * 0.6931471805599453);
+    if (inside) lp = (float)((((double)io.label_y[row] - (double)M) * (double)k - ls) * 0.6931471805599453);
   }
   logprob[row] = lp;
   if (entropy != nullptr) entropy[row] = H;
-  stats[row] = lse;
-  stats[(int64_t)n_rows + row] = rest;
+  stats[row] = M;
+  stats[(int64_t)n_rows + row] = sum;
   stats[2 * (int64_t)n_rows + row] = H;
 }
 
