@@ -6,18 +6,18 @@
 //   y_j = (z_j > 0 ? z_j / rep : z_j rep  where j is in the row's history)  - freq count_j - pres [count_j > 0] + bias_j,
 //   -inf where the row's mask has a 0 bit;  out = y / T;  log p = out - logsumexp(out).
 //
-// A wavefront owns 2048 consecutive ids of the vocabulary and walks a run of rows: the ids stay the same from row to row,
+// A wavefront owns 4 KB of consecutive ids of the vocabulary and walks a run of rows: the ids stay the same from row to row,
 // so what the histories do to them is kept where it is used (the sum of the additive terms in LDS, whether an id was
 // seen in a bit of the owning lane), and a row of a packed batch differs from the row before by ONE token.  Vectors are
 // loaded at whatever boundary a row of an odd vocabulary starts on, so that lanes keep their ids.
 #include "logits_rows.h"
+#include <type_traits>
 
 namespace axon {
 
-constexpr int kIds = 2048;               // ids of a wavefront
-constexpr int kLaneIds = kIds / kWave;   // 32, one bit each
+constexpr int kVecs = 4;                  // 16-byte vectors of a lane: a wavefront's chunk of a row is 4 KB
+constexpr int kChunkBytes = kVecs * kWave * 16;
 constexpr int kWaves = kBlock / kWave;
-constexpr int kGroupIds = kIds * kWaves;  // ids of a workgroup
 constexpr int kMaxRun = kWave;            // rows of a run: a lane holds what belongs to a row
 
 enum Mode { kStats, kGrad, kApply, kApplyGrad };
@@ -27,29 +27,35 @@ template <typename T> struct Unaligned;
 template <> struct Unaligned<float> {
   static constexpr int kPer = 4;
   typedef f32x4 Raw;
-  struct __attribute__((packed, aligned(4))) Box { Raw v; };
-  __device__ static Raw load(const float* p) { return reinterpret_cast<const Box*>(p)->v; }
+  typedef Raw Loose __attribute__((aligned(4)));
+  template <bool CACHED>
+  __device__ static Raw load(const float* p) {
+    const Loose* const q = reinterpret_cast<const Loose*>(p);
+    return CACHED ? *q : __builtin_nontemporal_load(q);
+  }
   __device__ static float get(const Raw& r, int j) { return r[j]; }
   __device__ static void set(Raw& r, int j, const float* p) { r[j] = *p; }
   __device__ static void store(float* p, const float* v) {
-    Box b;
-    b.v = Raw{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<Box*>(p) = b;
+    const Raw x = {v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(x, reinterpret_cast<Loose*>(p));
   }
 };
 template <> struct Unaligned<unsigned short> {
   static constexpr int kPer = 8;
   typedef uint32_t Raw __attribute__((ext_vector_type(4)));
-  struct __attribute__((packed, aligned(2))) Box { Raw v; };
-  __device__ static Raw load(const unsigned short* p) { return reinterpret_cast<const Box*>(p)->v; }
+  typedef Raw Loose __attribute__((aligned(2)));
+  template <bool CACHED>
+  __device__ static Raw load(const unsigned short* p) {
+    const Loose* const q = reinterpret_cast<const Loose*>(p);
+    return CACHED ? *q : __builtin_nontemporal_load(q);
+  }
   __device__ static float get(const Raw& r, int j) {
     return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16));
   }
   __device__ static void set(Raw& r, int j, const unsigned short* p) { r[j >> 1] |= (uint32_t)*p << ((j & 1) * 16); }  // of a 0
   __device__ static void store(unsigned short* p, const float* v) {
-    Box b;
-    b.v = Raw{f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
-    *reinterpret_cast<Box*>(p) = b;
+    const Raw x = {f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
+    __builtin_nontemporal_store(x, reinterpret_cast<Loose*>(p));
   }
 };
 
@@ -91,6 +97,7 @@ struct RowIo {
   float4* parts;              // [rows][chunks] (M, s, e), kStats
   const float* stats;         // [3][rows]: what controls_finish_kernel has left, kGrad
   const float *g_logprob, *g_entropy;
+  int cached_from;  // rows from here on are left in the cache in front of the memory, for a backward that follows
 };
 
 // The additive terms of a wavefront's ids in LDS, in the order in which the lanes read them: 16 bytes of neighbouring
@@ -107,15 +114,18 @@ __device__ __forceinline__ float pick(uint32_t mask, float yes, float no) {
 }
 
 template <typename T, Mode MODE, bool ADJ, bool MASK>
-__global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
+__global__ __launch_bounds__(kBlock, 4) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
                                                           axon_controls c, RowIo io, const T* other, int64_t ld_other, T* out,
                                                           int64_t ld_out) {
-  constexpr int kPer = Unaligned<T>::kPer, kVecs = kLaneIds / kPer;
-  constexpr uint32_t kVecBits = (1u << kPer) - 1;
+  constexpr int kPer = Unaligned<T>::kPer, kLaneIds = kVecs * kPer, kIds = kLaneIds * kWave, kGroupIds = kIds * kWaves;
+  constexpr uint32_t kVecBits = (1u << kPer) - 1, kAll = kLaneIds == 32 ? ~0u : (1u << (kLaneIds & 31)) - 1;
   __shared__ __align__(16) uint32_t s_adj[ADJ ? kGroupIds : 4];  // counts (bit 31: seen) while they are collected, then floats
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);  // bases in scalar registers
   const int groups = (chunks + kWaves - 1) / kWaves;
-  const int first = (int)(blockIdx.x / groups) * run, group = (int)(blockIdx.x % groups);
+  // kGrad from the last row to the first: the end of what the forward read last is still in the cache in front of the memory
+  const unsigned block = MODE == kGrad ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const int first = (int)(block / groups) * run, group = (int)(block % groups);
+  const bool cached = MODE == kStats && first >= io.cached_from;
   const int rows = min(run, n_rows - first);
   const int chunk = group * kWaves + wave, base = chunk * kIds;
 
@@ -170,11 +180,19 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
 
   uint32_t* const adj = s_adj + (ADJ ? wave * kIds : 0);
   uint32_t seen = 0;     // bit u * kPer + j: this lane's id of vector u, element j
-  uint32_t touched = 0;  // bit u: some lane's vector u is not left as it is
+  uint32_t touched = 0;  // bit i / 4: some lane's ids of these four bits are not left as they are; the same in all lanes
+  // A row's own token is counted with the run's first rows, for all rows at once: by a sum of additions as the rows go by, the
+  // term would drift.  count: how often the row's token is among the own tokens up to the row; bias: of that id.
+  const int mine_off = token < 0 ? -1 : (token & (kOwn - 1)) - base;
+  const bool in_chunk = ADJ && mine_off >= 0 && mine_off < kIds;
+  int count_l = 0;
+  float bias_l = 0.f;
   // counts and seen bits in LDS to additive terms, biases with them
   auto settle = [&](int row) {
     const float f = lane_value(freq_l, row), a = lane_value(pres_l, row);
     const int sq = lane_value(seq, row);
+    const bool of_it = in_chunk && start == lane_value(start, row);
+    const int before = of_it ? (int)(adj[slot<kPer>(mine_off)] & 0x7fffffffu) : 0;
     uint32_t any = 0;
     seen = 0;
 #pragma unroll
@@ -186,7 +204,9 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
         some |= w[j];
       }
       if (!__any(some != 0)) continue;  // 0 is 0.f
-      any |= 1u << u;
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4)
+        if (__any((w[j] | w[j + 1] | w[j + 2] | w[j + 3]) != 0)) any |= 1u << ((u * kPer + j) / 4);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         seen |= (w[j] >> 31) << (u * kPer + j);
@@ -199,60 +219,159 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
       const int64_t off = i < c.n_bias ? index_at(c.bias_ids, c.bias_ids_i64, at) - base : -1;
       const bool in = off >= 0 && off < kIds && off + base < vocab;
       if (in) atomicAdd(reinterpret_cast<float*>(adj) + slot<kPer>((int)off), -c.bias[at]);
-      const int u = in ? (int)off / (kWave * kPer) : -1;
+      const int quad = in ? ((int)off / (kWave * kPer) * kPer + (int)off % kPer) / 4 : -1;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v)
-        if (__any(u == v)) any |= 1u << v;
+      for (int v = 0; v < kLaneIds / 4; ++v)
+        if (__any(quad == v)) any |= 1u << v;
     }
-    touched = any;
+    touched = __builtin_amdgcn_readfirstlane(any);
     wave_sync();
+    if (of_it) {
+      count_l += before;
+      if (c.n_bias > 0) bias_l = penalty(before, f, a) - __uint_as_float(adj[slot<kPer>(mine_off)]);
+    }
   };
-
-  if (ADJ) {  // the history before the run's first row, by the whole workgroup (of the row itself, where a row is a sequence)
-    for (int i = tid; i < kGroupIds; i += kBlock) s_adj[i] = 0;
-    __syncthreads();
-    const int from = lane_value(start, 0);
-    const int64_t upto = c.every_position ? first : lane_value((int)end, 0);  // offsets are 32-bit integers
-    if (c.token_ids != nullptr)
-      for (int64_t i = from + tid; i < upto; i += kBlock) {
-        const int t = history_token(c, i, vocab);
-        const int off = t < 0 ? -1 : (t & (kOwn - 1)) - group * kGroupIds;
-        if (off >= 0 && off < kGroupIds) {
-          uint32_t* const w = s_adj + (off & ~(kIds - 1)) + slot<kPer>(off & (kIds - 1));
-          atomicOr(w, 0x80000000u);
-          if (t & kOwn) atomicAdd(w, 1u);
-        }
-      }
-    __syncthreads();
-  }
-  if (chunk >= chunks) return;
 
   // the ids of this lane that there are
   const bool whole = base + kIds <= vocab;
-  uint32_t there = ~0u;
+  uint32_t there = kAll;
   if (!whole) {
     there = 0;
 #pragma unroll
     for (int i = 0; i < kLaneIds; ++i) there |= (uint32_t)(base + ((i / kPer) * kWave + lane) * kPer + i % kPer < vocab) << i;
   }
-  auto mask_of = [&](int r) {  // what of them row r may keep
+  // What of them row r may keep, in two halves: the bytes are asked for a row before they are put together.
+  uint32_t bytes[MASK ? kVecs : 1];
+  auto ask_mask = [&](int r) {
     const int st = lane_value(state, r);
-    if (st < 0) return there;
-    const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(c.allowed + (int64_t)st * c.allowed_stride) + base / 8;
-    uint32_t m = 0;
+    const uint8_t* const from = reinterpret_cast<const uint8_t*>(c.allowed + (int64_t)max(st, 0) * c.allowed_stride) + base / 8;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int id0 = (u * kWave + lane) * kPer;
-      if (whole || base + id0 < vocab) m |= (bytes[id0 >> 3] >> (id0 & 7) & kVecBits) << (u * kPer);
+      bytes[MASK ? u : 0] = whole || base + id0 < vocab ? from[(uint32_t)id0 >> 3] : 0;
     }
-    return m & there;
+  };
+  auto mask_of = [&](int r) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) m |= (bytes[MASK ? u : 0] >> (kPer == 4 ? (lane & 1) * 4 : 0) & kVecBits) << (u * kPer);
+    return lane_value(state, r) < 0 ? there : m & there;
   };
 
-  uint32_t keep_next = MASK ? mask_of(0) : there;
+  // A row's vectors are asked for while the row before is worked on, as soon as the registers are free; its mask a row
+  // earlier, since what is not kept is not read either.  Where a mask leaves no lane more than kFew ids (a grammar's
+  // state that allows a handful of tokens), only these are looked at.
+  constexpr int kFew = 4;
+  static_assert(kFew <= kVecs, "");
+  typename Unaligned<T>::Raw raw[kVecs], raw_g[MODE == kApplyGrad ? kVecs : 1];
+  auto is_few = [&](uint32_t keep) {
+    if (MODE != kStats || !MASK) return false;
+    uint32_t x = keep;
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) x &= x - 1;
+    return !__any(x != 0);
+  };
+  auto read = [&](const T* from, uint32_t keep, int u, typename Unaligned<T>::Raw& into) {
+    const int id0 = (u * kWave + lane) * kPer;
+    if (MASK || !whole) {
+      into = typename Unaligned<T>::Raw{};
+      if ((keep >> (u * kPer) & kVecBits) == 0) return;
+      if (!whole && base + id0 + kPer > vocab) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (base + id0 + j < vocab) Unaligned<T>::set(into, j, from + id0 + j);
+        return;
+      }
+    }
+    into = cached ? Unaligned<T>::template load<true>(from + (uint32_t)id0) : Unaligned<T>::template load<false>(from + (uint32_t)id0);
+  };
+  const T* const from = logits + (int64_t)first * ld + base;
+  const T* const from_g = MODE == kApplyGrad ? other + (int64_t)first * ld_other + base : nullptr;
+  auto read_row = [&](int r, uint32_t keep, bool few) {
+    if (few) {
+      uint32_t x = keep;
+#pragma unroll
+      for (int i = 0; i < kFew; ++i, x &= x - 1) {
+        raw[i] = typename Unaligned<T>::Raw{};
+        const int bit = __builtin_ctz(x | 0x80000000u);
+        if (x != 0) Unaligned<T>::set(raw[i], 0, from + r * ld + (uint32_t)((bit / kPer * kWave + lane) * kPer + bit % kPer));
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      read(from + r * ld, keep, u, raw[u]);
+      if constexpr (MODE == kApplyGrad) read(from_g + r * ld_other, keep, u, raw_g[u]);
+    }
+  };
+
+  const bool works = chunk < chunks;
+  uint32_t keep_next = there;
+  bool few_next = false;
+  if (works) {  // on their way while the history is counted
+    if (MASK) ask_mask(0);
+    else read_row(0, keep_next, false);
+  }
+  if (ADJ) {  // the history before the run's first row, by the whole workgroup (of the row itself, where a row is a sequence)
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < kGroupIds / 4; i += kBlock) reinterpret_cast<uint4*>(s_adj)[i] = none;
+    __syncthreads();
+    const int from = lane_value(start, 0);
+    const int upto = c.every_position ? first : lane_value((int)end, 0);  // offsets are 32-bit integers
+    if (c.token_ids != nullptr) {
+      const auto count = [&](auto id_of, auto own_of) {
+        constexpr int kBatch = 8;  // loads in flight per thread
+        for (int i0 = from + tid; i0 < upto; i0 += kBlock * kBatch) {
+          int off[kBatch];
+          bool own[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * kBlock, at = min(i, upto - 1);
+            const int64_t id = id_of(at);
+            own[b] = own_of(at);
+            off[b] = i < upto && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b)
+            if (off[b] >= 0 && off[b] < kGroupIds) {
+              uint32_t* const w = s_adj + (off[b] & ~(kIds - 1)) + slot<kPer>(off[b] & (kIds - 1));
+              atomicOr(w, 0x80000000u);
+              if (own[b]) atomicAdd(w, 1u);
+            }
+        }
+      };
+      const auto with_ids = [&](auto id_of) {
+        const void* const m = c.own_mask;
+        if (m == nullptr) count(id_of, [](int) { return true; });
+        else if (c.mask_kind == AXON_MASK_I64) count(id_of, [m](int i) { return static_cast<const int64_t*>(m)[i] != 0; });
+        else count(id_of, [m](int i) { return static_cast<const float*>(m)[i] != 0.f; });
+      };
+      const void* const ids = c.token_ids;
+      if (c.token_ids_i64) with_ids([ids](int i) { return static_cast<const int64_t*>(ids)[i]; });
+      else with_ids([ids](int i) { return (int64_t)static_cast<const int32_t*>(ids)[i]; });
+    }
+    __syncthreads();
+  }
+  if (!works) return;
+  if (ADJ && c.every_position && __any(in_chunk))
+    for (int r = 0; r < rows; ++r)
+      count_l += lane >= r && token == lane_value(token, r) && start == lane_value(start, r);
+  if (MASK) {
+    keep_next = mask_of(0);
+    if (rows > 1) ask_mask(1);
+    few_next = is_few(keep_next);
+    read_row(0, keep_next, few_next);
+  }
+  float ref = kNoLogit;
   for (int r = 0; r < rows; ++r) {
     const int64_t row = first + r;
     const float inv_t = lane_value(inv_t_l, r), k = inv_t * kLog2e, rep = lane_value(rep_l, r), inv_rep = 1.f / rep;
     uint32_t keep = keep_next;
+    const bool few = few_next;
+    if (MASK) {
+      keep_next = r + 1 < rows ? mask_of(r + 1) : 0;
+      if (r + 2 < rows) ask_mask(r + 2);
+    }
     // masks of single bits are made where they are used: 32 of them held over the rows are 32 registers
     asm volatile("" : "+v"(keep), "+v"(seen));
     if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
@@ -266,67 +385,40 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
     if (ADJ && c.every_position) {
       const int t = lane_value(token, r);
       const int id = t & (kOwn - 1), off = id - base;
-      if (t >= 0 && off >= 0 && off < kIds) {  // the row's own token, counted anew: a sum of additions would drift
+      if (t >= 0 && off >= 0 && off < kIds) {  // the row's own token
         const int u = off / (kWave * kPer), at = off / kPer % kWave, j = off % kPer;
         if (lane == at) seen |= 1u << (u * kPer + j);
-        touched |= 1u << u;
+        touched |= 1u << ((u * kPer + j) / 4);
         if (t & kOwn) {
-          int count = 0;
-          for (int64_t i = lane_value(start, r) + lane; i <= row; i += kWave) count += history_token(c, i, vocab) == t;
-          count = (int)wave_sum((float)count);
-          float b = 0.f;
-          const int64_t at_bias = c.bias_per_seq ? (int64_t)lane_value(seq, r) * c.n_bias : 0;
-          for (int64_t i = 0; i < c.n_bias; ++i)
-            if (index_at(c.bias_ids, c.bias_ids_i64, at_bias + i) == id) b += c.bias[at_bias + i];
-          if (lane == at) adj[slot<kPer>(off)] = __float_as_uint(penalty(count, lane_value(freq_l, r), lane_value(pres_l, r)) - b);
+          const float p = penalty(lane_value(count_l, r), lane_value(freq_l, r), lane_value(pres_l, r)) - lane_value(bias_l, r);
+          if (lane == at) adj[slot<kPer>(off)] = __float_as_uint(p);
           wave_sync();
         }
       }
     }
-    const T* const x = logits + row * ld + base;
     const int l = MODE == kStats || MODE == kGrad ? lane_value(label, r) - base : -1;
     const bool has_label = l >= 0 && l < kIds;
     const int label_lane = l / kPer % kWave, label_at = l / (kWave * kPer) * kPer + l % kPer;
-
-    // what is not kept is not read either
-    typename Unaligned<T>::Raw raw[kVecs], raw_g[MODE == kApplyGrad ? kVecs : 1];
-    auto read = [&](const T* from, typename Unaligned<T>::Raw(&into)[kVecs]) {
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u) {
-        const int id0 = (u * kWave + lane) * kPer;
-        into[u] = typename Unaligned<T>::Raw{};
-        if (MASK || !whole) {
-          if ((keep >> (u * kPer) & kVecBits) == 0) continue;
-          if (!whole && base + id0 + kPer > vocab) {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-              if (base + id0 + j < vocab) Unaligned<T>::set(into[u], j, from + id0 + j);
-            continue;
-          }
-        }
-        into[u] = Unaligned<T>::load(from + id0);
-      }
-    };
-    read(x, raw);
-    if constexpr (MODE == kApplyGrad) read(other + row * ld_other + base, raw_g);
-    if (MASK) keep_next = r + 1 < rows ? mask_of(r + 1) : 0;
-    const bool masked = (MASK || !whole) && __any(keep != ~0u);
+    const bool masked = (MASK || !whole) && __any(keep != kAll);
     const bool repeats = ADJ && rep != 1.f;
+    const bool more = r + 1 < rows;
 
     // vector u under the controls, before the temperature; banned: what stands for -inf.  slope: dy / dz of every element.
     auto controlled = [&](int u, float banned, float (&y)[kPer], float (&slope)[kPer]) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) { y[j] = Unaligned<T>::get(raw[u], j); slope[j] = 1.f; }
-      if (ADJ && (touched >> u & 1)) {
-        float sub[kPer];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) sub[j] = __uint_as_float(adj[slot<kPer>((u * kWave + lane) * kPer + j)]);
+      for (int q = 0; q < kPer; q += 4) {
+        if (!ADJ || !(touched >> ((u * kPer + q) / 4) & 1)) continue;
+        float sub[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sub[j] = __uint_as_float(adj[slot<kPer>((u * kWave + lane) * kPer + q + j)]);
         if (repeats) {
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) slope[j] = pick(bit_mask(seen, u * kPer + j), y[j] > 0.f ? inv_rep : rep, 1.f);
+          for (int j = 0; j < 4; ++j) slope[q + j] = pick(bit_mask(seen, u * kPer + q + j), y[q + j] > 0.f ? inv_rep : rep, 1.f);
         }
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) y[j] = fmaf(y[j], slope[j], -sub[j]);
+        for (int j = 0; j < 4; ++j) y[q + j] = fmaf(y[q + j], slope[q + j], -sub[j]);
       }
       if (masked) {
 #pragma unroll
@@ -336,65 +428,94 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
 
     if constexpr (MODE == kStats) {
       float4* const part = io.parts + row * chunks + chunk;
-      if (masked && !__any(keep != 0)) {
-        if (lane == 0) *part = make_float4(kNoLogit, 0.f, 0.f, 0.f);
-        if (has_label && lane == label_lane) io.label_y[row] = -INFINITY;
+      // The sum of N logits of each lane, and weighted by their exponents, against the reference in use: the largest logit of an
+      // earlier row of this chunk will do as long as the sum stays in range.  Against c = ref k rounded it is one
+      // instruction per element, and what c is off by is the same for all of them and taken back at the end.
+      auto statistics = [&](auto n, auto& y, uint32_t bits) {
+        constexpr int N = decltype(n)::value;
+        auto largest = [&] {
+          float m = y[0];
+#pragma unroll
+          for (int i = 1; i < N; ++i) m = fmaxf(m, y[i]);
+          return wave_max(m);
+        };
+        if (!(ref > kBanned)) ref = largest();
+        const float cc = ref * k;
+        float s4[4] = {}, e4[4] = {}, s = 0.f, e = 0.f;
+        bool plain = fabsf(cc) < kFar && ref > kBanned;
+        if (plain) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float d = fmaf(y[i], k, -cc), f = __builtin_amdgcn_exp2f(d);
+            s4[i & 3] += f;
+            e4[i & 3] = fmaf(f, d, e4[i & 3]);
+          }
+          s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
+          e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
+          const float off = fmaf(ref, k, -cc), back = __builtin_amdgcn_exp2f(-off);  // 2^(y k - c) = 2^((y - ref) k + off)
+          e = fmaf(-off, s, e) * back;
+          s *= back;
+          plain = s > 0x1p-80f && s < 0x1p100f && e == e;
+        }
+        if (!plain) {  // another scale, logits far from 0, or infinite, or not numbers: by differences, what is banned at -inf
+          asm volatile("" : "+v"(bits));
+#pragma unroll
+          for (int i = 0; i < N; ++i) y[i] = pick(bit_mask(bits, i), y[i], -INFINITY);
+          ref = largest();
+          if (!(ref > -INFINITY)) ref = kNoLogit;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s4[i] = e4[i] = 0.f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float d = (y[i] - ref) * k, f = __builtin_amdgcn_exp2f(d);
+            s4[i & 3] += f;
+            e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
+          }
+          s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
+          e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
+        }
+        if (lane == 0) *part = make_float4(ref, s, e, 0.f);
+      };
+      if (MASK && few) {
+        float y[kFew];
+        uint32_t x = keep, there_are = 0;
+        float label_y = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kFew; ++i, x &= x - 1) {
+          const int bit = __builtin_ctz(x | 0x80000000u);
+          y[i] = Unaligned<T>::get(raw[i], 0);
+          if (ADJ && touched != 0) {
+            const float slope = repeats && (seen >> bit & 1) ? (y[i] > 0.f ? inv_rep : rep) : 1.f;
+            y[i] = fmaf(y[i], slope, -__uint_as_float(adj[slot<kPer>((bit / kPer * kWave + lane) * kPer + bit % kPer)]));
+          }
+          if (x != 0 && bit == label_at) label_y = y[i];
+          y[i] = x != 0 ? y[i] : kBanned;
+          there_are |= (uint32_t)(x != 0) << i;
+        }
+        few_next = is_few(keep_next);
+        if (more) read_row(r + 1, keep_next, few_next);
+        if (__any(keep != 0)) statistics(std::integral_constant<int, kFew>{}, y, there_are);
+        else if (lane == 0) *part = make_float4(kNoLogit, 0.f, 0.f, 0.f);
+        if (has_label && lane == label_lane) io.label_y[row] = label_y;
         continue;
       }
-      // y against a reference c in log2 units, c = M k rounded: one instruction per element, and what c is off by is the
-      // same for all of them and taken back at the end
-      float y[kLaneIds], m = -INFINITY;
+      float y[kLaneIds];
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) {
         float v[kPer], slope[kPer];
         controlled(u, kBanned, v, slope);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) { y[u * kPer + j] = v[j]; m = fmaxf(m, v[j]); }
+        for (int j = 0; j < kPer; ++j) y[u * kPer + j] = v[j];
       }
-      m = wave_max(m);
-      float M = m, cc = m * k;
-      bool plain = fabsf(cc) < kFar && m > kBanned;
-      float s4[4] = {}, e4[4] = {};
-      if (plain) {
-#pragma unroll
-        for (int i = 0; i < kLaneIds; ++i) {
-          const float d = fmaf(y[i], k, -cc), f = __builtin_amdgcn_exp2f(d);
-          s4[i & 3] += f;
-          e4[i & 3] = fmaf(f, d, e4[i & 3]);
-        }
-        plain = !__any(e4[0] + e4[1] + e4[2] + e4[3] != e4[0] + e4[1] + e4[2] + e4[3]);
-      }
-      if (!plain) {  // logits far from 0, or infinite, or not numbers: by differences, what is banned at -inf
-        cc = 0.f;
-        m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kLaneIds; ++i) {
-          if (masked) y[i] = pick(bit_mask(keep, i), y[i], -INFINITY);
-          m = fmaxf(m, y[i]);
-        }
-        m = wave_max(m);
-        M = m > -INFINITY ? m : kNoLogit;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s4[i] = e4[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kLaneIds; ++i) {
-          const float d = (y[i] - M) * k, f = __builtin_amdgcn_exp2f(d);
-          s4[i & 3] += f;
-          e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
-        }
-      }
-      float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
-      if (plain) {  // 2^(y k - c) = 2^((y - M) k + off)
-        const float off = fmaf(M, k, -cc), back = __builtin_amdgcn_exp2f(-off);
-        e = fmaf(-off, s, e) * back;
-        s *= back;
-      }
-      if (lane == 0) *part = make_float4(M, s, e, 0.f);
+      few_next = is_few(keep_next);
+      if (more) read_row(r + 1, keep_next, few_next);
+      statistics(std::integral_constant<int, kLaneIds>{}, y, keep);
       if (has_label) {
+        const int at = lane == label_lane ? label_at : -1;
         float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < kLaneIds; ++i) v = i == label_at ? y[i] : v;
-        if (lane == label_lane) io.label_y[row] = keep >> label_at & 1 ? v : -INFINITY;
+        for (int i = 0; i < kLaneIds; ++i) v = i == at ? y[i] : v;
+        if (at >= 0) io.label_y[row] = keep >> label_at & 1 ? v : -INFINITY;
       }
     } else {
       T* const o = out + row * ld_out + base;
@@ -416,17 +537,25 @@ __global__ __launch_bounds__(kBlock) void controls_kernel(const T* logits, int64
             d[j] = __builtin_amdgcn_exp2f(t) * fmaf(B, fmaxf(t, kTiny), A);
           }
         }
+        if (more) {
+          read(from + (r + 1) * ld, keep_next, u, raw[u]);
+          if constexpr (MODE == kApplyGrad) read(from_g + (r + 1) * ld_other, keep_next, u, raw_g[u]);
+        }
         if (MODE == kGrad && has_label && label_at / kPer == u) {
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
             if (lane == label_lane && label_at % kPer == j && y[j] != -INFINITY) d[j] += g_lp;
         }
-        if (MODE == kGrad && ADJ && (touched >> u & 1) && repeats) {
+        if (MODE == kGrad && ADJ && repeats) {
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) d[j] *= slope[j];
+          for (int q = 0; q < kPer; q += 4) {
+            if (!(touched >> ((u * kPer + q) / 4) & 1)) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[q + j] *= slope[q + j];
+          }
         }
         if (whole || base + id0 + kPer <= vocab) {
-          Unaligned<T>::store(o + id0, d);
+          Unaligned<T>::store(o + (uint32_t)id0, d);
         } else {
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
@@ -456,9 +585,12 @@ __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int
   double s = 0.0, e = 0.0;
   for (int i = lane; i < chunks; i += kWave) {
     const float4 p = io.parts[(int64_t)row * chunks + i];
-    const float d = fmaxf((p.x - M) * k, kTiny), f = __builtin_amdgcn_exp2f(d);
-    s += (double)p.y * f;
-    e += (double)(f * fmaf(p.y, d, p.z));
+    // the references are no maxima: a sum may be anything from 2^-80 to 2^100
+    const double d = ((double)p.x - (double)M) * (double)k, f = exp2(d);
+    if (f > 0.0 || p.y != p.y) {
+      s += (double)p.y * f;
+      e += f * ((double)p.y * d + (double)p.z);
+    }
   }
   s = wave_sum_d(s);
   e = wave_sum_d(e);
@@ -487,6 +619,8 @@ __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int
 using namespace axon;
 
 namespace {
+
+constexpr int64_t kCacheBytes = int64_t(256) << 20;
 
 int elem_bytes(int dtype) { return dtype == AXON_LOGITS_F32 ? 4 : 2; }
 
@@ -529,12 +663,12 @@ int check_controls(const axon_controls* c, int64_t n, int64_t v) {
   return AXON_OK;
 }
 
-int chunks_of(int64_t vocab) { return (int)((vocab + kIds - 1) / kIds); }
+int chunks_of(int64_t vocab, int dtype) { return (int)((vocab * elem_bytes(dtype) + kChunkBytes - 1) / kChunkBytes); }
 
-// Rows of a run: about eight rounds of the 4096 wavefronts that the part holds.
-int run_of(int64_t n, int64_t vocab) {
-  const int64_t r = n * chunks_of(vocab) / (8 * 4096);
-  return (int)(r < 1 ? 1 : (r < kMaxRun ? r : kMaxRun));
+// Rows of a run: about four rounds of the 4096 wavefronts that the part holds.
+int run_of(int64_t n, int chunks) {
+  const int64_t r = n * chunks / (4 * 4096);
+  return (int)(r < 1 ? 1 : (r < kMaxRun / 2 ? r : kMaxRun / 2));
 }
 
 template <Mode MODE>
@@ -544,8 +678,8 @@ int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, 
   const bool penalties = c.repetition || c.frequency || c.presence || c.repetition_all != 1.f || c.frequency_all != 0.f || c.presence_all != 0.f;
   if (!penalties) c.token_ids = nullptr;  // nobody asks for the history
   const bool adj = (penalties && c.token_ids) || c.n_bias > 0, mask = c.allowed != nullptr;
-  const int chunks = chunks_of(vocab), groups = (chunks + kWaves - 1) / kWaves;
-  const int run = adj && !c.every_position ? 1 : run_of(n, vocab);
+  const int chunks = chunks_of(vocab, dtype), groups = (chunks + kWaves - 1) / kWaves;
+  const int run = adj && !c.every_position ? 1 : run_of(n, chunks);
   const int64_t grid = (n + run - 1) / run * groups;
   if (grid >= INT32_MAX) return AXON_ERR_SHAPE;
 #define AXON_CONTROLS(T, A, M)                                                                                             \
@@ -590,24 +724,27 @@ extern "C" int axon_controls_apply_bwd(const void* logits, int dtype, int64_t ld
 
 extern "C" int64_t axon_controls_logprob_workspace_bytes(int64_t n, int64_t vocab) {
   if (n < 0 || vocab <= 0 || vocab >= kOwn) return AXON_ERR_ARG;
-  return n * (chunks_of(vocab) * (int64_t)sizeof(float4) + (int64_t)sizeof(float));
+  return n * (chunks_of(vocab, AXON_LOGITS_F32) * (int64_t)sizeof(float4) + (int64_t)sizeof(float));
 }
 
 extern "C" int axon_controls_logprob_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab,
                                          const axon_controls* controls, const void* labels, int labels_i64, float* logprob,
-                                         float* entropy, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+                                         float* entropy, float* stats, void* workspace, int64_t workspace_bytes, int bwd_follows,
+                                         void* stream) {
   int rc = check_rows(logits, dtype, ld, n, vocab);
   if (rc == AXON_OK) rc = check_controls(controls, n, vocab);
   if (rc != AXON_OK || n == 0) return rc;
   if (!labels || !logprob || !stats) return AXON_ERR_ARG;
   if (!workspace || workspace_bytes < axon_controls_logprob_workspace_bytes(n, vocab) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return AXON_ERR_WORKSPACE;
-  const int chunks = chunks_of(vocab);
+  const int chunks = chunks_of(vocab, dtype);
   RowIo io{};
   io.labels = labels;
   io.labels_i64 = labels_i64;
   io.parts = static_cast<float4*>(workspace);
   io.label_y = reinterpret_cast<float*>(io.parts + n * chunks);
+  const int64_t cached = bwd_follows ? kCacheBytes / (vocab * elem_bytes(dtype)) : 0;
+  io.cached_from = (int)(cached < n ? n - cached : 0);
   const hipStream_t st = (hipStream_t)stream;
   rc = launch<kStats>(logits, dtype, ld, n, vocab, *controls, io, nullptr, 0, nullptr, 0, st);
   if (rc != AXON_OK) return rc;

@@ -1070,7 +1070,7 @@ std::tuple<Tensor, Tensor> controlled_logprobs(const Tensor& logits, const Tenso
     const int64_t need = axon_controls_logprob_workspace_bytes(n, v);
     const Tensor ws = at::empty({std::max<int64_t>(need, 0)}, opts(rows, at::kByte));
     check(axon_controls_logprob_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, &c, lab.data_ptr(), is_i64(lab), lp.data_ptr<float>(),
-                                    entropy.data_ptr<float>(), stats.data_ptr<float>(), ws.data_ptr(), need, stream()),
+                                    entropy.data_ptr<float>(), stats.data_ptr<float>(), ws.data_ptr(), need, wants_grad, stream()),
           "axon_controls_logprob_fwd");
   }
   if (wants_grad) {

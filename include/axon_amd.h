@@ -769,11 +769,12 @@ int axon_controls_apply_bwd(const void* logits, int dtype, int64_t ld, int64_t n
                             const void* g_out, int64_t ld_g, void* dlogits, int64_t ld_d, void* stream);
 /* log softmax(out)[label] (0 for a label outside the vocabulary) and the entropy (may be NULL) of softmax(out), fp32; a row
  * that nothing is left of: -inf, 0 and no gradient.  stats [3][n]: what the backward reads.  Workspace 16-byte aligned.
+ * bwd_follows: whether the last rows are left in the cache for a backward (the results are the same).
  * dlogits may be the logits' own storage; g_logprob, g_entropy may be NULL. */
 int64_t axon_controls_logprob_workspace_bytes(int64_t n, int64_t vocab);
 int axon_controls_logprob_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
                               const void* labels, int labels_are_i64, float* logprob, float* entropy, float* stats, void* workspace,
-                              int64_t workspace_bytes, void* stream);
+                              int64_t workspace_bytes, int bwd_follows, void* stream);
 int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
                               const void* labels, int labels_are_i64, const float* stats, const float* g_logprob,
                               const float* g_entropy, void* dlogits, int64_t ld_d, void* stream);

@@ -107,7 +107,7 @@ def test_the_c_entry_points_check_their_arguments():
     assert ws > 0 and lib.axon_controls_logprob_workspace_bytes(-1, 100) < 0
 
     def fwd(labels=p, lp=p, stats=p, w=p, wb=ws):
-        return lib.axon_controls_logprob_fwd(p, 0, 100, 2, 100, ctypes.byref(s), labels, 1, lp, p, stats, w, wb, None)
+        return lib.axon_controls_logprob_fwd(p, 0, 100, 2, 100, ctypes.byref(s), labels, 1, lp, p, stats, w, wb, 0, None)
 
     assert fwd(labels=None) == fwd(lp=None) == fwd(stats=None) == -1
     assert fwd(w=None) == fwd(wb=ws - 1) == fwd(w=p + 8) == -3
