@@ -383,6 +383,351 @@ __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, i
     if (where[u] >= 0) Row<T>::store_one(out + where[u], again[u]);
 }
 
+// The loss and its gradient from ONE read of a row: a workgroup holds the row, NREG 16-byte vectors of every thread in registers and
+// NLDS in LDS, from its statistics to its gradient (what is longer is read again).  The given tokens are found by a byte per vector
+// in LDS that says which of its elements are given, and by a hash of the vector's number for the few vectors that have one; their
+// gradients are put in before the vector is stored.
+constexpr int kBuckets = 256;
+template <int THREADS, int NLDS, int VECS>
+struct RowLds {
+  uint4 tiles[NLDS > 0 ? NLDS * THREADS : 1];
+  uint32_t given[(VECS + 3) / 4];
+  int id[kMaxIds], heads[kBuckets];  // chains of the ids that come for the first time
+  int16_t next[kMaxIds];
+  float g[kMaxIds], total[kMaxIds];                 // G, and summed over equal ids
+  float red_m[THREADS / kWave], red_s[THREADS / kWave];
+  uint32_t single;
+  float lse, c_out, c_in;
+  int is_far;
+};
+
+template <typename T> struct Packed;
+template <> struct Packed<float> {
+  typedef float Loose __attribute__((ext_vector_type(4), aligned(4)));
+  __device__ static float get(const uint4& r, int j) { return __uint_as_float(j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w); }
+  __device__ static void store(float* p, const float (&v)[8]) {
+    const Loose x = {v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(x, reinterpret_cast<Loose*>(p));
+  }
+};
+template <> struct Packed<unsigned short> {
+  typedef uint32_t Loose __attribute__((ext_vector_type(4), aligned(2)));
+  __device__ static float get(const uint4& r, int j) {
+    const uint32_t w = j < 2 ? r.x : j < 4 ? r.y : j < 6 ? r.z : r.w;
+    return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  __device__ static void store(unsigned short* p, const float (&v)[8]) {
+    const Loose x = {f32x2_to_bf16(v[0], v[1]), f32x2_to_bf16(v[2], v[3]), f32x2_to_bf16(v[4], v[5]), f32x2_to_bf16(v[6], v[7])};
+    __builtin_nontemporal_store(x, reinterpret_cast<Loose*>(p));
+  }
+};
+constexpr float kFar = 1e9f;  // a reference in log2 units whose rounding (64) leaves the exponentials in range
+
+template <typename T, bool REST, int THREADS, int NREG, int NLDS, int VECS>
+__global__ __launch_bounds__(THREADS) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
+                                                              T* __restrict__ dlogits, int64_t ld_d) {
+  typedef RowLds<THREADS, NLDS, VECS> Lds;
+  __shared__ Lds s;
+  constexpr int kPer = Row<T>::kPer, kSlots = (kMaxIds + THREADS - 1) / THREADS;
+  const int row_i = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const T* const row = logits + (int64_t)row_i * ld;
+  T* const drow = dlogits + (int64_t)row_i * ld_d;
+  const RowSpan sp(row, vocab, true, 0, 1);
+  const T* const body = row + sp.head;
+  T* const dbody = drow + sp.head;
+  const float weight = t.weights[row_i];
+  if (weight == 0.f) {
+    const float none[8] = {};
+    for (int q = tid; q < sp.n_vec; q += THREADS) Packed<T>::store(dbody + (uint32_t)q * kPer, none);
+    if (tid < sp.n_scalar) Row<T>::store_one(drow + sp.scalar<T>(tid), 0.f);
+    if (tid == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
+    return;
+  }
+  // The row on its way, THREADS vectors (a tile) at a time: those of tile i start at a scalar address.  In the last tile a vector
+  // behind the row is the row's last again.
+  uint4 reg[NREG];
+  const int last_q = sp.n_vec - 1, full = sp.n_vec / THREADS, tiles = (sp.n_vec + THREADS - 1) / THREADS;
+  auto load = [&](int i) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const T* const from = body + (int64_t)i * THREADS * kPer;
+    const uint32_t at = i < full ? tid : min(tid, last_q - i * THREADS);
+    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + at * kPer));
+    return make_uint4(x.x, x.y, x.z, x.w);
+  };
+#pragma unroll
+  for (int i = 0; i < NREG; ++i) {
+    reg[i] = make_uint4(0, 0, 0, 0);
+    if (i < tiles) reg[i] = load(i);
+  }
+  const float single_z = tid < sp.n_scalar ? Row<T>::one(row + sp.scalar<T>(tid)) : -INFINITY;
+
+  // the given tokens: their logits, and where they lie
+  float z[kSlots], lq[kSlots];
+  int id[kSlots];
+  bool first[kSlots], twice[kSlots];
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * THREADS;
+    id[u] = -1;
+    lq[u] = z[u] = -INFINITY;
+    if (i < t.k) {
+      id[u] = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
+      if (id[u] >= 0) {
+        z[u] = Row<T>::one(row + id[u]);
+        lq[u] = t.logprobs[(int64_t)row_i * t.k + i];
+      }
+      s.id[i] = id[u];
+    }
+  }
+  for (int i = tid; i < (sp.n_vec + 3) / 4; i += THREADS) s.given[i] = 0;
+  for (int i = tid; i < kBuckets; i += THREADS) s.heads[i] = -1;
+  if (tid == 0) s.single = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * THREADS;
+    first[u] = id[u] >= 0;
+    twice[u] = false;
+    if (id[u] < 0) continue;
+    for (int j = 0; j < t.k; ++j) {
+      const bool same = s.id[j] == id[u] && j != i;
+      twice[u] |= same;
+      first[u] = first[u] && !(same && j < i);
+    }
+    if (!first[u]) continue;
+    const int in = id[u] - sp.head, q = in >= 0 ? in / kPer : -1;
+    if (q >= 0 && q < sp.n_vec) {
+      atomicOr(s.given + (q >> 2), 1u << ((q & 3) * 8 + in % kPer));
+      s.next[i] = (int16_t)atomicExch(s.heads + (q & (kBuckets - 1)), i);
+    } else {
+      atomicOr(&s.single, 1u << (in < 0 ? id[u] : id[u] - sp.n_vec * kPer));
+    }
+  }
+  __syncthreads();
+  const uint8_t* const given = reinterpret_cast<const uint8_t*>(s.given);
+
+  // Statistics.  Against a thread's own reference c = ref k rounded an element is one instruction beside its exponential, and
+  // what c is off by is taken back at the end; the largest of a few logits will do as long as the sum stays in range.
+  const float k = t.inv_t * kLog2e;
+  auto visit = [&](auto&& f) {  // f(vector, tile) for every vector of this thread
+#pragma unroll
+    for (int i = 0; i < NREG; ++i)
+      if (i < tiles) f(reg[i], i);
+#pragma unroll 1
+    for (int i = NREG; i < min(NREG + NLDS, tiles); ++i) f(s.tiles[(i - NREG) * THREADS + tid], i);
+#pragma unroll 1
+    for (int i = NREG + NLDS; i < tiles; ++i) f(load(i), i);
+  };
+#pragma unroll 1
+  for (int i = NREG; i < min(NREG + NLDS, tiles); ++i) s.tiles[(i - NREG) * THREADS + tid] = load(i);
+  const bool single_in = !(REST && tid < sp.n_scalar && (s.single >> tid & 1));
+  auto elements = [&](const uint4& r, int i, float (&v)[8]) {  // what is not there or not counted at -inf
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = Packed<T>::get(r, j);
+    uint32_t off = 0;
+    if (i < full) {
+      if (REST) off = given[i * THREADS + tid];
+    } else if (i * THREADS + tid > last_q) {
+      off = 0xff;
+    } else if (REST) {
+      off = given[i * THREADS + tid];
+    }
+    if (off != 0) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = (off >> j & 1) ? -INFINITY : v[j];
+    }
+  };
+  float ref = single_in ? single_z : -INFINITY;
+  if (sp.n_vec > 0) {
+    float v[8];
+    elements(reg[0], 0, v);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) ref = fmaxf(ref, v[j]);
+  }
+  ref = wave_max(ref);
+  float sum = 0.f;
+  const float cc = ref * k;
+  bool plain = fabsf(cc) < kFar;
+  if (plain) {
+    float s4[4] = {};
+    visit([&](const uint4& r, int i) {
+      float v[8];
+      elements(r, i, v);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(v[j], k, -cc));
+    });
+    if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
+    sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc));
+    plain = sum > 0x1p-60f && sum < 0x1p80f;
+  }
+  if (!plain) {  // another scale, logits far from 0, infinite, or not numbers: by differences from the largest
+    Sum st{kLowest, 0.f};
+    visit([&](const uint4& r, int i) {
+      float v[8];
+      elements(r, i, v);
+      fold<kPer>(st, v, k);
+    });
+    if (single_in) {
+      const float v[8] = {single_z};
+      fold<1>(st, v, k);
+    }
+    ref = wave_max(st.M);
+    sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - ref) * k));
+  }
+  if (lane == 0) { s.red_m[wave] = ref; s.red_s[wave] = sum; }
+  __syncthreads();
+
+  // the outcomes, in 64 bits
+  const double inv_t = (double)t.inv_t, kd = (double)k;
+  constexpr int kRowWaves = THREADS / kWave;
+  const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
+  float M = wave_max(part_m);
+  float best = -INFINITY, best_q = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    best = fmaxf(best, z[u]);
+    best_q = fmaxf(best_q, lq[u]);
+  }
+  best = wave_max(best);
+  best_q = wave_max(best_q);
+  constexpr int kIdWaves = (THREADS < kMaxIds ? THREADS : kMaxIds) / kWave;  // wavefronts that have given tokens: a power of two
+  __shared__ float red_id[2][kIdWaves];
+  __shared__ double red_d[2][4][kIdWaves];
+  if (lane == 0 && wave < kIdWaves) { red_id[0][wave] = best; red_id[1][wave] = best_q; }
+  __syncthreads();
+  M = fmaxf(M, wave_max(red_id[0][lane & (kIdWaves - 1)]));
+  best_q = wave_max(red_id[1][lane & (kIdWaves - 1)]);
+  // a wavefront's part of a sum over the given tokens to all threads, in a fixed order
+  auto all_sum = [&](int round, double (&v)[4], int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n && wave < kIdWaves) v[i] = wave_sum_d(v[i]);
+    if (lane == 0 && wave < kIdWaves)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red_d[round][i][wave] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) v[i] = wave_sum_d(lane < kIdWaves ? red_d[round][i][lane] : 0.0);
+  };
+  double v1[4] = {};
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    if (id[u] < 0) continue;
+    if (REST && first[u]) v1[0] += exp(((double)z[u] - (double)M) * inv_t);
+    if (t.tail == AXON_DISTILL_RENORMALIZE) v1[1] += exp((double)lq[u] - (double)best_q);
+    if (REST) v1[2] += exp((double)lq[u]);
+  }
+  all_sum(0, v1, 3);
+  // the whole range of 64 bits: what is left may be next to nothing
+  const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
+  const double s_rest = wave_sum_d(ldexp((double)part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
+  const double s_all = REST ? s_rest + v1[0] : s_rest;
+  const double ln_s = s_all > 0.0 ? log(s_all) : (double)NAN;  // a row of -inf alone has no softmax
+  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log(v1[1]) : 0.0;
+  double w1[4] = {};  // loss, sum of G, covered
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * THREADS;
+    if (i >= t.k) continue;
+    Term o{0.0, 0.0};
+    if (id[u] >= 0) {
+      const double lp = ((double)z[u] - (double)M) * inv_t - ln_s;
+      o = outcome(t, (double)lq[u] - norm_q, lp);
+      w1[2] += exp(lp);
+    }
+    w1[0] += o.loss;
+    w1[1] += o.g;
+    s.g[i] = (float)o.g;
+    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
+  }
+  all_sum(1, w1, 3);
+  const float g = weight * t.inv_t;
+  if (tid == 0) {
+    double out_scale = 0.0;
+    if (REST) {
+      const double lp_rest = log(s_rest) - ln_s;
+      const Term o = outcome(t, log(fmax(1.0 - v1[2], 0.0)), lp_rest);
+      w1[0] += o.loss;
+      w1[1] += o.g;
+      out_scale = s_rest > 0.0 ? o.g * exp(-lp_rest) : 0.0;
+    }
+    const float lse = (float)((double)M + ln_s / inv_t);
+    const float c_out = (float)(out_scale - w1[1]), c_in = (float)-w1[1];
+    const float rest = (float)((((double)M - (double)lse) * inv_t + ln_s) * 1.4426950408889634);
+    out.losses[row_i] = (float)w1[0];
+    out.covered[row_i] = (float)w1[2];
+    float* const c = out.coef + row_i;
+    c[(int64_t)kLse * out.n] = lse;
+    c[(int64_t)kRest * out.n] = rest;
+    c[(int64_t)kOut * out.n] = c_out;
+    c[(int64_t)kIn * out.n] = c_in;
+    // p = 2^(z k - off) f with off = lse k rounded; far from 0 by the difference from lse
+    const float off = lse * k;
+    const bool is_far = !(fabsf(off) < kFar);
+    const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)lse * kd)) - rest);
+    s.lse = is_far ? lse : off;
+    s.is_far = is_far;
+    s.c_out = g * c_out * f;
+    s.c_in = g * c_in * f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSlots; ++u) {
+    const int i = tid + u * THREADS;
+    if (!first[u]) continue;
+    float total = s.g[i];
+    if (twice[u]) {
+      total = 0.f;
+      for (int j = i; j < t.k; ++j)
+        if (s.id[j] == id[u]) total += s.g[j];
+    }
+    s.total[i] = g * total;
+  }
+  __syncthreads();
+
+  const float lse = s.lse, c_out = s.c_out, c_in = s.c_in;
+  const bool is_far = s.is_far != 0;
+  auto power = [&](float x) { return __builtin_amdgcn_exp2f(is_far ? (x - lse) * k : fmaf(x, k, -lse)); };
+  auto write = [&](const uint4& r, int i) {
+    const int q = i * THREADS + tid;
+    if (i >= full && q > last_q) return;
+    float v[8];
+    if (is_far) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = __builtin_amdgcn_exp2f((Packed<T>::get(r, j) - lse) * k) * c_out;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -lse)) * c_out;
+    }
+    if (given[q] != 0) {
+      const int id0 = sp.head + q * kPer;
+      for (int h = s.heads[q & (kBuckets - 1)]; h >= 0; h = s.next[h]) {
+        const int j = s.id[h] - id0;
+        if (j < 0 || j >= kPer) continue;
+        const float total = s.total[h];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (e == j) v[e] = fmaf(power(Packed<T>::get(r, e)), c_in, total);
+      }
+    }
+    Packed<T>::store(dbody + (int64_t)i * THREADS * kPer + (uint32_t)tid * kPer, v);
+  };
+  visit(write);
+  if (tid < sp.n_scalar) {
+    float v = power(single_z) * c_out;
+    if (s.single >> tid & 1) {
+      const int me = sp.scalar<T>(tid);
+      for (int i = 0; i < t.k; ++i)
+        if (s.id[i] == me) {
+          v = fmaf(power(single_z), c_in, s.total[i]);  // the first of them has the total
+          break;
+        }
+    }
+    Row<T>::store_one(drow + sp.scalar<T>(tid), v);
+  }
+}
+
 // sum_t w_t loss_t in 64 bits, in a fixed order.
 constexpr int kSumBlock = 1024;
 __global__ __launch_bounds__(kSumBlock) void distill_sum_kernel(const float* __restrict__ losses, const float* __restrict__ weights, int n,
@@ -513,16 +858,54 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
   return AXON_OK;
 }
 
+namespace {
+
+// One workgroup per row with the row in registers and LDS.  Rows of up to 64 KB: 256 threads, four workgroups on a compute unit;
+// up to 128 KB: 512, two; longer: 1024, one, of which 400 KB are held and the rest is read twice.
+constexpr int kMaxRowVecs = 38912;  // a byte per vector in LDS beside the rest of a row
+template <typename T, bool REST>
+int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const Teacher& t, const RowOut& out, void* dlogits, int64_t ld_d,
+                hipStream_t st) {
+  const int64_t vecs = vocab / Row<T>::kPer;
+#define AXON_ROW(THREADS, NREG, NLDS, VECS)                                                                                         \
+  hipLaunchKernelGGL((distill_row_kernel<T, REST, THREADS, NREG, NLDS, VECS>), dim3((unsigned)n), dim3(THREADS), 0, st,             \
+                     static_cast<const T*>(logits), ld, (int)vocab, t, out, static_cast<T*>(dlogits), ld_d)
+  if (vecs <= 256 * 16) AXON_ROW(256, 16, 0, 256 * 16);
+  else if (vecs <= 512 * 16) AXON_ROW(512, 16, 0, 512 * 16);
+  else AXON_ROW(1024, 18, 7, kMaxRowVecs);
+#undef AXON_ROW
+  AXON_CHECK_LAUNCH();
+  return AXON_OK;
+}
+
+}  // namespace
+
 extern "C" int axon_distill_loss(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_i64,
                                  const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
                                  float temperature, float* loss, float* losses, float* covered, float* grads, float* coef, void* dlogits,
                                  int64_t ld_d, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!loss || (n > 0 && !weights)) return AXON_ERR_ARG;
   int rc = dlogits ? check_rows(dlogits, dtype, ld_d, n, vocab) : AXON_OK;
-  if (rc == AXON_OK)
+  const bool rows = rc == AXON_OK && dlogits && n >= 1 && vocab * elem_bytes(dtype) / 16 <= kMaxRowVecs;
+  if (rows) {
+    rc = check_rows(logits, dtype, ld, n, vocab);
+    if (rc == AXON_OK) rc = check_teacher(ids, teacher_logprobs, k, divergence, tail, beta, temperature);
+    if (rc != AXON_OK) return rc;
+    if (!losses || !covered || !grads || !coef) return AXON_ERR_ARG;
+    const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail, beta, 1.f / temperature};
+    const RowOut out{losses, covered, grads, coef, (int)n};
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == AXON_LOGITS_F32)
+      rc = tail == AXON_DISTILL_REST ? launch_rows<float, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
+                                     : launch_rows<float, false>(logits, ld, n, vocab, t, out, dlogits, ld_d, st);
+    else
+      rc = tail == AXON_DISTILL_REST ? launch_rows<unsigned short, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
+                                     : launch_rows<unsigned short, false>(logits, ld, n, vocab, t, out, dlogits, ld_d, st);
+  } else if (rc == AXON_OK) {
     rc = axon_distill_fwd(logits, dtype, ld, n, vocab, ids, ids_i64, teacher_logprobs, k, weights, divergence, tail, beta, temperature, losses,
                           covered, grads, coef, workspace, workspace_bytes, stream);
-  if (rc == AXON_OK && dlogits)
+  }
+  if (rc == AXON_OK && dlogits && !rows)
     rc = axon_distill_bwd(logits, dtype, ld, n, vocab, ids, ids_i64, k, weights, temperature, grads, coef, nullptr, 0, dlogits, ld_d, stream);
   if (rc != AXON_OK) return rc;
   hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumBlock), 0, (hipStream_t)stream, losses, weights, (int)n, loss);
