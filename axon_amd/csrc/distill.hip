@@ -140,17 +140,27 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
   parts[blockIdx.x] = make_float4(M, (float)total, (float)(total - (float)total), 0.f);
 }
 
+// What one lane has written to LDS, for the others of its wavefront: LDS serves a wavefront in order, the compiler is told to.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// In 64 bits, as functions that are called: inlined a dozen times their registers and their code would be those of the kernel.
+__device__ __attribute__((noinline)) double exp64(double x) { return exp(x); }
+__device__ __attribute__((noinline)) double log64(double x) { return log(x); }
+
 // One outcome: its share of the loss and G.
 struct Term { double loss, g; };
 __device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) {
-  const double q = exp(lq), p = exp(lp);
+  const double q = exp64(lq), p = exp64(lp);
   if (t.divergence == AXON_DISTILL_FORWARD) return {q > 0.0 ? q * (lq - lp) : q - q, -q};
   if (t.divergence == AXON_DISTILL_REVERSE) {
     if (p == 0.0) return {0.0, 0.0};
     const double d = p * (lp - lq);
     return {d, d + p};
   }
-  const double b = (double)t.beta, lm = log(b * q + (1.0 - b) * p);
+  const double b = (double)t.beta, lm = log64(b * q + (1.0 - b) * p);
   const double mine = p == 0.0 ? 0.0 : (1.0 - b) * p * (lp - lm);
   return {(q == 0.0 ? 0.0 : b * q * (lq - lm)) + mine, mine};
 }
@@ -224,20 +234,20 @@ __device__ __forceinline__ void finish_row(int row_i, const T* row, int vocab, c
     M = fmaxf(M, (float)lds.red[w][0]);
     best_q = fmaxf(best_q, (float)lds.red[w][1]);
   }
-  const double scale_in = exp(((double)M_in - (double)M) * inv_t);  // of the statistics to the reference M
+  const double scale_in = exp64(((double)M_in - (double)M) * inv_t);  // of the statistics to the reference M
   double v[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
   for (int u = 0; u < kSlots; ++u) {
     if (id[u] < 0) continue;
-    if (REST && first[u]) v[0] += exp(((double)z[u] - (double)M) * inv_t);
-    if (t.tail == AXON_DISTILL_RENORMALIZE) v[1] += exp(lq[u] - (double)best_q);
-    if (REST) v[2] += exp(lq[u]);
+    if (REST && first[u]) v[0] += exp64(((double)z[u] - (double)M) * inv_t);
+    if (t.tail == AXON_DISTILL_RENORMALIZE) v[1] += exp64(lq[u] - (double)best_q);
+    if (REST) v[2] += exp64(lq[u]);
   }
   sum4(v, lds);
   const double s_rest = s_in * scale_in, s = REST ? s_rest + v[0] : s_rest;
-  const double ln_s = s > 0.0 ? log(s) : (double)NAN;  // a row of -inf alone has no softmax
-  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log(v[1]) : 0.0;
-  const double q_rest = fmax(1.0 - v[2], 0.0), lp_rest = log(s_rest) - ln_s;
+  const double ln_s = s > 0.0 ? log64(s) : (double)NAN;  // a row of -inf alone has no softmax
+  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log64(v[1]) : 0.0;
+  const double q_rest = fmax(1.0 - v[2], 0.0), lp_rest = log64(s_rest) - ln_s;
   double w[4] = {0.0, 0.0, 0.0, 0.0};  // loss, sum of G, covered
 #pragma unroll
   for (int u = 0; u < kSlots; ++u) {
@@ -247,7 +257,7 @@ __device__ __forceinline__ void finish_row(int row_i, const T* row, int vocab, c
     if (id[u] >= 0) {
       const double lp = ((double)z[u] - (double)M) * inv_t - ln_s;
       o = outcome(t, lq[u] - norm_q, lp);
-      w[2] += exp(lp);
+      w[2] += exp64(lp);
     }
     w[0] += o.loss;
     w[1] += o.g;
@@ -257,10 +267,10 @@ __device__ __forceinline__ void finish_row(int row_i, const T* row, int vocab, c
   if (tid != 0) return;
   double out_scale = 0.0;
   if (REST) {
-    const Term o = outcome(t, log(q_rest), lp_rest);
+    const Term o = outcome(t, log64(q_rest), lp_rest);
     w[0] += o.loss;
     w[1] += o.g;
-    out_scale = s_rest > 0.0 ? o.g * exp(-lp_rest) : 0.0;
+    out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
   }
   const float lse = (float)((double)M + ln_s / inv_t);
   out.losses[row_i] = (float)w[0];
@@ -286,7 +296,7 @@ __global__ __launch_bounds__(kBlock) void distill_finish_kernel(const T* __restr
   double s = 0.0;
   const float4 p = lane < n_parts ? parts[(int64_t)row_i * n_parts + lane] : make_float4(kLowest, 0.f, 0.f, 0.f);
   M = wave_max(p.x);
-  s = wave_sum_d(((double)p.y + (double)p.z) * exp(((double)p.x - (double)M) * (double)t.inv_t));
+  s = wave_sum_d(((double)p.y + (double)p.z) * exp64(((double)p.x - (double)M) * (double)t.inv_t));
   finish_row<T, REST>(row_i, logits + (int64_t)row_i * ld, vocab, t, out, M, s, lds);
 }
 
@@ -383,20 +393,21 @@ __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, i
     if (where[u] >= 0) Row<T>::store_one(out + where[u], again[u]);
 }
 
-// The loss and its gradient from ONE read of a row: a workgroup holds the row, NREG 16-byte vectors of every thread in registers and
-// NLDS in LDS, from its statistics to its gradient (what is longer is read again).  The given tokens are found by a byte per vector
-// in LDS that says which of its elements are given, and by a hash of the vector's number for the few vectors that have one; their
-// gradients are put in before the vector is stored.
-constexpr int kBuckets = 256;
-template <int THREADS, int NLDS, int VECS>
+// The loss and its gradient from ONE read of a row.  A workgroup walks rows; it holds a row, NREG 16-byte vectors of every thread in
+// registers and NLDS in LDS, from its statistics to its gradient (what is longer is read again), and asks for the next row's vectors
+// as those of the row leave.  ROW threads do that; the 64 threads behind them look after the given tokens: where they lie while the
+// row is on its way, the outcomes in 64 bits when its statistics are there.
+// A thread's vectors that hold a given token are marked by a bit; the passes over the row leave them out, and a short loop takes
+// them one by one, with the tokens found through a hash of the vector's number.
+constexpr int kBuckets = 256, kAgain = -2, kMaxTiles = 64;
+template <int ROW>
 struct RowLds {
-  uint4 tiles[NLDS > 0 ? NLDS * THREADS : 1];
-  uint32_t given[(VECS + 3) / 4];
+  uint32_t marks[2][ROW];            // bit i % 32 of word i / 32: this thread's vector of tile i holds a given token
   int id[kMaxIds], heads[kBuckets];  // chains of the ids that come for the first time
-  int16_t next[kMaxIds];
-  float g[kMaxIds], total[kMaxIds];                 // G, and summed over equal ids
-  float red_m[THREADS / kWave], red_s[THREADS / kWave];
-  uint32_t single;
+  int16_t next[kMaxIds];             // -1: the last of its chain, kAgain: an id that has come before, or none
+  float a[kMaxIds], b[kMaxIds];      // the teacher's log-probabilities, then G; the logits, then what is written in their place
+  float red_m[ROW / kWave], red_s[ROW / kWave];
+  uint32_t single;                   // a bit per element outside the vectors
   float lse, c_out, c_in;
   int is_far;
 };
@@ -423,308 +434,406 @@ template <> struct Packed<unsigned short> {
 };
 constexpr float kFar = 1e9f;  // a reference in log2 units whose rounding (64) leaves the exponentials in range
 
-template <typename T, bool REST, int THREADS, int NREG, int NLDS, int VECS>
-__global__ __launch_bounds__(THREADS) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
-                                                              T* __restrict__ dlogits, int64_t ld_d) {
-  typedef RowLds<THREADS, NLDS, VECS> Lds;
-  __shared__ Lds s;
-  constexpr int kPer = Row<T>::kPer, kSlots = (kMaxIds + THREADS - 1) / THREADS;
-  const int row_i = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const T* const row = logits + (int64_t)row_i * ld;
-  T* const drow = dlogits + (int64_t)row_i * ld_d;
-  const RowSpan sp(row, vocab, true, 0, 1);
-  const T* const body = row + sp.head;
-  T* const dbody = drow + sp.head;
-  const float weight = t.weights[row_i];
-  if (weight == 0.f) {
-    const float none[8] = {};
-    for (int q = tid; q < sp.n_vec; q += THREADS) Packed<T>::store(dbody + (uint32_t)q * kPer, none);
-    if (tid < sp.n_scalar) Row<T>::store_one(drow + sp.scalar<T>(tid), 0.f);
-    if (tid == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
-    return;
-  }
-  // The row on its way, THREADS vectors (a tile) at a time: those of tile i start at a scalar address.  In the last tile a vector
-  // behind the row is the row's last again.
-  uint4 reg[NREG];
-  const int last_q = sp.n_vec - 1, full = sp.n_vec / THREADS, tiles = (sp.n_vec + THREADS - 1) / THREADS;
-  auto load = [&](int i) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const T* const from = body + (int64_t)i * THREADS * kPer;
-    const uint32_t at = i < full ? tid : min(tid, last_q - i * THREADS);
-    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + at * kPer));
-    return make_uint4(x.x, x.y, x.z, x.w);
-  };
-#pragma unroll
-  for (int i = 0; i < NREG; ++i) {
-    reg[i] = make_uint4(0, 0, 0, 0);
-    if (i < tiles) reg[i] = load(i);
-  }
-  const float single_z = tid < sp.n_scalar ? Row<T>::one(row + sp.scalar<T>(tid)) : -INFINITY;
+// A barrier for what the threads have written to LDS themselves: loads on their way, to registers or to LDS, stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-  // the given tokens: their logits, and where they lie
-  float z[kSlots], lq[kSlots];
-  int id[kSlots];
-  bool first[kSlots], twice[kSlots];
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * THREADS;
-    id[u] = -1;
-    lq[u] = z[u] = -INFINITY;
-    if (i < t.k) {
-      id[u] = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
-      if (id[u] >= 0) {
-        z[u] = Row<T>::one(row + id[u]);
-        lq[u] = t.logprobs[(int64_t)row_i * t.k + i];
+// A row as its threads see it.
+template <typename T>
+struct RowView {
+  const T* row;
+  RowSpan sp;
+  __amdgpu_buffer_rsrc_t rsrc;  // of the vectors: behind the last a load gives zeros
+  __device__ __forceinline__ RowView(const T* logits, int64_t ld, int i, int vocab, bool wanted = true)
+      : row(logits + (int64_t)i * ld), sp(row, vocab, true, 0, 1),
+        rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row + sp.head), 0, wanted ? sp.n_vec * 16 : 0, 0x00020000)) {}
+};
+
+// The threads that look after the given tokens of a row (one wavefront).
+template <typename T, bool REST, int ROW>
+struct Outcomes {
+  RowLds<ROW>& s;
+  const Teacher& t;
+  const RowOut& out;
+  int vocab, lane;
+
+  // Where the given tokens lie.
+  __device__ __forceinline__ void mark(int row_i, const RowView<T>& v) {
+    constexpr int kPer = Row<T>::kPer;
+    for (int i = lane; i < ROW; i += kWave) s.marks[0][i] = s.marks[1][i] = 0;
+    for (int i = lane; i < kBuckets; i += kWave) s.heads[i] = -1;
+    if (lane == 0) s.single = 0;
+    for (int i = lane; i < t.k; i += kWave) {
+      const int id = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
+      const float lq = t.logprobs[(int64_t)row_i * t.k + i], z = Row<T>::one(v.row + max(id, 0));
+      s.id[i] = id;
+      s.a[i] = id < 0 ? -INFINITY : lq;
+      s.b[i] = id < 0 ? -INFINITY : z;
+    }
+    wave_sync();
+    for (int i = lane; i < t.k; i += kWave) {
+      const int id = s.id[i];
+      bool first = id >= 0;
+#pragma unroll 8
+      for (int j = 0; j < t.k; ++j) first = first && !(j < i && s.id[j] == id);
+      if (!first) {
+        s.next[i] = kAgain;
+        continue;
       }
-      s.id[i] = id[u];
+      const int in = id - v.sp.head, q = in >= 0 ? in / kPer : -1;
+      if (q >= 0 && q < v.sp.n_vec) {
+        atomicOr(&s.marks[q / ROW / 32][q % ROW], 1u << (q / ROW % 32));
+        s.next[i] = (int16_t)atomicExch(s.heads + (q & (kBuckets - 1)), i);
+      } else {
+        s.next[i] = -1;
+        atomicOr(&s.single, 1u << (in < 0 ? id : id - v.sp.n_vec * kPer));
+      }
     }
+    wave_sync();
   }
-  for (int i = tid; i < (sp.n_vec + 3) / 4; i += THREADS) s.given[i] = 0;
-  for (int i = tid; i < kBuckets; i += THREADS) s.heads[i] = -1;
-  if (tid == 0) s.single = 0;
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * THREADS;
-    first[u] = id[u] >= 0;
-    twice[u] = false;
-    if (id[u] < 0) continue;
-    for (int j = 0; j < t.k; ++j) {
-      const bool same = s.id[j] == id[u] && j != i;
-      twice[u] |= same;
-      first[u] = first[u] && !(same && j < i);
-    }
-    if (!first[u]) continue;
-    const int in = id[u] - sp.head, q = in >= 0 ? in / kPer : -1;
-    if (q >= 0 && q < sp.n_vec) {
-      atomicOr(s.given + (q >> 2), 1u << ((q & 3) * 8 + in % kPer));
-      s.next[i] = (int16_t)atomicExch(s.heads + (q & (kBuckets - 1)), i);
-    } else {
-      atomicOr(&s.single, 1u << (in < 0 ? id[u] : id[u] - sp.n_vec * kPer));
-    }
-  }
-  __syncthreads();
-  const uint8_t* const given = reinterpret_cast<const uint8_t*>(s.given);
 
-  // Statistics.  Against a thread's own reference c = ref k rounded an element is one instruction beside its exponential, and
-  // what c is off by is taken back at the end; the largest of a few logits will do as long as the sum stays in range.
-  const float k = t.inv_t * kLog2e;
-  auto visit = [&](auto&& f) {  // f(vector, tile) for every vector of this thread
-#pragma unroll
-    for (int i = 0; i < NREG; ++i)
-      if (i < tiles) f(reg[i], i);
+  // The outcomes from the statistics of the row (REST: of what is not given), and what is written in the given tokens' places.
+  __device__ __forceinline__ void finish(int row_i, float weight) {
+    const float k = t.inv_t * kLog2e, g = weight * t.inv_t;
+    const double inv_t = (double)t.inv_t;
+    constexpr int kRowWaves = ROW / kWave;
+    const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
+    float M = part_m, best_q = -INFINITY;
+    for (int i = lane; i < t.k; i += kWave) {
+      M = fmaxf(M, s.b[i]);
+      best_q = fmaxf(best_q, s.a[i]);
+    }
+    M = wave_max(M);
+    best_q = wave_max(best_q);
+    double e_first = 0.0, e_norm = 0.0, e_q = 0.0;
+    if (REST || t.tail == AXON_DISTILL_RENORMALIZE) {
 #pragma unroll 1
-    for (int i = NREG; i < min(NREG + NLDS, tiles); ++i) f(s.tiles[(i - NREG) * THREADS + tid], i);
+      for (int i = lane; i < t.k; i += kWave) {
+        if (s.id[i] < 0) continue;
+        if (REST && s.next[i] != kAgain) e_first += exp64(((double)s.b[i] - (double)M) * inv_t);
+        const double e = exp64((double)s.a[i] - (REST ? 0.0 : (double)best_q));
+        if (REST) e_q += e; else e_norm += e;
+      }
+      if (REST) {
+        e_first = wave_sum_d(e_first);
+        e_q = wave_sum_d(e_q);
+      } else {
+        e_norm = wave_sum_d(e_norm);
+      }
+    }
+    // the whole range of 64 bits: what is left may be next to nothing
+    const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
+    const double s_rest = wave_sum_d(ldexp((double)part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
+    const double s_all = REST ? s_rest + e_first : s_rest;
+    const double ln_s = s_all > 0.0 ? log64(s_all) : (double)NAN;  // a row of -inf alone has no softmax
+    const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log64(e_norm) : 0.0;
+    double loss = 0.0, sum_g = 0.0, covered = 0.0;
 #pragma unroll 1
-    for (int i = NREG + NLDS; i < tiles; ++i) f(load(i), i);
-  };
-#pragma unroll 1
-  for (int i = NREG; i < min(NREG + NLDS, tiles); ++i) s.tiles[(i - NREG) * THREADS + tid] = load(i);
-  const bool single_in = !(REST && tid < sp.n_scalar && (s.single >> tid & 1));
-  auto elements = [&](const uint4& r, int i, float (&v)[8]) {  // what is not there or not counted at -inf
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = Packed<T>::get(r, j);
-    uint32_t off = 0;
-    if (i < full) {
-      if (REST) off = given[i * THREADS + tid];
-    } else if (i * THREADS + tid > last_q) {
-      off = 0xff;
-    } else if (REST) {
-      off = given[i * THREADS + tid];
+    for (int i = lane; i < t.k; i += kWave) {
+      Term o{0.0, 0.0};
+      if (s.id[i] >= 0) {
+        const double lp = ((double)s.b[i] - (double)M) * inv_t - ln_s;
+        o = outcome(t, (double)s.a[i] - norm_q, lp);
+        covered += exp64(lp);
+      }
+      loss += o.loss;
+      sum_g += o.g;
+      s.a[i] = (float)o.g;
+      out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
     }
-    if (off != 0) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) v[j] = (off >> j & 1) ? -INFINITY : v[j];
-    }
-  };
-  float ref = single_in ? single_z : -INFINITY;
-  if (sp.n_vec > 0) {
-    float v[8];
-    elements(reg[0], 0, v);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) ref = fmaxf(ref, v[j]);
-  }
-  ref = wave_max(ref);
-  float sum = 0.f;
-  const float cc = ref * k;
-  bool plain = fabsf(cc) < kFar;
-  if (plain) {
-    float s4[4] = {};
-    visit([&](const uint4& r, int i) {
-      float v[8];
-      elements(r, i, v);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(v[j], k, -cc));
-    });
-    if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
-    sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc));
-    plain = sum > 0x1p-60f && sum < 0x1p80f;
-  }
-  if (!plain) {  // another scale, logits far from 0, infinite, or not numbers: by differences from the largest
-    Sum st{kLowest, 0.f};
-    visit([&](const uint4& r, int i) {
-      float v[8];
-      elements(r, i, v);
-      fold<kPer>(st, v, k);
-    });
-    if (single_in) {
-      const float v[8] = {single_z};
-      fold<1>(st, v, k);
-    }
-    ref = wave_max(st.M);
-    sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - ref) * k));
-  }
-  if (lane == 0) { s.red_m[wave] = ref; s.red_s[wave] = sum; }
-  __syncthreads();
-
-  // the outcomes, in 64 bits
-  const double inv_t = (double)t.inv_t, kd = (double)k;
-  constexpr int kRowWaves = THREADS / kWave;
-  const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
-  float M = wave_max(part_m);
-  float best = -INFINITY, best_q = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    best = fmaxf(best, z[u]);
-    best_q = fmaxf(best_q, lq[u]);
-  }
-  best = wave_max(best);
-  best_q = wave_max(best_q);
-  constexpr int kIdWaves = (THREADS < kMaxIds ? THREADS : kMaxIds) / kWave;  // wavefronts that have given tokens: a power of two
-  __shared__ float red_id[2][kIdWaves];
-  __shared__ double red_d[2][4][kIdWaves];
-  if (lane == 0 && wave < kIdWaves) { red_id[0][wave] = best; red_id[1][wave] = best_q; }
-  __syncthreads();
-  M = fmaxf(M, wave_max(red_id[0][lane & (kIdWaves - 1)]));
-  best_q = wave_max(red_id[1][lane & (kIdWaves - 1)]);
-  // a wavefront's part of a sum over the given tokens to all threads, in a fixed order
-  auto all_sum = [&](int round, double (&v)[4], int n) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n && wave < kIdWaves) v[i] = wave_sum_d(v[i]);
-    if (lane == 0 && wave < kIdWaves)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red_d[round][i][wave] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) v[i] = wave_sum_d(lane < kIdWaves ? red_d[round][i][lane] : 0.0);
-  };
-  double v1[4] = {};
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    if (id[u] < 0) continue;
-    if (REST && first[u]) v1[0] += exp(((double)z[u] - (double)M) * inv_t);
-    if (t.tail == AXON_DISTILL_RENORMALIZE) v1[1] += exp((double)lq[u] - (double)best_q);
-    if (REST) v1[2] += exp((double)lq[u]);
-  }
-  all_sum(0, v1, 3);
-  // the whole range of 64 bits: what is left may be next to nothing
-  const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
-  const double s_rest = wave_sum_d(ldexp((double)part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
-  const double s_all = REST ? s_rest + v1[0] : s_rest;
-  const double ln_s = s_all > 0.0 ? log(s_all) : (double)NAN;  // a row of -inf alone has no softmax
-  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log(v1[1]) : 0.0;
-  double w1[4] = {};  // loss, sum of G, covered
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * THREADS;
-    if (i >= t.k) continue;
-    Term o{0.0, 0.0};
-    if (id[u] >= 0) {
-      const double lp = ((double)z[u] - (double)M) * inv_t - ln_s;
-      o = outcome(t, (double)lq[u] - norm_q, lp);
-      w1[2] += exp(lp);
-    }
-    w1[0] += o.loss;
-    w1[1] += o.g;
-    s.g[i] = (float)o.g;
-    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
-  }
-  all_sum(1, w1, 3);
-  const float g = weight * t.inv_t;
-  if (tid == 0) {
+    loss = wave_sum_d(loss);
+    sum_g = wave_sum_d(sum_g);
+    covered = wave_sum_d(covered);
     double out_scale = 0.0;
     if (REST) {
-      const double lp_rest = log(s_rest) - ln_s;
-      const Term o = outcome(t, log(fmax(1.0 - v1[2], 0.0)), lp_rest);
-      w1[0] += o.loss;
-      w1[1] += o.g;
-      out_scale = s_rest > 0.0 ? o.g * exp(-lp_rest) : 0.0;
+      const double lp_rest = log64(s_rest) - ln_s;
+      const Term o = outcome(t, log64(fmax(1.0 - e_q, 0.0)), lp_rest);
+      loss += o.loss;
+      sum_g += o.g;
+      out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
     }
     const float lse = (float)((double)M + ln_s / inv_t);
-    const float c_out = (float)(out_scale - w1[1]), c_in = (float)-w1[1];
     const float rest = (float)((((double)M - (double)lse) * inv_t + ln_s) * 1.4426950408889634);
-    out.losses[row_i] = (float)w1[0];
-    out.covered[row_i] = (float)w1[2];
-    float* const c = out.coef + row_i;
-    c[(int64_t)kLse * out.n] = lse;
-    c[(int64_t)kRest * out.n] = rest;
-    c[(int64_t)kOut * out.n] = c_out;
-    c[(int64_t)kIn * out.n] = c_in;
+    const float coef_out = (float)(out_scale - sum_g), coef_in = (float)-sum_g;
     // p = 2^(z k - off) f with off = lse k rounded; far from 0 by the difference from lse
     const float off = lse * k;
     const bool is_far = !(fabsf(off) < kFar);
-    const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)lse * kd)) - rest);
-    s.lse = is_far ? lse : off;
-    s.is_far = is_far;
-    s.c_out = g * c_out * f;
-    s.c_in = g * c_in * f;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * THREADS;
-    if (!first[u]) continue;
-    float total = s.g[i];
-    if (twice[u]) {
-      total = 0.f;
-      for (int j = i; j < t.k; ++j)
-        if (s.id[j] == id[u]) total += s.g[j];
+    const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)lse * (double)k)) - rest);
+    const float base = is_far ? lse : off, c_in = g * coef_in * f;
+    if (lane == 0) {
+      out.losses[row_i] = (float)loss;
+      out.covered[row_i] = (float)covered;
+      float* const c = out.coef + row_i;
+      c[(int64_t)kLse * out.n] = lse;
+      c[(int64_t)kRest * out.n] = rest;
+      c[(int64_t)kOut * out.n] = coef_out;
+      c[(int64_t)kIn * out.n] = coef_in;
+      s.lse = base;
+      s.is_far = is_far;
+      s.c_out = g * coef_out * f;
+      s.c_in = c_in;
     }
-    s.total[i] = g * total;
+    wave_sync();
+    for (int i = lane; i < t.k; i += kWave) {
+      if (s.next[i] == kAgain) continue;
+      float total = s.a[i];
+#pragma unroll 8
+      for (int j = i + 1; j < t.k; ++j) total += s.id[j] == s.id[i] ? s.a[j] : 0.f;
+      const float z = s.b[i], p = __builtin_amdgcn_exp2f(is_far ? (z - base) * k : fmaf(z, k, -base));
+      s.b[i] = fmaf(p, c_in, g * total);
+    }
   }
-  __syncthreads();
+};
 
-  const float lse = s.lse, c_out = s.c_out, c_in = s.c_in;
-  const bool is_far = s.is_far != 0;
-  auto power = [&](float x) { return __builtin_amdgcn_exp2f(is_far ? (x - lse) * k : fmaf(x, k, -lse)); };
-  auto write = [&](const uint4& r, int i) {
-    const int q = i * THREADS + tid;
-    if (i >= full && q > last_q) return;
-    float v[8];
-    if (is_far) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) v[j] = __builtin_amdgcn_exp2f((Packed<T>::get(r, j) - lse) * k) * c_out;
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -lse)) * c_out;
+// GRID: the most workgroups of a launch.
+template <typename T, bool REST, int ROW, int NREG, int NLDS, int GRID>
+__global__ __launch_bounds__(ROW + kWave, 4) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
+                                                                     T* __restrict__ dlogits, int64_t ld_d) {
+  __shared__ RowLds<ROW> s;
+  __shared__ int s_count[GRID], s_list[2][kWave];
+  __shared__ uint4 s_tiles[NLDS * ROW];  // an array of its own: reads of the rest do not wait for what is on its way here
+  constexpr int kPer = Row<T>::kPer;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const float k = t.inv_t * kLog2e;
+  // Rows that are looked at and rows of weight 0 go round the workgroups by their number among their kind, 64 rows of each kind a
+  // workgroup at a time: list[0] and list[1].
+  const int grid = (int)gridDim.x, me = (int)blockIdx.x, n = out.n;
+  for (int64_t batch = 0; batch < n; batch += (int64_t)kWave * grid) {
+    const int rows = (int)min((int64_t)kWave * grid, n - batch), chunks = (rows + kWave - 1) / kWave;
+    lds_barrier();  // the lists of the batch before have been read
+    for (int c = wave; c < chunks; c += ROW / kWave + 1) {
+      const int at = c * kWave + lane;
+      const uint64_t on = __ballot(at < rows && t.weights[batch + min(at, rows - 1)] != 0.f);
+      if (lane == 0) s_count[c] = __popcll(on);
     }
-    if (given[q] != 0) {
-      const int id0 = sp.head + q * kPer;
-      for (int h = s.heads[q & (kBuckets - 1)]; h >= 0; h = s.next[h]) {
-        const int j = s.id[h] - id0;
-        if (j < 0 || j >= kPer) continue;
-        const float total = s.total[h];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (e == j) v[e] = fmaf(power(Packed<T>::get(r, e)), c_in, total);
+    lds_barrier();
+    for (int c = wave; c < chunks; c += ROW / kWave + 1) {
+      int before = 0;
+      for (int i = lane; i < c; i += kWave) before += s_count[i];
+      before = (int)wave_sum((float)before);  // at most 2^16
+      const int at = c * kWave + lane;
+      const bool there = at < rows, on = there && t.weights[batch + min(at, rows - 1)] != 0.f;
+      const uint64_t kind = __ballot(there && on), other = __ballot(there && !on), below = (1ull << lane) - 1;
+      const int rank = on ? before + __popcll(kind & below) : c * kWave - before + __popcll(other & below);
+      if (there && rank % grid == me) s_list[on ? 0 : 1][rank / grid] = at;
+    }
+    int total = 0;
+    lds_barrier();
+    for (int i = lane; i < chunks; i += kWave) total += s_count[i];
+    total = (int)wave_sum((float)total);
+    const int n_on = (total - me + grid - 1) / grid, n_off = (rows - total - me + grid - 1) / grid;  // (0 where me is beyond)
+    const int on_l = s_list[0][lane], off_l = s_list[1][lane];
+    const auto row_of = [&](int j) { return (int)batch + __builtin_amdgcn_readlane(on_l, j); };
+
+    if (wave == ROW / kWave) {
+      Outcomes<T, REST, ROW> o{s, t, out, vocab, lane};
+      if (lane < n_off) out.losses[batch + off_l] = out.covered[batch + off_l] = 0.f;
+      for (int j = 0; j < n_on; ++j) {
+        const int row_i = row_of(j);
+        o.mark(row_i, RowView<T>(logits, ld, row_i, vocab));
+        lds_barrier();  // the marks are there
+        lds_barrier();  // the statistics are there
+        o.finish(row_i, t.weights[row_i]);
+        lds_barrier();  // the row's constants are there
+        lds_barrier();  // the given tokens are written
       }
+      continue;
     }
-    Packed<T>::store(dbody + (int64_t)i * THREADS * kPer + (uint32_t)tid * kPer, v);
-  };
-  visit(write);
-  if (tid < sp.n_scalar) {
-    float v = power(single_z) * c_out;
-    if (s.single >> tid & 1) {
-      const int me = sp.scalar<T>(tid);
-      for (int i = 0; i < t.k; ++i)
-        if (s.id[i] == me) {
-          v = fmaf(power(single_z), c_in, s.total[i]);  // the first of them has the total
-          break;
+
+    // A tile: ROW vectors.  Buffer loads leave no branch between them, so that every tile is waited for by itself; those to LDS
+    // write there themselves, 64 vectors of a wavefront side by side.
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) void* LdsPtr;
+    int first = tid * 16;  // all of an offset in the lane's part: the bounds are of that
+    asm volatile("" : "+v"(first));  // offsets are made where they are used: held over the rows they are registers
+    auto load = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + i * ROW * 16, 0, 2);  // non-temporal
+      return make_uint4(x.x, x.y, x.z, x.w);
+    };
+    auto load_lds = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(s_tiles + i * ROW + wave * kWave), 16,
+                                               first + (NREG + i) * ROW * 16, 0, 0, 2);
+    };
+    uint4 reg[NREG];
+    float single_z;
+    {
+      const RowView<T> v(logits, ld, n_on > 0 ? row_of(0) : 0, vocab, n_on > 0);
+      single_z = tid < v.sp.n_scalar ? Row<T>::one(v.row + v.sp.template scalar<T>(tid)) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NREG; ++i) reg[i] = load(v.rsrc, i);
+#pragma unroll
+      for (int i = 0; i < NLDS; ++i) load_lds(v.rsrc, i);
+    }
+    // rows of weight 0, while the first row comes
+    for (int j = 0; j < n_off; ++j) {
+      const int row_i = (int)batch + __builtin_amdgcn_readlane(off_l, j);
+      const RowSpan sp(logits + (int64_t)row_i * ld, vocab, true, 0, 1);
+      T* const drow = dlogits + (int64_t)row_i * ld_d;
+      const float none[8] = {};
+      for (int q = tid; q < sp.n_vec; q += ROW) Packed<T>::store(drow + sp.head + (uint32_t)q * kPer, none);
+      if (tid < sp.n_scalar) Row<T>::store_one(drow + sp.scalar<T>(tid), 0.f);
+    }
+    for (int j = 0; j < n_on; ++j) {
+      const int row_i = row_of(j);
+      asm volatile("" : "+v"(first));  // offsets are made where they are used: held over the rows they are registers
+      const RowView<T> v(logits, ld, row_i, vocab);
+      const T* const body = v.row + v.sp.head;
+      T* const drow = dlogits + (int64_t)row_i * ld_d;
+      T* const dbody = drow + v.sp.head;
+      const int last_q = v.sp.n_vec - 1, tiles = (v.sp.n_vec + ROW - 1) / ROW;
+      // f(elements, vector) for every marked vector
+      const auto each_given = [&](int q, auto&& f) {  // f(element, number among the given) of vector q
+        const int id0 = v.sp.head + q * kPer;
+        for (int h = s.heads[q & (kBuckets - 1)]; h >= 0; h = s.next[h]) {
+          const int j = s.id[h] - id0;
+          if (j >= 0 && j < kPer) f(j, h);
         }
+      };
+      const auto read = [&](int q, float (&x)[8]) { Row<T>::template load<true>(body + (uint32_t)q * kPer, x); };
+      lds_barrier();  // the marks are there
+      const uint32_t mark_lo = s.marks[0][tid], mark_hi = s.marks[1][tid];
+      const auto marked = [&](int i) { return ((i < 32 ? mark_lo >> i : mark_hi >> (i - 32)) & 1) != 0; };
+      const auto take_out = [&](int q, float (&x)[8]) {
+        uint32_t off = 0;
+        each_given(q, [&](int j, int) { off |= 1u << j; });
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[j] = (off >> j & 1) ? -INFINITY : x[j];
+      };
+
+      // Statistics.  Against a reference c = ref k rounded an element is one instruction beside its exponential, and what c is off
+      // by is taken back at the end; the largest of a few logits will do as long as the sum stays in range.
+      const bool single_in = tid < v.sp.n_scalar && !(REST && (s.single >> tid & 1));
+      float ref = single_in ? single_z : -INFINITY;
+      if (tid <= last_q) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) ref = fmaxf(ref, Packed<T>::get(reg[0], j));
+      }
+      ref = wave_max(ref);
+      const float cc = ref * k;
+      float sum = 0.f;
+      bool plain = fabsf(cc) < kFar;
+      if (plain) {
+        float s4[4] = {};
+        const auto add = [&](const uint4& r) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -cc));
+        };
+#pragma unroll
+        for (int i = 0; i < NREG; ++i)
+          if (!marked(i) && i * ROW + tid <= last_q) add(reg[i]);
+        if (NREG < tiles) {
+          __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): the tiles in LDS are there
+          asm volatile("" ::: "memory");
+#pragma unroll 1
+          for (int i = NREG; i < tiles; ++i)
+            if (!marked(i) && i * ROW + tid <= last_q) add(i < NREG + NLDS ? s_tiles[(i - NREG) * ROW + tid] : load(v.rsrc, i));
+        }
+        for (uint64_t m = ((uint64_t)mark_hi << 32) | mark_lo; m != 0; m &= m - 1) {
+          const int q = __builtin_ctzll(m) * ROW + tid;
+          float x[8];
+          read(q, x);
+          if (REST) take_out(q, x);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[j], k, -cc));
+        }
+        if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
+        sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc));
+        plain = sum > 0x1p-60f && sum < 0x1p80f;
+      }
+      if (!plain) {  // another scale, logits far from 0, infinite, or not numbers: by differences from the largest, read again
+        Sum st{kLowest, 0.f};
+#pragma unroll 1
+        for (int q = tid; q <= last_q; q += ROW) {
+          float x[8];
+          read(q, x);
+          if (REST && marked(q / ROW)) take_out(q, x);
+          fold<kPer>(st, x, k);
+        }
+        if (single_in) {
+          const float x[8] = {single_z};
+          fold<1>(st, x, k);
+        }
+        ref = wave_max(st.M);
+        sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - ref) * k));
+      }
+      if (lane == 0) { s.red_m[wave] = ref; s.red_s[wave] = sum; }
+      lds_barrier();  // the statistics are there
+      lds_barrier();  // the row's constants are there
+
+      const float lse = s.lse, c_out = s.c_out;
+      const bool is_far = s.is_far != 0;
+      const auto power = [&](float x) { return __builtin_amdgcn_exp2f(is_far ? (x - lse) * k : fmaf(x, k, -lse)); };
+      for (uint64_t m = ((uint64_t)mark_hi << 32) | mark_lo; m != 0; m &= m - 1) {
+        const int q = __builtin_ctzll(m) * ROW + tid;
+        float x[8];
+        read(q, x);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[j] = power(x[j]) * c_out;
+        each_given(q, [&](int j, int h) {
+          const float y = s.b[h];
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) x[e] = e == j ? y : x[e];
+        });
+        Packed<T>::store(dbody + (uint32_t)q * kPer, x);
+      }
+      if (tid < v.sp.n_scalar) {
+        float x = power(single_z) * c_out;
+        if (s.single >> tid & 1) {
+          const int me = v.sp.template scalar<T>(tid);
+          for (int i = 0; i < t.k; ++i)
+            if (s.id[i] == me) {
+              x = s.b[i];  // the first of them has it all
+              break;
+            }
+        }
+        Row<T>::store_one(drow + v.sp.template scalar<T>(tid), x);
+      }
+      lds_barrier();  // the given tokens are written
+
+      // the rest of the row leaves, the next one comes
+      const bool more = j + 1 < n_on;
+      const RowView<T> next(logits, ld, more ? row_of(j + 1) : row_i, vocab, more);
+      const auto write = [&](const uint4& r, int i) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[j] = __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -lse)) * c_out;
+        Packed<T>::store(dbody + (int64_t)i * ROW * kPer + (uint32_t)tid * kPer, x);
+      };
+      if (is_far) {
+#pragma unroll 1
+        for (int q = tid; q <= last_q; q += ROW) {
+          if (marked(q / ROW)) continue;
+          float x[8];
+          read(q, x);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) x[j] = power(x[j]) * c_out;
+          Packed<T>::store(dbody + (uint32_t)q * kPer, x);
+        }
+      }
+      if (more && tid < next.sp.n_scalar) single_z = Row<T>::one(next.row + next.sp.template scalar<T>(tid));
+#pragma unroll
+      for (int i = 0; i < NREG; ++i) {
+        if (!is_far && !marked(i) && i * ROW + tid <= last_q) write(reg[i], i);
+        reg[i] = load(next.rsrc, i);
+      }
+#pragma unroll
+      for (int i = 0; i < NLDS; ++i) {
+        const int at = NREG + i;
+        if (!is_far && !marked(at) && at * ROW + tid <= last_q) write(s_tiles[i * ROW + tid], at);
+        asm volatile("" ::: "memory");  // the tile has been read
+        load_lds(next.rsrc, i);
+      }
+#pragma unroll 1
+      for (int i = NREG + NLDS; i < tiles; ++i)
+        if (!is_far && !marked(i) && i * ROW + tid <= last_q) write(load(v.rsrc, i), i);
     }
-    Row<T>::store_one(drow + sp.scalar<T>(tid), v);
+    // the loads that the last row has asked for come back before the tiles are asked for again
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("" ::: "memory");
   }
 }
 
@@ -860,19 +969,19 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
 
 namespace {
 
-// One workgroup per row with the row in registers and LDS.  Rows of up to 64 KB: 256 threads, four workgroups on a compute unit;
-// up to 128 KB: 512, two; longer: 1024, one, of which 400 KB are held and the rest is read twice.
-constexpr int kMaxRowVecs = 38912;  // a byte per vector in LDS beside the rest of a row
+// Rows of up to 64 KB: 192 threads that hold the row, four workgroups on a compute unit; up to 128 KB: 448, two; longer: 960, one, of
+// which 405 KB are held and the rest is read twice.
+constexpr int64_t kMaxRowVecs = kMaxTiles * 960;
 template <typename T, bool REST>
 int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const Teacher& t, const RowOut& out, void* dlogits, int64_t ld_d,
                 hipStream_t st) {
   const int64_t vecs = vocab / Row<T>::kPer;
-#define AXON_ROW(THREADS, NREG, NLDS, VECS)                                                                                         \
-  hipLaunchKernelGGL((distill_row_kernel<T, REST, THREADS, NREG, NLDS, VECS>), dim3((unsigned)n), dim3(THREADS), 0, st,             \
-                     static_cast<const T*>(logits), ld, (int)vocab, t, out, static_cast<T*>(dlogits), ld_d)
-  if (vecs <= 256 * 16) AXON_ROW(256, 16, 0, 256 * 16);
-  else if (vecs <= 512 * 16) AXON_ROW(512, 16, 0, 512 * 16);
-  else AXON_ROW(1024, 18, 7, kMaxRowVecs);
+#define AXON_ROW(ROW, NREG, NLDS, RESIDENT)                                                                                          \
+  hipLaunchKernelGGL((distill_row_kernel<T, REST, ROW, NREG, NLDS, 256 * RESIDENT>), dim3((unsigned)(n < 256 * RESIDENT ? n : 256 * RESIDENT)),       \
+                     dim3(ROW + kWave), 0, st, static_cast<const T*>(logits), ld, (int)vocab, t, out, static_cast<T*>(dlogits), ld_d)
+  if (vecs <= 192 * 22) AXON_ROW(192, 14, 8, 4);
+  else if (vecs <= 448 * 19) AXON_ROW(448, 14, 5, 2);
+  else AXON_ROW(960, 18, 9, 1);
 #undef AXON_ROW
   AXON_CHECK_LAUNCH();
   return AXON_OK;
