@@ -107,7 +107,7 @@ SIGNATURES: dict[str, tuple] = {
     "axon_controls_logprob_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "axon_distill_workspace_bytes": (_i64, [_i32, _i64, _i64]),
     "axon_distill_fwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _i64, _ptr, _i32, _i32, _f32, _f32, _ptr, _ptr,
-                                _ptr, _ptr, _ptr, _i64, _ptr]),
+                                _ptr, _ptr, _ptr, _i64, _i32, _ptr]),
     "axon_distill_bwd": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _i64, _ptr, _f32, _ptr, _ptr, _ptr, _i32, _ptr, _i64,
                                 _ptr]),
     "axon_distill_loss": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _i64, _ptr, _i32, _i32, _f32, _f32, _ptr, _ptr,

@@ -10,6 +10,7 @@
 // so that a row is its softmax statistics, k gathered logits, and one multiple of p_j for all tokens that are not given.  What
 // the student has left over is summed over these tokens themselves: 1 minus the rest has no digits where it matters.
 #include "logits_rows.h"
+#include <type_traits>
 
 namespace axon {
 
@@ -58,12 +59,12 @@ __device__ __forceinline__ void fold(Sum& a, const float (&z)[8], float k) {
 }
 
 // The bytes that say which elements of a share's vectors are given, and the same for the few elements outside vectors.
-struct Given {
+struct GivenBytes {
   uint32_t* bytes;   // LDS, a byte per vector of [q_lo, q_hi)
   uint32_t* single;  // LDS, a bit per element outside the vectors
 };
 template <typename T>
-__device__ __forceinline__ void mark_given(const Given& g, const Teacher& t, int64_t row, int vocab, const RowSpan& sp, int threads) {
+__device__ __forceinline__ void mark_given(const GivenBytes& g, const Teacher& t, int64_t row, int vocab, const RowSpan& sp, int threads) {
   constexpr int kPer = Row<T>::kPer;
   const int words = (sp.q_hi - sp.q_lo + 3) / 4;
   for (int i = threadIdx.x; i < words; i += threads) g.bytes[i] = 0;
@@ -87,7 +88,7 @@ __device__ __forceinline__ void mark_given(const Given& g, const Teacher& t, int
 // parts[row][part].
 template <typename T, bool REST>
 __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
-                                                               float4* __restrict__ parts) {
+                                                               float4* __restrict__ parts, int cached_from) {
   extern __shared__ __align__(16) uint32_t s_given[];
   __shared__ uint32_t s_single;
   __shared__ float red[2][kBlock / kWave];
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
   const T* row = logits + (int64_t)row_i * ld;
   constexpr int kPer = Row<T>::kPer;
   const RowSpan sp(row, vocab, true, part, n_parts);
-  if (REST) mark_given<T>(Given{s_given, &s_single}, t, row_i, vocab, sp, kBlock);
+  if (REST) mark_given<T>(GivenBytes{s_given, &s_single}, t, row_i, vocab, sp, kBlock);
   const uint8_t* const given = reinterpret_cast<const uint8_t*>(s_given);
   const T* body = row + sp.head;
   const float k = t.inv_t * kLog2e;
@@ -111,19 +112,24 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
     }
     fold<kPer>(st, v, k);
   };
-  int q = sp.q_lo + tid;
-  for (; q + kBlock < sp.q_hi; q += 2 * kBlock) {
-    float v0[8], v1[8];
-    Row<T>::load(body + (uint32_t)q * kPer, v0);
-    Row<T>::load(body + (uint32_t)(q + kBlock) * kPer, v1);
-    one(q, v0);
-    one(q + kBlock, v1);
-  }
-  for (; q < sp.q_hi; q += kBlock) {
-    float v[8];
-    Row<T>::load(body + (uint32_t)q * kPer, v);
-    one(q, v);
-  }
+  // rows from cached_from on are left in the cache in front of the memory, for a backward that follows
+  auto walk = [&](auto cached) {
+    constexpr bool kCached = decltype(cached)::value;
+    int q = sp.q_lo + tid;
+    for (; q + kBlock < sp.q_hi; q += 2 * kBlock) {
+      float v0[8], v1[8];
+      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v0);
+      Row<T>::template load<kCached>(body + (uint32_t)(q + kBlock) * kPer, v1);
+      one(q, v0);
+      one(q + kBlock, v1);
+    }
+    for (; q < sp.q_hi; q += kBlock) {
+      float v[8];
+      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v);
+      one(q, v);
+    }
+  };
+  if (row_i >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
   if (part == 0 && tid < sp.n_scalar && !(REST && (s_single >> tid & 1))) {
     const float v[8] = {Row<T>::one(row + sp.scalar<T>(tid))};
     fold<1>(st, v, k);
@@ -165,139 +171,130 @@ __device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) 
   return {(q == 0.0 ? 0.0 : b * q * (lq - lm)) + mine, mine};
 }
 
-struct FinishLds {
-  int id[kMaxIds];
-  double red[kBlock / kWave][4];
-  double total[4];
+// The given tokens of a row, in LDS.
+constexpr int kAgain = -2;
+struct Given {
+  int id[kMaxIds];               // -1: a filler
+  int16_t next[kMaxIds];         // kAgain: an id that has come before, or none; else -1, or the next of its chain
+  float a[kMaxIds], b[kMaxIds];  // the teacher's log-probabilities, then G; the logits, then what is written in their place
+  float best, best_q;            // the largest of either
+  double sum, sum_q;             // REST: of exp((z - best) / T), every token once, and of q; else of exp(lq - best_q)
 };
-__device__ __forceinline__ void sum4(double (&v)[4], FinishLds& s) {
-  const int wave = threadIdx.x / kWave;
-  __syncthreads();  // `total` of the sum before has been read
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = wave_sum_d(v[i]);
-  if ((threadIdx.x & (kWave - 1)) == 0 && wave < kBlock / kWave)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s.red[wave][i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = 0.0;
-    for (int w = 0; w < kBlock / kWave; ++w) v[i] += s.red[w][i];
-  }
-}
-
-// The outcomes of a row, given the statistics of the row (or, REST, of what is not given): losses, G, and the row's coefficients.
-// By the first kBlock threads of a workgroup; the others come along to the barriers.
+// By one wavefront; everything that can be known before the row's statistics.
 template <typename T, bool REST>
-__device__ __forceinline__ void finish_row(int row_i, const T* row, int vocab, const Teacher& t, const RowOut& out, float M_in, double s_in,
-                                           FinishLds& lds) {
-  constexpr int kSlots = kMaxIds / kBlock;
-  const int tid = threadIdx.x;
-  const bool mine = tid < kBlock;
-  const double inv_t = (double)t.inv_t;
-  float z[kSlots];
-  double lq[kSlots];
-  int id[kSlots];
-  bool first[kSlots];
-  float M = M_in;
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * kBlock;
-    id[u] = -1;
-    z[u] = -INFINITY;
-    lq[u] = -INFINITY;
-    if (mine && i < t.k) {
-      id[u] = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
-      if (id[u] >= 0) {
-        z[u] = Row<T>::one(row + id[u]);
-        lq[u] = (double)t.logprobs[(int64_t)row_i * t.k + i];
-      }
-      lds.id[i] = id[u];
-    }
+__device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_i, const T* row, int vocab, int lane) {
+  for (int i = lane; i < t.k; i += kWave) {
+    const int id = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
+    const float lq = t.logprobs[(int64_t)row_i * t.k + i], z = Row<T>::one(row + max(id, 0));
+    s.id[i] = id;
+    s.a[i] = id < 0 ? -INFINITY : lq;
+    s.b[i] = id < 0 ? -INFINITY : z;
   }
-  __syncthreads();
-  // the largest of the given ones, and of their teacher's log-probabilities, for all
+  wave_sync();
+  for (int i = lane; i < t.k; i += kWave) {
+    const int id = s.id[i];
+    bool first = id >= 0;
+#pragma unroll 8
+    for (int j = 0; j < t.k; ++j) first = first && !(j < i && s.id[j] == id);
+    s.next[i] = first ? -1 : kAgain;
+  }
   float best = -INFINITY, best_q = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    best = fmaxf(best, z[u]);
-    best_q = fmaxf(best_q, (float)lq[u]);
-    first[u] = id[u] >= 0;
-    if (REST && id[u] >= 0)
-      for (int j = 0; j < tid + u * kBlock; ++j) first[u] = first[u] && lds.id[j] != id[u];
+  for (int i = lane; i < t.k; i += kWave) {
+    best = fmaxf(best, s.b[i]);
+    best_q = fmaxf(best_q, s.a[i]);
   }
   best = wave_max(best);
   best_q = wave_max(best_q);
-  if (mine && (tid & (kWave - 1)) == 0) { lds.red[tid / kWave][0] = best; lds.red[tid / kWave][1] = best_q; }
-  __syncthreads();
-  for (int w = 0; w < kBlock / kWave; ++w) {
-    M = fmaxf(M, (float)lds.red[w][0]);
-    best_q = fmaxf(best_q, (float)lds.red[w][1]);
-  }
-  const double scale_in = exp64(((double)M_in - (double)M) * inv_t);  // of the statistics to the reference M
-  double v[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    if (id[u] < 0) continue;
-    if (REST && first[u]) v[0] += exp64(((double)z[u] - (double)M) * inv_t);
-    if (t.tail == AXON_DISTILL_RENORMALIZE) v[1] += exp64(lq[u] - (double)best_q);
-    if (REST) v[2] += exp64(lq[u]);
-  }
-  sum4(v, lds);
-  const double s_rest = s_in * scale_in, s = REST ? s_rest + v[0] : s_rest;
-  const double ln_s = s > 0.0 ? log64(s) : (double)NAN;  // a row of -inf alone has no softmax
-  const double norm_q = t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log64(v[1]) : 0.0;
-  const double q_rest = fmax(1.0 - v[2], 0.0), lp_rest = log64(s_rest) - ln_s;
-  double w[4] = {0.0, 0.0, 0.0, 0.0};  // loss, sum of G, covered
-#pragma unroll
-  for (int u = 0; u < kSlots; ++u) {
-    const int i = tid + u * kBlock;
-    if (!mine || i >= t.k) continue;
-    Term o{0.0, 0.0};
-    if (id[u] >= 0) {
-      const double lp = ((double)z[u] - (double)M) * inv_t - ln_s;
-      o = outcome(t, lq[u] - norm_q, lp);
-      w[2] += exp64(lp);
+  double sum = 0.0, sum_q = 0.0;
+  if (REST || t.tail == AXON_DISTILL_RENORMALIZE) {
+#pragma unroll 1
+    for (int i = lane; i < t.k; i += kWave) {
+      if (s.id[i] < 0) continue;
+      if (REST && s.next[i] != kAgain) sum += exp64(((double)s.b[i] - (double)best) * (double)t.inv_t);
+      sum_q += exp64((double)s.a[i] - (REST ? 0.0 : (double)best_q));
     }
-    w[0] += o.loss;
-    w[1] += o.g;
-    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
+    if (REST) sum = wave_sum_d(sum);
+    sum_q = wave_sum_d(sum_q);
   }
-  sum4(w, lds);
-  if (tid != 0) return;
-  double out_scale = 0.0;
-  if (REST) {
-    const Term o = outcome(t, log64(q_rest), lp_rest);
-    w[0] += o.loss;
-    w[1] += o.g;
-    out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
+  if (lane == 0) {
+    s.best = best;
+    s.best_q = best_q;
+    s.sum = sum;
+    s.sum_q = sum_q;
   }
-  const float lse = (float)((double)M + ln_s / inv_t);
-  out.losses[row_i] = (float)w[0];
-  out.covered[row_i] = (float)w[2];
-  float* const c = out.coef + row_i;
-  c[(int64_t)kLse * out.n] = lse;
-  c[(int64_t)kRest * out.n] = (float)((((double)M - (double)lse) * inv_t + ln_s) * 1.4426950408889634);
-  c[(int64_t)kOut * out.n] = (float)(out_scale - w[1]);
-  c[(int64_t)kIn * out.n] = (float)-w[1];
+  wave_sync();
 }
 
-// Rows whose statistics several workgroups have left, or one, by a workgroup per row.
+// The outcomes of a row in 64 bits, by one wavefront, from the statistics that its lanes have of parts of the row (REST: of what is not
+// given): losses, G (also in s.a), and the row's coefficients.
+struct RowCoefs { float lse, rest, c_out, c_in; };
+template <bool REST>
+__device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const RowOut& out, int row_i, float part_m, double part_s, int lane) {
+  const float k = t.inv_t * kLog2e;
+  const double inv_t = (double)t.inv_t;
+  const float best = s.best, M = fmaxf(wave_max(part_m), best);
+  // the whole range of 64 bits: what is left may be next to nothing
+  const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
+  const double s_rest = wave_sum_d(ldexp(part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
+  const double s_all = REST && best > -INFINITY ? s_rest + s.sum * exp64(((double)best - (double)M) * inv_t) : s_rest;
+  const double ln_s = s_all > 0.0 ? log64(s_all) : (double)NAN;  // a row of -inf alone has no softmax
+  const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE ? (double)s.best_q + log64(s.sum_q) : 0.0;
+  double loss = 0.0, sum_g = 0.0, covered = 0.0;
+#pragma unroll 1
+  for (int i = lane; i < t.k; i += kWave) {
+    Term o{0.0, 0.0};
+    if (s.id[i] >= 0) {
+      const double lp = ((double)s.b[i] - (double)M) * inv_t - ln_s;
+      o = outcome(t, (double)s.a[i] - norm_q, lp);
+      covered += exp64(lp);
+    }
+    loss += o.loss;
+    sum_g += o.g;
+    s.a[i] = (float)o.g;
+    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
+  }
+  loss = wave_sum_d(loss);
+  sum_g = wave_sum_d(sum_g);
+  covered = wave_sum_d(covered);
+  double out_scale = 0.0;
+  if (REST) {
+    const double lp_rest = log64(s_rest) - ln_s;
+    const Term o = outcome(t, log64(fmax(1.0 - s.sum_q, 0.0)), lp_rest);
+    loss += o.loss;
+    sum_g += o.g;
+    out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
+  }
+  RowCoefs r;
+  r.lse = (float)((double)M + ln_s / inv_t);
+  r.rest = (float)((((double)M - (double)r.lse) * inv_t + ln_s) * 1.4426950408889634);
+  r.c_out = (float)(out_scale - sum_g);
+  r.c_in = (float)-sum_g;
+  if (lane == 0) {
+    out.losses[row_i] = (float)loss;
+    out.covered[row_i] = (float)covered;
+    float* const c = out.coef + row_i;
+    c[(int64_t)kLse * out.n] = r.lse;
+    c[(int64_t)kRest * out.n] = r.rest;
+    c[(int64_t)kOut * out.n] = r.c_out;
+    c[(int64_t)kIn * out.n] = r.c_in;
+  }
+  wave_sync();
+  return r;
+}
+
+// The end of rows whose statistics are there, by a wavefront per row.
 template <typename T, bool REST>
-__global__ __launch_bounds__(kBlock) void distill_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
-                                                                const float4* __restrict__ parts, RowOut out) {
-  __shared__ FinishLds lds;
-  const int row_i = blockIdx.x, lane = threadIdx.x & (kWave - 1);
+__global__ __launch_bounds__(kWave) void distill_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
+                                                               const float4* __restrict__ parts, RowOut out) {
+  __shared__ Given s;
+  const int row_i = blockIdx.x, lane = threadIdx.x;
   if (t.weights != nullptr && t.weights[row_i] == 0.f) {
-    if (threadIdx.x == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
+    if (lane == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
     return;
   }
-  float M = kLowest;
-  double s = 0.0;
   const float4 p = lane < n_parts ? parts[(int64_t)row_i * n_parts + lane] : make_float4(kLowest, 0.f, 0.f, 0.f);
-  M = wave_max(p.x);
-  s = wave_sum_d(((double)p.y + (double)p.z) * exp64(((double)p.x - (double)M) * (double)t.inv_t));
-  finish_row<T, REST>(row_i, logits + (int64_t)row_i * ld, vocab, t, out, M, s, lds);
+  fetch_given<T, REST>(s, t, row_i, logits + (int64_t)row_i * ld, vocab, lane);
+  finish_row<REST>(s, t, out, row_i, p.x, (double)p.y + (double)p.z, lane);
 }
 
 // Workgroup (row, part): dlogits of its share.  The row is streamed without a look at the given tokens; their few elements are
@@ -394,21 +391,21 @@ __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, i
 }
 
 // The loss and its gradient from ONE read of a row.  A workgroup walks rows; it holds a row, NREG 16-byte vectors of every thread in
-// registers and NLDS in LDS, from its statistics to its gradient (what is longer is read again), and asks for the next row's vectors
-// as those of the row leave.  ROW threads do that; the 64 threads behind them look after the given tokens: where they lie while the
-// row is on its way, the outcomes in 64 bits when its statistics are there.
-// A thread's vectors that hold a given token are marked by a bit; the passes over the row leave them out, and a short loop takes
-// them one by one, with the tokens found through a hash of the vector's number.
-constexpr int kBuckets = 256, kAgain = -2, kMaxTiles = 64;
+// registers and NLDS in LDS, from its statistics to its gradient (what is longer is read again).  As the vectors of a row leave, those
+// of the next are asked for in their place, and looked at as they come: between the two there are only the sums over the workgroup and
+// the outcomes.  ROW threads do that; the wavefront behind them looks after the given tokens: where they lie, two rows ahead, and the
+// outcomes when a row's statistics are there.
+// A thread's vectors that hold a given token are marked by a bit; statistics leave them out and take them one by one, with the tokens
+// found through a hash of the vector's number, and the tokens' gradients are written over the vector's by the thread that has written it.
+constexpr int kBuckets = 256, kMaxTiles = 64, kAhead = 3;
 template <int ROW>
 struct RowLds {
-  uint32_t marks[2][ROW];            // bit i % 32 of word i / 32: this thread's vector of tile i holds a given token
-  int id[kMaxIds], heads[kBuckets];  // chains of the ids that come for the first time
-  int16_t next[kMaxIds];             // -1: the last of its chain, kAgain: an id that has come before, or none
-  float a[kMaxIds], b[kMaxIds];      // the teacher's log-probabilities, then G; the logits, then what is written in their place
+  Given given[kAhead];
+  int heads[kAhead][kBuckets];  // chains of the ids that come for the first time
+  uint32_t marks[kAhead][2][ROW];  // bit i % 32 of word i / 32: this thread's vector of tile i holds a given token
+  uint32_t single[kAhead];         // a bit per element outside the vectors
   float red_m[ROW / kWave], red_s[ROW / kWave];
-  uint32_t single;                   // a bit per element outside the vectors
-  float lse, c_out, c_in;
+  float lse, c_out;
   int is_far;
 };
 
@@ -453,141 +450,55 @@ struct RowView {
         rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row + sp.head), 0, wanted ? sp.n_vec * 16 : 0, 0x00020000)) {}
 };
 
-// The threads that look after the given tokens of a row (one wavefront).
+// Where the given tokens of a row lie, by one wavefront.
 template <typename T, bool REST, int ROW>
-struct Outcomes {
-  RowLds<ROW>& s;
-  const Teacher& t;
-  const RowOut& out;
-  int vocab, lane;
-
-  // Where the given tokens lie.
-  __device__ __forceinline__ void mark(int row_i, const RowView<T>& v) {
-    constexpr int kPer = Row<T>::kPer;
-    for (int i = lane; i < ROW; i += kWave) s.marks[0][i] = s.marks[1][i] = 0;
-    for (int i = lane; i < kBuckets; i += kWave) s.heads[i] = -1;
-    if (lane == 0) s.single = 0;
-    for (int i = lane; i < t.k; i += kWave) {
-      const int id = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
-      const float lq = t.logprobs[(int64_t)row_i * t.k + i], z = Row<T>::one(v.row + max(id, 0));
-      s.id[i] = id;
-      s.a[i] = id < 0 ? -INFINITY : lq;
-      s.b[i] = id < 0 ? -INFINITY : z;
-    }
-    wave_sync();
-    for (int i = lane; i < t.k; i += kWave) {
-      const int id = s.id[i];
-      bool first = id >= 0;
-#pragma unroll 8
-      for (int j = 0; j < t.k; ++j) first = first && !(j < i && s.id[j] == id);
-      if (!first) {
-        s.next[i] = kAgain;
-        continue;
-      }
-      const int in = id - v.sp.head, q = in >= 0 ? in / kPer : -1;
-      if (q >= 0 && q < v.sp.n_vec) {
-        atomicOr(&s.marks[q / ROW / 32][q % ROW], 1u << (q / ROW % 32));
-        s.next[i] = (int16_t)atomicExch(s.heads + (q & (kBuckets - 1)), i);
-      } else {
-        s.next[i] = -1;
-        atomicOr(&s.single, 1u << (in < 0 ? id : id - v.sp.n_vec * kPer));
-      }
-    }
-    wave_sync();
-  }
-
-  // The outcomes from the statistics of the row (REST: of what is not given), and what is written in the given tokens' places.
-  __device__ __forceinline__ void finish(int row_i, float weight) {
-    const float k = t.inv_t * kLog2e, g = weight * t.inv_t;
-    const double inv_t = (double)t.inv_t;
-    constexpr int kRowWaves = ROW / kWave;
-    const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
-    float M = part_m, best_q = -INFINITY;
-    for (int i = lane; i < t.k; i += kWave) {
-      M = fmaxf(M, s.b[i]);
-      best_q = fmaxf(best_q, s.a[i]);
-    }
-    M = wave_max(M);
-    best_q = wave_max(best_q);
-    double e_first = 0.0, e_norm = 0.0, e_q = 0.0;
-    if (REST || t.tail == AXON_DISTILL_RENORMALIZE) {
-#pragma unroll 1
-      for (int i = lane; i < t.k; i += kWave) {
-        if (s.id[i] < 0) continue;
-        if (REST && s.next[i] != kAgain) e_first += exp64(((double)s.b[i] - (double)M) * inv_t);
-        const double e = exp64((double)s.a[i] - (REST ? 0.0 : (double)best_q));
-        if (REST) e_q += e; else e_norm += e;
-      }
-      if (REST) {
-        e_first = wave_sum_d(e_first);
-        e_q = wave_sum_d(e_q);
-      } else {
-        e_norm = wave_sum_d(e_norm);
-      }
-    }
-    // the whole range of 64 bits: what is left may be next to nothing
-    const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
-    const double s_rest = wave_sum_d(ldexp((double)part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
-    const double s_all = REST ? s_rest + e_first : s_rest;
-    const double ln_s = s_all > 0.0 ? log64(s_all) : (double)NAN;  // a row of -inf alone has no softmax
-    const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE ? (double)best_q + log64(e_norm) : 0.0;
-    double loss = 0.0, sum_g = 0.0, covered = 0.0;
-#pragma unroll 1
-    for (int i = lane; i < t.k; i += kWave) {
-      Term o{0.0, 0.0};
-      if (s.id[i] >= 0) {
-        const double lp = ((double)s.b[i] - (double)M) * inv_t - ln_s;
-        o = outcome(t, (double)s.a[i] - norm_q, lp);
-        covered += exp64(lp);
-      }
-      loss += o.loss;
-      sum_g += o.g;
-      s.a[i] = (float)o.g;
-      out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
-    }
-    loss = wave_sum_d(loss);
-    sum_g = wave_sum_d(sum_g);
-    covered = wave_sum_d(covered);
-    double out_scale = 0.0;
-    if (REST) {
-      const double lp_rest = log64(s_rest) - ln_s;
-      const Term o = outcome(t, log64(fmax(1.0 - e_q, 0.0)), lp_rest);
-      loss += o.loss;
-      sum_g += o.g;
-      out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
-    }
-    const float lse = (float)((double)M + ln_s / inv_t);
-    const float rest = (float)((((double)M - (double)lse) * inv_t + ln_s) * 1.4426950408889634);
-    const float coef_out = (float)(out_scale - sum_g), coef_in = (float)-sum_g;
-    // p = 2^(z k - off) f with off = lse k rounded; far from 0 by the difference from lse
-    const float off = lse * k;
-    const bool is_far = !(fabsf(off) < kFar);
-    const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)lse * (double)k)) - rest);
-    const float base = is_far ? lse : off, c_in = g * coef_in * f;
-    if (lane == 0) {
-      out.losses[row_i] = (float)loss;
-      out.covered[row_i] = (float)covered;
-      float* const c = out.coef + row_i;
-      c[(int64_t)kLse * out.n] = lse;
-      c[(int64_t)kRest * out.n] = rest;
-      c[(int64_t)kOut * out.n] = coef_out;
-      c[(int64_t)kIn * out.n] = coef_in;
-      s.lse = base;
-      s.is_far = is_far;
-      s.c_out = g * coef_out * f;
-      s.c_in = c_in;
-    }
-    wave_sync();
-    for (int i = lane; i < t.k; i += kWave) {
-      if (s.next[i] == kAgain) continue;
-      float total = s.a[i];
-#pragma unroll 8
-      for (int j = i + 1; j < t.k; ++j) total += s.id[j] == s.id[i] ? s.a[j] : 0.f;
-      const float z = s.b[i], p = __builtin_amdgcn_exp2f(is_far ? (z - base) * k : fmaf(z, k, -base));
-      s.b[i] = fmaf(p, c_in, g * total);
+__device__ __forceinline__ void mark_row(RowLds<ROW>& s, int buf, const Teacher& t, int row_i, const RowView<T>& v, int vocab, int lane) {
+  constexpr int kPer = Row<T>::kPer;
+  Given& g = s.given[buf];
+  for (int i = lane; i < ROW; i += kWave) s.marks[buf][0][i] = s.marks[buf][1][i] = 0;
+  for (int i = lane; i < kBuckets; i += kWave) s.heads[buf][i] = -1;
+  if (lane == 0) s.single[buf] = 0;
+  fetch_given<T, REST>(g, t, row_i, v.row, vocab, lane);
+  for (int i = lane; i < t.k; i += kWave) {
+    if (g.next[i] == kAgain) continue;
+    const int id = g.id[i], in = id - v.sp.head, q = in >= 0 ? in / kPer : -1;
+    if (q >= 0 && q < v.sp.n_vec) {
+      atomicOr(&s.marks[buf][q / ROW / 32][q % ROW], 1u << (q / ROW % 32));
+      g.next[i] = (int16_t)atomicExch(&s.heads[buf][q & (kBuckets - 1)], i);
+    } else {
+      atomicOr(&s.single[buf], 1u << (in < 0 ? id : id - v.sp.n_vec * kPer));
     }
   }
-};
+  wave_sync();
+}
+
+// The constants of a row for its threads, and what is written in the given tokens' places (in given.b), by one wavefront.
+template <bool REST, int ROW>
+__device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teacher& t, const RowOut& out, int row_i, float weight, int lane) {
+  constexpr int kRowWaves = ROW / kWave;
+  Given& gv = s.given[buf];
+  const float k = t.inv_t * kLog2e, g = weight * t.inv_t;
+  const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
+  const RowCoefs r = finish_row<REST>(gv, t, out, row_i, part_m, (double)part_s, lane);
+  // p = 2^(z k - off) f with off = lse k rounded; far from 0 by the difference from lse
+  const float off = r.lse * k;
+  const bool is_far = !(fabsf(off) < kFar);
+  const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)r.lse * (double)k)) - r.rest);
+  const float base = is_far ? r.lse : off, c_in = g * r.c_in * f;
+  if (lane == 0) {
+    s.lse = base;
+    s.is_far = is_far;
+    s.c_out = g * r.c_out * f;
+  }
+  for (int i = lane; i < t.k; i += kWave) {
+    if (gv.next[i] == kAgain) continue;
+    float total = gv.a[i];
+#pragma unroll 8
+    for (int j = i + 1; j < t.k; ++j) total += gv.id[j] == gv.id[i] ? gv.a[j] : 0.f;
+    const float z = gv.b[i], p = __builtin_amdgcn_exp2f(is_far ? (z - base) * k : fmaf(z, k, -base));
+    gv.b[i] = fmaf(p, c_in, g * total);
+  }
+}
 
 // GRID: the most workgroups of a launch.
 template <typename T, bool REST, int ROW, int NREG, int NLDS, int GRID>
@@ -630,16 +541,20 @@ __global__ __launch_bounds__(ROW + kWave, 4) void distill_row_kernel(const T* __
     const auto row_of = [&](int j) { return (int)batch + __builtin_amdgcn_readlane(on_l, j); };
 
     if (wave == ROW / kWave) {
-      Outcomes<T, REST, ROW> o{s, t, out, vocab, lane};
       if (lane < n_off) out.losses[batch + off_l] = out.covered[batch + off_l] = 0.f;
+      const auto mark = [&](int j) {
+        if (j < n_on) mark_row<T, REST, ROW>(s, j % kAhead, t, row_of(j), RowView<T>(logits, ld, row_of(j), vocab), vocab, lane);
+      };
+      mark(0);
+      lds_barrier();  // the marks of row 0
+      mark(1);
       for (int j = 0; j < n_on; ++j) {
         const int row_i = row_of(j);
-        o.mark(row_i, RowView<T>(logits, ld, row_i, vocab));
-        lds_barrier();  // the marks are there
-        lds_barrier();  // the statistics are there
-        o.finish(row_i, t.weights[row_i]);
-        lds_barrier();  // the row's constants are there
-        lds_barrier();  // the given tokens are written
+        const float weight = t.weights[row_i];
+        lds_barrier();  // the statistics of row j, the marks of row j + 1
+        settle_row<REST, ROW>(s, j % kAhead, t, out, row_i, weight, lane);
+        lds_barrier();  // its constants
+        mark(j + 2);
       }
       continue;
     }
@@ -650,16 +565,92 @@ __global__ __launch_bounds__(ROW + kWave, 4) void distill_row_kernel(const T* __
     typedef __attribute__((address_space(3))) void* LdsPtr;
     int first = tid * 16;  // all of an offset in the lane's part: the bounds are of that
     asm volatile("" : "+v"(first));  // offsets are made where they are used: held over the rows they are registers
-    auto load = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
+    const auto load = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
       const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + i * ROW * 16, 0, 2);  // non-temporal
       return make_uint4(x.x, x.y, x.z, x.w);
     };
-    auto load_lds = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(s_tiles + i * ROW + wave * kWave), 16,
-                                               first + (NREG + i) * ROW * 16, 0, 0, 2);
+    const auto load_cached = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {  // what is read twice
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + i * ROW * 16, 0, 0);
+      return make_uint4(x.x, x.y, x.z, x.w);
+    };
+    const auto load_lds = [&](__amdgpu_buffer_rsrc_t rsrc, int i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(s_tiles + i * ROW + wave * kWave), 16, first + (NREG + i) * ROW * 16, 0, 0, 2);
     };
     uint4 reg[NREG];
     float single_z;
+
+    // Statistics of a row.  Against a reference c = ref k rounded (ref: the largest of its given tokens' logits) an element is one
+    // instruction beside its exponential, and what c is off by is taken back at the end.
+    float s4[4], cc = 0.f, ref = 0.f;
+    uint32_t mark_lo = 0, mark_hi = 0;
+    const auto marked = [&](int i) { return REST && ((i < 32 ? mark_lo >> i : mark_hi >> (i - 32)) & 1) != 0; };
+    const auto begin_stats = [&](int j) {
+      const int buf = j % kAhead;
+      ref = s.given[buf].best > -INFINITY ? s.given[buf].best : 0.f;
+      cc = ref * k;
+      mark_lo = s.marks[buf][0][tid];
+      mark_hi = s.marks[buf][1][tid];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s4[i] = 0.f;
+    };
+    const auto add = [&](const uint4& r) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -cc));
+    };
+    const auto each_given = [&](int buf, int id0, int q, auto&& f) {  // f(element, number among the given) of vector q
+      for (int h = s.heads[buf][q & (kBuckets - 1)]; h >= 0; h = s.given[buf].next[h]) {
+        const int e = s.given[buf].id[h] - id0;
+        if (e >= 0 && e < kPer) f(e, h);
+      }
+    };
+    const auto read_left = [&](int buf, const RowView<T>& v, int q, float (&x)[8]) {  // vector q without what is given
+      Row<T>::template load<true>(v.row + v.sp.head + (uint32_t)q * kPer, x);
+      uint32_t off = 0;
+      if (REST) each_given(buf, v.sp.head + q * kPer, q, [&](int e, int) { off |= 1u << e; });
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] = (off >> e & 1) ? -INFINITY : x[e];
+    };
+    const auto add_marked = [&](int j, const RowView<T>& v) {
+      if (!REST) return;
+      for (uint64_t m = ((uint64_t)mark_hi << 32) | mark_lo; m != 0; m &= m - 1) {
+        float x[8];
+        read_left(j % kAhead, v, __builtin_ctzll(m) * ROW + tid, x);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) s4[e & 3] += __builtin_amdgcn_exp2f(fmaf(x[e], k, -cc));
+      }
+    };
+    const auto add_beyond = [&](const RowView<T>& v) {  // tiles that are not held
+      const int last_q = v.sp.n_vec - 1, tiles = last_q / ROW + 1;
+#pragma unroll 1
+      for (int i = NREG + NLDS; i < tiles; i += 2) {
+        const uint4 r0 = load_cached(v.rsrc, i), r1 = load_cached(v.rsrc, i + 1);
+        if (i * ROW + tid <= last_q && !marked(i)) add(r0);
+        if ((i + 1) * ROW + tid <= last_q && !marked(i + 1)) add(r1);
+      }
+    };
+    const auto end_stats = [&](int j, const RowView<T>& v) {
+      const bool single_in = tid < v.sp.n_scalar && !(REST && (s.single[j % kAhead] >> tid & 1));
+      if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
+      float sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc)), m = ref;
+      if (!(fabsf(cc) < kFar && sum > 0x1p-60f && sum < 0x1p80f)) {
+        // another scale, logits far from 0, infinite, or not numbers: by differences from the largest, read again
+        Sum st{kLowest, 0.f};
+#pragma unroll 1
+        for (int q = tid; q < v.sp.n_vec; q += ROW) {
+          float x[8];
+          read_left(j % kAhead, v, q, x);
+          fold<kPer>(st, x, k);
+        }
+        if (single_in) {
+          const float x[8] = {single_z};
+          fold<1>(st, x, k);
+        }
+        m = wave_max(st.M);
+        sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
+      }
+      if (lane == 0) { s.red_m[wave] = m; s.red_s[wave] = sum; }
+    };
+
     {
       const RowView<T> v(logits, ld, n_on > 0 ? row_of(0) : 0, vocab, n_on > 0);
       single_z = tid < v.sp.n_scalar ? Row<T>::one(v.row + v.sp.template scalar<T>(tid)) : -INFINITY;
@@ -667,172 +658,120 @@ __global__ __launch_bounds__(ROW + kWave, 4) void distill_row_kernel(const T* __
       for (int i = 0; i < NREG; ++i) reg[i] = load(v.rsrc, i);
 #pragma unroll
       for (int i = 0; i < NLDS; ++i) load_lds(v.rsrc, i);
-    }
-    // rows of weight 0, while the first row comes
-    for (int j = 0; j < n_off; ++j) {
-      const int row_i = (int)batch + __builtin_amdgcn_readlane(off_l, j);
-      const RowSpan sp(logits + (int64_t)row_i * ld, vocab, true, 0, 1);
-      T* const drow = dlogits + (int64_t)row_i * ld_d;
-      const float none[8] = {};
-      for (int q = tid; q < sp.n_vec; q += ROW) Packed<T>::store(drow + sp.head + (uint32_t)q * kPer, none);
-      if (tid < sp.n_scalar) Row<T>::store_one(drow + sp.scalar<T>(tid), 0.f);
-    }
-    for (int j = 0; j < n_on; ++j) {
-      const int row_i = row_of(j);
-      asm volatile("" : "+v"(first));  // offsets are made where they are used: held over the rows they are registers
-      const RowView<T> v(logits, ld, row_i, vocab);
-      const T* const body = v.row + v.sp.head;
-      T* const drow = dlogits + (int64_t)row_i * ld_d;
-      T* const dbody = drow + v.sp.head;
-      const int last_q = v.sp.n_vec - 1, tiles = (v.sp.n_vec + ROW - 1) / ROW;
-      // f(elements, vector) for every marked vector
-      const auto each_given = [&](int q, auto&& f) {  // f(element, number among the given) of vector q
-        const int id0 = v.sp.head + q * kPer;
-        for (int h = s.heads[q & (kBuckets - 1)]; h >= 0; h = s.next[h]) {
-          const int j = s.id[h] - id0;
-          if (j >= 0 && j < kPer) f(j, h);
-        }
-      };
-      const auto read = [&](int q, float (&x)[8]) { Row<T>::template load<true>(body + (uint32_t)q * kPer, x); };
-      lds_barrier();  // the marks are there
-      const uint32_t mark_lo = s.marks[0][tid], mark_hi = s.marks[1][tid];
-      const auto marked = [&](int i) { return ((i < 32 ? mark_lo >> i : mark_hi >> (i - 32)) & 1) != 0; };
-      const auto take_out = [&](int q, float (&x)[8]) {
-        uint32_t off = 0;
-        each_given(q, [&](int j, int) { off |= 1u << j; });
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) x[j] = (off >> j & 1) ? -INFINITY : x[j];
-      };
-
-      // Statistics.  Against a reference c = ref k rounded an element is one instruction beside its exponential, and what c is off
-      // by is taken back at the end; the largest of a few logits will do as long as the sum stays in range.
-      const bool single_in = tid < v.sp.n_scalar && !(REST && (s.single >> tid & 1));
-      float ref = single_in ? single_z : -INFINITY;
-      if (tid <= last_q) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) ref = fmaxf(ref, Packed<T>::get(reg[0], j));
+      // rows of weight 0, while the first row comes
+      for (int j = 0; j < n_off; ++j) {
+        const int row_i = (int)batch + __builtin_amdgcn_readlane(off_l, j);
+        const RowSpan sp(logits + (int64_t)row_i * ld, vocab, true, 0, 1);
+        T* const drow = dlogits + (int64_t)row_i * ld_d;
+        const float none[8] = {};
+        for (int q = tid; q < sp.n_vec; q += ROW) Packed<T>::store(drow + sp.head + (uint32_t)q * kPer, none);
+        if (tid < sp.n_scalar) Row<T>::store_one(drow + sp.scalar<T>(tid), 0.f);
       }
-      ref = wave_max(ref);
-      const float cc = ref * k;
-      float sum = 0.f;
-      bool plain = fabsf(cc) < kFar;
-      if (plain) {
-        float s4[4] = {};
-        const auto add = [&](const uint4& r) {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -cc));
-        };
+      lds_barrier();  // the marks of row 0
+      if (n_on > 0) {
+        begin_stats(0);
+        const int last_q = v.sp.n_vec - 1;
 #pragma unroll
         for (int i = 0; i < NREG; ++i)
-          if (!marked(i) && i * ROW + tid <= last_q) add(reg[i]);
-        if (NREG < tiles) {
-          __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): the tiles in LDS are there
-          asm volatile("" ::: "memory");
+          if (i * ROW + tid <= last_q && !marked(i)) add(reg[i]);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the tiles in LDS are there
+        asm volatile("" ::: "memory");
 #pragma unroll 1
-          for (int i = NREG; i < tiles; ++i)
-            if (!marked(i) && i * ROW + tid <= last_q) add(i < NREG + NLDS ? s_tiles[(i - NREG) * ROW + tid] : load(v.rsrc, i));
-        }
-        for (uint64_t m = ((uint64_t)mark_hi << 32) | mark_lo; m != 0; m &= m - 1) {
-          const int q = __builtin_ctzll(m) * ROW + tid;
-          float x[8];
-          read(q, x);
-          if (REST) take_out(q, x);
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[j], k, -cc));
-        }
-        if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
-        sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc));
-        plain = sum > 0x1p-60f && sum < 0x1p80f;
+        for (int i = 0; i < NLDS; ++i)
+          if ((NREG + i) * ROW + tid <= last_q && !marked(NREG + i)) add(s_tiles[i * ROW + tid]);
+        add_beyond(v);
+        add_marked(0, v);
+        end_stats(0, v);
       }
-      if (!plain) {  // another scale, logits far from 0, infinite, or not numbers: by differences from the largest, read again
-        Sum st{kLowest, 0.f};
-#pragma unroll 1
-        for (int q = tid; q <= last_q; q += ROW) {
-          float x[8];
-          read(q, x);
-          if (REST && marked(q / ROW)) take_out(q, x);
-          fold<kPer>(st, x, k);
-        }
-        if (single_in) {
-          const float x[8] = {single_z};
-          fold<1>(st, x, k);
-        }
-        ref = wave_max(st.M);
-        sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - ref) * k));
-      }
-      if (lane == 0) { s.red_m[wave] = ref; s.red_s[wave] = sum; }
-      lds_barrier();  // the statistics are there
-      lds_barrier();  // the row's constants are there
-
+    }
+    for (int j = 0; j < n_on; ++j) {
+      const int buf = j % kAhead, row_i = row_of(j);
+      asm volatile("" : "+v"(first));
+      lds_barrier();  // the statistics of row j, the marks of row j + 1
+      const bool more = j + 1 < n_on;
+      const RowView<T> v(logits, ld, row_i, vocab), next(logits, ld, more ? row_of(j + 1) : row_i, vocab, more);
+      T* const drow = dlogits + (int64_t)row_i * ld_d;
+      T* const dbody = drow + v.sp.head;
+      const int last_q = v.sp.n_vec - 1, tiles = last_q / ROW + 1, next_q = more ? next.sp.n_vec - 1 : -1;
+      uint64_t mine = ((uint64_t)s.marks[buf][1][tid] << 32) | s.marks[buf][0][tid];
+      const float z_now = single_z;
+      if (more && tid < next.sp.n_scalar) single_z = Row<T>::one(next.row + next.sp.template scalar<T>(tid));
+      if (more) begin_stats(j + 1);
+      lds_barrier();  // its constants
       const float lse = s.lse, c_out = s.c_out;
       const bool is_far = s.is_far != 0;
       const auto power = [&](float x) { return __builtin_amdgcn_exp2f(is_far ? (x - lse) * k : fmaf(x, k, -lse)); };
-      for (uint64_t m = ((uint64_t)mark_hi << 32) | mark_lo; m != 0; m &= m - 1) {
-        const int q = __builtin_ctzll(m) * ROW + tid;
-        float x[8];
-        read(q, x);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) x[j] = power(x[j]) * c_out;
-        each_given(q, [&](int j, int h) {
-          const float y = s.b[h];
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) x[e] = e == j ? y : x[e];
-        });
-        Packed<T>::store(dbody + (uint32_t)q * kPer, x);
-      }
-      if (tid < v.sp.n_scalar) {
-        float x = power(single_z) * c_out;
-        if (s.single >> tid & 1) {
-          const int me = v.sp.template scalar<T>(tid);
-          for (int i = 0; i < t.k; ++i)
-            if (s.id[i] == me) {
-              x = s.b[i];  // the first of them has it all
-              break;
-            }
-        }
-        Row<T>::store_one(drow + v.sp.template scalar<T>(tid), x);
-      }
-      lds_barrier();  // the given tokens are written
-
-      // the rest of the row leaves, the next one comes
-      const bool more = j + 1 < n_on;
-      const RowView<T> next(logits, ld, more ? row_of(j + 1) : row_i, vocab, more);
       const auto write = [&](const uint4& r, int i) {
+        if (i * ROW + tid > last_q) return;
         float x[8];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) x[j] = __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -lse)) * c_out;
+        for (int e = 0; e < kPer; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, e), k, -lse)) * c_out;
         Packed<T>::store(dbody + (int64_t)i * ROW * kPer + (uint32_t)tid * kPer, x);
       };
-      if (is_far) {
-#pragma unroll 1
-        for (int q = tid; q <= last_q; q += ROW) {
-          if (marked(q / ROW)) continue;
-          float x[8];
-          read(q, x);
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) x[j] = power(x[j]) * c_out;
-          Packed<T>::store(dbody + (uint32_t)q * kPer, x);
-        }
-      }
-      if (more && tid < next.sp.n_scalar) single_z = Row<T>::one(next.row + next.sp.template scalar<T>(tid));
-#pragma unroll
-      for (int i = 0; i < NREG; ++i) {
-        if (!is_far && !marked(i) && i * ROW + tid <= last_q) write(reg[i], i);
-        reg[i] = load(next.rsrc, i);
-      }
+      const auto look = [&](const uint4& r, int i) {
+        if (i * ROW + tid <= next_q && !marked(i)) add(r);
+      };
 #pragma unroll
       for (int i = 0; i < NLDS; ++i) {
-        const int at = NREG + i;
-        if (!is_far && !marked(at) && at * ROW + tid <= last_q) write(s_tiles[i * ROW + tid], at);
+        write(s_tiles[i * ROW + tid], NREG + i);
         asm volatile("" ::: "memory");  // the tile has been read
         load_lds(next.rsrc, i);
       }
+      asm volatile("" ::: "memory");  // the loads that follow are behind these
+      constexpr int kLag = 3;  // tiles between a load and its use
+#pragma unroll
+      for (int i = 0; i < NREG + kLag; ++i) {
+        if (i < NREG) {
+          write(reg[i], i);
+          reg[i] = load(next.rsrc, i);
+        }
+        if (i == kLag) {  // as many loads behind those to LDS: these are there
+          __builtin_amdgcn_s_waitcnt(0x0F70 | kLag);
+          asm volatile("" ::: "memory");
+        }
+        if (i >= kLag) look(reg[i - kLag], i - kLag);
+        if (i > kLag && i - kLag - 1 < NLDS) look(s_tiles[(i - kLag - 1) * ROW + tid], NREG + i - kLag - 1);
+      }
 #pragma unroll 1
-      for (int i = NREG + NLDS; i < tiles; ++i)
-        if (!is_far && !marked(i) && i * ROW + tid <= last_q) write(load(v.rsrc, i), i);
+      for (int i = NREG + NLDS; i < tiles; i += 2) {
+        const uint4 r0 = load_cached(v.rsrc, i), r1 = load_cached(v.rsrc, i + 1);
+        write(r0, i);
+        write(r1, i + 1);
+      }
+      if (is_far) {
+#pragma unroll 1
+        for (int q = tid; q <= last_q; q += ROW) {
+          float x[8];
+          Row<T>::template load<true>(v.row + v.sp.head + (uint32_t)q * kPer, x);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) x[e] = power(x[e]) * c_out;
+          Packed<T>::store(dbody + (uint32_t)q * kPer, x);
+        }
+      }
+      // the given tokens, each by the thread that has written its vector
+      for (; mine != 0; mine &= mine - 1) {
+        const int q = __builtin_ctzll(mine) * ROW + tid, id0 = v.sp.head + q * kPer;
+        each_given(buf, id0, q, [&](int e, int h) { Row<T>::store_one(drow + id0 + e, s.given[buf].b[h]); });
+      }
+      if (tid < v.sp.n_scalar) {
+        const int at = v.sp.template scalar<T>(tid);
+        float x = power(z_now) * c_out;
+        if (s.single[buf] >> tid & 1)
+          for (int i = 0; i < t.k; ++i)
+            if (s.given[buf].id[i] == at) {
+              x = s.given[buf].b[i];  // the first of them has it all
+              break;
+            }
+        Row<T>::store_one(drow + at, x);
+      }
+      if (more) {
+        add_beyond(next);
+        add_marked(j + 1, next);
+        end_stats(j + 1, next);
+      }
     }
     // the loads that the last row has asked for come back before the tiles are asked for again
-    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
     asm volatile("" ::: "memory");
   }
 }
@@ -860,6 +799,8 @@ __global__ __launch_bounds__(kSumBlock) void distill_sum_kernel(const float* __r
 using namespace axon;
 
 namespace {
+
+constexpr int64_t kCacheBytes = int64_t(256) << 20;
 
 int elem_bytes(int dtype) { return dtype == AXON_LOGITS_F32 ? 4 : 2; }
 
@@ -911,7 +852,7 @@ extern "C" int64_t axon_distill_workspace_bytes(int dtype, int64_t n, int64_t vo
 extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_i64,
                                 const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
                                 float temperature, float* losses, float* covered, float* grads, float* coef, void* workspace,
-                                int64_t workspace_bytes, void* stream) {
+                                int64_t workspace_bytes, int bwd_follows, void* stream) {
   int rc = check_rows(logits, dtype, ld, n, vocab);
   if (rc == AXON_OK && n > 0) rc = check_teacher(ids, teacher_logprobs, k, divergence, tail, beta, temperature);
   if (rc != AXON_OK || n == 0) return rc;
@@ -923,13 +864,15 @@ extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64
   const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail, beta, 1.f / temperature};
   const RowOut out{losses, covered, grads, coef, (int)n};
   float4* const ws = static_cast<float4*>(workspace);
+  const int64_t cached = bwd_follows ? kCacheBytes / (vocab * eb) : 0;
+  const int cached_from = (int)(cached < n ? n - cached : 0);
   const unsigned lds = (unsigned)(((vocab * eb / 16 + parts - 1) / parts + 1 + 3) / 4 * 4);
 #define AXON_FWD(T, REST)                                                                                                          \
   do {                                                                                                                             \
     hipLaunchKernelGGL((distill_stats_kernel<T, REST>), dim3((unsigned)(n * parts)), dim3(kBlock), REST ? lds : 0, st,             \
-                       static_cast<const T*>(logits), ld, (int)vocab, parts, t, ws);                                               \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, t, ws, cached_from);                                  \
     AXON_CHECK_LAUNCH();                                                                                                           \
-    hipLaunchKernelGGL((distill_finish_kernel<T, REST>), dim3((unsigned)n), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
+    hipLaunchKernelGGL((distill_finish_kernel<T, REST>), dim3((unsigned)n), dim3(kWave), 0, st, static_cast<const T*>(logits), ld, \
                        (int)vocab, parts, t, ws, out);                                                                             \
   } while (0)
 #define AXON_FWD_OF(T) \
@@ -969,8 +912,8 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
 
 namespace {
 
-// Rows of up to 64 KB: 192 threads that hold the row, four workgroups on a compute unit; up to 128 KB: 448, two; longer: 960, one, of
-// which 405 KB are held and the rest is read twice.
+// Rows of up to 64 KB: 192 threads that hold the row, three workgroups on a compute unit; up to 128 KB: 448, two; longer: 960, one, of
+// which 375 KB are held and the rest is read twice.
 constexpr int64_t kMaxRowVecs = kMaxTiles * 960;
 template <typename T, bool REST>
 int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const Teacher& t, const RowOut& out, void* dlogits, int64_t ld_d,
@@ -979,9 +922,9 @@ int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const 
 #define AXON_ROW(ROW, NREG, NLDS, RESIDENT)                                                                                          \
   hipLaunchKernelGGL((distill_row_kernel<T, REST, ROW, NREG, NLDS, 256 * RESIDENT>), dim3((unsigned)(n < 256 * RESIDENT ? n : 256 * RESIDENT)),       \
                      dim3(ROW + kWave), 0, st, static_cast<const T*>(logits), ld, (int)vocab, t, out, static_cast<T*>(dlogits), ld_d)
-  if (vecs <= 192 * 22) AXON_ROW(192, 14, 8, 4);
+  if (vecs <= 192 * 22) AXON_ROW(192, 18, 4, 3);
   else if (vecs <= 448 * 19) AXON_ROW(448, 14, 5, 2);
-  else AXON_ROW(960, 18, 9, 1);
+  else AXON_ROW(960, 18, 7, 1);
 #undef AXON_ROW
   AXON_CHECK_LAUNCH();
   return AXON_OK;
@@ -1012,7 +955,7 @@ extern "C" int axon_distill_loss(const void* logits, int dtype, int64_t ld, int6
                                      : launch_rows<unsigned short, false>(logits, ld, n, vocab, t, out, dlogits, ld_d, st);
   } else if (rc == AXON_OK) {
     rc = axon_distill_fwd(logits, dtype, ld, n, vocab, ids, ids_i64, teacher_logprobs, k, weights, divergence, tail, beta, temperature, losses,
-                          covered, grads, coef, workspace, workspace_bytes, stream);
+                          covered, grads, coef, workspace, workspace_bytes, dlogits != nullptr, stream);
   }
   if (rc == AXON_OK && dlogits && !rows)
     rc = axon_distill_bwd(logits, dtype, ld, n, vocab, ids, ids_i64, k, weights, temperature, grads, coef, nullptr, 0, dlogits, ld_d, stream);

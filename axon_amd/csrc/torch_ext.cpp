@@ -1205,7 +1205,7 @@ std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& lo
     } else {
       check(axon_distill_fwd(rows.data_ptr(), dtype, row_stride(rows), n, v, ids.data_ptr(), is_i64(ids), (const float*)lq.data_ptr(), k, nullptr,
                              divergence, tail, (float)beta, (float)temperature, losses_p, covered_p, grads_p, coef_p, ws.data_ptr(), need,
-                             stream()),
+                             wants_grad, stream()),
             "axon_distill_fwd");
     }
   }

@@ -800,7 +800,7 @@ int64_t axon_distill_workspace_bytes(int dtype, int64_t n, int64_t vocab);
 int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
                      const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,
                      float temperature, float* losses, float* covered, float* grads, float* coef, void* workspace,
-                     int64_t workspace_bytes, void* stream);
+                     int64_t workspace_bytes, int bwd_follows, void* stream);
 int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
                      int64_t k, const float* weights, float temperature, const float* grads, const float* coef,
                      const float* upstream, int ready, void* dlogits, int64_t ld_d, void* stream);

@@ -53,7 +53,7 @@ def test_the_c_entry_points_check_their_arguments():
     assert ws > 0 and lib.axon_distill_workspace_bytes(0, -1, 100) < 0 and lib.axon_distill_workspace_bytes(5, 2, 100) < 0
 
     def fwd(z=p, dtype=0, ld=100, n=2, v=100, ids=p, lq=p, k=3, div=0, tail=1, beta=0.5, t=1.0, losses=p, cov=p, grads=p, coef=p, w=p, wb=ws):
-        return lib.axon_distill_fwd(z, dtype, ld, n, v, ids, 1, lq, k, None, div, tail, beta, t, losses, cov, grads, coef, w, wb, None)
+        return lib.axon_distill_fwd(z, dtype, ld, n, v, ids, 1, lq, k, None, div, tail, beta, t, losses, cov, grads, coef, w, wb, 0, None)
 
     assert fwd(n=0) == 0
     for bad in (dict(z=None), dict(z=p + 2), dict(dtype=2), dict(ld=99), dict(n=-1), dict(v=0), dict(ids=None), dict(lq=None), dict(div=3),
