@@ -84,68 +84,6 @@ __device__ __forceinline__ void mark_given(const GivenBytes& g, const Teacher& t
   __syncthreads();
 }
 
-// Workgroup (row, part): the statistics of its share of the row, of what is not given where that is an outcome (REST), in
-// parts[row][part].
-template <typename T, bool REST>
-__global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
-                                                               float4* __restrict__ parts, int cached_from) {
-  extern __shared__ __align__(16) uint32_t s_given[];
-  __shared__ uint32_t s_single;
-  __shared__ float red[2][kBlock / kWave];
-  const int row_i = blockIdx.x / n_parts, part = blockIdx.x % n_parts, tid = threadIdx.x;
-  if (t.weights != nullptr && t.weights[row_i] == 0.f) return;
-  const T* row = logits + (int64_t)row_i * ld;
-  constexpr int kPer = Row<T>::kPer;
-  const RowSpan sp(row, vocab, true, part, n_parts);
-  if (REST) mark_given<T>(GivenBytes{s_given, &s_single}, t, row_i, vocab, sp, kBlock);
-  const uint8_t* const given = reinterpret_cast<const uint8_t*>(s_given);
-  const T* body = row + sp.head;
-  const float k = t.inv_t * kLog2e;
-  Sum st{kLowest, 0.f};
-  auto one = [&](int q, float (&v)[8]) {
-    if (REST) {
-      const uint32_t out = given[q - sp.q_lo];
-      if (out != 0) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) v[j] = (out >> j & 1) ? -INFINITY : v[j];
-      }
-    }
-    fold<kPer>(st, v, k);
-  };
-  // rows from cached_from on are left in the cache in front of the memory, for a backward that follows
-  auto walk = [&](auto cached) {
-    constexpr bool kCached = decltype(cached)::value;
-    int q = sp.q_lo + tid;
-    for (; q + kBlock < sp.q_hi; q += 2 * kBlock) {
-      float v0[8], v1[8];
-      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v0);
-      Row<T>::template load<kCached>(body + (uint32_t)(q + kBlock) * kPer, v1);
-      one(q, v0);
-      one(q + kBlock, v1);
-    }
-    for (; q < sp.q_hi; q += kBlock) {
-      float v[8];
-      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v);
-      one(q, v);
-    }
-  };
-  if (row_i >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
-  if (part == 0 && tid < sp.n_scalar && !(REST && (s_single >> tid & 1))) {
-    const float v[8] = {Row<T>::one(row + sp.scalar<T>(tid))};
-    fold<1>(st, v, k);
-  }
-  const float m = wave_max(st.M);
-  const float s = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
-  if ((tid & (kWave - 1)) == 0) { red[0][tid / kWave] = m; red[1][tid / kWave] = s; }
-  __syncthreads();
-  if (tid != 0) return;
-  float M = red[0][0];
-  for (int w = 1; w < kBlock / kWave; ++w) M = fmaxf(M, red[0][w]);
-  double total = 0.0;
-  for (int w = 0; w < kBlock / kWave; ++w) total += (double)red[1][w] * __builtin_amdgcn_exp2f((red[0][w] - M) * k);
-  parts[blockIdx.x] = make_float4(M, (float)total, (float)(total - (float)total), 0.f);
-}
-
 // What one lane has written to LDS, for the others of its wavefront: LDS serves a wavefront in order, the compiler is told to.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -180,9 +118,9 @@ struct Given {
   float best, best_q;            // the largest of either
   double sum, sum_q;             // REST: of exp((z - best) / T), every token once, and of q; else of exp(lq - best_q)
 };
-// By one wavefront; everything that can be known before the row's statistics.
+// By one wavefront; everything that can be known before the row's statistics.  firsts: whether ids that come again are looked for.
 template <typename T, bool REST>
-__device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_i, const T* row, int vocab, int lane) {
+__device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_i, const T* row, int vocab, int lane, bool firsts = REST) {
   for (int i = lane; i < t.k; i += kWave) {
     const int id = teacher_id(t, (int64_t)row_i * t.k + i, vocab);
     const float lq = t.logprobs[(int64_t)row_i * t.k + i], z = Row<T>::one(row + max(id, 0));
@@ -194,8 +132,10 @@ __device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_
   for (int i = lane; i < t.k; i += kWave) {
     const int id = s.id[i];
     bool first = id >= 0;
+    if (firsts) {
 #pragma unroll 8
-    for (int j = 0; j < t.k; ++j) first = first && !(j < i && s.id[j] == id);
+      for (int j = 0; j < t.k; ++j) first = first && !(j < i && s.id[j] == id);
+    }
     s.next[i] = first ? -1 : kAgain;
   }
   float best = -INFINITY, best_q = -INFINITY;
@@ -282,7 +222,80 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
   return r;
 }
 
-// The end of rows whose statistics are there, by a wavefront per row.
+// Workgroup (row, part): the statistics of its share of the row, of what is not given where that is an outcome (REST), in
+// parts[row][part].  A row of one part is finished here, by a wavefront, while the compute unit's other workgroups read theirs.
+template <typename T, bool REST>
+__global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
+                                                               float4* __restrict__ parts, RowOut out, int cached_from) {
+  extern __shared__ __align__(16) uint32_t s_given[];
+  __shared__ uint32_t s_single;
+  __shared__ float red[2][kBlock / kWave];
+  __shared__ Given s_row;
+  const int row_i = blockIdx.x / n_parts, part = blockIdx.x % n_parts, tid = threadIdx.x;
+  if (t.weights != nullptr && t.weights[row_i] == 0.f) {
+    if (n_parts == 1 && tid == 0) out.losses[row_i] = out.covered[row_i] = 0.f;
+    return;
+  }
+  const T* row = logits + (int64_t)row_i * ld;
+  constexpr int kPer = Row<T>::kPer;
+  const RowSpan sp(row, vocab, true, part, n_parts);
+  if (REST) mark_given<T>(GivenBytes{s_given, &s_single}, t, row_i, vocab, sp, kBlock);
+  const uint8_t* const given = reinterpret_cast<const uint8_t*>(s_given);
+  const T* body = row + sp.head;
+  const float k = t.inv_t * kLog2e;
+  Sum st{kLowest, 0.f};
+  auto one = [&](int q, float (&v)[8]) {
+    if (REST) {
+      const uint32_t out = given[q - sp.q_lo];
+      if (out != 0) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] = (out >> j & 1) ? -INFINITY : v[j];
+      }
+    }
+    fold<kPer>(st, v, k);
+  };
+  // rows from cached_from on are left in the cache in front of the memory, for a backward that follows
+  auto walk = [&](auto cached) {
+    constexpr bool kCached = decltype(cached)::value;
+    int q = sp.q_lo + tid;
+    for (; q + kBlock < sp.q_hi; q += 2 * kBlock) {
+      float v0[8], v1[8];
+      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v0);
+      Row<T>::template load<kCached>(body + (uint32_t)(q + kBlock) * kPer, v1);
+      one(q, v0);
+      one(q + kBlock, v1);
+    }
+    for (; q < sp.q_hi; q += kBlock) {
+      float v[8];
+      Row<T>::template load<kCached>(body + (uint32_t)q * kPer, v);
+      one(q, v);
+    }
+  };
+  if (row_i >= cached_from) walk(std::true_type{}); else walk(std::false_type{});
+  if (part == 0 && tid < sp.n_scalar && !(REST && (s_single >> tid & 1))) {
+    const float v[8] = {Row<T>::one(row + sp.scalar<T>(tid))};
+    fold<1>(st, v, k);
+  }
+  const float m = wave_max(st.M);
+  const float s = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
+  if ((tid & (kWave - 1)) == 0) { red[0][tid / kWave] = m; red[1][tid / kWave] = s; }
+  __syncthreads();
+  if (n_parts == 1) {
+    if (tid >= kWave) return;
+    fetch_given<T, REST>(s_row, t, row_i, row, vocab, tid);
+    const bool mine = tid < kBlock / kWave;
+    finish_row<REST>(s_row, t, out, row_i, mine ? red[0][tid] : kLowest, mine ? (double)red[1][tid] : 0.0, tid);
+    return;
+  }
+  if (tid != 0) return;
+  float M = red[0][0];
+  for (int w = 1; w < kBlock / kWave; ++w) M = fmaxf(M, red[0][w]);
+  double total = 0.0;
+  for (int w = 0; w < kBlock / kWave; ++w) total += (double)red[1][w] * __builtin_amdgcn_exp2f((red[0][w] - M) * k);
+  parts[blockIdx.x] = make_float4(M, (float)total, (float)(total - (float)total), 0.f);
+}
+
+// The end of rows that several workgroups have read, by a wavefront per row.
 template <typename T, bool REST>
 __global__ __launch_bounds__(kWave) void distill_finish_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int n_parts, Teacher t,
                                                                const float4* __restrict__ parts, RowOut out) {
@@ -458,7 +471,7 @@ __device__ __forceinline__ void mark_row(RowLds<ROW>& s, int buf, const Teacher&
   for (int i = lane; i < ROW; i += kWave) s.marks[buf][0][i] = s.marks[buf][1][i] = 0;
   for (int i = lane; i < kBuckets; i += kWave) s.heads[buf][i] = -1;
   if (lane == 0) s.single[buf] = 0;
-  fetch_given<T, REST>(g, t, row_i, v.row, vocab, lane);
+  fetch_given<T, REST>(g, t, row_i, v.row, vocab, lane, true);
   for (int i = lane; i < t.k; i += kWave) {
     if (g.next[i] == kAgain) continue;
     const int id = g.id[i], in = id - v.sp.head, q = in >= 0 ? in / kPer : -1;
@@ -870,9 +883,10 @@ extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64
 #define AXON_FWD(T, REST)                                                                                                          \
   do {                                                                                                                             \
     hipLaunchKernelGGL((distill_stats_kernel<T, REST>), dim3((unsigned)(n * parts)), dim3(kBlock), REST ? lds : 0, st,             \
-                       static_cast<const T*>(logits), ld, (int)vocab, parts, t, ws, cached_from);                                  \
+                       static_cast<const T*>(logits), ld, (int)vocab, parts, t, ws, out, cached_from);                             \
     AXON_CHECK_LAUNCH();                                                                                                           \
-    hipLaunchKernelGGL((distill_finish_kernel<T, REST>), dim3((unsigned)n), dim3(kWave), 0, st, static_cast<const T*>(logits), ld, \
+    if (parts > 1)                                                                                                                 \
+      hipLaunchKernelGGL((distill_finish_kernel<T, REST>), dim3((unsigned)n), dim3(kWave), 0, st, static_cast<const T*>(logits), ld, \
                        (int)vocab, parts, t, ws, out);                                                                             \
   } while (0)
 #define AXON_FWD_OF(T) \

@@ -1101,7 +1101,7 @@ unsigned long long capture_id() {
 }
 
 struct DistillNode : torch::autograd::Node {
-  SavedVariable rows, ids, grads, coef, weights;
+  SavedVariable rows, ids, state, weights;  // state: coefficients [4][n], then the gradients of the tokens' log-probabilities [n][k]
   Tensor ready;  // with weights: the gradient of an upstream gradient of 1, which the forward has left
   unsigned long long captured = 0;  // ... into this graph
   std::vector<int64_t> shape;
@@ -1110,27 +1110,26 @@ struct DistillNode : torch::autograd::Node {
   static constexpr const char* kWhat = "distillation_backward";
   std::string name() const override { return "DistillationBackward"; }
   void release_variables() override {
-    for (SavedVariable* s : {&rows, &ids, &grads, &coef, &weights}) s->reset_data();
+    for (SavedVariable* s : {&rows, &ids, &state, &weights}) s->reset_data();
     ready.reset();
   }
   variable_list apply(variable_list&& g) override {
     if (!g[0].defined()) return {Tensor()};
     if (spent) throw AxonError("the logits' storage holds the gradient of an earlier backward (inplace_backward)");
-    const Tensor x = rows.unpack(), at = ids.unpack(), gr = grads.unpack(), co = coef.unpack(), w = weights.unpack();
+    const Tensor x = rows.unpack(), at = ids.unpack(), st = state.unpack(), w = weights.unpack();
     Tensor out;
     {
       const at::NoGradGuard no_grad;
       check_saved_rows(kWhat, x);
       const int64_t n = x.size(0), v = x.size(1);
       const Tensor up = f32(g[0]);
-      same_place(kWhat, x, {&at, &gr, &co, &w, &up});
+      same_place(kWhat, x, {&at, &st, &w, &up});
       const int dtype = logits_dtype(kWhat, x);
-      same_type(kWhat, at::kFloat, {&gr, &co, &w});
+      same_type(kWhat, at::kFloat, {&st, &w});
       if (!is_index(at) || at.dim() != 2) refuse(kWhat, "a saved tensor has come back in another type");
       const int64_t k = at.size(1);
       same_len(kWhat, "ids", n * k, at);
-      same_len(kWhat, "gradients", n * k, gr);
-      same_len(kWhat, "coefficients", 4 * n, co);
+      same_len(kWhat, "coefficients", n * (4 + k), st);
       same_len(kWhat, "upstream gradient", weighted ? 1 : n, up);
       if (weighted) same_len(kWhat, "token_weights", n, w);
       const c10::DeviceGuard device(x.device());
@@ -1140,7 +1139,7 @@ struct DistillNode : torch::autograd::Node {
       out = there ? ready : inplace ? x : at::empty({n, v}, x.options());
       ready.reset();
       check(axon_distill_bwd(x.data_ptr(), dtype, row_stride(x), n, v, at.data_ptr(), is_i64(at), k, (const float*)ptr(w), temperature,
-                             (const float*)gr.data_ptr(), (const float*)co.data_ptr(), (const float*)up.data_ptr(), there, out.data_ptr(),
+                             (const float*)st.data_ptr() + 4 * n, (const float*)st.data_ptr(), (const float*)up.data_ptr(), there, out.data_ptr(),
                              row_stride(out), ::stream()),
             "axon_distill_bwd");
       spent = inplace;
@@ -1157,7 +1156,7 @@ std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& lo
                                               bool inplace) {
   const bool wants_grad = at::GradMode::is_enabled() && logits.requires_grad();
   no_tangent(what, logits);
-  Tensor rows, ids, w, loss, losses, covered, grads, coef, ready;
+  Tensor rows, ids, w, loss, losses, covered, state, ready;
   {
     const at::NoGradGuard no_grad;
     rows = rows_of_logits(logits);
@@ -1189,12 +1188,11 @@ std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& lo
     if (token_weights) w = f32(*token_weights);
     losses = at::empty(batch, opts(rows));
     covered = at::empty(batch, opts(rows));
-    grads = at::empty({n, k}, opts(rows));
-    coef = at::empty({4, n}, opts(rows));
+    state = at::empty({n * (4 + k)}, opts(rows));
     const int64_t need = axon_distill_workspace_bytes(dtype, n, v);
     const Tensor ws = at::empty({std::max<int64_t>(need, 0)}, opts(rows, at::kByte));
-    float *const losses_p = losses.data_ptr<float>(), *const covered_p = covered.data_ptr<float>(), *const grads_p = grads.data_ptr<float>(),
-                *const coef_p = coef.data_ptr<float>();
+    float *const losses_p = losses.data_ptr<float>(), *const covered_p = covered.data_ptr<float>(), *const coef_p = state.data_ptr<float>(),
+                *const grads_p = coef_p + 4 * n;
     if (token_weights) {
       loss = at::empty({}, opts(rows));
       if (wants_grad) ready = at::empty({n, v}, rows.options());
@@ -1219,8 +1217,7 @@ std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& lo
     torch::autograd::set_history(node->weighted ? loss : losses, node);
     node->rows = SavedVariable(rows, false);
     node->ids = SavedVariable(ids, false);
-    node->grads = SavedVariable(grads, false);
-    node->coef = SavedVariable(coef, false);
+    node->state = SavedVariable(state, false);
     node->weights = SavedVariable(w, false);
     if (node->weighted) {
       const c10::DeviceGuard device(rows.device());
