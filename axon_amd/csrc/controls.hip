@@ -75,14 +75,14 @@ constexpr float kBanned = -1e30f;  // stands for -inf where a product with it ha
 constexpr float kFar = 1e9f;       // a reference in log2 units whose rounding (64) leaves the exponentials in range
 constexpr float kNoLogit = -3.402823466e38f;  // the reference of a set without a logit: any there is is at least as large
 
-// A token of a history: its id, or -1 where it counts for nothing; bit 30 where the model has generated it.
+// A token of a history: its id, or -1 where it counts for nothing; bit 30 where the model has generated it.  (Both loads at once.)
 constexpr int kOwn = 1 << 30;
 __device__ __forceinline__ int history_token(const axon_controls& c, int64_t at, int vocab) {
   const int64_t id = index_at(c.token_ids, c.token_ids_i64, at);
-  if (id < 0 || id >= vocab) return -1;
-  const bool own = c.own_mask == nullptr || (c.mask_kind == AXON_MASK_I64 ? static_cast<const int64_t*>(c.own_mask)[at] != 0
-                                                                         : static_cast<const float*>(c.own_mask)[at] != 0.f);
-  return (int)id | (own ? kOwn : 0);
+  bool own = true;
+  if (c.own_mask != nullptr)
+    own = c.mask_kind == AXON_MASK_I64 ? static_cast<const int64_t*>(c.own_mask)[at] != 0 : static_cast<const float*>(c.own_mask)[at] != 0.f;
+  return id < 0 || id >= vocab ? -1 : (int)id | (own ? kOwn : 0);
 }
 
 // The additive part of what controls do to one id.
@@ -132,17 +132,27 @@ __global__ __launch_bounds__(kBlock, 4) void controls_kernel(const T* logits, in
   // what belongs to row first + lane
   const int mine = min(first + lane, n_rows - 1);
   int seq = 0, start = 0, state = -1, label = -1, token = -1;
-  const int64_t n_seqs = c.n_seqs;
-  if (n_seqs > 0) {
+  const int n_seqs = (int)c.n_seqs;
+  int64_t begin = 0, end = 0;  // the row's history
+  const bool history = ADJ && c.token_ids != nullptr, offsets = c.uniform_len == 0 && c.cu_seqlens != nullptr;
+  if (n_seqs > 0 && c.every_position && offsets && n_seqs <= kWave) {
+    // few sequences: all of their ends in one load, a lane each, instead of a search with its loads one after the other
+    const int ends = c.cu_seqlens[min(lane + 1, n_seqs)], base0 = c.cu_seqlens[0];
+    for (int i = 0; i < n_seqs - 1; ++i) seq += lane_value(ends, i) <= mine;
+    end = __shfl(ends, seq, kWave);
+    begin = __shfl(ends, max(seq - 1, 0), kWave);
+    if (seq == 0) begin = base0;
+  } else if (n_seqs > 0) {
     if (!c.every_position) seq = mine;
     else if (c.uniform_len > 0) seq = (int)(mine / c.uniform_len);
-    else seq = RowFinder::upper4(c.cu_seqlens, 0, (int)n_seqs, mine);
-    seq = min(max(seq, 0), (int)n_seqs - 1);
+    else seq = RowFinder::upper4(c.cu_seqlens, 0, n_seqs, mine);
+    seq = min(max(seq, 0), n_seqs - 1);
+    if (history) {
+      begin = c.uniform_len > 0 ? (int64_t)seq * c.uniform_len : (int64_t)c.cu_seqlens[seq];
+      end = c.uniform_len > 0 ? begin + c.uniform_len : (int64_t)c.cu_seqlens[seq + 1];
+    }
   }
-  int64_t begin = 0, end = 0;  // the row's history
-  if (ADJ && c.token_ids != nullptr) {
-    begin = c.uniform_len > 0 ? (int64_t)seq * c.uniform_len : (int64_t)c.cu_seqlens[seq];
-    end = c.uniform_len > 0 ? begin + c.uniform_len : (int64_t)c.cu_seqlens[seq + 1];
+  if (history) {
     if (c.every_position) {
       if (mine < begin || mine >= end) begin = mine + 1;  // a position of no sequence
       end = (int64_t)mine + 1;
