@@ -113,21 +113,21 @@ __device__ __forceinline__ float pick(uint32_t mask, float yes, float no) {
   return __uint_as_float((mask & __float_as_uint(yes)) | (~mask & __float_as_uint(no)));
 }
 
-template <typename T, Mode MODE, bool ADJ, bool MASK>
-__global__ __launch_bounds__(kBlock, 4) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
+template <typename T, Mode MODE, bool ADJ, bool MASK, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* logits, int64_t ld, int n_rows, int vocab, int chunks, int run,
                                                           axon_controls c, RowIo io, const T* other, int64_t ld_other, T* out,
                                                           int64_t ld_out) {
-  constexpr int kPer = Unaligned<T>::kPer, kLaneIds = kVecs * kPer, kIds = kLaneIds * kWave, kGroupIds = kIds * kWaves;
+  constexpr int kPer = Unaligned<T>::kPer, kLaneIds = kVecs * kPer, kIds = kLaneIds * kWave, kGroupIds = kIds * WAVES, kThreads = WAVES * kWave;
   constexpr uint32_t kVecBits = (1u << kPer) - 1, kAll = kLaneIds == 32 ? ~0u : (1u << (kLaneIds & 31)) - 1;
   __shared__ __align__(16) uint32_t s_adj[ADJ ? kGroupIds : 4];  // counts (bit 31: seen) while they are collected, then floats
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);  // bases in scalar registers
-  const int groups = (chunks + kWaves - 1) / kWaves;
+  const int groups = (chunks + WAVES - 1) / WAVES;
   // kGrad from the last row to the first: the end of what the forward read last is still in the cache in front of the memory
   const unsigned block = MODE == kGrad ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const int first = (int)(block / groups) * run, group = (int)(block % groups);
   const bool cached = MODE == kStats && first >= io.cached_from;
   const int rows = min(run, n_rows - first);
-  const int chunk = group * kWaves + wave, base = chunk * kIds;
+  const int chunk = group * WAVES + wave, base = chunk * kIds;
 
   // what belongs to row first + lane
   const int mine = min(first + lane, n_rows - 1);
@@ -324,19 +324,19 @@ __global__ __launch_bounds__(kBlock, 4) void controls_kernel(const T* logits, in
   }
   if (ADJ) {  // the history before the run's first row, by the whole workgroup (of the row itself, where a row is a sequence)
     const uint4 none = make_uint4(0, 0, 0, 0);
-    for (int i = tid; i < kGroupIds / 4; i += kBlock) reinterpret_cast<uint4*>(s_adj)[i] = none;
+    for (int i = tid; i < kGroupIds / 4; i += kThreads) reinterpret_cast<uint4*>(s_adj)[i] = none;
     __syncthreads();
     const int from = lane_value(start, 0);
     const int upto = c.every_position ? first : lane_value((int)end, 0);  // offsets are 32-bit integers
     if (c.token_ids != nullptr) {
       const auto count = [&](auto id_of, auto own_of) {
         constexpr int kBatch = 8;  // loads in flight per thread
-        for (int i0 = from + tid; i0 < upto; i0 += kBlock * kBatch) {
+        for (int i0 = from + tid; i0 < upto; i0 += kThreads * kBatch) {
           int off[kBatch];
           bool own[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int i = i0 + b * kBlock, at = min(i, upto - 1);
+            const int i = i0 + b * kThreads, at = min(i, upto - 1);
             const int64_t id = id_of(at);
             own[b] = own_of(at);
             off[b] = i < upto && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
@@ -675,11 +675,27 @@ int check_controls(const axon_controls* c, int64_t n, int64_t v) {
 
 int chunks_of(int64_t vocab, int dtype) { return (int)((vocab * elem_bytes(dtype) + kChunkBytes - 1) / kChunkBytes); }
 
-// Rows of a run: about four rounds of the 4096 wavefronts that the part holds.
-int run_of(int64_t n, int chunks) {
-  const int64_t r = n * chunks / (4 * 4096);
-  return (int)(r < 1 ? 1 : (r < kMaxRun / 2 ? r : kMaxRun / 2));
+// Workgroups of a kernel that the device holds at once (it is the same for all devices that this is built for).
+template <typename K>
+int resident_of(K kernel, int threads) {
+  int dev = 0, cus = 0, per_cu = 0;
+  const bool known = hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess &&
+                     hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(kernel), threads, 0) == hipSuccess;
+  return known && cus * per_cu > 0 ? cus * per_cu : 1024;
 }
+
+// Rows of a run: three times as many workgroups as there is room for, so that the last ones to start are a small part, and what a
+// run costs by itself (the history before it, its terms) is shared by as many rows as that leaves.  Log-probabilities with gradients
+// of 2047 x 50257 bf16 take 154 us so, 151 to 154 with two, 159 with four; 4096 x 151936 under masks 284, 307 and 293 us.
+int run_of(int64_t n, int groups, int resident) {
+  const int64_t most = 3 * (int64_t)resident, r = (n * groups + most - 1) / most;
+  return (int)(r < 1 ? 1 : (r < kMaxRun ? r : kMaxRun));
+}
+
+// Wavefronts of a workgroup that holds additive terms: those of 8192 ids, 32 KB of LDS and five workgroups on a compute unit.  Each
+// reads the whole history, so fewer ids a workgroup cost reads (61 x 201088 fp32 with 4000 tokens each: 4 wavefronts 33 us, 8 30 us),
+// more cost workgroups that work while another waits (16: 39 us; 1024 x 32768 bf16 with 1500 tokens each: 4 38.7, 8 39.5, 16 43 us).
+template <typename T> constexpr int kAdjWaves = sizeof(T) == 4 ? 8 : 4;
 
 template <Mode MODE>
 int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls& given, const RowIo& io,
@@ -688,19 +704,24 @@ int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, 
   const bool penalties = c.repetition || c.frequency || c.presence || c.repetition_all != 1.f || c.frequency_all != 0.f || c.presence_all != 0.f;
   if (!penalties) c.token_ids = nullptr;  // nobody asks for the history
   const bool adj = (penalties && c.token_ids) || c.n_bias > 0, mask = c.allowed != nullptr;
-  const int chunks = chunks_of(vocab, dtype), groups = (chunks + kWaves - 1) / kWaves;
-  const int run = adj && !c.every_position ? 1 : run_of(n, chunks);
-  const int64_t grid = (n + run - 1) / run * groups;
-  if (grid >= INT32_MAX) return AXON_ERR_SHAPE;
-#define AXON_CONTROLS(T, A, M)                                                                                             \
-  hipLaunchKernelGGL((controls_kernel<T, MODE, A, M>), dim3((unsigned)grid), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
-                     (int)n, (int)vocab, chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out)
+  const int chunks = chunks_of(vocab, dtype);
+  const bool of_rows = !c.every_position;
+#define AXON_CONTROLS(T, A, M, WAVES)                                                                                      \
+  do {                                                                                                                     \
+    const auto kernel = controls_kernel<T, MODE, A, M, WAVES>;                                                             \
+    static const int resident = resident_of(kernel, WAVES * kWave);                                                        \
+    const int groups = (chunks + WAVES - 1) / WAVES, run = A && of_rows ? 1 : run_of(n, groups, resident);                 \
+    const int64_t grid = (n + run - 1) / run * groups;                                                                     \
+    if (grid >= INT32_MAX) return AXON_ERR_SHAPE;                                                                          \
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(WAVES * kWave), 0, st, static_cast<const T*>(logits), ld, (int)n, (int)vocab, \
+                       chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out);           \
+  } while (0)
 #define AXON_CONTROLS_OF(T)                                  \
   do {                                                       \
-    if (adj && mask) AXON_CONTROLS(T, true, true);           \
-    else if (adj) AXON_CONTROLS(T, true, false);             \
-    else if (mask) AXON_CONTROLS(T, false, true);            \
-    else AXON_CONTROLS(T, false, false);                     \
+    if (adj && mask) AXON_CONTROLS(T, true, true, kAdjWaves<T>);             \
+    else if (adj) AXON_CONTROLS(T, true, false, kAdjWaves<T>);               \
+    else if (mask) AXON_CONTROLS(T, false, true, 4);         \
+    else AXON_CONTROLS(T, false, false, 4);                  \
   } while (0)
   if (dtype == AXON_LOGITS_F32) AXON_CONTROLS_OF(float);
   else AXON_CONTROLS_OF(unsigned short);
