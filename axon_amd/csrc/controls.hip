@@ -178,6 +178,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   }
   // kGrad: dz = 2^t (A + B t) slope with t = (y - M) log2(e) / T, the row's constants in A and B
   float top_l = 0.f, a_l = 0.f, b_l = 0.f, glp_l = 0.f;
+  uint64_t live = ~0ull >> (kMaxRun - rows);  // rows that are looked at: of the others nothing is asked
   if (MODE == kGrad) {
     top_l = io.stats[mine];
     const float sum = io.stats[(int64_t)n_rows + mine], ls = __log2f(sum), H = io.stats[2 * (int64_t)n_rows + mine];
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
     glp_l = g_lp * inv_t_l;
     a_l = q * -fmaf(g_en, fmaf(-kLn2, ls, H), g_lp);
     b_l = q * -g_en * kLn2;
+    live &= __ballot(g_lp != 0.f || g_en != 0.f);
   }
 
   uint32_t* const adj = s_adj + (ADJ ? wave * kIds : 0);
@@ -318,9 +320,15 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   const bool works = chunk < chunks;
   uint32_t keep_next = there;
   bool few_next = false;
-  if (works) {  // on their way while the history is counted
-    if (MASK) ask_mask(0);
-    else read_row(0, keep_next, false);
+  const auto after = [&](int r) {  // the next row that is looked at, or rows
+    if (MODE != kGrad || r >= rows) return r;
+    const uint64_t left = live & ~0ull << r;
+    return left != 0 ? __builtin_ctzll(left) : rows;
+  };
+  int next = after(0), later = next;
+  if (works && next < rows) {  // on their way while the history is counted
+    if (MASK) ask_mask(next);
+    else read_row(next, keep_next, false);
   }
   if (ADJ) {  // the history before the run's first row, by the whole workgroup (of the row itself, where a row is a sequence)
     const uint4 none = make_uint4(0, 0, 0, 0);
@@ -366,24 +374,33 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   if (ADJ && c.every_position && __any(in_chunk))
     for (int r = 0; r < rows; ++r)
       count_l += lane >= r && token == lane_value(token, r) && start == lane_value(start, r);
-  if (MASK) {
-    keep_next = mask_of(0);
-    if (rows > 1) ask_mask(1);
+  if (MASK && next < rows) {
+    keep_next = mask_of(next);
+    later = after(next + 1);
+    if (later < rows) ask_mask(later);
     few_next = is_few(keep_next);
-    read_row(0, keep_next, few_next);
+    read_row(next, keep_next, few_next);
+  }
+  if (MODE == kGrad) {
+    for (int r = 0; r < rows; ++r) {
+      if (live >> r & 1) continue;
+      T* const o = out + (first + r) * ld_out + base;
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        const int id0 = (u * kWave + lane) * kPer;
+        const float none[kPer] = {};
+        if (whole || base + id0 + kPer <= vocab) {
+          Unaligned<T>::store(o + (uint32_t)id0, none);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (base + id0 + j < vocab) Row<T>::store_one(o + id0 + j, 0.f);
+        }
+      }
+    }
   }
   float ref = kNoLogit;
   for (int r = 0; r < rows; ++r) {
-    const int64_t row = first + r;
-    const float inv_t = lane_value(inv_t_l, r), k = inv_t * kLog2e, rep = lane_value(rep_l, r), inv_rep = 1.f / rep;
-    uint32_t keep = keep_next;
-    const bool few = few_next;
-    if (MASK) {
-      keep_next = r + 1 < rows ? mask_of(r + 1) : 0;
-      if (r + 2 < rows) ask_mask(r + 2);
-    }
-    // masks of single bits are made where they are used: 32 of them held over the rows are 32 registers
-    asm volatile("" : "+v"(keep), "+v"(seen));
     if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
       if (r > 0) {
 #pragma unroll
@@ -406,12 +423,27 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
         }
       }
     }
+    if (MODE == kGrad && r != next) continue;
+    const int64_t row = first + r;
+    const float inv_t = lane_value(inv_t_l, r), k = inv_t * kLog2e, rep = lane_value(rep_l, r), inv_rep = 1.f / rep;
+    uint32_t keep = keep_next;
+    const bool few = few_next;
+    if (MASK) {
+      next = later;
+      keep_next = next < rows ? mask_of(next) : 0;
+      later = after(next + 1);
+      if (later < rows) ask_mask(later);
+    } else {
+      next = after(r + 1);
+    }
+    // masks of single bits are made where they are used: 32 of them held over the rows are 32 registers
+    asm volatile("" : "+v"(keep), "+v"(seen));
     const int l = MODE == kStats || MODE == kGrad ? lane_value(label, r) - base : -1;
     const bool has_label = l >= 0 && l < kIds;
     const int label_lane = l / kPer % kWave, label_at = l / (kWave * kPer) * kPer + l % kPer;
     const bool masked = (MASK || !whole) && __any(keep != kAll);
     const bool repeats = ADJ && rep != 1.f;
-    const bool more = r + 1 < rows;
+    const bool more = next < rows;
 
     // vector u under the controls, before the temperature; banned: what stands for -inf.  slope: dy / dz of every element.
     auto controlled = [&](int u, float banned, float (&y)[kPer], float (&slope)[kPer]) {
@@ -503,7 +535,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           there_are |= (uint32_t)(x != 0) << i;
         }
         few_next = is_few(keep_next);
-        if (more) read_row(r + 1, keep_next, few_next);
+        if (more) read_row(next, keep_next, few_next);
         if (__any(keep != 0)) statistics(std::integral_constant<int, kFew>{}, y, there_are);
         else if (lane == 0) *part = make_float4(kNoLogit, 0.f, 0.f, 0.f);
         if (has_label && lane == label_lane) io.label_y[row] = label_y;
@@ -518,7 +550,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
         for (int j = 0; j < kPer; ++j) y[u * kPer + j] = v[j];
       }
       few_next = is_few(keep_next);
-      if (more) read_row(r + 1, keep_next, few_next);
+      if (more) read_row(next, keep_next, few_next);
       statistics(std::integral_constant<int, kLaneIds>{}, y, keep);
       if (has_label) {
         const int at = lane == label_lane ? label_at : -1;
@@ -548,8 +580,8 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           }
         }
         if (more) {
-          read(from + (r + 1) * ld, keep_next, u, raw[u]);
-          if constexpr (MODE == kApplyGrad) read(from_g + (r + 1) * ld_other, keep_next, u, raw_g[u]);
+          read(from + next * ld, keep_next, u, raw[u]);
+          if constexpr (MODE == kApplyGrad) read(from_g + next * ld_other, keep_next, u, raw_g[u]);
         }
         if (MODE == kGrad && has_label && label_at / kPer == u) {
 #pragma unroll

@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kWave) void distill_finish_kernel(const T* __restri
 // Workgroup (row, part): dlogits of its share.  The row is streamed without a look at the given tokens; their few elements are
 // written again afterwards, from logits that were read before (dlogits may be the logits' own storage).  Equal ids of a row add
 // up in their order, in the thread of the first of them.  upstream: of every row's loss, or (weights) one for all, and where that
-// is 1 the gradient is there already (`ready`).
+// is 1 the gradient is there already (`ready`).  Where it is 0 the row is not read.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, int64_t ld, int vocab, Teacher t, RowOut saved,
                                                               const float* __restrict__ upstream, int ready, T* dlogits, int64_t ld_d,
@@ -324,8 +324,8 @@ __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, i
   const float up = upstream != nullptr ? upstream[t.weights != nullptr ? 0 : row_i] : 1.f;
   if (ready && up == 1.f) return;
   const float w = t.weights != nullptr ? t.weights[row_i] : 1.f;
-  const bool skip = t.weights != nullptr && w == 0.f;
   const float g = up * w * t.inv_t;
+  const bool skip = w == 0.f || g == 0.f;  // nothing comes of the row, whatever it holds
   const T* row = logits + (int64_t)row_i * ld;
   T* out = dlogits + (int64_t)row_i * ld_d;
   const float* const c = saved.coef + row_i;
@@ -513,12 +513,12 @@ __device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teache
   }
 }
 
-// GRID: the most workgroups of a launch.
-template <typename T, bool REST, int ROW, int NREG, int NLDS, int GRID>
-__global__ __launch_bounds__(ROW + kWave, 4) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
+// RESIDENT: workgroups on a compute unit.
+template <typename T, bool REST, int ROW, int NREG, int NLDS, int RESIDENT>
+__global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
                                                                      T* __restrict__ dlogits, int64_t ld_d) {
   __shared__ RowLds<ROW> s;
-  __shared__ int s_count[GRID], s_list[2][kWave];
+  __shared__ int s_count[256 * RESIDENT], s_list[2][kWave];
   __shared__ uint4 s_tiles[NLDS * ROW];  // an array of its own: reads of the rest do not wait for what is on its way here
   constexpr int kPer = Row<T>::kPer;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -934,7 +934,7 @@ int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const 
                 hipStream_t st) {
   const int64_t vecs = vocab / Row<T>::kPer;
 #define AXON_ROW(ROW, NREG, NLDS, RESIDENT)                                                                                          \
-  hipLaunchKernelGGL((distill_row_kernel<T, REST, ROW, NREG, NLDS, 256 * RESIDENT>), dim3((unsigned)(n < 256 * RESIDENT ? n : 256 * RESIDENT)),       \
+  hipLaunchKernelGGL((distill_row_kernel<T, REST, ROW, NREG, NLDS, RESIDENT>), dim3((unsigned)(n < 256 * RESIDENT ? n : 256 * RESIDENT)),       \
                      dim3(ROW + kWave), 0, st, static_cast<const T*>(logits), ld, (int)vocab, t, out, static_cast<T*>(dlogits), ld_d)
   if (vecs <= 192 * 22) AXON_ROW(192, 18, 4, 3);
   else if (vecs <= 448 * 19) AXON_ROW(448, 14, 5, 2);

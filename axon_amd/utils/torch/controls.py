@@ -88,6 +88,7 @@ def controlled_logprobs_from_logits(logits: torch.Tensor, labels: torch.Tensor, 
                                     inplace_backward: bool = False):
     """``(logprobs, entropy)`` of shape ``logits.shape[:-1]``, fp32: the log-probability of ``labels`` (``-inf`` where the
     controls take it out, 0 for a label outside the vocabulary) and the entropy under ``controls``.  A row that they leave nothing
-    of has log-probability ``-inf``, entropy 0 and a zero gradient; one that holds a NaN that is not masked is NaN.  With
+    of has log-probability ``-inf``, entropy 0 and a zero gradient; one that holds a NaN that is not masked is NaN.  A row whose
+    upstream gradients are 0 (a prompt's, say) is not read by the backward: its gradient is 0, whatever it holds.  With
     ``inplace_backward`` the backward writes d loss / d logits over the logits' storage, and can run once."""
     return _lib.native().controlled_logprobs(logits, labels, _native(controls), bool(inplace_backward))
