@@ -11,7 +11,7 @@ The two side terms and the two entropy metrics come out of ONE kernel pass
 (``axon_side_terms``) instead of three ``agg_loss`` calls and an elementwise KL chain.
 
 A model with routed experts may return its ``router_logits`` too: their balance loss (``router_balance_loss``) is then one
-more term (the reference has none here).
+more term (the reference has none here).  So are the ``distill_losses`` of a model that compares itself with a teacher.
 """
 
 from __future__ import annotations
@@ -81,7 +81,7 @@ def _router_term(b, cu, entropy, args, router_logits, router_expert_ids):
     return balance, load.max(), misfit
 
 
-def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, router_expert_ids=None):
+def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, router_expert_ids=None, distill_losses=None):
     """Everything of ``forward_backward_fn`` after the model forward (fsdp_models.py:224-278).
 
     With ``loss_fn_args["router_aux_loss_coef"]`` the balance loss of ``router_logits`` times that coefficient is added, as
@@ -89,6 +89,10 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
     divided by counts over all of these), with ``router_top_k``, ``router_score_fn`` ("softmax") and
     ``router_balance_per_sequence`` (False) from the same arguments.  Routers that saw a padded batch packed (remove-padding)
     are recognised by their number of tokens, which has to be that of ``attention_mask``.
+
+    With ``loss_fn_args["distill_coef"]`` the ``distill_losses`` of the tokens (``distillation_from_logits``, in the shape of
+    ``entropy``; the reference has no such term), aggregated over ``response_mask`` as the KL penalty is, are added times that
+    coefficient.
 
     Returns ``(scaled_loss, metrics)``.  ``data.batch["log_probs"]`` is set; ``response_mask`` may be
     overwritten by the sampler correction hook, while the side terms keep the mask they were given
@@ -141,6 +145,17 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
         loss = loss - ent_agg * entropy_coef
     if kl_coef != 0:
         loss = loss + kl_agg * kl_coef
+    distill_coef = loss_fn_args.get("distill_coef", 0)
+    distill_vals = []
+    if distill_coef != 0:
+        if distill_losses is None:
+            raise ValueError("distill_coef is set, but the model returned no distill_losses")
+        if distill_losses.shape != entropy.shape:
+            raise ValueError(f"distill_losses {tuple(distill_losses.shape)} do not lie beside the tokens {tuple(entropy.shape)}")
+        kept = torch.where(response_mask != 0, distill_losses, 0.0)  # what another token's loss is does not matter
+        distill, _, _ = _SideTerms.apply(kept, None, None, response_mask, rows, 0, 0, agg)
+        loss = loss + distill * distill_coef
+        distill_vals = [distill.detach()]
     router_coef = loss_fn_args.get("router_aux_loss_coef", 0)
     router_vals = []
     if router_coef != 0:
@@ -148,7 +163,8 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
         loss = loss + balance * (router_coef / (n_micro_batches * dp_replicas))
         router_vals = [balance.detach(), load] + ([misfit] if misfit is not None else [])
     # one readback for pg_loss and the side-term metrics
-    vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4], *router_vals]).tolist()
+    vals = torch.stack([pg_loss.detach().float(), acc[0], acc[1], acc[2], acc[4], *distill_vals, *router_vals]).tolist()
+    distill_val = vals.pop(5) if distill_vals else None
     if vals[7:] and vals[7] != 0:
         raise ValueError("router_logits are neither of the padded batch's tokens nor of those that attention_mask keeps")
     metrics["pg_loss"] = vals[0] * n_micro_batches
@@ -157,6 +173,9 @@ def loss_from_outputs(data, log_prob, entropy, meta_info, router_logits=None, ro
     if kl_coef != 0:
         metrics["kl_loss"] = vals[2] * n_micro_batches
         metrics["kl_coef"] = kl_coef
+    if distill_vals:
+        metrics["distill_loss"] = distill_val * n_micro_batches
+        metrics["distill_coef"] = distill_coef
     if router_vals:
         metrics["router_balance_loss"] = vals[5]
         metrics["router_max_load"] = vals[6]
@@ -171,4 +190,4 @@ class CausalLM:
         model_inputs = {**data.batch, **data.non_tensor_batch}
         result = module(model_inputs, {**meta_info, "temperature": meta_info["temperature"], "calculate_entropy": True})
         return loss_from_outputs(data, result["log_probs"], result["entropys"], meta_info, result.get("router_logits", None),
-                                 result.get("router_expert_ids", None))
+                                 result.get("router_expert_ids", None), result.get("distill_losses", None))

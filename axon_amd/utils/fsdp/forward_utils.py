@@ -107,9 +107,33 @@ def _from_logits(logits, labels, temperature: float, calculate_entropy: bool):
     return logprobs_from_logits(logits, labels, inplace_backward=True), None
 
 
+_CONTROLS = ("repetition_penalty", "frequency_penalty", "presence_penalty", "bias_ids", "bias", "allowed", "allowed_index")
+
+
+def _controls_of(logit_controls, micro_batch, temperature, indices=None, cu_seqlens=None):
+    """``LogitControls`` of a batch's rows, padded or (with ``indices``) packed: row t scores token t + 1."""
+    from axon_amd.utils.torch.controls import LogitControls
+
+    unknown = sorted(set(logit_controls) - set(_CONTROLS))
+    if unknown:
+        raise ValueError(f"logit_controls may hold {', '.join(_CONTROLS)}, got {', '.join(unknown)}")
+    ids, own = micro_batch["input_ids"], micro_batch.get("response_mask", None)
+    kw = dict(logit_controls, temperature=temperature)
+    index = kw.pop("allowed_index", None)
+    if index is not None:
+        if index.shape != ids.shape:
+            raise ValueError(f"allowed_index {tuple(index.shape)} does not lie beside input_ids {tuple(ids.shape)}")
+        index = F.pad(index[:, 1:], (0, 1), value=-1)
+    if indices is None:
+        return LogitControls(ids, attention_mask=micro_batch["attention_mask"], response_mask=own,
+                             allowed_index=None if index is None else index.reshape(-1), **kw)
+    packed = [None if x is None else x.flatten()[indices] for x in (ids, own, index)]
+    return LogitControls(packed[0], cu_seqlens, response_mask=packed[1], allowed_index=packed[2], **kw)
+
+
 def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_entropy: bool = False, *,
                        use_remove_padding: bool = True, use_fused_kernels: bool = True, ulysses_sp_size: int = 1,
-                       skip_prompt_rows: bool = False, **_unused):
+                       skip_prompt_rows: bool = False, logit_controls: dict | None = None, **_unused):
     """Forward one micro-batch through a model whose ``forward`` is the fused-head one
     (``forward_with_hip_backend``) and return ``(entropy, log_probs)``, both ``[batch, seq]``: position 0 is 0,
     position t holds log P(token_t | tokens before it).  Mirror of the fused branches of ``fsdp_model_forward``
@@ -121,8 +145,19 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
     this build.
 
     ``skip_prompt_rows`` (no counterpart in the reference, off by default; fused branches only): positions where
-    ``micro_batch["response_mask"]`` ``[batch, seq]`` is zero come back as 0 and their rows stay out of the head."""
+    ``micro_batch["response_mask"]`` ``[batch, seq]`` is zero come back as 0 and their rows stay out of the head.
+
+    ``logit_controls`` (no counterpart in the reference; ``use_fused_kernels=False`` only): what the sampler did to the logits
+    before it drew the tokens, so that they are scored under the distribution that they were drawn from: the penalties, biases
+    and masks of ``axon_amd.utils.torch.controls.LogitControls`` by their names there, penalties for all or ``[batch]``,
+    ``allowed_index`` ``[batch, seq]`` with the mask that token t was drawn under at position t.  A history is the tokens of
+    ``attention_mask`` before the token; those of ``micro_batch["response_mask"]`` (all, where there is none) count as generated.
+    A token that the controls take out has log-probability ``-inf``."""
     head_kwargs = {}
+    if logit_controls is not None and use_fused_kernels:
+        raise ValueError("logit_controls need the logits: use_fused_kernels=False")
+    from axon_amd.utils.torch.controls import controlled_logprobs_from_logits
+
     if skip_prompt_rows and use_fused_kernels and "response_mask" in micro_batch:
         # hidden position t predicts token t + 1: keep it when the response mask covers t + 1
         keep = F.pad(micro_batch["response_mask"][:, 1:] != 0, (0, 1), value=False)
@@ -154,8 +189,12 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
             ent_packed = output.entropy.reshape(-1) if calculate_entropy else None
         else:  # the model writes the logits (forward_utils.py:287-292)
             output = module(input_ids=fwd_ids, attention_mask=None, position_ids=fwd_pos, use_cache=False)
-            lp_packed, ent_packed = _from_logits(output.logits.squeeze(0), labels.reshape(-1), temperature,
-                                                 calculate_entropy)
+            logits = output.logits.squeeze(0)
+            if logit_controls is None:
+                lp_packed, ent_packed = _from_logits(logits, labels.reshape(-1), temperature, calculate_entropy)
+            else:
+                controls = _controls_of(logit_controls, micro_batch, temperature, indices, cu_seqlens)
+                lp_packed, ent_packed = controlled_logprobs_from_logits(logits, labels.reshape(-1), controls)
         log_probs = rmpad_postprocess(lp_packed, indices=indices, batch_size=batch_size, seqlen=seqlen)
         entropy = None
         if calculate_entropy:
@@ -171,6 +210,10 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
         return entropy, log_probs
     # padded, non-fused (forward_utils.py:294-304): logits[:, t] predicts token t + 1
     output = module(input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids, use_cache=False)
+    if logit_controls is not None:  # all rows; the last one's label is outside the vocabulary, what it has is dropped
+        controls = _controls_of(logit_controls, micro_batch, temperature)
+        lp, ent = controlled_logprobs_from_logits(output.logits, F.pad(input_ids[:, 1:], (0, 1), value=-1), controls)
+        return (shift_to_token_positions(ent) if calculate_entropy else None), shift_to_token_positions(lp)
     lp, ent = _from_logits(output.logits[:, :-1, :], input_ids[:, 1:], temperature, calculate_entropy)
     log_probs = F.pad(lp, (1, 0), value=0.0)
     entropy = F.pad(ent, (1, 0), value=0.0) if calculate_entropy else None

@@ -113,3 +113,21 @@ def test_the_c_entry_points_check_their_arguments():
     assert fwd(w=None) == fwd(wb=ws - 1) == fwd(w=p + 8) == -3
     assert lib.axon_controls_logprob_bwd(p, 0, 100, 2, 100, ctypes.byref(s), p, 1, None, p, p, p, 100, None) == -1
     assert lib.axon_controls_apply_bwd(p, 0, 100, 2, 100, ctypes.byref(s), None, 100, p, 100, None) == -1
+
+
+def test_a_trainers_forward_refuses_what_it_cannot_score():
+    from axon_amd.utils.fsdp.forward_utils import fsdp_model_forward
+
+    ids = torch.zeros(2, 4, dtype=torch.int64)
+    batch = {"input_ids": ids, "attention_mask": torch.ones_like(ids), "position_ids": ids}
+    model = lambda **kw: type("Out", (), {"logits": torch.zeros(*kw["input_ids"].shape, 9)})()
+    with pytest.raises(ValueError, match="use_fused_kernels=False"):
+        fsdp_model_forward(model, batch, 1.0, logit_controls={"repetition_penalty": 1.1})
+    for padding in (True, False):
+        how = dict(use_fused_kernels=False, use_remove_padding=padding)
+        with pytest.raises(ValueError, match="got temperature, token_ids"):
+            fsdp_model_forward(model, batch, 1.0, logit_controls={"temperature": 2.0, "token_ids": ids}, **how)
+        with pytest.raises(ValueError, match="allowed_index"):
+            fsdp_model_forward(model, batch, 1.0, logit_controls={"allowed_index": ids[:, 1:]}, **how)
+        with pytest.raises(_lib.AxonAmdError):  # there is no kernel for logits on the host
+            fsdp_model_forward(model, batch, 1.0, logit_controls={"repetition_penalty": 1.1}, **how)

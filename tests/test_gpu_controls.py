@@ -398,3 +398,140 @@ def test_tensors_changed_before_the_backward_are_noticed():
     for t in (lp, out):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             t.sum().backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n_seqs,tokens_before", [(63, 0), (64, 3), (65, 0), (200, 2)])
+def test_rows_find_their_sequence(n_seqs, tokens_before, dtype):
+    """Few sequences and many, some empty, some tokens before the first: a penalty and a temperature for each."""
+    g = gen(n_seqs)
+    lens = torch.randint(0, 5, (n_seqs,), generator=g, device="cuda")
+    lens[0], lens[-1] = 0, 3
+    cu = torch.cat([torch.zeros(1, device="cuda"), lens.cumsum(0)]).int() + tokens_before
+    n, v = int(cu[-1]), 700
+    tokens = torch.randint(0, v, (n,), generator=g, device="cuda")
+    z = (torch.randn(n, v, generator=g, device="cuda") * 4).to(dtype)
+    rep, freq, t = (torch.rand(n_seqs, generator=g, device="cuda") + 0.7 for _ in range(3))
+    ctl = LogitControls(tokens, cu, repetition_penalty=rep, frequency_penalty=freq, temperature=t)
+    spans = [(i, a, p + 1) for i, (a, b) in enumerate(zip(cu.tolist(), cu[1:].tolist())) for p in range(a, b)]
+    want, slope, size = R.controlled(z[tokens_before:], spans, tokens, repetition=rep, frequency=freq, temperature=t)
+    got = controlled_logits(z, ctl)[tokens_before:].double().cpu()
+    bound = Y_ROUNDINGS * size + (2.0 ** -8 * want.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30
+    assert ((got - want).abs() <= bound).all()
+    labels = torch.randint(0, v, (n,), generator=g, device="cuda")
+    lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
+    zero = torch.zeros(n - tokens_before)
+    want_lp, want_ent, _, _ = R.scored(want, slope, labels[tokens_before:], zero, zero)
+    assert ((lp[tokens_before:].double().cpu() - want_lp).abs() <= LP_TOL).all()
+    assert ((ent[tokens_before:].double().cpu() - want_ent).abs() <= ENT_TOL).all()
+
+
+def test_more_rows_than_runs_have_room_for():
+    """300000 rows of 50 ids: the longest runs, many sequences in each; every block of them is the first one."""
+    lens, v, blocks = [37, 1, 62, 0, 25, 75], 50, 1500
+    z, args, ref = case(7, lens, v, "all", torch.float32, bias=4)
+    n = z.shape[0]
+    out, slope, _ = reference(z, ref)
+    cu = args.pop("cu_seqlens")[:-1].long()
+    cu = (cu[None] + n * torch.arange(blocks, device="cuda")[:, None]).reshape(-1)
+    args.update(token_ids=args["token_ids"].repeat(blocks), response_mask=args["response_mask"].repeat(blocks),
+                cu_seqlens=torch.cat([cu, torch.tensor([n * blocks], device="cuda")]).int())
+    labels = torch.randint(0, v, (n,), generator=gen(8), device="cuda")
+    g_lp, g_ent = torch.randn(n, generator=gen(9), device="cuda"), torch.randn(n, generator=gen(10), device="cuda")
+    lp, ent, grad, size = (x.cuda() for x in R.scored(out, slope, labels, g_lp, g_ent))
+    x = z.repeat(blocks, 1).requires_grad_(True)
+    got_lp, got_ent = controlled_logprobs_from_logits(x, labels.repeat(blocks), LogitControls(**args))
+    d, = torch.autograd.grad([got_lp, got_ent], x, [g_lp.repeat(blocks), g_ent.repeat(blocks)])
+    shaped = lambda t: t.detach().double().view(blocks, n, *t.shape[1:])
+    banned = lp == -math.inf
+    assert torch.equal(shaped(got_lp) == -math.inf, banned.expand(blocks, n))
+    assert ((shaped(got_lp) - lp).abs()[:, ~banned] <= LP_TOL).all() and ((shaped(got_ent) - ent).abs() <= ENT_TOL).all()
+    assert ((shaped(d) - grad).abs() <= 2 * ENT_TOL * size + 1e-30).all()
+
+
+@pytest.mark.parametrize("remove_padding", [True, False])
+@pytest.mark.parametrize("left", [False, True])
+def test_a_rollout_scored_as_it_was_sampled(remove_padding, left):
+    """A decoder samples under controls; the trainer's forward gives its tokens the log-probabilities that they were drawn with."""
+    from types import SimpleNamespace
+
+    from axon_amd.utils.fsdp.forward_utils import fsdp_model_forward
+
+    g = gen(5)
+    b, t, h, v, prompt = 3, 14, 32, 700, 4
+    emb, w = torch.randn(v, h, generator=g, device="cuda"), torch.randn(v, h, generator=g, device="cuda")
+    lens = [14, 9, 6]
+    keep = torch.rand(5, v, generator=g, device="cuda") < 0.6
+    rep, freq = torch.rand(b, generator=g, device="cuda") + 0.9, torch.rand(b, generator=g, device="cuda") * 0.5
+    common = dict(repetition_penalty=rep, frequency_penalty=freq, presence_penalty=0.2, bias_ids=torch.tensor([3, 9], device="cuda"),
+                  bias=torch.tensor([1.0, -math.inf], device="cuda"), allowed=R.pack(keep))
+    logits_of = lambda ids: emb[ids].float() @ w.t() / h ** 0.5
+    # sampled step by step: a sequence's tokens so far, and the mask of the state that it is in
+    rows, states, drawn = [], [], []
+    for i, n in enumerate(lens):
+        ids = torch.randint(0, v, (prompt,), generator=g, device="cuda")
+        state, lp = [-1] * prompt, [0.0] * prompt
+        for p in range(prompt, n):
+            s = p % 6 - 1
+            one = LogitControls(ids, torch.tensor([0, p], dtype=torch.int32, device="cuda"), positions="last", temperature=0.8,
+                                response_mask=(torch.arange(p, device="cuda") >= prompt).float(),
+                                allowed_index=torch.tensor([s], device="cuda"),
+                                **dict(common, repetition_penalty=rep[i : i + 1], frequency_penalty=freq[i : i + 1]))
+            y = controlled_logits(logits_of(ids[-1:]), one)[0]
+            token = torch.multinomial(torch.softmax(y, 0), 1, generator=g)
+            assert s < 0 or keep[s, token]
+            lp.append(torch.log_softmax(y.double(), 0)[token].item())
+            state.append(s)
+            ids = torch.cat([ids, token])
+        rows.append(ids), states.append(state), drawn.append(lp)
+    place = lambda x, fill, i: ([fill] * (t - lens[i]) + list(x)) if left else (list(x) + [fill] * (t - lens[i]))
+    batch = {"input_ids": torch.tensor([place(rows[i].tolist(), 0, i) for i in range(b)], device="cuda"),
+             "attention_mask": torch.tensor([place([1] * lens[i], 0, i) for i in range(b)], device="cuda"),
+             "response_mask": torch.tensor([place([0] * prompt + [1] * (lens[i] - prompt), 0, i) for i in range(b)], device="cuda"),
+             "position_ids": torch.zeros(b, t, dtype=torch.int64, device="cuda")}
+    index = torch.tensor([place(states[i], -1, i) for i in range(b)], device="cuda")
+    want = torch.tensor([place(drawn[i], 0.0, i) for i in range(b)], dtype=torch.float64)
+    bent = torch.ones(v, device="cuda", requires_grad=True)
+
+    class Model(torch.nn.Module):
+        def forward(self, input_ids=None, attention_mask=None, position_ids=None, use_cache=False):
+            return SimpleNamespace(logits=logits_of(input_ids) * bent)
+
+    how = dict(use_remove_padding=remove_padding, use_fused_kernels=False)
+    ent, lp = fsdp_model_forward(Model(), batch, 0.8, True, logit_controls=dict(common, allowed_index=index), **how)
+    none, again = fsdp_model_forward(Model(), batch, 0.8, False, logit_controls=dict(common, allowed_index=index), **how)
+    own = batch["response_mask"] != 0
+    assert none is None and torch.equal(again[own], lp[own]) and lp.shape == ent.shape == (b, t) and (lp[:, 0] == 0).all()
+    assert torch.isfinite(ent[own]).all()
+    # the logits differ by the order of a product's 32 terms (32 2^-24 of 20 before the division: 4e-5), both ways
+    assert ((lp.detach().double().cpu() - want).abs()[own.cpu()] <= 2 * (LP_TOL + 4e-5)).all()
+    torch.where(own, lp, 0.0).sum().backward()
+    assert torch.isfinite(bent.grad).all() and (bent.grad != 0).any() and bent.grad[9] == 0
+    _, plain = fsdp_model_forward(Model(), batch, 0.8, False, **how)
+    assert not torch.allclose(plain[own], lp[own], atol=0.05)
+
+
+@pytest.mark.parametrize("masks", ["none", "states", "shared"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("share", [0.0, 0.3, 1.0])
+def test_rows_without_an_upstream_gradient(masks, dtype, share):
+    """Their gradient is 0, whatever they hold; their tokens belong to the histories of the rows behind them all the same."""
+    lens, v = [60, 1, 140, 95], 9001
+    z, args, ref = case(17, lens, v, "all", dtype, masks=masks, bias=5, per_seq=True)
+    n = z.shape[0]
+    out, slope, _ = reference(z, ref)
+    labels = torch.randint(0, v, (n,), generator=gen(1), device="cuda")
+    on = torch.rand(n, generator=gen(2), device="cuda") < share
+    g_lp = torch.where(on, torch.randn(n, generator=gen(3), device="cuda"), 0.0)
+    g_ent = torch.where(on & (torch.rand(n, generator=gen(4), device="cuda") < 0.5), 1.0, 0.0)
+    _, _, grad, size = R.scored(out, slope, labels, g_lp, g_ent)
+    z[~on] = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=dtype)[torch.arange(n, device="cuda")[~on] % 3, None]
+    z.requires_grad_(True)
+    o = controlled_logprobs_from_logits(z, labels, LogitControls(**args))
+    got, = torch.autograd.grad(o, z, [g_lp, g_ent])
+    off = ~on.cpu()
+    assert (got[~on] == 0).all()
+    bound = 2 * ENT_TOL * size + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30
+    assert ((got.double().cpu() - grad).abs() <= bound)[~off].all()
+    alone, = torch.autograd.grad(controlled_logprobs_from_logits(z, labels, LogitControls(**args))[0], z, g_lp)
+    assert (alone[~on] == 0).all()

@@ -434,3 +434,142 @@ def test_a_student_under_a_grammar_learns_from_a_teacher_under_it():
     check(r.losses, losses, loss_bound(size) + 4e-5 * size)
     check(d, grad * slope, (grad_bound(grad, gsize, torch.float32) + 8e-5 * gsize) * slope + 1e-30)
     assert (d[~keep] == 0).all()
+
+
+@pytest.mark.parametrize("n,v,dtype,on_share", [
+    (50000, 40, torch.float32, 0.5),     # more rows than the workgroups' lists hold at once
+    (100001, 24, torch.bfloat16, 1.0),
+    (100001, 24, torch.bfloat16, 0.01),
+    (530, 34001, torch.bfloat16, 0.9),   # rows of 68 KB: more than there are workgroups
+    (3, 500003, torch.bfloat16, 1.0),    # longer rows than are held
+    (2, 250001, torch.float32, 1.0),
+])
+def test_weighted_rows_that_go_round(n, v, dtype, on_share):
+    z, ids, lq = batch(n + v, n, v, 3, dtype)
+    w = torch.rand(n, generator=gen(1), device="cuda") + 0.5
+    w[torch.rand(n, generator=gen(2), device="cuda") >= on_share] = 0.0
+    losses, covered, grad, gsize, size = reference(z, ids, lq, "forward", "rest", 0.5, 1.0, w)
+    on = w.cpu() != 0
+    z[w == 0] = math.nan
+    z.requires_grad_(True)
+    r = distillation_loss_from_logits(z, ids, lq, w)
+    d, = torch.autograd.grad(r.loss, z)
+    check(r.losses[on.cuda()], losses[on], loss_bound(size[on]))
+    check(r.covered[on.cuda()], covered[on], 2 * P_REL * covered[on] + 1e-30)
+    assert (r.losses.cpu()[~on] == 0).all() and (r.covered.cpu()[~on] == 0).all() and (d.cpu()[~on] == 0).all()
+    check(d[on.cuda()], grad[on], grad_bound(grad[on], gsize[on], dtype))
+
+
+@pytest.mark.parametrize("n,v", [(5, 900), (1000, 50257)])
+def test_weights_that_are_all_zero(n, v):
+    z = torch.full((n, v), math.nan, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    ids, lq = torch.zeros(n, 4, dtype=torch.int64, device="cuda"), torch.zeros(n, 4, device="cuda")
+    r = distillation_loss_from_logits(z, ids, lq, torch.zeros(n, device="cuda"))
+    d, = torch.autograd.grad(r.loss, z)
+    assert r.loss == 0 and (r.losses == 0).all() and (r.covered == 0).all() and (d == 0).all()
+
+
+@pytest.mark.parametrize("k", [1, 2, 257, 512])
+@pytest.mark.parametrize("v", [9, 4099, 70001])
+def test_one_token_given_many_times(k, v):
+    """Outcomes of one token: the teacher's probabilities differ, the student's is the same for all."""
+    n = 5
+    z = torch.randn(n, v, generator=gen(k), device="cuda") * 3
+    ids = torch.full((n, k), v // 2, dtype=torch.int64, device="cuda")
+    lq = torch.log_softmax(torch.randn(n, k + 1, generator=gen(k + 1), device="cuda"), 1)[:, :k]
+    w = torch.rand(n, generator=gen(3), device="cuda") + 0.5
+    losses, covered, grad, gsize, size = reference(z, ids, lq, "forward", "rest", 0.5, 1.0, w)
+    z.requires_grad_(True)
+    r = distillation_loss_from_logits(z, ids, lq, w)
+    check(r.losses, losses, loss_bound(size))
+    check(torch.autograd.grad(r.loss, z)[0], grad, grad_bound(grad, gsize, torch.float32))
+    each, _ = distillation_from_logits(z, ids, lq)
+    check(each, losses, loss_bound(size))
+    check(torch.autograd.grad(each, z, w)[0], grad, grad_bound(grad, gsize, torch.float32))
+
+
+@pytest.mark.parametrize("base,step", [(-2.0 ** 31, 256.0), (2.0 ** 31, 256.0), (-1e9, 64.0), (-3e38, 2.0 ** 104)])
+@pytest.mark.parametrize("v", [700, 20011])
+def test_logits_far_from_zero(base, step, v):
+    """Logits whose reference in units of log2 leaves no room for differences: they are formed first."""
+    n, k = 6, 8
+    z = base + step * torch.randint(0, 3, (n, v), generator=gen(v), device="cuda").float()
+    ids = torch.randint(0, v, (n, k), generator=gen(v + 1), device="cuda")
+    lq = torch.log_softmax(torch.randn(n, k + 1, generator=gen(3), device="cuda"), 1)[:, :k]
+    w = torch.rand(n, generator=gen(4), device="cuda") + 0.5
+    for divergence, how in (("forward", dict(tail="rest")), ("jsd", dict(tail="drop"))):
+        losses, covered, grad, gsize, size = reference(z, ids, lq, divergence, how["tail"], 0.5, 1.0, w)
+        x = z.clone().requires_grad_(True)
+        r = distillation_loss_from_logits(x, ids, lq, w, divergence=divergence, **how)
+        check(r.losses, losses, loss_bound(size))
+        check(r.covered, covered, 2 * P_REL * covered + 1e-30)
+        check(torch.autograd.grad(r.loss, x)[0], grad, grad_bound(grad, gsize, torch.float32))
+        each, _ = distillation_from_logits(x, ids, lq, divergence=divergence, **how)
+        check(each, losses, loss_bound(size))
+        check(torch.autograd.grad(each, x, w)[0], grad, grad_bound(grad, gsize, torch.float32))
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_as_a_term_of_the_trainers_loss(padded):
+    from axon_amd.models.fsdp_models import CausalLM
+    from axon_amd.protocol import DataProto
+    from axon_amd.trainer.algos.loss import agg_loss
+
+    n, v = 120, 500
+    z, ids, lq = batch(9, n, v, 8, torch.float32)
+    shape = (4, 30) if padded else (n,)
+    g = gen(4)
+    rand = lambda: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    lp, ent, old, adv = rand(), rand().abs(), rand(), rand()
+    mask = (torch.rand(*shape, generator=g, device="cuda") < 0.7).float()
+    cu = None if padded else torch.tensor([0, 50, 90, 120], dtype=torch.int32, device="cuda")
+    z[mask.reshape(-1) == 0] = math.nan  # what is no response has a loss that does not count
+    x = z.clone().requires_grad_(True)
+
+    def run(args, losses):
+        data = DataProto.from_dict(tensors={"old_log_probs": old, "advantages": adv, "response_mask": mask},
+                                   meta_info={} if padded else {"cu_seqlens": cu})
+        meta = {"loss_fn": "ppo", "loss_fn_args": args, "dp_replicas": 2, "n_micro_batches": 4, "temperature": 1.0}
+        module = lambda inputs, m: {"log_probs": lp, "entropys": ent, **({} if losses is None else {"distill_losses": losses})}  # noqa: E731
+        return CausalLM.forward_backward_fn(module, data, meta)
+
+    plain, metrics = run({}, None)
+    assert not any("distill" in key for key in metrics)
+    losses = distillation_from_logits(x, ids, lq)[0].view(shape)
+    loss, metrics = run({"distill_coef": 0.25}, losses)
+    want = agg_loss(torch.where(mask != 0, losses, 0.0), mask, cu_seqlens=cu)
+    # three roundings of fp32 numbers of the losses' size; both replicas count
+    assert abs(loss.item() - plain.item() - 2 * 0.25 * want.item()) <= 4 * 2.0 ** -24 * 2 * (abs(plain.item()) + abs(loss.item()) + 1)
+    assert metrics["distill_loss"] == 4 * want.item() and metrics["distill_coef"] == 0.25
+    d, = torch.autograd.grad(loss, x, retain_graph=True)
+    ref, = torch.autograd.grad(want, x)
+    keep = mask.reshape(-1) != 0
+    assert ((d - 0.5 * ref).abs()[keep] <= 4 * 2.0 ** -24 * ref.abs()[keep] + 1e-30).all() and (d[~keep] == 0).all()
+    with pytest.raises(ValueError, match="distill_losses"):
+        run({"distill_coef": 0.25}, None)
+    with pytest.raises(ValueError, match="do not lie beside"):
+        run({"distill_coef": 0.25}, losses.reshape(-1)[:-1])
+
+
+@pytest.mark.parametrize("n,v", [(40, 9001), (6, 151937), (700, 515)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_positions_without_an_upstream_gradient(n, v, dtype):
+    """Their gradient is 0, whatever they hold."""
+    z, ids, lq = batch(n + v, n, v, 12, dtype)
+    up = torch.randn(n, generator=gen(7), device="cuda")
+    up[torch.rand(n, generator=gen(8), device="cuda") < 0.5] = 0.0
+    up[0], up[1] = 0.0, -0.0
+    on = up != 0
+    losses, _, grad, gsize, size = reference(z, ids, lq, "forward", "rest", 0.5, 1.0, up)
+    z[~on] = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=dtype)[torch.arange(n, device="cuda")[~on] % 3, None]
+    z.requires_grad_(True)
+    got, _ = distillation_from_logits(z, ids, lq)
+    d, = torch.autograd.grad(got, z, up)
+    assert (d[~on] == 0).all()
+    check(got[on], losses[on.cpu()], loss_bound(size[on.cpu()]))
+    check(d[on], grad[on.cpu()], grad_bound(grad[on.cpu()], gsize[on.cpu()], dtype))
+    twin = z.detach().clone().requires_grad_(True)
+    over, _ = distillation_from_logits(twin * 1.0, ids, lq, inplace_backward=True)
+    assert torch.equal(torch.autograd.grad(over, twin, up)[0], d)
+    r = distillation_loss_from_logits(z, ids, lq, on.float())
+    assert (torch.autograd.grad(r.loss, z, torch.tensor(0.0, device="cuda"))[0] == 0).all()
