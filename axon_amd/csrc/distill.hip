@@ -9,6 +9,11 @@
 //   dz_j = (sum_{o: id_o = j} G_o - p_j sum_o G_o + [j is not given] G_rest p_j / p_rest) / T
 // so that a row is its softmax statistics, k gathered logits, and one multiple of p_j for all tokens that are not given.  What
 // the student has left over is summed over these tokens themselves: 1 minus the rest has no digits where it matters.
+//
+// Bound by memory (a large copy takes 4.8 TB/s).  Where the losses' weights are known a row is read once and written once: 4096 x 151936
+// bf16, a third of weight 0, 446 us (2.08 GB, 4.7 TB/s); 2500 x 201088 bf16 446 us (4.5 TB/s, a twentieth of a row is read twice); 1500 x
+// 151936 fp32 425 us (4.3 TB/s, a third of a row twice).  Where they are not, it is read for the statistics and again for the gradient:
+// 2047 x 50257 bf16 42 us (4.9 TB/s, what rows that start on 2 bytes reach) and 93 us (4.4 TB/s).
 #include "logits_rows.h"
 #include <type_traits>
 
@@ -841,7 +846,8 @@ int grad_parts(int64_t n, int64_t vocab, int eb) {
   const int64_t p = fill < work ? fill : work;
   return (int)(p < 1 ? 1 : (p < kMaxParts ? p : kMaxParts));
 }
-// ... and of the forward: about 2048 pieces, what the part holds at once, none of them beyond what LDS describes.
+// ... and of the forward: about 2048 pieces, what the part holds at once, none of them beyond what LDS describes.  One part where there
+// are as many rows finishes them without a second launch (2047 x 50257 bf16 with gradient 144 us, 158 with it).
 int stats_parts(int64_t n, int64_t vocab, int eb) {
   const int64_t fill = 2048 / (n > 0 ? n : 1), work = vocab * eb / (4 * 16 * kBlock), least = (vocab * eb / 16 + kMaxShare - 1) / kMaxShare;
   int64_t p = fill < work ? fill : work;
@@ -926,8 +932,10 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
 
 namespace {
 
-// Rows of up to 64 KB: 192 threads that hold the row, three workgroups on a compute unit; up to 128 KB: 448, two; longer: 960, one, of
-// which 375 KB are held and the rest is read twice.
+// Rows of up to 66 KB: 192 threads that hold the row, three workgroups on a compute unit; up to 133 KB: 448, two; longer: 960, one, of
+// which 375 KB are held and the rest is read twice.  More workgroups hide each other's outcomes, as many as hold their rows: 8192 x 33792
+// bf16 take 250, 269 and 428 us with 192, 448 and 960 threads, 4096 x 65536 217 with 448 and 268 with 960.  Beyond kMaxTiles the marks
+// of the given tokens have no room: such rows take the statistics and the gradient one after the other.
 constexpr int64_t kMaxRowVecs = kMaxTiles * 960;
 template <typename T, bool REST>
 int launch_rows(const void* logits, int64_t ld, int64_t n, int64_t vocab, const Teacher& t, const RowOut& out, void* dlogits, int64_t ld_d,

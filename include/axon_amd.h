@@ -770,7 +770,7 @@ int axon_controls_apply_bwd(const void* logits, int dtype, int64_t ld, int64_t n
 /* log softmax(out)[label] (0 for a label outside the vocabulary) and the entropy (may be NULL) of softmax(out), fp32; a row
  * that nothing is left of: -inf, 0 and no gradient.  stats [3][n]: what the backward reads.  Workspace 16-byte aligned.
  * bwd_follows: whether the last rows are left in the cache for a backward (the results are the same).
- * dlogits may be the logits' own storage; g_logprob, g_entropy may be NULL. */
+ * dlogits may be the logits' own storage; g_logprob, g_entropy may be NULL.  A row whose gradients are 0 is not read: 0. */
 int64_t axon_controls_logprob_workspace_bytes(int64_t n, int64_t vocab);
 int axon_controls_logprob_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const axon_controls* controls,
                               const void* labels, int labels_are_i64, float* logprob, float* entropy, float* stats, void* workspace,
@@ -788,10 +788,12 @@ int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t
  * left of both, 1 - sum q and the student's tokens that are not given, as one more outcome (AXON_DISTILL_REST).  An id that
  * comes twice is two outcomes.  1 <= k <= AXON_MAX_TOKEN_IDS, vocab at most 3145728.
  *   losses, covered [n]: the divergence, and the student's probability of the given tokens.  grads [n][k], coef [4][n]: what
- *        the backward reads.  Workspace 16-byte aligned.
+ *        the backward reads.  Workspace 16-byte aligned.  bwd_follows: whether the last rows are left in the cache for a
+ *        backward (the results are the same).
  *   weights [n] (may be NULL in _fwd): a row of weight 0 is not looked at: loss, covered and gradient are 0.
  *   _bwd: dlogits from the losses' gradients upstream [n], or, with weights, weights[row] * upstream[0] (upstream NULL: 1).  With
  *        `ready` the caller has the gradient of upstream 1 in dlogits, and nothing is written where upstream[0] is that.
+ *        A row whose gradient is 0 by that is not read.
  *        dlogits may be the logits' own storage.
  *   _loss: loss[0] = sum weights * losses, and dlogits (NULL: not wanted) of that loss beside it. */
 enum { AXON_DISTILL_FORWARD = 0, AXON_DISTILL_REVERSE = 1, AXON_DISTILL_JSD = 2 };
