@@ -756,7 +756,7 @@ int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, 
     static const int resident = resident_of(kernel, WAVES * kWave);                                                        \
     const int groups = (chunks + WAVES - 1) / WAVES, run = A && of_rows ? 1 : run_of(n, groups, resident);                 \
     const int64_t grid = (n + run - 1) / run * groups;                                                                     \
-    if (grid >= INT32_MAX) return AXON_ERR_SHAPE;                                                                          \
+    if (grid * (WAVES * kWave) > UINT32_MAX) return AXON_ERR_SHAPE;                                                                          \
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(WAVES * kWave), 0, st, static_cast<const T*>(logits), ld, (int)n, (int)vocab, \
                        chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out);           \
   } while (0)

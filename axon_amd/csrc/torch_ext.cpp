@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -803,7 +804,7 @@ class Controls {
       if (token_ids->numel() >= INT32_MAX) refuse(kWhat, "more tokens than 32 bits count");
       c_.n_tokens = token_ids->numel();
       hold(kTokens, token_ids->detach().contiguous());
-      c_.token_ids = held_[kTokens].data_ptr();
+      c_.token_ids = c_.n_tokens > 0 ? held_[kTokens].data_ptr() : nullptr;  // no tokens, no history
       c_.token_ids_i64 = is_i64(*token_ids);
     }
     if (own_mask) {
@@ -860,6 +861,8 @@ class Controls {
         c_.allowed_index_i64 = is_i64(*allowed_index);
       }
     }
+    for (const Tensor& t : held_)
+      if (t.defined() && t.is_cuda()) made_on_ = c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
   }
 
   // For n rows of v logits that lie where `like` does.
@@ -867,10 +870,16 @@ class Controls {
     axon_controls c = c_;
     for (const Tensor& t : held_)
       if (t.defined() && t.device() != like.device()) refuse(what, "logits and controls live on different devices");
-    if (c.every_position ? (c.token_ids && n != c.n_tokens) : (c.n_seqs >= 0 && n != c.n_seqs))
+    if (made_on_) {  // what is held may be a copy that nobody else knows of: its memory waits for other streams' launches too
+      const c10::Stream now = c10::impl::VirtualGuardImpl(like.device().type()).getStream(like.device());
+      if (now != *made_on_)
+        for (const Tensor& t : held_)
+          if (t.defined()) t.record_stream(now);
+    }
+    if (c.every_position ? (held_[kTokens].defined() && n != c.n_tokens) : (c.n_seqs >= 0 && n != c.n_seqs))
       refuse(what, std::to_string(n) + " rows of logits for controls of " +
                        (c.every_position ? std::to_string(c.n_tokens) + " positions" : std::to_string(c.n_seqs) + " sequences"));
-    if (c.every_position && !c.cu_seqlens && c.uniform_len == 0 && c.n_seqs >= 0)
+    if (n > 0 && c.every_position && !c.cu_seqlens && c.uniform_len == 0 && c.n_seqs >= 0)
       refuse(what, "values for each sequence need token_ids or cu_seqlens");
     if (c.n_seqs < 0) c.n_seqs = 0;
     if (c.allowed) {
@@ -905,6 +914,7 @@ class Controls {
 
   axon_controls c_{};
   std::array<Tensor, kCount> held_;
+  c10::optional<c10::Stream> made_on_;
   int64_t words_ = 0;
 };
 

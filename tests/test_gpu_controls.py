@@ -535,3 +535,46 @@ def test_rows_without_an_upstream_gradient(masks, dtype, share):
     assert ((got.double().cpu() - grad).abs() <= bound)[~off].all()
     alone, = torch.autograd.grad(controlled_logprobs_from_logits(z, labels, LogitControls(**args))[0], z, g_lp)
     assert (alone[~on] == 0).all()
+
+
+@pytest.mark.parametrize("shape", [(3, 0), (0,)])
+def test_sequences_without_tokens(shape):
+    """A decoder's first step, before there is a history, and batches of nothing."""
+    tokens = torch.zeros(shape, dtype=torch.int64, device="cuda")
+    rows, v = (3 if len(shape) == 2 else 1), 700
+    z = torch.randn(rows, v, generator=gen(1), device="cuda")
+    kw = dict(repetition_penalty=1.3, frequency_penalty=0.5, temperature=0.5)
+    want = z / 0.5
+    for ctl in (LogitControls(tokens, positions="last", **kw),
+                LogitControls(tokens.reshape(-1), torch.zeros(rows + 1, dtype=torch.int32, device="cuda"), positions="last", **kw)):
+        assert torch.equal(controlled_logits(z, ctl), want)
+        lp, ent = controlled_logprobs_from_logits(z, torch.zeros(rows, dtype=torch.int64, device="cuda"), ctl)
+        assert ((lp - torch.log_softmax(want.double(), 1)[:, 0]).abs() <= LP_TOL).all() and torch.isfinite(ent).all()
+    nothing = LogitControls(tokens, **kw)
+    empty = torch.zeros((*shape, v), device="cuda", requires_grad=True)
+    assert controlled_logits(empty, nothing).shape == (*shape, v)
+    lp, ent = controlled_logprobs_from_logits(empty, tokens, nothing)
+    assert lp.shape == ent.shape == shape
+    assert torch.autograd.grad(lp.sum() + ent.sum(), empty)[0].shape == empty.shape
+    with pytest.raises(ValueError, match="rows of logits"):
+        controlled_logits(z.repeat(2, 1), nothing)
+
+
+def test_controls_that_are_let_go_while_another_stream_reads_them():
+    v, n = 20000, 400
+    z = torch.randn(n, v, generator=gen(1), device="cuda")
+    tokens = torch.randint(0, v, (n,), generator=gen(2), device="cuda")
+    cu = torch.tensor([0, 130, n], device="cuda")  # 64 bits: a copy is held
+    make = lambda: LogitControls(tokens.reshape(1, n).expand(2, n)[:1].reshape(-1), cu, repetition_penalty=torch.full((2,), 1.3, device="cuda").double(),
+                                 frequency_penalty=0.5)
+    want = controlled_logits(z, make())
+    side = torch.cuda.Stream()
+    ctl = make()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        out = controlled_logits(z, ctl)
+    del ctl
+    junk = [torch.full((k,), 7, dtype=torch.int32, device="cuda") for k in (3, 2, 1, 4, 64, 128) * 20]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and len(junk) == 120

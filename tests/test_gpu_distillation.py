@@ -573,3 +573,13 @@ def test_positions_without_an_upstream_gradient(n, v, dtype):
     assert torch.equal(torch.autograd.grad(over, twin, up)[0], d)
     r = distillation_loss_from_logits(z, ids, lq, on.float())
     assert (torch.autograd.grad(r.loss, z, torch.tensor(0.0, device="cuda"))[0] == 0).all()
+
+
+def test_batches_of_nothing():
+    z = torch.zeros(2, 0, 50, device="cuda", requires_grad=True)
+    ids, lq = torch.zeros(2, 0, 4, dtype=torch.int64, device="cuda"), torch.zeros(2, 0, 4, device="cuda")
+    losses, covered = distillation_from_logits(z, ids, lq)
+    assert losses.shape == covered.shape == (2, 0)
+    assert torch.autograd.grad(losses.sum(), z)[0].shape == z.shape
+    r = distillation_loss_from_logits(z, ids, lq, torch.zeros(2, 0, device="cuda"))
+    assert r.loss == 0 and torch.autograd.grad(r.loss, z)[0].shape == z.shape
