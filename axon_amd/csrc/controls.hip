@@ -620,9 +620,9 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   }
 }
 
-// A row's chunks together, by a wavefront, in 64 bits (4 us for 187 rows of 75 chunks, 7 for 4096): log-probability of the label, entropy, and what the backward reads: the
+// A row's chunks together, by a wavefront, in 64 bits: log-probability of the label, entropy, and what the backward reads: the
 // largest y (before the temperature), the sum of 2^((y - M) log2(e) / T), the entropy.  A row that nothing is left of has
-// M = 0, of which its -inf are far enough.
+// M = 0, of which its -inf are far enough.  4 us for 187 rows of 75 chunks, 7 for 4096: latency.
 __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int vocab, int chunks, axon_controls c, RowIo io,
                                                                  float* logprob, float* entropy, float* stats) {
   const int row = (int)(blockIdx.x * kWaves + threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
@@ -750,15 +750,15 @@ int launch(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, 
   const bool adj = (penalties && c.token_ids) || c.n_bias > 0, mask = c.allowed != nullptr;
   const int chunks = chunks_of(vocab, dtype);
   const bool of_rows = !c.every_position;
-#define AXON_CONTROLS(T, A, M, WAVES)                                                                                      \
-  do {                                                                                                                     \
-    const auto kernel = controls_kernel<T, MODE, A, M, WAVES>;                                                             \
-    static const int resident = resident_of(kernel, WAVES * kWave);                                                        \
-    const int groups = (chunks + WAVES - 1) / WAVES, run = A && of_rows ? 1 : run_of(n, groups, resident);                 \
-    const int64_t grid = (n + run - 1) / run * groups;                                                                     \
-    if (grid * (WAVES * kWave) > UINT32_MAX) return AXON_ERR_SHAPE;                                                                          \
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(WAVES * kWave), 0, st, static_cast<const T*>(logits), ld, (int)n, (int)vocab, \
-                       chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out);           \
+#define AXON_CONTROLS(T, A, M, WAVES)                                                                                                           \
+  do {                                                                                                                                          \
+    const auto kernel = controls_kernel<T, MODE, A, M, WAVES>;                                                                                  \
+    static const int resident = resident_of(kernel, WAVES * kWave);                                                                             \
+    const int groups = (chunks + WAVES - 1) / WAVES, run = A && of_rows ? 1 : run_of(n, groups, resident);                                      \
+    const int64_t grid = (n + run - 1) / run * groups;                                                                                          \
+    if (grid * (WAVES * kWave) > UINT32_MAX) return AXON_ERR_SHAPE;                                                                             \
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(WAVES * kWave), 0, st, static_cast<const T*>(logits), ld, (int)n, (int)vocab,         \
+                       chunks, run, c, io, static_cast<const T*>(other), ld_other, static_cast<T*>(out), ld_out);                               \
   } while (0)
 #define AXON_CONTROLS_OF(T)                                  \
   do {                                                       \

@@ -520,8 +520,8 @@ __device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teache
 
 // RESIDENT: workgroups on a compute unit.
 template <typename T, bool REST, int ROW, int NREG, int NLDS, int RESIDENT>
-__global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void distill_row_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out,
-                                                                     T* __restrict__ dlogits, int64_t ld_d) {
+__global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void distill_row_kernel(
+    const T* __restrict__ logits, int64_t ld, int vocab, Teacher t, RowOut out, T* __restrict__ dlogits, int64_t ld_d) {
   __shared__ RowLds<ROW> s;
   __shared__ int s_count[256 * RESIDENT], s_list[2][kWave];
   __shared__ uint4 s_tiles[NLDS * ROW];  // an array of its own: reads of the rest do not wait for what is on its way here
