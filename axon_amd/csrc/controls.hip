@@ -12,8 +12,8 @@
 // loaded at whatever boundary a row of an odd vocabulary starts on, so that lanes keep their ids.
 //
 // Bound by memory, which takes 6.4 TB/s read and 4.8 copied in rows of whole vectors, 4.9 and 4.7 at a boundary of 2 bytes.
-//   log-probability and entropy   1500 x 151936 fp32 181 us (5.0 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 275 to
-//     290 us, without controls 225 (5.5 TB/s): what the penalties take of every element, and waves whose loads wait for arithmetic
+//   log-probability and entropy   1500 x 151936 fp32 181 us (5.0 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 285 to
+//     305 us, without controls 225 (5.5 TB/s): what the penalties take of every element, and waves whose loads wait for arithmetic
 //     (four to a SIMD: five spill, 666 us); 2047 x 50257 bf16 71 us, without controls 43 (4.8 TB/s): short runs
 //   their gradient                1500 x 151936 fp32 334 us (5.5 TB/s, in part from the cache in front of the memory), 2047 x 50257 bf16 88 us
 //   written out                   61 x 201088 fp32, histories of 4000 tokens, 30 us (17 without controls); 1024 x 32768 bf16, 1500
@@ -82,6 +82,7 @@ __device__ __forceinline__ void wave_sync() {
 }
 constexpr float kBanned = -1e30f;  // stands for -inf where a product with it has to stay finite
 constexpr float kFar = 1e9f;       // a reference in log2 units whose rounding (64) leaves the exponentials in range
+constexpr float kNear = 8.f;       // ... and of which a term is off by at most 2^-22 ln 2
 constexpr float kNoLogit = -3.402823466e38f;  // the reference of a set without a logit: any there is is at least as large
 
 // A token of a history: its id, or -1 where it counts for nothing; bit 30 where the model has generated it.  (Both loads at once.)
@@ -412,6 +413,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
     }
   }
   float ref = kNoLogit;
+  bool above_before = false;
   for (int r = 0; r < rows; ++r) {
     if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
       if (r > 0) {
@@ -482,9 +484,9 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
 
     if constexpr (MODE == kStats) {
       float4* const part = io.parts + row * chunks + chunk;
-      // The sum of N logits of each lane, and weighted by their exponents, against the reference in use: the largest logit of an
-      // earlier row of this chunk will do as long as the sum stays in range.  Against c = ref k rounded it is one
-      // instruction per element, and what c is off by is the same for all of them and taken back at the end.
+      // The sum of N logits of each lane, and weighted by their exponents, against the reference m: the largest logit of an
+      // earlier row of this chunk will do as long as the sum stays in range and the terms that count are near it.  Against
+      // c = m k rounded it is one instruction per element, and what c is off by is the same for all of them and taken back.
       auto statistics = [&](auto n, auto& y, uint32_t bits) {
         constexpr int N = decltype(n)::value;
         auto largest = [&] {
@@ -493,10 +495,11 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           for (int i = 1; i < N; ++i) m = fmaxf(m, y[i]);
           return wave_max(m);
         };
-        if (!(ref > kBanned)) ref = largest();
-        const float cc = ref * k;
+        constexpr bool kCarried = N == kLaneIds;  // the largest of a few is soon found, and says nothing about other rows
+        float m = kCarried && ref > kBanned ? ref : largest();
+        const float cc = m * k;
         float s4[4] = {}, e4[4] = {}, s = 0.f, e = 0.f;
-        bool plain = fabsf(cc) < kFar && ref > kBanned;
+        bool plain = fabsf(cc) < kFar && m > kBanned, above = false;
         if (plain) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -506,29 +509,34 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           }
           s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
           e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
-          const float off = fmaf(ref, k, -cc), back = __builtin_amdgcn_exp2f(-off);  // 2^(y k - c) = 2^((y - ref) k + off)
+          const float off = fmaf(m, k, -cc), back = __builtin_amdgcn_exp2f(-off);  // 2^(y k - c) = 2^((y - m) k + off)
           e = fmaf(-off, s, e) * back;
           s *= back;
-          plain = s > 0x1p-80f && s < 0x1p100f && e == e;
+          // e / s: how far the terms that count are from the reference, of which their exponents carry the rounding
+          plain = s > 0x1p-80f && s < 0x1p100f && fabsf(e) <= kNear * s;
+          above = e > kNear * s;
         }
-        if (!plain) {  // another scale, logits far from 0, or infinite, or not numbers: by differences, what is banned at -inf
+        if (!plain) {  // another scale (a likely token), logits far from 0, infinite, or not numbers: by differences, what is banned at -inf
           asm volatile("" : "+v"(bits));
 #pragma unroll
           for (int i = 0; i < N; ++i) y[i] = pick(bit_mask(bits, i), y[i], -INFINITY);
-          ref = largest();
-          if (!(ref > -INFINITY)) ref = kNoLogit;
+          m = largest();
+          if (!(m > -INFINITY)) m = kNoLogit;
 #pragma unroll
           for (int i = 0; i < 4; ++i) s4[i] = e4[i] = 0.f;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const float d = (y[i] - ref) * k, f = __builtin_amdgcn_exp2f(d);
+            const float d = (y[i] - m) * k, f = __builtin_amdgcn_exp2f(d);
             s4[i & 3] += f;
             e4[i & 3] = fmaf(f, fmaxf(d, kTiny), e4[i & 3]);
           }
           s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
           e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
         }
-        if (lane == 0) *part = make_float4(ref, s, e, 0.f);
+        const bool once = kCarried && above && !above_before;  // a likely token: what is like the rows before it stays the reference
+        if (kCarried && !once) ref = m;
+        if (kCarried) above_before = once;
+        if (lane == 0) *part = make_float4(m, s, e, 0.f);
       };
       if (MASK && few) {
         float y[kFew];
@@ -621,7 +629,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
 }
 
 // A row's chunks together, by a wavefront, in 64 bits: log-probability of the label, entropy, and what the backward reads: the
-// largest y (before the temperature), the sum of 2^((y - M) log2(e) / T), the entropy.  A row that nothing is left of has
+// logarithm M of the sum of exponentials (before the temperature, rounded), the sum of 2^((y - M) log2(e) / T), the entropy.  A row that nothing is left of has
 // M = 0, of which its -inf are far enough.  4 us for 187 rows of 75 chunks, 7 for 4096: latency.
 __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int vocab, int chunks, axon_controls c, RowIo io,
                                                                  float* logprob, float* entropy, float* stats) {
@@ -657,9 +665,16 @@ __global__ __launch_bounds__(kBlock) void controls_finish_kernel(int n_rows, int
     M = 0.f;
   } else {
     const double ls = log2(s);
-    sum = (float)s;
     H = (float)((ls - e / s) * 0.6931471805599453);
     if (inside) lp = (float)((((double)io.label_y[row] - (double)M) * (double)k - ls) * 0.6931471805599453);
+    // for the backward against the logarithm of the sum: what is likely has an exponent near 0
+    const float near = (float)((double)M + ls / (double)k);
+    if (fabsf(near) <= 3.402823466e38f) {
+      sum = (float)exp2(ls - ((double)near - (double)M) * (double)k);
+      M = near;
+    } else {
+      sum = (float)s;
+    }
   }
   logprob[row] = lp;
   if (entropy != nullptr) entropy[row] = H;

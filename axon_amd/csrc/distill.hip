@@ -45,8 +45,9 @@ struct RowOut {
   int n;
 };
 
-// Sum of 2^((z - M) log2(e) / T) over a set of logits and their largest.
-struct Sum { float M, s; };
+// Sum of 2^((z - M) log2(e) / T) over a set of logits and their largest.  A thread's sum is in 64 bits: beside a likely token's
+// term every other addition to it would round at that term's size.
+struct Sum { float M; double s; };
 constexpr float kLowest = -3.402823466e38f;
 template <int N>
 __device__ __forceinline__ void fold(Sum& a, const float (&z)[8], float k) {
@@ -54,13 +55,13 @@ __device__ __forceinline__ void fold(Sum& a, const float (&z)[8], float k) {
 #pragma unroll
   for (int j = 1; j < N; ++j) m = fmaxf(m, z[j]);
   if (m > a.M) {
-    a.s *= __builtin_amdgcn_exp2f((a.M - m) * k);
+    a.s *= (double)__builtin_amdgcn_exp2f((a.M - m) * k);
     a.M = m;
   }
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((z[j] - a.M) * k);
-  a.s += s;
+  a.s += (double)s;
 }
 
 // The bytes that say which elements of a share's vectors are given, and the same for the few elements outside vectors.
@@ -234,7 +235,8 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
                                                                float4* __restrict__ parts, RowOut out, int cached_from) {
   extern __shared__ __align__(16) uint32_t s_given[];
   __shared__ uint32_t s_single;
-  __shared__ float red[2][kBlock / kWave];
+  __shared__ float red_m[kBlock / kWave];
+  __shared__ double red_s[kBlock / kWave];
   __shared__ Given s_row;
   const int row_i = blockIdx.x / n_parts, part = blockIdx.x % n_parts, tid = threadIdx.x;
   if (t.weights != nullptr && t.weights[row_i] == 0.f) {
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
   const uint8_t* const given = reinterpret_cast<const uint8_t*>(s_given);
   const T* body = row + sp.head;
   const float k = t.inv_t * kLog2e;
-  Sum st{kLowest, 0.f};
+  Sum st{kLowest, 0.0};
   auto one = [&](int q, float (&v)[8]) {
     if (REST) {
       const uint32_t out = given[q - sp.q_lo];
@@ -282,21 +284,21 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(const T* __restri
     fold<1>(st, v, k);
   }
   const float m = wave_max(st.M);
-  const float s = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
-  if ((tid & (kWave - 1)) == 0) { red[0][tid / kWave] = m; red[1][tid / kWave] = s; }
+  const double s = wave_sum_d(st.s * (double)__builtin_amdgcn_exp2f((st.M - m) * k));
+  if ((tid & (kWave - 1)) == 0) { red_m[tid / kWave] = m; red_s[tid / kWave] = s; }
   __syncthreads();
   if (n_parts == 1) {
     if (tid >= kWave) return;
     fetch_given<T, REST>(s_row, t, row_i, row, vocab, tid);
     const bool mine = tid < kBlock / kWave;
-    finish_row<REST>(s_row, t, out, row_i, mine ? red[0][tid] : kLowest, mine ? (double)red[1][tid] : 0.0, tid);
+    finish_row<REST>(s_row, t, out, row_i, mine ? red_m[tid] : kLowest, mine ? red_s[tid] : 0.0, tid);
     return;
   }
   if (tid != 0) return;
-  float M = red[0][0];
-  for (int w = 1; w < kBlock / kWave; ++w) M = fmaxf(M, red[0][w]);
+  float M = red_m[0];
+  for (int w = 1; w < kBlock / kWave; ++w) M = fmaxf(M, red_m[w]);
   double total = 0.0;
-  for (int w = 0; w < kBlock / kWave; ++w) total += (double)red[1][w] * __builtin_amdgcn_exp2f((red[0][w] - M) * k);
+  for (int w = 0; w < kBlock / kWave; ++w) total += red_s[w] * (double)__builtin_amdgcn_exp2f((red_m[w] - M) * k);
   parts[blockIdx.x] = make_float4(M, (float)total, (float)(total - (float)total), 0.f);
 }
 
@@ -422,7 +424,8 @@ struct RowLds {
   int heads[kAhead][kBuckets];  // chains of the ids that come for the first time
   uint32_t marks[kAhead][2][ROW];  // bit i % 32 of word i / 32: this thread's vector of tile i holds a given token
   uint32_t single[kAhead];         // a bit per element outside the vectors
-  float red_m[ROW / kWave], red_s[ROW / kWave];
+  double red_s[ROW / kWave];
+  float red_m[ROW / kWave];
   float lse, c_out;
   int is_far;
 };
@@ -496,8 +499,9 @@ __device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teache
   constexpr int kRowWaves = ROW / kWave;
   Given& gv = s.given[buf];
   const float k = t.inv_t * kLog2e, g = weight * t.inv_t;
-  const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest, part_s = lane < kRowWaves ? s.red_s[lane] : 0.f;
-  const RowCoefs r = finish_row<REST>(gv, t, out, row_i, part_m, (double)part_s, lane);
+  const float part_m = lane < kRowWaves ? s.red_m[lane] : kLowest;
+  const double part_s = lane < kRowWaves ? s.red_s[lane] : 0.0;
+  const RowCoefs r = finish_row<REST>(gv, t, out, row_i, part_m, part_s, lane);
   // p = 2^(z k - off) f with off = lse k rounded; far from 0 by the difference from lse
   const float off = r.lse * k;
   const bool is_far = !(fabsf(off) < kFar);
@@ -599,7 +603,8 @@ __global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void d
 
     // Statistics of a row.  Against a reference c = ref k rounded (ref: the largest of its given tokens' logits) an element is one
     // instruction beside its exponential, and what c is off by is taken back at the end.
-    float s4[4], cc = 0.f, ref = 0.f;
+    double terms = 0.0;  // of a vector's sums, in 64 bits: beside a likely token's term others would be rounded at its size
+    float cc = 0.f, ref = 0.f;
     uint32_t mark_lo = 0, mark_hi = 0;
     const auto marked = [&](int i) { return REST && ((i < 32 ? mark_lo >> i : mark_hi >> (i - 32)) & 1) != 0; };
     const auto begin_stats = [&](int j) {
@@ -608,12 +613,13 @@ __global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void d
       cc = ref * k;
       mark_lo = s.marks[buf][0][tid];
       mark_hi = s.marks[buf][1][tid];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s4[i] = 0.f;
+      terms = 0.0;
     };
     const auto add = [&](const uint4& r) {
+      float s2[2] = {};
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) s4[j & 3] += __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -cc));
+      for (int j = 0; j < kPer; ++j) s2[j & 1] += __builtin_amdgcn_exp2f(fmaf(Packed<T>::get(r, j), k, -cc));
+      terms += (double)(s2[0] + s2[1]);
     };
     const auto each_given = [&](int buf, int id0, int q, auto&& f) {  // f(element, number among the given) of vector q
       for (int h = s.heads[buf][q & (kBuckets - 1)]; h >= 0; h = s.given[buf].next[h]) {
@@ -634,7 +640,7 @@ __global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void d
         float x[8];
         read_left(j % kAhead, v, __builtin_ctzll(m) * ROW + tid, x);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) s4[e & 3] += __builtin_amdgcn_exp2f(fmaf(x[e], k, -cc));
+        for (int e = 0; e < kPer; ++e) terms += (double)__builtin_amdgcn_exp2f(fmaf(x[e], k, -cc));
       }
     };
     const auto add_beyond = [&](const RowView<T>& v) {  // tiles that are not held
@@ -648,11 +654,12 @@ __global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void d
     };
     const auto end_stats = [&](int j, const RowView<T>& v) {
       const bool single_in = tid < v.sp.n_scalar && !(REST && (s.single[j % kAhead] >> tid & 1));
-      if (single_in) s4[0] += __builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
-      float sum = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3])) * __builtin_amdgcn_exp2f(fmaf(-ref, k, cc)), m = ref;
-      if (!(fabsf(cc) < kFar && sum > 0x1p-60f && sum < 0x1p80f)) {
+      if (single_in) terms += (double)__builtin_amdgcn_exp2f(fmaf(single_z, k, -cc));
+      double sum = wave_sum_d(terms) * (double)__builtin_amdgcn_exp2f(fmaf(-ref, k, cc));
+      float m = ref;
+      if (!(fabsf(cc) < kFar && sum > 0x1p-60 && sum < 0x1p80)) {
         // another scale, logits far from 0, infinite, or not numbers: by differences from the largest, read again
-        Sum st{kLowest, 0.f};
+        Sum st{kLowest, 0.0};
 #pragma unroll 1
         for (int q = tid; q < v.sp.n_vec; q += ROW) {
           float x[8];
@@ -664,7 +671,7 @@ __global__ __launch_bounds__(ROW + kWave, RESIDENT * (ROW + kWave) / 256) void d
           fold<1>(st, x, k);
         }
         m = wave_max(st.M);
-        sum = wave_sum(st.s * __builtin_amdgcn_exp2f((st.M - m) * k));
+        sum = wave_sum_d(st.s * (double)__builtin_amdgcn_exp2f((st.M - m) * k));
       }
       if (lane == 0) { s.red_m[wave] = m; s.red_s[wave] = sum; }
     };
