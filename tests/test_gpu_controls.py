@@ -578,3 +578,30 @@ def test_controls_that_are_let_go_while_another_stream_reads_them():
     junk = [torch.full((k,), 7, dtype=torch.int32, device="cuda") for k in (3, 2, 1, 4, 64, 128) * 20]
     torch.cuda.synchronize()
     assert torch.equal(out, want) and len(junk) == 120
+
+
+@pytest.mark.parametrize("every", [1, 2, 7])
+@pytest.mark.parametrize("v", [5000, 32768])
+def test_likely_tokens_are_exact_to_single_precision(v, every):
+    """Rows with a likely token among rows without one.  An exponent of the terms that count is below 16, off by 2^-21 ln 2 (3.3e-7) at
+    most, and most are far below; exponentials and the sums of 32 and 64 terms add 2e-7, the last rounding 2^-24 of the result."""
+    n = 150
+    z = torch.randn(n, v, generator=gen(v + every), device="cuda") * 2
+    at = torch.randint(0, 1000, (n,), generator=gen(every), device="cuda")
+    rows = torch.arange(0, n, every, device="cuda")
+    z[rows, at[rows]] += 14.0 + 5.0 * torch.rand(len(rows), generator=gen(3), device="cuda")
+    labels = torch.where(torch.rand(n, generator=gen(4), device="cuda") < 0.5, at, torch.randint(0, v, (n,), generator=gen(5), device="cuda"))
+    tokens = torch.full((n,), v - 1, dtype=torch.int64, device="cuda")  # a history that says nothing of the others
+    ctl = LogitControls(tokens[None], presence_penalty=1.0)
+    y = z.double()
+    y[:, -1] -= 1.0
+    want = torch.log_softmax(y, 1)
+    z.requires_grad_(True)
+    lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
+    ref = want.gather(1, labels[:, None])[:, 0]
+    assert ((lp.double() - ref).abs() <= 5.5e-7 + 2.0 ** -24 * ref.abs()).all()
+    d, = torch.autograd.grad(lp.sum(), z)
+    p = want.exp()
+    grad = torch.zeros_like(p).scatter_(1, labels[:, None], 1.0) - p
+    # a probability: the logarithm's error, and that of its own exponent -log2 p (and of M, near it) in 2^-24
+    assert ((d.double() - grad).abs() <= p * (8e-7 + 2.0 ** -23 * want.abs()) + 2.0 ** -24 * grad.abs() + 1e-30).all()

@@ -583,3 +583,40 @@ def test_batches_of_nothing():
     assert torch.autograd.grad(losses.sum(), z)[0].shape == z.shape
     r = distillation_loss_from_logits(z, ids, lq, torch.zeros(2, 0, device="cuda"))
     assert r.loss == 0 and torch.autograd.grad(r.loss, z)[0].shape == z.shape
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("v", [5000, 151936])
+def test_likely_tokens_are_exact_to_single_precision(v, weighted):
+    """Rows with a likely token that the teacher knows: beside its term all others' additions would round at its size.  What is off in the
+    sum: the others' share by the roundings of z - M and of its product with log2(e), 2^-24 of up to 30 each, that of log2(e), 1.4e-8 of
+    it, and 2^-23 of the exponential (3.6e-6); the likely one's exponential and the factor that takes its reference's rounding back, 2^-23
+    each; the three additions within its vector, 2^-24 each (all other additions are in 64 bits)."""
+    n, k = 40, 6
+    z = torch.randn(n, v, generator=gen(v), device="cuda") * 2
+    at = torch.randint(0, v, (n,), generator=gen(1), device="cuda")
+    z[torch.arange(n, device="cuda"), at] += 14.0 + 4.0 * torch.rand(n, generator=gen(3), device="cuda")
+    t = torch.log_softmax(z + torch.randn(n, v, generator=gen(4), device="cuda"), 1)
+    ids = t.topk(k, 1).indices
+    lq = t.gather(1, ids)
+    z.requires_grad_(True)
+    if weighted:
+        r = distillation_loss_from_logits(z, ids, lq, torch.ones(n, device="cuda"), tail="drop")
+        got, total = r.losses, r.loss
+    else:
+        got, _ = distillation_from_logits(z, ids, lq, tail="drop")
+        total = got.sum()
+    log_p = torch.log_softmax(z.detach().double(), 1)
+    q = lq.double().exp()
+    want = (q * (lq.double() - log_p.gather(1, ids))).sum(1)
+    share = 1.0 - log_p.exp().amax(1)
+    lse_bound = 3.6e-6 * share + 7 * 2.0 ** -24
+    assert ((got.double() - want).abs() <= q.sum(1) * lse_bound + 2.0 ** -24 * want.abs()).all()
+    d, = torch.autograd.grad(total, z)
+    p = log_p.exp()
+    grad = p * q.sum(1, keepdim=True) - torch.zeros_like(p).scatter_(1, ids, q)
+    # a probability: z - lse, its product with log2(e) and log2(e) itself, 2.5 2^-24 of the logarithm, and 2^-23; its factor and the product
+    # with it, three roundings; a given token's own q: three as well
+    bound = p * (lse_bound[:, None] + 5 * 2.0 ** -24 + 2.5 * 2.0 ** -24 * log_p.abs())
+    bound = bound + 3 * 2.0 ** -24 * (p + torch.zeros_like(p).scatter_(1, ids, q)) + 1e-30
+    assert ((d.double() - grad).abs() <= bound).all()
