@@ -12,10 +12,10 @@
 // loaded at whatever boundary a row of an odd vocabulary starts on, so that lanes keep their ids.
 //
 // Bound by memory, which takes 6.4 TB/s read and 4.8 copied in rows of whole vectors, 4.9 and 4.7 at a boundary of 2 bytes.
-//   log-probability and entropy   1500 x 151936 fp32 181 us (5.0 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 285 to
+//   log-probability and entropy   1500 x 151936 fp32 179 us (5.1 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 285 to
 //     305 us, without controls 225 (5.5 TB/s): what the penalties take of every element, and waves whose loads wait for arithmetic
-//     (four to a SIMD: five spill, 666 us); 2047 x 50257 bf16 71 us, without controls 43 (4.8 TB/s): short runs
-//   their gradient                1500 x 151936 fp32 334 us (5.5 TB/s, in part from the cache in front of the memory), 2047 x 50257 bf16 88 us
+//     (four to a SIMD: five spill, 666 us); 2047 x 50257 bf16 73 us, without controls 43 (4.8 TB/s): short runs
+//   their gradient                1500 x 151936 fp32 332 us (5.5 TB/s, in part from the cache in front of the memory), 2047 x 50257 bf16 88 us
 //   written out                   61 x 201088 fp32, histories of 4000 tokens, 30 us (17 without controls); 1024 x 32768 bf16, 1500
 //     tokens, 39 us (24 without controls): a workgroup's history and its terms are trips to memory and through
 //     LDS before the row's arithmetic, which the four other workgroups of a compute unit hide in part
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
       }
     }
   }
-  float ref = kNoLogit;
+  float refs[2] = {kNoLogit, kNoLogit};  // of whole rows, and of rows of few ids
   bool above_before = false;
   for (int r = 0; r < rows; ++r) {
     if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
@@ -495,8 +495,8 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           for (int i = 1; i < N; ++i) m = fmaxf(m, y[i]);
           return wave_max(m);
         };
-        constexpr bool kCarried = N == kLaneIds;  // the largest of a few is soon found, and says nothing about other rows
-        float m = kCarried && ref > kBanned ? ref : largest();
+        float& ref = refs[N == kFew];
+        float m = ref > kBanned ? ref : largest();
         const float cc = m * k;
         float s4[4] = {}, e4[4] = {}, s = 0.f, e = 0.f;
         bool plain = fabsf(cc) < kFar && m > kBanned, above = false;
@@ -533,9 +533,9 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
           s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
           e = wave_sum((e4[0] + e4[1]) + (e4[2] + e4[3]));
         }
-        const bool once = kCarried && above && !above_before;  // a likely token: what is like the rows before it stays the reference
-        if (kCarried && !once) ref = m;
-        if (kCarried) above_before = once;
+        const bool once = above && !above_before;  // a likely token: what is like the rows before it stays the reference
+        if (!once) ref = m;
+        above_before = once;
         if (lane == 0) *part = make_float4(m, s, e, 0.f);
       };
       if (MASK && few) {
