@@ -114,7 +114,7 @@ struct RowIo {
 // The additive terms of a wavefront's ids in LDS, in the order in which the lanes read them: 16 bytes of neighbouring
 // lanes lie side by side.
 template <int PER>
-__device__ __forceinline__ int slot(int off) {
+__device__ __forceinline__ constexpr int slot(int off) {
   return PER == 4 ? off : (off & ~511) | ((off & 4) << 6) | ((off & 0x1f8) >> 1) | (off & 3);
 }
 
@@ -288,6 +288,12 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   // 288 us, 307 with all elements of all rows.  kFew is what the row's registers hold one element to a vector.
   constexpr int kFew = 4;
   static_assert(kFew <= kVecs, "");
+  // The lane's id number `bit` as an offset from the wavefront's first, and the next one of those that are left: behind the last
+  // it is an id of the lane still, so that what is addressed by it lies in the wavefront's own terms.
+  auto offset_of = [&](int bit) { return (uint32_t)((bit / kPer * kWave + lane) * kPer + bit % kPer); };
+  constexpr uint32_t kLastId = 1u << (kLaneIds - 1);
+  static_assert((kLaneIds - 1) / kPer < kVecs && slot<kPer>(((kLaneIds - 1) / kPer * kWave + kWave - 1) * kPer + kPer - 1) < kIds, "");
+  auto first_of = [&](uint32_t left) { return __builtin_ctz(left | kLastId); };
   typename Unaligned<T>::Raw raw[kVecs], raw_g[MODE == kApplyGrad ? kVecs : 1];
   auto is_few = [&](uint32_t keep) {
     if (MODE != kStats || !MASK) return false;
@@ -318,8 +324,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
 #pragma unroll
       for (int i = 0; i < kFew; ++i, x &= x - 1) {
         raw[i] = typename Unaligned<T>::Raw{};
-        const int bit = __builtin_ctz(x | 0x80000000u);
-        if (x != 0) Unaligned<T>::set(raw[i], 0, from + r * ld + (uint32_t)((bit / kPer * kWave + lane) * kPer + bit % kPer));
+        if (x != 0) Unaligned<T>::set(raw[i], 0, from + r * ld + offset_of(first_of(x)));
       }
       return;
     }
@@ -544,11 +549,11 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
         float label_y = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kFew; ++i, x &= x - 1) {
-          const int bit = __builtin_ctz(x | 0x80000000u);
+          const int bit = first_of(x);
           y[i] = Unaligned<T>::get(raw[i], 0);
           if (ADJ && touched != 0) {
             const float slope = repeats && (seen >> bit & 1) ? (y[i] > 0.f ? inv_rep : rep) : 1.f;
-            y[i] = fmaf(y[i], slope, -__uint_as_float(adj[slot<kPer>((bit / kPer * kWave + lane) * kPer + bit % kPer)]));
+            y[i] = fmaf(y[i], slope, -__uint_as_float(adj[slot<kPer>((int)offset_of(bit))]));
           }
           if (x != 0 && bit == label_at) label_y = y[i];
           y[i] = x != 0 ? y[i] : kBanned;
