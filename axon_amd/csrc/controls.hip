@@ -357,15 +357,15 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
     if (c.token_ids != nullptr) {
       const auto count = [&](auto id_of, auto own_of) {
         constexpr int kBatch = 8;  // loads in flight per thread
-        for (int i0 = from + tid; i0 < upto; i0 += kThreads * kBatch) {
+        for (int left = upto - from - tid; left > 0; left -= kThreads * kBatch) {  // counted down: a position plus a step may pass 32 bits
           int off[kBatch];
           bool own[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int i = i0 + b * kThreads, at = min(i, upto - 1);
+            const int ahead = left - b * kThreads, at = upto - max(ahead, 1);
             const int64_t id = id_of(at);
             own[b] = own_of(at);
-            off[b] = i < upto && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
+            off[b] = ahead > 0 && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
           }
 #pragma unroll
           for (int b = 0; b < kBatch; ++b)

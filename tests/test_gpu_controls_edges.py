@@ -47,3 +47,17 @@ def test_rows_of_few_ids_under_penalties(v, dtype, most):
     assert gone[3] and torch.equal(lp.cpu() == -math.inf, gone)
     assert ((lp.double().cpu() - lp_want).abs()[~gone] <= LP_TOL).all()
     assert ((ent.double().cpu() - ent_want).abs() <= ENT_TOL).all()
+
+
+def test_a_history_that_ends_where_32_bits_do():
+    """The longest history that is taken, 2^31 - 2 tokens (8.6 GB), most of them padding."""
+    n, v = 2 ** 31 - 2, 8
+    tokens = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    at = torch.tensor([0, 1, 4096, 2 ** 30, n - 8192, n - 4097, n - 4096, n - 513, n - 512, n - 2, n - 1], device="cuda")
+    ids = torch.tensor([0, 1, 0, 2, 3, 3, 4, 3, 5, 5, 6], device="cuda")
+    tokens[at] = ids.int()
+    z = torch.linspace(-2.0, 2.0, v, device="cuda")[None]
+    ctl = LogitControls(tokens[None], positions="last", frequency_penalty=0.5, presence_penalty=0.25, repetition_penalty=2.0)
+    count = torch.bincount(ids, minlength=v).float()[None]
+    want = torch.where(count > 0, torch.where(z > 0, z / 2, z * 2), z) - 0.5 * count - 0.25 * (count > 0)
+    assert (controlled_logits(z, ctl) - want).abs().max() <= 8 * 2.0 ** -24 * 5
