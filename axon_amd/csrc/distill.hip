@@ -8,7 +8,9 @@
 //   jsd      m = b q + (1 - b) p:  sum b q (lq - lm) + (1 - b) p (lp - lm)   G = (1 - b) p (lp - lm)
 //   dz_j = (sum_{o: id_o = j} G_o - p_j sum_o G_o + [j is not given] G_rest p_j / p_rest) / T
 // so that a row is its softmax statistics, k gathered logits, and one multiple of p_j for all tokens that are not given.  What
-// the student has left over is summed over these tokens themselves: 1 minus the rest has no digits where it matters.
+// the student has left over is summed over these tokens themselves: 1 minus the rest has no digits where it matters.  With
+// what is left as an outcome their p_j is never formed: p_j / p_rest = 2^((z_j - lse_rest) log2(e) / T) against the log-sum-exp of
+// what is left, times G_rest - p_rest sum_o G_o, which stays in range however little that is.
 //
 // Bound by memory (a large copy takes 4.8 TB/s).  Where the losses' weights are known a row is read once and written once: 4096 x 151936
 // bf16, a third of weight 0, 446 us (2.08 GB, 4.7 TB/s); 2500 x 201088 bf16 446 us (4.5 TB/s, a twentieth of a row is read twice); 1500 x
@@ -35,12 +37,13 @@ __device__ __forceinline__ int teacher_id(const Teacher& t, int64_t at, int voca
   return id >= 0 && id < vocab ? (int)id : -1;
 }
 
-// What a row leaves for its backward: the student's log-sum-exp (of z, before the temperature) in two parts, the multiple of
-// p_j for tokens that are not given, and that for those that are.
+// What a row leaves for its backward: the log-sum-exp (of z, before the temperature) in two parts, of what is not given where that is
+// an outcome, else of the whole row; the multiple of 2^((z - lse) log2(e) / T) for tokens that are not given, and that for those that
+// are (0 where what is left is an outcome: the p_j sum G of a given token is in its own gradient then).
 enum Coef { kLse, kRest, kOut, kIn, kCoefs };
 struct RowOut {
   float *losses, *covered;
-  float* grads;  // [n][k]: G of every given token
+  float* grads;  // [n][k]: G of every given token, less p_j sum G of its id where what is left is an outcome
   float* coef;   // [kCoefs][n]
   int n;
 };
@@ -120,7 +123,7 @@ constexpr int kAgain = -2;
 struct Given {
   int id[kMaxIds];               // -1: a filler
   int16_t next[kMaxIds];         // kAgain: an id that has come before, or none; else -1, or the next of its chain
-  float a[kMaxIds], b[kMaxIds];  // the teacher's log-probabilities, then G; the logits, then what is written in their place
+  float a[kMaxIds], b[kMaxIds];  // the teacher's log-probabilities, then G; the logits, then p, then what is written in their place
   float best, best_q;            // the largest of either
   double sum, sum_q;             // REST: of exp((z - best) / T), every token once, and of q; else of exp(lq - best_q)
 };
@@ -172,49 +175,59 @@ __device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_
 }
 
 // The outcomes of a row in 64 bits, by one wavefront, from the statistics that its lanes have of parts of the row (REST: of what is not
-// given): losses, G (also in s.a), and the row's coefficients.
-struct RowCoefs { float lse, rest, c_out, c_in; };
+// given): losses, G (also in s.a), p (in s.b), and the row's coefficients.
+struct RowCoefs { float lse, rest, c_out; double sum_g; };
 template <bool REST>
 __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const RowOut& out, int row_i, float part_m, double part_s, int lane) {
   const float k = t.inv_t * kLog2e;
   const double inv_t = (double)t.inv_t;
-  const float best = s.best, M = fmaxf(wave_max(part_m), best);
-  // the whole range of 64 bits: what is left may be next to nothing
-  const float d = fmaxf((part_m - M) * k, -2000.f), n = rintf(d);
-  const double s_rest = wave_sum_d(ldexp(part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
-  const double s_all = REST && best > -INFINITY ? s_rest + s.sum * exp64(((double)best - (double)M) * inv_t) : s_rest;
+  // The parts against the largest of themselves: what is left over may be next to nothing beside what is given.
+  const float best = s.best, M_parts = wave_max(part_m), M = fmaxf(M_parts, best);
+  const float d = fmaxf((part_m - M_parts) * k, -2000.f), n = rintf(d);
+  const double s_parts = wave_sum_d(ldexp(part_s * (double)__builtin_amdgcn_exp2f(d - n), (int)n));
+  const double below = ((double)M_parts - (double)M) * inv_t, s_in_all = s_parts > 0.0 ? s_parts * exp64(below) : s_parts;
+  const double s_all = REST && best > -INFINITY ? s_in_all + s.sum * exp64(((double)best - (double)M) * inv_t) : s_in_all;
   const double ln_s = s_all > 0.0 ? log64(s_all) : (double)NAN;  // a row of -inf alone has no softmax
   const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE ? (double)s.best_q + log64(s.sum_q) : 0.0;
   double loss = 0.0, sum_g = 0.0, covered = 0.0;
 #pragma unroll 1
   for (int i = lane; i < t.k; i += kWave) {
     Term o{0.0, 0.0};
+    double p = 0.0;
     if (s.id[i] >= 0) {
       const double lp = ((double)s.b[i] - (double)M) * inv_t - ln_s;
       o = outcome(t, (double)s.a[i] - norm_q, lp);
-      covered += exp64(lp);
+      p = exp64(lp);
+      covered += p;
     }
     loss += o.loss;
     sum_g += o.g;
     s.a[i] = (float)o.g;
-    out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
+    s.b[i] = (float)p;
+    if (!REST) out.grads[(int64_t)row_i * t.k + i] = (float)o.g;
   }
   loss = wave_sum_d(loss);
   sum_g = wave_sum_d(sum_g);
   covered = wave_sum_d(covered);
-  double out_scale = 0.0;
+  // of the parts, against which the gradient of what is not given is formed; of what a row of no such logits has, the whole row's
+  const bool some = REST && s_parts > 0.0;
+  const double ln_ref = some ? log64(s_parts) : ln_s;
+  const float M_ref = some ? M_parts : M;
+  RowCoefs r;
+  r.lse = (float)((double)M_ref + ln_ref / inv_t);
+  r.rest = (float)((((double)M_ref - (double)r.lse) * inv_t + ln_ref) * 1.4426950408889634);
   if (REST) {
-    const double lp_rest = log64(s_rest) - ln_s;
+    const double lp_rest = some ? below + ln_ref - ln_s : log64(s_parts) - ln_s;
     const Term o = outcome(t, log64(fmax(1.0 - s.sum_q, 0.0)), lp_rest);
     loss += o.loss;
     sum_g += o.g;
-    out_scale = s_rest > 0.0 ? o.g * exp64(-lp_rest) : 0.0;
+    r.c_out = some ? (float)(o.g - exp64(lp_rest) * sum_g) : (float)(0.0 * s_all);
+    for (int i = lane; i < t.k; i += kWave)
+      out.grads[(int64_t)row_i * t.k + i] = s.next[i] == kAgain ? s.a[i] : (float)((double)s.a[i] - (double)s.b[i] * sum_g);
+  } else {
+    r.c_out = (float)-sum_g;
   }
-  RowCoefs r;
-  r.lse = (float)((double)M + ln_s / inv_t);
-  r.rest = (float)((((double)M - (double)r.lse) * inv_t + ln_s) * 1.4426950408889634);
-  r.c_out = (float)(out_scale - sum_g);
-  r.c_in = (float)-sum_g;
+  r.sum_g = sum_g;
   if (lane == 0) {
     out.losses[row_i] = (float)loss;
     out.covered[row_i] = (float)covered;
@@ -222,7 +235,7 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
     c[(int64_t)kLse * out.n] = r.lse;
     c[(int64_t)kRest * out.n] = r.rest;
     c[(int64_t)kOut * out.n] = r.c_out;
-    c[(int64_t)kIn * out.n] = r.c_in;
+    c[(int64_t)kIn * out.n] = REST ? 0.f : r.c_out;
   }
   wave_sync();
   return r;
@@ -367,7 +380,8 @@ __global__ __launch_bounds__(kBlock) void distill_grad_kernel(const T* logits, i
     }
     if (!first) continue;
     where[u] = id;
-    again[u] = fmaf(prob(Row<T>::one(row + id)), c_in, g * total);
+    const float p = prob(Row<T>::one(row + id));  // against what is left it may be any number, of which c_in takes nothing
+    again[u] = fmaf(p > 1.f ? 1.f : p, c_in, g * total);
   }
   __syncthreads();  // nothing of the row is written before these are read
   const T* body = row + sp.head;
@@ -506,9 +520,9 @@ __device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teache
   const float off = r.lse * k;
   const bool is_far = !(fabsf(off) < kFar);
   const float f = __builtin_amdgcn_exp2f((is_far ? 0.f : (float)((double)off - (double)r.lse * (double)k)) - r.rest);
-  const float base = is_far ? r.lse : off, c_in = g * r.c_in * f;
+  const float c_in = -g * (float)r.sum_g;
   if (lane == 0) {
-    s.lse = base;
+    s.lse = is_far ? r.lse : off;
     s.is_far = is_far;
     s.c_out = g * r.c_out * f;
   }
@@ -517,8 +531,7 @@ __device__ __forceinline__ void settle_row(RowLds<ROW>& s, int buf, const Teache
     float total = gv.a[i];
 #pragma unroll 8
     for (int j = i + 1; j < t.k; ++j) total += gv.id[j] == gv.id[i] ? gv.a[j] : 0.f;
-    const float z = gv.b[i], p = __builtin_amdgcn_exp2f(is_far ? (z - base) * k : fmaf(z, k, -base));
-    gv.b[i] = fmaf(p, c_in, g * total);
+    gv.b[i] = fmaf(gv.b[i], c_in, g * total);
   }
 }
 

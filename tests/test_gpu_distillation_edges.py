@@ -1,0 +1,111 @@
+"""Distillation where teacher or student have next to nothing left, against its definition in 64 bits, by logarithms throughout."""
+
+import math
+
+import pytest
+import torch
+
+from axon_amd.utils.torch.distillation import distillation_from_logits, distillation_loss_from_logits
+
+pytestmark = pytest.mark.gpu
+
+# As derived beside the tests of ordinary rows: a sum of exponentials, its logarithm absolutely, and every probability.
+P_REL = 4e-5
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def reference(z, ids, lq, divergence, tail, temperature=1.0, beta=0.5, q_rest=None):
+    """(losses, gradient of their sum, size of the losses' terms, size of the gradient's) of ids that differ."""
+    z, ids, lq = z.detach().double().cpu(), ids.cpu().long(), lq.double().cpu()
+    n, v = z.shape
+    ok = (ids >= 0) & (ids < v)
+    at = torch.where(ok, ids, torch.zeros_like(ids))
+    log_p = torch.log_softmax(z / temperature, 1)
+    given = torch.zeros(n, v, dtype=torch.int64).scatter_add_(1, at, ok.long()) > 0
+    lq = torch.where(ok, lq, -math.inf)
+    lp = torch.where(ok, log_p.gather(1, at), -math.inf)
+    left = torch.where(given, -math.inf, log_p)
+    if tail == "rest":
+        lp_rest = torch.logsumexp(left, 1, keepdim=True)
+        q_rest = (1.0 - lq.exp().sum(1)).clamp(min=0.0) if q_rest is None else q_rest
+        lq, lp = torch.cat([lq, q_rest.log()[:, None]], 1), torch.cat([lp, lp_rest], 1)
+    q, p = lq.exp(), lp.exp()
+    zero = torch.zeros_like(p)
+    if divergence == "forward":
+        terms, G = torch.where(q > 0, q * (lq - lp), zero), -q
+        size, gsize = torch.where(q > 0, q * (lq.abs() + lp.abs() + 1), zero), q
+    elif divergence == "reverse":
+        terms = torch.where(p > 0, p * (lp - lq), zero)
+        G = torch.where(p > 0, terms + p, zero)
+        size = torch.where(p > 0, p * (lq.abs() + lp.abs() + 1), zero)
+        gsize = size
+    else:
+        lm = (beta * q + (1 - beta) * p).log()
+        mine = torch.where(p > 0, (1 - beta) * p * (lp - lm), zero)
+        terms, G = torch.where(q > 0, beta * q * (lq - lm), zero) + mine, mine
+        gsize = torch.where(p > 0, p * (lp.abs() + lm.abs() + 1), zero)
+        size = torch.where(q > 0, q * (lq.abs() + lm.abs() + 1), zero) + gsize
+    p_all, k = log_p.exp(), ids.shape[1]
+    total, total_size = G.sum(1, keepdim=True), gsize.sum(1, keepdim=True)
+    d = torch.zeros(n, v, dtype=torch.float64).scatter_add_(1, at, torch.where(ok, G[:, :k], 0.0)) - p_all * total
+    dsize = torch.zeros(n, v, dtype=torch.float64).scatter_add_(1, at, torch.where(ok, gsize[:, :k], 0.0)) + p_all * total_size
+    if tail == "rest":
+        # by differences of the logits: beside the type's lowest value 64 bits have no room for the logarithm of a sum
+        share = torch.where(lp_rest > -math.inf, torch.softmax(torch.where(given, -math.inf, z / temperature), 1), 0.0)
+        d, dsize = d + share * G[:, -1:], dsize + share * gsize[:, -1:]
+    return terms.sum(1), d / temperature, size.sum(1), dsize / temperature
+
+
+def agrees(z, ids, lq, ref, dtype, **how):
+    """Both entry points, losses and gradients."""
+    losses, grad, size, gsize = ref
+    loss_bound = 2 * P_REL * size + 1e-12
+    grad_bound = 4 * P_REL * gsize + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30
+    x = z.clone().requires_grad_(True)
+    got, _ = distillation_from_logits(x, ids, lq, **how)
+    r = distillation_loss_from_logits(x, ids, lq, torch.ones(len(z), device="cuda"), **how)
+    for values, total in ((got, got.sum()), (r.losses, r.loss)):
+        assert ((values.detach().double().cpu() - losses).abs() <= loss_bound).all(), how
+        d, = torch.autograd.grad(total, x)
+        assert ((d.double().cpu() - grad).abs() <= grad_bound).all(), how
+    again, = torch.autograd.grad(distillation_loss_from_logits(x, ids, lq, torch.full((len(z),), 0.5, device="cuda"), **how).loss, x,
+                                 torch.tensor(2.0, device="cuda"))  # formed anew
+    assert ((again.double().cpu() - grad).abs() <= grad_bound).all(), how
+
+
+@pytest.mark.parametrize("gap", [60.0, 80.0, 95.0, 110.0, 400.0, 720.0, 800.0, 1e5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("many,v", [(1, 5000), (120, 5001), (1, 70000)])
+def test_next_to_nothing_left(gap, dtype, many, v):
+    """The student has e^-gap left, the teacher a fifth: every token that is not given gets its part of it, -inf gets nothing."""
+    n = 4 * many
+    z = torch.randn(n, v, generator=gen(v), device="cuda") - gap
+    z[::4, 10:] = -math.inf  # a grammar's row: five are left beside the given ones
+    z[1::4, torch.rand(v, generator=gen(1), device="cuda") < 0.5] = -math.inf
+    ids = torch.tensor([[0, 1, v // 2, v - 1, 4]], device="cuda").repeat(n, 1)
+    z.scatter_(1, ids, torch.randn(n, 5, generator=gen(2), device="cuda"))
+    z = z.to(dtype)
+    lq = torch.log_softmax(torch.randn(n, 5, generator=gen(3), device="cuda"), 1) + math.log(0.8)
+    for divergence in ("forward", "reverse", "jsd"):
+        agrees(z, ids, lq, reference(z, ids, lq, divergence, "rest"), dtype, divergence=divergence)
+    temperature = 0.4
+    ref = reference(z, ids, lq, "forward", "rest", temperature)
+    agrees(z, ids, lq, ref, dtype, temperature=temperature)
+
+
+@pytest.mark.parametrize("lowest", [True, False])
+def test_what_is_left_at_the_types_lowest(lowest):
+    """Tokens that a mask has set to the type's lowest value, or all but one of them to -inf: gradients stay numbers."""
+    n, v = 6, 3000
+    for dtype in (torch.float32, torch.bfloat16):
+        z = torch.full((n, v), torch.finfo(dtype).min if lowest else -math.inf, device="cuda", dtype=dtype)
+        if not lowest:
+            z[:, 77] = -200.0
+        z[:, :4] = torch.randn(n, 4, generator=gen(1), device="cuda").to(dtype)
+        ids = torch.arange(4, device="cuda").repeat(n, 1)
+        lq = torch.full((n, 4), math.log(0.2), device="cuda")
+        for divergence in ("forward", "reverse", "jsd"):
+            agrees(z, ids, lq, reference(z, ids, lq, divergence, "rest"), dtype, divergence=divergence)
