@@ -353,19 +353,20 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
     for (int i = tid; i < kGroupIds / 4; i += kThreads) reinterpret_cast<uint4*>(s_adj)[i] = none;
     __syncthreads();
     const int from = lane_value(start, 0);
-    const int upto = c.every_position ? first : lane_value((int)end, 0);  // offsets are 32-bit integers
+    const int upto = c.every_position ? first : max(lane_value((int)end, 0), 0);  // offsets are 32-bit integers
     if (c.token_ids != nullptr) {
       const auto count = [&](auto id_of, auto own_of) {
         constexpr int kBatch = 8;  // loads in flight per thread
-        for (int left = upto - from - tid; left > 0; left -= kThreads * kBatch) {  // counted down: a position plus a step may pass 32 bits
+        // a position plus a step may pass 32 bits: no step is added behind the last batch, and within it none beyond the last token
+        for (int i0 = from + tid, last = upto - 1 - i0; last >= 0; last -= kThreads * kBatch) {
           int off[kBatch];
           bool own[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int ahead = left - b * kThreads, at = upto - max(ahead, 1);
+            const int at = i0 + min(b * kThreads, last);
             const int64_t id = id_of(at);
             own[b] = own_of(at);
-            off[b] = ahead > 0 && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
+            off[b] = b * kThreads <= last && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
           }
 #pragma unroll
           for (int b = 0; b < kBatch; ++b)
@@ -374,6 +375,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
               atomicOr(w, 0x80000000u);
               if (own[b]) atomicAdd(w, 1u);
             }
+          i0 += min(kThreads * kBatch, last);
         }
       };
       const auto with_ids = [&](auto id_of) {
