@@ -30,8 +30,12 @@ struct Teacher {
   const float* logprobs;  // [n][k]
   const float* weights;   // [n], null: all rows count
   int ids_i64, k, divergence, tail;
-  float beta, inv_t;
+  float beta, inv_t, step;
 };
+// What the teacher has left, 1 - sum q, is known to the rounding of its log-probabilities: a softmax in 32 bits is off by about 2^-21 (1 +
+// |lq|) (up to 5.6 2^-24 (1 + |lq|) in all tokens alike, from 2 to 512 of them), and one that is stored in fewer bits by `step` |lq|: two
+// half steps of its type, since errors of the same sign add up.
+constexpr double kTeacherError = 0x1p-21;
 __device__ __forceinline__ int teacher_id(const Teacher& t, int64_t at, int vocab) {
   const int64_t id = t.ids_i64 ? static_cast<const int64_t*>(t.ids)[at] : (int64_t) static_cast<const int32_t*>(t.ids)[at];
   return id >= 0 && id < vocab ? (int)id : -1;
@@ -118,6 +122,19 @@ __device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) 
   return {(q == 0.0 ? 0.0 : b * q * (lq - lm)) + mine, mine};
 }
 
+// The outcome of what is left.  Where the teacher has no more than its error e of it, the list may well be complete:
+//   forward  what the student has no more of either counts 0: q log(q / p) of a rounding q is infinite where p is 0 (lists of all legal
+//            tokens).  Where it has none at all 8 e are let pass, which is what a softmax written as z - logsumexp(z) leaves with z up to 60.
+//   reverse  the teacher has e: against 0, p log(p / q) is infinite wherever a sure teacher's log-probability is rounded to 0.
+// The third is bounded either way.
+__device__ __forceinline__ Term what_is_left(const Teacher& t, double q, double e, double lp) {
+  if (t.divergence == AXON_DISTILL_FORWARD) {
+    const double p = exp64(lp);
+    if (p <= e && q <= (p == 0.0 ? 8.0 * e : e)) return {0.0, 0.0};
+  }
+  return outcome(t, log64(fmax(q, t.divergence == AXON_DISTILL_REVERSE ? e : 0.0)), lp);
+}
+
 // The given tokens of a row, in LDS.
 constexpr int kAgain = -2;
 struct Given {
@@ -126,6 +143,7 @@ struct Given {
   float a[kMaxIds], b[kMaxIds];  // the teacher's log-probabilities, then G; the logits, then p, then what is written in their place
   float best, best_q;            // the largest of either
   double sum, sum_q;             // REST: of exp((z - best) / T), every token once, and of q; else of exp(lq - best_q)
+  double error_q;                // REST: of 1 - sum q
 };
 // By one wavefront; everything that can be known before the row's statistics.  firsts: whether ids that come again are looked for.
 template <typename T, bool REST>
@@ -154,15 +172,20 @@ __device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_
   }
   best = wave_max(best);
   best_q = wave_max(best_q);
-  double sum = 0.0, sum_q = 0.0;
+  double sum = 0.0, sum_q = 0.0, error_q = 0.0;
   if (REST || t.tail == AXON_DISTILL_RENORMALIZE) {
 #pragma unroll 1
     for (int i = lane; i < t.k; i += kWave) {
       if (s.id[i] < 0) continue;
       if (REST && s.next[i] != kAgain) sum += exp64(((double)s.b[i] - (double)best) * (double)t.inv_t);
-      sum_q += exp64((double)s.a[i] - (REST ? 0.0 : (double)best_q));
+      const double lq = (double)s.a[i], q = exp64(lq - (REST ? 0.0 : (double)best_q));
+      sum_q += q;
+      if (REST && q > 0.0) error_q += q * (kTeacherError + fabs(lq) * (kTeacherError + (double)t.step));
     }
-    if (REST) sum = wave_sum_d(sum);
+    if (REST) {
+      sum = wave_sum_d(sum);
+      error_q = wave_sum_d(error_q);
+    }
     sum_q = wave_sum_d(sum_q);
   }
   if (lane == 0) {
@@ -170,6 +193,7 @@ __device__ __forceinline__ void fetch_given(Given& s, const Teacher& t, int row_
     s.best_q = best_q;
     s.sum = sum;
     s.sum_q = sum_q;
+    s.error_q = error_q;
   }
   wave_sync();
 }
@@ -218,7 +242,7 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
   r.rest = (float)((((double)M_ref - (double)r.lse) * inv_t + ln_ref) * 1.4426950408889634);
   if (REST) {
     const double lp_rest = some ? below + ln_ref - ln_s : log64(s_parts) - ln_s;
-    const Term o = outcome(t, log64(fmax(1.0 - s.sum_q, 0.0)), lp_rest);
+    const Term o = what_is_left(t, 1.0 - s.sum_q, s.error_q, lp_rest);
     loss += o.loss;
     sum_g += o.g;
     r.c_out = some ? (float)(o.g - exp64(lp_rest) * sum_g) : (float)(0.0 * s_all);
@@ -849,8 +873,13 @@ int check_rows(const void* p, int dtype, int64_t ld, int64_t n, int64_t v) {
   return AXON_OK;
 }
 
-int check_teacher(const void* ids, const float* logprobs, int64_t k, int divergence, int tail, float beta, float temperature) {
+// The tail's flags: the type that the teacher's log-probabilities were stored in.
+constexpr int kTailBits = 3, kTailFlags = AXON_DISTILL_FROM_BF16 | AXON_DISTILL_FROM_F16;
+float step_of(int tail) { return tail & AXON_DISTILL_FROM_BF16 ? 0x1p-7f : tail & AXON_DISTILL_FROM_F16 ? 0x1p-10f : 0.f; }
+
+int check_teacher(const void* ids, const float* logprobs, int64_t k, int divergence, int flagged_tail, float beta, float temperature) {
   if (k < 1 || k > kMaxIds) return AXON_ERR_SHAPE;
+  const int tail = flagged_tail & ~kTailFlags;
   if (!ids || !logprobs || divergence < AXON_DISTILL_FORWARD || divergence > AXON_DISTILL_JSD || tail < AXON_DISTILL_DROP ||
       tail > AXON_DISTILL_RENORMALIZE)
     return AXON_ERR_ARG;
@@ -900,7 +929,7 @@ extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64
     return AXON_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
   const int eb = elem_bytes(dtype), parts = stats_parts(n, vocab, eb);
-  const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail, beta, 1.f / temperature};
+  const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail & kTailBits, beta, 1.f / temperature, step_of(tail)};
   const RowOut out{losses, covered, grads, coef, (int)n};
   float4* const ws = static_cast<float4*>(workspace);
   const int64_t cached = bwd_follows ? kCacheBytes / (vocab * eb) : 0;
@@ -917,7 +946,7 @@ extern "C" int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64
   } while (0)
 #define AXON_FWD_OF(T) \
   do {                 \
-    if (tail == AXON_DISTILL_REST) AXON_FWD(T, true); else AXON_FWD(T, false); \
+    if (t.tail == AXON_DISTILL_REST) AXON_FWD(T, true); else AXON_FWD(T, false); \
   } while (0)
   AXON_ROWS(dtype, AXON_FWD_OF);
 #undef AXON_FWD_OF
@@ -939,7 +968,7 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
   // every row of dlogits sits on the same offset from a 16-byte boundary as the row of logits
   const int vec_ok = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0 &&
                      (n <= 1 || ((ld - ld_d) * eb) % 16 == 0);
-  const Teacher t{ids, nullptr, weights, ids_i64, (int)k, 0, 0, 0.f, 1.f / temperature};
+  const Teacher t{ids, nullptr, weights, ids_i64, (int)k, 0, 0, 0.f, 1.f / temperature, 0.f};
   const RowOut saved{nullptr, nullptr, const_cast<float*>(grads), const_cast<float*>(coef), (int)n};
 #define AXON_GRAD(T)                                                                                                              \
   hipLaunchKernelGGL((distill_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kBlock), 0, st, static_cast<const T*>(logits), ld, \
@@ -986,14 +1015,14 @@ extern "C" int axon_distill_loss(const void* logits, int dtype, int64_t ld, int6
     if (rc == AXON_OK) rc = check_teacher(ids, teacher_logprobs, k, divergence, tail, beta, temperature);
     if (rc != AXON_OK) return rc;
     if (!losses || !covered || !grads || !coef) return AXON_ERR_ARG;
-    const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail, beta, 1.f / temperature};
+    const Teacher t{ids, teacher_logprobs, weights, ids_i64, (int)k, divergence, tail & kTailBits, beta, 1.f / temperature, step_of(tail)};
     const RowOut out{losses, covered, grads, coef, (int)n};
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == AXON_LOGITS_F32)
-      rc = tail == AXON_DISTILL_REST ? launch_rows<float, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
+      rc = t.tail == AXON_DISTILL_REST ? launch_rows<float, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
                                      : launch_rows<float, false>(logits, ld, n, vocab, t, out, dlogits, ld_d, st);
     else
-      rc = tail == AXON_DISTILL_REST ? launch_rows<unsigned short, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
+      rc = t.tail == AXON_DISTILL_REST ? launch_rows<unsigned short, true>(logits, ld, n, vocab, t, out, dlogits, ld_d, st)
                                      : launch_rows<unsigned short, false>(logits, ld, n, vocab, t, out, dlogits, ld_d, st);
   } else if (rc == AXON_OK) {
     rc = axon_distill_fwd(logits, dtype, ld, n, vocab, ids, ids_i64, teacher_logprobs, k, weights, divergence, tail, beta, temperature, losses,

@@ -1195,6 +1195,8 @@ std::tuple<OptTensor, Tensor, Tensor> distill(const char* what, const Tensor& lo
     const c10::DeviceGuard device(rows.device());
     ids = teacher_ids.reshape({n, k}).contiguous();
     const Tensor lq = f32(teacher_logprobs);
+    if (teacher_logprobs.scalar_type() == at::kBFloat16) tail |= AXON_DISTILL_FROM_BF16;
+    else if (teacher_logprobs.scalar_type() == at::kHalf) tail |= AXON_DISTILL_FROM_F16;
     if (token_weights) w = f32(*token_weights);
     losses = at::empty(batch, opts(rows));
     covered = at::empty(batch, opts(rows));

@@ -15,6 +15,11 @@ over
     "drop"         the given tokens alone, their probabilities as they are
     "renormalize"  the given tokens alone, the teacher's probabilities divided by their sum (any logits will do then)
 
+What the teacher has left is known to the rounding of its log-probabilities only, ``e = sum q (2^-21 (1 + |log q|) + s |log q|)`` (``s``
+for those stored in fewer bits: 2^-7 for bf16, 2^-10 for fp16): a list of all tokens that there are, or of a teacher that is sure.
+So ``"rest"`` counts 0 in ``"forward"`` where neither teacher nor student has more than ``e`` left (the teacher ``8 e`` where the
+student has none), and the teacher has at least ``e`` left in ``"reverse"``: neither loss is infinite for a rounding.
+
 A row is read once for its softmax statistics; the outcomes and their gradients are formed in 64 bits.  What the student has left
 is a sum over the tokens that are not given, so that it is right where almost nothing is.
 """

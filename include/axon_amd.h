@@ -798,6 +798,11 @@ int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t
  *   _loss: loss[0] = sum weights * losses, and dlogits (NULL: not wanted) of that loss beside it. */
 enum { AXON_DISTILL_FORWARD = 0, AXON_DISTILL_REVERSE = 1, AXON_DISTILL_JSD = 2 };
 enum { AXON_DISTILL_DROP = 0, AXON_DISTILL_REST = 1, AXON_DISTILL_RENORMALIZE = 2 };
+/* Added to the tail: the type that the teacher's log-probabilities were stored in before they became fp32, which says how well
+ * 1 - sum q is known: e = sum q (2^-21 (1 + |log q|) + s |log q|), s = 2^-7, 2^-10 or 0.  What is left counts 0 in the forward
+ * divergence where neither has more than e of it (the teacher 8 e where the student has none), and as at least e of the teacher
+ * in the reverse one. */
+enum { AXON_DISTILL_FROM_BF16 = 4, AXON_DISTILL_FROM_F16 = 8 };
 int64_t axon_distill_workspace_bytes(int dtype, int64_t n, int64_t vocab);
 int axon_distill_fwd(const void* logits, int dtype, int64_t ld, int64_t n, int64_t vocab, const void* ids, int ids_are_i64,
                      const float* teacher_logprobs, int64_t k, const float* weights, int divergence, int tail, float beta,

@@ -109,3 +109,66 @@ def test_what_is_left_at_the_types_lowest(lowest):
         lq = torch.full((n, 4), math.log(0.2), device="cuda")
         for divergence in ("forward", "reverse", "jsd"):
             agrees(z, ids, lq, reference(z, ids, lq, divergence, "rest"), dtype, divergence=divergence)
+
+
+def error_of(lq, step=0.0):
+    """How well 1 - sum q is known."""
+    lq = lq.double().cpu()
+    return torch.where(lq > -math.inf, lq.exp() * (2.0 ** -21 * (1 + lq.abs()) + step * lq.abs()), 0.0).sum(1)
+
+
+def stored(z, how):
+    """(log-probabilities of all of z's tokens, how far two half steps of their type are apart) as programs compute and store them."""
+    lq = z - torch.logsumexp(z, 1, keepdim=True) if how == "difference" else torch.log_softmax(z, 1)
+    return {"bf16": (lq.bfloat16(), 2.0 ** -7), "fp16": (lq.half(), 2.0 ** -10), "fp64": (lq.double(), 0.0)}.get(how, (lq, 0.0))
+
+
+@pytest.mark.parametrize("how", ["fp32", "difference", "bf16", "fp16", "fp64"])
+@pytest.mark.parametrize("v,legal,scale", [(10, 10, 1.0), (3000, 10, 3.0), (3000, 2, 8.0), (40001, 300, 3.0)])
+@pytest.mark.parametrize("out", [-math.inf, "lowest"])
+def test_lists_of_all_tokens_that_there_are(how, v, legal, scale, out):
+    """A grammar leaves ``legal`` tokens, the teacher gives all of them, with fillers and impossible ones beside them: what 1 - sum q has
+    by rounding is no outcome."""
+    n, extra = 300, 3
+    allowed = torch.rand(n, v, generator=gen(1), device="cuda").topk(legal, 1).indices
+    student = torch.randn(n, legal, generator=gen(2), device="cuda") * scale
+    z = torch.full((n, v), torch.finfo(torch.float32).min if out == "lowest" else out, device="cuda").scatter_(1, allowed, student)
+    lq, step = stored(torch.randn(n, legal, generator=gen(3), device="cuda") * scale + 15.0, how)
+    ids = torch.cat([allowed, torch.tensor([[-1, v + 5, -1]], device="cuda").expand(n, extra)], 1)
+    lq = torch.cat([lq, torch.tensor([[-2.0, -math.inf, 0.0]], device="cuda", dtype=lq.dtype).expand(n, extra)], 1)
+    left = 1.0 - lq[:, :legal].double().exp().sum(1).cpu()
+    assert (left > 0).any() and (left <= 8 * error_of(lq[:, :legal], step)).all()
+    ref = reference(z, ids, lq, "forward", "rest", q_rest=torch.zeros(n, dtype=torch.float64))
+    assert torch.isfinite(ref[0]).all() and torch.isfinite(ref[1]).all()
+    agrees(z, ids, lq, ref, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sure", [17.0, 18.1, 25.0, 60.0])
+def test_teachers_that_are_sure(dtype, sure):
+    """log p of a sure teacher is rounded to 0, or its list adds up to more than 1: it has at least the rounding left."""
+    n, v = 60, 2500
+    teacher = torch.randn(n, v, generator=gen(1), device="cuda") * 0.1
+    teacher[:, 3] += sure + math.log(v)
+    lq = torch.log_softmax(teacher, 1)[:, 3:6]
+    ids = torch.arange(3, 6, device="cuda").repeat(n, 1)
+    left = 1.0 - lq.double().exp().sum(1).cpu()
+    e = error_of(lq)
+    assert sure < 25 or (left <= 0).any()
+    z = (torch.randn(n, v, generator=gen(2), device="cuda") * 2).to(dtype)
+    agrees(z, ids, lq, reference(z, ids, lq, "reverse", "rest", q_rest=torch.maximum(left, e)), dtype, divergence="reverse")
+    agrees(z, ids, lq, reference(z, ids, lq, "jsd", "rest"), dtype, divergence="jsd")
+    agrees(z, ids, lq, reference(z, ids, lq, "forward", "rest"), dtype)
+
+
+def test_what_a_teacher_has_left_in_earnest():
+    """More than a rounding, where the student has none: the forward divergence is infinite, as it is for a given token."""
+    n, v = 4, 900
+    z = torch.full((n, v), -math.inf, device="cuda")
+    z[:, :5] = torch.randn(n, 5, generator=gen(1), device="cuda")
+    ids = torch.arange(5, device="cuda").repeat(n, 1)
+    lq = torch.log_softmax(torch.randn(n, 5, generator=gen(2), device="cuda"), 1) - 1e-4
+    losses, _ = distillation_from_logits(z, ids, lq)
+    assert (losses == math.inf).all()
+    reverse, _ = distillation_from_logits(z, ids, lq, divergence="reverse")
+    assert torch.isfinite(reverse).all()
