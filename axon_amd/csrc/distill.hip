@@ -212,7 +212,8 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
   const double below = ((double)M_parts - (double)M) * inv_t, s_in_all = s_parts > 0.0 ? s_parts * exp64(below) : s_parts;
   const double s_all = REST && best > -INFINITY ? s_in_all + s.sum * exp64(((double)best - (double)M) * inv_t) : s_in_all;
   const double ln_s = s_all > 0.0 ? log64(s_all) : (double)NAN;  // a row of -inf alone has no softmax
-  const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE ? (double)s.best_q + log64(s.sum_q) : 0.0;
+  // given tokens that the teacher rules out all together have no sum to be divided by: they stay at 0
+  const double norm_q = !REST && t.tail == AXON_DISTILL_RENORMALIZE && s.best_q > -INFINITY ? (double)s.best_q + log64(s.sum_q) : 0.0;
   double loss = 0.0, sum_g = 0.0, covered = 0.0;
 #pragma unroll 1
   for (int i = lane; i < t.k; i += kWave) {

@@ -13,7 +13,8 @@ over
 
     "rest"         the given tokens and, as one more outcome, all others: 1 - sum q, and the student's probability of them
     "drop"         the given tokens alone, their probabilities as they are
-    "renormalize"  the given tokens alone, the teacher's probabilities divided by their sum (any logits will do then)
+    "renormalize"  the given tokens alone, the teacher's probabilities divided by their sum (any logits will do then; where it
+                   gives all of them none, they stay at 0)
 
 What the teacher has left is known to the rounding of its log-probabilities only, ``e = sum q (2^-21 (1 + |log q|) + s |log q|)`` (``s``
 for those stored in fewer bits: 2^-7 for bf16, 2^-10 for fp16): a list of all tokens that there are, or of a teacher that is sure.

@@ -172,3 +172,23 @@ def test_what_a_teacher_has_left_in_earnest():
     assert (losses == math.inf).all()
     reverse, _ = distillation_from_logits(z, ids, lq, divergence="reverse")
     assert torch.isfinite(reverse).all()
+
+
+@pytest.mark.parametrize("v", [700, 70000])
+@pytest.mark.parametrize("tail", ["renormalize", "drop"])
+def test_a_teacher_that_rules_out_all_that_is_given(tail, v):
+    """q = 0 for each of them: nothing of a forward divergence, p log(p / m) of the third, and against 0 an infinite reverse one."""
+    n, k = 8, 5
+    z = torch.randn(n, v, generator=gen(v), device="cuda")
+    ids = torch.randperm(v, generator=gen(1), device="cuda")[:k].repeat(n, 1)
+    lq = torch.log_softmax(torch.randn(n, k, generator=gen(2), device="cuda"), 1)
+    lq[::2] = -math.inf
+    ids[4, 1:] = -1
+    sums = torch.logsumexp(lq.double(), 1, keepdim=True) if tail == "renormalize" else torch.zeros(n, 1, device="cuda")
+    ref_lq = torch.where(lq > -math.inf, lq.double() - sums, -math.inf)
+    for divergence in ("forward", "jsd"):
+        ref = reference(z, ids, ref_lq, divergence, "drop")
+        assert torch.isfinite(ref[0]).all() and (divergence == "jsd" or (ref[0][::2] == 0).all() and (ref[1][::2] == 0).all())
+        agrees(z, ids, lq, ref, torch.float32, divergence=divergence, tail=tail)
+    losses, _ = distillation_from_logits(z, ids, lq, divergence="reverse", tail=tail)
+    assert (losses[::2] == math.inf).all() and torch.isfinite(losses[1::2]).all()
