@@ -131,6 +131,17 @@ def _controls_of(logit_controls, micro_batch, temperature, indices=None, cu_seql
     return LogitControls(packed[0], cu_seqlens, response_mask=packed[1], allowed_index=packed[2], **kw)
 
 
+def _labels_under_controls(micro_batch, indices=None):
+    """The token that each row scores, padded or (with ``indices``) packed, and -1 (log-probability 0, no gradient) where the sampler
+    drew none: the controls hold for what it drew, and what they rule out may well stand in a prompt, or begin the next sequence."""
+    ids, there, own = micro_batch["input_ids"], micro_batch["attention_mask"] != 0, micro_batch.get("response_mask", None)
+    drawn = there[:, :-1] & there[:, 1:]
+    if own is not None:
+        drawn = drawn & (own[:, 1:] != 0)
+    labels = F.pad(torch.where(drawn, ids[:, 1:], -1), (0, 1), value=-1)
+    return labels if indices is None else labels.flatten()[indices]
+
+
 def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_entropy: bool = False, *,
                        use_remove_padding: bool = True, use_fused_kernels: bool = True, ulysses_sp_size: int = 1,
                        skip_prompt_rows: bool = False, logit_controls: dict | None = None, **_unused):
@@ -151,8 +162,9 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
     before it drew the tokens, so that they are scored under the distribution that they were drawn from: the penalties, biases
     and masks of ``axon_amd.utils.torch.controls.LogitControls`` by their names there, penalties for all or ``[batch]``,
     ``allowed_index`` ``[batch, seq]`` with the mask that token t was drawn under at position t.  A history is the tokens of
-    ``attention_mask`` before the token; those of ``micro_batch["response_mask"]`` (all, where there is none) count as generated.
-    A token that the controls take out has log-probability ``-inf``."""
+    ``attention_mask`` before the token; those of ``micro_batch["response_mask"]`` (all, where there is none) count as generated,
+    and only they are scored: the log-probabilities of other positions come back as 0, with no gradient.  A generated token that the
+    controls take out has log-probability ``-inf``."""
     head_kwargs = {}
     if logit_controls is not None and use_fused_kernels:
         raise ValueError("logit_controls need the logits: use_fused_kernels=False")
@@ -194,7 +206,7 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
                 lp_packed, ent_packed = _from_logits(logits, labels.reshape(-1), temperature, calculate_entropy)
             else:
                 controls = _controls_of(logit_controls, micro_batch, temperature, indices, cu_seqlens)
-                lp_packed, ent_packed = controlled_logprobs_from_logits(logits, labels.reshape(-1), controls)
+                lp_packed, ent_packed = controlled_logprobs_from_logits(logits, _labels_under_controls(micro_batch, indices), controls)
         log_probs = rmpad_postprocess(lp_packed, indices=indices, batch_size=batch_size, seqlen=seqlen)
         entropy = None
         if calculate_entropy:
@@ -210,9 +222,9 @@ def fsdp_model_forward(module, micro_batch: dict, temperature: float, calculate_
         return entropy, log_probs
     # padded, non-fused (forward_utils.py:294-304): logits[:, t] predicts token t + 1
     output = module(input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids, use_cache=False)
-    if logit_controls is not None:  # all rows; the last one's label is outside the vocabulary, what it has is dropped
+    if logit_controls is not None:  # all rows; what the last one has is dropped
         controls = _controls_of(logit_controls, micro_batch, temperature)
-        lp, ent = controlled_logprobs_from_logits(output.logits, F.pad(input_ids[:, 1:], (0, 1), value=-1), controls)
+        lp, ent = controlled_logprobs_from_logits(output.logits, _labels_under_controls(micro_batch), controls)
         return (shift_to_token_positions(ent) if calculate_entropy else None), shift_to_token_positions(lp)
     lp, ent = _from_logits(output.logits[:, :-1, :], input_ids[:, 1:], temperature, calculate_entropy)
     log_probs = F.pad(lp, (1, 0), value=0.0)

@@ -61,3 +61,83 @@ def test_a_history_that_ends_where_32_bits_do():
     count = torch.bincount(ids, minlength=v).float()[None]
     want = torch.where(count > 0, torch.where(z > 0, z / 2, z * 2), z) - 0.5 * count - 0.25 * (count > 0)
     assert (controlled_logits(z, ctl) - want).abs().max() <= 8 * 2.0 ** -24 * 5
+
+
+@pytest.mark.parametrize("remove_padding", [True, False])
+@pytest.mark.parametrize("left", [False, True])
+@pytest.mark.parametrize("loss_fn,extra", [("ppo", {}), ("ppo", dict(kl_coef=0.1, kl_type="k1")), ("ppo", dict(kl_coef=0.1, kl_type="k2")),
+                                           ("ppo", dict(kl_coef=0.1, kl_type="abs+", entropy_coef=0.01)), ("reinforce", {})])
+def test_a_step_whose_prompts_hold_what_the_controls_rule_out(remove_padding, left, loss_fn, extra):
+    """A prompt, the padding and the first token of a sequence are no draws of the sampler: the step's loss, its metrics and its gradient are
+    numbers, and those of the same step with its log-probabilities kept at the response's positions only."""
+    from types import SimpleNamespace
+
+    from axon_amd.models.fsdp_models import CausalLM
+    from axon_amd.protocol import DataProto
+    from axon_amd.utils.fsdp.forward_utils import fsdp_model_forward
+
+    g = gen(7)
+    b, t, h, v, prompt = 3, 12, 32, 500, 4
+    lens = [12, 8, 5]
+    emb, w = torch.randn(v, h, generator=g, device="cuda"), torch.randn(v, h, generator=g, device="cuda")
+    place = lambda x, i: [0] * (t - lens[i]) + x if left else x + [0] * (t - lens[i])
+    row = lambda i: [9] + [3, 9, 40] + (torch.randint(10, 400, (lens[i] - prompt,), generator=g, device="cuda")).tolist()  # 9: ruled out
+    batch = {"input_ids": torch.tensor([place(row(i), i) for i in range(b)], device="cuda"),
+             "attention_mask": torch.tensor([place([1] * lens[i], i) for i in range(b)], device="cuda"),
+             "response_mask": torch.tensor([place([0] * prompt + [1] * (lens[i] - prompt), i) for i in range(b)], device="cuda"),
+             "position_ids": torch.zeros(b, t, dtype=torch.int64, device="cuda")}
+    keep = torch.ones(1, v, dtype=torch.bool, device="cuda")
+    keep[:, 3] = False
+    controls = dict(repetition_penalty=1.2, bias_ids=torch.tensor([9], device="cuda"), bias=torch.tensor([-math.inf], device="cuda"),
+                    allowed=R.pack(keep))
+    own = batch["response_mask"] != 0
+    bent = torch.ones(v, device="cuda", requires_grad=True)
+
+    class Model(torch.nn.Module):
+        def forward(self, input_ids=None, attention_mask=None, position_ids=None, use_cache=False):
+            return SimpleNamespace(logits=emb[input_ids] @ w.t() / h ** 0.5 * bent)
+
+    def forward(kept):
+        ent, lp = fsdp_model_forward(Model(), batch, 0.9, True, use_remove_padding=remove_padding, use_fused_kernels=False,
+                                     logit_controls=controls)
+        return (ent, lp) if not kept else (ent, torch.where(own, lp, 0.0))
+
+    noise = 0.1 * torch.randn(b, t, generator=g, device="cuda")
+    advantages = torch.randn(b, t, generator=g, device="cuda")
+
+    def step(kept):
+        with torch.no_grad():
+            _, old = forward(kept)
+        mask = batch["response_mask"].float()
+        data = DataProto.from_dict(tensors={"old_log_probs": old + noise * mask, "ref_log_prob": old - noise * mask, "advantages": advantages,
+                                            "response_mask": mask})
+        meta = {"loss_fn": loss_fn, "loss_fn_args": dict(extra), "dp_replicas": 1, "n_micro_batches": 1, "temperature": 0.9}
+        module = lambda inputs, m: dict(zip(("entropys", "log_probs"), forward(kept)))  # noqa: E731
+        loss, metrics = CausalLM.forward_backward_fn(module, data, meta)
+        return old, loss, metrics, *torch.autograd.grad(loss, bent)
+
+    old, loss, metrics, grad = step(False)
+    assert torch.isfinite(old).all() and (old[~own] == 0).all() and (old[own] < 0).all()
+    assert torch.isfinite(loss) and torch.isfinite(grad).all() and (grad != 0).any()
+    assert all(math.isfinite(float(x)) for x in metrics.values())
+    _, want, want_metrics, want_grad = step(True)
+    assert torch.equal(loss, want) and metrics == want_metrics and torch.equal(grad, want_grad)
+
+
+@pytest.mark.parametrize("remove_padding", [True, False])
+def test_a_step_without_a_response_mask_scores_what_is_there(remove_padding):
+    from types import SimpleNamespace
+
+    from axon_amd.utils.fsdp.forward_utils import fsdp_model_forward
+
+    ids = torch.tensor([[0, 5, 6, 7], [8, 9, 0, 0]], device="cuda")
+    there = torch.tensor([[0, 1, 1, 1], [1, 1, 0, 0]], device="cuda")
+    logits = torch.randn(2, 4, 50, generator=gen(3), device="cuda")
+    model = lambda **kw: SimpleNamespace(logits=logits if not remove_padding else logits[there != 0][None])  # noqa: E731
+    _, lp = fsdp_model_forward(model, {"input_ids": ids, "attention_mask": there, "position_ids": ids}, 1.0, use_fused_kernels=False,
+                               use_remove_padding=remove_padding, logit_controls=dict(presence_penalty=0.0))
+    want = torch.zeros(2, 4, dtype=torch.float64, device="cuda")
+    log_p = torch.log_softmax(logits.double(), 2)
+    for i, p in ((0, 2), (0, 3), (1, 1)):
+        want[i, p] = log_p[i, p - 1, ids[i, p]]
+    assert (lp - want).abs().max() <= LP_TOL
