@@ -506,7 +506,8 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
         float m = ref > kBanned ? ref : largest();
         const float cc = m * k;
         float s4[4] = {}, e4[4] = {}, s = 0.f, e = 0.f;
-        bool plain = fabsf(cc) < kFar && m > kBanned, above = false;
+        // what is banned has to be out of reach of the reference (at a temperature of 1e28 it is not)
+        bool plain = fabsf(cc) < kFar && (m - kBanned) * k > 2 * -kTiny, above = false;
         if (plain) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {

@@ -141,3 +141,31 @@ def test_a_step_without_a_response_mask_scores_what_is_there(remove_padding):
     for i, p in ((0, 2), (0, 3), (1, 1)):
         want[i, p] = log_p[i, p - 1, ids[i, p]]
     assert (lp - want).abs().max() <= LP_TOL
+
+
+@pytest.mark.parametrize("temperature", [1e20, 1e27, 1e29, 1e31, 3e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("per_seq", [False, True])
+def test_what_is_out_is_out_at_any_temperature(temperature, dtype, per_seq):
+    """Whole rows, rows of few ids, and a vocabulary that ends inside a wavefront's ids."""
+    n, v = 70, 3001
+    g = gen(5)
+    z = (torch.randn(n, v, generator=g, device="cuda") * 3).to(dtype)
+    keep = torch.rand(n, v, generator=g, device="cuda") < 0.5
+    keep[::3] = torch.rand(n, v, generator=g, device="cuda")[::3] < 0.002
+    keep[1::7] = True
+    keep[:, 11] = True
+    labels = torch.full((n,), 11, dtype=torch.int64, device="cuda")
+    value = torch.full((1,), temperature, device="cuda") if per_seq else temperature
+    ctl = LogitControls(cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device="cuda"), allowed=R.pack(keep), temperature=value)
+    out, slope, _ = R.controlled(z, R.spans_of([n], "all"), None, keep=list(keep), temperature=temperature)
+    ones = torch.ones(n, device="cuda")
+    lp_want, ent_want, grad, size = R.scored(out, slope, labels, ones, ones)
+    z.requires_grad_(True)
+    lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
+    assert ((lp.double().cpu() - lp_want).abs() <= LP_TOL).all() and ((ent.double().cpu() - ent_want).abs() <= ENT_TOL).all()
+    d, = torch.autograd.grad([lp, ent], z, [ones, ones])
+    # 1 / T and a gradient with it may be numbers that 32 bits hold in steps of 2^-149 (bf16: 2^-133)
+    step = 2.0 ** (-133 if dtype == torch.bfloat16 else -149)
+    bound = 2 * ENT_TOL * size + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + step * (2 + 3 * temperature * size)
+    assert ((d.double().cpu() - grad).abs() <= bound).all() and (d[~keep] == 0).all()
