@@ -732,7 +732,7 @@ int check_controls(const axon_controls* c, int64_t n, int64_t v) {
     if (c->allowed_rows < 1 || c->allowed_stride < (v + 31) / 32) return AXON_ERR_SHAPE;
     if (!c->allowed_index && c->allowed_rows != 1 && c->allowed_rows != n) return AXON_ERR_SHAPE;
   }
-  const auto positive = [](float x) { return x > 0.f && x <= 3.402823466e38f; };
+  const auto positive = [](float x) { return x >= 0x1p-126f && x <= 3.402823466e38f; };  // smaller ones have no reciprocal
   const auto finite = [](float x) { return x - x == 0.f; };
   if (!c->repetition && !positive(c->repetition_all)) return AXON_ERR_ARG;
   if (!c->temperature && !positive(c->temperature_all)) return AXON_ERR_ARG;

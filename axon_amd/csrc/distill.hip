@@ -878,13 +878,15 @@ int check_rows(const void* p, int dtype, int64_t ld, int64_t n, int64_t v) {
 constexpr int kTailBits = 3, kTailFlags = AXON_DISTILL_FROM_BF16 | AXON_DISTILL_FROM_F16;
 float step_of(int tail) { return tail & AXON_DISTILL_FROM_BF16 ? 0x1p-7f : tail & AXON_DISTILL_FROM_F16 ? 0x1p-10f : 0.f; }
 
+bool usable(float temperature) { return temperature >= 0x1p-126f && temperature <= 3.402823466e38f; }  // smaller ones have no reciprocal
+
 int check_teacher(const void* ids, const float* logprobs, int64_t k, int divergence, int flagged_tail, float beta, float temperature) {
   if (k < 1 || k > kMaxIds) return AXON_ERR_SHAPE;
   const int tail = flagged_tail & ~kTailFlags;
   if (!ids || !logprobs || divergence < AXON_DISTILL_FORWARD || divergence > AXON_DISTILL_JSD || tail < AXON_DISTILL_DROP ||
       tail > AXON_DISTILL_RENORMALIZE)
     return AXON_ERR_ARG;
-  if (!(temperature > 0.f) || !(temperature <= 3.402823466e38f)) return AXON_ERR_ARG;
+  if (!usable(temperature)) return AXON_ERR_ARG;
   if (divergence == AXON_DISTILL_JSD && !(beta > 0.f && beta < 1.f)) return AXON_ERR_ARG;
   return AXON_OK;
 }
@@ -963,7 +965,7 @@ extern "C" int axon_distill_bwd(const void* logits, int dtype, int64_t ld, int64
   if (rc == AXON_OK) rc = check_rows(dlogits, dtype, ld_d, n, vocab);
   if (rc != AXON_OK || n == 0) return rc;
   if (k < 1 || k > kMaxIds) return AXON_ERR_SHAPE;
-  if (!ids || !grads || !coef || !(temperature > 0.f) || (!upstream && !weights) || (ready && (!weights || !upstream))) return AXON_ERR_ARG;
+  if (!ids || !grads || !coef || !usable(temperature) || (!upstream && !weights) || (ready && (!weights || !upstream))) return AXON_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   const int eb = elem_bytes(dtype), parts = grad_parts(n, vocab, eb);
   // every row of dlogits sits on the same offset from a 16-byte boundary as the row of logits

@@ -822,9 +822,9 @@ class Controls {
     c_.frequency = value(kFrequency, frequency, "frequency_penalty");
     c_.presence = value(kPresence, presence, "presence_penalty");
     c_.temperature = value(kTemperature, temperature, "temperature");
-    const auto usable = [](float x, bool positive) { return std::isfinite(x) && (!positive || x > 0.f); };
-    if (!usable(c_.repetition_all, true)) refuse(kWhat, "repetition_penalty must be positive");
-    if (!usable(c_.temperature_all, true)) refuse(kWhat, "temperature must be positive");
+    const auto usable = [](float x, bool positive) { return std::isfinite(x) && (!positive || x >= 0x1p-126f); };
+    if (!usable(c_.repetition_all, true)) refuse(kWhat, "repetition_penalty must be positive (2^-126 or more)");
+    if (!usable(c_.temperature_all, true)) refuse(kWhat, "temperature must be positive (2^-126 or more)");
     if (!usable(c_.frequency_all, false) || !usable(c_.presence_all, false)) refuse(kWhat, "frequency_penalty and presence_penalty must be finite");
     if (!token_ids && (c_.repetition || c_.frequency || c_.presence || c_.repetition_all != 1.f || c_.frequency_all != 0.f || c_.presence_all != 0.f))
       refuse(kWhat, "penalties need token_ids");

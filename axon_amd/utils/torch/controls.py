@@ -47,7 +47,7 @@ class LogitControls:
     * ``response_mask`` (same arrangement as the tokens): which of them the model has generated, for ``frequency_penalty``
       and ``presence_penalty``; None: all.  ``repetition_penalty`` counts the prompt too.
     * penalties and ``temperature``: a number, or a float tensor with one for each sequence (whose values are not looked at:
-      a repetition penalty and a temperature have to be positive).
+      a repetition penalty and a temperature have to be positive, 2^-126 or more).
     * ``bias_ids`` and ``bias``: ``[k]`` for all rows, or ``[sequences, k]``; an id outside the vocabulary is a filler, one
       that comes twice gets both; ``-inf`` takes an id out.
     * ``allowed``: int32 bit masks ``[words]`` (for all rows) or ``[masks, words]``, bit i of word w for token ``32 w + i``, 1

@@ -56,8 +56,8 @@ def _how(what, divergence, tail, beta, temperature):
     beta, temperature = float(beta), float(temperature)
     if divergence == "jsd" and not 0.0 < beta < 1.0:
         raise ValueError(f"{what}: beta must be between 0 and 1, got {beta}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{what}: temperature must be positive, got {temperature}")
+    if not 2.0 ** -126 <= temperature <= torch.finfo(torch.float32).max:  # as a number of 32 bits that has a reciprocal
+        raise ValueError(f"{what}: temperature must be positive (2^-126 or more, finite in 32 bits), got {temperature}")
     return _DIVERGENCES[divergence], _TAILS[tail], beta, temperature
 
 

@@ -743,7 +743,7 @@ int axon_router_balance_bwd(const void* const* logits, int dtype, int64_t ld, in
  *   out = y / T
  * Sequences are rows of tokens (cu_seqlens, or uniform_len > 0 and NULL).  every_position 1: row r of the logits is position
  * r of the tokens and its history the tokens of its sequence up to and with r; 0: row r belongs to sequence r, whose tokens
- * are all its history.  Own tokens: those with own_mask != 0 (NULL: all).  An id outside [0, vocab) counts for nothing.
+ * are all its history.  rep and T: 2^-126 or more.  Own tokens: those with own_mask != 0 (NULL: all).  An id outside [0, vocab) counts for nothing.
  * Passed by the host; its pointers are device memory. */
 typedef struct axon_controls {
   const void* token_ids; /* [n_tokens] int32 or int64; NULL: no history */
@@ -781,7 +781,7 @@ int axon_controls_logprob_bwd(const void* logits, int dtype, int64_t ld, int64_t
 
 /* Distillation from a teacher's top logits (no reference counterpart).  Per position, with q the teacher's probabilities of k given
  * tokens (ids [n][k] int32 or int64, an id outside [0, vocab) is a filler; log-probabilities [n][k]) and p the student's,
- * softmax(logits / temperature) over the whole vocabulary:
+ * softmax(logits / temperature) over the whole vocabulary, temperature 2^-126 or more:
  *   AXON_DISTILL_FORWARD  sum q log(q / p),  AXON_DISTILL_REVERSE  sum p log(p / q),
  *   AXON_DISTILL_JSD      beta sum q log(q / m) + (1 - beta) sum p log(p / m),  m = beta q + (1 - beta) p,  0 < beta < 1
  * over the given tokens (AXON_DISTILL_DROP), over these with q divided by its sum (AXON_DISTILL_RENORMALIZE), or with what is
