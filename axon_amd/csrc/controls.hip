@@ -422,7 +422,8 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
   float refs[2] = {kNoLogit, kNoLogit};  // of whole rows, and of rows of few ids
   bool above_before = false;
   for (int r = 0; r < rows; ++r) {
-    if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1))) {  // another sequence
+    // another sequence (a row in front of the first one starts where that does)
+    if (ADJ && (r == 0 || lane_value(start, r) != lane_value(start, r - 1) || lane_value(seq, r) != lane_value(seq, r - 1))) {
       if (r > 0) {
 #pragma unroll
         for (int i = 0; i < kLaneIds; ++i) adj[i * kWave + lane] = 0;

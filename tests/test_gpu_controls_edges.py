@@ -169,3 +169,28 @@ def test_what_is_out_is_out_at_any_temperature(temperature, dtype, per_seq):
     step = 2.0 ** (-133 if dtype == torch.bfloat16 else -149)
     bound = 2 * ENT_TOL * size + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + step * (2 + 3 * temperature * size)
     assert ((d.double().cpu() - grad).abs() <= bound).all() and (d[~keep] == 0).all()
+
+
+@pytest.mark.parametrize("cu", [[3, 3, 9], [2, 2, 2, 7, 9], [3, 9], [1, 1, 6]])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("many", [9, 40000])  # rows: where there are many, a wavefront walks several of them
+def test_rows_in_front_of_the_first_sequence(cu, dtype, many):
+    """They have no history; the sequences behind them have their own, and their own biases."""
+    n, v, seqs = many, 2500 if many < 100 else 90, len(cu) - 1
+    g = gen(len(cu))
+    z = (torch.randn(n, v, generator=g, device="cuda") * 2).to(dtype)
+    tokens = torch.randint(0, 40, (n,), generator=g, device="cuda")
+    bias_ids = torch.randint(0, 60, (seqs, 20), generator=g, device="cuda")
+    bias = torch.randn(seqs, 20, generator=g, device="cuda")
+    freq = torch.rand(seqs, generator=g, device="cuda")
+    kw = dict(repetition_penalty=1.5, frequency_penalty=freq, bias_ids=bias_ids, bias=bias)
+    ctl = LogitControls(tokens, torch.tensor(cu, dtype=torch.int32, device="cuda"), **kw)
+    spans = [(i, a, p + 1) for i, (a, b) in enumerate(zip(cu[:-1], cu[1:])) for p in range(a, b)]
+    rows = slice(cu[0], cu[-1])
+    out, slope, size = R.controlled(z[rows], spans, tokens, repetition=1.5, frequency=freq.cpu(), bias_ids=bias_ids.cpu(), bias=bias.cpu())
+    got = controlled_logits(z, ctl)[rows].double().cpu()
+    assert ((got - out).abs() <= 7 * 2.0 ** -24 * size + (2.0 ** -8 * out.abs() if dtype == torch.bfloat16 else 0.0) + 1e-30).all()
+    labels = tokens.roll(-1)
+    lp_want, ent_want = R.scored(out, slope, labels[rows])
+    lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
+    assert ((lp[rows].double().cpu() - lp_want).abs() <= LP_TOL).all() and ((ent[rows].double().cpu() - ent_want).abs() <= ENT_TOL).all()
