@@ -239,7 +239,9 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
   const double ln_ref = some ? log64(s_parts) : ln_s;
   const float M_ref = some ? M_parts : M;
   RowCoefs r;
-  r.lse = (float)((double)M_ref + ln_ref / inv_t);
+  // a number of 32 bits (at a temperature of 1e38 the sum's logarithm is none): `rest` is what it lacks.  (NaN stays.)
+  const auto within = [](double x, double most) { return x > most ? most : x < -most ? -most : x; };
+  r.lse = (float)within((double)M_ref + within(ln_ref / inv_t, 0x1p126), 3.402823466e38);
   r.rest = (float)((((double)M_ref - (double)r.lse) * inv_t + ln_ref) * 1.4426950408889634);
   if (REST) {
     const double lp_rest = some ? below + ln_ref - ln_s : log64(s_parts) - ln_s;

@@ -192,3 +192,64 @@ def test_a_teacher_that_rules_out_all_that_is_given(tail, v):
         agrees(z, ids, lq, ref, torch.float32, divergence=divergence, tail=tail)
     losses, _ = distillation_from_logits(z, ids, lq, divergence="reverse", tail=tail)
     assert (losses[::2] == math.inf).all() and torch.isfinite(losses[1::2]).all()
+
+
+@pytest.mark.parametrize("temperature", [1e-37, 1e-20, 1e20, 1e30, 1e37, 2e38])
+@pytest.mark.parametrize("v,n", [(900, 3), (70001, 2), (600, 2000)])
+def test_temperatures_at_both_ends_of_the_range(temperature, v, n):
+    """Logits of the temperature's size, and logits that are all alike beside it."""
+    k = 6
+    ids = torch.stack([torch.randperm(v, generator=gen(i), device="cuda")[:k] for i in range(min(n, 5))]).repeat(-(-n // 5), 1)[:n]
+    lq = torch.log_softmax(torch.randn(n, k + 1, generator=gen(1), device="cuda"), 1)[:, :k]
+    w = torch.rand(n, generator=gen(2), device="cuda") + 0.5
+    for scale in (min(temperature, 1e37), 1.0) if temperature > 1 else (temperature,):
+        z = torch.randn(n, v, generator=gen(3), device="cuda") * scale
+        for divergence, tail in (("forward", "rest"), ("jsd", "drop"), ("reverse", "renormalize")):
+            ref_lq = lq.double() - (torch.logsumexp(lq.double(), 1, keepdim=True) if tail == "renormalize" else 0.0)
+            losses, grad, size, gsize = reference(z, ids, ref_lq, divergence, "rest" if tail == "rest" else "drop", temperature)
+            x = z.clone().requires_grad_(True)
+            how = dict(divergence=divergence, tail=tail, temperature=temperature)
+            got, _ = distillation_from_logits(x, ids, lq, **how)
+            r = distillation_loss_from_logits(x, ids, lq, w, **how)
+            for values in (got, r.losses):
+                assert ((values.detach().double().cpu() - losses).abs() <= 2 * P_REL * size + 1e-12).all(), how
+            each, = torch.autograd.grad(got, x, w)
+            once, = torch.autograd.grad(r.loss, x)
+            up = w.double().cpu()[:, None]
+            # a gradient and 1 / T may be numbers that 32 bits hold in steps of 2^-149
+            bound = 4 * P_REL * gsize * up + 2.0 ** -149 * (4 + 4 * temperature * gsize)
+            for d in (each, once):
+                assert ((d.double().cpu() - up * grad).abs() <= bound).all(), (how, scale)
+
+
+def test_rows_that_are_read_and_rows_that_are_not():
+    """Per position: rows without an upstream gradient get exactly 0 whatever they hold; with one, a row of the type's lowest logits and
+    one that gives a given token no probability have the gradient of their definition, though the latter's loss is infinite."""
+    v, n, k = 3000, 7, 5
+    z = torch.randn(n, v, generator=gen(1), device="cuda") * 3
+    ids = torch.stack([torch.randperm(v, generator=gen(i), device="cuda")[:k] for i in range(n)])
+    lq = torch.log_softmax(torch.randn(n, k + 1, generator=gen(2), device="cuda"), 1)[:, :k]
+    z[0, 77] = math.nan
+    z[1] = -math.inf
+    z[2, 5] = math.inf
+    z[3, ids[3, 2]] = -math.inf
+    z[4] = torch.finfo(torch.float32).min
+    for divergence in ("forward", "reverse", "jsd"):
+        for tail in ("rest", "drop", "renormalize"):
+            x = z.clone().requires_grad_(True)
+            out, _ = distillation_from_logits(x, ids, lq, divergence=divergence, tail=tail)
+            for i in (5, 4, 3):
+                up = torch.zeros(n, device="cuda")
+                up[i] = 1.0
+                d, = torch.autograd.grad(out, x, up, retain_graph=True)
+                rest = torch.arange(n) != i
+                assert (d[rest.cuda()] == 0).all(), (divergence, tail, i)
+                ref_lq = lq.double() - (torch.logsumexp(lq.double(), 1, keepdim=True) if tail == "renormalize" else 0.0)
+                _, grad, _, gsize = reference(z[i:i + 1], ids[i:i + 1], ref_lq[i:i + 1], divergence, "rest" if tail == "rest" else "drop")
+                assert ((d[i].double().cpu() - grad[0]).abs() <= 4 * P_REL * gsize[0] + 1e-30).all(), (divergence, tail, i)
+                w = torch.zeros(n, device="cuda")
+                w[i] = 1.0
+                r = distillation_loss_from_logits(x, ids, lq, w, divergence=divergence, tail=tail)
+                once, = torch.autograd.grad(r.loss, x)
+                assert (once[rest.cuda()] == 0).all() and (r.losses[rest.cuda()] == 0).all()
+                assert ((once[i].double().cpu() - grad[0]).abs() <= 4 * P_REL * gsize[0] + 1e-30).all(), (divergence, tail, i)
