@@ -194,3 +194,29 @@ def test_rows_in_front_of_the_first_sequence(cu, dtype, many):
     lp_want, ent_want = R.scored(out, slope, labels[rows])
     lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
     assert ((lp[rows].double().cpu() - lp_want).abs() <= LP_TOL).all() and ((ent[rows].double().cpu() - ent_want).abs() <= ENT_TOL).all()
+
+
+@pytest.mark.parametrize("temperature", [1.2e-38, 1e-30, 1e-3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_temperatures_next_to_nothing(temperature, dtype):
+    """Logits of the temperature's size: penalties beside them are all there is."""
+    n, v = 70, 3001
+    g = gen(6)
+    z = (torch.randn(n, v, generator=g, device="cuda") * 3 * temperature * 16).to(dtype)
+    keep = torch.rand(n, v, generator=g, device="cuda") < 0.5
+    keep[::3] = torch.rand(n, v, generator=g, device="cuda")[::3] < 0.002
+    keep[:, 11] = True
+    labels = torch.full((n,), 11, dtype=torch.int64, device="cuda")
+    ctl = LogitControls(allowed=R.pack(keep), temperature=temperature)
+    out, slope, _ = R.controlled(z, R.spans_of([n], "all"), None, keep=list(keep), temperature=temperature)
+    ones = torch.ones(n, device="cuda")
+    lp_want, ent_want, grad, size = R.scored(out, slope, labels, ones, ones)
+    z.requires_grad_(True)
+    lp, ent = controlled_logprobs_from_logits(z, labels, ctl)
+    # logits over the temperature of up to 220 instead of 80
+    assert ((lp.double().cpu() - lp_want).abs() <= 3 * LP_TOL).all() and ((ent.double().cpu() - ent_want).abs() <= 3 * ENT_TOL).all()
+    d, = torch.autograd.grad([lp, ent], z, [ones, ones])
+    # a probability below 2^-126 is 0, and up to 150 / T times that is missing (1.8e-36 / T); a row's constants are the upstream gradients
+    # times 1 + entropy over T, which at the smallest temperature is beyond 32 bits (8e37 * 5): there the gradient is not compared
+    bound = 6 * ENT_TOL * size + (2.0 ** -8 * grad.abs() if dtype == torch.bfloat16 else 0.0) + 1e-35 / temperature
+    assert temperature < 1e-37 or ((d.double().cpu() - grad).abs() <= bound).all() and (d[~keep] == 0).all()
