@@ -353,20 +353,21 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
     for (int i = tid; i < kGroupIds / 4; i += kThreads) reinterpret_cast<uint4*>(s_adj)[i] = none;
     __syncthreads();
     const int from = lane_value(start, 0);
-    const int upto = c.every_position ? first : max(lane_value((int)end, 0), 0);  // offsets are 32-bit integers
+    const int n_history = (c.every_position ? first : max(lane_value((int)end, 0), 0)) - from;  // offsets are 32-bit integers
     if (c.token_ids != nullptr) {
       const auto count = [&](auto id_of, auto own_of) {
         constexpr int kBatch = 8;  // loads in flight per thread
-        // a position plus a step may pass 32 bits: no step is added behind the last batch, and within it none beyond the last token
-        for (int i0 = from + tid, last = upto - 1 - i0; last >= 0; last -= kThreads * kBatch) {
+        // counted from the first token, and no step is added behind the last batch: positions may reach 2^31
+        for (int i0 = tid; i0 < n_history;) {
           int off[kBatch];
           bool own[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int at = i0 + min(b * kThreads, last);
+            const unsigned i = (unsigned)i0 + b * kThreads;
+            const int at = from + (int)min(i, (unsigned)(n_history - 1));
             const int64_t id = id_of(at);
             own[b] = own_of(at);
-            off[b] = b * kThreads <= last && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
+            off[b] = i < (unsigned)n_history && id >= 0 && id < vocab ? (int)id - group * kGroupIds : -1;
           }
 #pragma unroll
           for (int b = 0; b < kBatch; ++b)
@@ -375,7 +376,8 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void controls_kernel(const T* log
               atomicOr(w, 0x80000000u);
               if (own[b]) atomicAdd(w, 1u);
             }
-          i0 += min(kThreads * kBatch, last);
+          if (n_history - i0 <= kThreads * kBatch) break;
+          i0 += kThreads * kBatch;
         }
       };
       const auto with_ids = [&](auto id_of) {
