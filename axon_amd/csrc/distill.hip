@@ -107,10 +107,9 @@ __device__ __forceinline__ void wave_sync() {
 __device__ __attribute__((noinline)) double exp64(double x) { return exp(x); }
 __device__ __attribute__((noinline)) double log64(double x) { return log(x); }
 
-// One outcome: its share of the loss and G.
+// One outcome of which the teacher has q = exp(lq) and the student p = exp(lp): its share of the loss and G.
 struct Term { double loss, g; };
-__device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) {
-  const double q = exp64(lq), p = exp64(lp);
+__device__ __forceinline__ Term outcome(const Teacher& t, double q, double lq, double p, double lp) {
   if (t.divergence == AXON_DISTILL_FORWARD) return {q > 0.0 ? q * (lq - lp) : q - q, -q};
   if (t.divergence == AXON_DISTILL_REVERSE) {
     if (p == 0.0) return {0.0, 0.0};
@@ -127,12 +126,10 @@ __device__ __forceinline__ Term outcome(const Teacher& t, double lq, double lp) 
 //            tokens).  Where it has none at all 8 e are let pass, which is what a softmax written as z - logsumexp(z) leaves with z up to 60.
 //   reverse  the teacher has e: against 0, p log(p / q) is infinite wherever a sure teacher's log-probability is rounded to 0.
 // The third is bounded either way.
-__device__ __forceinline__ Term what_is_left(const Teacher& t, double q, double e, double lp) {
-  if (t.divergence == AXON_DISTILL_FORWARD) {
-    const double p = exp64(lp);
-    if (p <= e && q <= (p == 0.0 ? 8.0 * e : e)) return {0.0, 0.0};
-  }
-  return outcome(t, log64(fmax(q, t.divergence == AXON_DISTILL_REVERSE ? e : 0.0)), lp);
+__device__ __forceinline__ Term what_is_left(const Teacher& t, double q, double e, double p, double lp) {
+  if (t.divergence == AXON_DISTILL_FORWARD && p <= e && q <= (p == 0.0 ? 8.0 * e : e)) return {0.0, 0.0};
+  q = fmax(q, t.divergence == AXON_DISTILL_REVERSE ? e : 0.0);
+  return outcome(t, q, log64(q), p, lp);
 }
 
 // The given tokens of a row, in LDS.
@@ -221,8 +218,9 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
     double p = 0.0;
     if (s.id[i] >= 0) {
       const double lp = ((double)s.b[i] - (double)M) * inv_t - ln_s;
-      o = outcome(t, (double)s.a[i] - norm_q, lp);
+      const double lq = (double)s.a[i] - norm_q;
       p = exp64(lp);
+      o = outcome(t, exp64(lq), lq, p, lp);
       covered += p;
     }
     loss += o.loss;
@@ -245,10 +243,11 @@ __device__ __forceinline__ RowCoefs finish_row(Given& s, const Teacher& t, const
   r.rest = (float)((((double)M_ref - (double)r.lse) * inv_t + ln_ref) * 1.4426950408889634);
   if (REST) {
     const double lp_rest = some ? below + ln_ref - ln_s : log64(s_parts) - ln_s;
-    const Term o = what_is_left(t, 1.0 - s.sum_q, s.error_q, lp_rest);
+    const double p_rest = exp64(lp_rest);
+    const Term o = what_is_left(t, 1.0 - s.sum_q, s.error_q, p_rest, lp_rest);
     loss += o.loss;
     sum_g += o.g;
-    r.c_out = some ? (float)(o.g - exp64(lp_rest) * sum_g) : (float)(0.0 * s_all);
+    r.c_out = some ? (float)(o.g - p_rest * sum_g) : (float)(0.0 * s_all);
     for (int i = lane; i < t.k; i += kWave)
       out.grads[(int64_t)row_i * t.k + i] = s.next[i] == kAgain ? s.a[i] : (float)((double)s.a[i] - (double)s.b[i] * sum_g);
   } else {
