@@ -11,14 +11,17 @@
 // seen in a bit of the owning lane), and a row of a packed batch differs from the row before by ONE token.  Vectors are
 // loaded at whatever boundary a row of an odd vocabulary starts on, so that lanes keep their ids.
 //
-// Bound by memory, which takes 6.4 TB/s read and 4.8 copied in rows of whole vectors, 4.9 and 4.7 at a boundary of 2 bytes.
-//   log-probability and entropy   1500 x 151936 fp32 179 us (5.1 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 285 to
-//     305 us, without controls 225 (5.5 TB/s): what the penalties take of every element, and waves whose loads wait for arithmetic
-//     (four to a SIMD: five spill, 666 us); 2047 x 50257 bf16 73 us, without controls 43 (4.8 TB/s): short runs
-//   their gradient                1500 x 151936 fp32 332 us (5.5 TB/s, in part from the cache in front of the memory), 2047 x 50257 bf16 88 us
-//   written out                   61 x 201088 fp32, histories of 4000 tokens, 30 us (17 without controls); 1024 x 32768 bf16, 1500
-//     tokens, 39 us (24 without controls): a workgroup's history and its terms are trips to memory and through
+// Memory takes 6.4 TB/s read and 4.8 copied in rows of whole vectors, 4.9 and 4.7 at a boundary of 2 bytes.  It bounds fp32 rows and the
+// gradients; bf16 rows of log-probabilities are bound by instructions and by the loads that wait for them, since a row of few ids
+// takes as long as its loads do (masks that leave out half of all vectors save nothing).
+//   log-probability and entropy   1500 x 151936 fp32 174 us (5.2 TB/s); 4096 x 151936 bf16 under masks, penalties and 40 biases 300 to
+//     315 us, under the penalties alone 285, under the masks alone and without controls 244 (5.1 TB/s): what the penalties take of every
+//     element, four waves to a SIMD (five spill, 666 us); 2047 x 50257 bf16 75 us, without controls 50: short runs
+//   their gradient                1500 x 151936 fp32 329 us (5.5 TB/s, in part from the cache in front of the memory), 2047 x 50257 bf16 89 us
+//   written out                   61 x 201088 fp32, histories of 4000 tokens, 32 us (17 without controls); 1024 x 32768 bf16, 1500
+//     tokens, 42 us (24 without controls): a workgroup's history and its terms are trips to memory and through
 //     LDS before the row's arithmetic, which the four other workgroups of a compute unit hide in part
+//   their gradient                1024 x 151936 fp32, 1500 tokens, 325 us (5.8 TB/s of the two reads and the write), bf16 170 us (5.5)
 #include "logits_rows.h"
 #include <type_traits>
 

@@ -13,8 +13,8 @@
 // what is left, times G_rest - p_rest sum_o G_o, which stays in range however little that is.
 //
 // Bound by memory (a large copy takes 4.8 TB/s).  Where the losses' weights are known a row is read once and written once: 4096 x 151936
-// bf16, a third of weight 0, 446 us (2.08 GB, 4.7 TB/s); 2500 x 201088 bf16 446 us (4.5 TB/s, a twentieth of a row is read twice); 1500 x
-// 151936 fp32 425 us (4.3 TB/s, a third of a row twice).  Where they are not, it is read for the statistics and again for the gradient:
+// bf16, a third of weight 0, 446 us (2.08 GB, 4.7 TB/s); 2500 x 201088 bf16 448 us (4.5 TB/s, a twentieth of a row is read twice); 1500 x
+// 151936 fp32 428 us (4.3 TB/s, a third of a row twice).  Where they are not, it is read for the statistics and again for the gradient:
 // 2047 x 50257 bf16 42 us (4.9 TB/s, what rows that start on 2 bytes reach) and 93 us (4.4 TB/s).
 #include "logits_rows.h"
 #include <type_traits>

@@ -13,6 +13,9 @@ of a batch (a trainer):
     y  = -inf                                   what the row's mask forbids, whatever the logit is
     out = y / temperature
 
+in this order.  Samplers differ in it: one that adds its biases before the penalties draws from another distribution, for ids
+that are both biased and in the history, and its rollouts are not scored by this (biases added to the logits beforehand are).
+
 ``controlled_logits`` writes this out, ``controlled_logprobs_from_logits`` returns ``log softmax(out)[label]`` and the entropy of
 ``softmax(out)`` from one read of the logits.  Both are differentiable with respect to the logits; an id that is out
 (``-inf``) has no gradient.

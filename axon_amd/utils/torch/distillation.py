@@ -70,7 +70,9 @@ def distillation_from_logits(logits: torch.Tensor, teacher_ids: torch.Tensor, te
     ``teacher_ids`` (int32 or int64) and ``teacher_logprobs`` (floating point, constants): ``[..., k]``, at most 512 per
     position.  An id outside the vocabulary is a filler; one that comes twice is two outcomes.  A position without a token has
     loss 0 and no gradient; one whose logits hold a NaN, or nothing but -inf, is NaN.  A token that the student gives no
-    probability at all has an infinite forward divergence.  A position whose upstream gradient is 0 is not read by the backward:
+    probability at all has an infinite forward divergence, and so has ``"rest"`` where it leaves nothing and the teacher more than
+    the rounding named above; a token that the teacher gives none (``-inf``) and the student some has an infinite reverse one, whose
+    gradient is no number.  A position whose upstream gradient is 0 is not read by the backward:
     its gradient is 0, whatever it holds.  With ``inplace_backward`` the backward writes d loss / d logits over the logits'
     storage, and can run once.
 
